@@ -313,6 +313,93 @@ LARA_API int lara_gqa_decode_noalloc(const uint16_t* q, const uint16_t* k_cache,
                                      int chunk_tokens, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* 8-bit KV cache and q/k head norms (serving extensions; the reference keeps */
+/* one bf16 sequence in BRAM, hw/rtl/mem/kv_cache_ram.sv, and rotates q and k */
+/* without a norm, hw/rtl/core/rope_engine.sv).                              */
+/* ------------------------------------------------------------------------ */
+
+/* RMS norm of every query and key head with the position rotation, in one pass:
+ *   y = x * w / sqrt(mean_d(x^2) + eps)         (w NULL: y = x)
+ *   (y_a, y_b) -> (y_a c - y_b s, y_a s + y_b c) (cos_sin NULL: no rotation)
+ * in fp32 with one bf16 rounding (nearest even) at the end.  Token t of batch
+ * entry b sits at positions[b*n + t] and takes row positions[..] of
+ * cos_sin[max_pos][rot_dim] (fp32: rot_dim/2 cosines, then rot_dim/2 sines).
+ * Pair i is (2i, 2i+1) when interleaved != 0, else (i, i + rot_dim/2); dims
+ * rot_dim .. head_dim-1 are not rotated.  q, k and the outputs are strided
+ * (elements): x[b*sb + t*st + h*sh + d]; the outputs may be the inputs
+ * themselves.  q_weight, k_weight: bf16[head_dim], both or neither.
+ * head_dim 64 or 128, rot_dim a multiple of 8.  A position outside
+ * [0, max_pos) is flagged in the workspace status word (workspace may be NULL:
+ * no status) and takes the nearest table row. */
+LARA_API int lara_qk_norm_rope(const uint16_t* q, long long q_sb, long long q_st, long long q_sh, const uint16_t* k,
+                               long long k_sb, long long k_st, long long k_sh, uint16_t* q_out, long long qo_sb,
+                               long long qo_st, long long qo_sh, uint16_t* k_out, long long ko_sb, long long ko_st,
+                               long long ko_sh, int batch, int n, int n_q_heads, int n_kv_heads, int head_dim,
+                               const int32_t* positions, const float* cos_sin, int max_pos, int rot_dim,
+                               int interleaved, const uint16_t* q_weight, const uint16_t* k_weight, float eps,
+                               void* workspace, void* stream);
+
+/* A paged pool of 8-bit K/V rows.  One row = the head_dim values of one token
+ * and kv head: codes k/v_codes[num_pages][Hkv][page_size][D] and one fp32
+ * scale k/v_scales[num_pages][Hkv][page_size]; the row stands for code * scale.
+ * LARA_KVQ_INT8:     a = max(max|x|, 2^-100), code = rint(127 x / a) (ties to
+ *                    even, the quotient rounded once), scale = a / 127.
+ * LARA_KVQ_FP8_E4M3: scale = the smallest power of two >= 2^-100 with
+ *                    max|x| / scale <= 448, code = e4m3(x / scale) (nearest
+ *                    even); the NaN codes 0x7f / 0xff never occur.
+ * A row with a NaN or an infinity has scale NaN and codes 0.
+ * head_dim 64 or 128; page_size a power of two in [16, 65536]; codes 16-byte,
+ * scales 16-byte aligned.  block_table[b * pages_per_seq + j] as for
+ * lara_gqa_decode_paged. */
+#define LARA_KVQ_INT8 0
+#define LARA_KVQ_FP8_E4M3 1
+typedef struct lara_kvq_pool {
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  float* k_scales;
+  float* v_scales;
+  int32_t format;
+  int32_t num_pages;
+  int32_t n_kv_heads;
+  int32_t page_size;
+  int32_t head_dim;
+} lara_kvq_pool;
+
+/* Quantise new rows into the pool.  k_new/v_new are bf16, strided (elements):
+ * x[b*sb + h*sh + t*st + d].  Row t of sequence b lands at token starts[b] + t
+ * for t < counts[b] (counts NULL: n_new each; device int32[B]).  starts stays
+ * as it is; new_lens (NULL, or int32[B] apart from starts and counts) receives
+ * starts + counts, at most the capacity.  Rows past the capacity or naming a
+ * bad page are dropped and flagged in the workspace status word (workspace may
+ * be NULL: no status), as is a count outside [0, n_new] (it is clamped). */
+LARA_API int lara_kvq_append(const lara_kvq_pool* pool, const int32_t* block_table, int pages_per_seq,
+                             const int32_t* starts, const int32_t* counts, int32_t* new_lens, const uint16_t* k_new,
+                             long long k_sb, long long k_sh, long long k_st, const uint16_t* v_new, long long v_sb,
+                             long long v_sh, long long v_st, int batch, int n_new, void* workspace, void* stream);
+
+/* Read rows back as bf16: k/v_out[b*sb + h*sh + t*st + d] (strides in
+ * elements) = code * scale (one fp32 product, bf16 nearest even) of token
+ * starts[b] + t (starts NULL: t) of sequence b for t in [0, n_tokens); zeros
+ * for tokens at or past seq_lens[b].  The contiguous result is a cache that
+ * lara_gqa_prefill and the other bf16 kernels take.  A bad page reads as zeros
+ * and is flagged, as is a length past the capacity (clamped). */
+LARA_API int lara_kvq_read(const lara_kvq_pool* pool, const int32_t* block_table, int pages_per_seq,
+                           const int32_t* seq_lens, const int32_t* starts, uint16_t* k_out, long long k_sb,
+                           long long k_sh, long long k_st, uint16_t* v_out, long long v_sb, long long v_sh,
+                           long long v_st, int batch, int n_tokens, void* workspace, void* stream);
+
+/* Decode over an 8-bit pool: lara_gqa_decode_paged with k = code * scale and
+ * v = code * scale.  Any group size n_q_heads / n_kv_heads from 1 to 16.  A
+ * sequence of length 0 gives zeros.  Lengths stay on the device: the kernel
+ * spreads the cached tokens over the SMs by itself, so no plan depends on
+ * them.  Workspace: lara_kvq_decode_workspace_bytes, zeroed once by
+ * lara_workspace_init; a workspace serves one stream at a time. */
+LARA_API size_t lara_kvq_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim);
+LARA_API int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool, const int32_t* block_table,
+                                 int pages_per_seq, const int32_t* seq_lens, uint16_t* o, int batch, int n_q_heads,
+                                 float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Context API: the backing of the Python AttentionAccelerator.  The context */
 /* owns the HBM KV cache, device I/O buffers, a stream and timing events.   */
 /* Tensor pointers are host memory unless on_device != 0.                    */

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_size_t, c_uint16, c_uint64, c_void_p, c_double
+from ctypes import POINTER, c_char_p, c_float, c_int, c_longlong, c_size_t, c_uint16, c_uint64, c_void_p, c_double
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblara_b200.so"
@@ -30,6 +30,8 @@ LARA_ARITH_IEEE = 0
 LARA_ARITH_BOARD = 1
 LARA_DECODE_KERNEL_CUDA_CORE = 0
 LARA_DECODE_KERNEL_TENSOR = 1
+LARA_KVQ_INT8 = 0
+LARA_KVQ_FP8_E4M3 = 1
 
 
 class LaraError(RuntimeError):
@@ -65,6 +67,12 @@ class LaraDeviceInfo(ctypes.Structure):
                 ("runtime_version", c_int), ("total_mem_bytes", ctypes.c_ulonglong)]
 
 
+class LaraKvqPool(ctypes.Structure):
+    _fields_ = [("k_codes", c_void_p), ("v_codes", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+                ("format", c_int), ("num_pages", c_int), ("n_kv_heads", c_int), ("page_size", c_int),
+                ("head_dim", c_int)]
+
+
 _I32P = POINTER(ctypes.c_int32)
 _U16P = POINTER(c_uint16)
 
@@ -88,7 +96,7 @@ SIGNATURES = {
     "lara_gqa_decode_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                         c_int, c_int, c_float, c_int, c_int, c_void_p]),
     "lara_lse_combine": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "lara_lse_combine_strided": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_int, c_int,
+    "lara_lse_combine_strided": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int,
                                          c_int, c_void_p, c_void_p]),
     "lara_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                c_void_p, c_void_p]),
@@ -110,6 +118,18 @@ SIGNATURES = {
     "lara_layer_prologue": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                     c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_size_t,
                                     c_void_p]),
+    "lara_qk_norm_rope": (c_int, [*([c_void_p, c_longlong, c_longlong, c_longlong] * 4), c_int, c_int, c_int, c_int,
+                                  c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
+                                  c_void_p, c_void_p]),
+    "lara_kvq_append": (c_int, [POINTER(LaraKvqPool), c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                *([c_void_p, c_longlong, c_longlong, c_longlong] * 2), c_int, c_int, c_void_p,
+                                c_void_p]),
+    "lara_kvq_read": (c_int, [POINTER(LaraKvqPool), c_void_p, c_int, c_void_p, c_void_p,
+                              *([c_void_p, c_longlong, c_longlong, c_longlong] * 2), c_int, c_int, c_void_p,
+                              c_void_p]),
+    "lara_kvq_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "lara_gqa_decode_kvq": (c_int, [c_void_p, POINTER(LaraKvqPool), c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
+                                    c_float, c_void_p, c_size_t, c_void_p]),
     "lara_create": (c_int, [c_int, POINTER(c_void_p)]),
     "lara_destroy": (c_int, [c_void_p]),
     "lara_configure_heads": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int]),

@@ -304,6 +304,7 @@ std::string describe_status(int bits) {
   if (bits & lara::kDevBadLength) s += " bad-sequence-length";
   if (bits & lara::kDevAppendOverflow) s += " append-overflow";
   if (bits & lara::kDevBadPage) s += " bad-page-index";
+  if (bits & lara::kDevBadPosition) s += " bad-position";
   return s.empty() ? std::string(" unknown") : s;
 }
 

@@ -27,6 +27,7 @@ enum DeviceStatus : int {
   kDevBadLength = 1 << 1,      // a sequence length was outside [0, max_seq_len]
   kDevAppendOverflow = 1 << 2, // an appended row would pass max_seq_len
   kDevBadPage = 1 << 3,        // a block-table entry was outside [0, num_pages)
+  kDevBadPosition = 1 << 4,    // a token position was outside the rotation table
 };
 
 // One decode launch: queries of `batch` sequences (or of `batch` query rows

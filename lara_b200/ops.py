@@ -7,6 +7,7 @@ or 16-bit integer views of the same words.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -35,6 +36,29 @@ def _check_words(name: str, t: torch.Tensor, shape: tuple | None = None) -> None
         raise ValueError(f"{name} must be contiguous")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _strided(name: str, t: torch.Tensor, shape: tuple, device, written: bool = False) -> tuple:
+    """Strides of a bf16 tensor of contiguous rows (last dim), after checking it."""
+    if t.dtype not in _WORD_DTYPES:
+        raise TypeError(f"{name} must hold bf16 words (bfloat16/int16/uint16), got {t.dtype}")
+    if t.device != device or not t.is_cuda:
+        raise ValueError(f"{name} must be on the CUDA device {device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    st = t.stride()
+    if st[-1] != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    if written and any(s == 0 and n > 1 for s, n in zip(st, shape)):
+        raise ValueError(f"{name} is written and must not repeat elements (a stride of 0)")
+    return st
+
+
+def _on_device(device: torch.device):
+    """The device as the current one for a launch; free when it already is."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 @dataclass
@@ -284,3 +308,84 @@ def layer_prologue(x, w_qkv, rms_weight=None, *, n_q_heads=32, n_kv_heads=8, hea
                                   head_dim, q_pos_base, kv_pos_base, float(rms_eps), float(rope_base),
                                   ws.data_ptr(), ws.numel(), _stream(dev)), "lara_layer_prologue")
     return q, k, v
+
+
+def rope_table(max_pos: int, rot_dim: int, *, base: float = 10000.0, inv_freq=None, device="cuda:0") -> torch.Tensor:
+    """Rotation table for :func:`qk_norm_rope`: float32 ``[max_pos, rot_dim]``, cosines then sines.
+
+    The angles ``pos * base**(-2i/rot_dim)`` (or ``pos * inv_freq[i]`` for scaled frequencies) are taken in
+    float64, so the table is right to fp32 at every position.
+    """
+    if rot_dim < 8 or rot_dim % 8 or max_pos < 1:
+        raise ValueError("rot_dim must be a positive multiple of 8, max_pos >= 1")
+    if inv_freq is None:
+        f = base ** (-2.0 * torch.arange(rot_dim // 2, dtype=torch.float64, device=device) / rot_dim)
+    else:
+        f = torch.as_tensor(inv_freq, dtype=torch.float64, device=device)
+        if tuple(f.shape) != (rot_dim // 2,):
+            raise ValueError(f"inv_freq must have {rot_dim // 2} entries")
+    ang = torch.arange(max_pos, dtype=torch.float64, device=device)[:, None] * f
+    return torch.cat([ang.cos(), ang.sin()], -1).float()
+
+
+def _rope_args(cos_sin, head_dim: int, device) -> tuple:
+    if cos_sin is None:
+        return None, 0, 0
+    if cos_sin.dtype != torch.float32 or cos_sin.device != device or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+        raise ValueError(f"cos_sin must be a contiguous float32 [max_pos, rot_dim] tensor on {device}")
+    return cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1]
+
+
+def _norm_weights(q_weight, k_weight, head_dim: int, device) -> None:
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _check_words(name, w, (head_dim,))
+            if w.device != device:
+                raise ValueError(f"{name} must be on {device}")
+
+
+def qk_norm_rope(q, k, *, positions=None, cos_sin=None, q_weight=None, k_weight=None, eps: float = 1e-5,
+                 interleaved: bool = True, workspace=None, out=None):
+    """RMS norm of every query and key head and the position rotation, in one pass (``lara_qk_norm_rope``).
+
+    q ``[T, Hq, D]`` and k ``[T, Hkv, D]`` (or ``[B, n, H, D]``), bf16 with any strides over contiguous heads:
+    views of a packed projection output and transposed head-major tensors are taken as they are.  Token t sits
+    at ``positions[t]`` (int32 of shape ``[T]`` or ``[B, n]``) and takes that row of ``cos_sin`` (see
+    :func:`rope_table`; its width says how many dims rotate).  ``interleaved`` pairs dims (2i, 2i+1), the
+    pairing of :func:`layer_prologue`; otherwise (i, i + rot_dim/2).  ``q_weight``/``k_weight`` (bf16 ``[D]``)
+    norm the heads first; without them they are only rotated, and without ``cos_sin`` only normed.  Returns
+    (q, k) in new contiguous tensors, or in ``out``, which may be the inputs.  ``workspace`` collects the
+    status bit of a position outside the table (its nearest row is taken).
+    """
+    if q.dim() not in (3, 4) or k.dim() != q.dim():
+        raise ValueError("q and k must be [T, H, D] or [B, n, H, D]")
+    dev = q.device
+    lead, (hq, d), hkv = tuple(q.shape[:-2]), q.shape[-2:], k.shape[-2]
+    qs = _strided("q", q, (*lead, hq, d), dev)
+    ks = _strided("k", k, (*lead, hkv, d), dev)
+    if out is None:
+        qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    else:
+        qo, ko = out
+    qos = _strided("q out", qo, (*lead, hq, d), dev, written=True)
+    kos = _strided("k out", ko, (*lead, hkv, d), dev, written=True)
+    _norm_weights(q_weight, k_weight, d, dev)
+    table, max_pos, rot = _rope_args(cos_sin, d, dev)
+    if table is not None:
+        if positions is None:
+            raise ValueError("a rotation needs positions")
+        if (positions.dtype != torch.int32 or positions.device != dev or tuple(positions.shape) != lead
+                or not positions.is_contiguous()):
+            raise ValueError(f"positions must be a contiguous int32 tensor of shape {lead} on {dev}")
+    if len(lead) == 1:
+        B, n, qs, ks, qos, kos = 1, lead[0], (0, *qs), (0, *ks), (0, *qos), (0, *kos)
+    else:
+        B, n = lead
+    with _on_device(dev):
+        check(lib.lara_qk_norm_rope(q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
+                                    qo.data_ptr(), qos[0], qos[1], qos[2], ko.data_ptr(), kos[0], kos[1], kos[2],
+                                    B, n, hq, hkv, d, None if table is None else positions.data_ptr(), table, max_pos,
+                                    rot, int(bool(interleaved)), _ptr(q_weight), _ptr(k_weight), float(eps),
+                                    _ptr(workspace), _stream(dev)), "lara_qk_norm_rope")
+    return qo, ko

@@ -38,9 +38,7 @@ class PagedKVCache:
         self.page_size, self.n_kv_heads, self.head_dim = int(page_size), int(n_kv_heads), int(head_dim)
         self.num_pages, self.max_seqs = int(num_pages), int(max_seqs)
         self.pages_per_seq = int(math.ceil(max_seq_len / page_size))
-        shape = (self.num_pages, self.n_kv_heads, self.page_size, self.head_dim)
-        self.k_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
-        self.v_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+        self._alloc_pages()
         self._table = np.full((self.max_seqs, self.pages_per_seq), -1, np.int32)
         self.block_table = torch.from_numpy(self._table).to(self.device)
         self._lens = np.zeros(self.max_seqs, np.int32)
@@ -50,6 +48,11 @@ class PagedKVCache:
         self._active = np.zeros(self.max_seqs, bool)
         self._ws = None
         self._status = new_workspace(256, self.device)
+
+    def _alloc_pages(self) -> None:
+        shape = (self.num_pages, self.n_kv_heads, self.page_size, self.head_dim)
+        self.k_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+        self.v_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
 
     # ------------------------------------------------------------ allocation
     @property
