@@ -195,7 +195,7 @@ struct PoolIndex {
     }
     return ((((long long)page * n_kv_heads + h) << page_log2) + (pos & ((1 << page_log2) - 1)));
   }
-  __device__ __forceinline__ long long capacity() const { return (long long)pages_per_seq << page_log2; }
+  __host__ __device__ __forceinline__ long long capacity() const { return (long long)pages_per_seq << page_log2; }
 };
 
 // Host: the pool's pointers and geometry, checked; LARA_OK or an error code.

@@ -1,12 +1,43 @@
 // GQA decode over the paged 8-bit KV pool (declared in include/lara_b200.h).
 //
-//   o[b,h,:] = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q.k_t - m),
-//   k_t = ks_t ck_t, v_t = vs_t cv_t  (codes c, one fp32 scale per row)
+//   o[b,h,:] = sum_t p_t v_t / sum_t p_t,  p_t = 2^(s_t - R),  s_t = scale log2(e) q.k_t
+//   k_t = ks_t ck_t, v_t = vs_t cv_t       (codes c, one fp32 scale per row)
 //
-// One CTA per (sequence, query head); a warp takes every kWarps-th token, a
-// lane D / 32 dims, with a running maximum and sum in fp32; the warps are
-// joined at the end.
+// Bound by HBM: every cached row is read once, 2 (D + 4) bytes per token and kv
+// head, for 4 D G multiply-adds.  What a byte costs on the SM is kept far
+// below the time it takes to arrive:
+//
+//  * Products run on the tensor cores as mma.m16n8k16 (fp16 in, fp32 out) with
+//    the cache as the 16-row operand and the group's query heads as the 8
+//    columns: S^T[token][head] = K q^T, then O^T[dim][head] = V^T P^T.  The
+//    columns of S^T and O^T lie in the same lanes, so rescaling needs no
+//    exchange, and movmatrix turns a tile of P into the second operand.  At
+//    one byte per element the cache itself is the bound, and eight heads share
+//    each product, so the 5th-generation path (128-row tiles, TMEM, operands
+//    described per tile) has nothing to win here.
+//  * Codes become fp16 in registers, exactly: int8 by setting the exponent
+//    byte (0x6400 | code + 128 is 1152 + code) and one subtraction, e4m3 by
+//    moving its bits into place (the value times 2^-8; any byte is finite, so
+//    garbage past a sequence's end cannot reach a sum).  The order in which a
+//    lane's bytes meet q, and the output dims a lane ends up with, are chosen
+//    so that no byte has to be moved between lanes.
+//  * ks multiplies the fp32 scores, vs the fp32 weights.  Weights are rounded
+//    to fp16 (2^-11 each, below bf16's 2^-8 of the output); R follows the
+//    largest s_t + log2 vs_t, so the weights that carry the sum stay in fp16's
+//    normal range whatever the scales are.  R is moved only when a weight
+//    would pass 2^8, and by whole powers of two, so most tiles rescale nothing.
+//  * q is brought to fp16 by a power of two per head (exact within 2^-29 of
+//    the head's largest value).
+//
+// Work is split evenly, by the kernel itself: all (sequence, kv head) units
+// are laid end to end in tiles of 32 tokens, CTA c takes an equal share, and
+// its warps take tiles in turn, each through its own ring of cp.async stages
+// (no barrier per tile, no plan from the host, lengths stay on the device).
+// Warps join at the end of a unit; a unit that several CTAs share is joined by
+// the last of them to finish, in CTA order, so results do not depend on timing.
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "kvq.cuh"
 
@@ -16,8 +47,23 @@ using namespace kvq;
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 32;          // tokens per warp and stage
+constexpr int kMinTiles = kWarps;  // tiles per CTA below which fewer CTAs run
 constexpr size_t kStatusBytes = 256;
+
+template <int D, int NG>
+struct Cfg {
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kCtasPerSm = D == 128 ? 2 : 3;
+  static constexpr int kRowsBytes = kTile * D;                     // K (or V) codes of a stage
+  static constexpr int kStageBytes = 2 * kRowsBytes + 2 * kTile * 4;
+  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kMergeBytes = (kWarps - 1) * 8 * D * 4;     // one group of 8 heads at a time
+  static constexpr int kSmemBytes = kRingBytes + kMergeBytes;
+  static constexpr int kJoinChunk = kMergeBytes / (NG * 8 * 8);    // partial (R, l) the join stages at a time
+};
 
 struct KvqDecodeArgs {
   lara_kvq_pool pool;
@@ -25,76 +71,602 @@ struct KvqDecodeArgs {
   const uint16_t* q;
   const int32_t* lens;
   uint16_t* o;
-  int n_q_heads;
+  int batch, n_q_heads, group;
   float scale_log2;
   int* status;
+  int* counters;    // [batch * Hkv], zero between launches
+  float2* part_ml;  // [2 * grid][group] (R, l)
+  float* part_acc;  // [2 * grid][group][D]
 };
 
-template <int D, int FMT>
-__global__ void __launch_bounds__(kWarps * 32) kvq_decode_kernel(const __grid_constant__ KvqDecodeArgs a) {
-  constexpr int V = D / 32;
-  __shared__ float sm[kWarps], sl[kWarps], sacc[kWarps][D];
-  const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int kvh = h / (a.n_q_heads / a.pool.n_kv_heads);
-  int len = a.lens[b];
-  if (len < 0 || len > a.index.capacity()) {
-    if (threadIdx.x == 0) atomicOr(a.status, kDevBadLength);
-    len = len < 0 ? 0 : (int)a.index.capacity();
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// Bytes 0 and 2 (even) and bytes 1 and 3 (odd) of four codes as fp16 pairs.
+template <int FMT>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& even, uint32_t& odd) {
+  if constexpr (FMT == LARA_KVQ_INT8) {
+    const uint32_t x = w ^ 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    uint32_t e = __byte_perm(x, 0x64646464u, 0x4240), o = __byte_perm(x, 0x64646464u, 0x4341);
+    const __half2 he = __hsub2(reinterpret_cast<__half2&>(e), bias);
+    const __half2 ho = __hsub2(reinterpret_cast<__half2&>(o), bias);
+    even = reinterpret_cast<const uint32_t&>(he);
+    odd = reinterpret_cast<const uint32_t&>(ho);
+  } else {
+    // s eeee mmm -> s 0 eeee mmm 0000000: fp16 with the exponent 8 too small
+    even = ((w << 7) & 0x3f803f80u) | ((w << 8) & 0x80008000u);
+    odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
   }
-  const long long qrow = ((long long)b * a.n_q_heads + h) * D;
-  float q[V], acc[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    q[j] = __uint_as_float((uint32_t)a.q[qrow + lane * V + j] << 16);
-    acc[j] = 0.f;
+}
+
+// Where the 16-byte chunk c of a row lies in a stage, so that the eight lanes
+// of a shared-memory phase (rows 2t of V, or two rows of K) hit distinct banks.
+template <int D>
+__device__ __forceinline__ uint32_t chunk_offset(int row, int c) {
+  if constexpr (D == 128) return row * 128 + ((c ^ (row & 7)) << 4);
+  return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+}
+
+__device__ __forceinline__ int seq_tiles(const KvqDecodeArgs& a, int b, int* len_out = nullptr) {
+  int len = __ldcg(a.lens + b);
+  const long long cap = a.index.capacity();
+  if (len < 0 || len > cap) {
+    atomicOr(a.status, kDevBadLength);
+    len = len < 0 ? 0 : (int)cap;
   }
-  float m = -INFINITY, l = 0.f;
-  for (int t = warp; t < len; t += kWarps) {
-    long long row = a.index.row(b, kvh, t, a.status);
-    if (row < 0) row = 0;
-    uint32_t ck = 0, cv = 0;
-    if constexpr (V == 4) {
-      ck = *reinterpret_cast<const uint32_t*>(a.pool.k_codes + row * D + lane * V);
-      cv = *reinterpret_cast<const uint32_t*>(a.pool.v_codes + row * D + lane * V);
-    } else {
-      ck = *reinterpret_cast<const uint16_t*>(a.pool.k_codes + row * D + lane * V);
-      cv = *reinterpret_cast<const uint16_t*>(a.pool.v_codes + row * D + lane * V);
+  if (len_out) *len_out = len;
+  return (len + kTile - 1) / kTile;
+}
+
+// A position in the end-to-end order of tiles: unit (b, kvh) starts at `base`.
+struct Unit {
+  long long base;
+  int b, kvh, tiles, len;
+  __device__ __forceinline__ void next(const KvqDecodeArgs& a) {
+    base += tiles;
+    if (++kvh == a.pool.n_kv_heads) {
+      kvh = 0;
+      do {
+        ++b;
+        tiles = b < a.batch ? seq_tiles(a, b, &len) : 0x7fffffff;
+      } while (tiles == 0);
     }
-    float kf[4], vf[4];
-    codes_to_f32<FMT>(ck, kf);
-    codes_to_f32<FMT>(cv, vf);
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) s = fmaf(q[j], kf[j], s);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s = s * a.pool.k_scales[row] * a.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float corr = exp2f(m - mn), p = exp2f(s - mn);
-    const float pv = p * a.pool.v_scales[row];
-    m = mn;
-    l = fmaf(l, corr, p);
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = fmaf(acc[j], corr, pv * vf[j]);
   }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
+};
+
+template <int D, int FMT, int NG>
+__global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
+    kvq_decode_kernel(const __grid_constant__ KvqDecodeArgs a) {
+  using C = Cfg<D, NG>;
+  constexpr int KS = D / 16;   // k steps of the scores = dim blocks of the output
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_sum[kWarps];
+  __shared__ Unit s_first;
+  __shared__ float2 s_ml[kWarps][NG * 8];
+  __shared__ int s_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int G = a.group, hkv = a.pool.n_kv_heads;
+
+  allow_dependent_launch();
+  grid_dependency_wait();
+
+  // ---- this CTA's share [w0, w1) of all tiles, and the unit w0 lies in ----
+  const int per_thread = (a.batch + kThreads - 1) / kThreads;
+  const int b_lo = min(a.batch, (int)threadIdx.x * per_thread), b_hi = min(a.batch, b_lo + per_thread);
+  long long mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += seq_tiles(a, b);
+  long long incl = mine;
 #pragma unroll
-  for (int j = 0; j < V; ++j) sacc[warp][lane * V + j] = acc[j];
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += x;
+  }
+  if (lane == 31) s_sum[warp] = incl;
   __syncthreads();
-  if (threadIdx.x < D) {
-    float M = -INFINITY, L = 0.f, x = 0.f;
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm[w]);
-    for (int w = 0; w < kWarps; ++w) {
-      if (sm[w] == -INFINITY) continue;
-      const float c = exp2f(sm[w] - M);
-      L = fmaf(sl[w], c, L);
-      x = fmaf(sacc[w][threadIdx.x], c, x);
-    }
-    a.o[qrow + threadIdx.x] = (uint16_t)pack2_rn(len > 0 ? x / L : 0.f, 0.f);
+  long long before = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
   }
+  before *= hkv;
+  total *= hkv;
+  // sequences without tokens give zeros
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+    if (__ldcg(a.lens + b) <= 0)
+      for (int i = threadIdx.x; i < a.n_q_heads * D / 8; i += kThreads)
+        reinterpret_cast<uint4*>(a.o + (long long)b * a.n_q_heads * D)[i] = make_uint4(0, 0, 0, 0);
+  const int n_ctas = (int)min((long long)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+  if ((int)blockIdx.x >= n_ctas) return;
+  const long long per = total / n_ctas, rem = total % n_ctas;
+  auto cta_start = [&](long long c) { return c * per + min(c, rem); };
+  auto cta_of = [&](long long id) {
+    return (int)(id < rem * (per + 1) ? id / (per + 1) : rem + (id - rem * (per + 1)) / per);
+  };
+  const long long w0 = cta_start(blockIdx.x), w1 = cta_start(blockIdx.x + 1);
+  if (w0 >= before && w0 < before + mine * hkv) {
+    Unit u{before, b_lo, 0, 0, 0};
+    u.tiles = seq_tiles(a, u.b, &u.len);
+    while (w0 >= u.base + (long long)u.tiles * hkv) {  // by whole sequences (tiles may be 0)
+      u.base += (long long)u.tiles * hkv;
+      ++u.b;
+      u.tiles = seq_tiles(a, u.b, &u.len);
+    }
+    u.kvh = (int)((w0 - u.base) / u.tiles);
+    u.base += (long long)u.kvh * u.tiles;
+    s_first = u;
+  }
+  __syncthreads();
+
+  // ---- the warp's ring ----
+  const uint32_t ring = smem_addr(smem) + warp * (C::kStages * C::kStageBytes);
+  Unit pu = s_first;             // where the next tile to fetch lies
+  long long pid = w0 + warp;     // its number
+  int page[2];                   // its pages (one per 16 tokens), fetched a tile ahead
+  auto fetch_pages = [&] {
+    if (pid >= w1) return;
+    while (pid >= pu.base + pu.tiles) pu.next(a);
+    const int pos = (int)(pid - pu.base) * kTile;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      page[i] = pos + 16 * i < pu.len
+                    ? __ldcg(a.index.block_table + (long long)pu.b * a.index.pages_per_seq + ((pos + 16 * i) >> a.index.page_log2))
+                    : 0;
+  };
+  auto fetch_tile = [&](int stage) {
+    if (pid < w1) {
+      const uint32_t st = ring + stage * C::kStageBytes;
+      const int pos = (int)(pid - pu.base) * kTile;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (pos + 16 * i >= pu.len) break;
+        int pg = page[i];
+        if (pg < 0 || pg >= a.index.num_pages) {
+          atomicOr(a.status, kDevBadPage);
+          pg = 0;
+        }
+        const long long row = ((((long long)pg * hkv + pu.kvh) << a.index.page_log2) +
+                               ((pos + 16 * i) & ((1 << a.index.page_log2) - 1)));
+        constexpr int kChunks = D / 16, kRowsPer = 32 / kChunks;
+        const int r0 = lane / kChunks, c = lane % kChunks;
+        const uint8_t* ks = a.pool.k_codes + row * D + lane * 16;
+        const uint8_t* vs = a.pool.v_codes + row * D + lane * 16;
+#pragma unroll
+        for (int j = 0; j < 16 / kRowsPer; ++j) {
+          const uint32_t off = chunk_offset<D>(16 * i + j * kRowsPer + r0, c);
+          cp_async16(st + off, ks + j * 512);
+          cp_async16(st + C::kRowsBytes + off, vs + j * 512);
+        }
+        if (lane < 8) {  // 16 scales of K (lanes 0-3) and of V (lanes 4-7)
+          const float* sc = (lane < 4 ? a.pool.k_scales : a.pool.v_scales) + row + 4 * (lane & 3);
+          cp_async16(st + 2 * C::kRowsBytes + (lane < 4 ? 0 : kTile * 4) + (16 * i + 4 * (lane & 3)) * 4, sc);
+        }
+      }
+      pid += kWarps;
+      fetch_pages();
+    }
+    cp_async_commit();
+  };
+  fetch_pages();
+#pragma unroll
+  for (int s = 0; s < C::kStages - 1; ++s) fetch_tile(s);
+
+  // ---- units of this CTA ----
+  int stage = 0;
+  long long id = w0 + warp;      // next tile to work on
+  Unit u = s_first;
+  for (; u.base < w1; u.next(a)) {
+    const long long end = min(w1, u.base + u.tiles);
+    // q of the group's heads as the 8-column operand: column g, rows in the
+    // order in which codes_to_f16 hands out a lane's K bytes
+    uint32_t qf[NG][KS][2];
+    float qs[NG][2];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int h = n * 8 + g;
+      uint32_t w[D / 8];
+      if (h < G) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            a.q + ((long long)u.b * a.n_q_heads + u.kvh * G + h) * D + t4 * (D / 4));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = __ldcg(src + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) w[i] = 0;
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      m = max(m & 0xffffu, m >> 16);
+      // largest value to [2^14, 2^15); a NaN or infinity goes through as it is
+      const int e = m >= 0x7f80u ? 0 : max((int)(m >> 7) - 127, -100) - 14;
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const __half2 lo = __floats2half2_rn(bf16lo(w[2 * j]) * down, bf16lo(w[2 * j + 1]) * down);
+        const __half2 hi = __floats2half2_rn(bf16hi(w[2 * j]) * down, bf16hi(w[2 * j + 1]) * down);
+        qf[n][j][0] = reinterpret_cast<const uint32_t&>(lo);
+        qf[n][j][1] = reinterpret_cast<const uint32_t&>(hi);
+      }
+      // the score factor of heads 2 t4 and 2 t4 + 1, from the lanes that hold them
+      const float f = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2 *
+                      (FMT == LARA_KVQ_FP8_E4M3 ? 256.f : 1.f);
+      qs[n][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
+      qs[n][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+    }
+    float R[NG][2], l[NG][2], o[NG][KS][4];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      R[n][0] = R[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+
+    for (; id < end; id += kWarps) {
+      cp_async_wait<C::kStages - 2>();
+      __syncwarp();
+      fetch_tile(stage == 0 ? C::kStages - 1 : stage - 1);
+      const uint32_t st = ring + stage * C::kStageBytes;
+      stage = stage + 1 == C::kStages ? 0 : stage + 1;
+      const int valid = u.len - (int)(id - u.base) * kTile;
+
+      // ---- scores: s[mb][n][..] of tokens 16 mb + g (0, 1) and + 8 (2, 3) ----
+      float s[2][NG][4], vsc[2][2], lw[2][2];
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n) s[mb][n][0] = s[mb][n][1] = s[mb][n][2] = s[mb][n][3] = 0.f;
+        uint32_t k0[D / 16], k1[D / 16];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const int ch = t4 * (D / 64) + c;
+          *reinterpret_cast<uint4*>(k0 + 4 * c) = lds128(st + chunk_offset<D>(16 * mb + g, ch));
+          *reinterpret_cast<uint4*>(k1 + 4 * c) = lds128(st + chunk_offset<D>(16 * mb + g + 8, ch));
+        }
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          uint32_t a0, a1, a2, a3;
+          codes_to_f16<FMT>(k0[j], a0, a2);
+          codes_to_f16<FMT>(k1[j], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma_f16(s[mb][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int tok = 16 * mb + 8 * r + g;
+          const bool in = tok < valid;
+          const float ks = lds_f32(st + 2 * C::kRowsBytes + tok * 4);
+          const float vs = lds_f32(st + 2 * C::kRowsBytes + kTile * 4 + tok * 4);
+          vsc[mb][r] = in ? vs : 0.f;
+          lw[mb][r] = fmaxf(__log2f(vs), -100.f);
+#pragma unroll
+          for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float& x = s[mb][n][2 * r + c];
+              x = in ? x * qs[n][c] * ks : -INFINITY;
+            }
+        }
+      }
+
+      // ---- move R where a weight would pass 2^8 ----
+      bool over = false;
+      float top[NG][2];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          top[n][c] = fmaxf(fmaxf(s[0][n][c] + lw[0][0], s[0][n][2 + c] + lw[0][1]),
+                            fmaxf(s[1][n][c] + lw[1][0], s[1][n][2 + c] + lw[1][1]));
+          over |= top[n][c] > R[n][c] + 8.f;
+        }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = top[n][c];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            if (m > R[n][c] + 8.f) {
+              const float to = ceilf(m), f = ex2_ftz(R[n][c] - to);
+              R[n][c] = to;
+              l[n][c] *= f;
+#pragma unroll
+              for (int i = 0; i < KS; ++i) {
+                o[n][i][c] *= f;
+                o[n][i][2 + c] *= f;
+              }
+            }
+          }
+      }
+
+      // ---- weights, as the second operand: tokens 2 t4, +1 and + 8 of column g ----
+      uint32_t pf[2][NG][2];
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float p0 = ex2_ftz(s[mb][n][2 * r] - R[n][0]), p1 = ex2_ftz(s[mb][n][2 * r + 1] - R[n][1]);
+            l[n][0] += p0;
+            l[n][1] += p1;
+            const __half2 w = __floats2half2_rn(p0 * vsc[mb][r], p1 * vsc[mb][r]);
+            pf[mb][n][r] = transpose8x8(reinterpret_cast<const uint32_t&>(w));
+          }
+
+      // ---- O^T += V^T P^T: this lane's dims are 16 g' .. of four tokens ----
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+        uint32_t v[4][D / 32];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * mb + 2 * t4 + (r & 1) + 8 * (r >> 1);
+          const uint32_t base = st + C::kRowsBytes;
+          if constexpr (D == 128) {
+            *reinterpret_cast<uint4*>(v[r]) = lds128(base + chunk_offset<D>(row, g));
+          } else {
+            *reinterpret_cast<uint2*>(v[r]) = lds64(base + chunk_offset<D>(row, g >> 1) + 8 * (g & 1));
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint32_t sel = hf ? 0x7632 : 0x5410;
+            uint32_t a0, a1, a2, a3;
+            codes_to_f16<FMT>(__byte_perm(v[0][w], v[1][w], sel), a0, a1);
+            codes_to_f16<FMT>(__byte_perm(v[2][w], v[3][w], sel), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * w + hf], a0, a1, a2, a3, pf[mb][n][0], pf[mb][n][1]);
+          }
+      }
+    }
+
+    // ---- join the warps: R and l first, then the scaled sums ----
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
+        if (g == 0) s_ml[warp][n * 8 + 2 * t4 + c] = make_float2(R[n][c], l[n][c]);
+      }
+    __syncthreads();
+    float4* merge = reinterpret_cast<float4*>(smem + C::kRingBytes);
+    const bool whole = u.base >= w0 && u.base + u.tiles <= w1;
+    const int slot = 2 * (int)blockIdx.x + (u.base > w0 ? 1 : 0);
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      float L[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][n * 8 + 2 * t4 + c].x);
+        L[c] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = s_ml[w][n * 8 + 2 * t4 + c];
+          L[c] = fmaf(ml.y, ml.x == top ? 1.f : ex2_ftz(ml.x - top), L[c]);
+        }
+        const float f = R[n][c] == top ? 1.f : ex2_ftz(R[n][c] - top);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          o[n][i][c] *= f;
+          o[n][i][2 + c] *= f;
+        }
+        R[n][c] = top;
+      }
+      if (n > 0) __syncthreads();  // warp 0 has read the first eight heads
+      if (warp > 0)
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+          merge[((warp - 1) * KS + i) * 32 + lane] = make_float4(o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]);
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 0; w < kWarps - 1; ++w)
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            const float4 x = merge[(w * KS + i) * 32 + lane];
+            o[n][i][0] += x.x;
+            o[n][i][1] += x.y;
+            o[n][i][2] += x.z;
+            o[n][i][3] += x.w;
+          }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int h = n * 8 + 2 * t4 + c;
+          if (h >= G) continue;
+          if (whole) {
+            const float inv = (FMT == LARA_KVQ_FP8_E4M3 ? 256.f : 1.f) / L[c];
+            uint16_t* dst = a.o + ((long long)u.b * a.n_q_heads + u.kvh * G + h) * D + g * (D / 8);
+#pragma unroll
+            for (int i = 0; i < KS; i += 4)
+              *reinterpret_cast<uint4*>(dst + 2 * i) =
+                  make_uint4(pack2_rn(o[n][i][c] * inv, o[n][i][2 + c] * inv),
+                             pack2_rn(o[n][i + 1][c] * inv, o[n][i + 1][2 + c] * inv),
+                             pack2_rn(o[n][i + 2][c] * inv, o[n][i + 2][2 + c] * inv),
+                             pack2_rn(o[n][i + 3][c] * inv, o[n][i + 3][2 + c] * inv));
+          } else {
+            float* dst = a.part_acc + ((long long)slot * G + h) * D + g * (D / 8);
+#pragma unroll
+            for (int i = 0; i < KS; i += 2)
+              *reinterpret_cast<float4*>(dst + 2 * i) =
+                  make_float4(o[n][i][c], o[n][i][2 + c], o[n][i + 1][c], o[n][i + 1][2 + c]);
+            if (g == 0) a.part_ml[(long long)slot * G + h] = make_float2(R[n][c], L[c]);
+          }
+        }
+      }
+    }
+    if (whole) continue;
+
+    // ---- a unit of several CTAs: the last one joins the partial results ----
+    const int c_first = cta_of(u.base), c_last = cta_of(u.base + u.tiles - 1), parts = c_last - c_first + 1;
+    if (warp == 0) {
+      __threadfence();
+      __syncwarp();
+      if (lane == 0) {
+        int* ctr = a.counters + (long long)u.b * hkv + u.kvh;
+        const int last = atomicAdd(ctr, 1) == parts - 1;
+        if (last) *ctr = 0;
+        s_flag = last;
+      }
+    }
+    __syncthreads();
+    if (s_flag) {
+      __threadfence();
+      // thread -> four dims of a head, items G * D / 4; every (R, l) of a
+      // chunk of parts goes through shared memory
+      float2* ml = reinterpret_cast<float2*>(merge);
+      constexpr int kItemsMax = NG * 8 * D / 4;
+      constexpr int kPer = (kItemsMax + kThreads - 1) / kThreads;
+      float4 acc[kPer];
+      float top[kPer], L[kPer];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        top[k] = -INFINITY;
+        L[k] = 0.f;
+      }
+      auto slot_of = [&](int c) { return 2 * c + (u.base > cta_start(c) ? 1 : 0); };
+      for (int p0 = 0; p0 < parts; p0 += C::kJoinChunk) {
+        const int np = min(C::kJoinChunk, parts - p0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < np * G; i += kThreads)
+          ml[i] = __ldcg(a.part_ml + (long long)slot_of(c_first + p0 + i / G) * G + i % G);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int item = threadIdx.x + k * kThreads;
+          if (item >= G * D / 4) continue;
+          const int h = item / (D / 4), d = item % (D / 4);
+          float m = top[k];
+          for (int i = 0; i < np; ++i) m = fmaxf(m, ml[i * G + h].x);
+          const float f = top[k] == m ? 1.f : ex2_ftz(top[k] - m);
+          top[k] = m;
+          L[k] *= f;
+          acc[k].x *= f;
+          acc[k].y *= f;
+          acc[k].z *= f;
+          acc[k].w *= f;
+#pragma unroll 8
+          for (int i = 0; i < np; ++i) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(
+                                        a.part_acc + ((long long)slot_of(c_first + p0 + i) * G + h) * D) + d);
+            const float2 r = ml[i * G + h];
+            const float w = r.x == m ? 1.f : ex2_ftz(r.x - m);
+            L[k] = fmaf(r.y, w, L[k]);
+            acc[k].x = fmaf(x.x, w, acc[k].x);
+            acc[k].y = fmaf(x.y, w, acc[k].y);
+            acc[k].z = fmaf(x.z, w, acc[k].z);
+            acc[k].w = fmaf(x.w, w, acc[k].w);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int item = threadIdx.x + k * kThreads;
+        if (item >= G * D / 4) continue;
+        const int h = item / (D / 4), d = item % (D / 4);
+        const float inv = (FMT == LARA_KVQ_FP8_E4M3 ? 256.f : 1.f) / L[k];
+        *reinterpret_cast<uint2*>(a.o + ((long long)u.b * a.n_q_heads + u.kvh * G + h) * D + 4 * d) =
+            make_uint2(pack2_rn(acc[k].x * inv, acc[k].y * inv), pack2_rn(acc[k].z * inv, acc[k].w * inv));
+      }
+    }
+    __syncthreads();  // s_flag and the merge area are free again
+  }
+  cp_async_wait<0>();
+}
+
+// Workspace: status word | partial results (two slots per CTA) | counters.
+struct Layout {
+  size_t ml_off, acc_off, counters_off, total;
+};
+
+template <int D, int NG>
+int max_ctas() {
+  return device_sm_count() * Cfg<D, NG>::kCtasPerSm;
+}
+
+int max_ctas(int head_dim) { return head_dim == 128 ? max_ctas<128, 1>() : max_ctas<64, 1>(); }
+
+Layout layout(int batch, int group, int n_kv_heads, int head_dim) {
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t slots = 2 * (size_t)max_ctas(head_dim);
+  Layout w;
+  w.ml_off = kStatusBytes;
+  w.acc_off = w.ml_off + up(slots * group * sizeof(float2));
+  w.counters_off = w.acc_off + up(slots * group * head_dim * sizeof(float));
+  w.total = w.counters_off + up((size_t)batch * n_kv_heads * sizeof(int));
+  return w;
+}
+
+template <int D, int FMT, int NG>
+cudaError_t launch(const KvqDecodeArgs& a, cudaStream_t stream) {
+  using C = Cfg<D, NG>;
+  const void* fn = reinterpret_cast<const void*>(&kvq_decode_kernel<D, FMT, NG>);
+  {
+    static std::mutex mu;
+    static uint64_t done = 0;  // the shared-memory opt-in is per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev > 63 || !(done >> dev & 1)) {
+      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+      if (e != cudaSuccess) return e;
+      if (dev <= 63) done |= 1ull << dev;
+    }
+  }
+  // no more CTAs than tiles of a full cache could feed
+  const long long tiles = (long long)a.batch * a.pool.n_kv_heads * ((a.index.capacity() + kTile - 1) / kTile);
+  const long long ctas = std::min<long long>(max_ctas<D, NG>(), (tiles + kMinTiles - 1) / kMinTiles);
+  KvqDecodeArgs args = a;
+  void* p[] = {&args};
+  return launch_with_pdl(fn, dim3((unsigned)ctas), dim3(kThreads), p, C::kSmemBytes, stream);
 }
 
 }  // namespace
@@ -105,7 +677,7 @@ using namespace lara;
 
 extern "C" size_t lara_kvq_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
   if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || head_dim < 1) return 0;
-  return kStatusBytes;
+  return layout(batch, (n_q_heads + n_kv_heads - 1) / n_kv_heads, n_kv_heads, head_dim).total;
 }
 
 extern "C" int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool, const int32_t* block_table,
@@ -124,23 +696,29 @@ extern "C" int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool,
   if (!q || !seq_lens || !o || !workspace) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
   if (!aligned(q, 16) || !aligned(o, 16) || !aligned(seq_lens, 4) || !aligned(workspace, 256))
     return set_last_error(LARA_ERR_STREAM_DEST, "q and o must be 16-byte aligned, the workspace 256-byte");
-  if (workspace_bytes < lara_kvq_decode_workspace_bytes(batch, n_q_heads, pool->n_kv_heads, pool->head_dim))
-    return set_last_error(LARA_ERR_RESULT_LEN, "decode workspace too small");
+  a.group = n_q_heads / pool->n_kv_heads;
+  const Layout w = layout(batch, a.group, pool->n_kv_heads, pool->head_dim);
+  if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "decode workspace too small");
   a.pool = *pool;
   a.q = q;
   a.lens = seq_lens;
   a.o = o;
+  a.batch = batch;
   a.n_q_heads = n_q_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.status = static_cast<int*>(workspace);
-  const dim3 grid(n_q_heads, batch);
+  char* base = static_cast<char*>(workspace);
+  a.status = reinterpret_cast<int*>(base);
+  a.part_ml = reinterpret_cast<float2*>(base + w.ml_off);
+  a.part_acc = reinterpret_cast<float*>(base + w.acc_off);
+  a.counters = reinterpret_cast<int*>(base + w.counters_off);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define LARA_CASE(d, f) \
-  if (pool->head_dim == d && pool->format == f) kvq_decode_kernel<d, f><<<grid, kWarps * 32, 0, st>>>(a);
+  cudaError_t e = cudaErrorInvalidValue;
+#define LARA_CASE(d, f)                                  \
+  if (pool->head_dim == d && pool->format == f)          \
+    e = a.group <= 8 ? launch<d, f, 1>(a, st) : launch<d, f, 2>(a, st);
   LARA_CASE(128, LARA_KVQ_INT8) LARA_CASE(128, LARA_KVQ_FP8_E4M3)
   LARA_CASE(64, LARA_KVQ_INT8) LARA_CASE(64, LARA_KVQ_FP8_E4M3)
 #undef LARA_CASE
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)
     return set_last_error(LARA_ERR_CUDA, std::string("kvq decode launch: ") + cudaGetErrorString(e));
   return LARA_OK;

@@ -146,7 +146,10 @@ def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=No
 
 
 def decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device="cuda:0") -> torch.Tensor:
-    """A zeroed workspace for :func:`gqa_decode_kvq` calls of up to this batch; one stream at a time uses it."""
+    """A zeroed workspace for :func:`gqa_decode_kvq` calls with these heads and up to this batch.
+
+    One stream at a time uses it.
+    """
     dev = torch.device(device)
     with _on_device(dev):
         return new_workspace(int(lib.lara_kvq_decode_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim)), dev)
@@ -218,8 +221,9 @@ class QuantKVCache(PagedKVCache):
         _check_words("q", q, (len(slots), q.shape[1], self.head_dim))
         _, table, lens = self._rows(slots)
         need = int(lib.lara_kvq_decode_workspace_bytes(len(slots), q.shape[1], self.n_kv_heads, self.head_dim))
-        if self._ws is None or self._ws.numel() < need:
+        if self._ws is None or self._ws_heads != q.shape[1] or self._ws.numel() < need:
             self._ws = decode_workspace(len(slots), q.shape[1], self.n_kv_heads, self.head_dim, self.device)
+            self._ws_heads = q.shape[1]
         return gqa_decode_kvq(q, self.pool, table, lens, scale=scale, workspace=self._ws)
 
     def read(self, slots=None, out=None):
