@@ -3,15 +3,20 @@
 // for a quantised cache).
 //
 // Both are bound by HBM: append reads 2 D bytes of bf16 per row and writes
-// D + 4, read the reverse.  D / 8 lanes hold a row, and a lane group takes the
-// K and the V row of one (token, kv head), so both loads are in flight.
+// D + 4, read the reverse.  D / 8 lanes hold a row.  A warp takes kRows times
+// as many consecutive tokens of one (sequence, kv head) as it has lane groups,
+// K and V: the length, the start and the page of a row are looked up once per
+// warp (at most 16 tokens, so at most two pages), not once per row, and all the
+// tokens' loads are in flight together.
+#include <algorithm>
+
 #include "kvq.cuh"
 
 namespace lara {
 
 namespace kvq {
 
-int check_pool(const lara_kvq_pool* pool, const void* block_table, int pages_per_seq, PoolIndex* index) {
+int check_pool(const lara_kvq_pool* pool, const void* block_table, int pages_per_seq, int batch, PoolIndex* index) {
   if (!pool) return set_last_error(LARA_ERR_STREAM_DEST, "null pool");
   if (pool->format != LARA_KVQ_INT8 && pool->format != LARA_KVQ_FP8_E4M3)
     return set_last_error(LARA_ERR_UNSUPPORTED, "unknown code format");
@@ -22,7 +27,7 @@ int check_pool(const lara_kvq_pool* pool, const void* block_table, int pages_per
     return set_last_error(LARA_ERR_BAD_CFG, "page_size must be a power of two in [16, 65536]");
   if (pool->num_pages < 1 || pool->n_kv_heads < 1 || pages_per_seq < 1 || (long long)pages_per_seq * ps > 0x7fffffffll)
     return set_last_error(LARA_ERR_BAD_CFG, "bad pool geometry");
-  if (!pool->k_codes || !pool->v_codes || !pool->k_scales || !pool->v_scales || !block_table)
+  if (!pool->k_codes || !pool->v_codes || !pool->k_scales || !pool->v_scales || (!block_table && batch > 0))
     return set_last_error(LARA_ERR_STREAM_DEST, "null pool or block table pointer");
   if (!aligned(pool->k_codes, 16) || !aligned(pool->v_codes, 16) || !aligned(pool->k_scales, 16) ||
       !aligned(pool->v_scales, 16) || !aligned(block_table, 4))
@@ -54,97 +59,151 @@ struct RowArgs {
   Heads<const uint16_t> k, v;
   Heads<uint16_t> ko, vo;
   int batch, n;
-  uint32_t rows;
+  uint32_t tiles;          // warps' worth of work
+  FastDiv div_tiles, div_h;  // tiles per (sequence, kv head); kv heads
   int* status;
 };
 
-template <int D, int FMT, bool kVec>
+// A warp's tokens t0 .. t0 + kTokens - 1 of (b, h), and where their rows lie in
+// the pool: row p (a position in the sequence) is base + p, on its second page
+// base2 + p; a negative base is a bad page.
+template <int kTokens>
+struct WarpRows {
+  uint32_t b, h;
+  int t0, cross;
+  long long start, base, base2;
+  __device__ __forceinline__ bool init(const RowArgs& a) {
+    const uint32_t w = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / 32;
+    if (w >= a.tiles) return false;
+    uint32_t tile;
+    const uint32_t bh = a.div_tiles.div(w, tile);
+    b = a.div_h.div(bh, h);
+    t0 = tile * kTokens;
+    start = a.starts ? a.starts[b] : 0;
+    return true;
+  }
+  // The pages of positions [lo, hi], which span at most kTokens.
+  __device__ __forceinline__ void find(const RowArgs& a, long long lo, long long hi) {
+    const int log2 = a.index.page_log2;
+    cross = (int)((lo >> log2) + 1) << log2;
+    const long long first = a.index.row(b, h, (int)lo, a.status);
+    const long long second = hi >= cross ? a.index.row(b, h, cross, a.status) : 0;
+    base = first < 0 ? kBad : first - lo;
+    base2 = second < 0 ? kBad : second - cross;
+  }
+  __device__ __forceinline__ long long row(long long pos) const { return (pos < cross ? base : base2) + pos; }
+  static constexpr long long kBad = -(1ll << 62);
+};
+
+template <int D, int FMT, bool kVec, int kRows>
 __global__ void __launch_bounds__(kThreads) kvq_append_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int kLanes = D / 8;
-  const uint32_t tid = blockIdx.x * (uint32_t)kThreads + threadIdx.x;
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes;
+  allow_dependent_launch();
+  grid_dependency_wait();
   if (a.new_lens)
-    for (uint32_t b = tid; b < (uint32_t)a.batch; b += gridDim.x * (uint32_t)kThreads) {
+    for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.batch; b += gridDim.x * kThreads) {
       const int start = a.starts[b];
       const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
       a.new_lens[b] = start < 0 ? start : (int)min(end, max(a.index.capacity(), (long long)start));
     }
-  const uint32_t row = tid / kLanes;
-  if (row - (threadIdx.x & 31) / kLanes >= a.rows) return;  // the whole warp is past the end
-  const uint32_t r = min(row, a.rows - 1);
-  const int l = threadIdx.x % kLanes;
-  const int t = (int)(r % (uint32_t)a.n);
-  const uint32_t bh = r / (uint32_t)a.n;
-  const int h = (int)(bh % (uint32_t)a.pool.n_kv_heads), b = (int)(bh / (uint32_t)a.pool.n_kv_heads);
+  WarpRows<kRows * kGroups> rows;
+  if (!rows.init(a)) return;
+  const int l = threadIdx.x % kLanes, t = rows.t0 + (threadIdx.x & 31) / kLanes;
+  uint32_t w[kRows][2][4];
+#pragma unroll
+  for (int j = 0; j < kRows; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint16_t* src = (i ? a.v : a.k).row(rows.b, min(t + j * kGroups, a.n - 1), rows.h) + 8 * l;
+      if constexpr (kVec) {
+        *reinterpret_cast<uint4*>(w[j][i]) = __ldcs(reinterpret_cast<const uint4*>(src));  // read once
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) w[j][i][m] = (uint32_t)src[2 * m] | ((uint32_t)src[2 * m + 1] << 16);
+      }
+    }
   int count = a.n;
   if (a.counts) {
-    count = a.counts[b];
+    count = a.counts[rows.b];
     if ((count < 0 || count > a.n) && a.status) atomicOr(a.status, kDevBadLength);
+    count = min(max(count, 0), a.n);
   }
-  const int start = a.starts[b];
-  const long long pos = (long long)start + t;
-  long long dst = -1;
-  if (row < a.rows && t < count) {
-    if (start < 0 || pos >= a.index.capacity()) {
-      if (a.status) atomicOr(a.status, kDevAppendOverflow);
-    } else {
-      dst = a.index.row(b, h, (int)pos, a.status);
-    }
+  // tokens [t0, end) have a place in the sequence
+  int end = min(rows.t0 + kRows * kGroups, count);
+  if (end > rows.t0 && (rows.start < 0 || rows.start + end > a.index.capacity())) {
+    if (a.status) atomicOr(a.status, kDevAppendOverflow);
+    end = rows.start < 0 ? rows.t0 : (int)min((long long)end, a.index.capacity() - rows.start);
   }
-  uint32_t w[2][4];
+  if (end <= rows.t0) return;
+  rows.find(a, rows.start + rows.t0, rows.start + end - 1);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint16_t* src = (i ? a.v : a.k).row(b, t, h) + 8 * l;
-    if constexpr (kVec) {
-      *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(src);
-    } else {
+  for (int j = 0; j < kRows; ++j) {
+    const long long dst = rows.row(rows.start + t + j * kGroups);
+    const bool store = t + j * kGroups < end && dst >= 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[i][j] = (uint32_t)src[2 * j] | ((uint32_t)src[2 * j + 1] << 16);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint32_t codes[2];
-    const float scale = quantise_row<D, FMT>(w[i], codes);
-    if (dst >= 0) {
-      *reinterpret_cast<uint2*>((i ? a.pool.v_codes : a.pool.k_codes) + dst * D + 8 * l) =
-          make_uint2(codes[0], codes[1]);
-      if (l == 0) (i ? a.pool.v_scales : a.pool.k_scales)[dst] = scale;
+    for (int i = 0; i < 2; ++i) {
+      uint32_t codes[2];
+      const float scale = quantise_row<D, FMT>(w[j][i], codes);
+      if (store) {
+        *reinterpret_cast<uint2*>((i ? a.pool.v_codes : a.pool.k_codes) + dst * D + 8 * l) =
+            make_uint2(codes[0], codes[1]);
+        if (l == 0) (i ? a.pool.v_scales : a.pool.k_scales)[dst] = scale;
+      }
     }
   }
 }
 
-template <int D, int FMT, bool kVec>
+template <int D, int FMT, bool kVec, int kRows>
 __global__ void __launch_bounds__(kThreads) kvq_read_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int kLanes = D / 8;
-  const uint32_t row = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / kLanes;
-  if (row >= a.rows) return;
-  const int l = threadIdx.x % kLanes;
-  const int t = (int)(row % (uint32_t)a.n);
-  const uint32_t bh = row / (uint32_t)a.n;
-  const int h = (int)(bh % (uint32_t)a.pool.n_kv_heads), b = (int)(bh / (uint32_t)a.pool.n_kv_heads);
-  const int len = a.counts[b];
-  if ((len < 0 || len > a.index.capacity()) && a.status) atomicOr(a.status, kDevBadLength);
-  const long long pos = (a.starts ? (long long)a.starts[b] : 0) + t;
-  long long src = -1;
-  if (pos >= 0 && pos < len && pos < a.index.capacity()) src = a.index.row(b, h, (int)pos, a.status);
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes;
+  allow_dependent_launch();
+  grid_dependency_wait();
+  WarpRows<kRows * kGroups> rows;
+  if (!rows.init(a)) return;
+  const int l = threadIdx.x % kLanes, t = rows.t0 + (threadIdx.x & 31) / kLanes;
+  const int given = a.counts[rows.b];
+  const int len = min(max(given, 0), (int)a.index.capacity());
+  if (given != len && a.status) atomicOr(a.status, kDevBadLength);
+  // positions [lo, hi) of the warp's tokens are cached
+  const long long lo = max(rows.start + rows.t0, 0ll), hi = min(rows.start + rows.t0 + kRows * kGroups, (long long)len);
+  if (lo < hi) rows.find(a, lo, hi - 1);
+  uint2 c[kRows][2];
+  float scale[kRows][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (src >= 0) {
-      const uint2 c = *reinterpret_cast<const uint2*>((i ? a.pool.v_codes : a.pool.k_codes) + src * D + 8 * l);
-      const float scale = (i ? a.pool.v_scales : a.pool.k_scales)[src];
-      float f[8];
-      codes_to_f32<FMT>(c.x, f);
-      codes_to_f32<FMT>(c.y, f + 4);
+  for (int j = 0; j < kRows; ++j) {
+    const long long pos = rows.start + t + j * kGroups;
+    c[j][0] = c[j][1] = make_uint2(0, 0);
+    scale[j][0] = scale[j][1] = 0.f;
+    if (pos < lo || pos >= hi) continue;
+    const long long src = rows.row(pos);
+    if (src < 0) continue;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack2_rn(f[2 * j] * scale, f[2 * j + 1] * scale);
+    for (int i = 0; i < 2; ++i) {
+      c[j][i] = *reinterpret_cast<const uint2*>((i ? a.pool.v_codes : a.pool.k_codes) + src * D + 8 * l);
+      scale[j][i] = (i ? a.pool.v_scales : a.pool.k_scales)[src];
     }
-    uint16_t* dst = (i ? a.vo : a.ko).row(b, t, h) + 8 * l;
-    if constexpr (kVec) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+  }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dst[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+  for (int j = 0; j < kRows; ++j) {
+    if (t + j * kGroups >= a.n) break;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float2 f[4];
+      codes_to_f32<FMT>(c[j][i].x, f);
+      codes_to_f32<FMT>(c[j][i].y, f + 2);
+      uint32_t w[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        f[m] = mul2(f[m], make_float2(scale[j][i], scale[j][i]));
+        w[m] = pack2_rn(f[m].x, f[m].y);
+      }
+      uint16_t* dst = (i ? a.vo : a.ko).row(rows.b, t + j * kGroups, rows.h) + 8 * l;
+      if constexpr (kVec) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) dst[m] = (uint16_t)(w[m / 2] >> (16 * (m & 1)));
+      }
     }
   }
 }
@@ -155,19 +214,47 @@ bool vec_ok(const void* p, long long sb, int batch, long long sh, int heads, lon
   return aligned(p, 16) && (((batch > 1 ? sb : 0) | (heads > 1 ? sh : 0) | (n > 1 ? st : 0)) & 7) == 0;
 }
 
-// rows = batch * Hkv * n as a launch over D / 8 lanes each, or 0 when it does not fit one.
-long long row_blocks(const lara_kvq_pool& pool, int batch, int n, uint32_t* rows) {
-  const long long bh = (long long)batch * pool.n_kv_heads;
-  if (bh > 0x7fffffffll || bh * n > 0x7fffffffll / (pool.head_dim / 8)) return -1;
-  *rows = (uint32_t)(bh * n);
-  return (bh * n * (pool.head_dim / 8) + kThreads - 1) / kThreads;
+// Whether the rows of a call (at least one per warp) fit one launch.
+bool set_rows(RowArgs* a, const lara_kvq_pool& pool, int batch, int n) {
+  a->pool = pool;
+  a->batch = batch;
+  a->n = n;
+  a->div_h = FastDiv((uint32_t)pool.n_kv_heads);
+  return (long long)batch * pool.n_kv_heads <= 0x3ffffffll &&
+         (long long)batch * pool.n_kv_heads * n <= 0x3ffffffll;
 }
 
-template <typename F>
-cudaError_t launch_rows(F kernel, long long blocks, const RowArgs& a, void* stream) {
-  kernel<<<(unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  return cudaGetLastError();
+// Rows per lane group: with enough work for every SM, two (four tokens per
+// warp) halve the look-ups and keep the most bytes in flight; one row each is
+// quicker below that.  8192 tokens of 8 x 8 heads read back (head_dim 128): one
+// 76, two 70, four 78, eight 84 us; 2048 of 8 x 8 appended and read: one 50,
+// two 43, four 45, eight 51 us.
+constexpr int many(int d) { return d == 128 ? 2 : 1; }
+
+template <int D>
+cudaError_t launch_rows(const void* one, const void* several, RowArgs a, void* stream) {
+  constexpr int kGroups = 256 / D;
+  const long long bh = (long long)a.batch * a.pool.n_kv_heads;
+  const bool few = bh * a.n < (long long)device_sm_count() * 32 * many(D) * kGroups;
+  const int tokens = kGroups * (few ? 1 : many(D));
+  const int tiles = (a.n + tokens - 1) / tokens;
+  a.div_tiles = FastDiv((uint32_t)std::max(tiles, 1));
+  a.tiles = (uint32_t)(bh * tiles);
+  const unsigned blocks = std::max(1u, (a.tiles + kThreads / 32 - 1) / (kThreads / 32));  // no rows: new_lens alone
+  void* args[] = {&a};
+  return launch_with_pdl(few ? one : several, dim3(blocks), dim3(kThreads), args, 0,
+                         static_cast<cudaStream_t>(stream));
 }
+
+#define LARA_KVQ_LAUNCH(kernel, d, f, v)                                                             \
+  if (pool->head_dim == d && pool->format == f && vec == v)                                         \
+    e = launch_rows<d>(reinterpret_cast<const void*>(&kernel<d, f, v, 1>),                           \
+                       reinterpret_cast<const void*>(&kernel<d, f, v, many(d)>), a, stream);
+#define LARA_KVQ_LAUNCH_ALL(kernel)                                                                   \
+  LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_INT8, true) LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_INT8, false) \
+  LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_FP8_E4M3, true) LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_FP8_E4M3, false) \
+  LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_INT8, true) LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_INT8, false) \
+  LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_FP8_E4M3, true) LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_FP8_E4M3, false)
 
 bool overlap(const void* a, const void* b, size_t bytes) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
@@ -186,7 +273,7 @@ extern "C" int lara_kvq_append(const lara_kvq_pool* pool, const int32_t* block_t
                                long long v_sh, long long v_st, int batch, int n_new, void* workspace, void* stream) {
   LARA_NVTX("lara_kvq_append");
   RowArgs a{};
-  if (const int rc = check_pool(pool, block_table, pages_per_seq, &a.index)) return rc;
+  if (const int rc = check_pool(pool, block_table, pages_per_seq, batch, &a.index)) return rc;
   if (batch < 0 || n_new < 0) return set_last_error(LARA_ERR_BAD_CFG, "batch and n_new must not be negative");
   if (batch == 0) return LARA_OK;
   if (!starts || (n_new > 0 && (!k_new || !v_new))) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
@@ -195,32 +282,19 @@ extern "C" int lara_kvq_append(const lara_kvq_pool* pool, const int32_t* block_t
     return set_last_error(LARA_ERR_STREAM_DEST, "misaligned buffer");
   if (overlap(new_lens, starts, 4 * (size_t)batch) || overlap(new_lens, counts, 4 * (size_t)batch))
     return set_last_error(LARA_ERR_STREAM_DEST, "new_lens must not overlap starts or counts");
-  a.pool = *pool;
   a.starts = starts;
   a.counts = counts;
   a.new_lens = new_lens;
   a.k = {k_new, k_sb, k_st, k_sh};
   a.v = {v_new, v_sb, v_st, v_sh};
-  a.batch = batch;
-  a.n = n_new;
   a.status = static_cast<int*>(workspace);
-  long long blocks = row_blocks(*pool, batch, n_new, &a.rows);
-  if (blocks < 0) return set_last_error(LARA_ERR_BAD_CFG, "too many rows for one launch");
-  if (blocks == 0) {
-    if (!new_lens) return LARA_OK;
-    blocks = 1;
-  }
+  if (!set_rows(&a, *pool, batch, n_new)) return set_last_error(LARA_ERR_BAD_CFG, "too many rows for one launch");
+  if (n_new == 0 && !new_lens) return LARA_OK;
   const int heads = pool->n_kv_heads;
   const bool vec = vec_ok(k_new, k_sb, batch, k_sh, heads, k_st, n_new) &&
                    vec_ok(v_new, v_sb, batch, v_sh, heads, v_st, n_new);
   cudaError_t e = cudaErrorInvalidValue;
-#define LARA_CASE(d, f)                                                                        \
-  if (pool->head_dim == d && pool->format == f)                                                \
-    e = vec ? launch_rows(kvq_append_kernel<d, f, true>, blocks, a, stream)                    \
-            : launch_rows(kvq_append_kernel<d, f, false>, blocks, a, stream);
-  LARA_CASE(128, LARA_KVQ_INT8) LARA_CASE(128, LARA_KVQ_FP8_E4M3)
-  LARA_CASE(64, LARA_KVQ_INT8) LARA_CASE(64, LARA_KVQ_FP8_E4M3)
-#undef LARA_CASE
+  LARA_KVQ_LAUNCH_ALL(kvq_append_kernel)
   if (e != cudaSuccess)
     return set_last_error(LARA_ERR_CUDA, std::string("kvq_append launch: ") + cudaGetErrorString(e));
   return LARA_OK;
@@ -232,34 +306,24 @@ extern "C" int lara_kvq_read(const lara_kvq_pool* pool, const int32_t* block_tab
                              long long v_st, int batch, int n_tokens, void* workspace, void* stream) {
   LARA_NVTX("lara_kvq_read");
   RowArgs a{};
-  if (const int rc = check_pool(pool, block_table, pages_per_seq, &a.index)) return rc;
+  if (const int rc = check_pool(pool, block_table, pages_per_seq, batch, &a.index)) return rc;
   if (batch < 0 || n_tokens < 0) return set_last_error(LARA_ERR_BAD_CFG, "batch and n_tokens must not be negative");
   if (batch == 0 || n_tokens == 0) return LARA_OK;
   if (!seq_lens || !k_out || !v_out) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
   if (!aligned(k_out, 2) || !aligned(v_out, 2) || !aligned(starts, 4) || !aligned(seq_lens, 4) ||
       !aligned(workspace, 4))
     return set_last_error(LARA_ERR_STREAM_DEST, "misaligned buffer");
-  a.pool = *pool;
   a.starts = starts;
   a.counts = seq_lens;
   a.ko = {k_out, k_sb, k_st, k_sh};
   a.vo = {v_out, v_sb, v_st, v_sh};
-  a.batch = batch;
-  a.n = n_tokens;
   a.status = static_cast<int*>(workspace);
-  const long long blocks = row_blocks(*pool, batch, n_tokens, &a.rows);
-  if (blocks < 0) return set_last_error(LARA_ERR_BAD_CFG, "too many rows for one launch");
+  if (!set_rows(&a, *pool, batch, n_tokens)) return set_last_error(LARA_ERR_BAD_CFG, "too many rows for one launch");
   const int heads = pool->n_kv_heads;
   const bool vec = vec_ok(k_out, k_sb, batch, k_sh, heads, k_st, n_tokens) &&
                    vec_ok(v_out, v_sb, batch, v_sh, heads, v_st, n_tokens);
   cudaError_t e = cudaErrorInvalidValue;
-#define LARA_CASE(d, f)                                                                        \
-  if (pool->head_dim == d && pool->format == f)                                                \
-    e = vec ? launch_rows(kvq_read_kernel<d, f, true>, blocks, a, stream)                      \
-            : launch_rows(kvq_read_kernel<d, f, false>, blocks, a, stream);
-  LARA_CASE(128, LARA_KVQ_INT8) LARA_CASE(128, LARA_KVQ_FP8_E4M3)
-  LARA_CASE(64, LARA_KVQ_INT8) LARA_CASE(64, LARA_KVQ_FP8_E4M3)
-#undef LARA_CASE
+  LARA_KVQ_LAUNCH_ALL(kvq_read_kernel)
   if (e != cudaSuccess)
     return set_last_error(LARA_ERR_CUDA, std::string("kvq_read launch: ") + cudaGetErrorString(e));
   return LARA_OK;

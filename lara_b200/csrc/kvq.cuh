@@ -22,22 +22,6 @@ struct Heads {
   __device__ __forceinline__ T* row(int b, int t, int h) const { return p + b * sb + t * st + h * sh; }
 };
 
-// Eight values as two runs of four at element offsets o0 and o1.  kVec: 8-byte
-// accesses (the row is 8-byte aligned), else one element at a time.
-template <bool kVec>
-__device__ __forceinline__ void load8(const uint16_t* row, int o0, int o1, float x[8]) {
-  if constexpr (kVec) {
-    bf16x4_to_f32(*reinterpret_cast<const uint2*>(row + o0), x);
-    bf16x4_to_f32(*reinterpret_cast<const uint2*>(row + o1), x + 4);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = __uint_as_float((uint32_t)row[o0 + j] << 16);
-      x[4 + j] = __uint_as_float((uint32_t)row[o1 + j] << 16);
-    }
-  }
-}
-
 // Round to nearest even; NaN stays NaN (the reference packer's carry could
 // turn a NaN's payload over, and a NaN row has to read as one).
 __device__ __forceinline__ uint32_t pack2_rn(float lo, float hi) {
@@ -45,67 +29,200 @@ __device__ __forceinline__ uint32_t pack2_rn(float lo, float hi) {
   return reinterpret_cast<const uint32_t&>(v);
 }
 
-template <bool kVec>
-__device__ __forceinline__ void store8(uint16_t* row, int o0, int o1, const uint32_t w[4]) {
-  if constexpr (kVec) {
-    *reinterpret_cast<uint2*>(row + o0) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(row + o1) = make_uint2(w[2], w[3]);
+// Two fp32 values that one instruction works on.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+        "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+
+// n / d for 0 <= n < 2^31 by one multiplication: with s = 31 + ceil(log2 d) and
+// m = floor(2^s / d) + 1, n m / 2^s exceeds n / d by less than 1 / d.
+struct FastDiv {
+  uint32_t d, m, shift;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t divisor) : d(divisor), m(0), shift(0) {
+    if (d > 1) {
+      uint32_t lg = 0;
+      while ((1ull << lg) < d) ++lg;
+      shift = lg - 1;
+      m = (uint32_t)((1ull << (31 + lg)) / d + 1);
+    }
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n, uint32_t& rest) const {
+    const uint32_t q = d > 1 ? __umulhi(n, m) >> shift : n;
+    rest = n - q * d;
+    return q;
+  }
+};
+
+// How the q/k pass holds a head: D / 8 lanes, eight dims each, kept as four
+// rotation pairs: a[j] and b[j] make pair 4 * lane + j of the table.  Pairs
+// (2i, 2i+1) lie side by side in memory; pairs (i, i + rot/2) meet in one lane
+// because the first rot/8 lanes take four dims of each half, so the rotation
+// needs no exchange.  Lanes past rot hold eight dims in a row and do not rotate.
+struct HeadLane {
+  int o0, o1;      // the lane's two runs of four dims
+  bool rotated;
+  __device__ __forceinline__ HeadLane(int lane, int rot, bool interleaved) {
+    rotated = 8 * lane < rot;
+    const bool split = rotated && !interleaved;
+    o0 = split ? 4 * lane : 8 * lane;
+    o1 = split ? rot / 2 + 4 * lane : 8 * lane + 4;
+  }
+};
+
+// The lane's eight values as pairs: a = (x_a of pairs 0, 1), (2, 3); b alike.
+struct Pairs {
+  float2 a[2], b[2];
+};
+
+template <bool kInter, bool kVec>
+__device__ __forceinline__ Pairs load_pairs(const uint16_t* row, const HeadLane& ld) {
+  uint32_t w[4];
+  if constexpr (kVec && kInter) {
+    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(row + ld.o0);
+  } else if constexpr (kVec) {
+    *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(row + ld.o0);
+    *reinterpret_cast<uint2*>(w + 2) = *reinterpret_cast<const uint2*>(row + ld.o1);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      row[o0 + j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
-      row[o1 + j] = (uint16_t)(w[2 + j / 2] >> (16 * (j & 1)));
+      const uint16_t* p = row + (j < 2 ? ld.o0 + 2 * j : ld.o1 + 2 * j - 4);
+      w[j] = (uint32_t)p[0] | ((uint32_t)p[1] << 16);
+    }
+  }
+  Pairs x;
+  if constexpr (kInter) {
+    x.a[0] = make_float2(bf16lo(w[0]), bf16lo(w[1]));
+    x.b[0] = make_float2(bf16hi(w[0]), bf16hi(w[1]));
+    x.a[1] = make_float2(bf16lo(w[2]), bf16lo(w[3]));
+    x.b[1] = make_float2(bf16hi(w[2]), bf16hi(w[3]));
+  } else {
+    x.a[0] = make_float2(bf16lo(w[0]), bf16hi(w[0]));
+    x.a[1] = make_float2(bf16lo(w[1]), bf16hi(w[1]));
+    x.b[0] = make_float2(bf16lo(w[2]), bf16hi(w[2]));
+    x.b[1] = make_float2(bf16lo(w[3]), bf16hi(w[3]));
+  }
+  return x;
+}
+
+template <bool kInter>
+__device__ __forceinline__ void pack_pairs(const Pairs& x, uint32_t w[4]) {
+  if constexpr (kInter) {
+    w[0] = pack2_rn(x.a[0].x, x.b[0].x);
+    w[1] = pack2_rn(x.a[0].y, x.b[0].y);
+    w[2] = pack2_rn(x.a[1].x, x.b[1].x);
+    w[3] = pack2_rn(x.a[1].y, x.b[1].y);
+  } else {
+    w[0] = pack2_rn(x.a[0].x, x.a[0].y);
+    w[1] = pack2_rn(x.a[1].x, x.a[1].y);
+    w[2] = pack2_rn(x.b[0].x, x.b[0].y);
+    w[3] = pack2_rn(x.b[1].x, x.b[1].y);
+  }
+}
+
+template <bool kInter, bool kVec>
+__device__ __forceinline__ void store_pairs(uint16_t* row, const HeadLane& ld, const uint32_t w[4]) {
+  if constexpr (kVec && kInter) {
+    *reinterpret_cast<uint4*>(row + ld.o0) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if constexpr (kVec) {
+    *reinterpret_cast<uint2*>(row + ld.o0) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(row + ld.o1) = make_uint2(w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint16_t* p = row + (j < 2 ? ld.o0 + 2 * j : ld.o1 + 2 * j - 4);
+      p[0] = (uint16_t)w[j];
+      p[1] = (uint16_t)(w[j] >> 16);
     }
   }
 }
 
-// Which dims a lane of a row holds: pairs (2i, 2i+1) lie side by side; pairs
-// (i, i + rot/2) are brought together in one lane by giving the first rot/8
-// lanes four dims of each half, so the rotation needs no exchange.
-struct LaneDims {
-  int o0, o1;
-  bool rotated;
-  __device__ __forceinline__ LaneDims(int lane_in_row, int rot, bool interleaved) {
-    rotated = 8 * lane_in_row < rot;
-    const bool split = rotated && !interleaved;
-    o0 = split ? 4 * lane_in_row : 8 * lane_in_row;
-    o1 = split ? rot / 2 + 4 * lane_in_row : 8 * lane_in_row + 4;
-  }
+// What a token and a weight vector make of a pair, (a', b') = inv * (a ac - b bs,
+// a as + b bc): the weights are folded into the cosines and sines once per
+// token, so a head costs four products per pair and one with inv.
+struct Turn {
+  float2 ac[2], bs[2], as[2], bc[2];  // bs holds -w_b s
 };
 
-// Norm of one row: the sum of squares and every product in fp32, each step
-// written out so that all kernels that norm a row round alike.
-template <int D>
-__device__ __forceinline__ void norm_row(float x[8], const float w[8], float eps) {
-  float ss = 0.f;
+template <bool kInter>
+__device__ __forceinline__ Turn make_turn(const float4& c, const float4& s, const uint16_t* weight,
+                                          const HeadLane& ld) {
+  Turn t;
+  const float2 c2[2] = {make_float2(c.x, c.y), make_float2(c.z, c.w)};
+  const float2 s2[2] = {make_float2(s.x, s.y), make_float2(s.z, s.w)};
+  const float2 m2[2] = {make_float2(-s.x, -s.y), make_float2(-s.z, -s.w)};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) ss = __fmaf_rn(x[j], x[j], ss);
-#pragma unroll
-  for (int off = D / 16; off > 0; off >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, off));
-  const float inv = __frsqrt_rn(__fmaf_rn(ss, 1.f / D, eps));
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], inv), w[j]);
-}
-
-__device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s) {
-  const float y = __fmaf_rn(a, c, -__fmul_rn(b, s));
-  b = __fmaf_rn(a, s, __fmul_rn(b, c));
-  a = y;
-}
-
-// Pair j of the lane has table index 4 * lane_in_row + j in either pairing.
-__device__ __forceinline__ void rotate_row(float x[8], const float4& c, const float4& s, bool interleaved) {
-  if (interleaved) {
-    rotate_pair(x[0], x[1], c.x, s.x);
-    rotate_pair(x[2], x[3], c.y, s.y);
-    rotate_pair(x[4], x[5], c.z, s.z);
-    rotate_pair(x[6], x[7], c.w, s.w);
-  } else {
-    rotate_pair(x[0], x[4], c.x, s.x);
-    rotate_pair(x[1], x[5], c.y, s.y);
-    rotate_pair(x[2], x[6], c.z, s.z);
-    rotate_pair(x[3], x[7], c.w, s.w);
+  for (int i = 0; i < 2; ++i) {
+    t.ac[i] = t.bc[i] = c2[i];
+    t.as[i] = s2[i];
+    t.bs[i] = m2[i];
   }
+  if (weight) {
+    const Pairs w = load_pairs<kInter, true>(weight, ld);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t.ac[i] = mul2(t.ac[i], w.a[i]);
+      t.as[i] = mul2(t.as[i], w.a[i]);
+      t.bs[i] = mul2(t.bs[i], w.b[i]);
+      t.bc[i] = mul2(t.bc[i], w.b[i]);
+    }
+  }
+  return t;
+}
+
+// One head: the norm's factor (sum of squares in fp32) and the turn.  Every
+// step is a packed operation with its rounding, so all kernels that treat a
+// head give the same words.
+template <int D, bool kNorm>
+__device__ __forceinline__ Pairs turn_head(const Pairs& x, const Turn& t, bool rotated, float eps) {
+  Pairs y;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    y.a[i] = fma2(x.a[i], t.ac[i], mul2(x.b[i], t.bs[i]));
+    y.b[i] = fma2(x.a[i], t.as[i], mul2(x.b[i], t.bc[i]));
+  }
+  if (!rotated)  // an infinity in one dim stays out of its neighbour's
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      y.a[i] = mul2(x.a[i], t.ac[i]);
+      y.b[i] = mul2(x.b[i], t.bc[i]);
+    }
+  if constexpr (kNorm) {
+    float2 q = mul2(x.a[0], x.a[0]);
+    q = fma2(x.b[0], x.b[0], q);
+    q = fma2(x.a[1], x.a[1], q);
+    q = fma2(x.b[1], x.b[1], q);
+    float ss = __fadd_rn(q.x, q.y);
+#pragma unroll
+    for (int off = D / 16; off > 0; off >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, off));
+    const float inv = rsqrtf(__fmaf_rn(ss, 1.f / D, eps));
+    const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      y.a[i] = mul2(y.a[i], inv2);
+      y.b[i] = mul2(y.b[i], inv2);
+    }
+  }
+  return y;
 }
 
 constexpr uint32_t kTinyBits = 0x0D800000u;  // 2^-100 as fp32
@@ -126,26 +243,30 @@ __device__ __forceinline__ uint32_t row_amax(const uint32_t w[4]) {
 template <int D, int FMT>
 __device__ __forceinline__ float quantise_row(const uint32_t w[4], uint32_t codes[2]) {
   const uint32_t am = row_amax<D>(w);
-  const bool finite = am < 0x7f80u;
-  float x[8];
+  float2 x[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf16lo(w[i]);
-    x[2 * i + 1] = bf16hi(w[i]);
-  }
+  for (int i = 0; i < 4; ++i) x[i] = make_float2(bf16lo(w[i]), bf16hi(w[i]));
   float scale;
   if constexpr (FMT == LARA_KVQ_INT8) {
-    // 127 x is exact in fp32 (8 + 7 bits; rows past 2^100 are brought down by
-    // 2^-16 first, so that it stays finite) and the quotient is rounded once,
-    // so a code sits on a tie only where 127 x / a itself does.
-    const float down = am >= 0x7180u ? 0x1p-16f : 1.f;
-    const float a = __uint_as_float(max(am << 16, kTinyBits)) * down;
-    scale = __fdiv_rn(a, 127.f) / down;
-    uint32_t c[8];
+    // rint of the exact quotient 127 x / a, ties to even, from y = x (127 / a)
+    // with two roundings.  For bf16 x and a a quotient is either a tie exactly
+    // or at least 2^-17 of itself away from one, so y rounded to 18 significant
+    // bits (65 y - (65 y - y)) lies on the tie or on the quotient's side of it.
+    // Adding 1.5 * 2^23 then rounds to an integer, in the sum's low byte.
+    const float a = __uint_as_float(max(am << 16, kTinyBits));
+    scale = __fdiv_rn(a, 127.f);
+    const float r = __fdiv_rn(127.f, a);
+    const float2 r2 = make_float2(r, r), k65 = make_float2(65.f, 65.f), neg = make_float2(-1.f, -1.f);
+    const float2 magic = make_float2(0x1.8p23f, 0x1.8p23f);
+    uint32_t c[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = (uint32_t)__float2int_rn(__fdiv_rn(127.f * (x[j] * down), a)) & 0xffu;
-    codes[0] = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
-    codes[1] = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
+    for (int i = 0; i < 4; ++i) {
+      const float2 y = mul2(x[i], r2), y65 = mul2(y, k65);
+      const float2 n = add2(fma2(fma2(y, neg, y65), neg, y65), magic);
+      c[i] = __byte_perm(__float_as_uint(n.x), __float_as_uint(n.y), 0x0040);
+    }
+    codes[0] = __byte_perm(c[0], c[1], 0x5410);
+    codes[1] = __byte_perm(c[2], c[3], 0x5410);
   } else {
     // a = (1 + m/128) 2^(E-127); 448 = 1.75 * 2^8, and 1 + m/128 <= 1.75 at m <= 96.
     const int e = max((int)(am >> 7) - 135 + ((am & 0x7fu) > 96u ? 1 : 0), -100);
@@ -154,30 +275,34 @@ __device__ __forceinline__ float quantise_row(const uint32_t w[4], uint32_t code
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      h[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inv, x[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    codes[0] = h[0] | (h[1] << 16);
-    codes[1] = h[2] | (h[3] << 16);
+      h[i] = __nv_cvt_float2_to_fp8x2(mul2(x[i], make_float2(inv, inv)), __NV_SATFINITE, __NV_E4M3);
+    codes[0] = __byte_perm(h[0], h[1], 0x5410);
+    codes[1] = __byte_perm(h[2], h[3], 0x5410);
   }
-  if (!finite) {
+  if (am >= 0x7f80u) {
     codes[0] = codes[1] = 0;
     scale = __uint_as_float(0x7fffffffu);
   }
   return scale;
 }
 
-// Four codes as fp32.
+// Four codes as fp32, as pairs (0, 1) and (2, 3).
 template <int FMT>
-__device__ __forceinline__ void codes_to_f32(uint32_t w, float f[4]) {
+__device__ __forceinline__ void codes_to_f32(uint32_t w, float2 f[2]) {
   if constexpr (FMT == LARA_KVQ_INT8) {
+    // 2^23 + code + 128 by setting the upper bytes, minus 2^23 + 128
+    const uint32_t x = w ^ 0x80808080u;
+    const float2 bias = make_float2(-8388736.f, -8388736.f);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = (float)(int8_t)(w >> (8 * j));
+    for (int i = 0; i < 2; ++i)
+      f[i] = add2(make_float2(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7650 + 2 * i)),
+                              __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7651 + 2 * i))),
+                  bias);
   } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * j)), __NV_E4M3);
-      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      f[2 * j] = p.x;
-      f[2 * j + 1] = p.y;
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+      f[i] = __half22float2(*reinterpret_cast<const __half2*>(&h));
     }
   }
 }
@@ -199,7 +324,8 @@ struct PoolIndex {
 };
 
 // Host: the pool's pointers and geometry, checked; LARA_OK or an error code.
-int check_pool(const lara_kvq_pool* pool, const void* block_table, int pages_per_seq, PoolIndex* index);
+// Without sequences the block table may be null.
+int check_pool(const lara_kvq_pool* pool, const void* block_table, int pages_per_seq, int batch, PoolIndex* index);
 
 inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 

@@ -79,8 +79,12 @@ struct KvqDecodeArgs {
   float* part_acc;  // [2 * grid][group][D]
 };
 
+// 16 bytes from src + kSrc to dst + kDst (immediate offsets: one address pair
+// serves a tile's copies).
+template <int kDst, int kSrc>
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(kDst), "n"(kSrc)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -102,20 +106,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ float lds_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
+__device__ __forceinline__ float lg2_ftz(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Bytes 0 and 2 (even) and bytes 1 and 3 (odd) of four codes as fp16 pairs.
@@ -138,6 +132,7 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& even, uint32_
 
 // Where the 16-byte chunk c of a row lies in a stage, so that the eight lanes
 // of a shared-memory phase (rows 2t of V, or two rows of K) hit distinct banks.
+// Rows eight apart are laid out alike.
 template <int D>
 __device__ __forceinline__ uint32_t chunk_offset(int row, int c) {
   if constexpr (D == 128) return row * 128 + ((c ^ (row & 7)) << 4);
@@ -155,17 +150,17 @@ __device__ __forceinline__ int seq_tiles(const KvqDecodeArgs& a, int b, int* len
   return (len + kTile - 1) / kTile;
 }
 
-// A position in the end-to-end order of tiles: unit (b, kvh) starts at `base`.
+// A unit (b, kvh) in the end-to-end order of tiles; `base` is its first tile,
+// counted from the CTA's own first.
 struct Unit {
-  long long base;
-  int b, kvh, tiles, len;
+  int base, tiles, len, b, kvh;
   __device__ __forceinline__ void next(const KvqDecodeArgs& a) {
     base += tiles;
     if (++kvh == a.pool.n_kv_heads) {
       kvh = 0;
       do {
         ++b;
-        tiles = b < a.batch ? seq_tiles(a, b, &len) : 0x7fffffff;
+        tiles = b < a.batch ? seq_tiles(a, b, &len) : 0x3fffffff;
       } while (tiles == 0);
     }
   }
@@ -222,63 +217,73 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
   };
   const long long w0 = cta_start(blockIdx.x), w1 = cta_start(blockIdx.x + 1);
   if (w0 >= before && w0 < before + mine * hkv) {
-    Unit u{before, b_lo, 0, 0, 0};
+    Unit u{0, 0, 0, b_lo, 0};
     u.tiles = seq_tiles(a, u.b, &u.len);
-    while (w0 >= u.base + (long long)u.tiles * hkv) {  // by whole sequences (tiles may be 0)
-      u.base += (long long)u.tiles * hkv;
+    while (w0 >= before + (long long)u.tiles * hkv) {  // by whole sequences (tiles may be 0)
+      before += (long long)u.tiles * hkv;
       ++u.b;
       u.tiles = seq_tiles(a, u.b, &u.len);
     }
-    u.kvh = (int)((w0 - u.base) / u.tiles);
-    u.base += (long long)u.kvh * u.tiles;
+    u.kvh = (int)((w0 - before) / u.tiles);
+    u.base = (int)(before + (long long)u.kvh * u.tiles - w0);  // at most 0
     s_first = u;
   }
   __syncthreads();
+  const int share = (int)(w1 - w0);
 
   // ---- the warp's ring ----
-  const uint32_t ring = smem_addr(smem) + warp * (C::kStages * C::kStageBytes);
-  Unit pu = s_first;             // where the next tile to fetch lies
-  long long pid = w0 + warp;     // its number
-  int page[2];                   // its pages (one per 16 tokens), fetched a tile ahead
+  uint8_t* const ring = smem + warp * (C::kStages * C::kStageBytes);
+  constexpr int kChunks = D / 16, kRowsPer = 32 / kChunks;  // a warp copies kRowsPer rows (512 bytes) at a time
+  const uint32_t copy_even = chunk_offset<D>(lane / kChunks, lane % kChunks);
+  const uint32_t copy_odd = chunk_offset<D>(lane / kChunks + kRowsPer, lane % kChunks) - 512;
+  const uint32_t copy_scale = 2 * C::kRowsBytes + (lane & 3) * 16 + (lane < 4 ? 0 : kTile * 4);
+  Unit pu = s_first;     // where the next tile to fetch lies
+  int pid = warp;        // its number
+  int page[2];           // its pages (one per 16 tokens), fetched a tile ahead
+  const bool big_pages = a.index.page_log2 >= 5;
   auto fetch_pages = [&] {
-    if (pid >= w1) return;
+    if (pid >= share) return;
     while (pid >= pu.base + pu.tiles) pu.next(a);
-    const int pos = (int)(pid - pu.base) * kTile;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      page[i] = pos + 16 * i < pu.len
-                    ? __ldcg(a.index.block_table + (long long)pu.b * a.index.pages_per_seq + ((pos + 16 * i) >> a.index.page_log2))
-                    : 0;
+    const int pos = (pid - pu.base) * kTile;
+    const int32_t* entry = a.index.block_table + (long long)pu.b * a.index.pages_per_seq + (pos >> a.index.page_log2);
+    page[0] = __ldcg(entry);
+    page[1] = big_pages || pos + 16 >= pu.len ? 0 : __ldcg(entry + 1);
+  };
+  auto fetch_half = [&](uint32_t st, int half, int pg, int pos) {
+    if ((unsigned)pg >= (unsigned)a.index.num_pages) {
+      atomicOr(a.status, kDevBadPage);
+      pg = 0;
+    }
+    const long long row =
+        (((long long)pg * hkv + pu.kvh) << a.index.page_log2) + (pos & ((1 << a.index.page_log2) - 1));
+    const uint8_t* ks = a.pool.k_codes + row * D + lane * 16;
+    const uint8_t* vs = a.pool.v_codes + row * D + lane * 16;
+    const uint32_t even = st + half * (16 * D) + copy_even, odd = st + half * (16 * D) + copy_odd;
+    if constexpr (D == 128) {
+      cp_async16<0, 0>(even, ks);
+      cp_async16<512, 512>(odd, ks);
+      cp_async16<1024, 1024>(even, ks);
+      cp_async16<1536, 1536>(odd, ks);
+      cp_async16<C::kRowsBytes, 0>(even, vs);
+      cp_async16<C::kRowsBytes + 512, 512>(odd, vs);
+      cp_async16<C::kRowsBytes + 1024, 1024>(even, vs);
+      cp_async16<C::kRowsBytes + 1536, 1536>(odd, vs);
+    } else {
+      cp_async16<0, 0>(even, ks);
+      cp_async16<512, 512>(odd, ks);
+      cp_async16<C::kRowsBytes, 0>(even, vs);
+      cp_async16<C::kRowsBytes + 512, 512>(odd, vs);
+    }
+    if (lane < 8)  // 16 scales of K (lanes 0-3) and of V (lanes 4-7)
+      cp_async16<0, 0>(st + half * 64 + copy_scale,
+                       (lane < 4 ? a.pool.k_scales : a.pool.v_scales) + row + 4 * (lane & 3));
   };
   auto fetch_tile = [&](int stage) {
-    if (pid < w1) {
-      const uint32_t st = ring + stage * C::kStageBytes;
-      const int pos = (int)(pid - pu.base) * kTile;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (pos + 16 * i >= pu.len) break;
-        int pg = page[i];
-        if (pg < 0 || pg >= a.index.num_pages) {
-          atomicOr(a.status, kDevBadPage);
-          pg = 0;
-        }
-        const long long row = ((((long long)pg * hkv + pu.kvh) << a.index.page_log2) +
-                               ((pos + 16 * i) & ((1 << a.index.page_log2) - 1)));
-        constexpr int kChunks = D / 16, kRowsPer = 32 / kChunks;
-        const int r0 = lane / kChunks, c = lane % kChunks;
-        const uint8_t* ks = a.pool.k_codes + row * D + lane * 16;
-        const uint8_t* vs = a.pool.v_codes + row * D + lane * 16;
-#pragma unroll
-        for (int j = 0; j < 16 / kRowsPer; ++j) {
-          const uint32_t off = chunk_offset<D>(16 * i + j * kRowsPer + r0, c);
-          cp_async16(st + off, ks + j * 512);
-          cp_async16(st + C::kRowsBytes + off, vs + j * 512);
-        }
-        if (lane < 8) {  // 16 scales of K (lanes 0-3) and of V (lanes 4-7)
-          const float* sc = (lane < 4 ? a.pool.k_scales : a.pool.v_scales) + row + 4 * (lane & 3);
-          cp_async16(st + 2 * C::kRowsBytes + (lane < 4 ? 0 : kTile * 4) + (16 * i + 4 * (lane & 3)) * 4, sc);
-        }
-      }
+    if (pid < share) {
+      const uint32_t st = smem_addr(ring) + stage * C::kStageBytes;
+      const int pos = (pid - pu.base) * kTile;
+      fetch_half(st, 0, page[0], pos);
+      if (pos + 16 < pu.len) fetch_half(st, 1, big_pages ? page[0] : page[1], pos + 16);
       pid += kWarps;
       fetch_pages();
     }
@@ -288,16 +293,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
 #pragma unroll
   for (int s = 0; s < C::kStages - 1; ++s) fetch_tile(s);
 
+  // lane-constant places in a stage: the K chunks of rows g (+ 8, 16, 24), the
+  // V chunks of rows 2 t4 and 2 t4 + 1 (+ 8, 16, 24)
+  uint32_t k_at[D / 64], v_at[2];
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) k_at[c] = chunk_offset<D>(g, t4 * (D / 64) + c);
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+    v_at[r] = C::kRowsBytes + (D == 128 ? chunk_offset<D>(2 * t4 + r, g)
+                                        : chunk_offset<D>(2 * t4 + r, g >> 1) + 8 * (g & 1));
+
   // ---- units of this CTA ----
   int stage = 0;
-  long long id = w0 + warp;      // next tile to work on
+  int id = warp;         // next tile to work on
   Unit u = s_first;
-  for (; u.base < w1; u.next(a)) {
-    const long long end = min(w1, u.base + u.tiles);
+  for (; u.base < share; u.next(a)) {
+    const int end = min(share, u.base + u.tiles);
     // q of the group's heads as the 8-column operand: column g, rows in the
     // order in which codes_to_f16 hands out a lane's K bytes
     uint32_t qf[NG][KS][2];
-    float qs[NG][2];
+    float2 qs[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       const int h = n * 8 + g;
@@ -330,14 +345,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       // the score factor of heads 2 t4 and 2 t4 + 1, from the lanes that hold them
       const float f = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2 *
                       (FMT == LARA_KVQ_FP8_E4M3 ? 256.f : 1.f);
-      qs[n][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
-      qs[n][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+      qs[n].x = __shfl_sync(0xffffffffu, f, 8 * t4);
+      qs[n].y = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
     }
-    float R[NG][2], l[NG][2], o[NG][KS][4];
+    float R[NG][2], o[NG][KS][4];
+    float2 l2[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       R[n][0] = R[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
+      l2[n] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < KS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
@@ -346,72 +362,79 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       cp_async_wait<C::kStages - 2>();
       __syncwarp();
       fetch_tile(stage == 0 ? C::kStages - 1 : stage - 1);
-      const uint32_t st = ring + stage * C::kStageBytes;
+      const uint8_t* st = ring + stage * C::kStageBytes;
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
-      const int valid = u.len - (int)(id - u.base) * kTile;
 
-      // ---- scores: s[mb][n][..] of tokens 16 mb + g (0, 1) and + 8 (2, 3) ----
-      float s[2][NG][4], vsc[2][2], lw[2][2];
+      // ---- scores: s2[i][n], token 8 i + g of the tile, heads 2 t4 and 2 t4 + 1 ----
+      float s[2][NG][4];
+      uint32_t k[4][D / 16];
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb) {
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          *reinterpret_cast<uint4*>(k[i] + 4 * c) = *reinterpret_cast<const uint4*>(st + k_at[c] + i * 8 * D);
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
         for (int n = 0; n < NG; ++n) s[mb][n][0] = s[mb][n][1] = s[mb][n][2] = s[mb][n][3] = 0.f;
-        uint32_t k0[D / 16], k1[D / 16];
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const int ch = t4 * (D / 64) + c;
-          *reinterpret_cast<uint4*>(k0 + 4 * c) = lds128(st + chunk_offset<D>(16 * mb + g, ch));
-          *reinterpret_cast<uint4*>(k1 + 4 * c) = lds128(st + chunk_offset<D>(16 * mb + g + 8, ch));
-        }
+      for (int j = 0; j < KS; ++j)
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
+        for (int mb = 0; mb < 2; ++mb) {
           uint32_t a0, a1, a2, a3;
-          codes_to_f16<FMT>(k0[j], a0, a2);
-          codes_to_f16<FMT>(k1[j], a1, a3);
+          codes_to_f16<FMT>(k[2 * mb][j], a0, a2);
+          codes_to_f16<FMT>(k[2 * mb + 1][j], a1, a3);
 #pragma unroll
           for (int n = 0; n < NG; ++n) mma_f16(s[mb][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
         }
+      float2 s2[4][NG];
+      float vsc[4], lw[4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int tok = 16 * mb + 8 * r + g;
-          const bool in = tok < valid;
-          const float ks = lds_f32(st + 2 * C::kRowsBytes + tok * 4);
-          const float vs = lds_f32(st + 2 * C::kRowsBytes + kTile * 4 + tok * 4);
-          vsc[mb][r] = in ? vs : 0.f;
-          lw[mb][r] = fmaxf(__log2f(vs), -100.f);
+      for (int i = 0; i < 4; ++i) {
+        const float ks = *reinterpret_cast<const float*>(st + 2 * C::kRowsBytes + (8 * i + g) * 4);
+        vsc[i] = *reinterpret_cast<const float*>(st + 2 * C::kRowsBytes + (kTile + 8 * i + g) * 4);
+        lw[i] = fmaxf(lg2_ftz(vsc[i]), -100.f);
 #pragma unroll
-          for (int n = 0; n < NG; ++n)
+        for (int n = 0; n < NG; ++n)
+          s2[i][n] = mul2(mul2(make_float2(s[i / 2][n][2 * (i & 1)], s[i / 2][n][2 * (i & 1) + 1]), qs[n]),
+                          make_float2(ks, ks));
+      }
+      const int valid = u.len - (id - u.base) * kTile;
+      if (valid < kTile) {  // the sequence's last tile: nothing past its end counts, whatever lies there
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float& x = s[mb][n][2 * r + c];
-              x = in ? x * qs[n][c] * ks : -INFINITY;
-            }
-        }
+        for (int i = 0; i < 4; ++i)
+          if (8 * i + g >= valid) {
+            vsc[i] = 0.f;
+            lw[i] = -100.f;
+#pragma unroll
+            for (int n = 0; n < NG; ++n) s2[i][n] = make_float2(-INFINITY, -INFINITY);
+          }
       }
 
       // ---- move R where a weight would pass 2^8 ----
       bool over = false;
-      float top[NG][2];
+      float2 top[NG];
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < NG; ++n) {
+        float2 x[4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          top[n][c] = fmaxf(fmaxf(s[0][n][c] + lw[0][0], s[0][n][2 + c] + lw[0][1]),
-                            fmaxf(s[1][n][c] + lw[1][0], s[1][n][2 + c] + lw[1][1]));
-          over |= top[n][c] > R[n][c] + 8.f;
-        }
+        for (int i = 0; i < 4; ++i) x[i] = add2(s2[i][n], make_float2(lw[i], lw[i]));
+        top[n].x = fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x));
+        top[n].y = fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y));
+        over |= top[n].x > R[n][0] + 8.f || top[n].y > R[n][1] + 8.f;
+      }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int n = 0; n < NG; ++n)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float m = top[n][c];
+            float m = c ? top[n].y : top[n].x;
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
             if (m > R[n][c] + 8.f) {
               const float to = ceilf(m), f = ex2_ftz(R[n][c] - to);
               R[n][c] = to;
-              l[n][c] *= f;
+              (c ? l2[n].y : l2[n].x) *= f;
 #pragma unroll
               for (int i = 0; i < KS; ++i) {
                 o[n][i][c] *= f;
@@ -422,33 +445,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       }
 
       // ---- weights, as the second operand: tokens 2 t4, +1 and + 8 of column g ----
-      uint32_t pf[2][NG][2];
+      uint32_t pf[4][NG];
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float p0 = ex2_ftz(s[mb][n][2 * r] - R[n][0]), p1 = ex2_ftz(s[mb][n][2 * r + 1] - R[n][1]);
-            l[n][0] += p0;
-            l[n][1] += p1;
-            const __half2 w = __floats2half2_rn(p0 * vsc[mb][r], p1 * vsc[mb][r]);
-            pf[mb][n][r] = transpose8x8(reinterpret_cast<const uint32_t&>(w));
-          }
+        for (int n = 0; n < NG; ++n) {
+          float2 p = add2(s2[i][n], make_float2(-R[n][0], -R[n][1]));
+          p.x = ex2_ftz(p.x);
+          p.y = ex2_ftz(p.y);
+          l2[n] = add2(l2[n], p);
+          const float2 wv = mul2(p, make_float2(vsc[i], vsc[i]));
+          const __half2 w = __floats2half2_rn(wv.x, wv.y);
+          pf[i][n] = transpose8x8(reinterpret_cast<const uint32_t&>(w));
+        }
 
-      // ---- O^T += V^T P^T: this lane's dims are 16 g' .. of four tokens ----
+      // ---- O^T += V^T P^T: this lane's dims are D / 8 g .. of four tokens ----
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb) {
         uint32_t v[4][D / 32];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = 16 * mb + 2 * t4 + (r & 1) + 8 * (r >> 1);
-          const uint32_t base = st + C::kRowsBytes;
-          if constexpr (D == 128) {
-            *reinterpret_cast<uint4*>(v[r]) = lds128(base + chunk_offset<D>(row, g));
-          } else {
-            *reinterpret_cast<uint2*>(v[r]) = lds64(base + chunk_offset<D>(row, g >> 1) + 8 * (g & 1));
-          }
+          const uint8_t* at = st + v_at[r & 1] + (16 * mb + 8 * (r >> 1)) * D;
+          if constexpr (D == 128) *reinterpret_cast<uint4*>(v[r]) = *reinterpret_cast<const uint4*>(at);
+          else *reinterpret_cast<uint2*>(v[r]) = *reinterpret_cast<const uint2*>(at);
         }
 #pragma unroll
         for (int w = 0; w < D / 32; ++w)
@@ -459,9 +478,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
             codes_to_f16<FMT>(__byte_perm(v[0][w], v[1][w], sel), a0, a1);
             codes_to_f16<FMT>(__byte_perm(v[2][w], v[3][w], sel), a2, a3);
 #pragma unroll
-            for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * w + hf], a0, a1, a2, a3, pf[mb][n][0], pf[mb][n][1]);
+            for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * w + hf], a0, a1, a2, a3, pf[2 * mb][n], pf[2 * mb + 1][n]);
           }
       }
+    }
+    float l[NG][2];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      l[n][0] = l2[n].x;
+      l[n][1] = l2[n].y;
     }
 
     // ---- join the warps: R and l first, then the scaled sums ----
@@ -475,8 +500,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       }
     __syncthreads();
     float4* merge = reinterpret_cast<float4*>(smem + C::kRingBytes);
-    const bool whole = u.base >= w0 && u.base + u.tiles <= w1;
-    const int slot = 2 * (int)blockIdx.x + (u.base > w0 ? 1 : 0);
+    const bool whole = u.base >= 0 && u.base + u.tiles <= share;
+    const int slot = 2 * (int)blockIdx.x + (u.base > 0 ? 1 : 0);
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       float L[2];
@@ -544,7 +569,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     if (whole) continue;
 
     // ---- a unit of several CTAs: the last one joins the partial results ----
-    const int c_first = cta_of(u.base), c_last = cta_of(u.base + u.tiles - 1), parts = c_last - c_first + 1;
+    const long long first_tile = w0 + u.base;
+    const int c_first = cta_of(first_tile), c_last = cta_of(first_tile + u.tiles - 1), parts = c_last - c_first + 1;
     if (warp == 0) {
       __threadfence();
       __syncwarp();
@@ -571,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
         top[k] = -INFINITY;
         L[k] = 0.f;
       }
-      auto slot_of = [&](int c) { return 2 * c + (u.base > cta_start(c) ? 1 : 0); };
+      auto slot_of = [&](int c) { return 2 * c + (first_tile > cta_start(c) ? 1 : 0); };
       for (int p0 = 0; p0 < parts; p0 += C::kJoinChunk) {
         const int np = min(C::kJoinChunk, parts - p0);
         __syncthreads();
@@ -685,7 +711,7 @@ extern "C" int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool,
                                    float scale, void* workspace, size_t workspace_bytes, void* stream) {
   LARA_NVTX("lara_gqa_decode_kvq");
   KvqDecodeArgs a{};
-  if (const int rc = check_pool(pool, block_table, pages_per_seq, &a.index)) return rc;
+  if (const int rc = check_pool(pool, block_table, pages_per_seq, batch, &a.index)) return rc;
   if (batch < 0 || batch > 65535 || n_q_heads < 1 || n_q_heads % pool->n_kv_heads)
     return set_last_error(LARA_ERR_BAD_CFG, "batch must be at most 65535, n_q_heads a multiple of n_kv_heads");
   if (n_q_heads / pool->n_kv_heads > 16)

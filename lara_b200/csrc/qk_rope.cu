@@ -6,9 +6,9 @@
 //
 // Bound by HBM: every head is read and written once (4 D bytes), the table row
 // of a token once from HBM (4 rot bytes) and from L2 after that.  D / 8 lanes
-// hold a head in registers between the load and the store; a lane group takes
-// kHeads heads of one token, so it loads its cosines, sines and weights once
-// and has kHeads loads in flight.
+// hold a head in registers between the load and the store.  A lane group takes
+// kHeads heads of one token, all of q or all of k: it folds the weights into
+// the token's cosines and sines once, and has kHeads loads in flight.
 #include "kvq.cuh"
 
 namespace lara {
@@ -17,41 +17,45 @@ using namespace kvq;
 
 namespace {
 
-constexpr int kHeads = 4;
 constexpr int kThreads = 128;
 
 struct NormRopeArgs {
   Heads<const uint16_t> q, k;
   Heads<uint16_t> qo, ko;
-  int n, hq, heads, groups_per_token;
-  long long groups;
+  int hq, hkv, q_chunks;
+  uint32_t groups;   // tokens * chunks
+  FastDiv chunks, n;
   const int32_t* positions;
   const float* cos_sin;
-  int max_pos, rot, interleaved;
+  int max_pos, rot;
   const uint16_t* qw;
   const uint16_t* kw;
   float eps;
   int* status;
 };
 
-template <int D, bool kVec>
+// Lane group i takes chunk i % chunks (kHeads heads, of q first) of token
+// i / chunks, so that neighbours in the grid are neighbours in memory.
+template <int D, bool kInter, bool kNorm, bool kVec, int kHeads>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
   constexpr int kLanes = D / 8;
-  const long long gid = ((long long)blockIdx.x * kThreads + threadIdx.x) / kLanes;
+  allow_dependent_launch();
+  grid_dependency_wait();
+  const uint32_t group = blockIdx.x * (uint32_t)(kThreads / kLanes) + threadIdx.x / kLanes;
   const int l = threadIdx.x % kLanes;
-  const bool active = gid < a.groups;
-  const long long g = active ? gid : a.groups - 1;
-  const long long tok = g / a.groups_per_token;
-  const int h0 = (int)(g % a.groups_per_token) * kHeads;
-  const int b = (int)(tok / a.n), t = (int)(tok % a.n);
-  const LaneDims ld(l, a.cos_sin ? a.rot : 0, a.interleaved);
+  uint32_t t, chunk;
+  const uint32_t tok = a.chunks.div(min(group, a.groups - 1), chunk);
+  const uint32_t b = a.n.div(tok, t);
+  const bool is_k = (int)chunk >= a.q_chunks;
+  const int h0 = ((int)chunk - (is_k ? a.q_chunks : 0)) * kHeads;
+  const int heads = group < a.groups ? (is_k ? a.hkv : a.hq) - h0 : 0;  // to store, at most kHeads of them
+  const HeadLane ld(l, a.rot, kInter);
 
-  float x[kHeads][8];
+  const long long sh = is_k ? a.k.sh : a.q.sh;
+  const uint16_t* src = is_k ? a.k.row(b, t, h0) : a.q.row(b, t, h0);
+  Pairs x[kHeads];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = min(h0 + i, a.heads - 1);
-    load8<kVec>(h < a.hq ? a.q.row(b, t, h) : a.k.row(b, t, h - a.hq), ld.o0, ld.o1, x[i]);
-  }
+  for (int i = 0; i < kHeads; ++i) x[i] = load_pairs<kInter, kVec>(src + (i < heads ? i : 0) * sh, ld);
   float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (ld.rotated) {
     int pos = a.positions[tok];
@@ -63,28 +67,51 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
     c = *reinterpret_cast<const float4*>(row);
     s = *reinterpret_cast<const float4*>(row + a.rot / 2);
   }
+  const Turn turn = make_turn<kInter>(c, s, kNorm ? (is_k ? a.kw : a.qw) : nullptr, ld);
+  const long long osh = is_k ? a.ko.sh : a.qo.sh;
+  uint16_t* dst = is_k ? a.ko.row(b, t, h0) : a.qo.row(b, t, h0);
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
-    if (a.qw) {
-      float w[8];
-      load8<true>(h < a.hq ? a.qw : a.kw, ld.o0, ld.o1, w);
-      norm_row<D>(x[i], w, a.eps);
-    }
-    if (ld.rotated) rotate_row(x[i], c, s, a.interleaved);
-    if (active && h < a.heads) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack2_rn(x[i][2 * j], x[i][2 * j + 1]);
-      store8<kVec>(h < a.hq ? a.qo.row(b, t, h) : a.ko.row(b, t, h - a.hq), ld.o0, ld.o1, w);
-    }
+    const Pairs y = turn_head<D, kNorm>(x[i], turn, ld.rotated, a.eps);
+    uint32_t w[4];
+    pack_pairs<kInter>(y, w);
+    if (i < heads) store_pairs<kInter, kVec>(dst + i * osh, ld, w);
   }
 }
 
-// 8-byte accesses: the base and every stride that is taken (an extent of 1
+template <int D, bool kInter, bool kNorm, bool kVec, int kHeads>
+cudaError_t launch_heads(NormRopeArgs a, uint32_t tokens, cudaStream_t stream) {
+  a.q_chunks = (a.hq + kHeads - 1) / kHeads;
+  const uint32_t chunks = a.q_chunks + (a.hkv + kHeads - 1) / kHeads;
+  a.groups = tokens * chunks;
+  a.chunks = FastDiv(chunks);
+  const uint32_t per_block = kThreads / (D / 8);
+  const dim3 grid((a.groups + per_block - 1) / per_block);
+  void* args[] = {&a};
+  return launch_with_pdl(reinterpret_cast<const void*>(&qk_norm_rope_kernel<D, kInter, kNorm, kVec, kHeads>), grid,
+                         dim3(kThreads), args, 0, stream);
+}
+
+// Heads per lane group: 8 keeps eight loads in flight and shares a token's
+// turn; with fewer lane groups than the SMs hold, one head each is quicker.
+template <int D, bool kInter, bool kNorm, bool kVec>
+cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, cudaStream_t stream) {
+  const long long lanes = (long long)tokens * (a.hq + a.hkv) * (D / 8);
+  return lanes / 8 >= (long long)device_sm_count() * 512
+             ? launch_heads<D, kInter, kNorm, kVec, 8>(a, tokens, stream)
+             : launch_heads<D, kInter, kNorm, kVec, 1>(a, tokens, stream);
+}
+
+template <int D, bool kInter>
+cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, bool vec, cudaStream_t stream) {
+  if (a.qw) return vec ? launch<D, kInter, true, true>(a, tokens, stream) : launch<D, kInter, true, false>(a, tokens, stream);
+  return vec ? launch<D, kInter, false, true>(a, tokens, stream) : launch<D, kInter, false, false>(a, tokens, stream);
+}
+
+// 16-byte accesses: the base and every stride that is taken (an extent of 1
 // takes none).
 bool vec_ok(const void* p, long long sb, int batch, long long st, int n, long long sh, int heads) {
-  return aligned(p, 8) && (((batch > 1 ? sb : 0) | (n > 1 ? st : 0) | (heads > 1 ? sh : 0)) & 3) == 0;
+  return aligned(p, 16) && (((batch > 1 ? sb : 0) | (n > 1 ? st : 0) | (heads > 1 ? sh : 0)) & 7) == 0;
 }
 
 }  // namespace
@@ -103,9 +130,9 @@ extern "C" int lara_qk_norm_rope(const uint16_t* q, long long q_sb, long long q_
   LARA_NVTX("lara_qk_norm_rope");
   if (head_dim != 64 && head_dim != 128)
     return set_last_error(LARA_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
-  if (batch < 0 || n < 0 || n_q_heads < 1 || n_kv_heads < 1 || (long long)batch * n > 0x7fffffffll ||
-      (long long)n_q_heads + n_kv_heads > 65535)
-    return set_last_error(LARA_ERR_BAD_CFG, "bad geometry: batch, n >= 0 and head counts >= 1");
+  if (batch < 0 || n < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads > 65535 || n_kv_heads > 65535 ||
+      (long long)batch * n * (n_q_heads + n_kv_heads) > 0x7fffffffll)
+    return set_last_error(LARA_ERR_BAD_CFG, "bad geometry: batch, n >= 0, head counts in [1, 65535], below 2^31 heads in all");
   if (!q_weight != !k_weight) return set_last_error(LARA_ERR_BAD_CFG, "q_weight and k_weight go together");
   if (!q_weight && !cos_sin) return set_last_error(LARA_ERR_BAD_CFG, "neither norm weights nor a rotation table");
   if (cos_sin && (rot_dim < 8 || rot_dim > head_dim || rot_dim % 8 || max_pos < 1))
@@ -115,8 +142,8 @@ extern "C" int lara_qk_norm_rope(const uint16_t* q, long long q_sb, long long q_
   if (!q || !k || !q_out || !k_out || (cos_sin && !positions))
     return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
   if (!aligned(q, 2) || !aligned(k, 2) || !aligned(q_out, 2) || !aligned(k_out, 2) || !aligned(positions, 4) ||
-      !aligned(cos_sin, 16) || !aligned(q_weight, 8) || !aligned(k_weight, 8) || !aligned(workspace, 4))
-    return set_last_error(LARA_ERR_STREAM_DEST, "cos_sin must be 16-byte aligned, the weights 8-byte");
+      !aligned(cos_sin, 16) || !aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(workspace, 4))
+    return set_last_error(LARA_ERR_STREAM_DEST, "cos_sin and the weights must be 16-byte aligned");
   const bool vec = vec_ok(q, q_sb, batch, q_st, n, q_sh, n_q_heads) && vec_ok(k, k_sb, batch, k_st, n, k_sh, n_kv_heads) &&
                    vec_ok(q_out, qo_sb, batch, qo_st, n, qo_sh, n_q_heads) &&
                    vec_ok(k_out, ko_sb, batch, ko_st, n, ko_sh, n_kv_heads);
@@ -125,32 +152,23 @@ extern "C" int lara_qk_norm_rope(const uint16_t* q, long long q_sb, long long q_
   a.k = {k, k_sb, k_st, k_sh};
   a.qo = {q_out, qo_sb, qo_st, qo_sh};
   a.ko = {k_out, ko_sb, ko_st, ko_sh};
-  a.n = n;
+  const uint32_t tokens = (uint32_t)batch * (uint32_t)n;
   a.hq = n_q_heads;
-  a.heads = n_q_heads + n_kv_heads;
-  a.groups_per_token = (a.heads + kHeads - 1) / kHeads;
-  a.groups = (long long)batch * n * a.groups_per_token;
+  a.hkv = n_kv_heads;
+  a.n = FastDiv((uint32_t)n);
   a.positions = positions;
   a.cos_sin = cos_sin;
   a.max_pos = max_pos;
   a.rot = cos_sin ? rot_dim : 0;
-  a.interleaved = interleaved;
   a.qw = q_weight;
   a.kw = k_weight;
   a.eps = eps;
   a.status = static_cast<int*>(workspace);
-  const long long per_block = kThreads / (head_dim / 8);
-  const long long blocks = (a.groups + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffll) return set_last_error(LARA_ERR_BAD_CFG, "too many heads for one launch");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) {
-    if (vec) qk_norm_rope_kernel<128, true><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-    else qk_norm_rope_kernel<128, false><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-  } else {
-    if (vec) qk_norm_rope_kernel<64, true><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-    else qk_norm_rope_kernel<64, false><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-  }
-  const cudaError_t e = cudaGetLastError();
+  // without a rotation nothing is paired: side by side is the wider access
+  const bool inter = interleaved || !cos_sin;
+  const cudaError_t e = head_dim == 128 ? (inter ? launch<128, true>(a, tokens, vec, st) : launch<128, false>(a, tokens, vec, st))
+                                        : (inter ? launch<64, true>(a, tokens, vec, st) : launch<64, false>(a, tokens, vec, st));
   if (e != cudaSuccess)
     return set_last_error(LARA_ERR_CUDA, std::string("qk_norm_rope launch: ") + cudaGetErrorString(e));
   return LARA_OK;

@@ -26,11 +26,10 @@ from __future__ import annotations
 import ctypes
 import math
 
-import numpy as np
 import torch
 
-from ._native import LARA_KVQ_FP8_E4M3, LARA_KVQ_INT8, LaraKvqPool, check, lib
-from .ops import _check_words, _on_device, _ptr, _strided, _stream, new_workspace
+from ._native import LARA_KVQ_FP8_E4M3, LARA_KVQ_INT8, LaraKvqPool, lib
+from .ops import _BF16, _I32, _check_words, _launch, _ptr, _strided, new_workspace
 from .paged import PagedKVCache
 
 _FORMATS = {torch.int8: LARA_KVQ_INT8, torch.float8_e4m3fn: LARA_KVQ_FP8_E4M3}
@@ -64,7 +63,7 @@ class QuantPool:
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
-        self.device = k_codes.device
+        self.device, self.index = k_codes.device, k_codes.get_device()
         self._c = LaraKvqPool(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                               _FORMATS[k_codes.dtype], self.num_pages, self.n_kv_heads, self.page_size, self.head_dim)
         self._ref = ctypes.byref(self._c)
@@ -80,17 +79,19 @@ class QuantPool:
         return cls(*codes, *scales)
 
 
-def _check_i32(name: str, t: torch.Tensor, n: int, device) -> None:
-    if t.dtype != torch.int32 or t.device != device or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of length {n} on {device}")
+def _i32_ptr(name: str, t: torch.Tensor, n: int, index: int) -> int:
+    if t.dtype is not _I32 or t.get_device() != index or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of length {n} on the pool's device")
+    return t.data_ptr()
 
 
-def _check_table(table: torch.Tensor, batch: int, device) -> int:
-    if table.dtype != torch.int32 or table.device != device or table.dim() != 2 or not table.is_contiguous():
-        raise ValueError(f"block_table must be a contiguous int32 [batch, pages_per_seq] tensor on {device}")
-    if table.shape[0] != batch:
-        raise ValueError(f"block_table has {table.shape[0]} rows for a batch of {batch}")
-    return table.shape[1]
+def _table(table: torch.Tensor, batch: int, index: int) -> tuple:
+    if table.dtype is not _I32 or table.get_device() != index or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("block_table must be a contiguous int32 [batch, pages_per_seq] tensor on the pool's device")
+    rows, pages = table.shape
+    if rows != batch:
+        raise ValueError(f"block_table has {rows} rows for a batch of {batch}")
+    return table.data_ptr(), pages
 
 
 def kvq_append(pool: QuantPool, block_table, starts, k_new, v_new, *, counts=None, new_lens=None,
@@ -102,21 +103,15 @@ def kvq_append(pool: QuantPool, block_table, starts, k_new, v_new, *, counts=Non
     tensor) receives ``starts + counts``.  ``workspace`` (``ops.new_workspace(256, device)``) collects
     the status bits of dropped rows (``ops.workspace_status``).
     """
-    dev = pool.device
+    index = pool.index
     B, _, n, _ = k_new.shape
     shape = (B, pool.n_kv_heads, n, pool.head_dim)
-    ks = _strided("k_new", k_new, shape, dev)
-    vs = _strided("v_new", v_new, shape, dev)
-    pps = _check_table(block_table, B, dev)
-    _check_i32("starts", starts, B, dev)
-    if counts is not None:
-        _check_i32("counts", counts, B, dev)
-    if new_lens is not None:
-        _check_i32("new_lens", new_lens, B, dev)
-    with _on_device(dev):
-        check(lib.lara_kvq_append(pool._ref, block_table.data_ptr(), pps, starts.data_ptr(), _ptr(counts),
-                                  _ptr(new_lens), k_new.data_ptr(), ks[0], ks[1], ks[2], v_new.data_ptr(), vs[0],
-                                  vs[1], vs[2], B, n, _ptr(workspace), _stream(dev)), "lara_kvq_append")
+    ks = _strided("k_new", k_new, shape, index)
+    vs = _strided("v_new", v_new, shape, index)
+    _launch(lib.lara_kvq_append, index, pool._ref, *_table(block_table, B, index), _i32_ptr("starts", starts, B, index),
+            None if counts is None else _i32_ptr("counts", counts, B, index),
+            None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
+            k_new.data_ptr(), ks[0], ks[1], ks[2], v_new.data_ptr(), vs[0], vs[1], vs[2], B, n, _ptr(workspace))
 
 
 def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=None, out=None, workspace=None):
@@ -125,23 +120,19 @@ def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=No
     ``starts=None`` reads from token 0.  Tokens at or past ``seq_lens[b]`` read as zeros.  ``out`` may be
     two strided views, e.g. ``cache[:, :, :n]`` of a bf16 cache for :func:`lara_b200.ops.gqa_prefill`.
     """
-    dev = pool.device
+    index = pool.index
     B, n = seq_lens.numel(), int(n_tokens)
     shape = (B, pool.n_kv_heads, n, pool.head_dim)
     if out is None:
-        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        k, v = (torch.empty(shape, dtype=_BF16, device=pool.device) for _ in range(2))
     else:
         k, v = out
-    ks = _strided("k out", k, shape, dev, written=True)
-    vs = _strided("v out", v, shape, dev, written=True)
-    pps = _check_table(block_table, B, dev)
-    _check_i32("seq_lens", seq_lens, B, dev)
-    if starts is not None:
-        _check_i32("starts", starts, B, dev)
-    with _on_device(dev):
-        check(lib.lara_kvq_read(pool._ref, block_table.data_ptr(), pps, seq_lens.data_ptr(), _ptr(starts),
-                                k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], B, n,
-                                _ptr(workspace), _stream(dev)), "lara_kvq_read")
+    ks = _strided("k out", k, shape, index, written=True)
+    vs = _strided("v out", v, shape, index, written=True)
+    _launch(lib.lara_kvq_read, index, pool._ref, *_table(block_table, B, index),
+            _i32_ptr("seq_lens", seq_lens, B, index),
+            None if starts is None else _i32_ptr("starts", starts, B, index),
+            k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], B, n, _ptr(workspace))
     return k, v
 
 
@@ -151,7 +142,7 @@ def decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
     One stream at a time uses it.
     """
     dev = torch.device(device)
-    with _on_device(dev):
+    with torch.cuda.device(dev):
         return new_workspace(int(lib.lara_kvq_decode_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim)), dev)
 
 
@@ -161,23 +152,23 @@ def gqa_decode_kvq(q, pool: QuantPool, block_table, seq_lens, *, scale=None, wor
     ``Hq`` is any multiple of the pool's kv heads up to 16 per kv head.  A sequence of length 0 gives
     zeros.  ``workspace`` comes from :func:`decode_workspace` (``None`` allocates one for the call).
     """
-    dev = pool.device
+    index = pool.index
     B, hq, d = q.shape
-    _check_words("q", q, (B, hq, pool.head_dim))
-    if q.device != dev:
-        raise ValueError(f"q must be on {dev}")
-    pps = _check_table(block_table, B, dev)
-    _check_i32("seq_lens", seq_lens, B, dev)
+    shape = (B, hq, pool.head_dim)
+    _strided("q", q, shape, index)
+    if not q.is_contiguous():
+        raise ValueError("q must be contiguous")
     if out is None:
         out = torch.empty_like(q)
     else:
-        _check_words("out", out, (B, hq, d))
+        _strided("out", out, shape, index)
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
     if workspace is None:
-        workspace = decode_workspace(max(B, 1), hq, pool.n_kv_heads, d, dev)
-    with _on_device(dev):
-        check(lib.lara_gqa_decode_kvq(q.data_ptr(), pool._ref, block_table.data_ptr(), pps, seq_lens.data_ptr(),
-                                      out.data_ptr(), B, hq, 1.0 / math.sqrt(d) if scale is None else float(scale),
-                                      workspace.data_ptr(), workspace.numel(), _stream(dev)), "lara_gqa_decode_kvq")
+        workspace = decode_workspace(max(B, 1), hq, pool.n_kv_heads, d, pool.device)
+    _launch(lib.lara_gqa_decode_kvq, index, q.data_ptr(), pool._ref, *_table(block_table, B, index),
+            _i32_ptr("seq_lens", seq_lens, B, index), out.data_ptr(), B, hq,
+            1.0 / math.sqrt(d) if scale is None else float(scale), workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -206,8 +197,8 @@ class QuantKVCache(PagedKVCache):
         slots = self._slots(slots)
         n = int(k_new.shape[2])
         shape = (len(slots), self.n_kv_heads, n, self.head_dim)
-        _strided("k_new", k_new, shape, self.pool.device)
-        _strided("v_new", v_new, shape, self.pool.device)
+        _strided("k_new", k_new, shape, self.pool.index)
+        _strided("v_new", v_new, shape, self.pool.index)
         self.reserve(slots, n)
         idx, table, lens = self._rows(slots)
         new_lens = torch.empty_like(lens)

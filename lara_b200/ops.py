@@ -7,7 +7,6 @@ or 16-bit integer views of the same words.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -38,27 +37,34 @@ def _check_words(name: str, t: torch.Tensor, shape: tuple | None = None) -> None
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-def _strided(name: str, t: torch.Tensor, shape: tuple, device, written: bool = False) -> tuple:
-    """Strides of a bf16 tensor of contiguous rows (last dim), after checking it."""
-    if t.dtype not in _WORD_DTYPES:
+_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
+
+
+def _strided(name: str, t: torch.Tensor, shape: tuple, index: int, written: bool = False) -> tuple:
+    """Strides of a bf16 tensor of contiguous rows (last dim) on CUDA device ``index``, after checking it."""
+    if t.dtype is not _BF16 and t.dtype not in _WORD_DTYPES:
         raise TypeError(f"{name} must hold bf16 words (bfloat16/int16/uint16), got {t.dtype}")
-    if t.device != device or not t.is_cuda:
-        raise ValueError(f"{name} must be on the CUDA device {device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.get_device() != index or index < 0:
+        raise ValueError(f"{name} must be on the CUDA device of the call, got {t.device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     st = t.stride()
     if st[-1] != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    if written and any(s == 0 and n > 1 for s, n in zip(st, shape)):
+    if written and 0 in st and any(s == 0 and n > 1 for s, n in zip(st, shape)):
         raise ValueError(f"{name} is written and must not repeat elements (a stride of 0)")
     return st
 
 
-def _on_device(device: torch.device):
-    """The device as the current one for a launch; free when it already is."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(fn, index: int, *args) -> None:
+    """Call a C entry point whose last argument is the stream, on CUDA device ``index`` and its current stream."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, fn.__name__)
 
 
 @dataclass
@@ -328,20 +334,11 @@ def rope_table(max_pos: int, rot_dim: int, *, base: float = 10000.0, inv_freq=No
     return torch.cat([ang.cos(), ang.sin()], -1).float()
 
 
-def _rope_args(cos_sin, head_dim: int, device) -> tuple:
-    if cos_sin is None:
-        return None, 0, 0
-    if cos_sin.dtype != torch.float32 or cos_sin.device != device or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
-        raise ValueError(f"cos_sin must be a contiguous float32 [max_pos, rot_dim] tensor on {device}")
-    return cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1]
-
-
-def _norm_weights(q_weight, k_weight, head_dim: int, device) -> None:
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _check_words(name, w, (head_dim,))
-            if w.device != device:
-                raise ValueError(f"{name} must be on {device}")
+def _rope_table_args(cos_sin: torch.Tensor, index: int) -> tuple:
+    if (cos_sin.dtype is not _F32 or cos_sin.get_device() != index or cos_sin.dim() != 2
+            or not cos_sin.is_contiguous()):
+        raise ValueError("cos_sin must be a contiguous float32 [max_pos, rot_dim] tensor on the same device")
+    return cos_sin.data_ptr(), *cos_sin.shape
 
 
 def qk_norm_rope(q, k, *, positions=None, cos_sin=None, q_weight=None, k_weight=None, eps: float = 1e-5,
@@ -357,35 +354,36 @@ def qk_norm_rope(q, k, *, positions=None, cos_sin=None, q_weight=None, k_weight=
     (q, k) in new contiguous tensors, or in ``out``, which may be the inputs.  ``workspace`` collects the
     status bit of a position outside the table (its nearest row is taken).
     """
-    if q.dim() not in (3, 4) or k.dim() != q.dim():
+    shape = q.shape
+    if len(shape) not in (3, 4) or k.dim() != len(shape):
         raise ValueError("q and k must be [T, H, D] or [B, n, H, D]")
-    dev = q.device
-    lead, (hq, d), hkv = tuple(q.shape[:-2]), q.shape[-2:], k.shape[-2]
-    qs = _strided("q", q, (*lead, hq, d), dev)
-    ks = _strided("k", k, (*lead, hkv, d), dev)
-    if out is None:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    else:
-        qo, ko = out
-    qos = _strided("q out", qo, (*lead, hq, d), dev, written=True)
-    kos = _strided("k out", ko, (*lead, hkv, d), dev, written=True)
-    _norm_weights(q_weight, k_weight, d, dev)
-    table, max_pos, rot = _rope_args(cos_sin, d, dev)
-    if table is not None:
+    index = q.get_device()
+    *lead, hq, d = shape
+    k_shape = (*lead, k.shape[-2], d)
+    qs = _strided("q", q, shape, index)
+    ks = _strided("k", k, k_shape, index)
+    qo, ko = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)) if out is None else out
+    qos = _strided("q out", qo, shape, index, written=True)
+    kos = _strided("k out", ko, k_shape, index, written=True)
+    qw = kw = table = pos = None
+    max_pos = rot = 0
+    if q_weight is not None:
+        _strided("q_weight", q_weight, (d,), index)
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        _strided("k_weight", k_weight, (d,), index)
+        kw = k_weight.data_ptr()
+    if cos_sin is not None:
+        table, max_pos, rot = _rope_table_args(cos_sin, index)
         if positions is None:
             raise ValueError("a rotation needs positions")
-        if (positions.dtype != torch.int32 or positions.device != dev or tuple(positions.shape) != lead
+        if (positions.dtype is not _I32 or positions.get_device() != index or positions.shape != shape[:-2]
                 or not positions.is_contiguous()):
-            raise ValueError(f"positions must be a contiguous int32 tensor of shape {lead} on {dev}")
-    if len(lead) == 1:
-        B, n, qs, ks, qos, kos = 1, lead[0], (0, *qs), (0, *ks), (0, *qos), (0, *kos)
-    else:
-        B, n = lead
-    with _on_device(dev):
-        check(lib.lara_qk_norm_rope(q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
-                                    qo.data_ptr(), qos[0], qos[1], qos[2], ko.data_ptr(), kos[0], kos[1], kos[2],
-                                    B, n, hq, hkv, d, None if table is None else positions.data_ptr(), table, max_pos,
-                                    rot, int(bool(interleaved)), _ptr(q_weight), _ptr(k_weight), float(eps),
-                                    _ptr(workspace), _stream(dev)), "lara_qk_norm_rope")
+            raise ValueError(f"positions must be a contiguous int32 tensor of shape {tuple(lead)} on the same device")
+        pos = positions.data_ptr()
+    B, n = lead if len(lead) == 2 else (1, lead[0])
+    _launch(lib.lara_qk_norm_rope, index, q.data_ptr(), qs[0] if B > 1 else 0, qs[-3], qs[-2], k.data_ptr(),
+            ks[0] if B > 1 else 0, ks[-3], ks[-2], qo.data_ptr(), qos[0] if B > 1 else 0, qos[-3], qos[-2],
+            ko.data_ptr(), kos[0] if B > 1 else 0, kos[-3], kos[-2], B, n, hq, k_shape[-2], d, pos, table, max_pos,
+            rot, int(bool(interleaved)), qw, kw, eps, _ptr(workspace))
     return qo, ko

@@ -745,3 +745,51 @@ def test_quant_cache_manager(tmp_path, fmt):
     for x in (a, b, s):
         c.free_sequence(x)
     assert c.free_pages == c.num_pages
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_rotation_alone_keeps_infinities_apart(interleaved):
+    """Without a norm, dims past rot_dim pass through, infinities and NaN beside them or not."""
+    _need_gpu()
+    from lara_b200 import ops
+
+    g = torch.Generator().manual_seed(13)
+    x = _rand_bf16(g, (9, 3, 128))
+    x[1, 0, 70], x[2, 1, 127], x[3, 2, 96] = math.inf, -math.inf, math.nan
+    pos = torch.arange(9, dtype=torch.int32, device=DEV)
+    q, k = ops.qk_norm_rope(x.to(DEV), x[:, :1].to(DEV), positions=pos, cos_sin=ops.rope_table(9, 64, device=DEV),
+                            interleaved=interleaved)
+    for y in (q, k):
+        h = y.shape[1]
+        got, want = y[..., 64:].cpu(), x[:, :h, 64:]
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got.nan_to_num(7.0, math.inf, -math.inf), want.nan_to_num(7.0, math.inf, -math.inf))
+        assert torch.isfinite(y[..., :64]).all()
+
+
+@pytest.mark.gpu
+def test_small_batches_and_empty_calls():
+    _need_gpu()
+    from lara_b200 import kvquant, ops
+
+    case = Case([5, 3], 2, 64, 16, "fp8_e4m3", seed=1)
+    q = torch.empty((0, 4, 64), dtype=torch.bfloat16, device=DEV)
+    none = torch.empty((0,), dtype=torch.int32, device=DEV)
+    assert kvquant.gqa_decode_kvq(q, case.pool, case.dtable[:0], none).shape == (0, 4, 64)
+    k, v = kvquant.kvq_read(case.pool, case.dtable[:0], none, 7)
+    assert k.shape == v.shape == (0, 2, 7, 64)
+    kvquant.kvq_append(case.pool, case.dtable[:0], none, k, v)
+    a, b = ops.qk_norm_rope(q, q[:, :1], q_weight=torch.ones(64, dtype=torch.bfloat16, device=DEV),
+                            k_weight=torch.ones(64, dtype=torch.bfloat16, device=DEV))
+    assert a.shape == (0, 4, 64) and b.shape == (0, 1, 64)
+    with pytest.raises(ValueError, match="seq_lens"):
+        kvquant.kvq_read(case.pool, case.dtable, case.dlens.long(), 7)
+    with pytest.raises(ValueError, match="block_table"):
+        kvquant.kvq_read(case.pool, case.dtable[:1], case.dlens, 7)
+    with pytest.raises(ValueError, match="stride of 0"):
+        z = torch.zeros((1, 1, 1, 64), dtype=torch.bfloat16, device=DEV).expand(2, 2, 7, 64)
+        kvquant.kvq_read(case.pool, case.dtable, case.dlens, 7, out=(z, z))
+    with pytest.raises(ValueError, match="shape"):
+        kvquant.gqa_decode_kvq(torch.zeros((2, 4, 128), dtype=torch.bfloat16, device=DEV), case.pool, case.dtable,
+                               case.dlens)
