@@ -4,40 +4,42 @@
 //   k_t = ks_t ck_t, v_t = vs_t cv_t       (codes c, one fp32 scale per row)
 //
 // Bound by HBM: every cached row is read once, 2 (D + 4) bytes per token and kv
-// head, for 4 D G multiply-adds.  What a byte costs on the SM is kept far
-// below the time it takes to arrive:
+// head, for 4 D G multiply-adds.  What a byte costs on the SM is kept below the
+// time it takes to arrive:
 //
-//  * Products run on the tensor cores as mma.m16n8k16 (fp16 in, fp32 out) with
-//    the cache as the 16-row operand and the group's query heads as the 8
-//    columns: S^T[token][head] = K q^T, then O^T[dim][head] = V^T P^T.  The
-//    columns of S^T and O^T lie in the same lanes, so rescaling needs no
-//    exchange, and movmatrix turns a tile of P into the second operand.  At
-//    one byte per element the cache itself is the bound, and eight heads share
-//    each product, so the 5th-generation path (128-row tiles, TMEM, operands
-//    described per tile) has nothing to win here.
-//  * Codes become fp16 in registers, exactly: int8 by setting the exponent
-//    byte (0x6400 | code + 128 is 1152 + code) and one subtraction, e4m3 by
-//    moving its bits into place (the value times 2^-8; any byte is finite, so
-//    garbage past a sequence's end cannot reach a sum).  The order in which a
-//    lane's bytes meet q, and the output dims a lane ends up with, are chosen
-//    so that no byte has to be moved between lanes.
+//  * Products run on the tensor cores as warp-wide mma with the cache as the
+//    16-row operand and the group's query heads as the 8 columns:
+//    S^T[token][head] = K q^T, then O^T[dim][head] = V^T P^T.  The columns of
+//    both lie in the same lanes, so rescaling needs no exchange, and movmatrix
+//    turns a tile of P into the second operand.  At one byte per element the
+//    cache itself is the bound, and eight heads share each product, so the
+//    5th-generation path (128-row tiles, TMEM) has nothing to win here.
+//  * int8 K codes are multiplied as they are: q 2^k, rounded to 23 bits, is
+//    written as three signed base-256 digits once per unit, and the products
+//    are exact in int32 (at most 2^-22 of the head's largest |q| is lost per
+//    dim, and nothing of a bf16 q within 2^-14 of it).  e4m3 products of this
+//    kind would be taken apart into fp16 ones, once per digit, so e4m3 codes
+//    are converted to fp16 (exact), and q 2^k too (exact within 2^-29).
+//  * V codes become fp16 in registers, exactly (int8 by setting the exponent
+//    byte, 0x6400 | code + 128 is 1152 + code, and one subtraction), after
+//    ldmatrix has transposed the bytes.
 //  * ks multiplies the fp32 scores, vs the fp32 weights.  Weights are rounded
-//    to fp16 (2^-11 each, below bf16's 2^-8 of the output); R follows the
-//    largest s_t + log2 vs_t, so the weights that carry the sum stay in fp16's
-//    normal range whatever the scales are.  R is moved only when a weight
-//    would pass 2^8, and by whole powers of two, so most tiles rescale nothing.
-//  * q is brought to fp16 by a power of two per head (exact within 2^-29 of
-//    the head's largest value).
+//    to fp16 (2^-12 each on average, below bf16's 2^-8 of the output); R
+//    follows the largest s_t + log2 vs_t, so that weights keep 32 binary orders
+//    below the largest one whatever the scales are.  R moves only when a weight
+//    would pass 2^15, and by whole powers of two, so most tiles rescale nothing.
 //
-// Work is split evenly, by the kernel itself: all (sequence, kv head) units
-// are laid end to end in tiles of 32 tokens, CTA c takes an equal share, and
-// its warps take tiles in turn, each through its own ring of cp.async stages
-// (no barrier per tile, no plan from the host, lengths stay on the device).
-// Warps join at the end of a unit; a unit that several CTAs share is joined by
-// the last of them to finish, in CTA order, so results do not depend on timing.
+// Work is split by the kernel itself: all (sequence, kv head) units are laid
+// end to end in tiles of 32 tokens, CTA c takes an equal share, and its warps
+// take tiles in turn, each through its own ring of cp.async stages (no barrier
+// per tile, no plan from the host, lengths stay on the device).  Warps join at
+// the end of a unit; a unit that several CTAs share is joined by the last of
+// them to finish, in CTA order, so results do not depend on timing.  Short
+// units that fit the grid go to one CTA each, without that second join.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "kvq.cuh"
 
@@ -51,18 +53,35 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;          // tokens per warp and stage
 constexpr int kMinTiles = kWarps;  // tiles per CTA below which fewer CTAs run
+#ifndef WHOLE
+#define WHOLE 12
+#endif
+constexpr int kWholeTiles = WHOLE; // units up to this long are not split while each has a CTA
+constexpr int kFewParts = 4;       // parts of a unit that its last CTA joins without publishing its own
+constexpr int kLensCached = 1024;  // lengths kept in shared memory
 constexpr size_t kStatusBytes = 256;
 
+// Weights lie in fp16 between 2^kStart (the largest, when R is set) and 2^kHigh.
+constexpr float kStart = 7.f, kHigh = 15.f;
+
+#ifndef ST128
+#define ST128 2
+#define CTA128 3
+#define ST64 3
+#define CTA64 4
+#endif
 template <int D, int NG>
 struct Cfg {
-  static constexpr int kStages = D == 128 ? 3 : 4;
-  static constexpr int kCtasPerSm = D == 128 ? 2 : 3;
+  static constexpr int kStages = D == 128 ? ST128 : ST64;
+  static constexpr int kCtasPerSm = D == 128 ? (NG == 1 ? CTA128 : 2) : (NG == 1 ? CTA64 : 3);
   static constexpr int kRowsBytes = kTile * D;                     // K (or V) codes of a stage
   static constexpr int kStageBytes = 2 * kRowsBytes + 2 * kTile * 4;
-  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kMergeBytes = (kWarps - 1) * 8 * D * 4;     // one group of 8 heads at a time
-  static constexpr int kSmemBytes = kRingBytes + kMergeBytes;
-  static constexpr int kJoinChunk = kMergeBytes / (NG * 8 * 8);    // partial (R, l) the join stages at a time
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kSmemBytes = kWarps * kWarpBytes + 128;
+  static constexpr int kPitch = D + 4;  // floats per head in the join (lanes of a store hit distinct banks)
+  static constexpr int kJoinChunk = 8 * D * 4 / (NG * 8 * 8);  // partial (R, l) the join stages at a time
+  static_assert(kStageBytes % 128 == 0, "rows start on 128-byte boundaries");
+  static_assert(8 * kPitch * 4 <= kStageBytes, "a stage holds the sums of eight heads");
 };
 
 struct KvqDecodeArgs {
@@ -100,10 +119,27 @@ __device__ __forceinline__ void mma_f16(float c[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 32 products per row on the codes as they are.
+__device__ __forceinline__ void mma_s8(int c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+
+// Two 16 x 16 blocks of bytes, transposed: lanes 0-15 and 16-31 name the rows
+// (tokens) of one block each; the lane gets tokens 4 t4 .. + 3 of dims g (v[0],
+// v[2]) and g + 8 (v[1], v[3]).
+__device__ __forceinline__ void load_transposed(uint32_t v[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
 }
 
 __device__ __forceinline__ float lg2_ftz(float x) {
@@ -112,26 +148,108 @@ __device__ __forceinline__ float lg2_ftz(float x) {
   return y;
 }
 
-// Bytes 0 and 2 (even) and bytes 1 and 3 (odd) of four codes as fp16 pairs.
+// Bytes 0, 1 (lo) and 2, 3 (hi) of four codes as fp16 pairs.
 template <int FMT>
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& even, uint32_t& odd) {
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (FMT == LARA_KVQ_INT8) {
     const uint32_t x = w ^ 0x80808080u;
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-    uint32_t e = __byte_perm(x, 0x64646464u, 0x4240), o = __byte_perm(x, 0x64646464u, 0x4341);
-    const __half2 he = __hsub2(reinterpret_cast<__half2&>(e), bias);
-    const __half2 ho = __hsub2(reinterpret_cast<__half2&>(o), bias);
-    even = reinterpret_cast<const uint32_t&>(he);
-    odd = reinterpret_cast<const uint32_t&>(ho);
+    uint32_t l = __byte_perm(x, 0x64646464u, 0x4140), h = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 hl = __hsub2(reinterpret_cast<__half2&>(l), bias);
+    const __half2 hh = __hsub2(reinterpret_cast<__half2&>(h), bias);
+    lo = reinterpret_cast<const uint32_t&>(hl);
+    hi = reinterpret_cast<const uint32_t&>(hh);
   } else {
-    // s eeee mmm -> s 0 eeee mmm 0000000: fp16 with the exponent 8 too small
-    even = ((w << 7) & 0x3f803f80u) | ((w << 8) & 0x80008000u);
-    odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   }
 }
 
-// Where the 16-byte chunk c of a row lies in a stage, so that the eight lanes
-// of a shared-memory phase (rows 2t of V, or two rows of K) hit distinct banks.
+// q as the second operand, kWords registers per four dims.  m: the head's
+// largest |q| as bf16 magnitude bits; factor() brings a score back.
+template <int FMT>
+struct Query;
+
+// Three signed base-256 digits of q 2^-e, which is below 2^22.
+template <>
+struct Query<LARA_KVQ_INT8> {
+  static constexpr int kWords = 3;
+  static __device__ __forceinline__ int exponent(uint32_t m) { return max((int)(m >> 7) - 127, -100) - 21; }
+  static __device__ __forceinline__ float factor(int e) { return __uint_as_float((uint32_t)(127 + e + 8) << 23); }
+  static __device__ __forceinline__ void split(const float x[4], uint32_t out[3]) {
+    uint32_t d[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int v = __float2int_rn(x[i]);
+      const int v1 = (v + 128) >> 8, v2 = (v1 + 128) >> 8;  // digits in [-128, 127]
+      d[0][i] = v;
+      d[1][i] = v1;
+      d[2][i] = v2;
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      out[p] = __byte_perm(__byte_perm(d[p][0], d[p][1], 0x0040), __byte_perm(d[p][2], d[p][3], 0x0040), 0x5410);
+  }
+  // K q^T of 16 tokens (rows a and b of D / 16 words per lane), in units of 2^8
+  template <int D, int NG>
+  static __device__ __forceinline__ void scores(float (*s)[4], const uint32_t* a, const uint32_t* b,
+                                                const uint32_t (*q)[D / 16][3]) {
+    int acc[NG][3][4];
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int i = 0; i < 12; ++i) acc[n][i / 4][i % 4] = 0;
+#pragma unroll
+    for (int j = 0; j < D / 16; j += 2) {
+      const uint32_t x[4] = {a[j], b[j], a[j + 1], b[j + 1]};
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) mma_s8(acc[n][p], x, q[n][j][p], q[n][j + 1][p]);
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // below 2^29; the lowest digits' sum rounded down to the unit
+        s[n][i] = (float)(acc[n][2][i] * 256 + acc[n][1][i] + (acc[n][0][i] >> 8));
+  }
+};
+
+// q 2^-e, below 2^15, in fp16.
+template <>
+struct Query<LARA_KVQ_FP8_E4M3> {
+  static constexpr int kWords = 2;
+  static __device__ __forceinline__ int exponent(uint32_t m) { return max((int)(m >> 7) - 127, -100) - 14; }
+  static __device__ __forceinline__ float factor(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+  static __device__ __forceinline__ void split(const float x[4], uint32_t out[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      out[i] = reinterpret_cast<const uint32_t&>(h);
+    }
+  }
+  template <int D, int NG>
+  static __device__ __forceinline__ void scores(float (*s)[4], const uint32_t* a, const uint32_t* b,
+                                                const uint32_t (*q)[D / 16][2]) {
+#pragma unroll
+    for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t a0, a1, a2, a3;
+      codes_to_f16<LARA_KVQ_FP8_E4M3>(a[j], a0, a2);
+      codes_to_f16<LARA_KVQ_FP8_E4M3>(b[j], a1, a3);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) mma_f16(s[n], a0, a1, a2, a3, q[n][j][0], q[n][j][1]);
+    }
+  }
+};
+
+// Where the 16-byte chunk c of a row lies in a stage, so that the rows which a
+// shared-memory phase reads (two rows of K, eight of V) hit distinct banks.
 // Rows eight apart are laid out alike.
 template <int D>
 __device__ __forceinline__ uint32_t chunk_offset(int row, int c) {
@@ -139,151 +257,221 @@ __device__ __forceinline__ uint32_t chunk_offset(int row, int c) {
   return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
 }
 
-__device__ __forceinline__ int seq_tiles(const KvqDecodeArgs& a, int b, int* len_out = nullptr) {
-  int len = __ldcg(a.lens + b);
-  const long long cap = a.index.capacity();
-  if (len < 0 || len > cap) {
-    atomicOr(a.status, kDevBadLength);
-    len = len < 0 ? 0 : (int)cap;
-  }
-  if (len_out) *len_out = len;
-  return (len + kTile - 1) / kTile;
+__device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+
+// a / b, by 32-bit arithmetic where both fit.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 31) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
 }
 
 // A unit (b, kvh) in the end-to-end order of tiles; `base` is its first tile,
 // counted from the CTA's own first.
 struct Unit {
   int base, tiles, len, b, kvh;
-  __device__ __forceinline__ void next(const KvqDecodeArgs& a) {
-    base += tiles;
-    if (++kvh == a.pool.n_kv_heads) {
-      kvh = 0;
-      do {
-        ++b;
-        tiles = b < a.batch ? seq_tiles(a, b, &len) : 0x3fffffff;
-      } while (tiles == 0);
-    }
-  }
 };
+
+// Parts of a unit are joined as o = sum_i 2^(R_i - R) o_i / sum_i 2^(R_i - R) l_i
+// with R the largest R_i, i in CTA order, wherever it is done.
+__device__ __forceinline__ void join_start(float& top, float& L, float4& x) {
+  top = -INFINITY;
+  L = 0.f;
+  x = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ void join_top(float& top, const float2& ml) { top = fmaxf(top, ml.x); }
+__device__ __forceinline__ void join_add(float top, float& L, float4& x, const float2& ml, const float4& y) {
+  const float w = ml.x == top ? 1.f : ex2_ftz(ml.x - top);
+  L = __fmaf_rn(ml.y, w, L);
+  x.x = __fmaf_rn(y.x, w, x.x);
+  x.y = __fmaf_rn(y.y, w, x.y);
+  x.z = __fmaf_rn(y.z, w, x.z);
+  x.w = __fmaf_rn(y.w, w, x.w);
+}
+
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
 
 template <int D, int FMT, int NG>
 __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     kvq_decode_kernel(const __grid_constant__ KvqDecodeArgs a) {
   using C = Cfg<D, NG>;
-  constexpr int KS = D / 16;   // k steps of the scores = dim blocks of the output
-  extern __shared__ __align__(128) uint8_t smem[];
+  using Q = Query<FMT>;
+  constexpr int KS = D / 16;   // dim blocks of the output
+  extern __shared__ uint8_t smem_raw[];
   __shared__ long long s_sum[kWarps];
+  __shared__ int s_max[kWarps], s_some[kWarps];
   __shared__ Unit s_first;
   __shared__ float2 s_ml[kWarps][NG * 8];
-  __shared__ int s_flag;
+  __shared__ int s_flag, s_idle[kWarps];
+  __shared__ int s_lens[kLensCached];
+  // chunk_offset's rows start on 128-byte boundaries
+  uint8_t* const smem = smem_raw + (-smem_addr(smem_raw) & 127);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int G = a.group, hkv = a.pool.n_kv_heads;
+  const long long cap = a.index.capacity();
 
   allow_dependent_launch();
   grid_dependency_wait();
 
-  // ---- this CTA's share [w0, w1) of all tiles, and the unit w0 lies in ----
+  // ---- this CTA's share of all tiles, and the unit in which it starts ----
+  auto load_len = [&](int b) {
+    const int len = __ldcg(a.lens + b);
+    return (int)min((long long)max(len, 0), cap);
+  };
+  auto len_of = [&](int b) { return b < kLensCached ? s_lens[b] : load_len(b); };
+  auto next_unit = [&](Unit& u) {
+    u.base += u.tiles;
+    if (++u.kvh == hkv) {
+      u.kvh = 0;
+      do {
+        ++u.b;
+        u.len = u.b < a.batch ? len_of(u.b) : 0;
+        u.tiles = u.b < a.batch ? tiles_of(u.len) : 0x3fffffff;
+      } while (u.tiles == 0);
+    }
+  };
   const int per_thread = (a.batch + kThreads - 1) / kThreads;
   const int b_lo = min(a.batch, (int)threadIdx.x * per_thread), b_hi = min(a.batch, b_lo + per_thread);
   long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += seq_tiles(a, b);
+  int longest = 0, some = 0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int raw = __ldcg(a.lens + b);
+    const int len = (int)min((long long)max(raw, 0), cap);
+    if (raw != len) atomicOr(a.status, kDevBadLength);
+    if (b < kLensCached) s_lens[b] = len;
+    mine += tiles_of(len);
+    longest = max(longest, tiles_of(len));
+    some += len > 0;
+  }
   long long incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += x;
   }
-  if (lane == 31) s_sum[warp] = incl;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  some = __reduce_add_sync(0xffffffffu, some);
+  if (lane == 31) {
+    s_sum[warp] = incl;
+    s_max[warp] = longest;
+    s_some[warp] = some;
+  }
   __syncthreads();
   long long before = incl - mine, total = 0;
+  longest = some = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
+    longest = max(longest, s_max[w]);
+    some += s_some[w];
   }
   before *= hkv;
   total *= hkv;
   // sequences without tokens give zeros
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
-    if (__ldcg(a.lens + b) <= 0)
-      for (int i = threadIdx.x; i < a.n_q_heads * D / 8; i += kThreads)
-        reinterpret_cast<uint4*>(a.o + (long long)b * a.n_q_heads * D)[i] = make_uint4(0, 0, 0, 0);
-  const int n_ctas = (int)min((long long)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
-  if ((int)blockIdx.x >= n_ctas) return;
-  const long long per = total / n_ctas, rem = total % n_ctas;
+  if (some < a.batch)
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+      if (len_of(b) == 0)
+        for (int i = threadIdx.x; i < a.n_q_heads * D / 8; i += kThreads)
+          reinterpret_cast<uint4*>(a.o + (long long)b * a.n_q_heads * D)[i] = make_uint4(0, 0, 0, 0);
+  const bool one_each = longest <= kWholeTiles && (long long)a.batch * hkv <= gridDim.x;
+  long long per = 0, rem = 0, w0 = 0;
   auto cta_start = [&](long long c) { return c * per + min(c, rem); };
   auto cta_of = [&](long long id) {
-    return (int)(id < rem * (per + 1) ? id / (per + 1) : rem + (id - rem * (per + 1)) / per);
+    return (int)(id < rem * (per + 1) ? quotient(id, per + 1) : rem + quotient(id - rem * (per + 1), per));
   };
-  const long long w0 = cta_start(blockIdx.x), w1 = cta_start(blockIdx.x + 1);
-  if (w0 >= before && w0 < before + mine * hkv) {
-    Unit u{0, 0, 0, b_lo, 0};
-    u.tiles = seq_tiles(a, u.b, &u.len);
-    while (w0 >= before + (long long)u.tiles * hkv) {  // by whole sequences (tiles may be 0)
-      before += (long long)u.tiles * hkv;
-      ++u.b;
-      u.tiles = seq_tiles(a, u.b, &u.len);
+  int share;
+  if (one_each) {  // CTA c takes unit c
+    const int b = blockIdx.x / hkv;
+    if (b >= a.batch || len_of(b) == 0) return;
+    share = tiles_of(len_of(b));
+    if (threadIdx.x == 0) s_first = Unit{0, share, len_of(b), b, (int)blockIdx.x - b * hkv};
+  } else {
+    const long long want = max((total + kMinTiles - 1) / kMinTiles, (long long)some * hkv);
+    const int n_ctas = (int)min((long long)gridDim.x, want);
+    if ((int)blockIdx.x >= n_ctas) return;
+    per = quotient(total, n_ctas);
+    rem = total - per * n_ctas;
+    w0 = cta_start(blockIdx.x);
+    share = (int)(cta_start(blockIdx.x + 1) - w0);
+    if (w0 >= before && w0 < before + mine * hkv) {
+      Unit u{0, 0, len_of(b_lo), b_lo, 0};
+      u.tiles = tiles_of(u.len);
+      while (w0 >= before + (long long)u.tiles * hkv) {  // by whole sequences (tiles may be 0)
+        before += (long long)u.tiles * hkv;
+        ++u.b;
+        u.len = len_of(u.b);
+        u.tiles = tiles_of(u.len);
+      }
+      u.kvh = (int)quotient(w0 - before, u.tiles);
+      u.base = (int)(before + (long long)u.kvh * u.tiles - w0);  // at most 0
+      s_first = u;
     }
-    u.kvh = (int)((w0 - before) / u.tiles);
-    u.base = (int)(before + (long long)u.kvh * u.tiles - w0);  // at most 0
-    s_first = u;
   }
   __syncthreads();
-  const int share = (int)(w1 - w0);
 
   // ---- the warp's ring ----
-  uint8_t* const ring = smem + warp * (C::kStages * C::kStageBytes);
+  uint8_t* const ring = smem + warp * C::kWarpBytes;
   constexpr int kChunks = D / 16, kRowsPer = 32 / kChunks;  // a warp copies kRowsPer rows (512 bytes) at a time
   const uint32_t copy_even = chunk_offset<D>(lane / kChunks, lane % kChunks);
   const uint32_t copy_odd = chunk_offset<D>(lane / kChunks + kRowsPer, lane % kChunks) - 512;
-  const uint32_t copy_scale = 2 * C::kRowsBytes + (lane & 3) * 16 + (lane < 4 ? 0 : kTile * 4);
   Unit pu = s_first;     // where the next tile to fetch lies
   int pid = warp;        // its number
   int page[2];           // its pages (one per 16 tokens), fetched a tile ahead
-  const bool big_pages = a.index.page_log2 >= 5;
+  const int log2 = a.index.page_log2;
+  const bool big_pages = log2 >= 5;  // a tile lies in one page
   auto fetch_pages = [&] {
     if (pid >= share) return;
-    while (pid >= pu.base + pu.tiles) pu.next(a);
+    while (pid >= pu.base + pu.tiles) next_unit(pu);
     const int pos = (pid - pu.base) * kTile;
-    const int32_t* entry = a.index.block_table + (long long)pu.b * a.index.pages_per_seq + (pos >> a.index.page_log2);
+    const int32_t* entry = a.index.block_table + (long long)pu.b * a.index.pages_per_seq + (pos >> log2);
     page[0] = __ldcg(entry);
     page[1] = big_pages || pos + 16 >= pu.len ? 0 : __ldcg(entry + 1);
   };
-  auto fetch_half = [&](uint32_t st, int half, int pg, int pos) {
+  auto first_row = [&](int pg, int pos) {  // the pool's row of the unit's token `pos`
     if ((unsigned)pg >= (unsigned)a.index.num_pages) {
       atomicOr(a.status, kDevBadPage);
       pg = 0;
     }
-    const long long row =
-        (((long long)pg * hkv + pu.kvh) << a.index.page_log2) + (pos & ((1 << a.index.page_log2) - 1));
-    const uint8_t* ks = a.pool.k_codes + row * D + lane * 16;
-    const uint8_t* vs = a.pool.v_codes + row * D + lane * 16;
-    const uint32_t even = st + half * (16 * D) + copy_even, odd = st + half * (16 * D) + copy_odd;
+    return (((long long)pg * hkv + pu.kvh) << log2) + (pos & ((1 << log2) - 1));
+  };
+  auto fetch_half = [&](uint32_t st, const uint8_t* ks, const uint8_t* vs) {
+    const uint32_t even = st + copy_even, odd = st + copy_odd;
+    cp_async16<0, 0>(even, ks);
+    cp_async16<512, 512>(odd, ks);
+    cp_async16<C::kRowsBytes, 0>(even, vs);
+    cp_async16<C::kRowsBytes + 512, 512>(odd, vs);
     if constexpr (D == 128) {
-      cp_async16<0, 0>(even, ks);
-      cp_async16<512, 512>(odd, ks);
       cp_async16<1024, 1024>(even, ks);
       cp_async16<1536, 1536>(odd, ks);
-      cp_async16<C::kRowsBytes, 0>(even, vs);
-      cp_async16<C::kRowsBytes + 512, 512>(odd, vs);
       cp_async16<C::kRowsBytes + 1024, 1024>(even, vs);
       cp_async16<C::kRowsBytes + 1536, 1536>(odd, vs);
-    } else {
-      cp_async16<0, 0>(even, ks);
-      cp_async16<512, 512>(odd, ks);
-      cp_async16<C::kRowsBytes, 0>(even, vs);
-      cp_async16<C::kRowsBytes + 512, 512>(odd, vs);
     }
-    if (lane < 8)  // 16 scales of K (lanes 0-3) and of V (lanes 4-7)
-      cp_async16<0, 0>(st + half * 64 + copy_scale,
-                       (lane < 4 ? a.pool.k_scales : a.pool.v_scales) + row + 4 * (lane & 3));
   };
   auto fetch_tile = [&](int stage) {
     if (pid < share) {
       const uint32_t st = smem_addr(ring) + stage * C::kStageBytes;
       const int pos = (pid - pu.base) * kTile;
-      fetch_half(st, 0, page[0], pos);
-      if (pos + 16 < pu.len) fetch_half(st, 1, big_pages ? page[0] : page[1], pos + 16);
+      const bool two = pos + 16 < pu.len;
+      const long long row0 = first_row(page[0], pos);
+      const uint8_t* ks = a.pool.k_codes + row0 * D + lane * 16;
+      const uint8_t* vs = a.pool.v_codes + row0 * D + lane * 16;
+      fetch_half(st, ks, vs);
+      // scales: 16 bytes per lane, K by lanes 0-7 and V by lanes 8-15
+      const float* sc = (lane < 8 ? a.pool.k_scales : a.pool.v_scales) + row0 + 4 * (lane & 7);
+      if (two) {
+        if (!big_pages) {
+          const long long row1 = first_row(page[1], pos + 16);
+          ks = a.pool.k_codes + row1 * D + lane * 16 - 16 * D;
+          vs = a.pool.v_codes + row1 * D + lane * 16 - 16 * D;
+          if (lane & 4) sc += row1 - row0 - 16;
+        }
+        fetch_half(st + 16 * D, ks + 16 * D, vs + 16 * D);
+      }
+      if (lane < 16 && (two || !(lane & 4))) cp_async16<2 * C::kRowsBytes, 0>(st + lane * 16, sc);
       pid += kWarps;
       fetch_pages();
     }
@@ -293,38 +481,37 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
 #pragma unroll
   for (int s = 0; s < C::kStages - 1; ++s) fetch_tile(s);
 
-  // lane-constant places in a stage: the K chunks of rows g (+ 8, 16, 24), the
-  // V chunks of rows 2 t4 and 2 t4 + 1 (+ 8, 16, 24)
-  uint32_t k_at[D / 64], v_at[2];
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) k_at[c] = chunk_offset<D>(g, t4 * (D / 64) + c);
+  // Row g of a block of 16 scores is token 4 (g / 2) + g % 2 (row g + 8: two
+  // on), so that the weights of a lane's column end up in ldmatrix's order.
+  const int tok_at = 4 * (g >> 1) + (g & 1);
+  uint32_t k_at[2][D / 64];  // the lane's chunks of those two rows
 #pragma unroll
   for (int r = 0; r < 2; ++r)
-    v_at[r] = C::kRowsBytes + (D == 128 ? chunk_offset<D>(2 * t4 + r, g)
-                                        : chunk_offset<D>(2 * t4 + r, g >> 1) + 8 * (g & 1));
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) k_at[r][c] = chunk_offset<D>(tok_at + 2 * r, t4 * (D / 64) + c);
+  const uint32_t v_at = C::kRowsBytes + chunk_offset<D>(lane & 15, lane >> 4);
 
   // ---- units of this CTA ----
   int stage = 0;
   int id = warp;         // next tile to work on
   Unit u = s_first;
-  for (; u.base < share; u.next(a)) {
+  for (; u.base < share; next_unit(u)) {
     const int end = min(share, u.base + u.tiles);
-    // q of the group's heads as the 8-column operand: column g, rows in the
-    // order in which codes_to_f16 hands out a lane's K bytes
-    uint32_t qf[NG][KS][2];
+    // q of the group's heads as the 8-column operand: column g, this lane's
+    // dims D / 4 t4 .., which are those of its K chunks
+    uint32_t qf[NG][D / 16][Q::kWords];
     float2 qs[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       const int h = n * 8 + g;
       uint32_t w[D / 8];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) w[i] = 0;
       if (h < G) {
         const uint4* src = reinterpret_cast<const uint4*>(
             a.q + ((long long)u.b * a.n_q_heads + u.kvh * G + h) * D + t4 * (D / 4));
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = __ldcg(src + i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) w[i] = 0;
       }
       uint32_t m = 0;
 #pragma unroll
@@ -332,19 +519,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
       m = max(m & 0xffffu, m >> 16);
-      // largest value to [2^14, 2^15); a NaN or infinity goes through as it is
-      const int e = m >= 0x7f80u ? 0 : max((int)(m >> 7) - 127, -100) - 14;
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+      const bool finite = m < 0x7f80u;
+      const int e = Q::exponent(finite ? m : 0);
+      const float down = finite ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.f;
 #pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        const __half2 lo = __floats2half2_rn(bf16lo(w[2 * j]) * down, bf16lo(w[2 * j + 1]) * down);
-        const __half2 hi = __floats2half2_rn(bf16hi(w[2 * j]) * down, bf16hi(w[2 * j + 1]) * down);
-        qf[n][j][0] = reinterpret_cast<const uint32_t&>(lo);
-        qf[n][j][1] = reinterpret_cast<const uint32_t&>(hi);
+      for (int j = 0; j < D / 16; ++j) {
+        const float x[4] = {bf16lo(w[2 * j]) * down, bf16hi(w[2 * j]) * down, bf16lo(w[2 * j + 1]) * down,
+                            bf16hi(w[2 * j + 1]) * down};
+        Q::split(x, qf[n][j]);
       }
-      // the score factor of heads 2 t4 and 2 t4 + 1, from the lanes that hold them
-      const float f = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2 *
-                      (FMT == LARA_KVQ_FP8_E4M3 ? 256.f : 1.f);
+      // the score factor of heads 2 t4 and 2 t4 + 1, from the lanes that hold
+      // them; a NaN or an infinity in q makes its head NaN
+      const float f = finite ? Q::factor(e) * a.scale_log2 : __uint_as_float(0x7fffffffu);
       qs[n].x = __shfl_sync(0xffffffffu, f, 8 * t4);
       qs[n].y = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
     }
@@ -362,48 +548,48 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       cp_async_wait<C::kStages - 2>();
       __syncwarp();
       fetch_tile(stage == 0 ? C::kStages - 1 : stage - 1);
-      const uint8_t* st = ring + stage * C::kStageBytes;
+      const int at = stage;
+      const uint8_t* st = ring + at * C::kStageBytes;
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
 
-      // ---- scores: s2[i][n], token 8 i + g of the tile, heads 2 t4 and 2 t4 + 1 ----
-      float s[2][NG][4];
-      uint32_t k[4][D / 16];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          *reinterpret_cast<uint4*>(k[i] + 4 * c) = *reinterpret_cast<const uint4*>(st + k_at[c] + i * 8 * D);
-#pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-        for (int n = 0; n < NG; ++n) s[mb][n][0] = s[mb][n][1] = s[mb][n][2] = s[mb][n][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < KS; ++j)
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          uint32_t a0, a1, a2, a3;
-          codes_to_f16<FMT>(k[2 * mb][j], a0, a2);
-          codes_to_f16<FMT>(k[2 * mb + 1][j], a1, a3);
-#pragma unroll
-          for (int n = 0; n < NG; ++n) mma_f16(s[mb][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
-        }
+      // ---- scores: s2[2 mb + r][n] of token 16 mb + 2 r + tok_at, heads 2 t4 and 2 t4 + 1 ----
       float2 s2[4][NG];
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+        uint32_t k[2][D / 16];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            *reinterpret_cast<uint4*>(k[r] + 4 * c) =
+                *reinterpret_cast<const uint4*>(st + k_at[r][c] + mb * 16 * D);
+        float s[NG][4];
+        Q::template scores<D, NG>(s, k[0], k[1], qf);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          s2[2 * mb][n] = make_float2(s[n][0], s[n][1]);
+          s2[2 * mb + 1][n] = make_float2(s[n][2], s[n][3]);
+        }
+      }
       float vsc[4], lw[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float ks = *reinterpret_cast<const float*>(st + 2 * C::kRowsBytes + (8 * i + g) * 4);
-        vsc[i] = *reinterpret_cast<const float*>(st + 2 * C::kRowsBytes + (kTile + 8 * i + g) * 4);
+        const float* sc = reinterpret_cast<const float*>(st + 2 * C::kRowsBytes) + tok_at + 16 * (i / 2) + 2 * (i & 1);
+        vsc[i] = sc[kTile];
         lw[i] = fmaxf(lg2_ftz(vsc[i]), -100.f);
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
-          s2[i][n] = mul2(mul2(make_float2(s[i / 2][n][2 * (i & 1)], s[i / 2][n][2 * (i & 1) + 1]), qs[n]),
-                          make_float2(ks, ks));
+        for (int n = 0; n < NG; ++n) s2[i][n] = mul2(mul2(s2[i][n], qs[n]), make_float2(sc[0], sc[0]));
       }
       const int valid = u.len - (id - u.base) * kTile;
       if (valid < kTile) {  // the sequence's last tile: nothing past its end counts, whatever lies there
+        if (FMT == LARA_KVQ_FP8_E4M3) {  // e4m3 garbage may be NaN, and 0 NaN is NaN
+          for (int i = valid * (D / 16) + lane; i < C::kRowsBytes / 16; i += 32)
+            reinterpret_cast<uint4*>(ring + at * C::kStageBytes + C::kRowsBytes)[i] = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (8 * i + g >= valid) {
+          if (tok_at + 16 * (i / 2) + 2 * (i & 1) >= valid) {
             vsc[i] = 0.f;
             lw[i] = -100.f;
 #pragma unroll
@@ -411,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
           }
       }
 
-      // ---- move R where a weight would pass 2^8 ----
+      // ---- move R where a weight would pass 2^15 ----
       bool over = false;
       float2 top[NG];
 #pragma unroll
@@ -421,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
         for (int i = 0; i < 4; ++i) x[i] = add2(s2[i][n], make_float2(lw[i], lw[i]));
         top[n].x = fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x));
         top[n].y = fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y));
-        over |= top[n].x > R[n][0] + 8.f || top[n].y > R[n][1] + 8.f;
+        over |= top[n].x > R[n][0] + kHigh || top[n].y > R[n][1] + kHigh;
       }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -431,8 +617,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
             float m = c ? top[n].y : top[n].x;
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-            if (m > R[n][c] + 8.f) {
-              const float to = ceilf(m), f = ex2_ftz(R[n][c] - to);
+            if (m > R[n][c] + kHigh) {
+              const float to = ceilf(m) - kStart, f = ex2_ftz(R[n][c] - to);
               R[n][c] = to;
               (c ? l2[n].y : l2[n].x) *= f;
 #pragma unroll
@@ -444,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
           }
       }
 
-      // ---- weights, as the second operand: tokens 2 t4, +1 and + 8 of column g ----
+      // ---- weights, as the second operand: tokens 4 t4 .. + 3 of column g ----
       uint32_t pf[4][NG];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -459,27 +645,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
           pf[i][n] = transpose8x8(reinterpret_cast<const uint32_t&>(w));
         }
 
-      // ---- O^T += V^T P^T: this lane's dims are D / 8 g .. of four tokens ----
+      // ---- O^T += V^T P^T: block c holds dims 16 c + g and 16 c + g + 8 ----
+      const uint32_t v_base = smem_addr(st) + v_at;
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb) {
-        uint32_t v[4][D / 32];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint8_t* at = st + v_at[r & 1] + (16 * mb + 8 * (r >> 1)) * D;
-          if constexpr (D == 128) *reinterpret_cast<uint4*>(v[r]) = *reinterpret_cast<const uint4*>(at);
-          else *reinterpret_cast<uint2*>(v[r]) = *reinterpret_cast<const uint2*>(at);
-        }
+        for (int c = 0; c < KS; c += 2) {
+          uint32_t v[4];
+          load_transposed(v, (v_base ^ (c << 4)) + mb * 16 * D);
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const uint32_t sel = hf ? 0x7632 : 0x5410;
+          for (int i = 0; i < 2; ++i) {
             uint32_t a0, a1, a2, a3;
-            codes_to_f16<FMT>(__byte_perm(v[0][w], v[1][w], sel), a0, a1);
-            codes_to_f16<FMT>(__byte_perm(v[2][w], v[3][w], sel), a2, a3);
+            codes_to_f16<FMT>(v[2 * i], a0, a2);
+            codes_to_f16<FMT>(v[2 * i + 1], a1, a3);
 #pragma unroll
-            for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * w + hf], a0, a1, a2, a3, pf[2 * mb][n], pf[2 * mb + 1][n]);
+            for (int n = 0; n < NG; ++n) mma_f16(o[n][c + i], a0, a1, a2, a3, pf[2 * mb][n], pf[2 * mb + 1][n]);
           }
+        }
       }
     }
     float l[NG][2];
@@ -489,7 +671,25 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       l[n][1] = l2[n].y;
     }
 
-    // ---- join the warps: R and l first, then the scaled sums ----
+    // ---- join the warps: R and l, then the scaled sums, through the stage
+    // that held the warp's last tile (its next fetch will fill it) ----
+    const int idle = (stage == 0 ? C::kStages : stage) - 1;
+    float* const sums = reinterpret_cast<float*>(ring + idle * C::kStageBytes);
+    if (lane == 0) s_idle[warp] = warp * C::kWarpBytes + idle * C::kStageBytes;
+    const bool whole = u.base >= 0 && u.base + u.tiles <= share;
+    const int slot = 2 * (int)blockIdx.x + (u.base > 0 ? 1 : 0);
+    const long long out_row = (long long)u.b * a.n_q_heads + u.kvh * G;
+    // a unit of several CTAs: which ones, and whether all others are done
+    const long long first_tile = w0 + u.base;
+    const int c_first = whole ? 0 : cta_of(first_tile);
+    const int parts = whole ? 1 : cta_of(first_tile + u.tiles - 1) - c_first + 1;
+    int* const counter = a.counters + (long long)u.b * hkv + u.kvh;
+    auto slot_of = [&](int c) { return 2 * c + (first_tile > cta_start(c) ? 1 : 0); };
+    if (threadIdx.x == 0) {
+      const bool last = parts > 1 && parts <= kFewParts && load_acquire(counter) == parts - 1;
+      if (last) *counter = 0;
+      s_flag = last;
+    }
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -499,150 +699,130 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
         if (g == 0) s_ml[warp][n * 8 + 2 * t4 + c] = make_float2(R[n][c], l[n][c]);
       }
     __syncthreads();
-    float4* merge = reinterpret_cast<float4*>(smem + C::kRingBytes);
-    const bool whole = u.base >= 0 && u.base + u.tiles <= share;
-    const int slot = 2 * (int)blockIdx.x + (u.base > 0 ? 1 : 0);
+    const bool last_here = s_flag;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      float L[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][n * 8 + 2 * t4 + c].x);
-        L[c] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 ml = s_ml[w][n * 8 + 2 * t4 + c];
-          L[c] = fmaf(ml.y, ml.x == top ? 1.f : ex2_ftz(ml.x - top), L[c]);
-        }
         const float f = R[n][c] == top ? 1.f : ex2_ftz(R[n][c] - top);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          o[n][i][c] *= f;
-          o[n][i][2 + c] *= f;
+          sums[(2 * t4 + c) * C::kPitch + 16 * i + g] = o[n][i][c] * f;
+          sums[(2 * t4 + c) * C::kPitch + 16 * i + g + 8] = o[n][i][2 + c] * f;
         }
-        R[n][c] = top;
       }
-      if (n > 0) __syncthreads();  // warp 0 has read the first eight heads
-      if (warp > 0)
-#pragma unroll
-        for (int i = 0; i < KS; ++i)
-          merge[((warp - 1) * KS + i) * 32 + lane] = make_float4(o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]);
       __syncthreads();
-      if (warp == 0) {
+      const int heads = min(8, G - 8 * n);
+      for (int item = threadIdx.x; item < heads * (D / 4); item += kThreads) {
+        const int hl = item / (D / 4), d = item % (D / 4) * 4, h = 8 * n + hl;
+        float top = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps - 1; ++w)
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][h].x);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            const float4 x = merge[(w * KS + i) * 32 + lane];
-            o[n][i][0] += x.x;
-            o[n][i][1] += x.y;
-            o[n][i][2] += x.z;
-            o[n][i][3] += x.w;
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = s_ml[w][h];
+          L = fmaf(ml.y, ml.x == top ? 1.f : ex2_ftz(ml.x - top), L);
+          const float4 y = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(smem + s_idle[w]) + hl * C::kPitch + d);
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
+        }
+        if (last_here) {  // the other parts lie ready: join them here, in CTA order
+          float2 ml[kFewParts];
+          float4 y[kFewParts];
+#pragma unroll
+          for (int i = 0; i < kFewParts; ++i) {
+            const int c = c_first + i;
+            ml[i] = make_float2(top, L);
+            y[i] = x;
+            if (i < parts && c != (int)blockIdx.x) {
+              const long long at = (long long)slot_of(c) * G + h;
+              ml[i] = __ldcg(a.part_ml + at);
+              y[i] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + at * D + d));
+            }
           }
+          join_start(top, L, x);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int h = n * 8 + 2 * t4 + c;
-          if (h >= G) continue;
-          if (whole) {
-            const float inv = (FMT == LARA_KVQ_FP8_E4M3 ? 256.f : 1.f) / L[c];
-            uint16_t* dst = a.o + ((long long)u.b * a.n_q_heads + u.kvh * G + h) * D + g * (D / 8);
+          for (int i = 0; i < kFewParts; ++i)
+            if (i < parts) join_top(top, ml[i]);
 #pragma unroll
-            for (int i = 0; i < KS; i += 4)
-              *reinterpret_cast<uint4*>(dst + 2 * i) =
-                  make_uint4(pack2_rn(o[n][i][c] * inv, o[n][i][2 + c] * inv),
-                             pack2_rn(o[n][i + 1][c] * inv, o[n][i + 1][2 + c] * inv),
-                             pack2_rn(o[n][i + 2][c] * inv, o[n][i + 2][2 + c] * inv),
-                             pack2_rn(o[n][i + 3][c] * inv, o[n][i + 3][2 + c] * inv));
-          } else {
-            float* dst = a.part_acc + ((long long)slot * G + h) * D + g * (D / 8);
-#pragma unroll
-            for (int i = 0; i < KS; i += 2)
-              *reinterpret_cast<float4*>(dst + 2 * i) =
-                  make_float4(o[n][i][c], o[n][i][2 + c], o[n][i + 1][c], o[n][i + 1][2 + c]);
-            if (g == 0) a.part_ml[(long long)slot * G + h] = make_float2(R[n][c], L[c]);
-          }
+          for (int i = 0; i < kFewParts; ++i)
+            if (i < parts) join_add(top, L, x, ml[i], y[i]);
+        }
+        if (whole || last_here) {
+          const float inv = 1.f / L;
+          *reinterpret_cast<uint2*>(a.o + (out_row + h) * D + d) =
+              make_uint2(pack2_rn(x.x * inv, x.y * inv), pack2_rn(x.z * inv, x.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(a.part_acc + ((long long)slot * G + h) * D + d) = x;
+          if (d == 0) a.part_ml[(long long)slot * G + h] = make_float2(top, L);
         }
       }
+      if (n + 1 < NG || whole || last_here) __syncthreads();  // the idle stages may be filled again
     }
-    if (whole) continue;
+    if (whole || last_here) continue;
 
-    // ---- a unit of several CTAs: the last one joins the partial results ----
-    const long long first_tile = w0 + u.base;
-    const int c_first = cta_of(first_tile), c_last = cta_of(first_tile + u.tiles - 1), parts = c_last - c_first + 1;
-    if (warp == 0) {
-      __threadfence();
-      __syncwarp();
-      if (lane == 0) {
-        int* ctr = a.counters + (long long)u.b * hkv + u.kvh;
-        const int last = atomicAdd(ctr, 1) == parts - 1;
-        if (last) *ctr = 0;
-        s_flag = last;
-      }
+    // ---- this part is published; the last CTA to do so joins them all ----
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const bool last = atomicAdd(counter, 1) == parts - 1;
+      if (last) *counter = 0;
+      s_flag = last;
     }
     __syncthreads();
     if (s_flag) {
       __threadfence();
-      // thread -> four dims of a head, items G * D / 4; every (R, l) of a
-      // chunk of parts goes through shared memory
-      float2* ml = reinterpret_cast<float2*>(merge);
-      constexpr int kItemsMax = NG * 8 * D / 4;
-      constexpr int kPer = (kItemsMax + kThreads - 1) / kThreads;
+      // thread -> four dims of a head; every (R, l) of a chunk of parts goes
+      // through shared memory, and so does the largest R
+      float2* const ml = reinterpret_cast<float2*>(smem + s_idle[0]);
+      constexpr int kPer = (NG * 8 * D / 4 + kThreads - 1) / kThreads;
       float4 acc[kPer];
       float top[kPer], L[kPer];
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        top[k] = -INFINITY;
-        L[k] = 0.f;
-      }
-      auto slot_of = [&](int c) { return 2 * c + (first_tile > cta_start(c) ? 1 : 0); };
-      for (int p0 = 0; p0 < parts; p0 += C::kJoinChunk) {
-        const int np = min(C::kJoinChunk, parts - p0);
-        __syncthreads();
-        for (int i = threadIdx.x; i < np * G; i += kThreads)
-          ml[i] = __ldcg(a.part_ml + (long long)slot_of(c_first + p0 + i / G) * G + i % G);
-        __syncthreads();
+      for (int k = 0; k < kPer; ++k) join_start(top[k], L[k], acc[k]);
+      for (int pass = 0; pass < 2; ++pass)  // the largest R, then the sums
+        for (int p0 = 0; p0 < parts; p0 += C::kJoinChunk) {
+          const int np = min(C::kJoinChunk, parts - p0);
+          if (pass == 0 || parts > C::kJoinChunk) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < np * G; i += kThreads)
+              ml[i] = __ldcg(a.part_ml + (long long)slot_of(c_first + p0 + i / G) * G + i % G);
+            __syncthreads();
+          }
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-          const int item = threadIdx.x + k * kThreads;
-          if (item >= G * D / 4) continue;
-          const int h = item / (D / 4), d = item % (D / 4);
-          float m = top[k];
-          for (int i = 0; i < np; ++i) m = fmaxf(m, ml[i * G + h].x);
-          const float f = top[k] == m ? 1.f : ex2_ftz(top[k] - m);
-          top[k] = m;
-          L[k] *= f;
-          acc[k].x *= f;
-          acc[k].y *= f;
-          acc[k].z *= f;
-          acc[k].w *= f;
-#pragma unroll 8
-          for (int i = 0; i < np; ++i) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(
-                                        a.part_acc + ((long long)slot_of(c_first + p0 + i) * G + h) * D) + d);
-            const float2 r = ml[i * G + h];
-            const float w = r.x == m ? 1.f : ex2_ftz(r.x - m);
-            L[k] = fmaf(r.y, w, L[k]);
-            acc[k].x = fmaf(x.x, w, acc[k].x);
-            acc[k].y = fmaf(x.y, w, acc[k].y);
-            acc[k].z = fmaf(x.z, w, acc[k].z);
-            acc[k].w = fmaf(x.w, w, acc[k].w);
+          for (int k = 0; k < kPer; ++k) {
+            const int item = threadIdx.x + k * kThreads;
+            if (item >= G * D / 4) continue;
+            const int h = item / (D / 4), d = item % (D / 4);
+            if (pass == 0) {
+              for (int i = 0; i < np; ++i) join_top(top[k], ml[i * G + h]);
+            } else {
+#pragma unroll 16
+              for (int i = 0; i < np; ++i)
+                join_add(top[k], L[k], acc[k], ml[i * G + h],
+                         __ldcg(reinterpret_cast<const float4*>(
+                                    a.part_acc + ((long long)slot_of(c_first + p0 + i) * G + h) * D) + d));
+            }
           }
         }
-      }
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
         const int item = threadIdx.x + k * kThreads;
         if (item >= G * D / 4) continue;
         const int h = item / (D / 4), d = item % (D / 4);
-        const float inv = (FMT == LARA_KVQ_FP8_E4M3 ? 256.f : 1.f) / L[k];
-        *reinterpret_cast<uint2*>(a.o + ((long long)u.b * a.n_q_heads + u.kvh * G + h) * D + 4 * d) =
+        const float inv = 1.f / L[k];
+        *reinterpret_cast<uint2*>(a.o + (out_row + h) * D + 4 * d) =
             make_uint2(pack2_rn(acc[k].x * inv, acc[k].y * inv), pack2_rn(acc[k].z * inv, acc[k].w * inv));
       }
     }
-    __syncthreads();  // s_flag and the merge area are free again
+    __syncthreads();  // s_flag and the idle stages are free again
   }
   cp_async_wait<0>();
 }
@@ -687,9 +867,10 @@ cudaError_t launch(const KvqDecodeArgs& a, cudaStream_t stream) {
       if (dev <= 63) done |= 1ull << dev;
     }
   }
-  // no more CTAs than tiles of a full cache could feed
-  const long long tiles = (long long)a.batch * a.pool.n_kv_heads * ((a.index.capacity() + kTile - 1) / kTile);
-  const long long ctas = std::min<long long>(max_ctas<D, NG>(), (tiles + kMinTiles - 1) / kMinTiles);
+  // no more CTAs than a full cache could feed, one for each unit at least
+  const long long units = (long long)a.batch * a.pool.n_kv_heads;
+  const long long tiles = units * ((a.index.capacity() + kTile - 1) / kTile);
+  const long long ctas = std::min<long long>(max_ctas<D, NG>(), std::max(units, (tiles + kMinTiles - 1) / kMinTiles));
   KvqDecodeArgs args = a;
   void* p[] = {&args};
   return launch_with_pdl(fn, dim3((unsigned)ctas), dim3(kThreads), p, C::kSmemBytes, stream);
