@@ -52,11 +52,18 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;          // tokens per warp and stage
-constexpr int kMinTiles = kWarps;  // tiles per CTA below which fewer CTAs run
-#ifndef WHOLE
-#define WHOLE 12
-#endif
-constexpr int kWholeTiles = WHOLE; // units up to this long are not split while each has a CTA
+constexpr int kMinTiles = kWarps;    // tiles per CTA below which fewer CTAs run
+// Units up to this long are not split while each has a CTA: 8 units of 32 tiles
+// take 10.6 us, as long as split; of 19 tiles 8.1 against 12.9 us.
+constexpr int kWholeTiles = 32;
+// Units up to this long, and up to four times as long as there are units per
+// CTA, go to a warp each: 2400 units of 1-4 tiles 17 against 29 us, of 1-10
+// tiles 28 against 38, but 512 units of 10 tiles 20 against 16 us.
+constexpr int kSoloTiles = 16;
+// What a unit costs beside its tiles, in tiles, where shares are measured out
+// (2400 units of 1-10 tiles: 38 us; 78 us without).
+constexpr int kUnitCost = 8, kUnitCostSolo = 2;
+constexpr int kJoinUnroll = 8;     // parts whose sums a join loads together
 constexpr int kFewParts = 4;       // parts of a unit that its last CTA joins without publishing its own
 constexpr int kLensCached = 1024;  // lengths kept in shared memory
 constexpr size_t kStatusBytes = 256;
@@ -64,22 +71,15 @@ constexpr size_t kStatusBytes = 256;
 // Weights lie in fp16 between 2^kStart (the largest, when R is set) and 2^kHigh.
 constexpr float kStart = 7.f, kHigh = 15.f;
 
-#ifndef ST128
-#define ST128 2
-#define CTA128 3
-#define ST64 3
-#define CTA64 4
-#endif
 template <int D, int NG>
 struct Cfg {
-  static constexpr int kStages = D == 128 ? ST128 : ST64;
-  static constexpr int kCtasPerSm = D == 128 ? (NG == 1 ? CTA128 : 2) : (NG == 1 ? CTA64 : 3);
+  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr int kCtasPerSm = D == 128 ? (NG == 1 ? 3 : 2) : (NG == 1 ? 4 : 3);
   static constexpr int kRowsBytes = kTile * D;                     // K (or V) codes of a stage
   static constexpr int kStageBytes = 2 * kRowsBytes + 2 * kTile * 4;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kSmemBytes = kWarps * kWarpBytes + 128;
   static constexpr int kPitch = D + 4;  // floats per head in the join (lanes of a store hit distinct banks)
-  static constexpr int kJoinChunk = 8 * D * 4 / (NG * 8 * 8);  // partial (R, l) the join stages at a time
   static_assert(kStageBytes % 128 == 0, "rows start on 128-byte boundaries");
   static_assert(8 * kPitch * 4 <= kStageBytes, "a stage holds the sums of eight heads");
 };
@@ -265,20 +265,19 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
   return a / b;
 }
 
-// A unit (b, kvh) in the end-to-end order of tiles; `base` is its first tile,
-// counted from the CTA's own first.
+// A unit (b, kvh); `base` is its first tile, counted from the start of the
+// share that this CTA (or warp) works on.
 struct Unit {
   int base, tiles, len, b, kvh;
 };
 
 // Parts of a unit are joined as o = sum_i 2^(R_i - R) o_i / sum_i 2^(R_i - R) l_i
-// with R the largest R_i, i in CTA order, wherever it is done.
+// with R the largest R_i, i in CTA order: the same words whichever CTA does it.
 __device__ __forceinline__ void join_start(float& top, float& L, float4& x) {
   top = -INFINITY;
   L = 0.f;
   x = make_float4(0.f, 0.f, 0.f, 0.f);
 }
-__device__ __forceinline__ void join_top(float& top, const float2& ml) { top = fmaxf(top, ml.x); }
 __device__ __forceinline__ void join_add(float top, float& L, float4& x, const float2& ml, const float4& y) {
   const float w = ml.x == top ? 1.f : ex2_ftz(ml.x - top);
   L = __fmaf_rn(ml.y, w, L);
@@ -287,6 +286,73 @@ __device__ __forceinline__ void join_add(float top, float& L, float4& x, const f
   x.z = __fmaf_rn(y.z, w, x.z);
   x.w = __fmaf_rn(y.w, w, x.w);
 }
+
+// The published parts of one unit: slots `first` (an odd one where its CTA
+// started in another unit), then one per CTA; `own` is this CTA's.
+struct Join {
+  int first, parts, own;
+  __device__ __forceinline__ int slot(int i) const { return i == 0 ? first : (first & ~1) + 2 * i; }
+};
+
+// Joins the published parts of a unit, all threads together.  `ml` holds `room`
+// (R, l) pairs in shared memory: they are brought there first, so that the
+// sums' loads wait for nothing.
+template <int D, int kItems>
+__device__ __forceinline__ void join_published(const KvqDecodeArgs& a, const Join& j, long long out_row, float2* ml,
+                                               int room) {
+  const int G = a.group, most = room / G;
+  float4 x[kItems];
+  float top[kItems], L[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) join_start(top[k], L[k], x[k]);
+  for (int pass = 0; pass < 2; ++pass)  // the largest R, then the sums
+    for (int p0 = 0; p0 < j.parts; p0 += most) {
+      const int np = min(most, j.parts - p0);
+      if (pass == 0 || j.parts > most) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < np * G; i += kThreads)
+          ml[i] = __ldcg(a.part_ml + (long long)j.slot(p0 + i / G) * G + i % G);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) {
+        const int item = threadIdx.x + k * kThreads;
+        if (item >= G * (D / 4)) continue;
+        const int h = item / (D / 4), d = item % (D / 4) * 4;
+        if (pass == 0) {
+          for (int i = 0; i < np; ++i) top[k] = fmaxf(top[k], ml[i * G + h].x);
+        } else {
+#pragma unroll kJoinUnroll
+          for (int i = 0; i < np; ++i)
+            join_add(top[k], L[k], x[k], ml[i * G + h],
+                     __ldcg(reinterpret_cast<const float4*>(
+                         a.part_acc + ((long long)j.slot(p0 + i) * G + h) * D + d)));
+        }
+      }
+    }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int item = threadIdx.x + k * kThreads;
+    if (item >= G * (D / 4)) continue;
+    const float inv = 1.f / L[k];
+    *reinterpret_cast<uint2*>(a.o + (out_row + item / (D / 4)) * D + item % (D / 4) * 4) =
+        make_uint2(pack2_rn(x[k].x * inv, x[k].y * inv), pack2_rn(x[k].z * inv, x[k].w * inv));
+  }
+}
+
+// Equal shares: the first `rem` take one more.
+struct Shares {
+  long long per, rem;
+  __device__ __forceinline__ long long start(long long c) const { return c * per + min(c, rem); }
+  __device__ __forceinline__ int cta(long long tile) const {
+    return (int)(tile < rem * (per + 1) ? quotient(tile, per + 1) : rem + quotient(tile - rem * (per + 1), per));
+  }
+};
+
+// Few units: the first CTA of this one's unit, how many it has, this one's tiles.
+struct Part {
+  int first, parts, tiles;
+};
 
 __device__ __forceinline__ int load_acquire(const int* p) {
   int v;
@@ -303,7 +369,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long s_sum[kWarps];
   __shared__ int s_max[kWarps], s_some[kWarps];
-  __shared__ Unit s_first;
+  __shared__ Unit s_first[kWarps];
+  __shared__ Part s_part;
+  __shared__ Shares s_shares;
   __shared__ float2 s_ml[kWarps][NG * 8];
   __shared__ int s_flag, s_idle[kWarps];
   __shared__ int s_lens[kLensCached];
@@ -322,8 +390,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     return (int)min((long long)max(len, 0), cap);
   };
   auto len_of = [&](int b) { return b < kLensCached ? s_lens[b] : load_len(b); };
+  int gap = 0;  // units lie this far apart in the order that is shared out
   auto next_unit = [&](Unit& u) {
-    u.base += u.tiles;
+    u.base += u.tiles + gap;
     if (++u.kvh == hkv) {
       u.kvh = 0;
       do {
@@ -346,86 +415,140 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     longest = max(longest, tiles_of(len));
     some += len > 0;
   }
-  long long incl = mine;
+  // exclusive prefix of one number per thread, and the sum of all; reads and
+  // writes s_sum between two barriers
+  auto prefix = [&](long long x, long long& sum) {
+    long long incl = x;
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += x;
-  }
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += y;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    long long ahead = incl - x;
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) ahead += s_sum[w];
+      sum += s_sum[w];
+    }
+    return ahead;
+  };
+  const int mine_some = some;
   longest = __reduce_max_sync(0xffffffffu, longest);
   some = __reduce_add_sync(0xffffffffu, some);
   if (lane == 31) {
-    s_sum[warp] = incl;
     s_max[warp] = longest;
     s_some[warp] = some;
   }
-  __syncthreads();
-  long long before = incl - mine, total = 0;
+  // tiles in the low 40 bits, sequences that have some above
+  long long all;
+  const long long ahead = prefix(mine + ((long long)mine_some << 40), all);
+  constexpr long long kLow = (1ll << 40) - 1;
   longest = some = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
     longest = max(longest, s_max[w]);
     some += s_some[w];
   }
-  before *= hkv;
-  total *= hkv;
+  const long long total = (all & kLow) * hkv;
   // sequences without tokens give zeros
   if (some < a.batch)
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
       if (len_of(b) == 0)
         for (int i = threadIdx.x; i < a.n_q_heads * D / 8; i += kThreads)
           reinterpret_cast<uint4*>(a.o + (long long)b * a.n_q_heads * D)[i] = make_uint4(0, 0, 0, 0);
+  // How the tiles are shared.  Short units, each with a CTA: one each.  Few
+  // units: as many CTAs for a unit as it has tiles for, none with parts of two.
+  // Short units, more than CTAs: whole ones to each warp (solo).  Else equal
+  // shares for each CTA, across units, with a cost of its own for each unit.
+  const long long units = (long long)some * hkv;
   const bool one_each = longest <= kWholeTiles && (long long)a.batch * hkv <= gridDim.x;
-  long long per = 0, rem = 0, w0 = 0;
-  auto cta_start = [&](long long c) { return c * per + min(c, rem); };
-  auto cta_of = [&](long long id) {
-    return (int)(id < rem * (per + 1) ? quotient(id, per + 1) : rem + quotient(id - rem * (per + 1), per));
-  };
+  const bool few = !one_each && units * 8 <= gridDim.x;
+  const bool solo = !one_each && !few && longest <= kSoloTiles && (long long)longest * gridDim.x <= 4 * units;
+  if (!one_each && !few) gap = solo ? kUnitCostSolo : kUnitCost;
   int share;
-  if (one_each) {  // CTA c takes unit c
+  if (one_each) {
     const int b = blockIdx.x / hkv;
     if (b >= a.batch || len_of(b) == 0) return;
     share = tiles_of(len_of(b));
-    if (threadIdx.x == 0) s_first = Unit{0, share, len_of(b), b, (int)blockIdx.x - b * hkv};
+    if (threadIdx.x == 0) s_first[0] = Unit{0, share, len_of(b), b, (int)blockIdx.x - b * hkv};
+  } else if (few) {
+    const long long ctas = max(1ll, min(gridDim.x - units, quotient(total, kMinTiles)));
+    const long long per = quotient(total + ctas - 1, ctas);
+    auto parts_of = [&](int b) { return (int)quotient(tiles_of(len_of(b)) + per - 1, per); };
+    __syncthreads();  // s_sum is free again
+    mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) mine += parts_of(b);
+    long long before = prefix(mine, all) * hkv;
+    const int x = blockIdx.x;
+    if (x >= all * hkv) return;
+    if (x >= before && x < before + mine * hkv) {
+      int b = b_lo;
+      while (x >= before + (long long)parts_of(b) * hkv) before += (long long)parts_of(b++) * hkv;
+      const int n = parts_of(b), at = x - (int)before, kvh = at / n, part = at - kvh * n, tiles = tiles_of(len_of(b));
+      const int t0 = (int)quotient((long long)part * tiles, n), t1 = (int)quotient((long long)(part + 1) * tiles, n);
+      s_first[0] = Unit{-t0, tiles, len_of(b), b, kvh};
+      s_part = Part{x - part, n, t1 - t0};
+    }
+    __syncthreads();
+    share = s_part.tiles;
   } else {
-    const long long want = max((total + kMinTiles - 1) / kMinTiles, (long long)some * hkv);
-    const int n_ctas = (int)min((long long)gridDim.x, want);
-    if ((int)blockIdx.x >= n_ctas) return;
-    per = quotient(total, n_ctas);
-    rem = total - per * n_ctas;
-    w0 = cta_start(blockIdx.x);
-    share = (int)(cta_start(blockIdx.x + 1) - w0);
-    if (w0 >= before && w0 < before + mine * hkv) {
-      Unit u{0, 0, len_of(b_lo), b_lo, 0};
-      u.tiles = tiles_of(u.len);
-      while (w0 >= before + (long long)u.tiles * hkv) {  // by whole sequences (tiles may be 0)
-        before += (long long)u.tiles * hkv;
-        ++u.b;
+    const long long span = total + units * gap;
+    const int workers = solo ? (int)gridDim.x * kWarps
+                             : (int)min((long long)gridDim.x, max((total + kMinTiles - 1) / kMinTiles, units));
+    const Shares sh{quotient(span, workers), span - quotient(span, workers) * workers};
+    const int me = solo ? (int)blockIdx.x * kWarps + warp : (int)blockIdx.x;
+    if (!solo && me >= workers) return;
+    share = (int)(sh.start(me + 1) - sh.start(me));
+    if (threadIdx.x == 0) s_shares = sh;
+    // the unit in which each share starts: found by the thread that counted its sequence
+    const long long begin = ((ahead & kLow) + (ahead >> 40) * gap) * hkv;
+    const long long stop = begin + (mine + (long long)mine_some * gap) * hkv;
+    for (int w = 0; w < (solo ? kWarps : 1); ++w) {
+      const long long x = sh.start(solo ? (long long)blockIdx.x * kWarps + w : blockIdx.x);
+      if (x < begin || x >= stop) continue;
+      long long at = begin;
+      Unit u{0, 0, 0, b_lo, 0};
+      for (;; ++u.b) {  // by whole sequences
         u.len = len_of(u.b);
         u.tiles = tiles_of(u.len);
+        const long long span_b = u.tiles ? (long long)(u.tiles + gap) * hkv : 0;
+        if (x < at + span_b) break;
+        at += span_b;
       }
-      u.kvh = (int)quotient(w0 - before, u.tiles);
-      u.base = (int)(before + (long long)u.kvh * u.tiles - w0);  // at most 0
-      s_first = u;
+      u.kvh = (int)quotient(x - at, u.tiles + gap);
+      u.base = (int)(at + (long long)u.kvh * (u.tiles + gap) + gap - x);  // at most gap
+      if (solo && u.base < gap) next_unit(u);  // it belongs to the share that it starts in
+      s_first[w] = u;
     }
   }
   __syncthreads();
+  const Unit u0 = s_first[solo ? warp : 0];
+  const int step = solo ? 1 : kWarps, offset = solo ? 0 : warp;
+  // a unit starts in this share / its tiles of this share are [max(base, 0), tiles_end)
+  auto in_share = [&](const Unit& u) { return share > 0 && (solo ? u.base - gap : u.base) < share; };
+  auto tiles_end = [&](const Unit& u) { return solo ? u.base + u.tiles : min(share, u.base + u.tiles); };
 
   // ---- the warp's ring ----
   uint8_t* const ring = smem + warp * C::kWarpBytes;
   constexpr int kChunks = D / 16, kRowsPer = 32 / kChunks;  // a warp copies kRowsPer rows (512 bytes) at a time
   const uint32_t copy_even = chunk_offset<D>(lane / kChunks, lane % kChunks);
   const uint32_t copy_odd = chunk_offset<D>(lane / kChunks + kRowsPer, lane % kChunks) - 512;
-  Unit pu = s_first;     // where the next tile to fetch lies
-  int pid = warp;        // its number
-  int page[2];           // its pages (one per 16 tokens), fetched a tile ahead
+  Unit pu = u0;                           // where the next tile to fetch lies
+  int pid = max(pu.base, 0) + offset;     // its number
+  int page[2];                            // its pages (one per 16 tokens), fetched a tile ahead
+  bool more = in_share(pu);
   const int log2 = a.index.page_log2;
   const bool big_pages = log2 >= 5;  // a tile lies in one page
   auto fetch_pages = [&] {
-    if (pid >= share) return;
-    while (pid >= pu.base + pu.tiles) next_unit(pu);
+    while (more && pid >= tiles_end(pu)) {
+      next_unit(pu);
+      pid = pu.base + offset;
+      more = in_share(pu);
+    }
+    if (!more) return;
     const int pos = (pid - pu.base) * kTile;
     const int32_t* entry = a.index.block_table + (long long)pu.b * a.index.pages_per_seq + (pos >> log2);
     page[0] = __ldcg(entry);
@@ -452,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     }
   };
   auto fetch_tile = [&](int stage) {
-    if (pid < share) {
+    if (more) {
       const uint32_t st = smem_addr(ring) + stage * C::kStageBytes;
       const int pos = (pid - pu.base) * kTile;
       const bool two = pos + 16 < pu.len;
@@ -472,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
         fetch_half(st + 16 * D, ks + 16 * D, vs + 16 * D);
       }
       if (lane < 16 && (two || !(lane & 4))) cp_async16<2 * C::kRowsBytes, 0>(st + lane * 16, sc);
-      pid += kWarps;
+      pid += step;
       fetch_pages();
     }
     cp_async_commit();
@@ -493,10 +616,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
 
   // ---- units of this CTA ----
   int stage = 0;
-  int id = warp;         // next tile to work on
-  Unit u = s_first;
-  for (; u.base < share; next_unit(u)) {
-    const int end = min(share, u.base + u.tiles);
+  Unit u = u0;
+  for (; in_share(u); next_unit(u)) {
+    const int end = tiles_end(u);
     // q of the group's heads as the 8-column operand: column g, this lane's
     // dims D / 4 t4 .., which are those of its K chunks
     uint32_t qf[NG][D / 16][Q::kWords];
@@ -544,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       for (int i = 0; i < KS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
 
-    for (; id < end; id += kWarps) {
+    for (int id = max(u.base, 0) + offset; id < end; id += step) {
       cp_async_wait<C::kStages - 2>();
       __syncwarp();
       fetch_tile(stage == 0 ? C::kStages - 1 : stage - 1);
@@ -671,22 +793,60 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       l[n][1] = l2[n].y;
     }
 
-    // ---- join the warps: R and l, then the scaled sums, through the stage
-    // that held the warp's last tile (its next fetch will fill it) ----
+    // ---- the unit's end.  Sums go through the stage that held the warp's last
+    // tile (its next fetch will fill it) ----
     const int idle = (stage == 0 ? C::kStages : stage) - 1;
     float* const sums = reinterpret_cast<float*>(ring + idle * C::kStageBytes);
+    const long long out_row = (long long)u.b * a.n_q_heads + u.kvh * G;
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
+    if (solo) {  // this warp has all of it
+      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float inv = 1.f / l[n][c];
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            sums[(2 * t4 + c) * C::kPitch + 16 * i + g] = o[n][i][c] * inv;
+            sums[(2 * t4 + c) * C::kPitch + 16 * i + g + 8] = o[n][i][2 + c] * inv;
+          }
+        }
+        __syncwarp();
+        for (int item = lane; item < min(8, G - 8 * n) * (D / 4); item += 32) {
+          const int hl = item / (D / 4), d = item % (D / 4) * 4;
+          const float4 x = *reinterpret_cast<const float4*>(sums + hl * C::kPitch + d);
+          *reinterpret_cast<uint2*>(a.o + (out_row + 8 * n + hl) * D + d) =
+              make_uint2(pack2_rn(x.x, x.y), pack2_rn(x.z, x.w));
+        }
+        __syncwarp();
+      }
+      continue;
+    }
+    // join the warps: R and l, then the scaled sums
     if (lane == 0) s_idle[warp] = warp * C::kWarpBytes + idle * C::kStageBytes;
     const bool whole = u.base >= 0 && u.base + u.tiles <= share;
-    const int slot = 2 * (int)blockIdx.x + (u.base > 0 ? 1 : 0);
-    const long long out_row = (long long)u.b * a.n_q_heads + u.kvh * G;
     // a unit of several CTAs: which ones, and whether all others are done
-    const long long first_tile = w0 + u.base;
-    const int c_first = whole ? 0 : cta_of(first_tile);
-    const int parts = whole ? 1 : cta_of(first_tile + u.tiles - 1) - c_first + 1;
+    Join j{0, 1, 0};
+    if (!whole) {
+      if (few) {
+        j = Join{2 * s_part.first, s_part.parts, 2 * (int)blockIdx.x};
+      } else {
+        const long long tile0 = s_shares.start(blockIdx.x) + u.base;
+        const int c0 = s_shares.cta(tile0);
+        // a CTA shares at most two units: the one it starts in has slot 0, a later one slot 1
+        j = Join{2 * c0 + (tile0 > s_shares.start(c0) ? 1 : 0), s_shares.cta(tile0 + u.tiles - 1) - c0 + 1,
+                 2 * (int)blockIdx.x + (u.base > 0 ? 1 : 0)};
+      }
+    }
     int* const counter = a.counters + (long long)u.b * hkv + u.kvh;
-    auto slot_of = [&](int c) { return 2 * c + (first_tile > cta_start(c) ? 1 : 0); };
     if (threadIdx.x == 0) {
-      const bool last = parts > 1 && parts <= kFewParts && load_acquire(counter) == parts - 1;
+      const bool last = j.parts > 1 && j.parts <= kFewParts && load_acquire(counter) == j.parts - 1;
       if (last) *counter = 0;
       s_flag = last;
     }
@@ -694,8 +854,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
         if (g == 0) s_ml[warp][n * 8 + 2 * t4 + c] = make_float2(R[n][c], l[n][c]);
       }
     __syncthreads();
@@ -738,11 +896,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
           float4 y[kFewParts];
 #pragma unroll
           for (int i = 0; i < kFewParts; ++i) {
-            const int c = c_first + i;
             ml[i] = make_float2(top, L);
             y[i] = x;
-            if (i < parts && c != (int)blockIdx.x) {
-              const long long at = (long long)slot_of(c) * G + h;
+            if (i < j.parts && j.slot(i) != j.own) {
+              const long long at = (long long)j.slot(i) * G + h;
               ml[i] = __ldcg(a.part_ml + at);
               y[i] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + at * D + d));
             }
@@ -750,18 +907,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
           join_start(top, L, x);
 #pragma unroll
           for (int i = 0; i < kFewParts; ++i)
-            if (i < parts) join_top(top, ml[i]);
+            if (i < j.parts) top = fmaxf(top, ml[i].x);
 #pragma unroll
           for (int i = 0; i < kFewParts; ++i)
-            if (i < parts) join_add(top, L, x, ml[i], y[i]);
+            if (i < j.parts) join_add(top, L, x, ml[i], y[i]);
         }
         if (whole || last_here) {
           const float inv = 1.f / L;
           *reinterpret_cast<uint2*>(a.o + (out_row + h) * D + d) =
               make_uint2(pack2_rn(x.x * inv, x.y * inv), pack2_rn(x.z * inv, x.w * inv));
         } else {
-          *reinterpret_cast<float4*>(a.part_acc + ((long long)slot * G + h) * D + d) = x;
-          if (d == 0) a.part_ml[(long long)slot * G + h] = make_float2(top, L);
+          *reinterpret_cast<float4*>(a.part_acc + ((long long)j.own * G + h) * D + d) = x;
+          if (d == 0) a.part_ml[(long long)j.own * G + h] = make_float2(top, L);
         }
       }
       if (n + 1 < NG || whole || last_here) __syncthreads();  // the idle stages may be filled again
@@ -772,55 +929,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-      const bool last = atomicAdd(counter, 1) == parts - 1;
+      const bool last = atomicAdd(counter, 1) == j.parts - 1;
       if (last) *counter = 0;
       s_flag = last;
     }
     __syncthreads();
     if (s_flag) {
       __threadfence();
-      // thread -> four dims of a head; every (R, l) of a chunk of parts goes
-      // through shared memory, and so does the largest R
-      float2* const ml = reinterpret_cast<float2*>(smem + s_idle[0]);
-      constexpr int kPer = (NG * 8 * D / 4 + kThreads - 1) / kThreads;
-      float4 acc[kPer];
-      float top[kPer], L[kPer];
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) join_start(top[k], L[k], acc[k]);
-      for (int pass = 0; pass < 2; ++pass)  // the largest R, then the sums
-        for (int p0 = 0; p0 < parts; p0 += C::kJoinChunk) {
-          const int np = min(C::kJoinChunk, parts - p0);
-          if (pass == 0 || parts > C::kJoinChunk) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < np * G; i += kThreads)
-              ml[i] = __ldcg(a.part_ml + (long long)slot_of(c_first + p0 + i / G) * G + i % G);
-            __syncthreads();
-          }
-#pragma unroll
-          for (int k = 0; k < kPer; ++k) {
-            const int item = threadIdx.x + k * kThreads;
-            if (item >= G * D / 4) continue;
-            const int h = item / (D / 4), d = item % (D / 4);
-            if (pass == 0) {
-              for (int i = 0; i < np; ++i) join_top(top[k], ml[i * G + h]);
-            } else {
-#pragma unroll 16
-              for (int i = 0; i < np; ++i)
-                join_add(top[k], L[k], acc[k], ml[i * G + h],
-                         __ldcg(reinterpret_cast<const float4*>(
-                                    a.part_acc + ((long long)slot_of(c_first + p0 + i) * G + h) * D) + d));
-            }
-          }
-        }
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int item = threadIdx.x + k * kThreads;
-        if (item >= G * D / 4) continue;
-        const int h = item / (D / 4), d = item % (D / 4);
-        const float inv = 1.f / L[k];
-        *reinterpret_cast<uint2*>(a.o + (out_row + h) * D + 4 * d) =
-            make_uint2(pack2_rn(acc[k].x * inv, acc[k].y * inv), pack2_rn(acc[k].z * inv, acc[k].w * inv));
-      }
+      join_published<D, (NG * 8 * D / 4 + kThreads - 1) / kThreads>(a, j, out_row, reinterpret_cast<float2*>(smem + s_idle[0]),
+                                                                    C::kStageBytes / 8);
     }
     __syncthreads();  // s_flag and the idle stages are free again
   }

@@ -793,3 +793,52 @@ def test_small_batches_and_empty_calls():
     with pytest.raises(ValueError, match="shape"):
         kvquant.gqa_decode_kvq(torch.zeros((2, 4, 128), dtype=torch.bfloat16, device=DEV), case.pool, case.dtable,
                                case.dlens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,G", [(128, 4), (128, 12), (64, 8), (64, 16)])
+@pytest.mark.parametrize("B,hkv,n", [(150, 8, 100), (80, 8, 700), (7, 4, 3000)])
+def test_decode_shares(fmt, D, G, B, hkv, n):
+    """More (sequence, kv head) units than CTAs, short and long, and few long ones; ragged, some empty."""
+    g = torch.Generator().manual_seed(B + D + G)
+    lens = torch.randint(1, n + 1, (B,), generator=g).tolist()
+    lens[0], lens[3], lens[B - 1] = n, 0, 1
+    lens[4:6] = [0, 0]
+    # the same rows for every sequence keep the reference quick; their pages are their own
+    k, v = _rand_bf16(g, (1, hkv, n, D)), _rand_bf16(g, (1, hkv, n, D))
+    case = SharedRows(lens, hkv, D, 64, fmt, k[0], v[0], seed=n)
+    q = _rand_bf16(g, (B, hkv * G, D), False).to(DEV)
+    o = _decode_gpu(case, q)
+    case.check(q, o)
+    assert torch.equal(o, _decode_gpu(case, q))
+
+
+class SharedRows(Case):
+    """Every sequence holds the first rows of one K and V; written page by page."""
+
+    def __init__(self, lens, hkv, D, ps, fmt, k, v, seed=0):
+        from lara_b200 import kvquant
+
+        _need_gpu()
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.fmt, self.D, self.hkv, self.ps = list(lens), fmt, D, hkv, ps
+        n = max(lens)
+        per_seq = -(-n // ps)
+        self.table, pages = _table(g, lens, per_seq, ps)
+        pools, self.k64, self.v64 = [], [], []
+        for x, keep in ((k, self.k64), (v, self.v64)):
+            c, s = quantise64(torch.nn.functional.pad(x, (0, 0, 0, per_seq * ps - n)), fmt)
+            keep += [values64(c, s.float().double())[:, :m] for m in lens]
+            bits = (c.to(torch.int8) if fmt == "int8" else c.float().to(torch.float8_e4m3fn)).view(torch.uint8)
+            codes = torch.zeros((pages, hkv, ps, D), dtype=torch.uint8)
+            scales = torch.zeros((pages, hkv, ps))
+            for b, m in enumerate(lens):
+                for j in range(-(-m // ps)):
+                    p = int(self.table[b, j])
+                    codes[p] = bits[:, j * ps:(j + 1) * ps]
+                    scales[p] = s[:, j * ps:(j + 1) * ps].float()
+            pools.append((codes.to(DEV).view(DTYPES[fmt]), scales.to(DEV)))
+        self.pool = kvquant.QuantPool(pools[0][0], pools[1][0], pools[0][1], pools[1][1])
+        self.dtable = self.table.to(DEV)
+        self.dlens = torch.tensor(self.lens, dtype=torch.int32, device=DEV)
