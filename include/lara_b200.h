@@ -377,6 +377,23 @@ LARA_API int lara_kvq_append(const lara_kvq_pool* pool, const int32_t* block_tab
                              long long k_sb, long long k_sh, long long k_st, const uint16_t* v_new, long long v_sb,
                              long long v_sh, long long v_st, int batch, int n_new, void* workspace, void* stream);
 
+/* A serving step's row work in one launch: lara_qk_norm_rope on q and k, then
+ * lara_kvq_append of the k it gives and of v; the words are those of the two
+ * calls.  q, k, v and q_out are strided (elements): x[b*sb + t*st + h*sh + d],
+ * e.g. views of one projection output.  positions (NULL: starts[b] + t) is
+ * int32[B * n_new].  Weights, cos_sin and the workspace as for
+ * lara_qk_norm_rope (without weights and table k is stored as it is), starts,
+ * counts and new_lens as for lara_kvq_append; q_out is written for all n_new
+ * tokens. */
+LARA_API int lara_kvq_append_qkv(const lara_kvq_pool* pool, const int32_t* block_table, int pages_per_seq,
+                                 const int32_t* starts, const int32_t* counts, int32_t* new_lens, const uint16_t* q,
+                                 long long q_sb, long long q_st, long long q_sh, const uint16_t* k, long long k_sb,
+                                 long long k_st, long long k_sh, const uint16_t* v, long long v_sb, long long v_st,
+                                 long long v_sh, uint16_t* q_out, long long qo_sb, long long qo_st, long long qo_sh,
+                                 int batch, int n_new, int n_q_heads, const int32_t* positions, const float* cos_sin,
+                                 int max_pos, int rot_dim, int interleaved, const uint16_t* q_weight,
+                                 const uint16_t* k_weight, float eps, void* workspace, void* stream);
+
 /* Read rows back as bf16: k/v_out[b*sb + h*sh + t*st + d] (strides in
  * elements) = code * scale (one fp32 product, bf16 nearest even) of token
  * starts[b] + t (starts NULL: t) of sequence b for t in [0, n_tokens); zeros

@@ -124,6 +124,10 @@ SIGNATURES = {
     "lara_kvq_append": (c_int, [POINTER(LaraKvqPool), c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                 *([c_void_p, c_longlong, c_longlong, c_longlong] * 2), c_int, c_int, c_void_p,
                                 c_void_p]),
+    "lara_kvq_append_qkv": (c_int, [POINTER(LaraKvqPool), c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                    *([c_void_p, c_longlong, c_longlong, c_longlong] * 4), c_int, c_int, c_int,
+                                    c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p,
+                                    c_void_p]),
     "lara_kvq_read": (c_int, [POINTER(LaraKvqPool), c_void_p, c_int, c_void_p, c_void_p,
                               *([c_void_p, c_longlong, c_longlong, c_longlong] * 2), c_int, c_int, c_void_p,
                               c_void_p]),

@@ -3,11 +3,13 @@
 // for a quantised cache).
 //
 // Both are bound by HBM: append reads 2 D bytes of bf16 per row and writes
-// D + 4, read the reverse.  D / 8 lanes hold a row.  A warp takes kRows times
-// as many consecutive tokens of one (sequence, kv head) as it has lane groups,
-// K and V: the length, the start and the page of a row are looked up once per
-// warp (at most 16 tokens, so at most two pages), not once per row, and all the
-// tokens' loads are in flight together.
+// D + 4, read the reverse.  D / 16 lanes hold a row, 32 bytes of bf16 each (one
+// access where it is so aligned).  A warp takes as many consecutive tokens of
+// one (sequence, kv head) as it has lane groups, K and V: the length, the start
+// and the pages (two at most) are looked up once per warp, not once per row.
+// 8192 tokens of 8 x 8 heads (head_dim 128) are read back in 63 us, 0.98 of the
+// copy rate (16-byte accesses: 70 us; several rows per lane: 64-65 us), 2048 of
+// 8 x 8 appended and read in 34 us (0.92; 43 us).
 #include <algorithm>
 
 #include "kvq.cuh"
@@ -95,9 +97,42 @@ struct WarpRows {
   static constexpr long long kBad = -(1ll << 62);
 };
 
-template <int D, int FMT, bool kVec, int kRows>
+// How a lane's 16 bf16 values may be accessed: by element, in 16-byte halves, whole.
+enum Access { kElement, kHalf, kFull };
+
+template <Access kA>
+__device__ __forceinline__ void load16(const uint16_t* p, uint32_t w[8]) {
+  if constexpr (kA == kFull) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+  } else if constexpr (kA == kHalf) {
+    *reinterpret_cast<uint4*>(w) = __ldcs(reinterpret_cast<const uint4*>(p));
+    *reinterpret_cast<uint4*>(w + 4) = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+  }
+}
+template <Access kA>
+__device__ __forceinline__ void store16(uint16_t* p, const uint32_t w[8]) {
+  if constexpr (kA == kFull) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else if constexpr (kA == kHalf) {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+
+template <int D, int FMT, Access kA>
 __global__ void __launch_bounds__(kThreads) kvq_append_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int kLanes = D / 8, kGroups = 32 / kLanes;
+  constexpr int kLanes = D / 16, kGroups = 32 / kLanes;
   allow_dependent_launch();
   grid_dependency_wait();
   if (a.new_lens)
@@ -106,22 +141,12 @@ __global__ void __launch_bounds__(kThreads) kvq_append_kernel(const __grid_const
       const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
       a.new_lens[b] = start < 0 ? start : (int)min(end, max(a.index.capacity(), (long long)start));
     }
-  WarpRows<kRows * kGroups> rows;
+  WarpRows<kGroups> rows;
   if (!rows.init(a)) return;
   const int l = threadIdx.x % kLanes, t = rows.t0 + (threadIdx.x & 31) / kLanes;
-  uint32_t w[kRows][2][4];
+  uint32_t w[2][8];
 #pragma unroll
-  for (int j = 0; j < kRows; ++j)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint16_t* src = (i ? a.v : a.k).row(rows.b, min(t + j * kGroups, a.n - 1), rows.h) + 8 * l;
-      if constexpr (kVec) {
-        *reinterpret_cast<uint4*>(w[j][i]) = __ldcs(reinterpret_cast<const uint4*>(src));  // read once
-      } else {
-#pragma unroll
-        for (int m = 0; m < 4; ++m) w[j][i][m] = (uint32_t)src[2 * m] | ((uint32_t)src[2 * m + 1] << 16);
-      }
-    }
+  for (int i = 0; i < 2; ++i) load16<kA>((i ? a.v : a.k).row(rows.b, min(t, a.n - 1), rows.h) + 16 * l, w[i]);
   int count = a.n;
   if (a.counts) {
     count = a.counts[rows.b];
@@ -129,89 +154,77 @@ __global__ void __launch_bounds__(kThreads) kvq_append_kernel(const __grid_const
     count = min(max(count, 0), a.n);
   }
   // tokens [t0, end) have a place in the sequence
-  int end = min(rows.t0 + kRows * kGroups, count);
+  int end = min(rows.t0 + kGroups, count);
   if (end > rows.t0 && (rows.start < 0 || rows.start + end > a.index.capacity())) {
     if (a.status) atomicOr(a.status, kDevAppendOverflow);
     end = rows.start < 0 ? rows.t0 : (int)min((long long)end, a.index.capacity() - rows.start);
   }
   if (end <= rows.t0) return;
   rows.find(a, rows.start + rows.t0, rows.start + end - 1);
+  const long long dst = rows.row(rows.start + t);
+  const bool store = t < end && dst >= 0;
 #pragma unroll
-  for (int j = 0; j < kRows; ++j) {
-    const long long dst = rows.row(rows.start + t + j * kGroups);
-    const bool store = t + j * kGroups < end && dst >= 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t codes[2];
-      const float scale = quantise_row<D, FMT>(w[j][i], codes);
-      if (store) {
-        *reinterpret_cast<uint2*>((i ? a.pool.v_codes : a.pool.k_codes) + dst * D + 8 * l) =
-            make_uint2(codes[0], codes[1]);
-        if (l == 0) (i ? a.pool.v_scales : a.pool.k_scales)[dst] = scale;
-      }
+  for (int i = 0; i < 2; ++i) {
+    uint32_t codes[4];
+    const float scale = quantise_row<kLanes, 8, FMT>(w[i], codes);
+    if (store) {
+      *reinterpret_cast<uint4*>((i ? a.pool.v_codes : a.pool.k_codes) + dst * D + 16 * l) =
+          make_uint4(codes[0], codes[1], codes[2], codes[3]);
+      if (l == 0) (i ? a.pool.v_scales : a.pool.k_scales)[dst] = scale;
     }
   }
 }
 
-template <int D, int FMT, bool kVec, int kRows>
+template <int D, int FMT, Access kA>
 __global__ void __launch_bounds__(kThreads) kvq_read_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int kLanes = D / 8, kGroups = 32 / kLanes;
+  constexpr int kLanes = D / 16, kGroups = 32 / kLanes;
   allow_dependent_launch();
   grid_dependency_wait();
-  WarpRows<kRows * kGroups> rows;
+  WarpRows<kGroups> rows;
   if (!rows.init(a)) return;
   const int l = threadIdx.x % kLanes, t = rows.t0 + (threadIdx.x & 31) / kLanes;
   const int given = a.counts[rows.b];
   const int len = min(max(given, 0), (int)a.index.capacity());
   if (given != len && a.status) atomicOr(a.status, kDevBadLength);
   // positions [lo, hi) of the warp's tokens are cached
-  const long long lo = max(rows.start + rows.t0, 0ll), hi = min(rows.start + rows.t0 + kRows * kGroups, (long long)len);
+  const long long lo = max(rows.start + rows.t0, 0ll), hi = min(rows.start + rows.t0 + kGroups, (long long)len);
   if (lo < hi) rows.find(a, lo, hi - 1);
-  uint2 c[kRows][2];
-  float scale[kRows][2];
-#pragma unroll
-  for (int j = 0; j < kRows; ++j) {
-    const long long pos = rows.start + t + j * kGroups;
-    c[j][0] = c[j][1] = make_uint2(0, 0);
-    scale[j][0] = scale[j][1] = 0.f;
-    if (pos < lo || pos >= hi) continue;
-    const long long src = rows.row(pos);
-    if (src < 0) continue;
+  const long long pos = rows.start + t;
+  const long long src = pos >= lo && pos < hi ? rows.row(pos) : -1;
+  uint4 c[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  float scale[2] = {0.f, 0.f};
+  if (src >= 0) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      c[j][i] = *reinterpret_cast<const uint2*>((i ? a.pool.v_codes : a.pool.k_codes) + src * D + 8 * l);
-      scale[j][i] = (i ? a.pool.v_scales : a.pool.k_scales)[src];
+      c[i] = *reinterpret_cast<const uint4*>((i ? a.pool.v_codes : a.pool.k_codes) + src * D + 16 * l);
+      scale[i] = (i ? a.pool.v_scales : a.pool.k_scales)[src];
     }
   }
+  if (t >= a.n) return;
 #pragma unroll
-  for (int j = 0; j < kRows; ++j) {
-    if (t + j * kGroups >= a.n) break;
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t cw[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+    uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float2 f[4];
-      codes_to_f32<FMT>(c[j][i].x, f);
-      codes_to_f32<FMT>(c[j][i].y, f + 2);
-      uint32_t w[4];
+    for (int m = 0; m < 4; ++m) {
+      float2 f[2];
+      codes_to_f32<FMT>(cw[m], f);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        f[m] = mul2(f[m], make_float2(scale[j][i], scale[j][i]));
-        w[m] = pack2_rn(f[m].x, f[m].y);
-      }
-      uint16_t* dst = (i ? a.vo : a.ko).row(rows.b, t + j * kGroups, rows.h) + 8 * l;
-      if constexpr (kVec) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-#pragma unroll
-        for (int m = 0; m < 8; ++m) dst[m] = (uint16_t)(w[m / 2] >> (16 * (m & 1)));
+      for (int k = 0; k < 2; ++k) {
+        f[k] = mul2(f[k], make_float2(scale[i], scale[i]));
+        w[2 * m + k] = pack2_rn(f[k].x, f[k].y);
       }
     }
+    store16<kA>((i ? a.vo : a.ko).row(rows.b, t, rows.h) + 16 * l, w);
   }
 }
 
-// 16-byte accesses: the base and every stride that is taken (an extent of 1
-// takes none).
-bool vec_ok(const void* p, long long sb, int batch, long long sh, int heads, long long st, int n) {
-  return aligned(p, 16) && (((batch > 1 ? sb : 0) | (heads > 1 ? sh : 0) | (n > 1 ? st : 0)) & 7) == 0;
+// The widest access that the base and every stride allow (an extent of 1 takes
+// no stride).
+Access access_of(const void* p, long long sb, int batch, long long sh, int heads, long long st, int n) {
+  const long long bytes = 2 * ((batch > 1 ? sb : 0) | (heads > 1 ? sh : 0) | (n > 1 ? st : 0)) |
+                          (long long)reinterpret_cast<uintptr_t>(p);
+  return (bytes & 31) == 0 ? kFull : (bytes & 15) == 0 ? kHalf : kElement;
 }
 
 // Whether the rows of a call (at least one per warp) fit one launch.
@@ -224,42 +237,25 @@ bool set_rows(RowArgs* a, const lara_kvq_pool& pool, int batch, int n) {
          (long long)batch * pool.n_kv_heads * n <= 0x3ffffffll;
 }
 
-// Rows per lane group: with enough work for every SM, two (four tokens per
-// warp) halve the look-ups and keep the most bytes in flight; one row each is
-// quicker below that.  8192 tokens of 8 x 8 heads read back (head_dim 128): one
-// 76, two 70, four 78, eight 84 us; 2048 of 8 x 8 appended and read: one 50,
-// two 43, four 45, eight 51 us.
-constexpr int many(int d) { return d == 128 ? 2 : 1; }
-
 template <int D>
-cudaError_t launch_rows(const void* one, const void* several, RowArgs a, void* stream) {
-  constexpr int kGroups = 256 / D;
-  const long long bh = (long long)a.batch * a.pool.n_kv_heads;
-  const bool few = bh * a.n < (long long)device_sm_count() * 32 * many(D) * kGroups;
-  const int tokens = kGroups * (few ? 1 : many(D));
-  const int tiles = (a.n + tokens - 1) / tokens;
+cudaError_t launch_rows(const void* kernel, RowArgs a, void* stream) {
+  constexpr int kTokens = 512 / D;  // a warp's
+  const int tiles = (a.n + kTokens - 1) / kTokens;
   a.div_tiles = FastDiv((uint32_t)std::max(tiles, 1));
-  a.tiles = (uint32_t)(bh * tiles);
+  a.tiles = (uint32_t)((long long)a.batch * a.pool.n_kv_heads * tiles);
   const unsigned blocks = std::max(1u, (a.tiles + kThreads / 32 - 1) / (kThreads / 32));  // no rows: new_lens alone
   void* args[] = {&a};
-  return launch_with_pdl(few ? one : several, dim3(blocks), dim3(kThreads), args, 0,
-                         static_cast<cudaStream_t>(stream));
+  return launch_with_pdl(kernel, dim3(blocks), dim3(kThreads), args, 0, static_cast<cudaStream_t>(stream));
 }
 
-#define LARA_KVQ_LAUNCH(kernel, d, f, v)                                                             \
-  if (pool->head_dim == d && pool->format == f && vec == v)                                         \
-    e = launch_rows<d>(reinterpret_cast<const void*>(&kernel<d, f, v, 1>),                           \
-                       reinterpret_cast<const void*>(&kernel<d, f, v, many(d)>), a, stream);
-#define LARA_KVQ_LAUNCH_ALL(kernel)                                                                   \
-  LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_INT8, true) LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_INT8, false) \
-  LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_FP8_E4M3, true) LARA_KVQ_LAUNCH(kernel, 128, LARA_KVQ_FP8_E4M3, false) \
-  LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_INT8, true) LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_INT8, false) \
-  LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_FP8_E4M3, true) LARA_KVQ_LAUNCH(kernel, 64, LARA_KVQ_FP8_E4M3, false)
-
-bool overlap(const void* a, const void* b, size_t bytes) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return a && b && x < y + bytes && y < x + bytes;
-}
+#define LARA_KVQ_LAUNCH(kernel, d, f, v)                            \
+  if (pool->head_dim == d && pool->format == f && access == v)     \
+    e = launch_rows<d>(reinterpret_cast<const void*>(&kernel<d, f, v>), a, stream);
+#define LARA_KVQ_LAUNCH_ACCESS(kernel, d, f) \
+  LARA_KVQ_LAUNCH(kernel, d, f, kElement) LARA_KVQ_LAUNCH(kernel, d, f, kHalf) LARA_KVQ_LAUNCH(kernel, d, f, kFull)
+#define LARA_KVQ_LAUNCH_ALL(kernel)                                                                       \
+  LARA_KVQ_LAUNCH_ACCESS(kernel, 128, LARA_KVQ_INT8) LARA_KVQ_LAUNCH_ACCESS(kernel, 128, LARA_KVQ_FP8_E4M3) \
+  LARA_KVQ_LAUNCH_ACCESS(kernel, 64, LARA_KVQ_INT8) LARA_KVQ_LAUNCH_ACCESS(kernel, 64, LARA_KVQ_FP8_E4M3)
 
 }  // namespace
 
@@ -291,8 +287,8 @@ extern "C" int lara_kvq_append(const lara_kvq_pool* pool, const int32_t* block_t
   if (!set_rows(&a, *pool, batch, n_new)) return set_last_error(LARA_ERR_BAD_CFG, "too many rows for one launch");
   if (n_new == 0 && !new_lens) return LARA_OK;
   const int heads = pool->n_kv_heads;
-  const bool vec = vec_ok(k_new, k_sb, batch, k_sh, heads, k_st, n_new) &&
-                   vec_ok(v_new, v_sb, batch, v_sh, heads, v_st, n_new);
+  const Access access = std::min(access_of(k_new, k_sb, batch, k_sh, heads, k_st, n_new),
+                                 access_of(v_new, v_sb, batch, v_sh, heads, v_st, n_new));
   cudaError_t e = cudaErrorInvalidValue;
   LARA_KVQ_LAUNCH_ALL(kvq_append_kernel)
   if (e != cudaSuccess)
@@ -320,8 +316,8 @@ extern "C" int lara_kvq_read(const lara_kvq_pool* pool, const int32_t* block_tab
   a.status = static_cast<int*>(workspace);
   if (!set_rows(&a, *pool, batch, n_tokens)) return set_last_error(LARA_ERR_BAD_CFG, "too many rows for one launch");
   const int heads = pool->n_kv_heads;
-  const bool vec = vec_ok(k_out, k_sb, batch, k_sh, heads, k_st, n_tokens) &&
-                   vec_ok(v_out, v_sb, batch, v_sh, heads, v_st, n_tokens);
+  const Access access = std::min(access_of(k_out, k_sb, batch, k_sh, heads, k_st, n_tokens),
+                                 access_of(v_out, v_sb, batch, v_sh, heads, v_st, n_tokens));
   cudaError_t e = cudaErrorInvalidValue;
   LARA_KVQ_LAUNCH_ALL(kvq_read_kernel)
   if (e != cudaSuccess)

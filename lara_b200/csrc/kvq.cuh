@@ -1,7 +1,8 @@
 // Rows of the 8-bit KV pool and of the q/k head pass (sm_100a).
 //
 // A row is the D values of one (token, head).  D / 8 lanes hold it, eight
-// values each, and reduce over it with shuffles; a warp holds 256 / D rows.
+// values each (D / 16 and sixteen where the pool is written or read), and
+// reduce over it with shuffles.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -228,24 +229,22 @@ __device__ __forceinline__ Pairs turn_head(const Pairs& x, const Turn& t, bool r
 constexpr uint32_t kTinyBits = 0x0D800000u;  // 2^-100 as fp32
 
 // Largest |x| of a row of bf16 values as its 15 magnitude bits (which order
-// like the magnitudes, with infinities and NaN above every number).
-template <int D>
-__device__ __forceinline__ uint32_t row_amax(const uint32_t w[4]) {
+// like the magnitudes, with infinities and NaN above every number); kLanes
+// lanes hold the row, kWords words each.
+template <int kLanes, int kWords>
+__device__ __forceinline__ uint32_t row_amax(const uint32_t* w) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
 #pragma unroll
-  for (int off = D / 16; off > 0; off >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, off));
+  for (int off = kLanes / 2; off > 0; off >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, off));
   return max(m & 0xffffu, m >> 16);
 }
 
-// The row's scale and the lane's eight codes.
-template <int D, int FMT>
-__device__ __forceinline__ float quantise_row(const uint32_t w[4], uint32_t codes[2]) {
-  const uint32_t am = row_amax<D>(w);
-  float2 x[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = make_float2(bf16lo(w[i]), bf16hi(w[i]));
+// The row's scale and the lane's codes, in the order of its words.
+template <int kLanes, int kWords, int FMT>
+__device__ __forceinline__ float quantise_row(const uint32_t* w, uint32_t* codes) {
+  const uint32_t am = row_amax<kLanes, kWords>(w);
   float scale;
   if constexpr (FMT == LARA_KVQ_INT8) {
     // rint of the exact quotient 127 x / a, ties to even, from y = x (127 / a)
@@ -258,29 +257,36 @@ __device__ __forceinline__ float quantise_row(const uint32_t w[4], uint32_t code
     const float r = __fdiv_rn(127.f, a);
     const float2 r2 = make_float2(r, r), k65 = make_float2(65.f, 65.f), neg = make_float2(-1.f, -1.f);
     const float2 magic = make_float2(0x1.8p23f, 0x1.8p23f);
-    uint32_t c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 y = mul2(x[i], r2), y65 = mul2(y, k65);
-      const float2 n = add2(fma2(fma2(y, neg, y65), neg, y65), magic);
-      c[i] = __byte_perm(__float_as_uint(n.x), __float_as_uint(n.y), 0x0040);
+    for (int i = 0; i < kWords; i += 2) {
+      uint32_t c[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 y = mul2(make_float2(bf16lo(w[i + k]), bf16hi(w[i + k])), r2), y65 = mul2(y, k65);
+        const float2 n = add2(fma2(fma2(y, neg, y65), neg, y65), magic);
+        c[k] = __byte_perm(__float_as_uint(n.x), __float_as_uint(n.y), 0x0040);
+      }
+      codes[i / 2] = __byte_perm(c[0], c[1], 0x5410);
     }
-    codes[0] = __byte_perm(c[0], c[1], 0x5410);
-    codes[1] = __byte_perm(c[2], c[3], 0x5410);
   } else {
     // a = (1 + m/128) 2^(E-127); 448 = 1.75 * 2^8, and 1 + m/128 <= 1.75 at m <= 96.
     const int e = max((int)(am >> 7) - 135 + ((am & 0x7fu) > 96u ? 1 : 0), -100);
     scale = __uint_as_float((uint32_t)(e + 127) << 23);
     const float inv = __uint_as_float((uint32_t)(127 - e) << 23);  // exact: a power of two
-    uint32_t h[4];
+    const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      h[i] = __nv_cvt_float2_to_fp8x2(mul2(x[i], make_float2(inv, inv)), __NV_SATFINITE, __NV_E4M3);
-    codes[0] = __byte_perm(h[0], h[1], 0x5410);
-    codes[1] = __byte_perm(h[2], h[3], 0x5410);
+    for (int i = 0; i < kWords; i += 2) {
+      uint32_t h[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        h[k] = __nv_cvt_float2_to_fp8x2(mul2(make_float2(bf16lo(w[i + k]), bf16hi(w[i + k])), inv2), __NV_SATFINITE,
+                                        __NV_E4M3);
+      codes[i / 2] = __byte_perm(h[0], h[1], 0x5410);
+    }
   }
   if (am >= 0x7f80u) {
-    codes[0] = codes[1] = 0;
+#pragma unroll
+    for (int i = 0; i < kWords / 2; ++i) codes[i] = 0;
     scale = __uint_as_float(0x7fffffffu);
   }
   return scale;
@@ -328,6 +334,18 @@ struct PoolIndex {
 int check_pool(const lara_kvq_pool* pool, const void* block_table, int pages_per_seq, int batch, PoolIndex* index);
 
 inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Whether two arrays of `bytes` bytes overlap (a null one overlaps nothing).
+inline bool overlap(const void* a, const void* b, size_t bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + bytes && y < x + bytes;
+}
+
+// 16-byte accesses: the base and every stride that is taken (an extent of 1
+// takes none).
+inline bool vec_ok(const void* p, long long sb, int batch, long long st, int n, long long sh, int heads) {
+  return aligned(p, 16) && (((batch > 1 ? sb : 0) | (n > 1 ? st : 0) | (heads > 1 ? sh : 0)) & 7) == 0;
+}
 
 }  // namespace kvq
 }  // namespace lara

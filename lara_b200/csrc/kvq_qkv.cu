@@ -1,0 +1,226 @@
+// The row work of a serving step in one launch (declared in include/lara_b200.h):
+// q and k heads are normed and rotated, k and v quantised into the paged pool.
+//
+// Bound by latency at a decode step (a few hundred rows; one launch in place of
+// two, and k does not go to memory as bf16 in between), by HBM for prompts:
+// q 4 D bytes per head, k and v 2 D + D + 4.  Heads are held, normed and
+// rotated as in qk_rope.cu; k is rounded to bf16 and quantised from there, so
+// the pool gets the words of the two calls.  A lane group takes kHeads heads of
+// one token, all of q, all of k or all of v.
+#include "kvq.cuh"
+
+namespace lara {
+
+using namespace kvq;
+
+namespace {
+
+constexpr int kThreads = 128;
+
+struct QkvArgs {
+  lara_kvq_pool pool;
+  PoolIndex index;
+  const int32_t* starts;
+  const int32_t* counts;
+  int32_t* new_lens;
+  Heads<const uint16_t> q, k, v;
+  Heads<uint16_t> qo;
+  int batch, n, hq, q_chunks, k_chunks;
+  uint32_t groups;  // tokens * chunks
+  FastDiv chunks, div_n;
+  const int32_t* positions;
+  const float* cos_sin;
+  int max_pos, rot;
+  const uint16_t* qw;
+  const uint16_t* kw;
+  float eps;
+  int* status;
+};
+
+template <int D, int FMT, bool kInter, bool kNorm, bool kVec, int kHeads>
+__global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_constant__ QkvArgs a) {
+  constexpr int kLanes = D / 8;
+  allow_dependent_launch();
+  grid_dependency_wait();
+  const long long cap = a.index.capacity();
+  if (a.new_lens)
+    for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.batch; b += gridDim.x * kThreads) {
+      const int start = a.starts[b];
+      const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
+      a.new_lens[b] = start < 0 ? start : (int)min(end, max(cap, (long long)start));
+    }
+  if (a.groups == 0) return;
+  const uint32_t group = blockIdx.x * (uint32_t)(kThreads / kLanes) + threadIdx.x / kLanes;
+  const int l = threadIdx.x % kLanes;
+  uint32_t t, chunk;
+  const uint32_t tok = a.chunks.div(min(group, a.groups - 1), chunk);
+  const uint32_t b = a.div_n.div(tok, t);
+  const int kind = (int)chunk < a.q_chunks ? 0 : (int)chunk < a.q_chunks + a.k_chunks ? 1 : 2;  // q, k, v
+  const int h0 = ((int)chunk - (kind == 0 ? 0 : kind == 1 ? a.q_chunks : a.q_chunks + a.k_chunks)) * kHeads;
+  const int heads = group < a.groups ? (kind == 0 ? a.hq : a.pool.n_kv_heads) - h0 : 0;  // to store, at most kHeads
+  // v keeps its order of dims and is not turned
+  const HeadLane ld(l, kind == 2 ? 0 : a.rot, kInter);
+
+  const Heads<const uint16_t>& x_in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+  const uint16_t* src = x_in.row(b, t, h0);
+  Pairs x[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) x[i] = load_pairs<kInter, kVec>(src + (i < heads ? i : 0) * x_in.sh, ld);
+  const int start = a.starts[b];
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (ld.rotated) {
+    long long pos = a.positions ? a.positions[tok] : (long long)start + t;
+    if (pos < 0 || pos >= a.max_pos) {
+      if (a.status) atomicOr(a.status, kDevBadPosition);
+      pos = pos < 0 ? 0 : a.max_pos - 1;
+    }
+    const float* row = a.cos_sin + pos * a.rot + 4 * l;
+    c = *reinterpret_cast<const float4*>(row);
+    s = *reinterpret_cast<const float4*>(row + a.rot / 2);
+  }
+  const Turn turn = make_turn<kInter>(c, s, kNorm && kind < 2 ? (kind == 0 ? a.qw : a.kw) : nullptr, ld);
+
+  // where the token's first row lies: its heads are a page's rows apart
+  long long dst = -1;
+  if (kind != 0 && heads > 0) {
+    int count = a.n;
+    if (a.counts) {
+      count = a.counts[b];
+      if ((count < 0 || count > a.n) && a.status) atomicOr(a.status, kDevBadLength);
+    }
+    if ((int)t < count) {
+      const long long pos = (long long)start + t;
+      if (start < 0 || pos >= cap) {
+        if (a.status) atomicOr(a.status, kDevAppendOverflow);
+      } else {
+        dst = a.index.row((int)b, h0, (int)pos, a.status);
+      }
+    }
+  }
+  uint8_t* const codes_out = kind == 1 ? a.pool.k_codes : a.pool.v_codes;
+  float* const scales_out = kind == 1 ? a.pool.k_scales : a.pool.v_scales;
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    // all lanes of the warp take part in the sums, whatever their heads are
+    Pairs y = turn_head<D, kNorm>(x[i], turn, ld.rotated, a.eps);
+    if (kind == 2) y = x[i];
+    uint32_t w[4], codes[2];
+    pack_pairs<kInter>(y, w);
+    const float scale = quantise_row<kLanes, 4, FMT>(w, codes);
+    if (i >= heads) continue;
+    if (kind == 0) {
+      store_pairs<kInter, kVec>(a.qo.row(b, t, h0 + i), ld, w);
+    } else if (dst >= 0) {
+      const long long row = dst + ((long long)i << a.index.page_log2);
+      *reinterpret_cast<uint32_t*>(codes_out + row * D + ld.o0) = codes[0];
+      *reinterpret_cast<uint32_t*>(codes_out + row * D + ld.o1) = codes[1];
+      if (l == 0) scales_out[row] = scale;
+    }
+  }
+}
+
+template <int D, int FMT, bool kInter, bool kNorm, bool kVec, int kHeads>
+cudaError_t launch_heads(QkvArgs a, uint32_t tokens, cudaStream_t stream) {
+  a.q_chunks = (a.hq + kHeads - 1) / kHeads;
+  a.k_chunks = (a.pool.n_kv_heads + kHeads - 1) / kHeads;
+  const uint32_t chunks = a.q_chunks + 2 * a.k_chunks;
+  a.groups = tokens * chunks;
+  a.chunks = FastDiv(chunks);
+  const uint32_t per_block = kThreads / (D / 8);
+  const dim3 grid(a.groups ? (a.groups + per_block - 1) / per_block : 1);
+  void* args[] = {&a};
+  return launch_with_pdl(reinterpret_cast<const void*>(&kvq_append_qkv_kernel<D, FMT, kInter, kNorm, kVec, kHeads>),
+                         grid, dim3(kThreads), args, 0, stream);
+}
+
+// Heads per lane group, by the rule of qk_rope.cu.
+template <int D, int FMT, bool kInter, bool kNorm, bool kVec>
+cudaError_t launch(const QkvArgs& a, uint32_t tokens, cudaStream_t stream) {
+  const long long lanes = (long long)tokens * (a.hq + 2 * a.pool.n_kv_heads) * (D / 8);
+  return lanes / 4 >= (long long)device_sm_count() * 512
+             ? launch_heads<D, FMT, kInter, kNorm, kVec, 4>(a, tokens, stream)
+             : launch_heads<D, FMT, kInter, kNorm, kVec, 1>(a, tokens, stream);
+}
+
+template <int D, int FMT, bool kInter>
+cudaError_t launch(const QkvArgs& a, uint32_t tokens, bool vec, cudaStream_t st) {
+  if (a.qw)
+    return vec ? launch<D, FMT, kInter, true, true>(a, tokens, st) : launch<D, FMT, kInter, true, false>(a, tokens, st);
+  return vec ? launch<D, FMT, kInter, false, true>(a, tokens, st) : launch<D, FMT, kInter, false, false>(a, tokens, st);
+}
+
+template <int D, int FMT>
+cudaError_t launch(const QkvArgs& a, uint32_t tokens, bool inter, bool vec, cudaStream_t st) {
+  return inter ? launch<D, FMT, true>(a, tokens, vec, st) : launch<D, FMT, false>(a, tokens, vec, st);
+}
+
+}  // namespace
+
+}  // namespace lara
+
+using namespace lara;
+
+extern "C" int lara_kvq_append_qkv(const lara_kvq_pool* pool, const int32_t* block_table, int pages_per_seq,
+                                   const int32_t* starts, const int32_t* counts, int32_t* new_lens, const uint16_t* q,
+                                   long long q_sb, long long q_st, long long q_sh, const uint16_t* k, long long k_sb,
+                                   long long k_st, long long k_sh, const uint16_t* v, long long v_sb, long long v_st,
+                                   long long v_sh, uint16_t* q_out, long long qo_sb, long long qo_st, long long qo_sh,
+                                   int batch, int n_new, int n_q_heads, const int32_t* positions, const float* cos_sin,
+                                   int max_pos, int rot_dim, int interleaved, const uint16_t* q_weight,
+                                   const uint16_t* k_weight, float eps, void* workspace, void* stream) {
+  LARA_NVTX("lara_kvq_append_qkv");
+  QkvArgs a{};
+  if (const int rc = check_pool(pool, block_table, pages_per_seq, batch, &a.index)) return rc;
+  const int hkv = pool->n_kv_heads;
+  if (batch < 0 || n_new < 0 || n_q_heads < 1 || n_q_heads > 65535 || hkv > 65535 ||
+      (long long)batch * n_new > 0x7fffffffll / (n_q_heads + 2 * hkv))
+    return set_last_error(LARA_ERR_BAD_CFG, "bad geometry: batch, n_new >= 0, below 2^31 heads in all");
+  if (!q_weight != !k_weight) return set_last_error(LARA_ERR_BAD_CFG, "q_weight and k_weight go together");
+  if (cos_sin && (rot_dim < 8 || rot_dim > pool->head_dim || rot_dim % 8 || max_pos < 1))
+    return set_last_error(LARA_ERR_BAD_CFG, "rot_dim must be a multiple of 8 up to head_dim, max_pos >= 1");
+  if (!(eps >= 0.f)) return set_last_error(LARA_ERR_BAD_CFG, "eps must not be negative");
+  if (batch == 0) return LARA_OK;
+  if (!starts || (n_new > 0 && (!q || !k || !v || !q_out))) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
+  if (!aligned(q, 2) || !aligned(k, 2) || !aligned(v, 2) || !aligned(q_out, 2) || !aligned(starts, 4) ||
+      !aligned(counts, 4) || !aligned(new_lens, 4) || !aligned(positions, 4) || !aligned(cos_sin, 16) ||
+      !aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(workspace, 4))
+    return set_last_error(LARA_ERR_STREAM_DEST, "cos_sin and the weights must be 16-byte aligned");
+  if (overlap(new_lens, starts, 4 * (size_t)batch) || overlap(new_lens, counts, 4 * (size_t)batch))
+    return set_last_error(LARA_ERR_STREAM_DEST, "new_lens must not overlap starts or counts");
+  if (n_new == 0 && !new_lens) return LARA_OK;
+  const bool vec = vec_ok(q, q_sb, batch, q_st, n_new, q_sh, n_q_heads) && vec_ok(k, k_sb, batch, k_st, n_new, k_sh, hkv) &&
+                   vec_ok(v, v_sb, batch, v_st, n_new, v_sh, hkv) &&
+                   vec_ok(q_out, qo_sb, batch, qo_st, n_new, qo_sh, n_q_heads);
+  a.pool = *pool;
+  a.starts = starts;
+  a.counts = counts;
+  a.new_lens = new_lens;
+  a.q = {q, q_sb, q_st, q_sh};
+  a.k = {k, k_sb, k_st, k_sh};
+  a.v = {v, v_sb, v_st, v_sh};
+  a.qo = {q_out, qo_sb, qo_st, qo_sh};
+  a.batch = batch;
+  a.n = n_new;
+  a.hq = n_q_heads;
+  a.div_n = FastDiv((uint32_t)n_new);
+  a.positions = positions;
+  a.cos_sin = cos_sin;
+  a.max_pos = max_pos;
+  a.rot = cos_sin ? rot_dim : 0;
+  a.qw = q_weight;
+  a.kw = k_weight;
+  a.eps = eps;
+  a.status = static_cast<int*>(workspace);
+  const uint32_t tokens = (uint32_t)batch * (uint32_t)n_new;
+  const bool inter = interleaved || !cos_sin;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaErrorInvalidValue;
+#define LARA_CASE(d, f) \
+  if (pool->head_dim == d && pool->format == f) e = launch<d, f>(a, tokens, inter, vec, st);
+  LARA_CASE(128, LARA_KVQ_INT8) LARA_CASE(128, LARA_KVQ_FP8_E4M3)
+  LARA_CASE(64, LARA_KVQ_INT8) LARA_CASE(64, LARA_KVQ_FP8_E4M3)
+#undef LARA_CASE
+  if (e != cudaSuccess)
+    return set_last_error(LARA_ERR_CUDA, std::string("kvq_append_qkv launch: ") + cudaGetErrorString(e));
+  return LARA_OK;
+}

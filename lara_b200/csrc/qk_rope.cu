@@ -108,12 +108,6 @@ cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, bool vec, cudaStream_
   return vec ? launch<D, kInter, false, true>(a, tokens, stream) : launch<D, kInter, false, false>(a, tokens, stream);
 }
 
-// 16-byte accesses: the base and every stride that is taken (an extent of 1
-// takes none).
-bool vec_ok(const void* p, long long sb, int batch, long long st, int n, long long sh, int heads) {
-  return aligned(p, 16) && (((batch > 1 ? sb : 0) | (n > 1 ? st : 0) | (heads > 1 ? sh : 0)) & 7) == 0;
-}
-
 }  // namespace
 
 }  // namespace lara

@@ -13,10 +13,11 @@ step reads about half as much.  Two formats:
 
 A row with a NaN or an infinity reads back as NaN.
 
-``QuantPool`` holds the device buffers.  ``kvq_append``, ``kvq_read`` and
-``gqa_decode_kvq`` are the stateless calls (``include/lara_b200.h``: lengths,
-block tables and results stay on the device, nothing synchronises, and the calls
-can be captured in a CUDA graph); ``QuantKVCache`` adds the page allocator of
+``QuantPool`` holds the device buffers.  ``kvq_append``, ``kvq_append_qkv`` (with the
+q/k norm and rotation of :func:`lara_b200.ops.qk_norm_rope` in the same launch),
+``kvq_read`` and ``gqa_decode_kvq`` are the stateless calls (``include/lara_b200.h``:
+lengths, block tables and results stay on the device, nothing synchronises, and the
+calls can be captured in a CUDA graph); ``QuantKVCache`` adds the page allocator of
 :class:`lara_b200.paged.PagedKVCache`.  The FPGA keeps one bf16 sequence in BRAM
 (hw/rtl/mem/kv_cache_ram.sv); it has no quantised cache.
 """
@@ -29,7 +30,7 @@ import math
 import torch
 
 from ._native import LARA_KVQ_FP8_E4M3, LARA_KVQ_INT8, LaraKvqPool, lib
-from .ops import _BF16, _I32, _check_words, _launch, _ptr, _strided, new_workspace
+from .ops import _BF16, _I32, _check_words, _launch, _ptr, _rope_table_args, _strided, new_workspace
 from .paged import PagedKVCache
 
 _FORMATS = {torch.int8: LARA_KVQ_INT8, torch.float8_e4m3fn: LARA_KVQ_FP8_E4M3}
@@ -112,6 +113,46 @@ def kvq_append(pool: QuantPool, block_table, starts, k_new, v_new, *, counts=Non
             None if counts is None else _i32_ptr("counts", counts, B, index),
             None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
             k_new.data_ptr(), ks[0], ks[1], ks[2], v_new.data_ptr(), vs[0], vs[1], vs[2], B, n, _ptr(workspace))
+
+
+def kvq_append_qkv(pool: QuantPool, block_table, starts, q, k, v, *, positions=None, cos_sin=None, q_weight=None,
+                   k_weight=None, eps: float = 1e-5, interleaved: bool = True, counts=None, new_lens=None,
+                   workspace=None, out=None):
+    """A serving step's row work in one launch: q and k are normed and rotated, k and v quantised into the pool.
+
+    q ``[B, n, Hq, D]``, k and v ``[B, n, Hkv, D]`` (bf16, any strides over contiguous heads: views of one
+    projection output are taken as they are).  The words are those of :func:`lara_b200.ops.qk_norm_rope` followed
+    by :func:`kvq_append`, whose arguments these are; ``positions`` (int32 ``[B, n]``) default to
+    ``starts[b] + t``.  Returns the new q, ``[B, n, Hq, D]`` (``out``, which may be q itself).
+    """
+    index = pool.index
+    B, n, hq, d = q.shape
+    kv_shape = (B, n, pool.n_kv_heads, pool.head_dim)
+    q_shape = (B, n, hq, pool.head_dim)
+    qs = _strided("q", q, q_shape, index)
+    ks = _strided("k", k, kv_shape, index)
+    vs = _strided("v", v, kv_shape, index)
+    qo = torch.empty(q_shape, dtype=q.dtype, device=pool.device) if out is None else out
+    qos = _strided("out", qo, q_shape, index, written=True)
+    qw = kw = table = pos = None
+    max_pos = rot = 0
+    if q_weight is not None:
+        _strided("q_weight", q_weight, (d,), index)
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        _strided("k_weight", k_weight, (d,), index)
+        kw = k_weight.data_ptr()
+    if cos_sin is not None:
+        table, max_pos, rot = _rope_table_args(cos_sin, index)
+    if positions is not None:
+        pos = _i32_ptr("positions", positions, B * n, index)
+    _launch(lib.lara_kvq_append_qkv, index, pool._ref, *_table(block_table, B, index),
+            _i32_ptr("starts", starts, B, index), None if counts is None else _i32_ptr("counts", counts, B, index),
+            None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
+            q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+            qo.data_ptr(), qos[0], qos[1], qos[2], B, n, hq, pos, table, max_pos, rot, int(bool(interleaved)), qw, kw,
+            eps, _ptr(workspace))
+    return qo
 
 
 def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=None, out=None, workspace=None):
@@ -205,6 +246,23 @@ class QuantKVCache(PagedKVCache):
         kvq_append(self.pool, table, lens, k_new, v_new, new_lens=new_lens, workspace=self._status)
         self.lens.index_copy_(0, idx, new_lens)
         self._lens[slots] += n
+
+    def append_qkv(self, q, k, v, slots=None, *, cos_sin=None, q_weight=None, k_weight=None, eps: float = 1e-5,
+                   interleaved: bool = True):
+        """:func:`kvq_append_qkv` for the given slots, at positions that follow their cached tokens; returns q."""
+        slots = self._slots(slots)
+        n = int(k.shape[1])
+        shape = (len(slots), n, self.n_kv_heads, self.head_dim)
+        _strided("k", k, shape, self.pool.index)
+        _strided("v", v, shape, self.pool.index)
+        self.reserve(slots, n)
+        idx, table, lens = self._rows(slots)
+        new_lens = torch.empty_like(lens)
+        q = kvq_append_qkv(self.pool, table, lens, q, k, v, cos_sin=cos_sin, q_weight=q_weight, k_weight=k_weight,
+                           eps=eps, interleaved=interleaved, new_lens=new_lens, workspace=self._status)
+        self.lens.index_copy_(0, idx, new_lens)
+        self._lens[slots] += n
+        return q
 
     def decode(self, q, slots=None, scale=None):
         """q ``[n_seq, Hq, D]`` (bf16) -> o ``[n_seq, Hq, D]`` over each slot's cached tokens."""

@@ -168,6 +168,30 @@ def _norm_rope(q=P, hd=128, n=1, hq=8, hkv=2, pos=P, table=P, max_pos=16, rot=12
                                         kw, eps, None, None)
 
 
+def _append_qkv(pool, q=P, v=P, starts=P, new_lens=None, batch=1, n=1, hq=8, table=P, rot=128, qw=P, kw=P, eps=1e-5):
+    z = (0, 0, 0)
+    return _lib().lib.lara_kvq_append_qkv(ctypes.byref(pool), P, 4, starts, None, new_lens, q, *z, P, *z, v, *z, P, *z,
+                                          batch, n, hq, None, table, 16, rot, 1, qw, kw, eps, None, None)
+
+
+def test_append_qkv_refusals():
+    pool = _pool_struct()
+    assert _append_qkv(_pool_struct(head_dim=80)) == 0x22
+    assert _append_qkv(pool, rot=12) == 0x01
+    assert _append_qkv(pool, hq=0) == 0x01
+    assert _append_qkv(pool, n=-1) == 0x01
+    assert _append_qkv(pool, batch=1 << 20, n=1 << 10) == 0x01
+    assert _append_qkv(pool, kw=None) == 0x01
+    assert _append_qkv(pool, eps=-1.0) == 0x01
+    assert _append_qkv(pool, q=None) == 0x11
+    assert _append_qkv(pool, v=None) == 0x11
+    assert _append_qkv(pool, starts=None) == 0x11
+    assert _append_qkv(pool, new_lens=P) == 0x11
+    assert _append_qkv(pool, qw=ctypes.c_void_p(4104)) == 0x11
+    assert _append_qkv(pool, batch=0) == 0
+    assert _append_qkv(pool, n=0, q=None, v=None) == 0
+
+
 def test_norm_rope_refusals():
     assert _norm_rope(hd=96) == 0x22
     assert _norm_rope(hq=0) == 0x01
@@ -514,6 +538,76 @@ def test_read_into_a_cache_slice_and_odd_strides():
         assert torch.count_nonzero(k[b, :, n:]) == 0
 
 
+# ------------------------------------------------------------------ the two in one launch
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,rot", [(128, 128), (128, 64), (64, 64)])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("B,n,hq,hkv", [(3, 1, 8, 2), (2, 37, 5, 5), (40, 60, 16, 8)])
+def test_append_qkv_equals_the_two_calls(fmt, D, rot, interleaved, B, n, hq, hkv):
+    _need_gpu()
+    from lara_b200 import kvquant, ops
+
+    g = torch.Generator().manual_seed(B + n + D)
+    ps, cap = 16, 160
+    x = _rand_bf16(g, (B, n, hq + 2 * hkv, D))
+    x[0, 0, hq, 5] = math.inf  # a k row that reads back as NaN
+    x = x.to(DEV)
+    q, k, v = x[:, :, :hq], x[:, :, hq:hq + hkv], x[:, :, hq + hkv:]
+    starts = torch.randint(0, 90, (B,), generator=g).to(torch.int32)
+    counts = torch.randint(0, n + 1, (B,), generator=g).to(torch.int32)
+    counts[0] = n
+    table, pages = _table(g, [cap] * B, cap // ps, ps)
+    table, dstarts, dcounts = table.to(DEV), starts.to(DEV), counts.to(DEV)
+    w = _rand_bf16(g, (2, D), False).to(DEV)
+    tab = ops.rope_table(256, rot, device=DEV)
+    pos = dstarts[:, None] + torch.arange(n, dtype=torch.int32, device=DEV)
+    for norm, rope, odd in ((True, True, False), (True, False, False), (False, True, True), (False, False, False)):
+        kw = dict(q_weight=w[0] if norm else None, k_weight=w[1] if norm else None, cos_sin=tab if rope else None,
+                  interleaved=interleaved)
+        pools = [kvquant.QuantPool.empty(pages, ps, hkv, D, fmt, DEV) for _ in range(2)]
+        new = [torch.zeros(B, dtype=torch.int32, device=DEV) for _ in range(2)]
+        qq, kk, vv = q, k, v
+        if odd:
+            qq, kk, vv = (torch.nn.functional.pad(z, (1, 2))[..., 1:D + 1] for z in (q, k, v))
+        q2, k2 = ops.qk_norm_rope(q, k, positions=pos if rope else None, **kw) if norm or rope else (q, k)
+        kvquant.kvq_append(pools[0], table, dstarts, k2.transpose(1, 2), v.transpose(1, 2), counts=dcounts,
+                           new_lens=new[0])
+        st = ops.new_workspace(256, DEV)
+        q1 = kvquant.kvq_append_qkv(pools[1], table, dstarts, qq, kk, vv, counts=dcounts, new_lens=new[1],
+                                    positions=pos if norm else None, workspace=st, **kw)
+        assert ops.workspace_status(st) == 0
+        assert torch.equal(q1, q2) and torch.equal(new[0], new[1])
+        for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+            a, b = (getattr(p, name) for p in pools)
+            if a.dtype == torch.float32:
+                a, b = a.view(torch.int32), b.view(torch.int32)
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), name
+
+
+@pytest.mark.gpu
+def test_append_qkv_reports_what_it_drops():
+    _need_gpu()
+    from lara_b200 import kvquant, ops
+
+    pool = kvquant.QuantPool.empty(4, 16, 1, 64, "int8", DEV)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    table = i32([[0, 1], [2, 77]])
+    g = torch.Generator().manual_seed(2)
+    x = _rand_bf16(g, (2, 4, 3, 64)).to(DEV)
+    st, new = ops.new_workspace(256, DEV), i32([0, 0])
+    args = (x[:, :, :1], x[:, :, 1:2], x[:, :, 2:])
+    tab = ops.rope_table(30, 64, device=DEV)
+    kvquant.kvq_append_qkv(pool, table, i32([30, 14]), *args, cos_sin=tab, new_lens=new, workspace=st)
+    assert ops.workspace_status(st) == 0x4 | 0x8 | 0x10  # past the capacity, page 77, positions past the table
+    assert new.tolist() == [32, 18]
+    kvquant.kvq_append_qkv(pool, table, i32([3, 4]), *(z[:, :0] for z in args), cos_sin=tab, new_lens=new,
+                           workspace=st)
+    assert ops.workspace_status(st) == 0 and new.tolist() == [3, 4]
+    with pytest.raises(ValueError, match="shape"):
+        kvquant.kvq_append_qkv(pool, table, i32([3, 4]), args[0], args[1], args[0][:, :1])
+
+
 # ------------------------------------------------------------------ decode
 LENS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 65, 127, 128, 129, 300, 777]
 
@@ -842,3 +936,26 @@ class SharedRows(Case):
         self.pool = kvquant.QuantPool(pools[0][0], pools[1][0], pools[0][1], pools[1][1])
         self.dtable = self.table.to(DEV)
         self.dlens = torch.tensor(self.lens, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,bound", [("int8", 0.02), ("fp8_e4m3", 0.08)])
+def test_example_runs_them_together(fmt, bound):
+    """``examples/quantised_cache.py``: prompts, then steps from a CUDA graph.
+
+    The bounds are the formats' own errors: int8 rounds to 1/254 of a row's largest value (about 3 of a normal
+    row's deviations), 0.7 % of a value's deviation in K and V; e4m3 to 2^-4, 2.6 % on average; each counts in the
+    weights and in the values, with a factor of two for the worst sequence and a little for bf16.
+    """
+    _need_gpu()
+    import importlib.util
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location(
+        "quantised_cache", Path(__file__).resolve().parents[1] / "examples" / "quantised_cache.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    r = mod.run(fmt=fmt, batch=5, prompt=200, steps=7)
+    assert r["status"] == 0
+    assert r["lens"] == r["expected_lens"]
+    assert r["relative_error"] < bound
