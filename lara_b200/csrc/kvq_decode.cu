@@ -73,7 +73,7 @@ constexpr float kStart = 7.f, kHigh = 15.f;
 
 template <int D, int NG>
 struct Cfg {
-  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr int kStages = 2;
   static constexpr int kCtasPerSm = D == 128 ? (NG == 1 ? 3 : 2) : (NG == 1 ? 4 : 3);
   static constexpr int kRowsBytes = kTile * D;                     // K (or V) codes of a stage
   static constexpr int kStageBytes = 2 * kRowsBytes + 2 * kTile * 4;

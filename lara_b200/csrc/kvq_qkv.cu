@@ -5,8 +5,10 @@
 // two, and k does not go to memory as bf16 in between), by HBM for prompts:
 // q 4 D bytes per head, k and v 2 D + D + 4.  Heads are held, normed and
 // rotated as in qk_rope.cu; k is rounded to bf16 and quantised from there, so
-// the pool gets the words of the two calls.  A lane group takes kHeads heads of
-// one token, all of q, all of k or all of v.
+// the pool gets the words of the two calls.  A block takes q, k or v alone, a
+// lane group kHeads heads of one token.
+#include <algorithm>
+
 #include "kvq.cuh"
 
 namespace lara {
@@ -25,9 +27,9 @@ struct QkvArgs {
   int32_t* new_lens;
   Heads<const uint16_t> q, k, v;
   Heads<uint16_t> qo;
-  int batch, n, hq, q_chunks, k_chunks;
-  uint32_t groups;  // tokens * chunks
-  FastDiv chunks, div_n;
+  int batch, n, hq;
+  uint32_t tokens, blocks[2];  // blocks of q, of k (and of v)
+  FastDiv chunks[2], div_n;    // chunks of heads per token: of q, of k and v
   const int32_t* positions;
   const float* cos_sin;
   int max_pos, rot;
@@ -49,40 +51,56 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
       const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
       a.new_lens[b] = start < 0 ? start : (int)min(end, max(cap, (long long)start));
     }
-  if (a.groups == 0) return;
-  const uint32_t group = blockIdx.x * (uint32_t)(kThreads / kLanes) + threadIdx.x / kLanes;
+  if (a.tokens == 0) return;
+  const uint32_t x = blockIdx.x;
+  const int kind = x < a.blocks[0] ? 0 : x < a.blocks[0] + a.blocks[1] ? 1 : 2;  // q, k, v
+  const uint32_t block = x - (kind == 0 ? 0 : a.blocks[0] + (kind == 1 ? 0 : a.blocks[1]));
+  const FastDiv& chunks = a.chunks[kind == 0 ? 0 : 1];
+  const uint32_t group = block * (uint32_t)(kThreads / kLanes) + threadIdx.x / kLanes;
   const int l = threadIdx.x % kLanes;
+  const bool active = group < a.tokens * chunks.d;
   uint32_t t, chunk;
-  const uint32_t tok = a.chunks.div(min(group, a.groups - 1), chunk);
+  const uint32_t tok = chunks.div(active ? group : 0, chunk);
   const uint32_t b = a.div_n.div(tok, t);
-  const int kind = (int)chunk < a.q_chunks ? 0 : (int)chunk < a.q_chunks + a.k_chunks ? 1 : 2;  // q, k, v
-  const int h0 = ((int)chunk - (kind == 0 ? 0 : kind == 1 ? a.q_chunks : a.q_chunks + a.k_chunks)) * kHeads;
-  const int heads = group < a.groups ? (kind == 0 ? a.hq : a.pool.n_kv_heads) - h0 : 0;  // to store, at most kHeads
-  // v keeps its order of dims and is not turned
-  const HeadLane ld(l, kind == 2 ? 0 : a.rot, kInter);
+  const int h0 = (int)chunk * kHeads;
+  const int heads = active ? (kind == 0 ? a.hq : a.pool.n_kv_heads) - h0 : 0;  // to store, at most kHeads
+  const HeadLane ld(l, kind == 2 ? 0 : a.rot, kInter);  // v is not turned
 
-  const Heads<const uint16_t>& x_in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-  const uint16_t* src = x_in.row(b, t, h0);
-  Pairs x[kHeads];
+  const Heads<const uint16_t>& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+  const uint16_t* src = in.row(b, t, h0);
+  Pairs y[kHeads];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) x[i] = load_pairs<kInter, kVec>(src + (i < heads ? i : 0) * x_in.sh, ld);
+  for (int i = 0; i < kHeads; ++i) y[i] = load_pairs<kInter, kVec>(src + (i < heads ? i : 0) * in.sh, ld);
   const int start = a.starts[b];
-  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (ld.rotated) {
-    long long pos = a.positions ? a.positions[tok] : (long long)start + t;
-    if (pos < 0 || pos >= a.max_pos) {
-      if (a.status) atomicOr(a.status, kDevBadPosition);
-      pos = pos < 0 ? 0 : a.max_pos - 1;
+  if (kind != 2) {
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (ld.rotated) {
+      long long pos = a.positions ? a.positions[tok] : (long long)start + t;
+      if (pos < 0 || pos >= a.max_pos) {
+        if (a.status) atomicOr(a.status, kDevBadPosition);
+        pos = pos < 0 ? 0 : a.max_pos - 1;
+      }
+      const float* row = a.cos_sin + pos * a.rot + 4 * l;
+      c = *reinterpret_cast<const float4*>(row);
+      s = *reinterpret_cast<const float4*>(row + a.rot / 2);
     }
-    const float* row = a.cos_sin + pos * a.rot + 4 * l;
-    c = *reinterpret_cast<const float4*>(row);
-    s = *reinterpret_cast<const float4*>(row + a.rot / 2);
+    const Turn turn = make_turn<kInter>(c, s, kNorm ? (kind == 0 ? a.qw : a.kw) : nullptr, ld);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) y[i] = turn_head<D, kNorm>(y[i], turn, ld.rotated, a.eps);
   }
-  const Turn turn = make_turn<kInter>(c, s, kNorm && kind < 2 ? (kind == 0 ? a.qw : a.kw) : nullptr, ld);
-
+  if (kind == 0) {
+    uint16_t* dst = a.qo.row(b, t, h0);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      uint32_t w[4];
+      pack_pairs<kInter>(y[i], w);
+      if (i < heads) store_pairs<kInter, kVec>(dst + i * a.qo.sh, ld, w);
+    }
+    return;
+  }
   // where the token's first row lies: its heads are a page's rows apart
   long long dst = -1;
-  if (kind != 0 && heads > 0) {
+  if (heads > 0) {
     int count = a.n;
     if (a.counts) {
       count = a.counts[b];
@@ -101,16 +119,10 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
   float* const scales_out = kind == 1 ? a.pool.k_scales : a.pool.v_scales;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    // all lanes of the warp take part in the sums, whatever their heads are
-    Pairs y = turn_head<D, kNorm>(x[i], turn, ld.rotated, a.eps);
-    if (kind == 2) y = x[i];
     uint32_t w[4], codes[2];
-    pack_pairs<kInter>(y, w);
+    pack_pairs<kInter>(y[i], w);
     const float scale = quantise_row<kLanes, 4, FMT>(w, codes);
-    if (i >= heads) continue;
-    if (kind == 0) {
-      store_pairs<kInter, kVec>(a.qo.row(b, t, h0 + i), ld, w);
-    } else if (dst >= 0) {
+    if (i < heads && dst >= 0) {
       const long long row = dst + ((long long)i << a.index.page_log2);
       *reinterpret_cast<uint32_t*>(codes_out + row * D + ld.o0) = codes[0];
       *reinterpret_cast<uint32_t*>(codes_out + row * D + ld.o1) = codes[1];
@@ -121,25 +133,29 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
 
 template <int D, int FMT, bool kInter, bool kNorm, bool kVec, int kHeads>
 cudaError_t launch_heads(QkvArgs a, uint32_t tokens, cudaStream_t stream) {
-  a.q_chunks = (a.hq + kHeads - 1) / kHeads;
-  a.k_chunks = (a.pool.n_kv_heads + kHeads - 1) / kHeads;
-  const uint32_t chunks = a.q_chunks + 2 * a.k_chunks;
-  a.groups = tokens * chunks;
-  a.chunks = FastDiv(chunks);
   const uint32_t per_block = kThreads / (D / 8);
-  const dim3 grid(a.groups ? (a.groups + per_block - 1) / per_block : 1);
+  const int heads[2] = {a.hq, a.pool.n_kv_heads};
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t chunks = (heads[i] + kHeads - 1) / kHeads;
+    a.chunks[i] = FastDiv(chunks);
+    a.blocks[i] = (tokens * chunks + per_block - 1) / per_block;
+  }
+  a.tokens = tokens;
+  const dim3 grid(std::max(1u, a.blocks[0] + 2 * a.blocks[1]));  // no tokens: new_lens alone
   void* args[] = {&a};
   return launch_with_pdl(reinterpret_cast<const void*>(&kvq_append_qkv_kernel<D, FMT, kInter, kNorm, kVec, kHeads>),
                          grid, dim3(kThreads), args, 0, stream);
 }
 
-// Heads per lane group, by the rule of qk_rope.cu.
+// Heads per lane group, on the grounds of qk_rope.cu.  32 + 8 + 8 heads
+// (head_dim 128, int8) of 64 single tokens take 2.8 us (four each: 3.0; the two
+// calls: 4.2), of 500 tokens 4.3 us with four (one each: 5.4; the two calls: 5.4), of 8192
+// tokens 41 us (eight each: 47; the two calls: 39, so a long prompt gains nothing).
 template <int D, int FMT, bool kInter, bool kNorm, bool kVec>
 cudaError_t launch(const QkvArgs& a, uint32_t tokens, cudaStream_t stream) {
-  const long long lanes = (long long)tokens * (a.hq + 2 * a.pool.n_kv_heads) * (D / 8);
-  return lanes / 4 >= (long long)device_sm_count() * 512
-             ? launch_heads<D, FMT, kInter, kNorm, kVec, 4>(a, tokens, stream)
-             : launch_heads<D, FMT, kInter, kNorm, kVec, 1>(a, tokens, stream);
+  const double fill = (double)tokens * (a.hq + 2 * a.pool.n_kv_heads) * (D / 8) / (device_sm_count() * 2048.0);
+  return fill < 0.6 ? launch_heads<D, FMT, kInter, kNorm, kVec, 1>(a, tokens, stream)
+                    : launch_heads<D, FMT, kInter, kNorm, kVec, 4>(a, tokens, stream);
 }
 
 template <int D, int FMT, bool kInter>

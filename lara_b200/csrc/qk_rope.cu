@@ -92,14 +92,19 @@ cudaError_t launch_heads(NormRopeArgs a, uint32_t tokens, cudaStream_t stream) {
                          dim3(kThreads), args, 0, stream);
 }
 
-// Heads per lane group: 8 keeps eight loads in flight and shares a token's
-// turn; with fewer lane groups than the SMs hold, one head each is quicker.
+// Heads per lane group.  More of them share a token's turn and keep more loads
+// in flight, fewer spread a small call over more lanes; what counts is how often
+// the call would fill the GPU's lanes with one head each.  72 heads (head_dim
+// 128) of 128, 256, 1024, 16384 tokens: one each 2.7, 4.1, 11.3, 165 us; two
+// 2.7, 2.9, 7.7, 130; four 2.9, 3.5, 6.3, 98; eight 3.0, 4.4, 6.8, 93 us (0.99
+// of the copy rate).
 template <int D, bool kInter, bool kNorm, bool kVec>
 cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, cudaStream_t stream) {
-  const long long lanes = (long long)tokens * (a.hq + a.hkv) * (D / 8);
-  return lanes / 8 >= (long long)device_sm_count() * 512
-             ? launch_heads<D, kInter, kNorm, kVec, 8>(a, tokens, stream)
-             : launch_heads<D, kInter, kNorm, kVec, 1>(a, tokens, stream);
+  const double fill = (double)tokens * (a.hq + a.hkv) * (D / 8) / (device_sm_count() * 2048.0);
+  if (fill < 0.5) return launch_heads<D, kInter, kNorm, kVec, 1>(a, tokens, stream);
+  if (fill < 1.5) return launch_heads<D, kInter, kNorm, kVec, 2>(a, tokens, stream);
+  if (fill < 7.0) return launch_heads<D, kInter, kNorm, kVec, 4>(a, tokens, stream);
+  return launch_heads<D, kInter, kNorm, kVec, 8>(a, tokens, stream);
 }
 
 template <int D, bool kInter>

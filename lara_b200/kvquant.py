@@ -29,8 +29,9 @@ import math
 
 import torch
 
-from ._native import LARA_KVQ_FP8_E4M3, LARA_KVQ_INT8, LaraKvqPool, lib
-from .ops import _BF16, _I32, _check_words, _launch, _ptr, _rope_table_args, _strided, new_workspace
+from ._native import LARA_KVQ_FP8_E4M3, LARA_KVQ_INT8, LaraKvqPool, check, lib
+from .ops import (_BF16, _I32, _check_words, _current_device, _ptr, _raw_stream, _rope_table_args, _strided,
+                  new_workspace)
 from .paged import PagedKVCache
 
 _FORMATS = {torch.int8: LARA_KVQ_INT8, torch.float8_e4m3fn: LARA_KVQ_FP8_E4M3}
@@ -109,10 +110,18 @@ def kvq_append(pool: QuantPool, block_table, starts, k_new, v_new, *, counts=Non
     shape = (B, pool.n_kv_heads, n, pool.head_dim)
     ks = _strided("k_new", k_new, shape, index)
     vs = _strided("v_new", v_new, shape, index)
-    _launch(lib.lara_kvq_append, index, pool._ref, *_table(block_table, B, index), _i32_ptr("starts", starts, B, index),
-            None if counts is None else _i32_ptr("counts", counts, B, index),
-            None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
-            k_new.data_ptr(), ks[0], ks[1], ks[2], v_new.data_ptr(), vs[0], vs[1], vs[2], B, n, _ptr(workspace))
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kvq_append(pool, block_table, starts, k_new, v_new, counts=counts, new_lens=new_lens,
+                              workspace=workspace)
+    table, pages = _table(block_table, B, index)
+    rc = lib.lara_kvq_append(pool._ref, table, pages, _i32_ptr("starts", starts, B, index),
+                             None if counts is None else _i32_ptr("counts", counts, B, index),
+                             None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
+                             k_new.data_ptr(), ks[0], ks[1], ks[2], v_new.data_ptr(), vs[0], vs[1], vs[2], B, n,
+                             _ptr(workspace), _raw_stream(index))
+    if rc:
+        check(rc, "lara_kvq_append")
 
 
 def kvq_append_qkv(pool: QuantPool, block_table, starts, q, k, v, *, positions=None, cos_sin=None, q_weight=None,
@@ -146,12 +155,21 @@ def kvq_append_qkv(pool: QuantPool, block_table, starts, q, k, v, *, positions=N
         table, max_pos, rot = _rope_table_args(cos_sin, index)
     if positions is not None:
         pos = _i32_ptr("positions", positions, B * n, index)
-    _launch(lib.lara_kvq_append_qkv, index, pool._ref, *_table(block_table, B, index),
-            _i32_ptr("starts", starts, B, index), None if counts is None else _i32_ptr("counts", counts, B, index),
-            None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
-            q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-            qo.data_ptr(), qos[0], qos[1], qos[2], B, n, hq, pos, table, max_pos, rot, int(bool(interleaved)), qw, kw,
-            eps, _ptr(workspace))
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kvq_append_qkv(pool, block_table, starts, q, k, v, positions=positions, cos_sin=cos_sin,
+                                  q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
+                                  counts=counts, new_lens=new_lens, workspace=workspace, out=qo)
+    blocks, pages = _table(block_table, B, index)
+    rc = lib.lara_kvq_append_qkv(pool._ref, blocks, pages, _i32_ptr("starts", starts, B, index),
+                                 None if counts is None else _i32_ptr("counts", counts, B, index),
+                                 None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
+                                 q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(),
+                                 vs[0], vs[1], vs[2], qo.data_ptr(), qos[0], qos[1], qos[2], B, n, hq, pos, table,
+                                 max_pos, rot, 1 if interleaved else 0, qw, kw, eps, _ptr(workspace),
+                                 _raw_stream(index))
+    if rc:
+        check(rc, "lara_kvq_append_qkv")
     return qo
 
 
@@ -170,10 +188,16 @@ def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=No
         k, v = out
     ks = _strided("k out", k, shape, index, written=True)
     vs = _strided("v out", v, shape, index, written=True)
-    _launch(lib.lara_kvq_read, index, pool._ref, *_table(block_table, B, index),
-            _i32_ptr("seq_lens", seq_lens, B, index),
-            None if starts is None else _i32_ptr("starts", starts, B, index),
-            k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], B, n, _ptr(workspace))
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kvq_read(pool, block_table, seq_lens, n, starts=starts, out=(k, v), workspace=workspace)
+    table, pages = _table(block_table, B, index)
+    rc = lib.lara_kvq_read(pool._ref, table, pages, _i32_ptr("seq_lens", seq_lens, B, index),
+                           None if starts is None else _i32_ptr("starts", starts, B, index),
+                           k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], B, n,
+                           _ptr(workspace), _raw_stream(index))
+    if rc:
+        check(rc, "lara_kvq_read")
     return k, v
 
 
@@ -207,9 +231,15 @@ def gqa_decode_kvq(q, pool: QuantPool, block_table, seq_lens, *, scale=None, wor
             raise ValueError("out must be contiguous")
     if workspace is None:
         workspace = decode_workspace(max(B, 1), hq, pool.n_kv_heads, d, pool.device)
-    _launch(lib.lara_gqa_decode_kvq, index, q.data_ptr(), pool._ref, *_table(block_table, B, index),
-            _i32_ptr("seq_lens", seq_lens, B, index), out.data_ptr(), B, hq,
-            1.0 / math.sqrt(d) if scale is None else float(scale), workspace.data_ptr(), workspace.numel())
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return gqa_decode_kvq(q, pool, block_table, seq_lens, scale=scale, workspace=workspace, out=out)
+    table, pages = _table(block_table, B, index)
+    rc = lib.lara_gqa_decode_kvq(q.data_ptr(), pool._ref, table, pages, _i32_ptr("seq_lens", seq_lens, B, index),
+                                 out.data_ptr(), B, hq, 1.0 / math.sqrt(d) if scale is None else scale,
+                                 workspace.data_ptr(), workspace.numel(), _raw_stream(index))
+    if rc:
+        check(rc, "lara_gqa_decode_kvq")
     return out
 
 

@@ -56,15 +56,9 @@ def _strided(name: str, t: torch.Tensor, shape: tuple, index: int, written: bool
     return st
 
 
-def _launch(fn, index: int, *args) -> None:
-    """Call a C entry point whose last argument is the stream, on CUDA device ``index`` and its current stream."""
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        check(rc, fn.__name__)
+# The current device and its stream as the numbers that the C calls take.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 @dataclass
@@ -381,9 +375,15 @@ def qk_norm_rope(q, k, *, positions=None, cos_sin=None, q_weight=None, k_weight=
                 or not positions.is_contiguous()):
             raise ValueError(f"positions must be a contiguous int32 tensor of shape {tuple(lead)} on the same device")
         pos = positions.data_ptr()
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return qk_norm_rope(q, k, positions=positions, cos_sin=cos_sin, q_weight=q_weight, k_weight=k_weight,
+                                eps=eps, interleaved=interleaved, workspace=workspace, out=(qo, ko))
     B, n = lead if len(lead) == 2 else (1, lead[0])
-    _launch(lib.lara_qk_norm_rope, index, q.data_ptr(), qs[0] if B > 1 else 0, qs[-3], qs[-2], k.data_ptr(),
-            ks[0] if B > 1 else 0, ks[-3], ks[-2], qo.data_ptr(), qos[0] if B > 1 else 0, qos[-3], qos[-2],
-            ko.data_ptr(), kos[0] if B > 1 else 0, kos[-3], kos[-2], B, n, hq, k_shape[-2], d, pos, table, max_pos,
-            rot, int(bool(interleaved)), qw, kw, eps, _ptr(workspace))
+    rc = lib.lara_qk_norm_rope(q.data_ptr(), qs[0], qs[-3], qs[-2], k.data_ptr(), ks[0], ks[-3], ks[-2],
+                               qo.data_ptr(), qos[0], qos[-3], qos[-2], ko.data_ptr(), kos[0], kos[-3], kos[-2], B, n,
+                               hq, k_shape[-2], d, pos, table, max_pos, rot, 1 if interleaved else 0, qw, kw, eps,
+                               _ptr(workspace), _raw_stream(index))
+    if rc:
+        check(rc, "lara_qk_norm_rope")
     return qo, ko
