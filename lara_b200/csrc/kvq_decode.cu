@@ -29,13 +29,23 @@
 //    below the largest one whatever the scales are.  R moves only when a weight
 //    would pass 2^15, and by whole powers of two, so most tiles rescale nothing.
 //
-// Work is split by the kernel itself: all (sequence, kv head) units are laid
-// end to end in tiles of 32 tokens, CTA c takes an equal share, and its warps
-// take tiles in turn, each through its own ring of cp.async stages (no barrier
-// per tile, no plan from the host, lengths stay on the device).  Warps join at
+// Work is split by the kernel itself, so that no plan from the host depends on
+// the lengths: all (sequence, kv head) units are laid end to end in tiles of 32
+// tokens, CTA c takes an equal share, and its warps take tiles in turn, each
+// through its own ring of cp.async stages (no barrier per tile).  Warps join at
 // the end of a unit; a unit that several CTAs share is joined by the last of
-// them to finish, in CTA order, so results do not depend on timing.  Short
-// units that fit the grid go to one CTA each, without that second join.
+// them to finish, in CTA order, so results do not depend on timing.  Short or
+// few units are shared out otherwise, see below.
+//
+// Measured (head_dim 128, 8 kv heads, int8 where not said): 64 sequences of
+// 4096 tokens 88 us, 0.96 of the copy rate of 6534 GB/s (e4m3 87 us; 64 query
+// heads 90 us; 128 query heads 110 us, e4m3 97 us, bound by the products' issue
+// and latency with eight warps per SM), of 8192 tokens 167 us (1.02); one of
+// 1,048,576 tokens 318 us (1.07: it only reads); one of 300 tokens 6.5 us.
+// About 10 us of a large call do not stream: 2 us until a CTA knows its share,
+// 3 us until its first rows arrive, and at the end CTAs finish over 10 us.
+// Two of three stages with two CTAs per SM, separate K and V slots (K fetched
+// two tiles ahead) and L2 prefetch hints were no faster.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -52,7 +62,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;          // tokens per warp and stage
-constexpr int kMinTiles = kWarps;    // tiles per CTA below which fewer CTAs run
+constexpr int kMinTiles = kWarps;  // tiles per CTA below which fewer CTAs run
 // Units up to this long are not split while each has a CTA: 8 units of 32 tiles
 // take 10.6 us, as long as split; of 19 tiles 8.1 against 12.9 us.
 constexpr int kWholeTiles = 32;
@@ -459,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       if (len_of(b) == 0)
         for (int i = threadIdx.x; i < a.n_q_heads * D / 8; i += kThreads)
           reinterpret_cast<uint4*>(a.o + (long long)b * a.n_q_heads * D)[i] = make_uint4(0, 0, 0, 0);
+  if (total == 0) return;
   // How the tiles are shared.  Short units, each with a CTA: one each.  Few
   // units: as many CTAs for a unit as it has tiles for, none with parts of two.
   // Short units, more than CTAs: whole ones to each warp (solo).  Else equal

@@ -892,7 +892,7 @@ def test_small_batches_and_empty_calls():
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("D,G", [(128, 4), (128, 12), (64, 8), (64, 16)])
-@pytest.mark.parametrize("B,hkv,n", [(150, 8, 100), (80, 8, 700), (7, 4, 3000)])
+@pytest.mark.parametrize("B,hkv,n", [(150, 8, 100), (80, 8, 700), (7, 4, 3000), (1300, 1, 60), (1300, 1, 900)])
 def test_decode_shares(fmt, D, G, B, hkv, n):
     """More (sequence, kv head) units than CTAs, short and long, and few long ones; ragged, some empty."""
     g = torch.Generator().manual_seed(B + D + G)
@@ -959,3 +959,16 @@ def test_example_runs_them_together(fmt, bound):
     assert r["status"] == 0
     assert r["lens"] == r["expected_lens"]
     assert r["relative_error"] < bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 5, 900])
+def test_decode_of_empty_sequences_alone(B):
+    case = SharedRows([1] * B, 1, 128, 16, "int8", torch.zeros((1, 1, 128)), torch.zeros((1, 1, 128)))
+    from lara_b200 import kvquant, ops
+
+    ws = kvquant.decode_workspace(B, 4, 1, 128, DEV)
+    q = torch.ones((B, 4, 128), dtype=torch.bfloat16, device=DEV)
+    out = torch.full_like(q, 3.0)
+    kvquant.gqa_decode_kvq(q, case.pool, case.dtable, torch.zeros_like(case.dlens), workspace=ws, out=out)
+    assert ops.workspace_status(ws) == 0 and torch.count_nonzero(out) == 0
