@@ -1,21 +1,26 @@
-"""Build liblara_b200.so in-tree with nvcc for sm_100a.
+"""Build liblara_b200.so in-tree with nvcc for sm_100a, and its Python binding.
 
 ``python -m lara_b200.build [--verbose]`` compiles every ``csrc/*.cu`` to an
 object with ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` and
 links them into ``lara_b200/liblara_b200.so`` (cudart linked statically, so
 the library does not depend on which ``libcudart`` a host process has
 loaded).  Objects go to ``lara_b200/_build``; a source newer than the library
-triggers a rebuild.
+triggers a rebuild.  ``csrc/binding.cpp``, the binding of the calls made once per
+layer and token, is compiled with g++ against the installed torch into
+``lara_b200/_binding.so`` (without torch it is left out: only the torch front end
+uses it).
 """
 
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -23,6 +28,7 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "liblara_b200.so"
+BINDING = PKG / "_binding.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -52,6 +58,31 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in sources() + headers() + [Path(__file__)])
 
 
+def _torch_include() -> Path | None:
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.origin).parent / "include" if spec and spec.origin else None
+
+
+def build_binding(force: bool = False) -> Path | None:
+    """Compile the Python binding; returns its path, or None without torch."""
+    src, inc = CSRC / "binding.cpp", _torch_include()
+    if inc is None:
+        return None
+    newest = max(p.stat().st_mtime for p in (src, INCLUDE / "lara_b200.h", Path(__file__)))
+    if not force and BINDING.exists() and BINDING.stat().st_mtime > newest:
+        return BINDING
+    cuda = Path(nvcc()).resolve().parents[1] / "include"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", "-I", str(inc), "-I",
+           str(inc / "torch" / "csrc" / "api" / "include"), "-I", sysconfig.get_paths()["include"], "-I", str(cuda)]
+    tmp = BINDING.with_suffix(".so.tmp")
+    libs = ["-L", str(inc.parent / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run([*cmd, str(src), "-o", str(tmp), *libs], capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def _compile(src: Path, verbose: bool) -> Path:
     obj = BUILD / (src.stem + ".o")
     cmd = [nvcc(), *ARCH_FLAGS, *COMMON_FLAGS, "-c", str(src), "-o", str(obj)]
@@ -66,7 +97,8 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile and link the library; returns its path."""
+    """Compile and link the library and its Python binding; returns the library's path."""
+    build_binding(force)
     if not force and not needs_build():
         return LIB
     BUILD.mkdir(exist_ok=True)

@@ -30,8 +30,7 @@ import math
 import torch
 
 from ._native import LARA_KVQ_FP8_E4M3, LARA_KVQ_INT8, LaraKvqPool, check, lib
-from .ops import (_BF16, _I32, _check_words, _current_device, _ptr, _raw_stream, _rope_table_args, _strided,
-                  new_workspace)
+from .ops import _binding, _check_words, _strided, new_workspace
 from .paged import PagedKVCache
 
 _FORMATS = {torch.int8: LARA_KVQ_INT8, torch.float8_e4m3fn: LARA_KVQ_FP8_E4M3}
@@ -68,7 +67,8 @@ class QuantPool:
         self.device, self.index = k_codes.device, k_codes.get_device()
         self._c = LaraKvqPool(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                               _FORMATS[k_codes.dtype], self.num_pages, self.n_kv_heads, self.page_size, self.head_dim)
-        self._ref = ctypes.byref(self._c)
+        self.address = ctypes.addressof(self._c)
+        self.scale = 1.0 / math.sqrt(self.head_dim)  # of the scores, where a call gives none
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, fmt: str = "int8",
@@ -81,21 +81,6 @@ class QuantPool:
         return cls(*codes, *scales)
 
 
-def _i32_ptr(name: str, t: torch.Tensor, n: int, index: int) -> int:
-    if t.dtype is not _I32 or t.get_device() != index or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of length {n} on the pool's device")
-    return t.data_ptr()
-
-
-def _table(table: torch.Tensor, batch: int, index: int) -> tuple:
-    if table.dtype is not _I32 or table.get_device() != index or table.dim() != 2 or not table.is_contiguous():
-        raise ValueError("block_table must be a contiguous int32 [batch, pages_per_seq] tensor on the pool's device")
-    rows, pages = table.shape
-    if rows != batch:
-        raise ValueError(f"block_table has {rows} rows for a batch of {batch}")
-    return table.data_ptr(), pages
-
-
 def kvq_append(pool: QuantPool, block_table, starts, k_new, v_new, *, counts=None, new_lens=None,
                workspace=None) -> None:
     """Quantise ``k_new``/``v_new[B, Hkv, n, D]`` (bf16, any strides over contiguous rows) into the pool.
@@ -105,21 +90,7 @@ def kvq_append(pool: QuantPool, block_table, starts, k_new, v_new, *, counts=Non
     tensor) receives ``starts + counts``.  ``workspace`` (``ops.new_workspace(256, device)``) collects
     the status bits of dropped rows (``ops.workspace_status``).
     """
-    index = pool.index
-    B, _, n, _ = k_new.shape
-    shape = (B, pool.n_kv_heads, n, pool.head_dim)
-    ks = _strided("k_new", k_new, shape, index)
-    vs = _strided("v_new", v_new, shape, index)
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return kvq_append(pool, block_table, starts, k_new, v_new, counts=counts, new_lens=new_lens,
-                              workspace=workspace)
-    table, pages = _table(block_table, B, index)
-    rc = lib.lara_kvq_append(pool._ref, table, pages, _i32_ptr("starts", starts, B, index),
-                             None if counts is None else _i32_ptr("counts", counts, B, index),
-                             None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
-                             k_new.data_ptr(), ks[0], ks[1], ks[2], v_new.data_ptr(), vs[0], vs[1], vs[2], B, n,
-                             _ptr(workspace), _raw_stream(index))
+    rc = _binding.append(pool.address, pool.index, block_table, starts, k_new, v_new, counts, new_lens, workspace)
     if rc:
         check(rc, "lara_kvq_append")
 
@@ -134,43 +105,13 @@ def kvq_append_qkv(pool: QuantPool, block_table, starts, q, k, v, *, positions=N
     by :func:`kvq_append`, whose arguments these are; ``positions`` (int32 ``[B, n]``) default to
     ``starts[b] + t``.  Returns the new q, ``[B, n, Hq, D]`` (``out``, which may be q itself).
     """
-    index = pool.index
-    B, n, hq, d = q.shape
-    kv_shape = (B, n, pool.n_kv_heads, pool.head_dim)
-    q_shape = (B, n, hq, pool.head_dim)
-    qs = _strided("q", q, q_shape, index)
-    ks = _strided("k", k, kv_shape, index)
-    vs = _strided("v", v, kv_shape, index)
-    qo = torch.empty(q_shape, dtype=q.dtype, device=pool.device) if out is None else out
-    qos = _strided("out", qo, q_shape, index, written=True)
-    qw = kw = table = pos = None
-    max_pos = rot = 0
-    if q_weight is not None:
-        _strided("q_weight", q_weight, (d,), index)
-        qw = q_weight.data_ptr()
-    if k_weight is not None:
-        _strided("k_weight", k_weight, (d,), index)
-        kw = k_weight.data_ptr()
-    if cos_sin is not None:
-        table, max_pos, rot = _rope_table_args(cos_sin, index)
-    if positions is not None:
-        pos = _i32_ptr("positions", positions, B * n, index)
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return kvq_append_qkv(pool, block_table, starts, q, k, v, positions=positions, cos_sin=cos_sin,
-                                  q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
-                                  counts=counts, new_lens=new_lens, workspace=workspace, out=qo)
-    blocks, pages = _table(block_table, B, index)
-    rc = lib.lara_kvq_append_qkv(pool._ref, blocks, pages, _i32_ptr("starts", starts, B, index),
-                                 None if counts is None else _i32_ptr("counts", counts, B, index),
-                                 None if new_lens is None else _i32_ptr("new_lens", new_lens, B, index),
-                                 q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(),
-                                 vs[0], vs[1], vs[2], qo.data_ptr(), qos[0], qos[1], qos[2], B, n, hq, pos, table,
-                                 max_pos, rot, 1 if interleaved else 0, qw, kw, eps, _ptr(workspace),
-                                 _raw_stream(index))
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    rc = _binding.append_qkv(pool.address, pool.index, block_table, starts, q, k, v, out, positions, cos_sin, q_weight,
+                             k_weight, eps, interleaved, counts, new_lens, workspace)
     if rc:
         check(rc, "lara_kvq_append_qkv")
-    return qo
+    return out
 
 
 def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=None, out=None, workspace=None):
@@ -179,23 +120,11 @@ def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=No
     ``starts=None`` reads from token 0.  Tokens at or past ``seq_lens[b]`` read as zeros.  ``out`` may be
     two strided views, e.g. ``cache[:, :, :n]`` of a bf16 cache for :func:`lara_b200.ops.gqa_prefill`.
     """
-    index = pool.index
-    B, n = seq_lens.numel(), int(n_tokens)
-    shape = (B, pool.n_kv_heads, n, pool.head_dim)
     if out is None:
-        k, v = (torch.empty(shape, dtype=_BF16, device=pool.device) for _ in range(2))
-    else:
-        k, v = out
-    ks = _strided("k out", k, shape, index, written=True)
-    vs = _strided("v out", v, shape, index, written=True)
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return kvq_read(pool, block_table, seq_lens, n, starts=starts, out=(k, v), workspace=workspace)
-    table, pages = _table(block_table, B, index)
-    rc = lib.lara_kvq_read(pool._ref, table, pages, _i32_ptr("seq_lens", seq_lens, B, index),
-                           None if starts is None else _i32_ptr("starts", starts, B, index),
-                           k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], B, n,
-                           _ptr(workspace), _raw_stream(index))
+        shape = (seq_lens.numel(), pool.n_kv_heads, n_tokens, pool.head_dim)
+        out = tuple(torch.empty(shape, dtype=torch.bfloat16, device=pool.device) for _ in range(2))
+    k, v = out
+    rc = _binding.read(pool.address, pool.index, block_table, seq_lens, n_tokens, starts, k, v, workspace)
     if rc:
         check(rc, "lara_kvq_read")
     return k, v
@@ -217,27 +146,13 @@ def gqa_decode_kvq(q, pool: QuantPool, block_table, seq_lens, *, scale=None, wor
     ``Hq`` is any multiple of the pool's kv heads up to 16 per kv head.  A sequence of length 0 gives
     zeros.  ``workspace`` comes from :func:`decode_workspace` (``None`` allocates one for the call).
     """
-    index = pool.index
-    B, hq, d = q.shape
-    shape = (B, hq, pool.head_dim)
-    _strided("q", q, shape, index)
-    if not q.is_contiguous():
-        raise ValueError("q must be contiguous")
     if out is None:
         out = torch.empty_like(q)
-    else:
-        _strided("out", out, shape, index)
-        if not out.is_contiguous():
-            raise ValueError("out must be contiguous")
     if workspace is None:
-        workspace = decode_workspace(max(B, 1), hq, pool.n_kv_heads, d, pool.device)
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return gqa_decode_kvq(q, pool, block_table, seq_lens, scale=scale, workspace=workspace, out=out)
-    table, pages = _table(block_table, B, index)
-    rc = lib.lara_gqa_decode_kvq(q.data_ptr(), pool._ref, table, pages, _i32_ptr("seq_lens", seq_lens, B, index),
-                                 out.data_ptr(), B, hq, 1.0 / math.sqrt(d) if scale is None else scale,
-                                 workspace.data_ptr(), workspace.numel(), _raw_stream(index))
+        workspace = decode_workspace(max(q.shape[0], 1), q.shape[1], pool.n_kv_heads, pool.head_dim, pool.device)
+    if scale is None:
+        scale = pool.scale
+    rc = _binding.decode(pool.address, pool.index, q, block_table, seq_lens, out, scale, workspace)
     if rc:
         check(rc, "lara_gqa_decode_kvq")
     return out

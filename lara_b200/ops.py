@@ -15,6 +15,15 @@ import torch
 
 from ._native import check, lib
 
+try:
+    from . import _binding
+except ImportError as e:
+    raise ImportError(f"lara_b200/_binding.so cannot be loaded ({e}); run `python -m lara_b200.build`") from e
+
+_binding.init(*(ctypes.cast(f, ctypes.c_void_p).value
+                for f in (lib.lara_qk_norm_rope, lib.lara_kvq_append, lib.lara_kvq_append_qkv, lib.lara_kvq_read,
+                          lib.lara_gqa_decode_kvq)))
+
 _WORD_DTYPES = (torch.bfloat16, torch.int16, torch.uint16)
 
 
@@ -37,28 +46,16 @@ def _check_words(name: str, t: torch.Tensor, shape: tuple | None = None) -> None
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
-
-
-def _strided(name: str, t: torch.Tensor, shape: tuple, index: int, written: bool = False) -> tuple:
-    """Strides of a bf16 tensor of contiguous rows (last dim) on CUDA device ``index``, after checking it."""
-    if t.dtype is not _BF16 and t.dtype not in _WORD_DTYPES:
+def _strided(name: str, t: torch.Tensor, shape: tuple, index: int) -> None:
+    """Check a bf16 tensor of contiguous rows (last dim) on CUDA device ``index``."""
+    if t.dtype not in _WORD_DTYPES:
         raise TypeError(f"{name} must hold bf16 words (bfloat16/int16/uint16), got {t.dtype}")
     if t.get_device() != index or index < 0:
         raise ValueError(f"{name} must be on the CUDA device of the call, got {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    st = t.stride()
-    if st[-1] != 1:
+    if t.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    if written and 0 in st and any(s == 0 and n > 1 for s, n in zip(st, shape)):
-        raise ValueError(f"{name} is written and must not repeat elements (a stride of 0)")
-    return st
-
-
-# The current device and its stream as the numbers that the C calls take.
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 @dataclass
@@ -328,13 +325,6 @@ def rope_table(max_pos: int, rot_dim: int, *, base: float = 10000.0, inv_freq=No
     return torch.cat([ang.cos(), ang.sin()], -1).float()
 
 
-def _rope_table_args(cos_sin: torch.Tensor, index: int) -> tuple:
-    if (cos_sin.dtype is not _F32 or cos_sin.get_device() != index or cos_sin.dim() != 2
-            or not cos_sin.is_contiguous()):
-        raise ValueError("cos_sin must be a contiguous float32 [max_pos, rot_dim] tensor on the same device")
-    return cos_sin.data_ptr(), *cos_sin.shape
-
-
 def qk_norm_rope(q, k, *, positions=None, cos_sin=None, q_weight=None, k_weight=None, eps: float = 1e-5,
                  interleaved: bool = True, workspace=None, out=None):
     """RMS norm of every query and key head and the position rotation, in one pass (``lara_qk_norm_rope``).
@@ -348,42 +338,10 @@ def qk_norm_rope(q, k, *, positions=None, cos_sin=None, q_weight=None, k_weight=
     (q, k) in new contiguous tensors, or in ``out``, which may be the inputs.  ``workspace`` collects the
     status bit of a position outside the table (its nearest row is taken).
     """
-    shape = q.shape
-    if len(shape) not in (3, 4) or k.dim() != len(shape):
-        raise ValueError("q and k must be [T, H, D] or [B, n, H, D]")
-    index = q.get_device()
-    *lead, hq, d = shape
-    k_shape = (*lead, k.shape[-2], d)
-    qs = _strided("q", q, shape, index)
-    ks = _strided("k", k, k_shape, index)
-    qo, ko = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)) if out is None else out
-    qos = _strided("q out", qo, shape, index, written=True)
-    kos = _strided("k out", ko, k_shape, index, written=True)
-    qw = kw = table = pos = None
-    max_pos = rot = 0
-    if q_weight is not None:
-        _strided("q_weight", q_weight, (d,), index)
-        qw = q_weight.data_ptr()
-    if k_weight is not None:
-        _strided("k_weight", k_weight, (d,), index)
-        kw = k_weight.data_ptr()
-    if cos_sin is not None:
-        table, max_pos, rot = _rope_table_args(cos_sin, index)
-        if positions is None:
-            raise ValueError("a rotation needs positions")
-        if (positions.dtype is not _I32 or positions.get_device() != index or positions.shape != shape[:-2]
-                or not positions.is_contiguous()):
-            raise ValueError(f"positions must be a contiguous int32 tensor of shape {tuple(lead)} on the same device")
-        pos = positions.data_ptr()
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return qk_norm_rope(q, k, positions=positions, cos_sin=cos_sin, q_weight=q_weight, k_weight=k_weight,
-                                eps=eps, interleaved=interleaved, workspace=workspace, out=(qo, ko))
-    B, n = lead if len(lead) == 2 else (1, lead[0])
-    rc = lib.lara_qk_norm_rope(q.data_ptr(), qs[0], qs[-3], qs[-2], k.data_ptr(), ks[0], ks[-3], ks[-2],
-                               qo.data_ptr(), qos[0], qos[-3], qos[-2], ko.data_ptr(), kos[0], kos[-3], kos[-2], B, n,
-                               hq, k_shape[-2], d, pos, table, max_pos, rot, 1 if interleaved else 0, qw, kw, eps,
-                               _ptr(workspace), _raw_stream(index))
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo, ko = out
+    rc = _binding.norm_rope(q, k, qo, ko, positions, cos_sin, q_weight, k_weight, eps, interleaved, workspace)
     if rc:
         check(rc, "lara_qk_norm_rope")
     return qo, ko
