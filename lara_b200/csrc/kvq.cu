@@ -103,10 +103,7 @@ enum Access { kElement, kHalf, kFull };
 template <Access kA>
 __device__ __forceinline__ void load16(const uint16_t* p, uint32_t w[8]) {
   if constexpr (kA == kFull) {
-    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                 : "l"(p)
-                 : "memory");
+    load32(p, w);
   } else if constexpr (kA == kHalf) {
     *reinterpret_cast<uint4*>(w) = __ldcs(reinterpret_cast<const uint4*>(p));
     *reinterpret_cast<uint4*>(w + 4) = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
@@ -118,9 +115,7 @@ __device__ __forceinline__ void load16(const uint16_t* p, uint32_t w[8]) {
 template <Access kA>
 __device__ __forceinline__ void store16(uint16_t* p, const uint32_t w[8]) {
   if constexpr (kA == kFull) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
+    store32(p, w);
   } else if constexpr (kA == kHalf) {
     reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
     reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
@@ -219,12 +214,9 @@ __global__ void __launch_bounds__(kThreads) kvq_read_kernel(const __grid_constan
   }
 }
 
-// The widest access that the base and every stride allow (an extent of 1 takes
-// no stride).
 Access access_of(const void* p, long long sb, int batch, long long sh, int heads, long long st, int n) {
-  const long long bytes = 2 * ((batch > 1 ? sb : 0) | (heads > 1 ? sh : 0) | (n > 1 ? st : 0)) |
-                          (long long)reinterpret_cast<uintptr_t>(p);
-  return (bytes & 31) == 0 ? kFull : (bytes & 15) == 0 ? kHalf : kElement;
+  const int bytes = row_alignment(p, sb, batch, st, n, sh, heads);
+  return bytes >= 32 ? kFull : bytes >= 16 ? kHalf : kElement;
 }
 
 // Whether the rows of a call (at least one per warp) fit one launch.

@@ -1,8 +1,7 @@
 // Rows of the 8-bit KV pool and of the q/k head pass (sm_100a).
 //
-// A row is the D values of one (token, head).  D / 8 lanes hold it, eight
-// values each (D / 16 and sixteen where the pool is written or read), and
-// reduce over it with shuffles.
+// A row is the D values of one (token, head).  D / 16 lanes hold it, sixteen
+// values each, and reduce over it with shuffles.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -74,85 +73,109 @@ struct FastDiv {
   }
 };
 
-// How the q/k pass holds a head: D / 8 lanes, eight dims each, kept as four
-// rotation pairs: a[j] and b[j] make pair 4 * lane + j of the table.  Pairs
-// (2i, 2i+1) lie side by side in memory; pairs (i, i + rot/2) meet in one lane
-// because the first rot/8 lanes take four dims of each half, so the rotation
-// needs no exchange.  Lanes past rot hold eight dims in a row and do not rotate.
+// A lane's 32 bytes in one access.
+__device__ __forceinline__ void load32(const void* p, uint32_t w[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t w[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// How the q/k pass holds a head: D / 2W lanes, 2W dims each (W = 8, or 4 where
+// rot or the addresses are not so divisible), kept as W rotation pairs: a[j]
+// and b[j] make pair W * lane + j of the table.  Pairs (2i, 2i+1) lie side by
+// side in memory; pairs (i, i + rot/2) meet in one lane because the first
+// rot / 2W lanes take W dims of each half, so the rotation needs no exchange.
+// Lanes past rot hold 2W dims in a row and do not rotate.
+template <int W>
 struct HeadLane {
-  int o0, o1;      // the lane's two runs of four dims
+  int o0, o1;      // the lane's two runs of W dims
   bool rotated;
   __device__ __forceinline__ HeadLane(int lane, int rot, bool interleaved) {
-    rotated = 8 * lane < rot;
+    rotated = 2 * W * lane < rot;
     const bool split = rotated && !interleaved;
-    o0 = split ? 4 * lane : 8 * lane;
-    o1 = split ? rot / 2 + 4 * lane : 8 * lane + 4;
+    o0 = split ? W * lane : 2 * W * lane;
+    o1 = split ? rot / 2 + W * lane : 2 * W * lane + W;
   }
 };
 
-// The lane's eight values as pairs: a = (x_a of pairs 0, 1), (2, 3); b alike.
+// The lane's values: a[i] = (x_a of pairs 2i, 2i + 1), b alike.
+template <int W>
 struct Pairs {
-  float2 a[2], b[2];
+  float2 a[W / 2], b[W / 2];
 };
 
-template <bool kInter, bool kVec>
-__device__ __forceinline__ Pairs load_pairs(const uint16_t* row, const HeadLane& ld) {
-  uint32_t w[4];
-  if constexpr (kVec && kInter) {
+// The lane's 2W values as words in memory order: run o0, then run o1.
+template <int W, bool kInter, bool kVec>
+__device__ __forceinline__ void load_words(const uint16_t* row, const HeadLane<W>& ld, uint32_t w[W]) {
+  if constexpr (kVec && kInter && W == 8) {
+    load32(row + ld.o0, w);
+  } else if constexpr (kVec && (kInter || W == 8)) {
     *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(row + ld.o0);
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(w + 4) = *reinterpret_cast<const uint4*>(row + ld.o1);
   } else if constexpr (kVec) {
     *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(row + ld.o0);
     *reinterpret_cast<uint2*>(w + 2) = *reinterpret_cast<const uint2*>(row + ld.o1);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint16_t* p = row + (j < 2 ? ld.o0 + 2 * j : ld.o1 + 2 * j - 4);
+    for (int j = 0; j < W; ++j) {
+      const uint16_t* p = row + (j < W / 2 ? ld.o0 + 2 * j : ld.o1 + 2 * j - W);
       w[j] = (uint32_t)p[0] | ((uint32_t)p[1] << 16);
     }
   }
-  Pairs x;
-  if constexpr (kInter) {
-    x.a[0] = make_float2(bf16lo(w[0]), bf16lo(w[1]));
-    x.b[0] = make_float2(bf16hi(w[0]), bf16hi(w[1]));
-    x.a[1] = make_float2(bf16lo(w[2]), bf16lo(w[3]));
-    x.b[1] = make_float2(bf16hi(w[2]), bf16hi(w[3]));
-  } else {
-    x.a[0] = make_float2(bf16lo(w[0]), bf16hi(w[0]));
-    x.a[1] = make_float2(bf16lo(w[1]), bf16hi(w[1]));
-    x.b[0] = make_float2(bf16lo(w[2]), bf16hi(w[2]));
-    x.b[1] = make_float2(bf16lo(w[3]), bf16hi(w[3]));
-  }
-  return x;
 }
 
-template <bool kInter>
-__device__ __forceinline__ void pack_pairs(const Pairs& x, uint32_t w[4]) {
-  if constexpr (kInter) {
-    w[0] = pack2_rn(x.a[0].x, x.b[0].x);
-    w[1] = pack2_rn(x.a[0].y, x.b[0].y);
-    w[2] = pack2_rn(x.a[1].x, x.b[1].x);
-    w[3] = pack2_rn(x.a[1].y, x.b[1].y);
-  } else {
-    w[0] = pack2_rn(x.a[0].x, x.a[0].y);
-    w[1] = pack2_rn(x.a[1].x, x.a[1].y);
-    w[2] = pack2_rn(x.b[0].x, x.b[0].y);
-    w[3] = pack2_rn(x.b[1].x, x.b[1].y);
-  }
-}
-
-template <bool kInter, bool kVec>
-__device__ __forceinline__ void store_pairs(uint16_t* row, const HeadLane& ld, const uint32_t w[4]) {
-  if constexpr (kVec && kInter) {
+template <int W, bool kInter, bool kVec>
+__device__ __forceinline__ void store_words(uint16_t* row, const HeadLane<W>& ld, const uint32_t w[W]) {
+  if constexpr (kVec && kInter && W == 8) {
+    store32(row + ld.o0, w);
+  } else if constexpr (kVec && (kInter || W == 8)) {
     *reinterpret_cast<uint4*>(row + ld.o0) = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(row + ld.o1) = make_uint4(w[4], w[5], w[6], w[7]);
   } else if constexpr (kVec) {
     *reinterpret_cast<uint2*>(row + ld.o0) = make_uint2(w[0], w[1]);
     *reinterpret_cast<uint2*>(row + ld.o1) = make_uint2(w[2], w[3]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint16_t* p = row + (j < 2 ? ld.o0 + 2 * j : ld.o1 + 2 * j - 4);
+    for (int j = 0; j < W; ++j) {
+      uint16_t* p = row + (j < W / 2 ? ld.o0 + 2 * j : ld.o1 + 2 * j - W);
       p[0] = (uint16_t)w[j];
       p[1] = (uint16_t)(w[j] >> 16);
+    }
+  }
+}
+
+template <int W, bool kInter>
+__device__ __forceinline__ Pairs<W> pairs_of(const uint32_t w[W]) {
+  Pairs<W> x;
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    if constexpr (kInter) {
+      x.a[i] = make_float2(bf16lo(w[2 * i]), bf16lo(w[2 * i + 1]));
+      x.b[i] = make_float2(bf16hi(w[2 * i]), bf16hi(w[2 * i + 1]));
+    } else {
+      x.a[i] = make_float2(bf16lo(w[i]), bf16hi(w[i]));
+      x.b[i] = make_float2(bf16lo(w[W / 2 + i]), bf16hi(w[W / 2 + i]));
+    }
+  }
+  return x;
+}
+
+template <int W, bool kInter>
+__device__ __forceinline__ void words_of(const Pairs<W>& x, uint32_t w[W]) {
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    if constexpr (kInter) {
+      w[2 * i] = pack2_rn(x.a[i].x, x.b[i].x);
+      w[2 * i + 1] = pack2_rn(x.a[i].y, x.b[i].y);
+    } else {
+      w[i] = pack2_rn(x.a[i].x, x.a[i].y);
+      w[W / 2 + i] = pack2_rn(x.b[i].x, x.b[i].y);
     }
   }
 }
@@ -160,65 +183,82 @@ __device__ __forceinline__ void store_pairs(uint16_t* row, const HeadLane& ld, c
 // What a token and a weight vector make of a pair, (a', b') = inv * (a ac - b bs,
 // a as + b bc): the weights are folded into the cosines and sines once per
 // token, so a head costs four products per pair and one with inv.
+template <int W>
 struct Turn {
-  float2 ac[2], bs[2], as[2], bc[2];  // bs holds -w_b s
+  float2 ac[W / 2], bs[W / 2], as[W / 2], bc[W / 2];  // bs holds -w_b s
 };
 
-template <bool kInter>
-__device__ __forceinline__ Turn make_turn(const float4& c, const float4& s, const uint16_t* weight,
-                                          const HeadLane& ld) {
-  Turn t;
-  const float2 c2[2] = {make_float2(c.x, c.y), make_float2(c.z, c.w)};
-  const float2 s2[2] = {make_float2(s.x, s.y), make_float2(s.z, s.w)};
-  const float2 m2[2] = {make_float2(-s.x, -s.y), make_float2(-s.z, -s.w)};
+// row: the token's row of the table (cosines, then sines), null for no rotation.
+template <int W, bool kInter>
+__device__ __forceinline__ Turn<W> make_turn(const float* row, int rot, int lane, const uint16_t* weight,
+                                             const HeadLane<W>& ld) {
+  Turn<W> t;
+  float c[W], s[W];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    t.ac[i] = t.bc[i] = c2[i];
-    t.as[i] = s2[i];
-    t.bs[i] = m2[i];
+  for (int i = 0; i < W; i += 4) {
+    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (ld.rotated) {
+      c4 = *reinterpret_cast<const float4*>(row + W * lane + i);
+      s4 = *reinterpret_cast<const float4*>(row + rot / 2 + W * lane + i);
+    }
+    *reinterpret_cast<float4*>(c + i) = c4;
+    *reinterpret_cast<float4*>(s + i) = s4;
+  }
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    t.ac[i] = t.bc[i] = make_float2(c[2 * i], c[2 * i + 1]);
+    t.as[i] = make_float2(s[2 * i], s[2 * i + 1]);
+    t.bs[i] = make_float2(-s[2 * i], -s[2 * i + 1]);
   }
   if (weight) {
-    const Pairs w = load_pairs<kInter, true>(weight, ld);
+    uint32_t w[W];
+    load_words<W, false, true>(weight, ld, w);
+    const Pairs<W> x = pairs_of<W, kInter>(w);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      t.ac[i] = mul2(t.ac[i], w.a[i]);
-      t.as[i] = mul2(t.as[i], w.a[i]);
-      t.bs[i] = mul2(t.bs[i], w.b[i]);
-      t.bc[i] = mul2(t.bc[i], w.b[i]);
+    for (int i = 0; i < W / 2; ++i) {
+      t.ac[i] = mul2(t.ac[i], x.a[i]);
+      t.as[i] = mul2(t.as[i], x.a[i]);
+      t.bs[i] = mul2(t.bs[i], x.b[i]);
+      t.bc[i] = mul2(t.bc[i], x.b[i]);
     }
   }
   return t;
 }
 
 // One head: the norm's factor (sum of squares in fp32) and the turn.  Every
-// step is a packed operation with its rounding, so all kernels that treat a
-// head give the same words.
-template <int D, bool kNorm>
-__device__ __forceinline__ Pairs turn_head(const Pairs& x, const Turn& t, bool rotated, float eps) {
-  Pairs y;
+// step is an operation with its rounding, and the sum a tree over runs of eight
+// dims, so every kernel and either W give the same words.
+template <int D, int W, bool kNorm>
+__device__ __forceinline__ Pairs<W> turn_head(const Pairs<W>& x, const Turn<W>& t, bool rotated, float eps) {
+  Pairs<W> y;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < W / 2; ++i) {
     y.a[i] = fma2(x.a[i], t.ac[i], mul2(x.b[i], t.bs[i]));
     y.b[i] = fma2(x.a[i], t.as[i], mul2(x.b[i], t.bc[i]));
   }
   if (!rotated)  // an infinity in one dim stays out of its neighbour's
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < W / 2; ++i) {
       y.a[i] = mul2(x.a[i], t.ac[i]);
       y.b[i] = mul2(x.b[i], t.bc[i]);
     }
   if constexpr (kNorm) {
-    float2 q = mul2(x.a[0], x.a[0]);
-    q = fma2(x.b[0], x.b[0], q);
-    q = fma2(x.a[1], x.a[1], q);
-    q = fma2(x.b[1], x.b[1], q);
-    float ss = __fadd_rn(q.x, q.y);
+    float part[W / 4];
 #pragma unroll
-    for (int off = D / 16; off > 0; off >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, off));
+    for (int j = 0; j < W / 4; ++j) {
+      float2 q = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 2 * j; i < 2 * j + 2; ++i) q = fma2(x.b[i], x.b[i], fma2(x.a[i], x.a[i], q));
+      part[j] = __fadd_rn(q.x, q.y);
+    }
+    float ss = part[0];
+    if constexpr (W == 8) ss = __fadd_rn(part[0], part[1]);
+#pragma unroll
+    for (int off = 1; off < D / (2 * W); off <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, off));
     const float inv = rsqrtf(__fmaf_rn(ss, 1.f / D, eps));
     const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < W / 2; ++i) {
       y.a[i] = mul2(y.a[i], inv2);
       y.b[i] = mul2(y.b[i], inv2);
     }
@@ -341,10 +381,12 @@ inline bool overlap(const void* a, const void* b, size_t bytes) {
   return a && b && x < y + bytes && y < x + bytes;
 }
 
-// 16-byte accesses: the base and every stride that is taken (an extent of 1
-// takes none).
-inline bool vec_ok(const void* p, long long sb, int batch, long long st, int n, long long sh, int heads) {
-  return aligned(p, 16) && (((batch > 1 ? sb : 0) | (n > 1 ? st : 0) | (heads > 1 ? sh : 0)) & 7) == 0;
+// The alignment in bytes, up to 32, of every row of a strided tensor (an extent
+// of 1 takes no stride).
+inline int row_alignment(const void* p, long long sb, int batch, long long st, int n, long long sh, int heads) {
+  const long long bytes = 2 * ((batch > 1 ? sb : 0) | (n > 1 ? st : 0) | (heads > 1 ? sh : 0)) |
+                          (long long)reinterpret_cast<uintptr_t>(p) | 32;
+  return (int)(bytes & -bytes);
 }
 
 }  // namespace kvq

@@ -39,9 +39,9 @@ struct QkvArgs {
   int* status;
 };
 
-template <int D, int FMT, bool kInter, bool kNorm, bool kVec, int kHeads>
+template <int D, int W, int FMT, bool kInter, bool kNorm, bool kVec, int kHeads>
 __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_constant__ QkvArgs a) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / (2 * W);
   allow_dependent_launch();
   grid_dependency_wait();
   const long long cap = a.index.capacity();
@@ -64,38 +64,34 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
   const uint32_t b = a.div_n.div(tok, t);
   const int h0 = (int)chunk * kHeads;
   const int heads = active ? (kind == 0 ? a.hq : a.pool.n_kv_heads) - h0 : 0;  // to store, at most kHeads
-  const HeadLane ld(l, kind == 2 ? 0 : a.rot, kInter);  // v is not turned
+  const HeadLane<W> ld(l, kind == 2 ? 0 : a.rot, kInter);  // v is not turned
 
   const Heads<const uint16_t>& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
   const uint16_t* src = in.row(b, t, h0);
-  Pairs y[kHeads];
+  uint32_t w[kHeads][W];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) y[i] = load_pairs<kInter, kVec>(src + (i < heads ? i : 0) * in.sh, ld);
+  for (int i = 0; i < kHeads; ++i) load_words<W, kInter, kVec>(src + (i < heads ? i : 0) * in.sh, ld, w[i]);
   const int start = a.starts[b];
   if (kind != 2) {
-    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* row = nullptr;
     if (ld.rotated) {
       long long pos = a.positions ? a.positions[tok] : (long long)start + t;
       if (pos < 0 || pos >= a.max_pos) {
         if (a.status) atomicOr(a.status, kDevBadPosition);
         pos = pos < 0 ? 0 : a.max_pos - 1;
       }
-      const float* row = a.cos_sin + pos * a.rot + 4 * l;
-      c = *reinterpret_cast<const float4*>(row);
-      s = *reinterpret_cast<const float4*>(row + a.rot / 2);
+      row = a.cos_sin + pos * a.rot;
     }
-    const Turn turn = make_turn<kInter>(c, s, kNorm ? (kind == 0 ? a.qw : a.kw) : nullptr, ld);
+    const Turn<W> turn = make_turn<W, kInter>(row, a.rot, l, kNorm ? (kind == 0 ? a.qw : a.kw) : nullptr, ld);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) y[i] = turn_head<D, kNorm>(y[i], turn, ld.rotated, a.eps);
+    for (int i = 0; i < kHeads; ++i)
+      words_of<W, kInter>(turn_head<D, W, kNorm>(pairs_of<W, kInter>(w[i]), turn, ld.rotated, a.eps), w[i]);
   }
   if (kind == 0) {
     uint16_t* dst = a.qo.row(b, t, h0);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      uint32_t w[4];
-      pack_pairs<kInter>(y[i], w);
-      if (i < heads) store_pairs<kInter, kVec>(dst + i * a.qo.sh, ld, w);
-    }
+    for (int i = 0; i < kHeads; ++i)
+      if (i < heads) store_words<W, kInter, kVec>(dst + i * a.qo.sh, ld, w[i]);
     return;
   }
   // where the token's first row lies: its heads are a page's rows apart
@@ -119,21 +115,26 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
   float* const scales_out = kind == 1 ? a.pool.k_scales : a.pool.v_scales;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    uint32_t w[4], codes[2];
-    pack_pairs<kInter>(y[i], w);
-    const float scale = quantise_row<kLanes, 4, FMT>(w, codes);
+    uint32_t codes[W / 2];
+    const float scale = quantise_row<kLanes, W, FMT>(w[i], codes);
     if (i < heads && dst >= 0) {
       const long long row = dst + ((long long)i << a.index.page_log2);
-      *reinterpret_cast<uint32_t*>(codes_out + row * D + ld.o0) = codes[0];
-      *reinterpret_cast<uint32_t*>(codes_out + row * D + ld.o1) = codes[1];
+      uint8_t *c0 = codes_out + row * D + ld.o0, *c1 = codes_out + row * D + ld.o1;
+      if constexpr (W == 8) {
+        *reinterpret_cast<uint2*>(c0) = make_uint2(codes[0], codes[1]);
+        *reinterpret_cast<uint2*>(c1) = make_uint2(codes[2], codes[3]);
+      } else {
+        *reinterpret_cast<uint32_t*>(c0) = codes[0];
+        *reinterpret_cast<uint32_t*>(c1) = codes[1];
+      }
       if (l == 0) scales_out[row] = scale;
     }
   }
 }
 
-template <int D, int FMT, bool kInter, bool kNorm, bool kVec, int kHeads>
+template <int D, int W, int FMT, bool kInter, bool kNorm, bool kVec, int kHeads>
 cudaError_t launch_heads(QkvArgs a, uint32_t tokens, cudaStream_t stream) {
-  const uint32_t per_block = kThreads / (D / 8);
+  const uint32_t per_block = kThreads / (D / (2 * W));
   const int heads[2] = {a.hq, a.pool.n_kv_heads};
   for (int i = 0; i < 2; ++i) {
     const uint32_t chunks = (heads[i] + kHeads - 1) / kHeads;
@@ -143,31 +144,35 @@ cudaError_t launch_heads(QkvArgs a, uint32_t tokens, cudaStream_t stream) {
   a.tokens = tokens;
   const dim3 grid(std::max(1u, a.blocks[0] + 2 * a.blocks[1]));  // no tokens: new_lens alone
   void* args[] = {&a};
-  return launch_with_pdl(reinterpret_cast<const void*>(&kvq_append_qkv_kernel<D, FMT, kInter, kNorm, kVec, kHeads>),
+  return launch_with_pdl(reinterpret_cast<const void*>(&kvq_append_qkv_kernel<D, W, FMT, kInter, kNorm, kVec, kHeads>),
                          grid, dim3(kThreads), args, 0, stream);
 }
 
 // Heads per lane group, on the grounds of qk_rope.cu.  32 + 8 + 8 heads
-// (head_dim 128, int8) of 64 single tokens take 2.8 us (four each: 3.0; the two
-// calls: 4.2), of 500 tokens 4.3 us with four (one each: 5.4; the two calls: 5.4), of 8192
-// tokens 41 us (eight each: 47; the two calls: 39, so a long prompt gains nothing).
-template <int D, int FMT, bool kInter, bool kNorm, bool kVec>
+// (head_dim 128, int8) of 64 single tokens take 2.7 us (the two calls 4.2), of
+// 2000 tokens 8.9 us (11.1), of 8192 tokens 37 us (41; 0.76 of the copy rate).
+template <int D, int W, int FMT, bool kInter, bool kNorm, bool kVec>
 cudaError_t launch(const QkvArgs& a, uint32_t tokens, cudaStream_t stream) {
   const double fill = (double)tokens * (a.hq + 2 * a.pool.n_kv_heads) * (D / 8) / (device_sm_count() * 2048.0);
-  return fill < 0.6 ? launch_heads<D, FMT, kInter, kNorm, kVec, 1>(a, tokens, stream)
-                    : launch_heads<D, FMT, kInter, kNorm, kVec, 4>(a, tokens, stream);
+  return fill < 0.6 ? launch_heads<D, W, FMT, kInter, kNorm, kVec, 1>(a, tokens, stream)
+                    : launch_heads<D, W, FMT, kInter, kNorm, kVec, 4>(a, tokens, stream);
 }
 
-template <int D, int FMT, bool kInter>
-cudaError_t launch(const QkvArgs& a, uint32_t tokens, bool vec, cudaStream_t st) {
-  if (a.qw)
-    return vec ? launch<D, FMT, kInter, true, true>(a, tokens, st) : launch<D, FMT, kInter, true, false>(a, tokens, st);
-  return vec ? launch<D, FMT, kInter, false, true>(a, tokens, st) : launch<D, FMT, kInter, false, false>(a, tokens, st);
+// W by the rule of qk_rope.cu.
+template <int D, int FMT, bool kInter, bool kNorm>
+cudaError_t launch(const QkvArgs& a, uint32_t tokens, int alignment, cudaStream_t st) {
+  if (alignment >= 32 && a.rot % 16 == 0) return launch<D, 8, FMT, kInter, kNorm, true>(a, tokens, st);
+  return alignment >= 16 ? launch<D, 4, FMT, kInter, kNorm, true>(a, tokens, st)
+                         : launch<D, 4, FMT, kInter, kNorm, false>(a, tokens, st);
 }
 
 template <int D, int FMT>
-cudaError_t launch(const QkvArgs& a, uint32_t tokens, bool inter, bool vec, cudaStream_t st) {
-  return inter ? launch<D, FMT, true>(a, tokens, vec, st) : launch<D, FMT, false>(a, tokens, vec, st);
+cudaError_t launch(const QkvArgs& a, uint32_t tokens, bool inter, int alignment, cudaStream_t st) {
+  if (a.qw)
+    return inter ? launch<D, FMT, true, true>(a, tokens, alignment, st)
+                 : launch<D, FMT, false, true>(a, tokens, alignment, st);
+  return inter ? launch<D, FMT, true, false>(a, tokens, alignment, st)
+               : launch<D, FMT, false, false>(a, tokens, alignment, st);
 }
 
 }  // namespace
@@ -204,9 +209,10 @@ extern "C" int lara_kvq_append_qkv(const lara_kvq_pool* pool, const int32_t* blo
   if (overlap(new_lens, starts, 4 * (size_t)batch) || overlap(new_lens, counts, 4 * (size_t)batch))
     return set_last_error(LARA_ERR_STREAM_DEST, "new_lens must not overlap starts or counts");
   if (n_new == 0 && !new_lens) return LARA_OK;
-  const bool vec = vec_ok(q, q_sb, batch, q_st, n_new, q_sh, n_q_heads) && vec_ok(k, k_sb, batch, k_st, n_new, k_sh, hkv) &&
-                   vec_ok(v, v_sb, batch, v_st, n_new, v_sh, hkv) &&
-                   vec_ok(q_out, qo_sb, batch, qo_st, n_new, qo_sh, n_q_heads);
+  const int alignment = std::min({row_alignment(q, q_sb, batch, q_st, n_new, q_sh, n_q_heads),
+                                  row_alignment(k, k_sb, batch, k_st, n_new, k_sh, hkv),
+                                  row_alignment(v, v_sb, batch, v_st, n_new, v_sh, hkv),
+                                  row_alignment(q_out, qo_sb, batch, qo_st, n_new, qo_sh, n_q_heads)});
   a.pool = *pool;
   a.starts = starts;
   a.counts = counts;
@@ -232,7 +238,7 @@ extern "C" int lara_kvq_append_qkv(const lara_kvq_pool* pool, const int32_t* blo
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaErrorInvalidValue;
 #define LARA_CASE(d, f) \
-  if (pool->head_dim == d && pool->format == f) e = launch<d, f>(a, tokens, inter, vec, st);
+  if (pool->head_dim == d && pool->format == f) e = launch<d, f>(a, tokens, inter, alignment, st);
   LARA_CASE(128, LARA_KVQ_INT8) LARA_CASE(128, LARA_KVQ_FP8_E4M3)
   LARA_CASE(64, LARA_KVQ_INT8) LARA_CASE(64, LARA_KVQ_FP8_E4M3)
 #undef LARA_CASE

@@ -5,10 +5,12 @@
 //   y = x w / sqrt(mean(x^2) + eps);  (y_a, y_b) -> (y_a c - y_b s, y_a s + y_b c)
 //
 // Bound by HBM: every head is read and written once (4 D bytes), the table row
-// of a token once from HBM (4 rot bytes) and from L2 after that.  D / 8 lanes
+// of a token once from HBM (4 rot bytes) and from L2 after that.  D / 16 lanes
 // hold a head in registers between the load and the store.  A lane group takes
 // kHeads heads of one token, all of q or all of k: it folds the weights into
 // the token's cosines and sines once, and has kHeads loads in flight.
+#include <algorithm>
+
 #include "kvq.cuh"
 
 namespace lara {
@@ -36,9 +38,9 @@ struct NormRopeArgs {
 
 // Lane group i takes chunk i % chunks (kHeads heads, of q first) of token
 // i / chunks, so that neighbours in the grid are neighbours in memory.
-template <int D, bool kInter, bool kNorm, bool kVec, int kHeads>
+template <int D, int W, bool kInter, bool kNorm, bool kVec, int kHeads>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / (2 * W);
   allow_dependent_launch();
   grid_dependency_wait();
   const uint32_t group = blockIdx.x * (uint32_t)(kThreads / kLanes) + threadIdx.x / kLanes;
@@ -49,68 +51,75 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
   const bool is_k = (int)chunk >= a.q_chunks;
   const int h0 = ((int)chunk - (is_k ? a.q_chunks : 0)) * kHeads;
   const int heads = group < a.groups ? (is_k ? a.hkv : a.hq) - h0 : 0;  // to store, at most kHeads of them
-  const HeadLane ld(l, a.rot, kInter);
+  const HeadLane<W> ld(l, a.rot, kInter);
 
   const long long sh = is_k ? a.k.sh : a.q.sh;
   const uint16_t* src = is_k ? a.k.row(b, t, h0) : a.q.row(b, t, h0);
-  Pairs x[kHeads];
+  uint32_t x[kHeads][W];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) x[i] = load_pairs<kInter, kVec>(src + (i < heads ? i : 0) * sh, ld);
-  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < kHeads; ++i) load_words<W, kInter, kVec>(src + (i < heads ? i : 0) * sh, ld, x[i]);
+  const float* row = nullptr;
   if (ld.rotated) {
     int pos = a.positions[tok];
     if (pos < 0 || pos >= a.max_pos) {
       if (a.status) atomicOr(a.status, kDevBadPosition);
       pos = pos < 0 ? 0 : a.max_pos - 1;
     }
-    const float* row = a.cos_sin + (long long)pos * a.rot + 4 * l;
-    c = *reinterpret_cast<const float4*>(row);
-    s = *reinterpret_cast<const float4*>(row + a.rot / 2);
+    row = a.cos_sin + (long long)pos * a.rot;
   }
-  const Turn turn = make_turn<kInter>(c, s, kNorm ? (is_k ? a.kw : a.qw) : nullptr, ld);
+  const Turn<W> turn = make_turn<W, kInter>(row, a.rot, l, kNorm ? (is_k ? a.kw : a.qw) : nullptr, ld);
   const long long osh = is_k ? a.ko.sh : a.qo.sh;
   uint16_t* dst = is_k ? a.ko.row(b, t, h0) : a.qo.row(b, t, h0);
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    const Pairs y = turn_head<D, kNorm>(x[i], turn, ld.rotated, a.eps);
-    uint32_t w[4];
-    pack_pairs<kInter>(y, w);
-    if (i < heads) store_pairs<kInter, kVec>(dst + i * osh, ld, w);
+    const Pairs<W> y = turn_head<D, W, kNorm>(pairs_of<W, kInter>(x[i]), turn, ld.rotated, a.eps);
+    uint32_t w[W];
+    words_of<W, kInter>(y, w);
+    if (i < heads) store_words<W, kInter, kVec>(dst + i * osh, ld, w);
   }
 }
 
-template <int D, bool kInter, bool kNorm, bool kVec, int kHeads>
+template <int D, int W, bool kInter, bool kNorm, bool kVec, int kHeads>
 cudaError_t launch_heads(NormRopeArgs a, uint32_t tokens, cudaStream_t stream) {
   a.q_chunks = (a.hq + kHeads - 1) / kHeads;
   const uint32_t chunks = a.q_chunks + (a.hkv + kHeads - 1) / kHeads;
   a.groups = tokens * chunks;
   a.chunks = FastDiv(chunks);
-  const uint32_t per_block = kThreads / (D / 8);
+  const uint32_t per_block = kThreads / (D / (2 * W));
   const dim3 grid((a.groups + per_block - 1) / per_block);
   void* args[] = {&a};
-  return launch_with_pdl(reinterpret_cast<const void*>(&qk_norm_rope_kernel<D, kInter, kNorm, kVec, kHeads>), grid,
+  return launch_with_pdl(reinterpret_cast<const void*>(&qk_norm_rope_kernel<D, W, kInter, kNorm, kVec, kHeads>), grid,
                          dim3(kThreads), args, 0, stream);
 }
 
 // Heads per lane group.  More of them share a token's turn and keep more loads
 // in flight, fewer spread a small call over more lanes; what counts is how often
-// the call would fill the GPU's lanes with one head each.  72 heads (head_dim
-// 128) of 128, 256, 1024, 16384 tokens: one each 2.7, 4.1, 11.3, 165 us; two
-// 2.7, 2.9, 7.7, 130; four 2.9, 3.5, 6.3, 98; eight 3.0, 4.4, 6.8, 93 us (0.99
-// of the copy rate).
-template <int D, bool kInter, bool kNorm, bool kVec>
+// the call would fill the GPU's threads with eight dims each.  72 heads
+// (head_dim 128) of 128, 512, 1024, 16384 tokens: one each 2.8, 5.0, 8.2,
+// 143 us; two 2.8, 4.6, 7.2, 132; four 2.8, 3.9, 6.2, 101; eight 3.0, 4.8, 5.4,
+// 93 us (1.0 of the copy rate; 102 us with inputs that no earlier call left in
+// L2).  8 dims per lane instead of 16: 1024 tokens 6.3, 2048 10.8 against 9.5 us.
+template <int D, int W, bool kInter, bool kNorm, bool kVec>
 cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, cudaStream_t stream) {
   const double fill = (double)tokens * (a.hq + a.hkv) * (D / 8) / (device_sm_count() * 2048.0);
-  if (fill < 0.5) return launch_heads<D, kInter, kNorm, kVec, 1>(a, tokens, stream);
-  if (fill < 1.5) return launch_heads<D, kInter, kNorm, kVec, 2>(a, tokens, stream);
-  if (fill < 7.0) return launch_heads<D, kInter, kNorm, kVec, 4>(a, tokens, stream);
-  return launch_heads<D, kInter, kNorm, kVec, 8>(a, tokens, stream);
+  if (fill < 0.5) return launch_heads<D, W, kInter, kNorm, kVec, 1>(a, tokens, stream);
+  if (fill < 1.5) return launch_heads<D, W, kInter, kNorm, kVec, 2>(a, tokens, stream);
+  if (fill < 3.5) return launch_heads<D, W, kInter, kNorm, kVec, 4>(a, tokens, stream);
+  return launch_heads<D, W, kInter, kNorm, kVec, 8>(a, tokens, stream);
+}
+
+// W = 8 where rows start on 32-byte boundaries and rot allows it.
+template <int D, bool kInter, bool kNorm>
+cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, int alignment, cudaStream_t stream) {
+  if (alignment >= 32 && a.rot % 16 == 0) return launch<D, 8, kInter, kNorm, true>(a, tokens, stream);
+  return alignment >= 16 ? launch<D, 4, kInter, kNorm, true>(a, tokens, stream)
+                         : launch<D, 4, kInter, kNorm, false>(a, tokens, stream);
 }
 
 template <int D, bool kInter>
-cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, bool vec, cudaStream_t stream) {
-  if (a.qw) return vec ? launch<D, kInter, true, true>(a, tokens, stream) : launch<D, kInter, true, false>(a, tokens, stream);
-  return vec ? launch<D, kInter, false, true>(a, tokens, stream) : launch<D, kInter, false, false>(a, tokens, stream);
+cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, int alignment, cudaStream_t stream) {
+  return a.qw ? launch<D, kInter, true>(a, tokens, alignment, stream)
+              : launch<D, kInter, false>(a, tokens, alignment, stream);
 }
 
 }  // namespace
@@ -143,9 +152,10 @@ extern "C" int lara_qk_norm_rope(const uint16_t* q, long long q_sb, long long q_
   if (!aligned(q, 2) || !aligned(k, 2) || !aligned(q_out, 2) || !aligned(k_out, 2) || !aligned(positions, 4) ||
       !aligned(cos_sin, 16) || !aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(workspace, 4))
     return set_last_error(LARA_ERR_STREAM_DEST, "cos_sin and the weights must be 16-byte aligned");
-  const bool vec = vec_ok(q, q_sb, batch, q_st, n, q_sh, n_q_heads) && vec_ok(k, k_sb, batch, k_st, n, k_sh, n_kv_heads) &&
-                   vec_ok(q_out, qo_sb, batch, qo_st, n, qo_sh, n_q_heads) &&
-                   vec_ok(k_out, ko_sb, batch, ko_st, n, ko_sh, n_kv_heads);
+  const int alignment = std::min({row_alignment(q, q_sb, batch, q_st, n, q_sh, n_q_heads),
+                                  row_alignment(k, k_sb, batch, k_st, n, k_sh, n_kv_heads),
+                                  row_alignment(q_out, qo_sb, batch, qo_st, n, qo_sh, n_q_heads),
+                                  row_alignment(k_out, ko_sb, batch, ko_st, n, ko_sh, n_kv_heads)});
   NormRopeArgs a{};
   a.q = {q, q_sb, q_st, q_sh};
   a.k = {k, k_sb, k_st, k_sh};
@@ -166,8 +176,8 @@ extern "C" int lara_qk_norm_rope(const uint16_t* q, long long q_sb, long long q_
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // without a rotation nothing is paired: side by side is the wider access
   const bool inter = interleaved || !cos_sin;
-  const cudaError_t e = head_dim == 128 ? (inter ? launch<128, true>(a, tokens, vec, st) : launch<128, false>(a, tokens, vec, st))
-                                        : (inter ? launch<64, true>(a, tokens, vec, st) : launch<64, false>(a, tokens, vec, st));
+  const cudaError_t e = head_dim == 128 ? (inter ? launch<128, true>(a, tokens, alignment, st) : launch<128, false>(a, tokens, alignment, st))
+                                        : (inter ? launch<64, true>(a, tokens, alignment, st) : launch<64, false>(a, tokens, alignment, st));
   if (e != cudaSuccess)
     return set_last_error(LARA_ERR_CUDA, std::string("qk_norm_rope launch: ") + cudaGetErrorString(e));
   return LARA_OK;
