@@ -287,23 +287,30 @@ __device__ __forceinline__ float quantise_row(const uint32_t* w, uint32_t* codes
   const uint32_t am = row_amax<kLanes, kWords>(w);
   float scale;
   if constexpr (FMT == LARA_KVQ_INT8) {
-    // rint of the exact quotient 127 x / a, ties to even, from y = x (127 / a)
-    // with two roundings.  For bf16 x and a a quotient is either a tie exactly
-    // or at least 2^-17 of itself away from one, so y rounded to 18 significant
-    // bits (65 y - (65 y - y)) lies on the tie or on the quotient's side of it.
-    // Adding 1.5 * 2^23 then rounds to an integer, in the sum's low byte.
-    const float a = __uint_as_float(max(am << 16, kTinyBits));
-    scale = __fdiv_rn(a, 127.f);
-    const float r = __fdiv_rn(127.f, a);
-    const float2 r2 = make_float2(r, r), k65 = make_float2(65.f, 65.f), neg = make_float2(-1.f, -1.f);
-    const float2 magic = make_float2(0x1.8p23f, 0x1.8p23f);
+    // rint of the exact quotient 127 x / a, ties to even, as x r rounded by
+    // adding 1.5 * 2^23 (the integer is the sum's low byte).  For bf16 x and a a
+    // quotient that is not a tie is at least 2^-17 of itself away from one.  Ties
+    // are x = a / 2 (63.5, to 64) and, where a's significand is 254, any half:
+    // there 127 / a is a power of two and x r exact.  Elsewhere r is taken a few
+    // units in the last place above 127 / a, which settles a / 2 as it should.
+    const uint32_t ab = max(am << 16, kTinyBits), expo = (ab & 0x7f800000u) - 0x3f800000u, sig = ab & 0x7fffffu;
+    const float a = __uint_as_float(ab);
+    float rcp;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(__uint_as_float(sig | 0x3f800000u)));  // off by 2^-23 at most
+    const uint32_t r127 = sig == 0x7e0000u ? 0x42800000u : __float_as_uint(127.f * rcp) + 6u;
+    const float r = __uint_as_float(r127 - expo);
+    // a / 127, rounded once: the product's error is put right by a fused step
+    constexpr float kInv127 = 1.f / 127.f;
+    const float q = __fmul_rn(a, kInv127);
+    scale = __fmaf_rn(__fmaf_rn(-127.f, q, a), kInv127, q);
+    const float2 r2 = make_float2(r, r), magic = make_float2(0x1.8p23f, 0x1.8p23f);
 #pragma unroll
     for (int i = 0; i < kWords; i += 2) {
       uint32_t c[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float2 y = mul2(make_float2(bf16lo(w[i + k]), bf16hi(w[i + k])), r2), y65 = mul2(y, k65);
-        const float2 n = add2(fma2(fma2(y, neg, y65), neg, y65), magic);
+        // the product is rounded by itself: a fused step could see past a tie
+        const float2 n = add2(mul2(make_float2(bf16lo(w[i + k]), bf16hi(w[i + k])), r2), magic);
         c[k] = __byte_perm(__float_as_uint(n.x), __float_as_uint(n.y), 0x0040);
       }
       codes[i / 2] = __byte_perm(c[0], c[1], 0x5410);

@@ -972,3 +972,31 @@ def test_decode_of_empty_sequences_alone(B):
     out = torch.full_like(q, 3.0)
     kvquant.gqa_decode_kvq(q, case.pool, case.dtable, torch.zeros_like(case.dlens), workspace=ws, out=out)
     assert ops.workspace_status(ws) == 0 and torch.count_nonzero(out) == 0
+
+
+@pytest.mark.gpu
+def test_int8_codes_of_every_ratio():
+    """Every pair of bf16 significands and 20 exponents apart: the code is the exact quotient's, ties to even."""
+    _need_gpu()
+    from lara_b200 import kvquant
+
+    top = torch.arange(128, 256, dtype=torch.float64)                      # a
+    x = (torch.arange(128, 256, dtype=torch.float64)[None, :] * 2.0 ** -torch.arange(0, 20, dtype=torch.float64)[:, None])
+    x = torch.cat([x.flatten(), -x.flatten()])                             # 5120 values
+    per = 127
+    n = -(-x.numel() // per)
+    xs = torch.nn.functional.pad(x, (0, n * per - x.numel())).view(n, per)
+    for scale in (2.0 ** -100, 2.0 ** -40, 1.0, 2.0 ** 115):
+        k = torch.zeros((128, 1, n, 128), dtype=torch.float64)
+        k[..., 0] = top[:, None, None]
+        k[..., 1:] = torch.where(xs.abs()[None] <= top[:, None, None], xs[None], 0.0)[:, None]
+        k = (k * scale).to(torch.bfloat16)
+        pages = 128 * (-(-n // 16))
+        pool = kvquant.QuantPool.empty(pages, 16, 1, 128, "int8", DEV)
+        table = torch.arange(pages, dtype=torch.int32, device=DEV).view(128, -1)
+        zero = torch.zeros(128, dtype=torch.int32, device=DEV)
+        kvquant.kvq_append(pool, table, zero, k.to(DEV), k.to(DEV))
+        c64, s64 = quantise64(k, "int8")
+        codes = pool.k_codes.view(128, -1, 128)[:, :n].cpu()
+        assert torch.equal(codes, c64[:, 0].to(torch.int8))
+        assert torch.equal(pool.k_scales.view(128, -1)[:, :n].cpu(), s64[:, 0].float())
