@@ -73,6 +73,14 @@ constexpr int kSoloTiles = 16;
 // What a unit costs beside its tiles, in tiles, where shares are measured out
 // (2400 units of 1-10 tiles: 38 us; 78 us without).
 constexpr int kUnitCost = 8, kUnitCostSolo = 2;
+// Where a unit has CTAs of its own: in microseconds, a tile takes a CTA kTileUs,
+// a part its join kPartUs per head and dim, and a join in two steps (of groups of
+// parts, then of the groups; more than kOneJoin parts) kTwoStepsUs on top.  One
+// kv head, 4 query heads, of 16384, 65536, 262144 tokens: 14, 24, 43 us with the
+// parts that pay in one step, 19, 45, 52 with one for every CTA, 16, 21, 28 so in
+// two steps; 16 query heads 25, 43, 77; 49, 119, 128; 30, 36, 46.
+constexpr float kTileUs = 0.21f, kPartUs = 0.025f / 128.f, kTwoStepsUs = 6.f;
+constexpr int kOneJoin = 64;
 constexpr int kJoinUnroll = 8;     // parts whose sums a join loads together
 constexpr int kFewParts = 4;       // parts of a unit that its last CTA joins without publishing its own
 constexpr int kLensCached = 1024;  // lengths kept in shared memory
@@ -103,7 +111,8 @@ struct KvqDecodeArgs {
   int batch, n_q_heads, group;
   float scale_log2;
   int* status;
-  int* counters;    // [batch * Hkv], zero between launches
+  int* group_counters;  // [2 * grid] and
+  int* counters;        // [batch * Hkv], zero between launches
   float2* part_ml;  // [2 * grid][group] (R, l)
   float* part_acc;  // [2 * grid][group][D]
 };
@@ -304,24 +313,25 @@ struct Join {
   __device__ __forceinline__ int slot(int i) const { return i == 0 ? first : (first & ~1) + 2 * i; }
 };
 
-// Joins the published parts of a unit, all threads together.  `ml` holds `room`
-// (R, l) pairs in shared memory: they are brought there first, so that the
-// sums' loads wait for nothing.
+// Joins published parts first, first + step, .. (`parts` of them) of a unit, all
+// threads together, into slot `dest` or, where that is negative, the output.
+// `ml` holds `room` (R, l) pairs in shared memory: they are brought there first,
+// so that the sums' loads wait for nothing.
 template <int D, int kItems>
-__device__ __forceinline__ void join_published(const KvqDecodeArgs& a, const Join& j, long long out_row, float2* ml,
-                                               int room) {
+__device__ __forceinline__ void join_published(const KvqDecodeArgs& a, const Join& j, int first, int step, int parts,
+                                               int dest, long long out_row, float2* ml, int room) {
   const int G = a.group, most = room / G;
   float4 x[kItems];
   float top[kItems], L[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) join_start(top[k], L[k], x[k]);
   for (int pass = 0; pass < 2; ++pass)  // the largest R, then the sums
-    for (int p0 = 0; p0 < j.parts; p0 += most) {
-      const int np = min(most, j.parts - p0);
-      if (pass == 0 || j.parts > most) {
+    for (int p0 = 0; p0 < parts; p0 += most) {
+      const int np = min(most, parts - p0);
+      if (pass == 0 || parts > most) {
         __syncthreads();
         for (int i = threadIdx.x; i < np * G; i += kThreads)
-          ml[i] = __ldcg(a.part_ml + (long long)j.slot(p0 + i / G) * G + i % G);
+          ml[i] = __ldcg(a.part_ml + (long long)j.slot(first + (p0 + i / G) * step) * G + i % G);
         __syncthreads();
       }
 #pragma unroll
@@ -336,7 +346,7 @@ __device__ __forceinline__ void join_published(const KvqDecodeArgs& a, const Joi
           for (int i = 0; i < np; ++i)
             join_add(top[k], L[k], x[k], ml[i * G + h],
                      __ldcg(reinterpret_cast<const float4*>(
-                         a.part_acc + ((long long)j.slot(p0 + i) * G + h) * D + d)));
+                         a.part_acc + ((long long)j.slot(first + (p0 + i) * step) * G + h) * D + d)));
         }
       }
     }
@@ -344,9 +354,15 @@ __device__ __forceinline__ void join_published(const KvqDecodeArgs& a, const Joi
   for (int k = 0; k < kItems; ++k) {
     const int item = threadIdx.x + k * kThreads;
     if (item >= G * (D / 4)) continue;
-    const float inv = 1.f / L[k];
-    *reinterpret_cast<uint2*>(a.o + (out_row + item / (D / 4)) * D + item % (D / 4) * 4) =
-        make_uint2(pack2_rn(x[k].x * inv, x[k].y * inv), pack2_rn(x[k].z * inv, x[k].w * inv));
+    const int h = item / (D / 4), d = item % (D / 4) * 4;
+    if (dest < 0) {
+      const float inv = 1.f / L[k];
+      *reinterpret_cast<uint2*>(a.o + (out_row + h) * D + d) =
+          make_uint2(pack2_rn(x[k].x * inv, x[k].y * inv), pack2_rn(x[k].z * inv, x[k].w * inv));
+    } else {
+      *reinterpret_cast<float4*>(a.part_acc + ((long long)dest * G + h) * D + d) = x[k];
+      if (d == 0) a.part_ml[(long long)dest * G + h] = make_float2(top[k], L[k]);
+    }
   }
 }
 
@@ -488,7 +504,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
   } else if (few) {
     const long long ctas = max(1ll, min(gridDim.x - units, quotient(total, kMinTiles)));
     const long long per = quotient(total + ctas - 1, ctas);
-    auto parts_of = [&](int b) { return (int)quotient(tiles_of(len_of(b)) + per - 1, per); };
+    auto parts_of = [&](int b) {
+      const int tiles = tiles_of(len_of(b));
+      const int most = (int)quotient(tiles + per - 1, per);
+      const float t = kTileUs * tiles, c = kPartUs * (G * D);
+      const int one = min(min(max((int)sqrtf(t / c), 1), kOneJoin), most);
+      const bool two_steps =
+          most > kOneJoin && t / most + 2.f * c * sqrtf((float)most) + kTwoStepsUs < t / one + c * one;
+      return two_steps ? most : one;  // none without tiles
+    };
     __syncthreads();  // s_sum is free again
     mine = 0;
     for (int b = b_lo; b < b_hi; ++b) mine += parts_of(b);
@@ -936,19 +960,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     }
     if (whole || last_here) continue;
 
-    // ---- this part is published; the last CTA to do so joins them all ----
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const bool last = atomicAdd(counter, 1) == j.parts - 1;
-      if (last) *counter = 0;
-      s_flag = last;
-    }
-    __syncthreads();
-    if (s_flag) {
+    // ---- this part is published; the last CTA to do so joins them all, or,
+    // of many parts, those of its group, and the last group's the groups' ----
+    auto last_of = [&](int* ctr, int n) {
       __threadfence();
-      join_published<D, (NG * 8 * D / 4 + kThreads - 1) / kThreads>(a, j, out_row, reinterpret_cast<float2*>(smem + s_idle[0]),
-                                                                    C::kStageBytes / 8);
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const bool last = atomicAdd(ctr, 1) == n - 1;
+        if (last) *ctr = 0;
+        s_flag = last;
+      }
+      __syncthreads();
+      const bool last = s_flag;
+      if (last) __threadfence();
+      return last;
+    };
+    constexpr int kItems = (NG * 8 * D / 4 + kThreads - 1) / kThreads;
+    float2* const ml = reinterpret_cast<float2*>(smem + s_idle[0]);
+    if (j.parts <= kOneJoin) {
+      if (last_of(counter, j.parts))
+        join_published<D, kItems>(a, j, 0, 1, j.parts, -1, out_row, ml, C::kStageBytes / 8);
+    } else {
+      const int size = (int)ceilf(sqrtf((float)j.parts)), lead = (j.own / 2 - j.first / 2) / size * size;
+      const int groups = (j.parts + size - 1) / size, here = min(size, j.parts - lead), dest = j.slot(lead);
+      if (last_of(a.group_counters + dest, here)) {
+        join_published<D, kItems>(a, j, lead, 1, here, dest, out_row, ml, C::kStageBytes / 8);
+        if (last_of(counter, groups))
+          join_published<D, kItems>(a, j, 0, size, groups, -1, out_row, ml, C::kStageBytes / 8);
+      }
     }
     __syncthreads();  // s_flag and the idle stages are free again
   }
@@ -957,7 +996,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
 
 // Workspace: status word | partial results (two slots per CTA) | counters.
 struct Layout {
-  size_t ml_off, acc_off, counters_off, total;
+  size_t ml_off, acc_off, groups_off, counters_off, total;
 };
 
 template <int D, int NG>
@@ -973,7 +1012,8 @@ Layout layout(int batch, int group, int n_kv_heads, int head_dim) {
   Layout w;
   w.ml_off = kStatusBytes;
   w.acc_off = w.ml_off + up(slots * group * sizeof(float2));
-  w.counters_off = w.acc_off + up(slots * group * head_dim * sizeof(float));
+  w.groups_off = w.acc_off + up(slots * group * head_dim * sizeof(float));
+  w.counters_off = w.groups_off + up(slots * sizeof(int));
   w.total = w.counters_off + up((size_t)batch * n_kv_heads * sizeof(int));
   return w;
 }
@@ -1045,6 +1085,7 @@ extern "C" int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool,
   a.status = reinterpret_cast<int*>(base);
   a.part_ml = reinterpret_cast<float2*>(base + w.ml_off);
   a.part_acc = reinterpret_cast<float*>(base + w.acc_off);
+  a.group_counters = reinterpret_cast<int*>(base + w.groups_off);
   a.counters = reinterpret_cast<int*>(base + w.counters_off);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaErrorInvalidValue;

@@ -1000,3 +1000,18 @@ def test_int8_codes_of_every_ratio():
         codes = pool.k_codes.view(128, -1, 128)[:, :n].cpu()
         assert torch.equal(codes, c64[:, 0].to(torch.int8))
         assert torch.equal(pool.k_scales.view(128, -1)[:, :n].cpu(), s64[:, 0].float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lens,hkv,G,D", [([140000], 1, 2, 64), ([40000, 3, 0], 1, 4, 128), ([9000] * 4, 1, 16, 128)])
+def test_decode_few_long_sequences(fmt, lens, hkv, G, D):
+    """Units that many CTAs share: joined in one step, and in two."""
+    g = torch.Generator().manual_seed(len(lens) + G)
+    n = max(lens)
+    k, v = _rand_bf16(g, (hkv, n, D)), _rand_bf16(g, (hkv, n, D))
+    case = SharedRows(lens, hkv, D, 256, fmt, k, v, seed=n)
+    q = _rand_bf16(g, (len(lens), hkv * G, D), False).to(DEV)
+    o = _decode_gpu(case, q)
+    case.check(q, o)
+    assert torch.equal(o, _decode_gpu(case, q))
