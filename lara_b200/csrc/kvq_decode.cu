@@ -44,8 +44,8 @@
 // 1,048,576 tokens 318 us (1.07: it only reads); one of 300 tokens 6.5 us.
 // About 10 us of a large call do not stream: 2 us until a CTA knows its share,
 // 3 us until its first rows arrive, and at the end CTAs finish over 10 us.
-// Two of three stages with two CTAs per SM, separate K and V slots (K fetched
-// two tiles ahead) and L2 prefetch hints were no faster.
+// Three stages with two CTAs per SM, separate K and V slots (K fetched two
+// tiles ahead) and L2 prefetch hints were no faster.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
