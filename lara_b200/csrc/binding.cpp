@@ -108,7 +108,10 @@ void* workspace(PyObject* o, int index, size_t* bytes = nullptr) {
   if (o == Py_None) return nullptr;
   const at::Tensor& t = tensor(o, "workspace");
   if (index_of(t) != index || !t.is_contiguous()) throw BadValue("workspace must be a contiguous tensor on the same device");
-  if (bytes) *bytes = t.nbytes();
+  if (bytes)
+    *bytes = t.nbytes();  // checked by the call
+  else if (t.nbytes() < 256 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 4)
+    throw BadValue("workspace must hold at least 256 bytes, 4-byte aligned (ops.new_workspace)");
   return t.data_ptr();
 }
 
@@ -130,7 +133,14 @@ long long integer(PyObject* o) {
   return x;
 }
 
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o) {
+  const int x = PyObject_IsTrue(o);
+  if (x < 0) {
+    PyErr_Clear();
+    throw BadType("a truth value is needed, got " + std::string(Py_TYPE(o)->tp_name));
+  }
+  return x == 1;
+}
 
 const lara_kvq_pool* pool_of(PyObject* o) {
   return reinterpret_cast<const lara_kvq_pool*>(static_cast<uintptr_t>(integer(o)));

@@ -890,6 +890,29 @@ def test_small_batches_and_empty_calls():
 
 
 @pytest.mark.gpu
+def test_small_workspaces_and_odd_flags_are_refused():
+    _need_gpu()
+    from lara_b200 import kvquant, ops
+
+    case = Case([5, 3], 2, 64, 16, "int8", seed=1)
+    small = torch.zeros(255, dtype=torch.uint8, device=DEV)
+    k = torch.zeros((2, 2, 1, 64), dtype=torch.bfloat16, device=DEV)
+    heads = torch.zeros((2, 1, 2, 64), dtype=torch.bfloat16, device=DEV)
+    for call in (lambda ws: kvquant.kvq_read(case.pool, case.dtable, case.dlens, 7, workspace=ws),
+                 lambda ws: kvquant.kvq_append(case.pool, case.dtable, case.dlens, k, k, workspace=ws),
+                 lambda ws: kvquant.kvq_append_qkv(case.pool, case.dtable, case.dlens, heads, heads, heads, workspace=ws),
+                 lambda ws: ops.qk_norm_rope(heads, heads, workspace=ws)):
+        for ws in (small, small[:0], torch.zeros(400, dtype=torch.uint8, device=DEV)[1:300]):
+            with pytest.raises(ValueError, match="256 bytes"):
+                call(ws)
+    for call in (lambda flag: ops.qk_norm_rope(heads, heads, interleaved=flag),
+                 lambda flag: kvquant.kvq_append_qkv(case.pool, case.dtable, case.dlens, heads, heads, heads,
+                                                     interleaved=flag)):
+        with pytest.raises(TypeError, match="truth value"):
+            call(torch.zeros(2))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("D,G", [(128, 4), (128, 12), (64, 8), (64, 16)])
 @pytest.mark.parametrize("B,hkv,n", [(150, 8, 100), (80, 8, 700), (7, 4, 3000), (1300, 1, 60), (1300, 1, 900)])
