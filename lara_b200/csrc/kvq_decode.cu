@@ -39,7 +39,7 @@
 //
 // Measured (head_dim 128, 8 kv heads, int8 where not said): 64 sequences of
 // 4096 tokens 88 us, 0.96 of the copy rate of 6534 GB/s (e4m3 87 us; 64 query
-// heads 90 us; 128 query heads 110 us, e4m3 97 us, bound by the products' issue
+// heads 90 us; 128 query heads 109 us, e4m3 98 us, bound by the products' issue
 // and latency with eight warps per SM), of 8192 tokens 167 us (1.02); one of
 // 1,048,576 tokens 318 us (1.07: it only reads); one of 300 tokens 6.5 us.
 // About 10 us of a large call do not stream: 2 us until a CTA knows its share,
@@ -63,9 +63,11 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;          // tokens per warp and stage
 constexpr int kMinTiles = kWarps;  // tiles per CTA below which fewer CTAs run
-// Units up to this long are not split while each has a CTA: 8 units of 32 tiles
-// take 10.6 us, as long as split; of 19 tiles 8.1 against 12.9 us.
-constexpr int kWholeTiles = 32;
+// Units up to this long are not split while each has a CTA.  8 units of 20 tiles
+// take 8.5 us, 9.7 split; of 25 tiles 10.2 against 9.8, of 32 tiles 11.0 against
+// 10.7, 48 units of 32 tiles 14.8 against 12.4; with 16 heads to a unit 12.0
+// against 14.6, 14.1 against 15.3, 15.1 against 14.8.
+constexpr int kWholeTiles = 24;
 // Units up to this long, and up to four times as long as there are units per
 // CTA, go to a warp each: 2400 units of 1-4 tiles 17 against 29 us, of 1-10
 // tiles 28 against 38, but 512 units of 10 tiles 20 against 16 us.
@@ -76,12 +78,11 @@ constexpr int kUnitCost = 8, kUnitCostSolo = 2;
 // Where a unit has CTAs of its own: in microseconds, a tile takes a CTA kTileUs,
 // a part its join kPartUs per head and dim, and a join in two steps (of groups of
 // parts, then of the groups; more than kOneJoin parts) kTwoStepsUs on top.  One
-// kv head, 4 query heads, of 16384, 65536, 262144 tokens: 14, 24, 43 us with the
-// parts that pay in one step, 19, 45, 52 with one for every CTA, 16, 21, 28 so in
-// two steps; 16 query heads 25, 43, 77; 49, 119, 128; 30, 36, 46.
+// kv head, 4 query heads, of 16384, 65536, 262144 tokens: 14, 25, 51 us with the
+// parts that pay in one step, 19, 44, 51 with one for every CTA, 15, 19, 25 so in
+// two steps; 16 query heads 25, 44, 77; 44, 102, 111; 26, 35, 44.
 constexpr float kTileUs = 0.21f, kPartUs = 0.025f / 128.f, kTwoStepsUs = 6.f;
 constexpr int kOneJoin = 64;
-constexpr int kJoinUnroll = 8;     // parts whose sums a join loads together
 constexpr int kFewParts = 4;       // parts of a unit that its last CTA joins without publishing its own
 constexpr int kLensCached = 1024;  // lengths kept in shared memory
 constexpr size_t kStatusBytes = 256;
@@ -315,46 +316,66 @@ struct Join {
 
 // Joins published parts first, first + step, .. (`parts` of them) of a unit, all
 // threads together, into slot `dest` or, where that is negative, the output.
-// `ml` holds `room` (R, l) pairs in shared memory: they are brought there first,
-// so that the sums' loads wait for nothing.
+// `room` bytes at `mine`, the warp's own, take as many parts at a time as they
+// hold: each lane copies the 16 bytes of every sum that it adds up, so that the
+// loads of a whole round are in flight at once without registers of their own
+// (9 sequences of 7007 tokens, one kv head of 8 query heads: 17.0 us, and 20.4 with
+// eight loads at a time in registers; of 28000 tokens, 8 kv heads of 16: 101, 107).
 template <int D, int kItems>
 __device__ __forceinline__ void join_published(const KvqDecodeArgs& a, const Join& j, int first, int step, int parts,
-                                               int dest, long long out_row, float2* ml, int room) {
-  const int G = a.group, most = room / G;
+                                               int dest, long long out_row, uint8_t* mine, int room) {
+  constexpr int kHeads = 128 / D;  // heads of a warp's 32 items
+  const int G = a.group, lane = threadIdx.x & 31;
+  const int items = (G * (D / 4) + kThreads - 1) / kThreads;  // of a thread, at most
+  const int most = room / (items * (512 + 8 * kHeads));
+  float2* const ml = reinterpret_cast<float2*>(mine + most * items * 512);
+  const uint32_t to = smem_addr(mine) + lane * 16;
+  const int h0 = threadIdx.x / (D / 4), hw = (threadIdx.x & ~31) / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  constexpr int kHeadStep = kThreads / (D / 4);  // from a thread's item to its next
   float4 x[kItems];
   float top[kItems], L[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) join_start(top[k], L[k], x[k]);
-  for (int pass = 0; pass < 2; ++pass)  // the largest R, then the sums
-    for (int p0 = 0; p0 < parts; p0 += most) {
-      const int np = min(most, parts - p0);
-      if (pass == 0 || parts > most) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < np * G; i += kThreads)
-          ml[i] = __ldcg(a.part_ml + (long long)j.slot(first + (p0 + i / G) * step) * G + i % G);
-        __syncthreads();
-      }
+  for (int p0 = 0; p0 < parts; p0 += most) {
+    const int np = min(most, parts - p0);
+    for (int i = 0; i < np; ++i) {
+      const long long row = (long long)j.slot(first + (p0 + i) * step) * G;
 #pragma unroll
-      for (int k = 0; k < kItems; ++k) {
-        const int item = threadIdx.x + k * kThreads;
-        if (item >= G * (D / 4)) continue;
-        const int h = item / (D / 4), d = item % (D / 4) * 4;
-        if (pass == 0) {
-          for (int i = 0; i < np; ++i) top[k] = fmaxf(top[k], ml[i * G + h].x);
-        } else {
-#pragma unroll kJoinUnroll
-          for (int i = 0; i < np; ++i)
-            join_add(top[k], L[k], x[k], ml[i * G + h],
-                     __ldcg(reinterpret_cast<const float4*>(
-                         a.part_acc + ((long long)j.slot(first + (p0 + i) * step) * G + h) * D + d)));
-        }
-      }
+      for (int k = 0; k < kItems; ++k)
+        if (h0 + k * kHeadStep < G)
+          cp_async16<0, 0>(to + (i * items + k) * 512, a.part_acc + (row + h0 + k * kHeadStep) * D + d);
     }
+    cp_async_commit();
+    for (int i = lane; i < np * items * kHeads; i += 32) {
+      const int p = i / (items * kHeads), r = i - p * (items * kHeads), h = hw + r / kHeads * kHeadStep + r % kHeads;
+      if (h < G) ml[i] = __ldcg(a.part_ml + (long long)j.slot(first + (p0 + p) * step) * G + h);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      if (h0 + k * kHeadStep >= G) continue;
+      float m = top[k];
+      for (int i = 0; i < np; ++i) m = fmaxf(m, ml[(i * items + k) * kHeads + h0 - hw].x);
+      const float f = top[k] == m ? 1.f : ex2_ftz(top[k] - m);
+      top[k] = m;
+      L[k] *= f;
+      x[k] = make_float4(x[k].x * f, x[k].y * f, x[k].z * f, x[k].w * f);
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      if (h0 + k * kHeadStep >= G) continue;
+#pragma unroll 4
+      for (int i = 0; i < np; ++i)
+        join_add(top[k], L[k], x[k], ml[(i * items + k) * kHeads + h0 - hw],
+                 *reinterpret_cast<const float4*>(mine + (i * items + k) * 512 + lane * 16));
+    }
+    __syncwarp();
+  }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const int item = threadIdx.x + k * kThreads;
-    if (item >= G * (D / 4)) continue;
-    const int h = item / (D / 4), d = item % (D / 4) * 4;
+    const int h = h0 + k * kHeadStep;
+    if (h >= G) continue;
     if (dest < 0) {
       const float inv = 1.f / L[k];
       *reinterpret_cast<uint2*>(a.o + (out_row + h) * D + d) =
@@ -976,17 +997,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       return last;
     };
     constexpr int kItems = (NG * 8 * D / 4 + kThreads - 1) / kThreads;
-    float2* const ml = reinterpret_cast<float2*>(smem + s_idle[0]);
+    // no copy is under way where each CTA has one part
+    uint8_t* const mine = few ? ring : ring + idle * C::kStageBytes;
+    const int room = few ? C::kWarpBytes : C::kStageBytes;
     if (j.parts <= kOneJoin) {
       if (last_of(counter, j.parts))
-        join_published<D, kItems>(a, j, 0, 1, j.parts, -1, out_row, ml, C::kStageBytes / 8);
+        join_published<D, kItems>(a, j, 0, 1, j.parts, -1, out_row, mine, room);
     } else {
       const int size = (int)ceilf(sqrtf((float)j.parts)), lead = (j.own / 2 - j.first / 2) / size * size;
       const int groups = (j.parts + size - 1) / size, here = min(size, j.parts - lead), dest = j.slot(lead);
       if (last_of(a.group_counters + dest, here)) {
-        join_published<D, kItems>(a, j, lead, 1, here, dest, out_row, ml, C::kStageBytes / 8);
+        join_published<D, kItems>(a, j, lead, 1, here, dest, out_row, mine, room);
         if (last_of(counter, groups))
-          join_published<D, kItems>(a, j, 0, size, groups, -1, out_row, ml, C::kStageBytes / 8);
+          join_published<D, kItems>(a, j, 0, size, groups, -1, out_row, mine, room);
       }
     }
     __syncthreads();  // s_flag and the idle stages are free again
