@@ -14,15 +14,13 @@
 //    turns a tile of P into the second operand.  At one byte per element the
 //    cache itself is the bound, and eight heads share each product, so the
 //    5th-generation path (128-row tiles, TMEM) has nothing to win here.
-//  * int8 K codes are multiplied as they are: q 2^k, rounded to 23 bits, is
-//    written as three signed base-256 digits once per unit, and the products
-//    are exact in int32 (at most 2^-22 of the head's largest |q| is lost per
-//    dim, and nothing of a bf16 q within 2^-14 of it).  e4m3 products of this
-//    kind would be taken apart into fp16 ones, once per digit, so e4m3 codes
-//    are converted to fp16 (exact), and q 2^k too (exact within 2^-29).
-//  * V codes become fp16 in registers, exactly (int8 by setting the exponent
-//    byte, 0x6400 | code + 128 is 1152 + code, and one subtraction), after
-//    ldmatrix has transposed the bytes.
+//  * K codes become fp16 in registers, exactly (int8 by setting the exponent
+//    byte, 0x6400 | code + 128 is 1152 + code, and one subtraction), and so does
+//    q 2^k (exactly within 2^-29 of the head's largest).  8-bit products instead
+//    were slower: of int8 codes with q in three base-256 digits, 128 query heads
+//    109 against 101 us, one sequence of 300 tokens 6.7 against 6.4; of e4m3, which
+//    are taken apart into fp16 ones once per digit, 99 against 87.
+//  * V codes become fp16 the same way, after ldmatrix has transposed the bytes.
 //  * ks multiplies the fp32 scores, vs the fp32 weights.  Weights are rounded
 //    to fp16 (2^-12 each on average, below bf16's 2^-8 of the output); R
 //    follows the largest s_t + log2 vs_t, so that weights keep 32 binary orders
@@ -39,7 +37,7 @@
 //
 // Measured (head_dim 128, 8 kv heads, int8 where not said): 64 sequences of
 // 4096 tokens 88 us, 0.96 of the copy rate of 6534 GB/s (e4m3 87 us; 64 query
-// heads 90 us; 128 query heads 109 us, e4m3 98 us, bound by the products' issue
+// heads 90 us; 128 query heads 101 us, e4m3 97 us, bound by the products' issue
 // and latency with eight warps per SM), of 8192 tokens 167 us (1.02); one of
 // 1,048,576 tokens 318 us (1.07: it only reads); one of 300 tokens 6.5 us.
 // About 10 us of a large call do not stream: 2 us until a CTA knows its share,
@@ -139,13 +137,6 @@ __device__ __forceinline__ void mma_f16(float c[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 32 products per row on the codes as they are.
-__device__ __forceinline__ void mma_s8(int c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -189,60 +180,11 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
-// q as the second operand, kWords registers per four dims.  m: the head's
-// largest |q| as bf16 magnitude bits; factor() brings a score back.
-template <int FMT>
-struct Query;
-
-// Three signed base-256 digits of q 2^-e, which is below 2^22.
-template <>
-struct Query<LARA_KVQ_INT8> {
-  static constexpr int kWords = 3;
-  static __device__ __forceinline__ int exponent(uint32_t m) { return max((int)(m >> 7) - 127, -100) - 21; }
-  static __device__ __forceinline__ float factor(int e) { return __uint_as_float((uint32_t)(127 + e + 8) << 23); }
-  static __device__ __forceinline__ void split(const float x[4], uint32_t out[3]) {
-    uint32_t d[3][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int v = __float2int_rn(x[i]);
-      const int v1 = (v + 128) >> 8, v2 = (v1 + 128) >> 8;  // digits in [-128, 127]
-      d[0][i] = v;
-      d[1][i] = v1;
-      d[2][i] = v2;
-    }
-#pragma unroll
-    for (int p = 0; p < 3; ++p)
-      out[p] = __byte_perm(__byte_perm(d[p][0], d[p][1], 0x0040), __byte_perm(d[p][2], d[p][3], 0x0040), 0x5410);
-  }
-  // K q^T of 16 tokens (rows a and b of D / 16 words per lane), in units of 2^8
-  template <int D, int NG>
-  static __device__ __forceinline__ void scores(float (*s)[4], const uint32_t* a, const uint32_t* b,
-                                                const uint32_t (*q)[D / 16][3]) {
-    int acc[NG][3][4];
-#pragma unroll
-    for (int n = 0; n < NG; ++n)
-#pragma unroll
-      for (int i = 0; i < 12; ++i) acc[n][i / 4][i % 4] = 0;
-#pragma unroll
-    for (int j = 0; j < D / 16; j += 2) {
-      const uint32_t x[4] = {a[j], b[j], a[j + 1], b[j + 1]};
-#pragma unroll
-      for (int n = 0; n < NG; ++n)
-#pragma unroll
-        for (int p = 0; p < 3; ++p) mma_s8(acc[n][p], x, q[n][j][p], q[n][j + 1][p]);
-    }
-#pragma unroll
-    for (int n = 0; n < NG; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)  // below 2^29; the lowest digits' sum rounded down to the unit
-        s[n][i] = (float)(acc[n][2][i] * 256 + acc[n][1][i] + (acc[n][0][i] >> 8));
-  }
-};
-
-// q 2^-e, below 2^15, in fp16.
-template <>
-struct Query<LARA_KVQ_FP8_E4M3> {
-  static constexpr int kWords = 2;
+// q 2^-e, below 2^15, in fp16 as the second operand, two registers per four
+// dims.  m: the head's largest |q| as bf16 magnitude bits; factor() brings a
+// score back.
+template <int FMT, int NG>
+struct Query {
   static __device__ __forceinline__ int exponent(uint32_t m) { return max((int)(m >> 7) - 127, -100) - 14; }
   static __device__ __forceinline__ float factor(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
   static __device__ __forceinline__ void split(const float x[4], uint32_t out[2]) {
@@ -252,7 +194,7 @@ struct Query<LARA_KVQ_FP8_E4M3> {
       out[i] = reinterpret_cast<const uint32_t&>(h);
     }
   }
-  template <int D, int NG>
+  template <int D>
   static __device__ __forceinline__ void scores(float (*s)[4], const uint32_t* a, const uint32_t* b,
                                                 const uint32_t (*q)[D / 16][2]) {
 #pragma unroll
@@ -260,8 +202,8 @@ struct Query<LARA_KVQ_FP8_E4M3> {
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       uint32_t a0, a1, a2, a3;
-      codes_to_f16<LARA_KVQ_FP8_E4M3>(a[j], a0, a2);
-      codes_to_f16<LARA_KVQ_FP8_E4M3>(b[j], a1, a3);
+      codes_to_f16<FMT>(a[j], a0, a2);
+      codes_to_f16<FMT>(b[j], a1, a3);
 #pragma unroll
       for (int n = 0; n < NG; ++n) mma_f16(s[n], a0, a1, a2, a3, q[n][j][0], q[n][j][1]);
     }
@@ -411,7 +353,7 @@ template <int D, int FMT, int NG>
 __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     kvq_decode_kernel(const __grid_constant__ KvqDecodeArgs a) {
   using C = Cfg<D, NG>;
-  using Q = Query<FMT>;
+  using Q = Query<FMT, NG>;
   constexpr int KS = D / 16;   // dim blocks of the output
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long s_sum[kWarps];
@@ -677,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     const int end = tiles_end(u);
     // q of the group's heads as the 8-column operand: column g, this lane's
     // dims D / 4 t4 .., which are those of its K chunks
-    uint32_t qf[NG][D / 16][Q::kWords];
+    uint32_t qf[NG][D / 16][2];
     float2 qs[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -742,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
             *reinterpret_cast<uint4*>(k[r] + 4 * c) =
                 *reinterpret_cast<const uint4*>(st + k_at[r][c] + mb * 16 * D);
         float s[NG][4];
-        Q::template scores<D, NG>(s, k[0], k[1], qf);
+        Q::template scores<D>(s, k[0], k[1], qf);
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           s2[2 * mb][n] = make_float2(s[n][0], s[n][1]);
