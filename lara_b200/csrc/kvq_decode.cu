@@ -39,7 +39,7 @@
 // 4096 tokens 88 us, 0.96 of the copy rate of 6534 GB/s (e4m3 87 us; 64 query
 // heads 90 us; 128 query heads 101 us, e4m3 97 us, bound by the products' issue
 // and latency with eight warps per SM), of 8192 tokens 167 us (1.02); one of
-// 1,048,576 tokens 318 us (1.07: it only reads); one of 300 tokens 6.5 us.
+// 1,048,576 tokens 318 us (1.07: it only reads); one of 300 tokens 6.4 us.
 // About 10 us of a large call do not stream: 2 us until a CTA knows its share,
 // 3 us until its first rows arrive, and at the end CTAs finish over 10 us.
 // Three stages with two CTAs per SM, separate K and V slots (K fetched two
@@ -70,8 +70,14 @@ constexpr int kWholeTiles = 24;
 // CTA, go to a warp each: 2400 units of 1-4 tiles 17 against 29 us, of 1-10
 // tiles 28 against 38, but 512 units of 10 tiles 20 against 16 us.
 constexpr int kSoloTiles = 16;
+// Units up to this long, more than CTAs, go to CTAs whole: shares end between
+// units (8 query heads and 16, by head blocks).  512 units of 7 tiles 12.9 us,
+// 14.3 cut, of 16 tiles 18.7 as cut, of 24 tiles 25.9 against 23.4; with 16 heads
+// 16.1 against 22.9, 22.6 against 28.6, 29.9 against 35.8, of 47 tiles as cut.
+constexpr int kUncutTiles[2] = {16, 24};
 // What a unit costs beside its tiles, in tiles, where shares are measured out
-// (2400 units of 1-10 tiles: 38 us; 78 us without).
+// (2400 units of 1-10 tiles: 38 us; 78 us without), for each block of eight
+// heads (2400 units of 1-47 tiles, 16 heads: 127 us; 147 with 8, 130 with 24).
 constexpr int kUnitCost = 8, kUnitCostSolo = 2;
 // Where a unit has CTAs of its own: in microseconds, a tile takes a CTA kTileUs,
 // a part its join kPartUs per head and dim, and a join in two steps (of groups of
@@ -451,13 +457,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
   if (total == 0) return;
   // How the tiles are shared.  Short units, each with a CTA: one each.  Few
   // units: as many CTAs for a unit as it has tiles for, none with parts of two.
-  // Short units, more than CTAs: whole ones to each warp (solo).  Else equal
-  // shares for each CTA, across units, with a cost of its own for each unit.
+  // Short units, more than CTAs: whole ones to each warp (solo) or CTA (uncut).
+  // Else equal shares for each CTA, across units, with a cost of its own for each
+  // unit.
   const long long units = (long long)some * hkv;
   const bool one_each = longest <= kWholeTiles && (long long)a.batch * hkv <= gridDim.x;
   const bool few = !one_each && units * 8 <= gridDim.x;
   const bool solo = !one_each && !few && longest <= kSoloTiles && (long long)longest * gridDim.x <= 4 * units;
-  if (!one_each && !few) gap = solo ? kUnitCostSolo : kUnitCost;
+  const bool uncut = !one_each && !few && !solo && longest <= kUncutTiles[NG - 1];
+  const bool entire = solo || uncut;  // a share has the units that start in it
+  if (!one_each && !few) gap = solo ? kUnitCostSolo : NG * kUnitCost;
   int share;
   if (one_each) {
     const int b = blockIdx.x / hkv;
@@ -518,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       }
       u.kvh = (int)quotient(x - at, u.tiles + gap);
       u.base = (int)(at + (long long)u.kvh * (u.tiles + gap) + gap - x);  // at most gap
-      if (solo && u.base < gap) next_unit(u);  // it belongs to the share that it starts in
+      if (entire && u.base < gap) next_unit(u);  // it belongs to the share that it starts in
       s_first[w] = u;
     }
   }
@@ -526,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
   const Unit u0 = s_first[solo ? warp : 0];
   const int step = solo ? 1 : kWarps, offset = solo ? 0 : warp;
   // a unit starts in this share / its tiles of this share are [max(base, 0), tiles_end)
-  auto in_share = [&](const Unit& u) { return share > 0 && (solo ? u.base - gap : u.base) < share; };
-  auto tiles_end = [&](const Unit& u) { return solo ? u.base + u.tiles : min(share, u.base + u.tiles); };
+  auto in_share = [&](const Unit& u) { return share > 0 && (entire ? u.base - gap : u.base) < share; };
+  auto tiles_end = [&](const Unit& u) { return entire ? u.base + u.tiles : min(share, u.base + u.tiles); };
 
   // ---- the warp's ring ----
   uint8_t* const ring = smem + warp * C::kWarpBytes;
@@ -828,7 +837,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     }
     // join the warps: R and l, then the scaled sums
     if (lane == 0) s_idle[warp] = warp * C::kWarpBytes + idle * C::kStageBytes;
-    const bool whole = u.base >= 0 && u.base + u.tiles <= share;
+    const bool whole = uncut || (u.base >= 0 && u.base + u.tiles <= share);
     // a unit of several CTAs: which ones, and whether all others are done
     Join j{0, 1, 0};
     if (!whole) {

@@ -931,6 +931,24 @@ def test_decode_shares(fmt, D, G, B, hkv, n):
     assert torch.equal(o, _decode_gpu(case, q))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,G", [(128, 5), (128, 16), (64, 8), (64, 9)])
+@pytest.mark.parametrize("B,hkv,n,filled", [(90, 8, 510, 90), (41, 16, 512, 40), (900, 1, 700, 66), (700, 1, 480, 699)])
+def test_decode_whole_units(fmt, D, G, B, hkv, n, filled):
+    """Units too short to be cut, more than CTAs; and fewer, of a batch that is mostly empty."""
+    g = torch.Generator().manual_seed(B + D + G)
+    lens = torch.zeros(B, dtype=torch.int64)
+    lens[torch.randperm(B, generator=g)[:filled]] = torch.randint(n // 2, n + 1, (filled,), generator=g)
+    lens = lens.tolist()
+    k, v = _rand_bf16(g, (1, hkv, n, D)), _rand_bf16(g, (1, hkv, n, D))
+    case = SharedRows(lens, hkv, D, 32, fmt, k[0], v[0], seed=n)
+    q = _rand_bf16(g, (B, hkv * G, D), False).to(DEV)
+    o = _decode_gpu(case, q)
+    case.check(q, o)
+    assert torch.equal(o, _decode_gpu(case, q))
+
+
 class SharedRows(Case):
     """Every sequence holds the first rows of one K and V; written page by page."""
 
