@@ -67,17 +67,18 @@ constexpr int kMinTiles = kWarps;  // tiles per CTA below which fewer CTAs run
 // against 14.6, 14.1 against 15.3, 15.1 against 14.8.
 constexpr int kWholeTiles = 24;
 // Units up to this long, and up to four times as long as there are units per
-// CTA, go to a warp each: 2400 units of 1-4 tiles 17 against 29 us, of 1-10
-// tiles 28 against 38, but 512 units of 10 tiles 20 against 16 us.
+// CTA, go to a warp each: 2400 units of 1-4 tiles 17 us, 26 by CTA, of 1-10 tiles
+// 29 against 35; 512 units of 7 tiles would take 16 us against 13.
 constexpr int kSoloTiles = 16;
 // Units up to this long, more than CTAs, go to CTAs whole: shares end between
 // units (8 query heads and 16, by head blocks).  512 units of 7 tiles 12.9 us,
 // 14.3 cut, of 16 tiles 18.7 as cut, of 24 tiles 25.9 against 23.4; with 16 heads
 // 16.1 against 22.9, 22.6 against 28.6, 29.9 against 35.8, of 47 tiles as cut.
 constexpr int kUncutTiles[2] = {16, 24};
-// What a unit costs beside its tiles, in tiles, where shares are measured out
-// (2400 units of 1-10 tiles: 38 us; 78 us without), for each block of eight
-// heads (2400 units of 1-47 tiles, 16 heads: 127 us; 147 with 8, 130 with 24).
+// What a unit costs beside its tiles, in tiles, where shares are measured out, for
+// each block of eight heads: 2400 units of 1-47 tiles 85 us, 94 with 4, 123 with
+// none; with 16 heads 126 us (8 per block), 146, 219.  Where units go to a warp:
+// 2400 of 1-10 tiles 29 us, 31 with none, 30 with 4; with 16 heads 40, 55, 40.
 constexpr int kUnitCost = 8, kUnitCostSolo = 2;
 // Where a unit has CTAs of its own: in microseconds, a tile takes a CTA kTileUs,
 // a part its join kPartUs per head and dim, and a join in two steps (of groups of
