@@ -73,7 +73,8 @@ constexpr int kSoloTiles = 16;
 // Units up to this long, more than CTAs, go to CTAs whole: shares end between
 // units (8 query heads and 16, by head blocks).  512 units of 7 tiles 12.9 us,
 // 14.3 cut, of 16 tiles 18.7 as cut, of 24 tiles 25.9 against 23.4; with 16 heads
-// 16.1 against 22.9, 22.6 against 28.6, 29.9 against 35.8, of 47 tiles as cut.
+// 16.1 against 22.9, 22.6 against 28.6, 29.9 against 35.8, of 47 tiles 47 against
+// 51, but 904 of them 86 against 79.
 constexpr int kUncutTiles[2] = {16, 24};
 // What a unit costs beside its tiles, in tiles, where shares are measured out, for
 // each block of eight heads: 2400 units of 1-47 tiles 85 us, 94 with 4, 123 with
