@@ -21,11 +21,15 @@
 //    109 against 101 us, one sequence of 300 tokens 6.7 against 6.4; of e4m3, which
 //    are taken apart into fp16 ones once per digit, 99 against 87.
 //  * V codes become fp16 the same way, after ldmatrix has transposed the bytes.
-//  * ks multiplies the fp32 scores, vs the fp32 weights.  Weights are rounded
-//    to fp16 (2^-12 each on average, below bf16's 2^-8 of the output); R
-//    follows the largest s_t + log2 vs_t, so that weights keep 32 binary orders
-//    below the largest one whatever the scales are.  R moves only when a weight
-//    would pass 2^15, and by whole powers of two, so most tiles rescale nothing.
+//  * ks multiplies the fp32 scores, vs the fp32 weights.  A weight is the sum of
+//    two fp16 numbers, the second what the first leaves, and what both leave is
+//    2^-22 of it: one alone leaves 2^-11, which shows wherever values nearly cancel
+//    in an output.  The second product costs up to eight heads 1 % (64 x 4096 tokens
+//    87.9 -> 88.6 us), 16 heads, bound by the products, 12 % (100.3 -> 112.6; e4m3
+//    97.0 -> 103.8).  R follows the largest s_t + log2 vs_t, so that weights keep 32
+//    binary orders below the largest one whatever the scales are.  R moves only when
+//    a weight would pass 2^15, and by whole powers of two, so most tiles rescale
+//    nothing.
 //
 // Work is split by the kernel itself, so that no plan from the host depends on
 // the lengths: all (sequence, kv head) units are laid end to end in tiles of 32
@@ -761,8 +765,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
           }
       }
 
-      // ---- weights, as the second operand: tokens 4 t4 .. + 3 of column g ----
-      uint32_t pf[4][NG];
+      // ---- weights, as the second operand: tokens 4 t4 .. + 3 of column g.  What fp16
+      // leaves of a weight is a second one ----
+      uint32_t pf[4][NG], pr[4][NG];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -773,7 +778,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
           l2[n] = add2(l2[n], p);
           const float2 wv = mul2(p, make_float2(vsc[i], vsc[i]));
           const __half2 w = __floats2half2_rn(wv.x, wv.y);
+          const float2 back = __half22float2(w);
+          const __half2 rest = __floats2half2_rn(wv.x - back.x, wv.y - back.y);
           pf[i][n] = transpose8x8(reinterpret_cast<const uint32_t&>(w));
+          pr[i][n] = transpose8x8(reinterpret_cast<const uint32_t&>(rest));
         }
 
       // ---- O^T += V^T P^T: block c holds dims 16 c + g and 16 c + g + 8 ----
@@ -790,7 +798,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
             codes_to_f16<FMT>(v[2 * i], a0, a2);
             codes_to_f16<FMT>(v[2 * i + 1], a1, a3);
 #pragma unroll
-            for (int n = 0; n < NG; ++n) mma_f16(o[n][c + i], a0, a1, a2, a3, pf[2 * mb][n], pf[2 * mb + 1][n]);
+            for (int n = 0; n < NG; ++n) {
+              mma_f16(o[n][c + i], a0, a1, a2, a3, pf[2 * mb][n], pf[2 * mb + 1][n]);
+              mma_f16(o[n][c + i], a0, a1, a2, a3, pr[2 * mb][n], pr[2 * mb + 1][n]);
+            }
           }
         }
       }

@@ -1,0 +1,63 @@
+"""Closer checks of the 8-bit KV cache operators and the q/k head pass than worst-case sums over all tokens.
+
+``attend64_close`` bounds the decode by what its sums are: a weight is two fp16 numbers (2^-20 of itself, the
+exponential's error with it), a score 136 fp32 roundings (2^-24 of ``sum_d |q_d k_d|``, twice: above and below the
+line), the sums over tokens chains of ``chain`` fp32 additions (2^-23 of ``kappa = sum_t p_t |v_t|``), weights too
+small for fp16's last place 2^-30 of the row's largest kappa each, and one bf16 rounding at the end (2^-8).
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_kvquant import DEV, FORMATS, Case, _decode_gpu, _rand_bf16  # noqa: E402
+
+
+# ------------------------------------------------------------------ bounds
+def attend64_close(q, k, v, scale, chain):
+    """q [G, D], k/v [n, D] float64 -> (o [G, D], absolute tolerance [G, D])."""
+    n = k.shape[0]
+    s = (q @ k.T) * scale
+    mag = (q.abs() @ k.abs().T) * scale
+    p = torch.softmax(s, -1)
+    o, kappa = p @ v, p @ v.abs()
+    rel = 2.0 ** -20 + 2 * 136 * 2.0 ** -24 * mag.amax(-1, keepdim=True) + chain * 2.0 ** -23
+    return o, 2.0 ** -8 * o.abs() + rel * kappa + n * 2.0 ** -30 * kappa.amax(-1, keepdim=True) + 2.0 ** -133
+
+
+def check_close(case, q, o, chain, scale=None):
+    sc = 1.0 / math.sqrt(case.D) if scale is None else scale
+    G = q.shape[1] // case.hkv
+    o, q = o.double().cpu(), q.double().cpu()
+    for b, n in enumerate(case.lens):
+        for h in range(case.hkv):
+            got = o[b, h * G:(h + 1) * G]
+            if n == 0:
+                assert torch.count_nonzero(got) == 0
+                continue
+            ref, tol = attend64_close(q[b, h * G:(h + 1) * G], case.k64[b][h], case.v64[b][h], sc, chain)
+            assert ((got - ref).abs() <= tol).all(), (b, h, n, ((got - ref).abs() / tol).max())
+
+
+# ------------------------------------------------------------------ decode
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,G", [(128, 1), (128, 4), (128, 8), (128, 16), (64, 3), (64, 9)])
+def test_decode_weights_keep_more_than_fp16(fmt, D, G):
+    """Two tokens of nearly equal weight and opposite values: what is left is the weights' difference.
+
+    Scores of a few tenths out of two dims, so that their roundings stay below those of an fp16 weight.
+    """
+    g = torch.Generator().manual_seed(D + G)
+    B, hkv = 40, 2
+    k = torch.zeros((B, hkv, 2, D))
+    k[..., 0] = 1.0
+    k[..., 1] = torch.randint(-2, 3, (B, hkv, 2), generator=g) * 2.0 ** -6
+    v = _rand_bf16(g, (B, hkv, 1, D)).float()
+    case = Case([2] * B, hkv, D, 16, fmt, k_rows=k.to(torch.bfloat16), v_rows=torch.cat([v, -v], 2).to(torch.bfloat16))
+    q = (0.2 * torch.randn((B, hkv * G, D), generator=g) * math.sqrt(D)).to(torch.bfloat16).to(DEV)
+    check_close(case, q, _decode_gpu(case, q), chain=8)
