@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(kThreads) kvq_append_kernel(const __grid_const
   allow_dependent_launch();
   grid_dependency_wait();
   if (a.new_lens)
-    for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.batch; b += gridDim.x * kThreads) {
+    for (long long b = blockIdx.x * (long long)kThreads + threadIdx.x; b < a.batch;
+         b += gridDim.x * (long long)kThreads) {  // a large grid has more than 2^31 threads
       const int start = a.starts[b];
       const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
       a.new_lens[b] = start < 0 ? start : (int)min(end, max(a.index.capacity(), (long long)start));

@@ -46,7 +46,8 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
   grid_dependency_wait();
   const long long cap = a.index.capacity();
   if (a.new_lens)
-    for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.batch; b += gridDim.x * kThreads) {
+    for (long long b = blockIdx.x * (long long)kThreads + threadIdx.x; b < a.batch;
+         b += gridDim.x * (long long)kThreads) {  // a large grid has more than 2^31 threads
       const int start = a.starts[b];
       const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
       a.new_lens[b] = start < 0 ? start : (int)min(end, max(cap, (long long)start));

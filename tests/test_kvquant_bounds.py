@@ -61,3 +61,61 @@ def test_decode_weights_keep_more_than_fp16(fmt, D, G):
     case = Case([2] * B, hkv, D, 16, fmt, k_rows=k.to(torch.bfloat16), v_rows=torch.cat([v, -v], 2).to(torch.bfloat16))
     q = (0.2 * torch.randn((B, hkv * G, D), generator=g) * math.sqrt(D)).to(torch.bfloat16).to(DEV)
     check_close(case, q, _decode_gpu(case, q), chain=8)
+
+
+# ------------------------------------------------------------------ append: grids of more than 2^31 threads
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _large_batch(B):
+    """starts 0 .. 14, counts 0 but for a few, a table whose every sequence has page 0, and those with rows their own."""
+    starts = torch.arange(B, dtype=torch.int32, device=DEV) % 15
+    counts = torch.zeros(B, dtype=torch.int32, device=DEV)
+    table = torch.zeros((B, 1), dtype=torch.int32, device=DEV)
+    some = [0, 1, B // 2, B - 2, B - 1]
+    counts[some] = 1
+    table[some, 0] = torch.arange(len(some), dtype=torch.int32, device=DEV)
+    return starts, counts, table, some
+
+
+@pytest.mark.gpu
+def test_append_lengths_of_a_large_grid():
+    """One row each of 2^26 - 1 sequences: the grid has 2^31 threads, and each length is written once."""
+    from lara_b200 import kvquant, ops
+
+    B = 2 ** 26 - 1
+    starts, counts, table, some = _large_batch(B)
+    pool = kvquant.QuantPool.empty(len(some), 16, 1, 64, "int8", DEV)
+    row = torch.arange(64, device=DEV).to(torch.bfloat16)
+    x = row.expand(B, 1, 1, 64)
+    new, st = torch.full_like(starts, -7), ops.new_workspace(256, DEV)
+    kvquant.kvq_append(pool, table, starts, x, x, counts=counts, new_lens=new, workspace=st)
+    assert ops.workspace_status(st) == 0
+    assert torch.equal(new, starts + counts)
+    for i, b in enumerate(some):
+        at = int(starts[b])
+        assert torch.count_nonzero(pool.k_scales[i, 0]) == 1 and torch.count_nonzero(pool.v_codes[i, 0].sum(-1)) == 1
+        assert torch.equal(pool.k_codes[i, 0, at], torch.round(127.0 * row.float() / 63.0).to(torch.int8))
+
+
+@pytest.mark.gpu
+def test_append_qkv_lengths_of_a_large_grid():
+    """One token each of 2^27 sequences, three heads of sixteen lanes: more than 2^32 threads."""
+    from lara_b200 import kvquant, ops
+
+    B, D = 2 ** 27, 128
+    starts, counts, table, some = _large_batch(B)
+    pool = kvquant.QuantPool.empty(len(some), 16, 1, D, "int8", DEV)
+    row = torch.arange(D, device=DEV).to(torch.bfloat16)
+    x = row.expand(B, 1, 1, D)
+    out = torch.empty((B, 1, 1, D), dtype=torch.bfloat16, device=DEV)
+    tab = torch.cat([torch.ones((16, 4), device=DEV), torch.zeros((16, 4), device=DEV)], -1)  # a turn by nothing
+    new, st = torch.full_like(starts, -7), ops.new_workspace(256, DEV)
+    kvquant.kvq_append_qkv(pool, table, starts, x, x, x, cos_sin=tab, counts=counts, new_lens=new, workspace=st, out=out)
+    assert ops.workspace_status(st) == 0
+    assert torch.equal(new, starts + counts)
+    for i, b in enumerate(some):
+        assert torch.equal(out[b, 0, 0], row)
+        assert torch.count_nonzero(pool.k_scales[i, 0]) == 1
+        assert torch.equal(pool.k_codes[i, 0, int(starts[b])], torch.round(127.0 * row.float() / 127.0).to(torch.int8))
