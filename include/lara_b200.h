@@ -371,7 +371,8 @@ typedef struct lara_kvq_pool {
  * as it is; new_lens (NULL, or int32[B] apart from starts and counts) receives
  * starts + counts, at most the capacity.  Rows past the capacity or naming a
  * bad page are dropped and flagged in the workspace status word (workspace may
- * be NULL: no status), as is a count outside [0, n_new] (it is clamped). */
+ * be NULL: no status), as is a count outside [0, n_new] (it is clamped).  At most
+ * 2^30 tokens, and batch * n_kv_heads * ceil(n_new / (512 / head_dim)) < 2^31. */
 LARA_API int lara_kvq_append(const lara_kvq_pool* pool, const int32_t* block_table, int pages_per_seq,
                              const int32_t* starts, const int32_t* counts, int32_t* new_lens, const uint16_t* k_new,
                              long long k_sb, long long k_sh, long long k_st, const uint16_t* v_new, long long v_sb,
@@ -399,7 +400,8 @@ LARA_API int lara_kvq_append_qkv(const lara_kvq_pool* pool, const int32_t* block
  * starts[b] + t (starts NULL: t) of sequence b for t in [0, n_tokens); zeros
  * for tokens at or past seq_lens[b].  The contiguous result is a cache that
  * lara_gqa_prefill and the other bf16 kernels take.  A bad page reads as zeros
- * and is flagged, as is a length past the capacity (clamped). */
+ * and is flagged, as is a length past the capacity (clamped).  At most as many
+ * rows as lara_kvq_append takes. */
 LARA_API int lara_kvq_read(const lara_kvq_pool* pool, const int32_t* block_table, int pages_per_seq,
                            const int32_t* seq_lens, const int32_t* starts, uint16_t* k_out, long long k_sb,
                            long long k_sh, long long k_st, uint16_t* v_out, long long v_sb, long long v_sh,

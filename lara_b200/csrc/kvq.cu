@@ -75,7 +75,7 @@ struct WarpRows {
   int t0, cross;
   long long start, base, base2;
   __device__ __forceinline__ bool init(const RowArgs& a) {
-    const uint32_t w = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / 32;
+    const uint32_t w = blockIdx.x * (uint32_t)(kThreads / 32) + threadIdx.x / 32;  // below 2^31, unlike the thread's index
     if (w >= a.tiles) return false;
     uint32_t tile;
     const uint32_t bh = a.div_tiles.div(w, tile);
@@ -220,22 +220,22 @@ Access access_of(const void* p, long long sb, int batch, long long sh, int heads
   return bytes >= 32 ? kFull : bytes >= 16 ? kHalf : kElement;
 }
 
-// Whether the rows of a call (at least one per warp) fit one launch.
+// Whether the rows of a call fit one launch: warps are counted in 31 bits, and so
+// are the positions up to a warp's last.
 bool set_rows(RowArgs* a, const lara_kvq_pool& pool, int batch, int n) {
   a->pool = pool;
   a->batch = batch;
   a->n = n;
   a->div_h = FastDiv((uint32_t)pool.n_kv_heads);
-  return (long long)batch * pool.n_kv_heads <= 0x3ffffffll &&
-         (long long)batch * pool.n_kv_heads * n <= 0x3ffffffll;
+  const int tokens = 512 / pool.head_dim;  // a warp's
+  const uint32_t tiles = ((uint32_t)n + tokens - 1) / tokens;
+  if (n > 1 << 30 || (tiles > 0 && (long long)batch * pool.n_kv_heads > 0x7fffffffll / tiles)) return false;
+  a->div_tiles = FastDiv(std::max(tiles, 1u));
+  a->tiles = (uint32_t)batch * (uint32_t)pool.n_kv_heads * tiles;
+  return true;
 }
 
-template <int D>
 cudaError_t launch_rows(const void* kernel, RowArgs a, void* stream) {
-  constexpr int kTokens = 512 / D;  // a warp's
-  const int tiles = (a.n + kTokens - 1) / kTokens;
-  a.div_tiles = FastDiv((uint32_t)std::max(tiles, 1));
-  a.tiles = (uint32_t)((long long)a.batch * a.pool.n_kv_heads * tiles);
   const unsigned blocks = std::max(1u, (a.tiles + kThreads / 32 - 1) / (kThreads / 32));  // no rows: new_lens alone
   void* args[] = {&a};
   return launch_with_pdl(kernel, dim3(blocks), dim3(kThreads), args, 0, static_cast<cudaStream_t>(stream));
@@ -243,7 +243,7 @@ cudaError_t launch_rows(const void* kernel, RowArgs a, void* stream) {
 
 #define LARA_KVQ_LAUNCH(kernel, d, f, v)                            \
   if (pool->head_dim == d && pool->format == f && access == v)     \
-    e = launch_rows<d>(reinterpret_cast<const void*>(&kernel<d, f, v>), a, stream);
+    e = launch_rows(reinterpret_cast<const void*>(&kernel<d, f, v>), a, stream);
 #define LARA_KVQ_LAUNCH_ACCESS(kernel, d, f) \
   LARA_KVQ_LAUNCH(kernel, d, f, kElement) LARA_KVQ_LAUNCH(kernel, d, f, kHalf) LARA_KVQ_LAUNCH(kernel, d, f, kFull)
 #define LARA_KVQ_LAUNCH_ALL(kernel)                                                                       \

@@ -119,3 +119,59 @@ def test_append_qkv_lengths_of_a_large_grid():
         assert torch.equal(out[b, 0, 0], row)
         assert torch.count_nonzero(pool.k_scales[i, 0]) == 1
         assert torch.equal(pool.k_codes[i, 0, int(starts[b])], torch.round(127.0 * row.float() / 127.0).to(torch.int8))
+
+
+@pytest.mark.gpu
+def test_append_of_more_than_2_32_threads():
+    """2^20 sequences of 256 kv heads: 2^28 warps, the last of which write the last sequences' rows."""
+    from lara_b200 import kvquant, ops
+
+    B, hkv, D = 2 ** 20, 256, 64
+    starts, counts, table, some = _large_batch(B)
+    pool = kvquant.QuantPool.empty(len(some), 16, hkv, D, "int8", DEV)
+    rows = torch.randint(-127, 128, (hkv, 1, D), device=DEV)
+    rows[..., 0] = 127
+    x = rows.to(torch.bfloat16).expand(B, hkv, 1, D)
+    new, st = torch.full_like(starts, -7), ops.new_workspace(256, DEV)
+    kvquant.kvq_append(pool, table, starts, x, x, counts=counts, new_lens=new, workspace=st)
+    assert ops.workspace_status(st) == 0
+    assert torch.equal(new, starts + counts)
+    for i, b in enumerate(some):
+        for codes in (pool.k_codes, pool.v_codes):
+            assert torch.equal(codes[i, :, int(starts[b])], rows[:, 0].to(torch.int8))
+        assert torch.count_nonzero(pool.k_scales[i]) == hkv
+
+
+@pytest.mark.gpu
+def test_append_and_read_of_2_26_rows():
+    """64 sequences of 8 kv heads padded to 131072 tokens, of which the last has any."""
+    from lara_b200 import kvquant, ops
+
+    B, hkv, n, D, ps = 64, 8, 131072, 64, 256
+    table = torch.zeros((B, n // ps), dtype=torch.int32, device=DEV)
+    table[-1] = torch.randperm(n // ps, device=DEV).to(torch.int32)
+    pool = kvquant.QuantPool.empty(n // ps, ps, hkv, D, "int8", DEV)
+    rows = torch.randint(-127, 128, (n, D), device=DEV)
+    rows[:, 0] = 127
+    x = rows.to(torch.bfloat16).expand(B, hkv, n, D)
+    counts = torch.zeros(B, dtype=torch.int32, device=DEV)
+    counts[-1] = n
+    new, st = torch.full_like(counts, -7), ops.new_workspace(256, DEV)
+    kvquant.kvq_append(pool, table, torch.zeros_like(counts), x, x, counts=counts, new_lens=new, workspace=st)
+    assert torch.equal(new, counts)
+    k, v = kvquant.kvq_read(pool, table, new, n, workspace=st)
+    assert ops.workspace_status(st) == 0
+    for y in (k, v):
+        assert torch.equal(y[-1], x[-1]) and all(torch.count_nonzero(y[b]) == 0 for b in range(B - 1))
+
+
+def test_rows_past_one_launch_are_refused():
+    from test_kvquant import _append, _pool_struct, _read
+
+    pool = _pool_struct()  # 2 kv heads, head_dim 128: a warp takes four tokens
+    assert _append(pool, batch=1 << 12, n=1 << 20) == 0x01   # 2^31 warps
+    assert _read(pool, batch=1 << 12, n=1 << 20) == 0x01
+    assert _append(pool, batch=1 << 30, n=1) == 0x01
+    assert _append(pool, batch=1, n=(1 << 30) + 1) == 0x01
+    assert _append(pool, batch=0x7fffffff, n=0x7fffffff) == 0x01
+    assert _append(pool, batch=1 << 30, n=0, k=None, v=None, new_lens=None) == 0
