@@ -139,7 +139,7 @@ extern "C" int lara_qk_norm_rope(const uint16_t* q, long long q_sb, long long q_
   if (head_dim != 64 && head_dim != 128)
     return set_last_error(LARA_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
   if (batch < 0 || n < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads > 65535 || n_kv_heads > 65535 ||
-      (long long)batch * n * (n_q_heads + n_kv_heads) > 0x7fffffffll)
+      (long long)batch * n > 0x7fffffffll / (n_q_heads + n_kv_heads))
     return set_last_error(LARA_ERR_BAD_CFG, "bad geometry: batch, n >= 0, head counts in [1, 65535], below 2^31 heads in all");
   if (!q_weight != !k_weight) return set_last_error(LARA_ERR_BAD_CFG, "q_weight and k_weight go together");
   if (!q_weight && !cos_sin) return set_last_error(LARA_ERR_BAD_CFG, "neither norm weights nor a rotation table");

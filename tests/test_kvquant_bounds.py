@@ -175,3 +175,16 @@ def test_rows_past_one_launch_are_refused():
     assert _append(pool, batch=1, n=(1 << 30) + 1) == 0x01
     assert _append(pool, batch=0x7fffffff, n=0x7fffffff) == 0x01
     assert _append(pool, batch=1 << 30, n=0, k=None, v=None, new_lens=None) == 0
+
+
+# ------------------------------------------------------------------ q/k head pass
+def test_norm_rope_heads_past_31_bits_are_refused():
+    """Products of the sizes that pass 64 bits among them (2^30 * 2^30 * 16 is 0 there)."""
+    import ctypes
+
+    from lara_b200._native import lib
+
+    p, z = ctypes.c_void_p(4096), (0, 0, 0)
+    for batch, n in ((1 << 30, 1 << 30), (1 << 16, 1 << 14), (0x7fffffff, 0x7fffffff), (1, 1 << 28)):
+        assert lib.lara_qk_norm_rope(p, *z, p, *z, p, *z, p, *z, batch, n, 14, 2, 128, p, p, 16, 128, 1, p, p, 1e-5, None,
+                                     None) == 0x01
