@@ -99,6 +99,11 @@ constexpr size_t kStatusBytes = 256;
 
 // Weights lie in fp16 between 2^kStart (the largest, when R is set) and 2^kHigh.
 constexpr float kStart = 7.f, kHigh = 15.f;
+// No scale of V counts as less than 2^kFloor when R is set, so that a term of the
+// plain sum of 2^(s - R), which has no scale, is at most 2^(kHigh - kFloor): the
+// sum is finite up to 2^28 tokens of zeros.  The smallest scale, 2^-107, still has
+// its weights at 2^-15, 2^-10 of which fp16's last place is.
+constexpr float kFloor = -85.f;
 
 template <int D, int NG>
 struct Cfg {
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
       for (int i = 0; i < 4; ++i) {
         const float* sc = reinterpret_cast<const float*>(st + 2 * C::kRowsBytes) + tok_at + 16 * (i / 2) + 2 * (i & 1);
         vsc[i] = sc[kTile];
-        lw[i] = fmaxf(lg2_ftz(vsc[i]), -100.f);
+        lw[i] = fmaxf(lg2_ftz(vsc[i]), kFloor);
 #pragma unroll
         for (int n = 0; n < NG; ++n) s2[i][n] = mul2(mul2(s2[i][n], qs[n]), make_float2(sc[0], sc[0]));
       }
@@ -726,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
         for (int i = 0; i < 4; ++i)
           if (tok_at + 16 * (i / 2) + 2 * (i & 1) >= valid) {
             vsc[i] = 0.f;
-            lw[i] = -100.f;
+            lw[i] = kFloor;
 #pragma unroll
             for (int n = 0; n < NG; ++n) s2[i][n] = make_float2(-INFINITY, -INFINITY);
           }

@@ -188,3 +188,39 @@ def test_norm_rope_heads_past_31_bits_are_refused():
     for batch, n in ((1 << 30, 1 << 30), (1 << 16, 1 << 14), (0x7fffffff, 0x7fffffff), (1, 1 << 28)):
         assert lib.lara_qk_norm_rope(p, *z, p, *z, p, *z, p, *z, batch, n, 14, 2, 128, p, p, 16, 128, 1, p, p, 1e-5, None,
                                      None) == 0x01
+
+
+# ------------------------------------------------------------------ decode: scales of V far from one another
+def _page(rows, fmt):
+    """rows [tokens, D] of one page of one kv head -> (codes, scales, values in 64 bits)."""
+    from test_kvquant import DTYPES, quantise64, values64
+
+    c, s = quantise64(rows, fmt)
+    bits = c.to(torch.int8) if fmt == "int8" else c.float().to(torch.float8_e4m3fn)
+    return bits.view(DTYPES[fmt]), s.float(), values64(c, s.float().double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_decode_many_tokens_without_values(fmt):
+    """Hundreds of thousands of tokens whose V is zero, under rising scores, before as many whose V is one.
+
+    The score is 0 for the first page and 7.9 octaves after it: the sum of weights is at its largest.
+    """
+    from lara_b200 import kvquant, ops
+
+    B, D, ps, each = 64, 64, 256, 1536  # pages of zeros, pages of ones; every sequence has the same pages
+    k, v = torch.zeros((3, ps, D)), torch.zeros((3, ps, D))
+    k[1:, :, 0], v[2] = 1.0, 1.0
+    pages = [[_page(x[i].to(torch.bfloat16), fmt) for i in range(3)] for x in (k, v)]
+    codes = [torch.stack([p[0].view(torch.uint8) for p in q])[:, None].to(DEV).view(q[0][0].dtype) for q in pages]
+    scales = [torch.stack([p[1] for p in q])[:, None].to(DEV) for q in pages]
+    pool = kvquant.QuantPool(*codes, *scales)
+    table = torch.tensor([0] + [1] * each + [2] * each, dtype=torch.int32, device=DEV).expand(B, -1).contiguous()
+    lens = torch.full((B,), table.shape[1] * ps, dtype=torch.int32, device=DEV)
+    q = torch.zeros((B, 2, D), dtype=torch.bfloat16, device=DEV)
+    q[..., 0] = 1.0
+    ws = kvquant.decode_workspace(B, 2, 1, D, DEV)
+    o = kvquant.gqa_decode_kvq(q, pool, table, lens, scale=7.9 * math.log(2.0), workspace=ws)
+    assert ops.workspace_status(ws) == 0
+    assert ((o.double() - each / (2 * each + 2.0 ** -7.9)).abs() <= 2.0 ** -8 * 0.5).all()
