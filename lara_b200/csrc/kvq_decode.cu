@@ -102,7 +102,9 @@ constexpr float kStart = 7.f, kHigh = 15.f;
 // No scale of V counts as less than 2^kFloor when R is set, so that a term of the
 // plain sum of 2^(s - R), which has no scale, is at most 2^(kHigh - kFloor): the
 // sum is finite up to 2^28 tokens of zeros.  The smallest scale, 2^-107, still has
-// its weights at 2^-15, 2^-10 of which fp16's last place is.
+// its weights at 2^-15, 2^-10 of which fp16's last place is.  At the other end, a
+// term is 0 below 2^-126: with scales of V up to 2^100 (values up to 1e32) that is
+// a token 33 octaves less likely than the one that set R.
 constexpr float kFloor = -85.f;
 
 template <int D, int NG>
@@ -174,6 +176,17 @@ __device__ __forceinline__ float lg2_ftz(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Sums of tokens of zeros have terms up to 2^100, at an R so low that beside rows
+// of large values 2^(R - top) alone is below fp32.  l 2^d, f = 2^d, for a whole d <= 0:
+__device__ __forceinline__ float scale_down(float l, float f, float d) {
+  return f > 0.f ? l * f : l * 0x1p-126f * ex2_ftz(d + 126.f);
+}
+// and (R, l) as joins take it: what l has past 2^32 goes to R.
+__device__ __forceinline__ float2 to_join(float R, float l) {
+  const int e = max((int)(__float_as_uint(l) >> 23) - (127 + 32), 0);
+  return make_float2(R + (float)e, l * __uint_as_float((uint32_t)(127 - e) << 23));
 }
 
 // Bytes 0, 1 (lo) and 2, 3 (hi) of four codes as fp16 pairs.
@@ -759,8 +772,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
             for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
             if (m > R[n][c] + kHigh) {
               const float to = ceilf(m) - kStart, f = ex2_ftz(R[n][c] - to);
+              (c ? l2[n].y : l2[n].x) = scale_down(c ? l2[n].y : l2[n].x, f, R[n][c] - to);
               R[n][c] = to;
-              (c ? l2[n].y : l2[n].x) *= f;
 #pragma unroll
               for (int i = 0; i < KS; ++i) {
                 o[n][i][c] *= f;
@@ -879,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        if (g == 0) s_ml[warp][n * 8 + 2 * t4 + c] = make_float2(R[n][c], l[n][c]);
+        if (g == 0) s_ml[warp][n * 8 + 2 * t4 + c] = to_join(R[n][c], l[n][c]);
       }
     __syncthreads();
     const bool last_here = s_flag;

@@ -224,3 +224,20 @@ def test_decode_many_tokens_without_values(fmt):
     o = kvquant.gqa_decode_kvq(q, pool, table, lens, scale=7.9 * math.log(2.0), workspace=ws)
     assert ops.workspace_status(ws) == 0
     assert ((o.double() - each / (2 * each + 2.0 ** -7.9)).abs() <= 2.0 ** -8 * 0.5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lens,G,D", [([768], 4, 64), ([512] * 1800, 2, 64), ([40000], 3, 128), ([4100] * 90, 9, 64)])
+@pytest.mark.parametrize("large", [1e8, 1e20, 1e32])
+def test_decode_zero_values_beside_large_ones(fmt, lens, G, D, large):
+    """As many tokens of zeros as of large values, equally likely: in a warp's tiles, its neighbours', other CTAs'."""
+    from test_kvquant import SharedRows
+
+    n = max(lens)
+    g = torch.Generator().manual_seed(n)
+    k, v = torch.zeros((1, n, D)), large * torch.randn((1, n, D), generator=g)
+    k[:, :, 0], v[:, :n // 2] = 0.01 * torch.randn((1, n), generator=g), 0.0
+    case = SharedRows(lens, 1, D, 64, fmt, k.to(torch.bfloat16), v.to(torch.bfloat16), seed=n)
+    q = _rand_bf16(g, (len(lens), G, D), False).to(DEV)
+    check_close(case, q, _decode_gpu(case, q), chain=384)
