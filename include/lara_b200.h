@@ -385,7 +385,8 @@ LARA_API int lara_kvq_append(const lara_kvq_pool* pool, const int32_t* block_tab
  * int32[B * n_new].  Weights, cos_sin and the workspace as for
  * lara_qk_norm_rope (without weights and table k is stored as it is), starts,
  * counts and new_lens as for lara_kvq_append; q_out is written for all n_new
- * tokens. */
+ * tokens.  A token t >= counts[b] is padding: its position is not checked (the
+ * nearest table row is taken), and nothing of it is stored or flagged. */
 LARA_API int lara_kvq_append_qkv(const lara_kvq_pool* pool, const int32_t* block_table, int pages_per_seq,
                                  const int32_t* starts, const int32_t* counts, int32_t* new_lens, const uint16_t* q,
                                  long long q_sb, long long q_st, long long q_sh, const uint16_t* k, long long k_sb,

@@ -73,12 +73,14 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) load_words<W, kInter, kVec>(src + (i < heads ? i : 0) * in.sh, ld, w[i]);
   const int start = a.starts[b];
+  // tokens past the count are padding: nothing is stored or reported for them
+  auto given_count = [&] { return a.counts ? a.counts[b] : a.n; };
   if (kind != 2) {
     const float* row = nullptr;
     if (ld.rotated) {
       long long pos = a.positions ? a.positions[tok] : (long long)start + t;
       if (pos < 0 || pos >= a.max_pos) {
-        if (a.status) atomicOr(a.status, kDevBadPosition);
+        if (a.status && (int)t < given_count()) atomicOr(a.status, kDevBadPosition);
         pos = pos < 0 ? 0 : a.max_pos - 1;
       }
       row = a.cos_sin + pos * a.rot;
@@ -98,11 +100,8 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
   // where the token's first row lies: its heads are a page's rows apart
   long long dst = -1;
   if (heads > 0) {
-    int count = a.n;
-    if (a.counts) {
-      count = a.counts[b];
-      if ((count < 0 || count > a.n) && a.status) atomicOr(a.status, kDevBadLength);
-    }
+    const int count = given_count();
+    if ((count < 0 || count > a.n) && a.status) atomicOr(a.status, kDevBadLength);
     if ((int)t < count) {
       const long long pos = (long long)start + t;
       if (start < 0 || pos >= cap) {

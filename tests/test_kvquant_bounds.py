@@ -241,3 +241,31 @@ def test_decode_zero_values_beside_large_ones(fmt, lens, G, D, large):
     case = SharedRows(lens, 1, D, 64, fmt, k.to(torch.bfloat16), v.to(torch.bfloat16), seed=n)
     q = _rand_bf16(g, (len(lens), G, D), False).to(DEV)
     check_close(case, q, _decode_gpu(case, q), chain=384)
+
+
+# ------------------------------------------------------------------ the one-launch step: padding
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", [False, True])
+def test_append_qkv_positions_of_padding_are_not_reported(given):
+    """Ragged prompts padded past the rotation table; a counted row past it is reported."""
+    from lara_b200 import kvquant, ops
+
+    g = torch.Generator().manual_seed(3)
+    B, n, hq, hkv, D, max_pos = 3, 200, 4, 2, 64, 1000
+    x = _rand_bf16(g, (B, n, hq + 2 * hkv, D)).to(DEV)
+    args = (x[:, :, :hq], x[:, :, hq:hq + hkv], x[:, :, hq + hkv:])
+    table = torch.arange(3 * 20, dtype=torch.int32, device=DEV).view(3, 20)
+    pool = kvquant.QuantPool.empty(60, 64, hkv, D, "int8", DEV)
+    tab = ops.rope_table(max_pos, D, device=DEV)
+    starts = _i32([900, 0, 999])
+    pos = (starts[:, None] + torch.arange(n, dtype=torch.int32, device=DEV)) if given else None
+    if given:
+        pos[1, 150:] = -5
+    st, new = ops.new_workspace(256, DEV), _i32([0] * 3)
+    for counts, bits in (([100, 150, 1], 0), ([0, 0, 0], 0), ([101, 1, 1], 0x10), ([1, 1, 2], 0x10), ([-1, 201, 1], 0x2)):
+        if given and counts[1] > 150:
+            bits |= 0x10
+        kvquant.kvq_append_qkv(pool, table, starts, *args, positions=pos, cos_sin=tab, counts=_i32(counts), new_lens=new,
+                               workspace=st)
+        assert ops.workspace_status(st) == bits, counts
+        assert new.tolist() == [s + min(max(c, 0), n) for s, c in zip((900, 0, 999), counts)]
