@@ -413,8 +413,9 @@ LARA_API int lara_kvq_read(const lara_kvq_pool* pool, const int32_t* block_table
  * sequence of length 0 gives zeros.  Lengths stay on the device: the kernel
  * spreads the cached tokens over the SMs by itself, so no plan depends on
  * them.  Workspace: lara_kvq_decode_workspace_bytes, zeroed once by
- * lara_workspace_init; a workspace serves one stream at a time, one head
- * geometry and any batch up to the one it was sized for. */
+ * lara_workspace_init; a workspace serves one stream at a time, and any batch
+ * and heads that its size is enough for (the size does not depend on the
+ * batch; a smaller one is refused).  o may be q. */
 LARA_API size_t lara_kvq_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim);
 LARA_API int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool, const int32_t* block_table,
                                  int pages_per_seq, const int32_t* seq_lens, uint16_t* o, int batch, int n_q_heads,

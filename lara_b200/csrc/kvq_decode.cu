@@ -129,8 +129,8 @@ struct KvqDecodeArgs {
   int batch, n_q_heads, group;
   float scale_log2;
   int* status;
-  int* group_counters;  // [2 * grid] and
-  int* counters;        // [batch * Hkv], zero between launches
+  int* counters;        // [2 * grid], of a unit by its first slot, and
+  int* group_counters;  // [2 * grid], of a group of parts; zero between launches
   float2* part_ml;  // [2 * grid][group] (R, l)
   float* part_acc;  // [2 * grid][group][D]
 };
@@ -882,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
                  2 * (int)blockIdx.x + (u.base > 0 ? 1 : 0)};
       }
     }
-    int* const counter = a.counters + (long long)u.b * hkv + u.kvh;
+    int* const counter = a.counters + j.first;  // no other unit's
     if (threadIdx.x == 0) {
       const bool last = j.parts > 1 && j.parts <= kFewParts && load_acquire(counter) == j.parts - 1;
       if (last) *counter = 0;
@@ -999,27 +999,28 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
   cp_async_wait<0>();
 }
 
-// Workspace: status word | partial results (two slots per CTA) | counters.
-struct Layout {
-  size_t ml_off, acc_off, groups_off, counters_off, total;
-};
-
 template <int D, int NG>
 int max_ctas() {
   return device_sm_count() * Cfg<D, NG>::kCtasPerSm;
 }
 
-int max_ctas(int head_dim) { return head_dim == 128 ? max_ctas<128, 1>() : max_ctas<64, 1>(); }
+// Workspace: status word | counters | partial results (two slots per CTA).  The
+// counters lie at the same place for every batch and geometry, and no call writes
+// its partial results over them, so that a workspace serves any call that it is
+// large enough for.
+struct Layout {
+  size_t counters_off, groups_off, ml_off, acc_off, total;
+};
 
-Layout layout(int batch, int group, int n_kv_heads, int head_dim) {
+Layout layout(int group, int head_dim) {
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t slots = 2 * (size_t)max_ctas(head_dim);
+  const size_t slots = 2 * (size_t)std::max(max_ctas<64, 1>(), max_ctas<128, 1>());
   Layout w;
-  w.ml_off = kStatusBytes;
+  w.counters_off = kStatusBytes;
+  w.groups_off = w.counters_off + up(slots * sizeof(int));
+  w.ml_off = w.groups_off + up(slots * sizeof(int));
   w.acc_off = w.ml_off + up(slots * group * sizeof(float2));
-  w.groups_off = w.acc_off + up(slots * group * head_dim * sizeof(float));
-  w.counters_off = w.groups_off + up(slots * sizeof(int));
-  w.total = w.counters_off + up((size_t)batch * n_kv_heads * sizeof(int));
+  w.total = w.acc_off + up(slots * group * head_dim * sizeof(float));
   return w;
 }
 
@@ -1057,7 +1058,7 @@ using namespace lara;
 
 extern "C" size_t lara_kvq_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
   if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || head_dim < 1) return 0;
-  return layout(batch, (n_q_heads + n_kv_heads - 1) / n_kv_heads, n_kv_heads, head_dim).total;
+  return layout((n_q_heads + n_kv_heads - 1) / n_kv_heads, head_dim).total;
 }
 
 extern "C" int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool, const int32_t* block_table,
@@ -1077,7 +1078,7 @@ extern "C" int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool,
   if (!aligned(q, 16) || !aligned(o, 16) || !aligned(seq_lens, 4) || !aligned(workspace, 256))
     return set_last_error(LARA_ERR_STREAM_DEST, "q and o must be 16-byte aligned, the workspace 256-byte");
   a.group = n_q_heads / pool->n_kv_heads;
-  const Layout w = layout(batch, a.group, pool->n_kv_heads, pool->head_dim);
+  const Layout w = layout(a.group, pool->head_dim);
   if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "decode workspace too small");
   a.pool = *pool;
   a.q = q;

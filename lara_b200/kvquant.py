@@ -131,7 +131,7 @@ def kvq_read(pool: QuantPool, block_table, seq_lens, n_tokens: int, *, starts=No
 
 
 def decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device="cuda:0") -> torch.Tensor:
-    """A zeroed workspace for :func:`gqa_decode_kvq` calls with these heads and up to this batch.
+    """A zeroed workspace for :func:`gqa_decode_kvq` calls of any batch with these or fewer query heads per kv head.
 
     One stream at a time uses it.
     """
@@ -144,7 +144,8 @@ def gqa_decode_kvq(q, pool: QuantPool, block_table, seq_lens, *, scale=None, wor
     """One new token per sequence: ``q[B, Hq, D]`` (bf16) attends its cached tokens; returns ``o[B, Hq, D]``.
 
     ``Hq`` is any multiple of the pool's kv heads up to 16 per kv head.  A sequence of length 0 gives
-    zeros.  ``workspace`` comes from :func:`decode_workspace` (``None`` allocates one for the call).
+    zeros.  ``workspace`` comes from :func:`decode_workspace` (``None`` allocates one for the call).  ``out`` may be
+    ``q``.
     """
     if out is None:
         out = torch.empty_like(q)
@@ -215,9 +216,8 @@ class QuantKVCache(PagedKVCache):
         _check_words("q", q, (len(slots), q.shape[1], self.head_dim))
         _, table, lens = self._rows(slots)
         need = int(lib.lara_kvq_decode_workspace_bytes(len(slots), q.shape[1], self.n_kv_heads, self.head_dim))
-        if self._ws is None or self._ws_heads != q.shape[1] or self._ws.numel() < need:
+        if self._ws is None or self._ws.numel() < need:
             self._ws = decode_workspace(len(slots), q.shape[1], self.n_kv_heads, self.head_dim, self.device)
-            self._ws_heads = q.shape[1]
         return gqa_decode_kvq(q, self.pool, table, lens, scale=scale, workspace=self._ws)
 
     def read(self, slots=None, out=None):

@@ -14,7 +14,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_kvquant import DEV, FORMATS, Case, _decode_gpu, _rand_bf16  # noqa: E402
+from test_kvquant import DEV, FORMATS, Case, SharedRows, _decode_gpu, _rand_bf16  # noqa: E402
 
 
 # ------------------------------------------------------------------ bounds
@@ -232,8 +232,6 @@ def test_decode_many_tokens_without_values(fmt):
 @pytest.mark.parametrize("large", [1e8, 1e20, 1e32])
 def test_decode_zero_values_beside_large_ones(fmt, lens, G, D, large):
     """As many tokens of zeros as of large values, equally likely: in a warp's tiles, its neighbours', other CTAs'."""
-    from test_kvquant import SharedRows
-
     n = max(lens)
     g = torch.Generator().manual_seed(n)
     k, v = torch.zeros((1, n, D)), large * torch.randn((1, n, D), generator=g)
@@ -269,3 +267,36 @@ def test_append_qkv_positions_of_padding_are_not_reported(given):
                                workspace=st)
         assert ops.workspace_status(st) == bits, counts
         assert new.tolist() == [s + min(max(c, 0), n) for s, c in zip((900, 0, 999), counts)]
+
+
+# ------------------------------------------------------------------ decode: workspaces
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_decode_workspace_of_other_calls(fmt):
+    """One workspace, made for the most heads: every geometry, batch and way of joining after every other."""
+    from lara_b200 import kvquant, ops
+
+    g = torch.Generator().manual_seed(17)
+    cases = []
+    for lens, hkv, G, D in (([2000] * 70, 2, 16, 128), ([9000, 20], 1, 16, 128), ([6000], 2, 4, 64),
+                            ([2000] * 70, 2, 1, 128), ([30000], 1, 5, 64), ([700] * 200, 4, 12, 64),
+                            ([300], 8, 4, 128), ([40000], 1, 3, 128)):
+        rows = [_rand_bf16(g, (hkv, max(lens), D)) for _ in range(2)]
+        case = SharedRows(lens, hkv, D, 64, fmt, *rows, seed=len(lens))
+        q = _rand_bf16(g, (len(lens), hkv * G, D), False).to(DEV)
+        cases.append((case, q, _decode_gpu(case, q)))
+    ws = kvquant.decode_workspace(1, 16, 1, 128, DEV)
+    for i in torch.randperm(4 * len(cases), generator=g).tolist():
+        case, q, want = cases[i % len(cases)]
+        own = q.clone()
+        for query, out in ((q, torch.full_like(q, 3.0)), (own, own)):  # into another tensor, and into the queries
+            kvquant.gqa_decode_kvq(query, case.pool, case.dtable, case.dlens, workspace=ws, out=out)
+            assert torch.equal(out, want), i % len(cases)
+    assert ops.workspace_status(ws) == 0
+
+
+def test_decode_workspace_bytes_do_not_depend_on_the_batch():
+    from lara_b200._native import lib
+
+    b = lib.lara_kvq_decode_workspace_bytes
+    assert b(1, 32, 8, 128) == b(4096, 32, 8, 128) == b(7, 4, 1, 128) > b(1, 8, 8, 128) > 0
