@@ -5,10 +5,10 @@ object with ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` and
 links them into ``lara_b200/liblara_b200.so`` (cudart linked statically, so
 the library does not depend on which ``libcudart`` a host process has
 loaded).  Objects go to ``lara_b200/_build``; a source newer than the library
-triggers a rebuild.  ``csrc/binding.cpp``, the binding of the calls made once per
-layer and token, is compiled with g++ against the installed torch into
-``lara_b200/_binding.so`` (without torch it is left out: only the torch front end
-uses it).
+triggers a rebuild.  After it ``csrc/binding.cpp``, the binding of the calls made
+once per layer and token, is compiled with g++ against the installed torch into
+``lara_b200/_binding.so``; without what that needs (a torch with CUDA, g++,
+Python's headers) it is left out, and the library alone is built.
 """
 
 from __future__ import annotations
@@ -63,11 +63,27 @@ def _torch_include() -> Path | None:
     return Path(spec.origin).parent / "include" if spec and spec.origin else None
 
 
-def build_binding(force: bool = False) -> Path | None:
-    """Compile the Python binding; returns its path, or None without torch."""
-    src, inc = CSRC / "binding.cpp", _torch_include()
+def binding_lacks() -> str | None:
+    """What the Python binding needs and this machine has not, or None."""
+    inc = _torch_include()
     if inc is None:
+        return "torch is not installed"
+    if not (inc.parent / "lib" / "libc10_cuda.so").exists():
+        return "the installed torch has no CUDA"
+    if shutil.which("g++") is None:
+        return "g++ was not found"
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return "Python's headers are not installed"
+    return None
+
+
+def build_binding(force: bool = False) -> Path | None:
+    """Compile the Python binding; returns its path, or None where something for it is lacking."""
+    lacks = binding_lacks()
+    if lacks:
+        sys.stderr.write(f"lara_b200: {BINDING.name} is left out: {lacks}\n")
         return None
+    src, inc = CSRC / "binding.cpp", _torch_include()
     newest = max(p.stat().st_mtime for p in (src, INCLUDE / "lara_b200.h", Path(__file__)))
     if not force and BINDING.exists() and BINDING.stat().st_mtime > newest:
         return BINDING
@@ -98,7 +114,13 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile and link the library and its Python binding; returns the library's path."""
+    build_library(force, verbose)
     build_binding(force)
+    return LIB
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    """Compile and link the library; returns its path."""
     if not force and not needs_build():
         return LIB
     BUILD.mkdir(exist_ok=True)
