@@ -7,8 +7,9 @@ the library does not depend on which ``libcudart`` a host process has
 loaded).  Objects go to ``lara_b200/_build``; a source newer than the library
 triggers a rebuild.  After it ``csrc/binding.cpp``, the binding of the calls made
 once per layer and token, is compiled with g++ against the installed torch into
-``lara_b200/_binding.so``; without what that needs (a torch with CUDA, g++,
-Python's headers) it is left out, and the library alone is built.
+``lara_b200/_binding.<Python's tag>.so``, again whenever torch is another one;
+without what it needs (a torch with CUDA, g++, Python's headers) it is left out,
+and the library alone is built.
 """
 
 from __future__ import annotations
@@ -28,7 +29,7 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "liblara_b200.so"
-BINDING = PKG / "_binding.so"
+BINDING = PKG / ("_binding" + sysconfig.get_config_var("EXT_SUFFIX"))  # one Python's: another does not find it
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -85,17 +86,21 @@ def build_binding(force: bool = False) -> Path | None:
         return None
     src, inc = CSRC / "binding.cpp", _torch_include()
     newest = max(p.stat().st_mtime for p in (src, INCLUDE / "lara_b200.h", Path(__file__)))
-    if not force and BINDING.exists() and BINDING.stat().st_mtime > newest:
+    stamp, torch_is = BUILD / "binding.torch", (inc.parent / "version.py").read_text()
+    same_torch = stamp.exists() and stamp.read_text() == torch_is
+    if not force and BINDING.exists() and BINDING.stat().st_mtime > newest and same_torch:
         return BINDING
     cuda = Path(nvcc()).resolve().parents[1] / "include"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", "-I", str(inc), "-I",
            str(inc / "torch" / "csrc" / "api" / "include"), "-I", sysconfig.get_paths()["include"], "-I", str(cuda)]
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = BINDING.with_name(BINDING.name + ".tmp")
     libs = ["-L", str(inc.parent / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     res = subprocess.run([*cmd, str(src), "-o", str(tmp), *libs], capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, BINDING)
+    BUILD.mkdir(exist_ok=True)
+    stamp.write_text(torch_is)
     return BINDING
 
 

@@ -17,8 +17,11 @@ from ._native import check, lib
 
 try:
     from . import _binding
+
+    if _binding.torch_version != torch.__version__.split("+")[0]:
+        raise ImportError(f"it was built for torch {_binding.torch_version}, this is {torch.__version__}")
 except ImportError as e:
-    raise ImportError(f"lara_b200/_binding.so cannot be loaded ({e}); run `python -m lara_b200.build`") from e
+    raise ImportError(f"lara_b200._binding cannot be loaded ({e}); run `python -m lara_b200.build --force`") from e
 
 _binding.init(*(ctypes.cast(f, ctypes.c_void_p).value
                 for f in (lib.lara_qk_norm_rope, lib.lara_kvq_append, lib.lara_kvq_append_qkv, lib.lara_kvq_read,

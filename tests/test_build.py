@@ -53,3 +53,50 @@ def test_the_binding_is_left_out_without_what_it_needs(monkeypatch, no_library, 
     assert build.build() == no_library
     assert no_library.exists() and not (tmp_path / "_binding.so").exists()
     assert "left out" in capsys.readouterr().err
+
+
+def _fake_torch(monkeypatch, tmp_path):
+    root = tmp_path / "torch"
+    (root / "lib").mkdir(parents=True)
+    (root / "lib" / "libc10_cuda.so").write_bytes(b"")
+    monkeypatch.setattr(build, "_torch_include", lambda: root / "include")
+    return root / "version.py"
+
+
+def test_the_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    version = _fake_torch(monkeypatch, tmp_path)
+    out, built = tmp_path / build.BINDING.name, []
+    monkeypatch.setattr(build, "BINDING", out)
+    monkeypatch.setattr(build, "BUILD", tmp_path / "_build")
+
+    def compiler(cmd, **kw):
+        built.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "wb").close()
+        return build.subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    for text, times in (("__version__ = '2.11.0'", 1), ("__version__ = '2.11.0'", 1), ("__version__ = '2.12.0'", 2),
+                        ("__version__ = '2.12.0'", 2)):
+        version.write_text(text)
+        assert build.build_binding() == out and out.exists()
+        assert len(built) == times
+
+
+def test_the_binding_names_its_python_and_torch():
+    import sysconfig
+
+    import torch
+
+    from lara_b200 import _binding
+
+    assert build.BINDING.name.endswith(sysconfig.get_config_var("EXT_SUFFIX")) and "cpython" in build.BINDING.name
+    assert torch.__version__.startswith(_binding.torch_version)
+
+
+def test_a_binding_of_another_torch_is_refused():
+    import subprocess
+    import sys
+
+    code = "import torch; torch.__version__ = '1.0.0'; import lara_b200.ops as o; o.qk_norm_rope(torch.zeros(1), 0)"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=build.PKG.parent)
+    assert r.returncode != 0 and "built for torch" in r.stderr and "--force" in r.stderr
