@@ -15,17 +15,28 @@ import torch
 
 from ._native import check, lib
 
+
+class _NoBinding:
+    """Stands for a binding that cannot be loaded: its calls say so; all else works without it."""
+
+    def __init__(self, reason):
+        self._reason = reason
+
+    def __getattr__(self, name):
+        raise ImportError(f"lara_b200._binding cannot be loaded ({self._reason}); run "
+                          "`python -m lara_b200.build --force`")
+
+
 try:
     from . import _binding
 
     if _binding.torch_version != torch.__version__.split("+")[0]:
         raise ImportError(f"it was built for torch {_binding.torch_version}, this is {torch.__version__}")
+    _binding.init(*(ctypes.cast(f, ctypes.c_void_p).value
+                    for f in (lib.lara_qk_norm_rope, lib.lara_kvq_append, lib.lara_kvq_append_qkv, lib.lara_kvq_read,
+                              lib.lara_gqa_decode_kvq)))
 except ImportError as e:
-    raise ImportError(f"lara_b200._binding cannot be loaded ({e}); run `python -m lara_b200.build --force`") from e
-
-_binding.init(*(ctypes.cast(f, ctypes.c_void_p).value
-                for f in (lib.lara_qk_norm_rope, lib.lara_kvq_append, lib.lara_kvq_append_qkv, lib.lara_kvq_read,
-                          lib.lara_gqa_decode_kvq)))
+    _binding = _NoBinding(str(e))
 
 _WORD_DTYPES = (torch.bfloat16, torch.int16, torch.uint16)
 

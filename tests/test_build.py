@@ -97,6 +97,28 @@ def test_a_binding_of_another_torch_is_refused():
     import subprocess
     import sys
 
-    code = "import torch; torch.__version__ = '1.0.0'; import lara_b200.ops as o; o.qk_norm_rope(torch.zeros(1), 0)"
+    code = "import torch; torch.__version__ = '1.0.0'; import lara_b200.ops as o; x = torch.zeros((1, 1, 64)); o.qk_norm_rope(x, x)"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=build.PKG.parent)
     assert r.returncode != 0 and "built for torch" in r.stderr and "--force" in r.stderr
+
+
+def test_the_front_end_works_without_the_binding():
+    """Its own calls name what is missing; those that do not use it are there."""
+    import subprocess
+    import sys
+
+    code = """if True:
+        import sys
+        sys.modules["lara_b200._binding"] = None
+        import torch
+        from lara_b200 import kvquant, ops, paged, parallel
+        assert ops.Decoder and ops.gqa_prefill and paged.PagedKVCache and ops.rope_table(8, 8, device="cpu").shape == (8, 8)
+        x = torch.zeros((3, 2, 64), dtype=torch.bfloat16)
+        try:
+            ops.qk_norm_rope(x, x)
+        except ImportError as e:
+            print("refused:", e)
+    """
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=build.PKG.parent)
+    assert r.returncode == 0, r.stderr
+    assert "refused: lara_b200._binding cannot be loaded" in r.stdout and "lara_b200.build" in r.stdout
