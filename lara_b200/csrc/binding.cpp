@@ -82,13 +82,18 @@ int32_t* ints(PyObject* o, const char* name, int64_t n, int index) {
   return static_cast<int32_t*>(t.data_ptr());
 }
 
+int checked_int(int64_t n, const char* name) {
+  if (n > 0x7fffffff) throw BadValue(std::string(name) + " is too large");
+  return (int)n;
+}
+
 const int32_t* block_table(PyObject* o, int64_t batch, int index, int* pages) {
   const at::Tensor& t = tensor(o, "block_table");
   if (t.scalar_type() != at::kInt || index_of(t) != index || t.dim() != 2 || !t.is_contiguous())
     throw BadValue("block_table must be a contiguous int32 [batch, pages_per_seq] tensor on the pool's device");
   if (t.size(0) != batch)
     throw BadValue("block_table has " + std::to_string(t.size(0)) + " rows for a batch of " + std::to_string(batch));
-  *pages = (int)t.size(1);
+  *pages = checked_int(t.size(1), "block_table's pages per sequence");
   return static_cast<const int32_t*>(t.data_ptr());
 }
 
@@ -102,7 +107,8 @@ Table rope_table(PyObject* o, int index) {
   const at::Tensor& t = tensor(o, "cos_sin");
   if (t.scalar_type() != at::kFloat || index_of(t) != index || t.dim() != 2 || !t.is_contiguous())
     throw BadValue("cos_sin must be a contiguous float32 [max_pos, rot_dim] tensor on the same device");
-  return {static_cast<const float*>(t.data_ptr()), (int)t.size(0), (int)t.size(1)};
+  return {static_cast<const float*>(t.data_ptr()), checked_int(t.size(0), "cos_sin's positions"),
+          checked_int(t.size(1), "rot_dim")};
 }
 
 void* workspace(PyObject* o, int index, size_t* bytes = nullptr) {
@@ -145,11 +151,6 @@ bool truth(PyObject* o) {
 
 const lara_kvq_pool* pool_of(PyObject* o) {
   return reinterpret_cast<const lara_kvq_pool*>(static_cast<uintptr_t>(integer(o)));
-}
-
-int checked_int(int64_t n, const char* name) {
-  if (n > 0x7fffffff) throw BadValue(std::string(name) + " is too large");
-  return (int)n;
 }
 
 // Runs f; Python exceptions for C++ ones.
@@ -214,11 +215,12 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const float eps = (float)number(a[8]);
     const int inter = truth(a[9]), batch = checked_int(B, "batch"), tokens = checked_int(n, "n");
     const int hq = checked_int(qs[nd - 2], "heads"), hkv = checked_int(k_dims[nd - 2], "heads");
+    const int head_dim = checked_int(d, "head_dim");
     void* const ws = workspace(a[10], index);
     return launch(index, [&](void* stream) {
       return f_norm_rope(qp, q.stride(0), q.stride(nd - 3), q.stride(nd - 2), kp, k.stride(0), k.stride(nd - 3),
                          k.stride(nd - 2), qop, qo.stride(0), qo.stride(nd - 3), qo.stride(nd - 2), kop, ko.stride(0),
-                         ko.stride(nd - 3), ko.stride(nd - 2), batch, tokens, hq, hkv, (int)d, pos, table.p,
+                         ko.stride(nd - 3), ko.stride(nd - 2), batch, tokens, hq, hkv, head_dim, pos, table.p,
                          table.max_pos, table.rot, inter, qw, kw, eps, ws, stream);
     });
   });
@@ -228,7 +230,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded(n_args, 9, [&] {
     const lara_kvq_pool* pool = pool_of(a[0]);
-    const int index = (int)integer(a[1]);
+    const int index = checked_int(integer(a[1]), "device");
     const at::Tensor &k = tensor(a[4], "k_new"), &v = tensor(a[5], "v_new");
     if (k.dim() != 4) throw BadValue("k_new must be [B, Hkv, n, D]");
     const int64_t B = k.size(0), n = k.size(2);
@@ -255,7 +257,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 PyObject* append_qkv(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded(n_args, 17, [&] {
     const lara_kvq_pool* pool = pool_of(a[0]);
-    const int index = (int)integer(a[1]);
+    const int index = checked_int(integer(a[1]), "device");
     const at::Tensor &q = tensor(a[4], "q"), &k = tensor(a[5], "k"), &v = tensor(a[6], "v"), &qo = tensor(a[7], "out");
     if (q.dim() != 4) throw BadValue("q must be [B, n, Hq, D]");
     const int64_t B = q.size(0), n = q.size(1), hq = q.size(2), d = pool->head_dim;
@@ -291,7 +293,7 @@ PyObject* append_qkv(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded(n_args, 9, [&] {
     const lara_kvq_pool* pool = pool_of(a[0]);
-    const int index = (int)integer(a[1]);
+    const int index = checked_int(integer(a[1]), "device");
     const at::Tensor& lens = tensor(a[3], "seq_lens");
     const int64_t B = lens.numel(), n = integer(a[4]);
     const int64_t shape[4] = {B, pool->n_kv_heads, n, pool->head_dim};
@@ -315,7 +317,7 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded(n_args, 8, [&] {
     const lara_kvq_pool* pool = pool_of(a[0]);
-    const int index = (int)integer(a[1]);
+    const int index = checked_int(integer(a[1]), "device");
     const at::Tensor &q = tensor(a[2], "q"), &o = tensor(a[5], "out");
     if (q.dim() != 3) throw BadValue("q must be [B, Hq, D]");
     const int64_t B = q.size(0), hq = q.size(1);

@@ -300,3 +300,23 @@ def test_decode_workspace_bytes_do_not_depend_on_the_batch():
 
     b = lib.lara_kvq_decode_workspace_bytes
     assert b(1, 32, 8, 128) == b(4096, 32, 8, 128) == b(7, 4, 1, 128) > b(1, 8, 8, 128) > 0
+
+
+# ------------------------------------------------------------------ sizes past 32 bits in Python's calls
+@pytest.mark.gpu
+def test_sizes_past_32_bits_are_refused():
+    """2^32 + 128 must not be taken for 128; the tensors are empty and take no memory."""
+    from lara_b200 import kvquant, ops
+
+    big = (1 << 32) + 128
+    pool = kvquant.QuantPool.empty(2, 16, 1, 64, "int8", DEV)
+    none = torch.empty((0,), dtype=torch.int32, device=DEV)
+    rows = torch.empty((0, 1, 1, 64), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="pages per sequence is too large"):
+        kvquant.kvq_append(pool, torch.empty((0, big), dtype=torch.int32, device=DEV), none, rows, rows)
+    x = torch.empty((0, 1, big), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="head_dim is too large"):
+        ops.qk_norm_rope(x, x, cos_sin=torch.empty((4, 64), device=DEV), positions=none)
+    x = torch.empty((0, 1, 64), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="rot_dim is too large"):
+        ops.qk_norm_rope(x, x, cos_sin=torch.empty((0, big), device=DEV), positions=none)
