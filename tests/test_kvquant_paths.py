@@ -255,3 +255,38 @@ def test_append_qkv_in_64_bits(fmt, D, rot, interleaved, B, n, hq, hkv, half):
     for x, y in zip((turned, v), back):
         c, s = quantise64(x.transpose(1, 2).cpu(), fmt)
         assert torch.equal(y.cpu(), (c.float() * s.float()[..., None]).to(torch.bfloat16))
+
+
+# ------------------------------------------------------------------ the documented loop
+@pytest.mark.gpu
+def test_the_documented_serving_loop():
+    """INTEGRATION.md's loop over views of one projection output: every step appends behind the last one's token."""
+    import re
+    from pathlib import Path
+
+    from lara_b200 import kvquant, ops
+
+    text = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
+    code = next(c for c in re.findall(r"```python\n(.*?)```", text, re.S) if "decode_workspace" in c)
+    B, Hq, Hkv, D, ps = 3, 8, 2, 64, 16
+    g = torch.Generator().manual_seed(5)
+    x = _rows(g, B, 1, Hq + 2 * Hkv, D).to(DEV)
+    q, k, v = x[:, :, :Hq], x[:, :, Hq:Hq + Hkv], x[:, :, Hq + Hkv:]
+    pool = kvquant.QuantPool.empty(12, ps, Hkv, D, "int8", DEV)
+    table = torch.arange(12, dtype=torch.int32, device=DEV).view(B, 4)
+    lens = torch.tensor([0, 15, 20], dtype=torch.int32, device=DEV)
+    want = [int(n) for n in lens]
+    env = dict(torch=torch, kvquant=kvquant, ops=ops, B=B, Hq=Hq, Hkv=Hkv, D=D, pool=pool, block_table=table, lens=lens,
+               q=q, k=k, v=v, o=torch.empty((B, Hq, D), dtype=torch.bfloat16, device=DEV),
+               cos_sin=ops.rope_table(64, D, device=DEV))
+    exec(code, env)
+    for _ in range(2):
+        env["step"]()
+    assert lens.tolist() == [n + 3 for n in want]
+    vb = kvquant.kvq_read(pool, table, lens, 23)[1]
+    c, s = quantise64(v[:, 0].cpu(), "int8")
+    row = (c.float() * s.float()[..., None]).to(torch.bfloat16).to(DEV)
+    for b, n in enumerate(want):
+        for t in range(n, n + 3):
+            assert torch.equal(vb[b, :, t], row[b])
+    assert torch.isfinite(env["o"]).all()
