@@ -148,13 +148,16 @@ cudaError_t launch_heads(QkvArgs a, uint32_t tokens, cudaStream_t stream) {
                          grid, dim3(kThreads), args, 0, stream);
 }
 
-// Heads per lane group, on the grounds of qk_rope.cu.  32 + 8 + 8 heads
-// (head_dim 128, int8) of 64 single tokens take 2.7 us (the two calls 4.2), of
-// 2000 tokens 8.9 us (11.1), of 8192 tokens 37 us (41; 0.76 of the copy rate).
+// Heads per lane group, on the grounds of qk_rope.cu; the boundary by 32 + 8 + 8
+// heads (head_dim 128, int8) that would fill the GPU 0.6, 0.75, 1.2, 2 times: one each 3.5,
+// 3.5, 3.9, 5.5 us, four 3.9, 4.2, 4.6, 4.9 (8 + 2 + 2 heads of 64 dims: 3.3, 3.3, 3.8, 5.3
+// and 4.1, 3.7, 4.4, 5.4).  Those heads of 64 single tokens take 2.7 us (the two
+// calls 4.1), of 2000 tokens 8.4 us (10.2), of 8192 tokens 36 us (39; 0.78 of the
+// copy rate).
 template <int D, int W, int FMT, bool kInter, bool kNorm, bool kVec>
 cudaError_t launch(const QkvArgs& a, uint32_t tokens, cudaStream_t stream) {
   const double fill = (double)tokens * (a.hq + 2 * a.pool.n_kv_heads) * (D / 8) / (device_sm_count() * 2048.0);
-  return fill < 0.6 ? launch_heads<D, W, FMT, kInter, kNorm, kVec, 1>(a, tokens, stream)
+  return fill < 1.5 ? launch_heads<D, W, FMT, kInter, kNorm, kVec, 1>(a, tokens, stream)
                     : launch_heads<D, W, FMT, kInter, kNorm, kVec, 4>(a, tokens, stream);
 }
 

@@ -99,6 +99,8 @@ cudaError_t launch_heads(NormRopeArgs a, uint32_t tokens, cudaStream_t stream) {
 // 143 us; two 2.8, 4.6, 7.2, 132; four 2.8, 3.9, 6.2, 101; eight 3.0, 4.8, 5.4,
 // 93 us (1.0 of the copy rate; 102 us with inputs that no earlier call left in
 // L2).  8 dims per lane instead of 16: 1024 tokens 6.3, 2048 10.8 against 9.5 us.
+// Heads that leave the last group short lose by more of them: 8 + 2 heads of 64
+// dims at eight times the GPU's threads 13.4 us with two, 14.6, 15.7 with eight.
 template <int D, int W, bool kInter, bool kNorm, bool kVec>
 cudaError_t launch(const NormRopeArgs& a, uint32_t tokens, cudaStream_t stream) {
   const double fill = (double)tokens * (a.hq + a.hkv) * (D / 8) / (device_sm_count() * 2048.0);
