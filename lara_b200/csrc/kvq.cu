@@ -130,13 +130,15 @@ __global__ void __launch_bounds__(kThreads) kvq_append_kernel(const __grid_const
   constexpr int kLanes = D / 16, kGroups = 32 / kLanes;
   allow_dependent_launch();
   grid_dependency_wait();
-  if (a.new_lens)
-    for (long long b = blockIdx.x * (long long)kThreads + threadIdx.x; b < a.batch;
-         b += gridDim.x * (long long)kThreads) {  // a large grid has more than 2^31 threads
+  // a large grid has more than 2^31 threads: those of the first blocks write the lengths
+  if (a.new_lens && blockIdx.x <= (uint32_t)(a.batch - 1) / kThreads) {
+    const uint32_t b = blockIdx.x * (uint32_t)kThreads + threadIdx.x;
+    if (b < (uint32_t)a.batch) {
       const int start = a.starts[b];
       const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
       a.new_lens[b] = start < 0 ? start : (int)min(end, max(a.index.capacity(), (long long)start));
     }
+  }
   WarpRows<kGroups> rows;
   if (!rows.init(a)) return;
   const int l = threadIdx.x % kLanes, t = rows.t0 + (threadIdx.x & 31) / kLanes;
@@ -236,7 +238,9 @@ bool set_rows(RowArgs* a, const lara_kvq_pool& pool, int batch, int n) {
 }
 
 cudaError_t launch_rows(const void* kernel, RowArgs a, void* stream) {
-  const unsigned blocks = std::max(1u, (a.tiles + kThreads / 32 - 1) / (kThreads / 32));  // no rows: new_lens alone
+  // a thread for each length: without rows they alone are written
+  const unsigned blocks = std::max(((unsigned)a.batch + kThreads - 1) / kThreads,
+                                   (a.tiles + kThreads / 32 - 1) / (kThreads / 32));
   void* args[] = {&a};
   return launch_with_pdl(kernel, dim3(blocks), dim3(kThreads), args, 0, static_cast<cudaStream_t>(stream));
 }

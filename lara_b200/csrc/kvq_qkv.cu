@@ -45,13 +45,15 @@ __global__ void __launch_bounds__(kThreads) kvq_append_qkv_kernel(const __grid_c
   allow_dependent_launch();
   grid_dependency_wait();
   const long long cap = a.index.capacity();
-  if (a.new_lens)
-    for (long long b = blockIdx.x * (long long)kThreads + threadIdx.x; b < a.batch;
-         b += gridDim.x * (long long)kThreads) {  // a large grid has more than 2^31 threads
+  // a large grid has more than 2^31 threads: those of the first blocks write the lengths
+  if (a.new_lens && blockIdx.x <= (uint32_t)(a.batch - 1) / kThreads) {
+    const uint32_t b = blockIdx.x * (uint32_t)kThreads + threadIdx.x;
+    if (b < (uint32_t)a.batch) {
       const int start = a.starts[b];
       const long long end = (long long)start + (a.counts ? min(max(a.counts[b], 0), a.n) : a.n);
       a.new_lens[b] = start < 0 ? start : (int)min(end, max(cap, (long long)start));
     }
+  }
   if (a.tokens == 0) return;
   const uint32_t x = blockIdx.x;
   const int kind = x < a.blocks[0] ? 0 : x < a.blocks[0] + a.blocks[1] ? 1 : 2;  // q, k, v
@@ -142,7 +144,8 @@ cudaError_t launch_heads(QkvArgs a, uint32_t tokens, cudaStream_t stream) {
     a.blocks[i] = (tokens * chunks + per_block - 1) / per_block;
   }
   a.tokens = tokens;
-  const dim3 grid(std::max(1u, a.blocks[0] + 2 * a.blocks[1]));  // no tokens: new_lens alone
+  // a thread for each length: without tokens they alone are written
+  const dim3 grid(std::max(((unsigned)a.batch + kThreads - 1) / kThreads, a.blocks[0] + 2 * a.blocks[1]));
   void* args[] = {&a};
   return launch_with_pdl(reinterpret_cast<const void*>(&kvq_append_qkv_kernel<D, W, FMT, kInter, kNorm, kVec, kHeads>),
                          grid, dim3(kThreads), args, 0, stream);

@@ -320,3 +320,22 @@ def test_sizes_past_32_bits_are_refused():
     x = torch.empty((0, 1, 64), dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError, match="rot_dim is too large"):
         ops.qk_norm_rope(x, x, cos_sin=torch.empty((0, big), device=DEV), positions=none)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 127, 128, 129, 5000])
+def test_append_lengths_without_rows(B):
+    """n = 0: the lengths of every sequence, by as many blocks as they need."""
+    from lara_b200 import kvquant
+
+    pool = kvquant.QuantPool.empty(1, 16, 1, 64, "int8", DEV)
+    table = torch.zeros((B, 1), dtype=torch.int32, device=DEV)
+    starts = torch.arange(B, dtype=torch.int32, device=DEV) % 17
+    none = torch.empty((B, 1, 0, 64), dtype=torch.bfloat16, device=DEV)
+    new = torch.full_like(starts, -7)
+    kvquant.kvq_append(pool, table, starts, none, none, new_lens=new)
+    assert torch.equal(new, starts)
+    new.fill_(-7)
+    heads = none.transpose(1, 2)
+    kvquant.kvq_append_qkv(pool, table, starts, heads, heads, heads, new_lens=new)
+    assert torch.equal(new, starts)
