@@ -8,7 +8,7 @@
 * ``lara_b200.paged`` / ``lara_b200.kvquant`` -- paged KV caches in bf16 and in 8
   bits (int8, fp8 e4m3), with the decode that reads them.
 * ``lara_b200.workloads`` -- seeded synthetic inputs of the benchmark configs.
-* ``lara_b200.build`` -- compiles liblara_b200.so (nvcc) and the _binding.so of
+* ``lara_b200.build`` -- compiles liblara_b200.so (nvcc) and the _binding of
   the calls made once per layer and token, in-tree.
 
 The library is loaded by ``lara_b200._native`` (on first use of ``lib`` /

@@ -17,9 +17,9 @@
 //  * K codes become fp16 in registers, exactly (int8 by setting the exponent
 //    byte, 0x6400 | code + 128 is 1152 + code, and one subtraction), and so does
 //    q 2^k (exactly within 2^-29 of the head's largest).  8-bit products instead
-//    were slower: of int8 codes with q in three base-256 digits, 128 query heads
-//    109 against 101 us, one sequence of 300 tokens 6.7 against 6.4; of e4m3, which
-//    are taken apart into fp16 ones once per digit, 99 against 87.
+//    were slower (measured with weights of one fp16 number): of int8 codes with q
+//    in three base-256 digits, 128 query heads 109 against 101 us, one sequence of
+//    300 tokens 6.7 against 6.4; of e4m3 codes with q in e4m3 digits 99 against 87.
 //  * V codes become fp16 the same way, after ldmatrix has transposed the bytes.
 //  * ks multiplies the fp32 scores, vs the fp32 weights.  A weight is the sum of
 //    two fp16 numbers, the second what the first leaves, and what both leave is
@@ -40,10 +40,11 @@
 // few units are shared out otherwise, see below.
 //
 // Measured (head_dim 128, 8 kv heads, int8 where not said): 64 sequences of
-// 4096 tokens 88 us, 0.96 of the copy rate of 6534 GB/s (e4m3 87 us; 64 query
-// heads 90 us; 128 query heads 101 us, e4m3 97 us, bound by the products' issue
-// and latency with eight warps per SM), of 8192 tokens 167 us (1.02); one of
-// 1,048,576 tokens 318 us (1.07: it only reads); one of 300 tokens 6.4 us.
+// 4096 tokens 88 us, 0.97 of the copy rate of 6534 GB/s (e4m3 87 us; 64 query
+// heads 91 us; 128 query heads 114 us, e4m3 104 us, bound by the products' issue
+// and latency with eight warps per SM), of 8192 tokens 167 us (1.02; head_dim 64
+// 93 us, 0.94, of 4096 tokens 53 us, 0.82); one of 1,048,576 tokens 317 us (1.07: it
+// only reads); one of 300 tokens 6.5 us.
 // About 10 us of a large call do not stream: 2 us until a CTA knows its share,
 // 3 us until its first rows arrive, and at the end CTAs finish over 10 us.
 // Three stages with two CTAs per SM, separate K and V slots (K fetched two
@@ -66,31 +67,36 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;          // tokens per warp and stage
 constexpr int kMinTiles = kWarps;  // tiles per CTA below which fewer CTAs run
 // Units up to this long are not split while each has a CTA.  8 units of 20 tiles
-// take 8.5 us, 9.7 split; of 25 tiles 10.2 against 9.8, of 32 tiles 11.0 against
-// 10.7, 48 units of 32 tiles 14.8 against 12.4; with 16 heads to a unit 12.0
-// against 14.6, 14.1 against 15.3, 15.1 against 14.8.
+// take 8.5 us, 9.6 split; of 25 tiles 10.3 against 9.6, of 32 tiles 11.2 against
+// 10.7, 48 units of 32 tiles 16.1 against 12.4; with 16 heads to a unit 11.6
+// against 12.3, 13.7 against 14.4, 14.9 against 14.3, 19.3 against 16.1.
 constexpr int kWholeTiles = 24;
 // Units up to this long, and up to four times as long as there are units per
-// CTA, go to a warp each: 2400 units of 1-4 tiles 17 us, 26 by CTA, of 1-10 tiles
-// 29 against 35; 512 units of 7 tiles would take 16 us against 13.
+// CTA, go to a warp each: 2400 units of 1-4 tiles 18 us, 27 by CTA, of 1-10 tiles
+// 30 against 37; 512 units of 7 tiles would take 18 us against 14.
 constexpr int kSoloTiles = 16;
 // Units up to this long, more than CTAs, go to CTAs whole: shares end between
-// units (8 query heads and 16, by head blocks).  512 units of 7 tiles 12.9 us,
-// 14.3 cut, of 16 tiles 18.7 as cut, of 24 tiles 25.9 against 23.4; with 16 heads
-// 16.1 against 22.9, 22.6 against 28.6, 29.9 against 35.8, of 47 tiles 47 against
-// 51, but 904 of them 86 against 79.
+// units (8 query heads and 16, by head blocks).  512 units of 7 tiles 13.6 us,
+// 15.2 cut, of 16 tiles 20.2 against 19.7 (800 of them 23.9 against 27.6), of 17
+// 21.7 against 20.2, of 24 28.2 against 25.0; with 16 heads, of 16, 24, 25, 47 tiles
+// 24.8, 33.4, 35.3, 53 against 30.5, 38.2, 39.9, 56, but 904 of 47 tiles 96 against 89.
 constexpr int kUncutTiles[2] = {16, 24};
 // What a unit costs beside its tiles, in tiles, where shares are measured out, for
-// each block of eight heads: 2400 units of 1-47 tiles 85 us, 94 with 4, 123 with
-// none; with 16 heads 126 us (8 per block), 146, 219.  Where units go to a warp:
-// 2400 of 1-10 tiles 29 us, 31 with none, 30 with 4; with 16 heads 40, 55, 40.
+// each block of eight heads: 2400 units of 1-47 tiles 88 us, 98 with 4, 129 with
+// none; with 16 heads 142 us (8 per block), 158, 236.  Where units go to a warp:
+// 2400 of 1-10 tiles 30 us, 32 with none, 31 with 4; with 16 heads 45, 59, 45.
 constexpr int kUnitCost = 8, kUnitCostSolo = 2;
+// Units have CTAs of their own where each can have this many on average.  48 units of
+// 8000 tokens 23.2 us, 23.3 in equal shares (64 query heads 24.6 against 26.2), of 2000
+// tokens 13.3 against 12.6; 56 units of 8000 tokens 27.4 either way (29.0 against 30.2),
+// of 2000 tokens 14.1 against 13.2.
+constexpr int kFewCtas = 8;
 // Where a unit has CTAs of its own: in microseconds, a tile takes a CTA kTileUs,
 // a part its join kPartUs per head and dim, and a join in two steps (of groups of
 // parts, then of the groups; more than kOneJoin parts) kTwoStepsUs on top.  One
-// kv head, 4 query heads, of 16384, 65536, 262144 tokens: 14, 25, 51 us with the
-// parts that pay in one step, 19, 44, 51 with one for every CTA, 15, 19, 25 so in
-// two steps; 16 query heads 25, 44, 77; 44, 102, 111; 26, 35, 44.
+// kv head, 4 query heads, of 16384, 65536, 262144 tokens: 14, 26, 64 us with the
+// parts that pay in one step, 18, 42, 51 with one for every CTA, 15, 19, 26 so in
+// two steps; 16 query heads 24, 45, 82; 44, 105, 114; 25, 34, 44.
 constexpr float kTileUs = 0.21f, kPartUs = 0.025f / 128.f, kTwoStepsUs = 6.f;
 constexpr int kOneJoin = 64;
 constexpr int kFewParts = 4;       // parts of a unit that its last CTA joins without publishing its own
@@ -291,8 +297,9 @@ struct Join {
 // `room` bytes at `mine`, the warp's own, take as many parts at a time as they
 // hold: each lane copies the 16 bytes of every sum that it adds up, so that the
 // loads of a whole round are in flight at once without registers of their own
-// (9 sequences of 7007 tokens, one kv head of 8 query heads: 17.0 us, and 20.4 with
-// eight loads at a time in registers; of 28000 tokens, 8 kv heads of 16: 101, 107).
+// (9 sequences of 7007 tokens, one kv head of 8 query heads: 17.5 us; with weights of
+// one fp16 number 17.0, and 20.4 with eight loads at a time in registers; of 28000
+// tokens, 8 kv heads of 16: 104; 101 and 107).
 template <int D, int kItems>
 __device__ __forceinline__ void join_published(const KvqDecodeArgs& a, const Join& j, int first, int step, int parts,
                                                int dest, long long out_row, uint8_t* mine, int room) {
@@ -486,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm)
   // unit.
   const long long units = (long long)some * hkv;
   const bool one_each = longest <= kWholeTiles && (long long)a.batch * hkv <= gridDim.x;
-  const bool few = !one_each && units * 8 <= gridDim.x;
+  const bool few = !one_each && units * kFewCtas <= gridDim.x;
   const bool solo = !one_each && !few && longest <= kSoloTiles && (long long)longest * gridDim.x <= 4 * units;
   const bool uncut = !one_each && !few && !solo && longest <= kUncutTiles[NG - 1];
   const bool entire = solo || uncut;  // a share has the units that start in it
