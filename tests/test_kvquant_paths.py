@@ -260,7 +260,7 @@ def test_append_qkv_in_64_bits(fmt, D, rot, interleaved, B, n, hq, hkv, half):
 # ------------------------------------------------------------------ the documented loop
 @pytest.mark.gpu
 def test_the_documented_serving_loop():
-    """INTEGRATION.md's loop over views of one projection output: every step appends behind the last one's token."""
+    """The integration guide's loop over views of one projection output: every step appends behind the last one's token."""
     import re
     from pathlib import Path
 
