@@ -422,6 +422,66 @@ LARA_API int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool, c
                                  float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Many or long sequences in a paged bf16 cache (serving extensions; the      */
+/* reference attends one sequence out of BRAM, hw/rtl/mem/kv_cache_ram.sv).   */
+/* The caches are those of lara_gqa_decode_paged; head_dim 64 or 128, up to   */
+/* 16 query heads per kv head, q and o contiguous and 16-byte aligned,        */
+/* sequences of less than 2^30 tokens.  Lengths and tables stay on the        */
+/* device and nothing synchronises, so the calls can be captured.  A          */
+/* workspace (zeroed once by lara_workspace_init) serves one stream at a      */
+/* time and any call that it is large enough for; a length outside            */
+/* [0, capacity] and a bad page are flagged in its status word, the length    */
+/* clamped, page 0 read and nothing written for the bad page.                 */
+/* ------------------------------------------------------------------------ */
+
+/* lara_gqa_decode_paged for a batch whose sequences begin with the same pages:
+ * the first shared_pages entries of every row of block_table name the same
+ * pages, which are read once for all sequences that are at least that long
+ * (from row 0's entries), instead of once for each.  A sequence that ends
+ * within them is read through its own row, whatever that holds.  A sequence
+ * of length 0 gives zeros.  o may be q. */
+LARA_API size_t lara_decode_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim);
+LARA_API int lara_gqa_decode_shared(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
+                                    const int32_t* block_table, const int32_t* seq_lens, uint16_t* o, int batch,
+                                    int n_q_heads, int n_kv_heads, int head_dim, int page_size, int pages_per_seq,
+                                    int num_pages, int shared_pages, float scale, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* lara_gqa_decode_paged that also adds to each cached slot's weight what
+ * attention it got:
+ *   weights_out[slot] = weights[slot] + sum over the kv head's query heads of softmax(scale q.K)[slot]
+ * for the slots below seq_lens[b], fp32 [num_pages][Hkv][page_size]; others
+ * are left as they are.  weights_out may be weights.  The sequences of one
+ * call share no pages (where they do, the shared slots' weights are undefined,
+ * and where the pages named are more than the pool has, the rest is left
+ * as it is and flagged).  o may be q. */
+LARA_API size_t lara_decode_scored_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim,
+                                                   int page_size, int pages_per_seq, int num_pages);
+LARA_API int lara_gqa_decode_scored(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
+                                    const float* weights, float* weights_out, const int32_t* block_table,
+                                    const int32_t* seq_lens, uint16_t* o, int batch, int n_q_heads, int n_kv_heads,
+                                    int head_dim, int page_size, int pages_per_seq, int num_pages, float scale,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Cut every sequence of more than `keep` tokens down to `keep`, for each kv
+ * head by itself: its first `first` slots stay, its last `last`, and of the
+ * rest the heaviest (ties to the lowest slot; NaN is heavier than all).  Kept
+ * rows of K and V in slots from `keep` on move, in ascending order, into the
+ * slots below it that are given up, in ascending order, with their weights:
+ *   weights_out: kept slots' weights below `keep`, 0 from there to the old length
+ *   sources[b][h][j] (NULL, or int32 [B][Hkv][keep]): the slot that slot j's row came from
+ *                (j where it stayed, -1 at and past the new length)
+ *   new_lens[b] (NULL, or int32 [B], apart from seq_lens) = min(seq_lens[b], keep)
+ * seq_lens stays as it is; weights_out may be weights.  The order of the slots
+ * no longer is that of the positions, which no decode needs.  A page belongs to
+ * one sequence of the call.  keep >= 1, first + last <= keep. */
+LARA_API size_t lara_kv_evict_workspace_bytes(int batch, int n_kv_heads, int keep);
+LARA_API int lara_kv_evict(uint16_t* k_pages, uint16_t* v_pages, const float* weights, float* weights_out,
+                           const int32_t* block_table, const int32_t* seq_lens, int32_t* new_lens, int32_t* sources,
+                           int batch, int n_kv_heads, int head_dim, int page_size, int pages_per_seq, int num_pages,
+                           int keep, int first, int last, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Context API: the backing of the Python AttentionAccelerator.  The context */
 /* owns the HBM KV cache, device I/O buffers, a stream and timing events.   */
 /* Tensor pointers are host memory unless on_device != 0.                    */

@@ -134,6 +134,12 @@ SIGNATURES = {
     "lara_kvq_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "lara_gqa_decode_kvq": (c_int, [c_void_p, POINTER(LaraKvqPool), c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                                     c_float, c_void_p, c_size_t, c_void_p]),
+    "lara_decode_shared_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "lara_gqa_decode_shared": (c_int, [*([c_void_p] * 6), *([c_int] * 8), c_float, c_void_p, c_size_t, c_void_p]),
+    "lara_decode_scored_workspace_bytes": (c_size_t, [c_int] * 7),
+    "lara_gqa_decode_scored": (c_int, [*([c_void_p] * 8), *([c_int] * 7), c_float, c_void_p, c_size_t, c_void_p]),
+    "lara_kv_evict_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "lara_kv_evict": (c_int, [*([c_void_p] * 8), *([c_int] * 9), c_void_p, c_size_t, c_void_p]),
     "lara_create": (c_int, [c_int, POINTER(c_void_p)]),
     "lara_destroy": (c_int, [c_void_p]),
     "lara_configure_heads": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int]),

@@ -1,5 +1,6 @@
 // Python binding of the calls that run once per layer and token (the q/k head
-// pass and the 8-bit cache), for lara_b200.ops and lara_b200.kvquant.
+// pass, the 8-bit cache, the paged cache's serving operators), for
+// lara_b200.ops, lara_b200.kvquant and lara_b200.paged.
 //
 // A decode step's kernels take 3 to 7 us each, and checking six to nine tensors
 // in Python and converting up to forty arguments with ctypes took 7 to 11 us a
@@ -30,6 +31,9 @@ decltype(&lara_kvq_append) f_append = nullptr;
 decltype(&lara_kvq_append_qkv) f_append_qkv = nullptr;
 decltype(&lara_kvq_read) f_read = nullptr;
 decltype(&lara_gqa_decode_kvq) f_decode = nullptr;
+decltype(&lara_gqa_decode_shared) f_decode_shared = nullptr;
+decltype(&lara_gqa_decode_scored) f_decode_scored = nullptr;
+decltype(&lara_kv_evict) f_evict = nullptr;
 
 struct BadType : std::runtime_error {
   using std::runtime_error::runtime_error;
@@ -339,14 +343,149 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
-// The addresses of the five C entry points, in the order of this file.
+// A paged bf16 cache's pages and geometry.
+struct Pages {
+  uint16_t *k, *v;
+  int index, num_pages, hkv, page_size, head_dim;
+};
+
+Pages pages_of(PyObject* k_obj, PyObject* v_obj, bool written) {
+  const at::Tensor &k = tensor(k_obj, "k_pages"), &v = tensor(v_obj, "v_pages");
+  if (k.dim() != 4) throw BadValue("k_pages must be [num_pages, Hkv, page_size, D]");
+  const int index = index_of(k);
+  Pages p;
+  p.k = rows(k, "k_pages", k.sizes(), index, written);
+  p.v = rows(v, "v_pages", k.sizes(), index, written);
+  if (!k.is_contiguous() || !v.is_contiguous()) throw BadValue("k_pages and v_pages must be contiguous");
+  p.index = index;
+  p.num_pages = checked_int(k.size(0), "num_pages");
+  p.hkv = checked_int(k.size(1), "Hkv");
+  p.page_size = checked_int(k.size(2), "page_size");
+  p.head_dim = checked_int(k.size(3), "head_dim");
+  return p;
+}
+
+float* slot_weights(PyObject* o, const char* name, const Pages& p) {
+  const at::Tensor& t = tensor(o, name);
+  const int64_t shape[3] = {p.num_pages, p.hkv, p.page_size};
+  if (t.scalar_type() != at::kFloat) throw BadType(std::string(name) + " must be float32");
+  if (index_of(t) != p.index || t.sizes() != at::IntArrayRef(shape) || !t.is_contiguous())
+    throw BadValue(std::string(name) + " must be a contiguous " + text(shape) + " tensor on the pages' device");
+  return static_cast<float*>(t.data_ptr());
+}
+
+// q and out of a decode over pages: contiguous [B, Hq, D].
+struct Queries {
+  const uint16_t* q;
+  uint16_t* o;
+  int64_t batch;
+  int heads;
+};
+
+Queries queries(PyObject* q_obj, PyObject* o_obj, const Pages& p) {
+  const at::Tensor &q = tensor(q_obj, "q"), &o = tensor(o_obj, "out");
+  if (q.dim() != 3) throw BadValue("q must be [B, Hq, D]");
+  const int64_t shape[3] = {q.size(0), q.size(1), p.head_dim};
+  Queries r{rows(q, "q", shape, p.index), rows(o, "out", shape, p.index, true), q.size(0), 0};
+  if (!q.is_contiguous() || !o.is_contiguous()) throw BadValue("q and out must be contiguous");
+  checked_int(r.batch, "batch");
+  r.heads = checked_int(q.size(1), "heads");
+  return r;
+}
+
+const int32_t* lengths(PyObject* o, int64_t batch, int index) {
+  if (o == Py_None) throw BadValue("seq_lens must be a tensor");
+  return ints(o, "seq_lens", batch, index);
+}
+
+void* sized_workspace(PyObject* o, int index, size_t* bytes) {
+  if (o == Py_None) throw BadValue("workspace must be a tensor");
+  return workspace(o, index, bytes);
+}
+
+// q, k_pages, v_pages, block_table, seq_lens, shared_pages, out, scale, workspace
+PyObject* decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded(n_args, 9, [&] {
+    const Pages p = pages_of(a[1], a[2], false);
+    const Queries r = queries(a[0], a[6], p);
+    int per_seq = 0;
+    const int32_t* table = block_table(a[3], r.batch, p.index, &per_seq);
+    const int32_t* lens = lengths(a[4], r.batch, p.index);
+    const int shared = checked_int(integer(a[5]), "shared_pages");
+    const float scale = (float)number(a[7]);
+    size_t bytes = 0;
+    void* const ws = sized_workspace(a[8], p.index, &bytes);
+    return launch(p.index, [&](void* stream) {
+      return f_decode_shared(r.q, p.k, p.v, table, lens, r.o, (int)r.batch, r.heads, p.hkv, p.head_dim, p.page_size,
+                             per_seq, p.num_pages, shared, scale, ws, bytes, stream);
+    });
+  });
+}
+
+// q, k_pages, v_pages, weights, weights_out, block_table, seq_lens, out, scale, workspace
+PyObject* decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded(n_args, 10, [&] {
+    const Pages p = pages_of(a[1], a[2], false);
+    const Queries r = queries(a[0], a[7], p);
+    const float* w_in = slot_weights(a[3], "weights", p);
+    float* w_out = slot_weights(a[4], "weights_out", p);
+    int per_seq = 0;
+    const int32_t* table = block_table(a[5], r.batch, p.index, &per_seq);
+    const int32_t* lens = lengths(a[6], r.batch, p.index);
+    const float scale = (float)number(a[8]);
+    size_t bytes = 0;
+    void* const ws = sized_workspace(a[9], p.index, &bytes);
+    return launch(p.index, [&](void* stream) {
+      return f_decode_scored(r.q, p.k, p.v, w_in, w_out, table, lens, r.o, (int)r.batch, r.heads, p.hkv, p.head_dim,
+                             p.page_size, per_seq, p.num_pages, scale, ws, bytes, stream);
+    });
+  });
+}
+
+// k_pages, v_pages, weights, weights_out, block_table, seq_lens, new_lens, sources, keep, first, last, workspace
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded(n_args, 12, [&] {
+    const Pages p = pages_of(a[0], a[1], true);
+    const float* w_in = slot_weights(a[2], "weights", p);
+    float* w_out = slot_weights(a[3], "weights_out", p);
+    if (a[5] == Py_None) throw BadValue("seq_lens must be a tensor");
+    const int64_t batch = tensor(a[5], "seq_lens").numel();
+    const int32_t* lens = lengths(a[5], batch, p.index);
+    int per_seq = 0;
+    const int32_t* table = block_table(a[4], batch, p.index, &per_seq);
+    int32_t* new_lens = ints(a[6], "new_lens", batch, p.index);
+    const int keep = checked_int(integer(a[8]), "keep"), first = checked_int(integer(a[9]), "first"),
+              last = checked_int(integer(a[10]), "last");
+    int32_t* sources = nullptr;
+    if (a[7] != Py_None) {
+      const at::Tensor& t = tensor(a[7], "sources");
+      const int64_t shape[3] = {batch, p.hkv, keep};
+      if (t.scalar_type() != at::kInt || index_of(t) != p.index || t.sizes() != at::IntArrayRef(shape) ||
+          !t.is_contiguous())
+        throw BadValue("sources must be a contiguous int32 " + text(shape) + " tensor on the pages' device");
+      sources = static_cast<int32_t*>(t.data_ptr());
+    }
+    const int n = checked_int(batch, "batch");
+    size_t bytes = 0;
+    void* const ws = sized_workspace(a[11], p.index, &bytes);
+    return launch(p.index, [&](void* stream) {
+      return f_evict(p.k, p.v, w_in, w_out, table, lens, new_lens, sources, n, p.hkv, p.head_dim, p.page_size, per_seq,
+                     p.num_pages, keep, first, last, ws, bytes, stream);
+    });
+  });
+}
+
+// The addresses of the eight C entry points, in the order of this file.
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-  return guarded(n_args, 5, [&] {
+  return guarded(n_args, 8, [&] {
     f_norm_rope = reinterpret_cast<decltype(f_norm_rope)>(static_cast<uintptr_t>(integer(a[0])));
     f_append = reinterpret_cast<decltype(f_append)>(static_cast<uintptr_t>(integer(a[1])));
     f_append_qkv = reinterpret_cast<decltype(f_append_qkv)>(static_cast<uintptr_t>(integer(a[2])));
     f_read = reinterpret_cast<decltype(f_read)>(static_cast<uintptr_t>(integer(a[3])));
     f_decode = reinterpret_cast<decltype(f_decode)>(static_cast<uintptr_t>(integer(a[4])));
+    f_decode_shared = reinterpret_cast<decltype(f_decode_shared)>(static_cast<uintptr_t>(integer(a[5])));
+    f_decode_scored = reinterpret_cast<decltype(f_decode_scored)>(static_cast<uintptr_t>(integer(a[6])));
+    f_evict = reinterpret_cast<decltype(f_evict)>(static_cast<uintptr_t>(integer(a[7])));
     return 0;
   });
 }
@@ -354,7 +493,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 #define LARA_METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LARA_METHOD(init), LARA_METHOD(norm_rope), LARA_METHOD(append), LARA_METHOD(append_qkv),
-                         LARA_METHOD(read), LARA_METHOD(decode),    {nullptr, nullptr, 0, nullptr}};
+                         LARA_METHOD(read), LARA_METHOD(decode), LARA_METHOD(decode_shared),
+                         LARA_METHOD(decode_scored), LARA_METHOD(evict), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

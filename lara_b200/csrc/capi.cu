@@ -305,6 +305,7 @@ std::string describe_status(int bits) {
   if (bits & lara::kDevAppendOverflow) s += " append-overflow";
   if (bits & lara::kDevBadPage) s += " bad-page-index";
   if (bits & lara::kDevBadPosition) s += " bad-position";
+  if (bits & lara::kDevScoreRoom) s += " score-room";
   return s.empty() ? std::string(" unknown") : s;
 }
 

@@ -28,6 +28,7 @@ enum DeviceStatus : int {
   kDevAppendOverflow = 1 << 2, // an appended row would pass max_seq_len
   kDevBadPage = 1 << 3,        // a block-table entry was outside [0, num_pages)
   kDevBadPosition = 1 << 4,    // a token position was outside the rotation table
+  kDevScoreRoom = 1 << 5,      // sequences of one scored decode share pages: some got no weights
 };
 
 // One decode launch: queries of `batch` sequences (or of `batch` query rows

@@ -1,0 +1,817 @@
+// Decode over the paged bf16 cache, with each slot's attention weight gathered
+// (lara_gqa_decode_scored) or behind a prefix that the batch shares
+// (lara_gqa_decode_shared); declared in include/lara_b200.h.
+//
+//   s_t = scale log2(e) q.k_t,  o = sum_t 2^(s_t - R) v_t / sum_t 2^(s_t - R)
+//   w_t += sum over the group's heads of 2^(s_t - M) / L   (M, L: the whole row's R and sum)
+//
+// Two launches.  The first reads every cached row once and leaves partial
+// results (R, l, acc) of each unit, a (sequence, kv head), or of the parts that
+// several CTAs take of it; the second joins them, and, scoring, turns the
+// scores that the first left into weights (G fp32 numbers per token and kv head
+// written and read beside the 4 D bytes of its rows: at G = 4, D = 128 6 % of
+// them, against 50 % for reading K twice).
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
+#include "paged.cuh"
+
+namespace lara {
+
+using namespace paged;
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 16;            // tokens per warp and stage: never across pages
+constexpr int kMinTiles = kWarps;    // tiles per CTA below which fewer CTAs run
+constexpr int kUnitCost = 8;         // what a unit costs beside its tiles, in tiles
+constexpr int kLensCached = 1024;    // lengths kept in shared memory
+// R moves only when a score passes it by this much (log2): weights stay below 2^8.
+constexpr float kSlack = 8.f;
+
+template <int D, int NG>
+struct Cfg {
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kCtasPerSm = 2;
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kRowsBytes = kTile * kRowBytes;  // K (or V) of a stage
+  static constexpr int kStageBytes = 2 * kRowsBytes;
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kSmemBytes = kWarps * kWarpBytes + 128;
+  static constexpr int kPitch = D + 4;  // floats per head in the join (lanes of a store hit distinct banks)
+  static_assert(8 * kPitch * 4 <= kStageBytes, "a stage holds the sums of eight heads");
+};
+
+struct Args {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  PoolIndex index;
+  const int32_t* lens;
+  uint16_t* o;
+  int batch, n_q_heads, group;
+  float scale_log2;
+  int* status;
+  UnitParts* units;  // [batch * kv heads]
+  float2* part_ml;   // [units + CTAs][group] (R, l)
+  float* part_acc;   // [units + CTAs][group][D]
+  // scoring
+  float* scores;          // [tiles][kTile][group], in the order of the units
+  long long score_tiles;  // that there is room for
+  const float* w_in;      // [pages][kv heads][page]
+  float* w_out;
+};
+
+template <int kDst>
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16;" ::"r"(dst), "l"(src), "n"(kDst) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix(uint32_t v[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t v[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 31) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
+// A unit (b, kvh); `base` is the place of its first tile, counted from the
+// start of the CTA's share, `tile0` among the tiles of all units.
+struct Unit {
+  long long tile0;
+  int base, tiles, len, b, kvh;
+};
+
+// Equal shares of the span: the first `rem` take one more.
+struct Shares {
+  long long per, rem;
+  __device__ __forceinline__ long long start(long long c) const { return c * per + min(c, rem); }
+  __device__ __forceinline__ int cta(long long at) const {
+    return (int)(at < rem * (per + 1) ? quotient(at, per + 1) : rem + quotient(at - rem * (per + 1), per));
+  }
+};
+
+// The products run as warp-wide mma with the cache as the 16-row operand and
+// the group's heads as the 8 columns: S^T[token][head] = K q^T, O^T[dim][head]
+// = V^T P^T.  The columns of both lie in the same lanes, so rescaling needs no
+// exchange, and movmatrix turns a tile of P into the second operand.  P is the
+// sum of two bf16 numbers (what both leave is 2^-17 of it), since one alone
+// would show wherever values nearly cancel in an output.
+template <int D, int NG, bool kScored>
+__global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_kernel(const __grid_constant__ Args a) {
+  using C = Cfg<D, NG>;
+  constexpr int KS = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long s_sum[kWarps];
+  __shared__ Unit s_first;
+  __shared__ float2 s_ml[kWarps][NG * 8];
+  __shared__ int s_idle[kWarps];
+  __shared__ int s_lens[kLensCached];
+  uint8_t* const smem = smem_raw + (-smem_addr(smem_raw) & 127);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int G = a.group, hkv = a.index.n_kv_heads;
+  const long long cap = a.index.capacity();
+
+  allow_dependent_launch();
+  grid_dependency_wait();
+
+  // ---- this CTA's share of all tiles, and the unit in which it starts ----
+  auto load_len = [&](int b) { return (int)min((long long)max(__ldcg(a.lens + b), 0), cap); };
+  auto len_of = [&](int b) { return b < kLensCached ? s_lens[b] : load_len(b); };
+  auto next_unit = [&](Unit& u) {
+    u.base += u.tiles + kUnitCost;
+    u.tile0 += u.tiles;
+    if (++u.kvh == hkv) {
+      u.kvh = 0;
+      do {
+        ++u.b;
+        u.len = u.b < a.batch ? len_of(u.b) : 0;
+        u.tiles = u.b < a.batch ? tiles_of(u.len) : 0x3fffffff;
+      } while (u.tiles == 0);
+    }
+  };
+  const int per_thread = (a.batch + kThreads - 1) / kThreads;
+  const int b_lo = min(a.batch, (int)threadIdx.x * per_thread), b_hi = min(a.batch, b_lo + per_thread);
+  long long mine = 0;  // tiles in the low 40 bits, sequences that have some above
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int raw = __ldcg(a.lens + b);
+    const int len = (int)min((long long)max(raw, 0), cap);
+    if (raw != len) atomicOr(a.status, kDevBadLength);
+    if (b < kLensCached) s_lens[b] = len;
+    mine += tiles_of(len) + (len > 0 ? 1ll << 40 : 0);
+  }
+  long long ahead = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, ahead, off);
+    if (lane >= off) ahead += y;
+  }
+  if (lane == 31) s_sum[warp] = ahead;
+  __syncthreads();
+  ahead -= mine;
+  long long all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) ahead += s_sum[w];
+    all += s_sum[w];
+  }
+  constexpr long long kLow = (1ll << 40) - 1;
+  const long long total = (all & kLow) * hkv, units = (all >> 40) * hkv;
+  if (total == 0) return;
+  const long long span = total + units * kUnitCost;
+  const int workers = (int)min((long long)gridDim.x, max((total + kMinTiles - 1) / kMinTiles, units));
+  const int me = blockIdx.x;
+  if (me >= workers) return;
+  const Shares sh{quotient(span, workers), span - quotient(span, workers) * workers};
+  const int share = (int)(sh.start(me + 1) - sh.start(me));
+  {
+    // found by the thread that counted the sequence in which the share starts
+    const long long begin = ((ahead & kLow) + (ahead >> 40) * kUnitCost) * hkv;
+    const long long stop = begin + ((mine & kLow) + (mine >> 40) * kUnitCost) * hkv;
+    const long long x = sh.start(me);
+    if (x >= begin && x < stop) {
+      long long at = begin, tile0 = (ahead & kLow) * hkv;
+      Unit u{0, 0, 0, 0, b_lo, 0};
+      for (;; ++u.b) {  // by whole sequences
+        u.len = len_of(u.b);
+        u.tiles = tiles_of(u.len);
+        const long long span_b = u.tiles ? (long long)(u.tiles + kUnitCost) * hkv : 0;
+        if (x < at + span_b) break;
+        at += span_b;
+        tile0 += (long long)u.tiles * hkv;
+      }
+      u.kvh = (int)quotient(x - at, u.tiles + kUnitCost);
+      u.base = (int)(at + (long long)u.kvh * (u.tiles + kUnitCost) + kUnitCost - x);
+      u.tile0 = tile0 + (long long)u.kvh * u.tiles;
+      s_first = u;
+    }
+  }
+  __syncthreads();
+  const Unit u0 = s_first;
+  auto in_share = [&](const Unit& u) { return u.base < share; };
+  auto tiles_end = [&](const Unit& u) { return min(share, u.base + u.tiles); };
+
+  // ---- the warp's ring ----
+  uint8_t* const ring = smem + warp * C::kWarpBytes;
+  constexpr int kChunks = D / 8, kRowsPer = 32 / kChunks;  // a warp copies kRowsPer rows (512 bytes) at a time
+  // chunk c of row r lies at r kRowBytes + ((c ^ (r & 7)) << 4): eight rows of a matrix hit distinct banks
+  const int c_row = lane / kChunks;
+  const uint32_t copy_at = c_row * C::kRowBytes + (((lane % kChunks) ^ c_row) << 4);
+  Unit pu = u0;                           // where the next tile to fetch lies
+  int pid = max(pu.base, 0) + warp;       // its number
+  int page = 0;                           // its page, fetched a tile ahead
+  bool more = in_share(pu);
+  const int log2 = a.index.page_log2;
+  auto fetch_page = [&] {
+    while (more && pid >= tiles_end(pu)) {
+      next_unit(pu);
+      pid = pu.base + warp;
+      more = in_share(pu);
+    }
+    if (!more) return;
+    const int pos = (pid - pu.base) * kTile;
+    page = __ldcg(a.index.block_table + (long long)pu.b * a.index.pages_per_seq + (pos >> log2));
+  };
+  auto fetch_tile = [&](int stage) {
+    if (more) {
+      const uint32_t st = smem_addr(ring) + stage * C::kStageBytes + copy_at;
+      const int pos = (pid - pu.base) * kTile;
+      if ((unsigned)page >= (unsigned)a.index.num_pages) {
+        atomicOr(a.status, kDevBadPage);
+        page = 0;
+      }
+      const long long row0 = (((long long)page * hkv + pu.kvh) << log2) + (pos & ((1 << log2) - 1));
+      const char* ks = reinterpret_cast<const char*>(a.k + row0 * D) + lane * 16;
+      const char* vs = reinterpret_cast<const char*>(a.v + row0 * D) + lane * 16;
+#pragma unroll
+      for (int i = 0; i < kTile / kRowsPer; ++i) {
+        const uint32_t to = (st ^ ((i * kRowsPer & 7) << 4)) + i * 512;
+        cp_async16<0>(to, ks + i * 512);
+        cp_async16<C::kRowsBytes>(to, vs + i * 512);
+      }
+      pid += kWarps;
+      fetch_page();
+    }
+    cp_async_commit();
+  };
+  fetch_page();
+#pragma unroll
+  for (int s = 0; s < C::kStages - 1; ++s) fetch_tile(s);
+
+  // ldmatrix addresses: K rows as they are (tokens), V's transposed (dims)
+  const uint32_t k_row = (lane & 7) + (lane & 8), v_row = (lane & 7) + (lane >> 4 << 3);
+  const uint32_t k_at = k_row * C::kRowBytes + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_at = C::kRowsBytes + v_row * C::kRowBytes + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+
+  // ---- units of this CTA ----
+  int stage = 0;
+  for (Unit u = u0; in_share(u); next_unit(u)) {
+    const int end = tiles_end(u);
+    uint32_t qf[NG][KS][2];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int h = n * 8 + g;
+      const uint32_t* src =
+          reinterpret_cast<const uint32_t*>(a.q + ((long long)u.b * a.n_q_heads + u.kvh * G + h) * D) + t4;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        qf[n][j][0] = h < G ? __ldcg(src + 8 * j) : 0;
+        qf[n][j][1] = h < G ? __ldcg(src + 8 * j + 4) : 0;
+      }
+    }
+    float R[NG][2], l[NG][2], o[NG][KS][4];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      R[n][0] = R[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+
+    for (int id = max(u.base, 0) + warp; id < end; id += kWarps) {
+      cp_async_wait<C::kStages - 2>();
+      __syncwarp();
+      fetch_tile(stage == 0 ? C::kStages - 1 : stage - 1);
+      uint8_t* const st = ring + stage * C::kStageBytes;
+      const uint32_t sa = smem_addr(st);
+      stage = stage + 1 == C::kStages ? 0 : stage + 1;
+
+      // ---- scores of tokens g (0, 1) and g + 8 (2, 3), heads 2 t4 and 2 t4 + 1 ----
+      float s[NG][4];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        uint32_t k[4];
+        ldmatrix(k, sa + (k_at ^ (j << 5)));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mma_bf16(s[n], k, qf[n][j][0], qf[n][j][1]);
+      }
+      const int first = (id - u.base) * kTile, valid = u.len - first;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= a.scale_log2;
+      if (valid < kTile) {  // the sequence's last tile: nothing past its end counts, whatever lies there
+        for (int i = max(valid, 0) * kChunks + lane; i < kTile * kChunks; i += 32)
+          reinterpret_cast<uint4*>(st + C::kRowsBytes)[i] = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (g + 8 * (i >> 1) >= valid) s[n][i] = -INFINITY;
+      }
+      if constexpr (kScored) {
+        const long long tile = u.tile0 + (id - u.base);
+        if (tile < a.score_tiles) {
+          float* dst = a.scores + (tile * kTile + g) * G + 2 * t4;
+#pragma unroll
+          for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float* const to = dst + 8 * i * G + 8 * n;
+              if (!(G & 1) && 8 * n + 2 * t4 < G) {
+                *reinterpret_cast<float2*>(to) = make_float2(s[n][2 * i], s[n][2 * i + 1]);
+              } else {
+                if (8 * n + 2 * t4 < G) to[0] = s[n][2 * i];
+                if (8 * n + 2 * t4 + 1 < G) to[1] = s[n][2 * i + 1];
+              }
+            }
+        }
+      }
+
+      // ---- move R where a score passes it by far ----
+      bool over = false;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+        over |= fmaxf(s[n][0], s[n][2]) > R[n][0] + kSlack || fmaxf(s[n][1], s[n][3]) > R[n][1] + kSlack;
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = fmaxf(s[n][c], s[n][2 + c]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            if (m > R[n][c] + kSlack) {
+              const float f = ex2_ftz(R[n][c] - m);
+              R[n][c] = m;
+              l[n][c] *= f;
+#pragma unroll
+              for (int i = 0; i < KS; ++i) {
+                o[n][i][c] *= f;
+                o[n][i][2 + c] *= f;
+              }
+            }
+          }
+      }
+
+      // ---- weights as the second operand: tokens 2 t4, 2 t4 + 1 (and + 8) of column g ----
+      uint32_t pf[NG][2], pr[NG][2];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float p0 = ex2_ftz(s[n][2 * i] - R[n][0]), p1 = ex2_ftz(s[n][2 * i + 1] - R[n][1]);
+          l[n][0] += p0;
+          l[n][1] += p1;
+          const uint32_t hi = pack2_rn(p0, p1);
+          pf[n][i] = transpose8x8(hi);
+          pr[n][i] = transpose8x8(pack2_rn(p0 - bf16lo(hi), p1 - bf16hi(hi)));
+        }
+
+      // ---- O^T += V^T P^T: block c holds dims 16 c + g and 16 c + g + 8 ----
+#pragma unroll
+      for (int c = 0; c < KS; ++c) {
+        uint32_t v[4];
+        ldmatrix_trans(v, sa + (v_at ^ (c << 5)));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          mma_bf16(o[n][c], v, pf[n][0], pf[n][1]);
+          mma_bf16(o[n][c], v, pr[n][0], pr[n][1]);
+        }
+      }
+      __syncwarp();
+    }
+
+    // ---- the unit's end: the warps join through the stages that held their last tiles ----
+    const int idle = (stage == 0 ? C::kStages : stage) - 1;
+    float* const sums = reinterpret_cast<float*>(ring + idle * C::kStageBytes);
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
+        if (g == 0) s_ml[warp][n * 8 + 2 * t4 + c] = make_float2(R[n][c], l[n][c]);
+      }
+    if (lane == 0) s_idle[warp] = warp * C::kWarpBytes + idle * C::kStageBytes;
+    const long long at0 = sh.start(me) + u.base;
+    const int index = u.b * hkv + u.kvh, slot = index + me;
+    if (threadIdx.x == 0 && u.base >= 0)  // the unit starts here
+      a.units[index] = UnitParts{u.tile0, slot, sh.cta(at0 + u.tiles - 1) - me + 1};
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][n * 8 + 2 * t4 + c].x);
+        const float f = R[n][c] == top ? 1.f : ex2_ftz(R[n][c] - top);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          sums[(2 * t4 + c) * C::kPitch + 16 * i + g] = o[n][i][c] * f;
+          sums[(2 * t4 + c) * C::kPitch + 16 * i + g + 8] = o[n][i][2 + c] * f;
+        }
+      }
+      __syncthreads();
+      const int heads = min(8, G - 8 * n);
+      for (int item = threadIdx.x; item < heads * (D / 4); item += kThreads) {
+        const int hl = item / (D / 4), d = item % (D / 4) * 4, h = 8 * n + hl;
+        float top = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][h].x);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = s_ml[w][h];
+          L = fmaf(ml.y, ml.x == top ? 1.f : ex2_ftz(ml.x - top), L);
+          const float4 y = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(smem + s_idle[w]) + hl * C::kPitch + d);
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
+        }
+        *reinterpret_cast<float4*>(a.part_acc + ((long long)slot * G + h) * D + d) = x;
+        if (d == 0) a.part_ml[(long long)slot * G + h] = make_float2(top, L);
+      }
+      __syncthreads();  // the idle stages may be filled again
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// ---- the second launch ----
+constexpr int kJoinThreads = 128;
+
+// Joins the parts of one output row per warp (few parts) or, row after row, per block.
+template <int D>
+__device__ __forceinline__ void join_rows(const Args& a, int block) {
+  constexpr int kLanes = D / 4, kSub = kJoinThreads / kLanes;  // lanes of a row, rows in flight
+  __shared__ float4 s_x[kSub][kLanes];
+  __shared__ float s_l[kSub];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.group;
+  const long long rows = (long long)a.batch * a.n_q_heads;
+  for (int r = 0; r < kJoinThreads / 32; ++r) {
+    const long long row = (long long)block * (kJoinThreads / 32) + r;
+    if (row >= rows) return;
+    const int b = (int)(row / a.n_q_heads), hq = (int)(row % a.n_q_heads), kvh = hq / G, h = hq % G;
+    uint16_t* const out = a.o + row * D;
+    const int len = __ldcg(a.lens + b);
+    const int sub = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
+    if (len <= 0) {
+      if (threadIdx.x < D / 8) reinterpret_cast<uint4*>(out)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const UnitParts up = a.units[b * a.index.n_kv_heads + kvh];
+    float M = -INFINITY;
+    for (int i = lane; i < up.parts; i += 32) M = fmaxf(M, __ldcg(a.part_ml + (long long)(up.slot0 + i) * G + h).x);
+#pragma unroll
+    for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f;
+#pragma unroll 4
+    for (int i = sub; i < up.parts; i += kSub) {
+      const long long p = (long long)(up.slot0 + i) * G + h;
+      const float2 ml = __ldcg(a.part_ml + p);
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_acc + p * D) + at);
+      const float f = ml.x == M ? 1.f : ex2_ftz(ml.x - M);
+      L = fmaf(ml.y, f, L);
+      x.x = fmaf(y.x, f, x.x);
+      x.y = fmaf(y.y, f, x.y);
+      x.z = fmaf(y.z, f, x.z);
+      x.w = fmaf(y.w, f, x.w);
+    }
+    __syncthreads();
+    s_x[sub][at] = x;
+    if (at == 0) s_l[sub] = L;
+    __syncthreads();
+    if (warp == 0 && lane < kLanes) {
+      x = make_float4(0.f, 0.f, 0.f, 0.f);
+      L = 0.f;
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        const float4 y = s_x[i][lane];
+        L += s_l[i];
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
+      }
+      const float inv = 1.f / L;
+      reinterpret_cast<uint2*>(out)[lane] = make_uint2(pack2_rn(x.x * inv, x.y * inv), pack2_rn(x.z * inv, x.w * inv));
+    }
+  }
+}
+
+// Adds the weights of the tokens of one unit that lie in tiles [t0, t1) of all.
+__device__ __forceinline__ void add_weights(const Args& a, int block, int blocks) {
+  __shared__ float s_m[16], s_inv[16];
+  __shared__ long long s_total;
+  const int G = a.group, hkv = a.index.n_kv_heads;
+  const int n_units = a.batch * hkv;
+  const long long cap = a.index.capacity();
+  auto len_of = [&](int b) { return (int)min((long long)max(__ldcg(a.lens + b), 0), cap); };
+  // the last unit with tokens says how many tiles there are
+  if (threadIdx.x == 0) {
+    int b = a.batch - 1;
+    while (b >= 0 && len_of(b) == 0) --b;
+    s_total = b < 0 ? 0 : a.units[b * hkv + hkv - 1].tile0 + tiles_of(len_of(b));
+  }
+  __syncthreads();
+  const long long total = s_total;
+  const long long per = (total + blocks - 1) / blocks;
+  const long long lo = block * per, hi = min(total, lo + per);
+  if (lo >= hi) return;
+  if (hi > a.score_tiles) {
+    if (threadIdx.x == 0) atomicOr(a.status, kDevScoreRoom);
+  }
+  long long at = 0;  // tiles before unit i
+  for (int i = 0; i < n_units && at < hi; ++i) {
+    const int b = i / hkv, len = len_of(b), tiles = tiles_of(len);
+    if (at + tiles <= lo || tiles == 0) {
+      at += tiles;
+      continue;
+    }
+    const UnitParts up = a.units[i];
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      for (int h = 0; h < G; ++h) {
+        float M = -INFINITY, L = 0.f;
+        for (int p = threadIdx.x; p < up.parts; p += 32)
+          M = fmaxf(M, __ldcg(a.part_ml + (long long)(up.slot0 + p) * G + h).x);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+        for (int p = threadIdx.x; p < up.parts; p += 32) {
+          const float2 ml = __ldcg(a.part_ml + (long long)(up.slot0 + p) * G + h);
+          L = fmaf(ml.y, ml.x == M ? 1.f : ex2_ftz(ml.x - M), L);
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+        if (threadIdx.x == 0) {
+          s_m[h] = M;
+          s_inv[h] = 1.f / L;
+        }
+      }
+    }
+    __syncthreads();
+    const long long t0 = max(lo, at), t1 = min(min(hi, at + tiles), a.score_tiles);
+    for (long long x = t0 * kTile + threadIdx.x; x < t1 * kTile; x += blockDim.x) {
+      const int t = (int)(x - at * kTile);
+      if (t >= len) break;
+      const long long row = a.index.row(b, i % hkv, t, nullptr);
+      if (row < 0) continue;  // flagged where its rows were read
+      float w = 0.f;
+      for (int h = 0; h < G; ++h) w = fmaf(ex2_ftz(__ldcg(a.scores + x * G + h) - s_m[h]), s_inv[h], w);
+      a.w_out[row] = a.w_in[row] + w;
+    }
+    at += tiles;
+  }
+}
+
+template <int D, bool kScored>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args a, int join_blocks) {
+  allow_dependent_launch();
+  grid_dependency_wait();
+  if ((int)blockIdx.x < join_blocks) {
+    join_rows<D>(a, blockIdx.x);
+  } else if constexpr (kScored) {
+    add_weights(a, blockIdx.x - join_blocks, gridDim.x - join_blocks);
+  }
+}
+
+int max_ctas() { return device_sm_count() * 2; }
+
+// Workspace: status word | units | partial results | scores.
+struct Layout {
+  size_t units_off, ml_off, acc_off, scores_off, total;
+  long long score_tiles;
+};
+
+Layout layout(int batch, int n_kv_heads, int group, int head_dim, long long score_tokens) {
+  const size_t units = (size_t)batch * n_kv_heads, slots = units + max_ctas();
+  Layout w;
+  w.units_off = kStatusBytes;
+  w.ml_off = w.units_off + up256(units * sizeof(UnitParts));
+  w.acc_off = w.ml_off + up256(slots * group * sizeof(float2));
+  w.scores_off = w.acc_off + up256(slots * group * head_dim * sizeof(float));
+  w.score_tiles = score_tokens / kTile * n_kv_heads;
+  w.total = w.scores_off + up256((size_t)w.score_tiles * kTile * group * sizeof(float));
+  return w;
+}
+
+template <int D, int NG, bool kScored>
+cudaError_t launch(const Args& a, cudaStream_t stream) {
+  using C = Cfg<D, NG>;
+  const void* fn = reinterpret_cast<const void*>(&own_tokens_kernel<D, NG, kScored>);
+  {
+    static std::mutex mu;
+    static uint64_t done = 0;  // the shared-memory opt-in is per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev > 63 || !(done >> dev & 1)) {
+      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+      if (e != cudaSuccess) return e;
+      if (dev <= 63) done |= 1ull << dev;
+    }
+  }
+  // no more CTAs than a full cache could feed, one for each unit at least
+  const long long units = (long long)a.batch * a.index.n_kv_heads;
+  const long long tiles = units * ((a.index.capacity() + kTile - 1) / kTile);
+  const long long ctas = std::min<long long>(max_ctas(), std::max(units, (tiles + kMinTiles - 1) / kMinTiles));
+  Args args = a;
+  void* p[] = {&args};
+  cudaError_t e = launch_with_pdl(fn, dim3((unsigned)ctas), dim3(kThreads), p, C::kSmemBytes, stream);
+  if (e != cudaSuccess) return e;
+  const long long rows = (long long)a.batch * a.n_q_heads;
+  int join_blocks = (int)((rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+  int blocks = join_blocks;
+  if (kScored) blocks += (int)std::min<long long>(device_sm_count() * 8, (tiles + 7) / 8);
+  void* p2[] = {&args, &join_blocks};
+  return launch_with_pdl(reinterpret_cast<const void*>(&join_kernel<D, kScored>), dim3((unsigned)blocks),
+                         dim3(kJoinThreads), p2, 0, stream);
+}
+
+}  // namespace
+
+namespace paged {
+
+int check_paged_pool(const void* k_pages, const void* v_pages, const void* block_table, int n_kv_heads, int head_dim,
+                     int page_size, int pages_per_seq, int num_pages, int batch, PoolIndex* index) {
+  if (head_dim != 64 && head_dim != 128) return set_last_error(LARA_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)))
+    return set_last_error(LARA_ERR_BAD_CFG, "page_size must be a power of two in [16, 65536]");
+  if (batch < 0 || batch > 65535) return set_last_error(LARA_ERR_BAD_CFG, "batch must be in [0, 65535]");
+  if (n_kv_heads < 1 || n_kv_heads > 65535 || num_pages < 1 || pages_per_seq < 1 ||
+      (long long)pages_per_seq * page_size > 0x3fffffffll || (long long)batch * n_kv_heads > 0x3fffffffll ||
+      (double)batch * n_kv_heads * pages_per_seq * page_size > 0x1p40)
+    return set_last_error(LARA_ERR_BAD_CFG,
+                          "bad paged-cache geometry (at most 2^30 - 1 tokens a sequence, 2^40 rows in all)");
+  if (batch == 0) return LARA_OK;
+  if (!k_pages || !v_pages || !block_table) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
+  if (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(block_table, 4))
+    return set_last_error(LARA_ERR_STREAM_DEST, "k_pages and v_pages must be 16-byte aligned");
+  index->block_table = static_cast<const int32_t*>(block_table);
+  index->pages_per_seq = pages_per_seq;
+  index->page_log2 = __builtin_ctz(page_size);
+  index->num_pages = num_pages;
+  index->n_kv_heads = n_kv_heads;
+  return LARA_OK;
+}
+
+int check_weights(const float* in, const float* out, int n_kv_heads, int page_size, int num_pages) {
+  if (!in || !out) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
+  if (!aligned(in, 4) || !aligned(out, 4)) return set_last_error(LARA_ERR_STREAM_DEST, "weights must be 4-byte aligned");
+  if (in != out && kvq::overlap(in, out, (size_t)num_pages * n_kv_heads * page_size * 4))
+    return set_last_error(LARA_ERR_STREAM_DEST, "weights_out must be weights or lie apart from them");
+  return LARA_OK;
+}
+
+}  // namespace paged
+
+}  // namespace lara
+
+using namespace lara;
+
+namespace {
+
+// The checks and arguments that the two decodes have in common.
+int decode_args(Args& a, const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
+                const int32_t* block_table, const int32_t* seq_lens, uint16_t* o, int batch, int n_q_heads,
+                int n_kv_heads, int head_dim, int page_size, int pages_per_seq, int num_pages, float scale,
+                const void* workspace) {
+  if (const int rc = check_paged_pool(k_pages, v_pages, block_table, n_kv_heads, head_dim, page_size, pages_per_seq,
+                                      num_pages, batch, &a.index))
+    return rc;
+  if (n_q_heads < 1 || n_q_heads % n_kv_heads)
+    return set_last_error(LARA_ERR_BAD_CFG, "n_q_heads must be a multiple of n_kv_heads");
+  if (n_q_heads / n_kv_heads > 16)
+    return set_last_error(LARA_ERR_UNSUPPORTED, "groups of at most 16 query heads per kv head");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return set_last_error(LARA_ERR_BAD_CFG, "scale must be positive and finite");
+  if (batch == 0) return LARA_OK;
+  if (!q || !seq_lens || !o || !workspace) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
+  if (!aligned(q, 16) || !aligned(o, 16) || !aligned(seq_lens, 4) || !aligned(workspace, 256))
+    return set_last_error(LARA_ERR_STREAM_DEST, "q and o must be 16-byte aligned, the workspace 256-byte");
+  a.q = q;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.lens = seq_lens;
+  a.o = o;
+  a.batch = batch;
+  a.n_q_heads = n_q_heads;
+  a.group = n_q_heads / n_kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return LARA_OK;
+}
+
+void place(Args& a, const Layout& w, void* workspace) {
+  char* base = static_cast<char*>(workspace);
+  a.status = reinterpret_cast<int*>(base);
+  a.units = reinterpret_cast<UnitParts*>(base + w.units_off);
+  a.part_ml = reinterpret_cast<float2*>(base + w.ml_off);
+  a.part_acc = reinterpret_cast<float*>(base + w.acc_off);
+  a.scores = reinterpret_cast<float*>(base + w.scores_off);
+  a.score_tiles = w.score_tiles;
+}
+
+template <bool kScored>
+cudaError_t launch_any(const Args& a, int head_dim, cudaStream_t st) {
+  if (head_dim == 128) return a.group <= 8 ? launch<128, 1, kScored>(a, st) : launch<128, 2, kScored>(a, st);
+  return a.group <= 8 ? launch<64, 1, kScored>(a, st) : launch<64, 2, kScored>(a, st);
+}
+
+// Tokens whose scores a call can leave: those of every page its tables can name.
+long long score_tokens(int batch, int page_size, int pages_per_seq, int num_pages) {
+  return std::min<long long>((long long)batch * pages_per_seq, num_pages) * page_size;
+}
+
+}  // namespace
+
+extern "C" size_t lara_decode_scored_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim,
+                                                     int page_size, int pages_per_seq, int num_pages) {
+  if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || head_dim < 1 || page_size < 1 || pages_per_seq < 1 ||
+      num_pages < 1)
+    return 0;
+  return layout(batch, n_kv_heads, (n_q_heads + n_kv_heads - 1) / n_kv_heads, head_dim,
+                score_tokens(batch, page_size, pages_per_seq, num_pages))
+      .total;
+}
+
+extern "C" int lara_gqa_decode_scored(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
+                                      const float* weights, float* weights_out, const int32_t* block_table,
+                                      const int32_t* seq_lens, uint16_t* o, int batch, int n_q_heads, int n_kv_heads,
+                                      int head_dim, int page_size, int pages_per_seq, int num_pages, float scale,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  LARA_NVTX("lara_gqa_decode_scored");
+  Args a{};
+  if (const int rc = decode_args(a, q, k_pages, v_pages, block_table, seq_lens, o, batch, n_q_heads, n_kv_heads,
+                                 head_dim, page_size, pages_per_seq, num_pages, scale, workspace))
+    return rc;
+  if (batch == 0) return LARA_OK;
+  if (const int rc = check_weights(weights, weights_out, n_kv_heads, page_size, num_pages)) return rc;
+  const Layout w = layout(batch, n_kv_heads, a.group, head_dim,
+                          score_tokens(batch, page_size, pages_per_seq, num_pages));
+  if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "scored decode workspace too small");
+  place(a, w, workspace);
+  a.w_in = weights;
+  a.w_out = weights_out;
+  const cudaError_t e = launch_any<true>(a, head_dim, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess)
+    return set_last_error(LARA_ERR_CUDA, std::string("scored decode launch: ") + cudaGetErrorString(e));
+  return LARA_OK;
+}
+
+extern "C" size_t lara_decode_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
+  if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || head_dim < 1) return 0;
+  return layout(batch, n_kv_heads, (n_q_heads + n_kv_heads - 1) / n_kv_heads, head_dim, 0).total;
+}
+
+extern "C" int lara_gqa_decode_shared(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
+                                      const int32_t* block_table, const int32_t* seq_lens, uint16_t* o, int batch,
+                                      int n_q_heads, int n_kv_heads, int head_dim, int page_size, int pages_per_seq,
+                                      int num_pages, int shared_pages, float scale, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  LARA_NVTX("lara_gqa_decode_shared");
+  Args a{};
+  if (const int rc = decode_args(a, q, k_pages, v_pages, block_table, seq_lens, o, batch, n_q_heads, n_kv_heads,
+                                 head_dim, page_size, pages_per_seq, num_pages, scale, workspace))
+    return rc;
+  if (shared_pages < 0 || shared_pages > pages_per_seq)
+    return set_last_error(LARA_ERR_BAD_CFG, "shared_pages must be in [0, pages_per_seq]");
+  if (batch == 0) return LARA_OK;
+  const Layout w = layout(batch, n_kv_heads, a.group, head_dim, 0);
+  if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "shared decode workspace too small");
+  place(a, w, workspace);
+  const cudaError_t e = launch_any<false>(a, head_dim, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess)
+    return set_last_error(LARA_ERR_CUDA, std::string("shared decode launch: ") + cudaGetErrorString(e));
+  return LARA_OK;
+}

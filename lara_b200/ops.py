@@ -34,7 +34,8 @@ try:
         raise ImportError(f"it was built for torch {_binding.torch_version}, this is {torch.__version__}")
     _binding.init(*(ctypes.cast(f, ctypes.c_void_p).value
                     for f in (lib.lara_qk_norm_rope, lib.lara_kvq_append, lib.lara_kvq_append_qkv, lib.lara_kvq_read,
-                              lib.lara_gqa_decode_kvq)))
+                              lib.lara_gqa_decode_kvq, lib.lara_gqa_decode_shared, lib.lara_gqa_decode_scored,
+                              lib.lara_kv_evict)))
 except ImportError as e:
     _binding = _NoBinding(str(e))
 

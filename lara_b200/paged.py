@@ -13,7 +13,18 @@ sequences (``share_prefix``); an append never writes into a shared page.
 
 The kernels are ``lara_gqa_decode_paged`` / ``lara_kv_append_paged``
 (include/lara_b200.h); a decode over a paged cache returns the same words as
-over a contiguous cache holding the same tokens.  ``save`` / ``load`` use the
+over a contiguous cache holding the same tokens.
+
+For batches behind a common prefix and for contexts that outgrow their room there
+are, as stateless calls on the same pages and as methods of the cache:
+
+* :func:`gqa_decode_shared`: a decode that reads the pages which all sequences begin
+  with once for the batch, instead of once for each sequence;
+* :func:`gqa_decode_scored`: a decode that also adds to every cached slot's weight the
+  attention it got, summed over the query heads of its kv head;
+* :func:`kv_evict`: cuts sequences down to a number of slots for each kv head: the first
+  ones, the last ones, and the heaviest of the rest.
+  ``save`` / ``load`` use the
 ``lara-kv-v1`` file format of :mod:`lara_b200.kvfile`.
 """
 
@@ -26,12 +37,114 @@ import torch
 
 from . import kvfile
 from ._native import check, lib
-from .ops import _check_words, _stream, new_workspace
+from .ops import _binding, _check_words, _stream, new_workspace
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor:
+    dev = torch.device(device)
+    with torch.cuda.device(dev):
+        return new_workspace(nbytes, dev)
+
+
+def shared_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device="cuda:0") -> torch.Tensor:
+    """A zeroed workspace for :func:`gqa_decode_shared` calls of this or a smaller batch and group of query heads.
+
+    One stream at a time uses it.
+    """
+    return _workspace(int(lib.lara_decode_shared_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim)), device)
+
+
+def gqa_decode_shared(q, k_pages, v_pages, block_table, seq_lens, shared_pages: int, *, scale=None, workspace=None,
+                      out=None):
+    """One new token per sequence, of a batch whose sequences begin with the same pages (``lara_gqa_decode_shared``).
+
+    q ``[B, Hq, D]`` (bf16) attends the first ``seq_lens[b]`` tokens that ``block_table[b]`` names in ``k_pages`` and
+    ``v_pages`` ``[num_pages, Hkv, page_size, D]``.  The first ``shared_pages`` columns of the table are the same in
+    every row: they are read once for all sequences that are at least as long (a shorter sequence is read by itself).
+    ``Hq`` is any multiple of ``Hkv`` up to 16 per kv head, ``D`` 64 or 128.  A sequence of length 0 gives zeros.
+    ``workspace`` comes from :func:`shared_workspace` (``None`` allocates one for the call).  Returns ``o[B, Hq, D]``
+    (``out``, which may be q).
+    """
+    if out is None:
+        out = torch.empty_like(q)
+    if workspace is None:
+        workspace = shared_workspace(max(q.shape[0], 1), q.shape[1], k_pages.shape[1], q.shape[2], k_pages.device)
+    sc = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+    rc = _binding.decode_shared(q, k_pages, v_pages, block_table, seq_lens, shared_pages, out, sc, workspace)
+    if rc:
+        check(rc, "lara_gqa_decode_shared")
+    return out
+
+
+def scored_workspace(batch: int, n_q_heads: int, k_pages, pages_per_seq: int) -> torch.Tensor:
+    """A zeroed workspace for :func:`gqa_decode_scored` calls over a pool and tables of these sizes, or smaller batches.
+
+    It holds ``n_q_heads`` fp32 scores for every token that ``batch`` sequences can have in the pool.  One stream at a
+    time uses it.
+    """
+    num_pages, hkv, page_size, d = k_pages.shape
+    return _workspace(int(lib.lara_decode_scored_workspace_bytes(batch, n_q_heads, hkv, d, page_size, pages_per_seq,
+                                                                 num_pages)), k_pages.device)
+
+
+def gqa_decode_scored(q, k_pages, v_pages, weights, block_table, seq_lens, *, weights_out=None, scale=None,
+                      workspace=None, out=None):
+    """One new token per sequence, with the attention that every cached slot gets (``lara_gqa_decode_scored``).
+
+    As :func:`gqa_decode_shared` without a shared part, and ``weights_out[slot] = weights[slot] + sum`` over the kv
+    head's query heads of the slot's softmax weight: float32 ``[num_pages, Hkv, page_size]``, for the slots below
+    ``seq_lens[b]`` alone (``weights_out=None``: in place).  The sequences of one call share no pages.  ``workspace``
+    comes from :func:`scored_workspace`.
+    """
+    if out is None:
+        out = torch.empty_like(q)
+    if workspace is None:
+        workspace = scored_workspace(max(q.shape[0], 1), q.shape[1], k_pages, block_table.shape[1])
+    sc = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+    rc = _binding.decode_scored(q, k_pages, v_pages, weights, weights if weights_out is None else weights_out,
+                                block_table, seq_lens, out, sc, workspace)
+    if rc:
+        check(rc, "lara_gqa_decode_scored")
+    return out
+
+
+def evict_workspace(batch: int, n_kv_heads: int, keep: int, device="cuda:0") -> torch.Tensor:
+    """A zeroed workspace for :func:`kv_evict` calls of these or smaller sizes.  One stream at a time uses it."""
+    return _workspace(int(lib.lara_kv_evict_workspace_bytes(batch, n_kv_heads, keep)), device)
+
+
+def kv_evict(k_pages, v_pages, weights, block_table, seq_lens, keep: int, *, first: int = 0, last: int = 0,
+             weights_out=None, new_lens=None, sources=None, workspace=None):
+    """Cut every sequence of more than ``keep`` tokens down to ``keep``, each kv head by itself (``lara_kv_evict``).
+
+    The first ``first`` slots stay, the last ``last``, and of the rest the heaviest by ``weights`` (ties to the lowest
+    slot).  Kept rows from slot ``keep`` on move, in order, into the slots below it that are given up, in order, with
+    their weights; weights from ``keep`` to the old length become 0 (``weights_out=None``: in place).  The order of the
+    slots is no longer that of the positions, which a decode does not need.  ``seq_lens`` stays as it is; ``new_lens``
+    (int32 ``[B]``, another tensor; ``None``: a new one) receives ``min(seq_lens, keep)`` and is returned.  ``sources``
+    (int32 ``[B, Hkv, keep]``) receives the slot that each slot's row came from, -1 past the new length.  The sequences
+    of one call share no pages.
+    """
+    if new_lens is None:
+        new_lens = torch.empty_like(seq_lens)
+    if workspace is None:
+        workspace = evict_workspace(max(seq_lens.numel(), 1), k_pages.shape[1], max(int(keep), 1), k_pages.device)
+    rc = _binding.evict(k_pages, v_pages, weights, weights if weights_out is None else weights_out, block_table,
+                        seq_lens, new_lens, sources, keep, first, last, workspace)
+    if rc:
+        check(rc, "lara_kv_evict")
+    return new_lens
 
 
 class PagedKVCache:
+    """Page pool, block tables and lengths of many sequences.
+
+    ``scored=True`` also keeps a weight for every slot and kv head (``weights``, float32), the attention it has got from
+    :meth:`decode_scored` since its token was appended, by which :meth:`evict` chooses.
+    """
+
     def __init__(self, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, max_seqs: int,
-                 max_seq_len: int, device="cuda:0"):
+                 max_seq_len: int, device="cuda:0", scored: bool = False):
         if page_size < 16 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two >= 16")
         self.device = torch.device(device)
@@ -39,6 +152,10 @@ class PagedKVCache:
         self.num_pages, self.max_seqs = int(num_pages), int(max_seqs)
         self.pages_per_seq = int(math.ceil(max_seq_len / page_size))
         self._alloc_pages()
+        self.weights = None
+        if scored:
+            self.weights = torch.zeros((self.num_pages, self.n_kv_heads, self.page_size), dtype=torch.float32,
+                                       device=self.device)
         self._table = np.full((self.max_seqs, self.pages_per_seq), -1, np.int32)
         self.block_table = torch.from_numpy(self._table).to(self.device)
         self._lens = np.zeros(self.max_seqs, np.int32)
@@ -47,6 +164,7 @@ class PagedKVCache:
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._active = np.zeros(self.max_seqs, bool)
         self._ws = None
+        self._serving_ws = {}  # of decode_shared, decode_scored and evict
         self._status = new_workspace(256, self.device)
 
     def _alloc_pages(self) -> None:
@@ -102,7 +220,7 @@ class PagedKVCache:
 
     def reserve(self, slots, n_new: int) -> None:
         """Make sure each slot has pages for n_new more tokens."""
-        changed = []
+        changed, fresh = [], []
         for slot in slots:
             need_end = int(self._lens[slot]) + int(n_new)
             if need_end > self.capacity:
@@ -120,6 +238,9 @@ class PagedKVCache:
                     self._refs[page] = 1
                     self._table[slot, j] = page
                     changed.append(slot)
+                    fresh.append(page)
+        if fresh and self.weights is not None:  # what an earlier sequence's tokens gathered
+            self.weights.index_fill_(0, torch.as_tensor(np.asarray(fresh, np.int64), device=self.device), 0.0)
         if changed:
             self._sync_rows(sorted(set(changed)))
 
@@ -186,13 +307,84 @@ class PagedKVCache:
               "lara_gqa_decode_paged")
         return o
 
+    def _serving(self, name: str, nbytes: int) -> torch.Tensor:
+        ws = self._serving_ws.get(name)
+        if ws is None or ws.numel() < nbytes:
+            ws = self._serving_ws[name] = _workspace(nbytes, self.device)
+        return ws
+
+    def _rows_of(self, slots):
+        idx = torch.as_tensor(slots, device=self.device)
+        return idx, self.block_table.index_select(0, idx), self.lens.index_select(0, idx)
+
+    def _own_pages(self, slots, what: str) -> None:
+        """Refuse slots whose pages another sequence has too."""
+        for slot in slots:
+            pages = self._table[slot]
+            if np.any(self._refs[pages[pages >= 0]] > 1):
+                raise ValueError(f"{what}: sequence {int(slot)} has pages in common with another")
+        if len(set(slots.tolist())) != len(slots):
+            raise ValueError(f"{what}: a slot is named twice")
+
+    def _need_weights(self, what: str) -> None:
+        if self.weights is None:
+            raise ValueError(f"{what} needs a cache with weights (scored=True)")
+
+    def shared_pages(self, slots=None) -> int:
+        """How many pages all of the slots begin with in common."""
+        rows = self._table[self._slots(slots)]
+        same = (rows == rows[0]).all(0) & (rows[0] >= 0)
+        return int(same.size if same.all() else same.argmin())
+
+    def decode_shared(self, q, slots=None, scale=None):
+        """:meth:`decode`, reading the pages that all slots begin with (:meth:`share_prefix`) once for the batch."""
+        slots = self._slots(slots)
+        _check_words("q", q, (len(slots), q.shape[1], self.head_dim))
+        _, table, lens = self._rows_of(slots)
+        ws = self._serving("shared", int(lib.lara_decode_shared_workspace_bytes(len(slots), q.shape[1],
+                                                                                self.n_kv_heads, self.head_dim)))
+        shared = self.shared_pages(slots) if len(slots) > 1 else 0
+        return gqa_decode_shared(q, self.k_pages, self.v_pages, table, lens, shared, scale=scale, workspace=ws)
+
+    def decode_scored(self, q, slots=None, scale=None):
+        """:meth:`decode` that adds to each slot's weight what attention it gets (a cache with ``scored=True``)."""
+        self._need_weights("decode_scored")
+        slots = self._slots(slots)
+        _check_words("q", q, (len(slots), q.shape[1], self.head_dim))
+        self._own_pages(slots, "decode_scored")
+        _, table, lens = self._rows_of(slots)
+        ws = self._serving("scored", int(lib.lara_decode_scored_workspace_bytes(
+            len(slots), q.shape[1], self.n_kv_heads, self.head_dim, self.page_size, self.pages_per_seq,
+            self.num_pages)))
+        return gqa_decode_scored(q, self.k_pages, self.v_pages, self.weights, table, lens, scale=scale, workspace=ws)
+
+    def evict(self, keep: int, slots=None, *, first: int = 0, last: int = 0, sources=None) -> None:
+        """:func:`kv_evict` of the given slots (default: all active); pages behind ``keep`` are free again."""
+        self._need_weights("evict")
+        slots = self._slots(slots)
+        self._own_pages(slots, "evict")
+        idx, table, lens = self._rows_of(slots)
+        ws = self._serving("evict", int(lib.lara_kv_evict_workspace_bytes(len(slots), self.n_kv_heads,
+                                                                          max(int(keep), 1))))
+        new_lens = kv_evict(self.k_pages, self.v_pages, self.weights, table, lens, keep, first=first, last=last,
+                            sources=sources, workspace=ws)
+        self.lens.index_copy_(0, idx, new_lens)
+        self._lens[slots] = np.minimum(self._lens[slots], keep)
+        for slot in slots:
+            for j in range(-(-int(self._lens[slot]) // self.page_size), self.pages_per_seq):
+                if self._table[slot, j] >= 0:
+                    self._release(int(self._table[slot, j]))
+                    self._table[slot, j] = -1
+        self._sync_rows(slots)
+
     def status(self) -> int:
-        """Device status bits of the last appends and decodes (read and cleared)."""
+        """Device status bits of the last appends, decodes and evictions (read and cleared)."""
         from .ops import workspace_status
 
         bits = workspace_status(self._status)
-        if self._ws is not None:
-            bits |= workspace_status(self._ws)
+        for ws in (self._ws, *self._serving_ws.values()):
+            if ws is not None:
+                bits |= workspace_status(ws)
         return bits
 
     # ------------------------------------------------------------ contents

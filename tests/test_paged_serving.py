@@ -1,0 +1,324 @@
+"""Serving operators of the paged bf16 cache (``lara_b200.paged``): the decode behind a shared prefix, the decode that
+scores its cache, and eviction by gathered weight.
+
+Each is compared with its definition in 64 bits.  Tolerances:
+
+* decode, one bf16 rounding of the result (2^-8 of it), and relative to ``kappa = sum_t p_t |v_t|``: weights held in
+  two bf16 numbers (2^-8 of 2^-8), the exponential and its products (2^-21), the score in fp32 (D + 8 roundings of at
+  most 2^-23 of ``A = max_t scale sum_d |q_d k_td|``, above and below the line), and sums over n tokens (n 2^-22: a
+  tensor core may cut where it adds);
+* weights: the same without V, and one fp32 rounding of each of the sum's terms (2^-23);
+* eviction moves words and is exact.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+GEOMETRIES = [(1, 1, 128), (4, 1, 64), (8, 2, 128), (10, 2, 64), (21, 3, 128), (16, 2, 128), (15, 1, 64), (32, 2, 128)]
+
+
+# ------------------------------------------------------------------ inputs
+def make_cache(lens, hkv, d, page, seed, shared=0, spare=0):
+    """Pools with a NaN in every row that no sequence has, a table of pages in random order; all on the CPU."""
+    g = torch.Generator().manual_seed(seed)
+    per_seq = max(1, -(-max(lens) // page)) + spare
+    used = [max(0, -(-n // page) - shared) for n in lens]
+    pages = shared + sum(used) + 2
+    order = torch.randperm(pages, generator=g).to(torch.int32)
+    table = torch.full((len(lens), per_seq), -1, dtype=torch.int32)
+    table[:, :shared] = order[:shared]
+    at = shared
+    for b, u in enumerate(used):
+        table[b, shared:shared + u] = order[at:at + u]
+        at += u
+    k = torch.randn((pages, hkv, page, d), generator=g)
+    k[..., 1::d // 4] *= 6.0
+    v = torch.randn((pages, hkv, page, d), generator=g)
+    there = torch.zeros((pages, page), dtype=torch.bool)
+    for b, n in enumerate(lens):
+        t = torch.arange(n)
+        there[table[b].long()[t // page], t % page] = True
+    for x in (k, v):
+        x.masked_fill_(~there[:, None, :, None], math.nan)
+    return k.bfloat16(), v.bfloat16(), table, torch.tensor(lens, dtype=torch.int32)
+
+
+def rows64(x, table, b, n, page):
+    t = torch.arange(n)
+    return x[table[b].long()[t // page], :, t % page].double()  # [n, hkv, d]
+
+
+def decode64(q, k, v, table, lens, page, scale):
+    """o, kappa, A [B, Hq, D or 1], and the weights p [B][hkv, G, n]."""
+    B, hq, d = q.shape
+    hkv = k.shape[1]
+    o = torch.zeros((B, hq, d), dtype=torch.float64)
+    kappa, A, ps = torch.zeros_like(o), torch.zeros((B, hq, 1), dtype=torch.float64), []
+    for b in range(B):
+        n = int(lens[b])
+        if n == 0:
+            ps.append(None)
+            continue
+        ks, vs = (rows64(x, table, b, n, page).transpose(0, 1) for x in (k, v))
+        qs = q[b].double().view(hkv, -1, d)
+        p = torch.softmax(qs @ ks.transpose(1, 2) * scale, -1)
+        ps.append(p)
+        o[b] = (p @ vs).view(hq, d)
+        kappa[b] = (p @ vs.abs()).view(hq, d)
+        A[b] = ((qs.abs() @ ks.abs().transpose(1, 2)) * scale).amax(-1).view(hq, 1)
+    return o, kappa, A, ps
+
+
+def relative(A, d, n):
+    return 2.0 ** -16 + 2.0 ** -21 + 2 * (d + 8) * 2.0 ** -23 * A + n * 2.0 ** -22
+
+
+def check_out(got, o, kappa, A, lens):
+    n = lens.double().view(-1, 1, 1)
+    tol = 2.0 ** -8 * o.abs() + kappa * relative(A, o.shape[-1], n)
+    err = (got.cpu().double() - o).abs()
+    assert torch.isfinite(got.float()).all()
+    assert (err <= tol).all(), f"{float((err - tol).max())} over the tolerance, {int((err > tol).sum())} values"
+
+
+def check_weights(got, before, ps, A, table, lens, page, d):
+    want, tol = before.double().clone(), 2.0 ** -23 * before.double().abs()
+    touched = torch.zeros(before.shape, dtype=torch.bool)
+    for b, p in enumerate(ps):
+        if p is None:
+            continue
+        n, (hkv, G) = p.shape[2], p.shape[:2]
+        rel = relative(A[b].view(hkv, G, 1), d, n) + G * 2.0 ** -23
+        t = torch.arange(n)
+        at = (table[b].long()[t // page], slice(None), t % page)
+        want[at] += p.sum(1).t()
+        tol[at] += (p * rel).sum(1).t() + 2.0 ** -23 * want[at].abs()
+        touched[at] = True
+    got = got.cpu()
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), f"{float((err - tol).max())} over the tolerance"
+    assert torch.equal(got[~touched], before[~touched])
+
+
+def evict64(k, v, w, table, lens, page, keep, first, last):
+    """The definition, slot by slot: new k, v, w, sources, lengths."""
+    k, v, w = k.clone(), v.clone(), w.clone()
+    B, hkv = len(lens), k.shape[1]
+    src = torch.full((B, hkv, keep), -1, dtype=torch.int32)
+    for b in range(B):
+        n = int(lens[b])
+        page_of = [int(x) for x in table[b]]
+        for h in range(hkv):
+            if n <= keep:
+                src[b, h, :n] = torch.arange(n)
+                continue
+            at = [(page_of[t // page], h, t % page) for t in range(n)]
+            ws = [float(w[x]) for x in at]
+            heavy = lambda t: (math.inf if math.isnan(ws[t]) else ws[t], math.isnan(ws[t]))  # noqa: E731
+            middle = sorted(range(first, n - last), key=lambda t: (heavy(t), -t), reverse=True)
+            kept = set(range(first)) | set(range(n - last, n)) | set(middle[:keep - first - last])
+            holes = [t for t in range(keep) if t not in kept]
+            movers = sorted(t for t in kept if t >= keep)
+            assert len(holes) == len(movers)
+            src[b, h] = torch.arange(keep)
+            for t, s in zip(holes, movers):
+                k[at[t]], v[at[t]], w[at[t]] = k[at[s]], v[at[s]], w[at[s]]
+                src[b, h, t] = s
+            for t in range(keep, n):
+                w[at[t]] = 0.0
+    return k, v, w, src, torch.clamp(lens, max=keep)
+
+
+def words(x):
+    return x.cpu().contiguous().view(torch.int16 if x.dtype == torch.bfloat16 else torch.int32)
+
+
+def dev(*xs):
+    return [x.cuda() for x in xs]
+
+
+# ------------------------------------------------------------------ decode with scores
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", GEOMETRIES)
+@pytest.mark.parametrize("page,lens", [(16, [1]), (16, [17, 0, 1, 16, 300, 33]), (64, [1000, 0, 63, 64, 65]),
+                                       (256, [5000])])
+def test_scored_decode(hq, hkv, d, page, lens):
+    from lara_b200 import ops, paged
+
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=hq * 7 + d + page, spare=2)
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn((len(lens), hq, d), generator=g).bfloat16()
+    w = torch.rand(k.shape[:3], generator=g)
+    scale = 1.0 / math.sqrt(d)
+    o, kappa, A, ps = decode64(q, k, v, table, n, page, scale)
+    qd, kd, vd, wd, td, nd = dev(q, k, v, w, table, n)
+    ws = paged.scored_workspace(len(lens), hq, kd, table.shape[1])
+    apart = torch.full_like(wd, -7.0)
+    for _ in range(2):  # the weights apart from the old ones, twice, then in place
+        got = paged.gqa_decode_scored(qd, kd, vd, wd, td, nd, weights_out=apart, workspace=ws)
+        check_out(got, o, kappa, A, n)
+    again = paged.gqa_decode_scored(qd, kd, vd, wd, td, nd)
+    assert torch.equal(words(again), words(got))
+    check_weights(wd, w, ps, A, table, n, page, d)
+    there = apart != -7.0
+    assert torch.equal(apart[there], wd[there])
+    assert torch.equal(wd.cpu()[~there.cpu()], w[~there.cpu()])
+    assert ops.workspace_status(ws) == 0
+
+
+# ------------------------------------------------------------------ decode behind a shared prefix
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", GEOMETRIES)
+@pytest.mark.parametrize("page,shared,lens", [
+    (16, 1, [17, 16, 40]), (16, 9, [150, 144, 145, 0, 143, 16, 1]), (64, 5, [400, 321, 320, 100]),
+    (16, 63, [1009] * 40 + [1008, 5]), (256, 4, [1300, 1024]), (32, 0, [70, 3]), (32, 4, [128] * 3)])
+def test_shared_decode(hq, hkv, d, page, shared, lens):
+    from lara_b200 import ops, paged
+
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=hq + d + page + shared, shared=shared)
+    q = torch.randn((len(lens), hq, d), generator=torch.Generator().manual_seed(9)).bfloat16()
+    o, kappa, A, _ = decode64(q, k, v, table, n, page, 0.11)
+    qd, kd, vd, td, nd = dev(q, k, v, table, n)
+    ws = paged.shared_workspace(len(lens), hq, hkv, d, "cuda")
+    got = paged.gqa_decode_shared(qd, kd, vd, td, nd, shared, scale=0.11, workspace=ws)
+    check_out(got, o, kappa, A, n)
+    assert torch.equal(words(paged.gqa_decode_shared(qd, kd, vd, td, nd, shared, scale=0.11, workspace=ws)), words(got))
+    out = qd.clone()
+    paged.gqa_decode_shared(out, kd, vd, td, nd, shared, scale=0.11, workspace=ws, out=out)
+    assert torch.equal(words(out), words(got))
+    assert ops.workspace_status(ws) == 0
+
+
+# ------------------------------------------------------------------ eviction
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,lens,keep,first,last", [
+    (16, [2], 1, 0, 0), (16, [40, 0, 17, 16, 15, 1], 16, 0, 0), (16, [40, 33, 300], 32, 32, 0),
+    (16, [40, 33, 300], 32, 0, 32), (64, [1000, 513, 700], 512, 4, 100), (256, [3000], 700, 3, 7),
+    (16, [500, 90], 100, 30, 70), (16, [64, 10], 640, 1, 1), (32, [9000], 8999, 2, 2), (32, [9000], 1, 0, 0)])
+@pytest.mark.parametrize("hkv,d", [(1, 64), (3, 128)])
+@pytest.mark.parametrize("kind", ["any", "ties", "special"])
+def test_evict(page, lens, keep, first, last, hkv, d, kind):
+    from lara_b200 import ops, paged
+
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=keep + d, spare=1)
+    g = torch.Generator().manual_seed(3)
+    w = torch.exp(torch.randn(k.shape[:3], generator=g) * 3)
+    if kind == "ties":
+        w = torch.randint(0, 4, w.shape, generator=g).float()
+    if kind == "special":
+        pick = torch.randint(0, 9, w.shape, generator=g)
+        for i, x in enumerate((math.inf, -math.inf, math.nan, 0.0, -0.0, 1e-42, -1e-42)):
+            w[pick == i] = x
+        w[pick == 7] *= -1.0
+    want = evict64(k, v, w, table, n, page, keep, first, last)
+    for apart in (False, True):
+        kd, vd, wd, td, nd = dev(k, v, w, table, n)
+        w_out = wd.clone() if apart else wd
+        src = torch.full((len(lens), hkv, keep), 99, dtype=torch.int32, device="cuda")
+        ws = paged.evict_workspace(len(lens), hkv, keep, "cuda")
+        new = paged.kv_evict(kd, vd, wd, td, nd, keep, first=first, last=last, weights_out=w_out, sources=src,
+                             workspace=ws)
+        assert torch.equal(new.cpu(), want[4]) and torch.equal(nd.cpu(), n)
+        assert torch.equal(src.cpu(), want[3])
+        for got, x in zip((kd, vd, w_out), want):
+            assert torch.equal(words(got), words(x))
+        if apart:
+            assert torch.equal(words(wd), words(w))
+        assert ops.workspace_status(ws) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,keep", [([70000, 5, 40001], 1003), ([300000], 150001)])
+def test_evict_long(lens, keep):
+    """Units that a cluster of CTAs selects from, against a sort."""
+    from lara_b200 import paged
+
+    hkv, d, page = 2, 64, 64
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=1)
+    w = torch.randint(0, 5000, k.shape[:3], generator=torch.Generator().manual_seed(2)).float() / 64
+    kd, vd, wd, td, nd = dev(k, v, w, table, n)
+    src = torch.empty((len(lens), hkv, keep), dtype=torch.int32, device="cuda")
+    paged.kv_evict(kd, vd, wd, td, nd, keep, first=3, last=77, sources=src)
+    src, w_new = src.cpu(), wd.cpu()
+    for b, m in enumerate(lens):
+        t = torch.arange(m)
+        at = (table[b].long()[t // page], t % page)
+        for h in range(hkv):
+            if m <= keep:
+                assert src[b, h].tolist() == list(range(m)) + [-1] * (keep - m)
+                continue
+            x = w[at[0], h, at[1]]
+            x[:3] = x[m - 77:] = math.inf
+            kept = torch.zeros(m, dtype=torch.bool)
+            kept[torch.sort(x, descending=True, stable=True).indices[:keep]] = True
+            want = torch.arange(keep)
+            want[~kept[:keep]] = torch.nonzero(kept[keep:]).flatten() + keep
+            assert torch.equal(src[b, h].long(), want)
+            now = w_new[at[0], h, at[1]]
+            assert torch.equal(now[:keep], w[at[0], h, at[1]][want]) and not now[keep:].any()
+            for new, old in ((kd, k), (vd, v)):
+                assert torch.equal(words(new[:, h].cpu()[at[0], at[1]][:keep]), words(old[at[0], h, at[1]][want]))
+
+
+# ------------------------------------------------------------------ the cache's methods, together
+@pytest.mark.gpu
+def test_serving_loop():
+    """Prompts behind a shared prefix decode; then scored steps, evictions and appends, against a model on the CPU."""
+    from lara_b200.paged import PagedKVCache
+
+    hq, hkv, d, page = 8, 2, 64, 16
+    g = torch.Generator().manual_seed(11)
+    rows = lambda n: torch.randn((1, hkv, n, d), generator=g).bfloat16()  # noqa: E731
+    cache = PagedKVCache(64, page, hkv, d, 4, 320, "cuda")
+    cache.new_sequence()
+    doc = rows(70), rows(70)
+    cache.append(doc[0].cuda(), doc[1].cuda(), [0])
+    own = {}
+    for s in (1, 2):
+        assert cache.new_sequence() == s
+        assert cache.share_prefix(0, s, 70) == 64
+        own[s] = rows(s * 9), rows(s * 9)
+        cache.append(own[s][0].cuda(), own[s][1].cuda(), [s])
+    assert cache.shared_pages() == 4
+    q = torch.randn((3, hq, d), generator=g).bfloat16()
+    got = cache.decode_shared(q.cuda())
+    lens = torch.tensor([70, 73, 82])
+    args = decode64(q, cache.k_pages.cpu(), cache.v_pages.cpu(), cache.block_table.cpu(), lens, page, d ** -0.5)
+    check_out(got, *args[:3], lens)
+    assert cache.status() == 0
+
+    cache = PagedKVCache(24, page, hkv, d, 2, 160, "cuda", scored=True)
+    have = {}
+    for s, n in ((0, 100), (1, 31)):
+        assert cache.new_sequence() == s
+        x = rows(n), rows(n)
+        cache.append(x[0].cuda(), x[1].cuda(), [s])
+        have[s] = n
+    for step in range(40):
+        new = torch.randn((2, hkv, 1, d), generator=g).bfloat16(), torch.randn((2, hkv, 1, d), generator=g).bfloat16()
+        cache.append(new[0].cuda(), new[1].cuda())
+        have = {s: n + 1 for s, n in have.items()}
+        before = cache.weights.cpu()
+        q = torch.randn((2, hq, d), generator=g).bfloat16()
+        got = cache.decode_scored(q.cuda())
+        lens = torch.tensor([have[0], have[1]], dtype=torch.int32)
+        table = cache.block_table.cpu()
+        args = decode64(q, cache.k_pages.cpu(), cache.v_pages.cpu(), table, lens, page, d ** -0.5)
+        check_out(got, *args[:3], lens)
+        check_weights(cache.weights, before, args[3], args[2], table, lens, page, d)
+        if step % 5 == 4:
+            state = [x.cpu() for x in (cache.k_pages, cache.v_pages, cache.weights)]
+            want = evict64(*state, table, lens, page, 48, 2, 5)
+            src = torch.empty((2, hkv, 48), dtype=torch.int32, device="cuda")
+            cache.evict(48, first=2, last=5, sources=src)
+            have = {s: min(n, 48) for s, n in have.items()}
+            for x, y in zip((cache.k_pages, cache.v_pages, cache.weights, src, cache.lens), want):
+                assert torch.equal(words(x), words(y))
+            assert [cache.seq_len(s) for s in (0, 1)] == [have[0], have[1]]
+            assert cache.free_pages == 24 - sum(-(-n // page) for n in have.values())
+    assert cache.status() == 0
