@@ -180,8 +180,9 @@ int device_sm_count();
 // Launch `fn` with programmatic stream serialization, so its CTAs may be
 // scheduled while the previous kernel in the stream finishes (the kernel must
 // call grid_dependency_wait() before touching global memory).  LARA_PDL=0
-// launches it the ordinary way.
-cudaError_t launch_with_pdl(const void* fn, dim3 grid, dim3 block, void** args, size_t smem, cudaStream_t stream);
+// launches it the ordinary way.  `cluster`: CTAs of a thread-block cluster.
+cudaError_t launch_with_pdl(const void* fn, dim3 grid, dim3 block, void** args, size_t smem, cudaStream_t stream,
+                            int cluster = 1);
 
 // Record the calling thread's last error message (lara_last_error_string)
 // and return `code`.

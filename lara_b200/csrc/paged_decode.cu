@@ -55,11 +55,12 @@ struct Args {
   int batch, n_q_heads, group;
   float scale_log2;
   int* status;
-  UnitParts* units;  // [batch * kv heads]
+  UnitParts* units;  // [batch * kv heads]; of sequences without tokens, undefined
+  long long* seq_tiles;  // [batch + 1] tiles of one kv head of the sequences before this one
   float2* part_ml;   // [units + CTAs][group] (R, l)
   float* part_acc;   // [units + CTAs][group][D]
   // scoring
-  float* scores;          // [tiles][kTile][group], in the order of the units
+  float* scores;          // [tiles][group][kTile], in the order of the units
   long long score_tiles;  // that there is room for
   const float* w_in;      // [pages][kv heads][page]
   float* w_out;
@@ -187,6 +188,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     all += s_sum[w];
   }
   constexpr long long kLow = (1ll << 40) - 1;
+  if (kScored && blockIdx.x == 0) {
+    long long at = ahead & kLow;
+    for (int b = b_lo; b < b_hi; ++b) {
+      a.seq_tiles[b] = at;
+      at += tiles_of(len_of(b));
+    }
+    if (b_hi == a.batch) a.seq_tiles[a.batch] = at;  // of every thread at or behind the last sequence, alike
+  }
   const long long total = (all & kLow) * hkv, units = (all >> 40) * hkv;
   if (total == 0) return;
   const long long span = total + units * kUnitCost;
@@ -336,19 +345,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
       if constexpr (kScored) {
         const long long tile = u.tile0 + (id - u.base);
         if (tile < a.score_tiles) {
-          float* dst = a.scores + (tile * kTile + g) * G + 2 * t4;
+          float* const dst = a.scores + (tile * G + 2 * t4) * kTile + g;
 #pragma unroll
           for (int n = 0; n < NG; ++n)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float* const to = dst + 8 * i * G + 8 * n;
-              if (!(G & 1) && 8 * n + 2 * t4 < G) {
-                *reinterpret_cast<float2*>(to) = make_float2(s[n][2 * i], s[n][2 * i + 1]);
-              } else {
-                if (8 * n + 2 * t4 < G) to[0] = s[n][2 * i];
-                if (8 * n + 2 * t4 + 1 < G) to[1] = s[n][2 * i + 1];
-              }
-            }
+            for (int i = 0; i < 4; ++i)
+              if (8 * n + 2 * t4 + (i & 1) < G) dst[(8 * n + (i & 1)) * kTile + 8 * (i >> 1)] = s[n][i];
         }
       }
 
@@ -467,36 +469,33 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
 
 // ---- the second launch ----
 constexpr int kJoinThreads = 128;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kAhead = 4;      // tokens of a lane whose scores are in flight
+constexpr int kFewParts = 16;  // parts of a row that one warp joins
 
-// Joins the parts of one output row per warp (few parts) or, row after row, per block.
+// Joins the parts of kJoinWarps output rows: a warp to a row, and the rows of many
+// parts by the whole block, one after the other.
 template <int D>
 __device__ __forceinline__ void join_rows(const Args& a, int block) {
-  constexpr int kLanes = D / 4, kSub = kJoinThreads / kLanes;  // lanes of a row, rows in flight
+  constexpr int kLanes = D / 4, kSub = kJoinThreads / kLanes;  // lanes of a row, parts in flight
   __shared__ float4 s_x[kSub][kLanes];
   __shared__ float s_l[kSub];
+  __shared__ UnitParts s_many[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.group;
-  const long long rows = (long long)a.batch * a.n_q_heads;
-  for (int r = 0; r < kJoinThreads / 32; ++r) {
-    const long long row = (long long)block * (kJoinThreads / 32) + r;
-    if (row >= rows) return;
-    const int b = (int)(row / a.n_q_heads), hq = (int)(row % a.n_q_heads), kvh = hq / G, h = hq % G;
-    uint16_t* const out = a.o + row * D;
-    const int len = __ldcg(a.lens + b);
-    const int sub = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
-    if (len <= 0) {
-      if (threadIdx.x < D / 8) reinterpret_cast<uint4*>(out)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    const UnitParts up = a.units[b * a.index.n_kv_heads + kvh];
+  const long long rows = (long long)a.batch * a.n_q_heads, row0 = (long long)block * kJoinWarps;
+  auto largest = [&](const UnitParts& up, int h) {
     float M = -INFINITY;
     for (int i = lane; i < up.parts; i += 32) M = fmaxf(M, __ldcg(a.part_ml + (long long)(up.slot0 + i) * G + h).x);
 #pragma unroll
     for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    return M;
+  };
+  // parts i0, i0 + step, ..
+  auto sum = [&](const UnitParts& up, int h, float M, int i0, int step, int at, float& L) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
 #pragma unroll 4
-    for (int i = sub; i < up.parts; i += kSub) {
+    for (int i = i0; i < up.parts; i += step) {
       const long long p = (long long)(up.slot0 + i) * G + h;
       const float2 ml = __ldcg(a.part_ml + p);
       const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_acc + p * D) + at);
@@ -507,101 +506,155 @@ __device__ __forceinline__ void join_rows(const Args& a, int block) {
       x.z = fmaf(y.z, f, x.z);
       x.w = fmaf(y.w, f, x.w);
     }
-    __syncthreads();
-    s_x[sub][at] = x;
+    return x;
+  };
+  auto store = [&](long long row, int at, const float4& x, float L) {
+    const float inv = 1.f / L;
+    reinterpret_cast<uint2*>(a.o + row * D)[at] =
+        make_uint2(pack2_rn(x.x * inv, x.y * inv), pack2_rn(x.z * inv, x.w * inv));
+  };
+  {
+    const long long row = row0 + warp;
+    UnitParts up{0, 0, 0};
+    if (row < rows) {
+      const int b = (int)(row / a.n_q_heads), hq = (int)(row % a.n_q_heads), h = hq % G;
+      const int len = __ldcg(a.lens + b);
+      if (len > 0) up = a.units[b * a.index.n_kv_heads + hq / G];
+      const int at = lane % kLanes;
+      if (len <= 0) {
+        if (lane < kLanes) reinterpret_cast<uint2*>(a.o + row * D)[at] = make_uint2(0, 0);
+      } else if (up.parts <= kFewParts) {
+        float L = 0.f;
+        const float4 x = sum(up, h, largest(up, h), 0, 1, at, L);
+        if (lane < kLanes) store(row, at, x, L);
+      }
+    }
+    if (lane == 0) s_many[warp] = up;
+  }
+  __syncthreads();
+  for (int r = 0; r < kJoinWarps; ++r) {
+    const UnitParts up = s_many[r];
+    if (up.parts <= kFewParts) continue;
+    const int h = (int)((row0 + r) % a.n_q_heads) % G, sub = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
+    float L = 0.f;
+    const float4 part = sum(up, h, largest(up, h), sub, kSub, at, L);
+    s_x[sub][at] = part;
     if (at == 0) s_l[sub] = L;
     __syncthreads();
-    if (warp == 0 && lane < kLanes) {
-      x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (threadIdx.x < kLanes) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       L = 0.f;
 #pragma unroll
       for (int i = 0; i < kSub; ++i) {
-        const float4 y = s_x[i][lane];
+        const float4 y = s_x[i][at];
         L += s_l[i];
         x.x += y.x;
         x.y += y.y;
         x.z += y.z;
         x.w += y.w;
       }
-      const float inv = 1.f / L;
-      reinterpret_cast<uint2*>(out)[lane] = make_uint2(pack2_rn(x.x * inv, x.y * inv), pack2_rn(x.z * inv, x.w * inv));
+      store(row0 + r, at, x, L);
     }
+    __syncthreads();
   }
 }
 
-// Adds the weights of the tokens of one unit that lie in tiles [t0, t1) of all.
-__device__ __forceinline__ void add_weights(const Args& a, int block, int blocks) {
-  __shared__ float s_m[16], s_inv[16];
-  __shared__ long long s_total;
+// Adds the weights of the tiles [lo, hi) of all, which one warp takes, a token to a lane.
+__device__ __forceinline__ void add_weights(const Args& a, long long warp, long long warps, float2* ml) {
+  const int lane = threadIdx.x & 31;
   const int G = a.group, hkv = a.index.n_kv_heads;
-  const int n_units = a.batch * hkv;
-  const long long cap = a.index.capacity();
-  auto len_of = [&](int b) { return (int)min((long long)max(__ldcg(a.lens + b), 0), cap); };
-  // the last unit with tokens says how many tiles there are
-  if (threadIdx.x == 0) {
-    int b = a.batch - 1;
-    while (b >= 0 && len_of(b) == 0) --b;
-    s_total = b < 0 ? 0 : a.units[b * hkv + hkv - 1].tile0 + tiles_of(len_of(b));
-  }
-  __syncthreads();
-  const long long total = s_total;
-  const long long per = (total + blocks - 1) / blocks;
-  const long long lo = block * per, hi = min(total, lo + per);
+  const int log2 = a.index.page_log2;
+  const long long total = __ldcg(a.seq_tiles + a.batch) * hkv;
+  const long long room = min(total, a.score_tiles);
+  if (room < total && warp == 0 && lane == 0) atomicOr(a.status, kDevScoreRoom);
+  const long long per = (room + warps - 1) / warps;
+  const long long lo = warp * per, hi = min(room, lo + per);
   if (lo >= hi) return;
-  if (hi > a.score_tiles) {
-    if (threadIdx.x == 0) atomicOr(a.status, kDevScoreRoom);
-  }
-  long long at = 0;  // tiles before unit i
-  for (int i = 0; i < n_units && at < hi; ++i) {
-    const int b = i / hkv, len = len_of(b), tiles = tiles_of(len);
-    if (at + tiles <= lo || tiles == 0) {
-      at += tiles;
-      continue;
-    }
-    const UnitParts up = a.units[i];
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      for (int h = 0; h < G; ++h) {
-        float M = -INFINITY, L = 0.f;
-        for (int p = threadIdx.x; p < up.parts; p += 32)
-          M = fmaxf(M, __ldcg(a.part_ml + (long long)(up.slot0 + p) * G + h).x);
-#pragma unroll
-        for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-        for (int p = threadIdx.x; p < up.parts; p += 32) {
-          const float2 ml = __ldcg(a.part_ml + (long long)(up.slot0 + p) * G + h);
-          L = fmaf(ml.y, ml.x == M ? 1.f : ex2_ftz(ml.x - M), L);
-        }
-#pragma unroll
-        for (int off = 16; off; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-        if (threadIdx.x == 0) {
-          s_m[h] = M;
-          s_inv[h] = 1.f / L;
-        }
+  int b = 0;  // the last sequence that starts at or before tile lo, and so one with tokens
+  for (int step = 1 << (31 - __clz(a.batch)); step; step >>= 1)
+    if (b + step < a.batch && __ldcg(a.seq_tiles + b + step) * hkv <= lo) b += step;
+  long long first = __ldcg(a.seq_tiles + b);
+  int tiles = (int)(__ldcg(a.seq_tiles + b + 1) - first);
+  int kvh = (int)quotient(lo - first * hkv, tiles);
+  long long at = first * hkv + (long long)kvh * tiles;  // the unit's first tile
+  while (true) {
+    const int unit = b * hkv + kvh;
+    const UnitParts up = a.units[unit];
+    const int len = (int)min((long long)__ldcg(a.lens + b), a.index.capacity());
+    // each head's (M, 1 / L): lanes h and h + 16 take every other part
+    float M = -INFINITY, L = 0.f;
+    const int h = lane & 15;
+    const float2* const src = a.part_ml + (long long)up.slot0 * G + h;
+    if (h < G)
+      for (int p = lane >> 4; p < up.parts; p += 2) M = fmaxf(M, __ldcg(src + (long long)p * G).x);
+    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+    if (h < G)
+      for (int p = lane >> 4; p < up.parts; p += 2) {
+        const float2 x = __ldcg(src + (long long)p * G);
+        L = fmaf(x.y, x.x == M ? 1.f : ex2_ftz(x.x - M), L);
       }
-    }
-    __syncthreads();
-    const long long t0 = max(lo, at), t1 = min(min(hi, at + tiles), a.score_tiles);
-    for (long long x = t0 * kTile + threadIdx.x; x < t1 * kTile; x += blockDim.x) {
-      const int t = (int)(x - at * kTile);
-      if (t >= len) break;
-      const long long row = a.index.row(b, i % hkv, t, nullptr);
-      if (row < 0) continue;  // flagged where its rows were read
-      float w = 0.f;
-      for (int h = 0; h < G; ++h) w = fmaf(ex2_ftz(__ldcg(a.scores + x * G + h) - s_m[h]), s_inv[h], w);
-      a.w_out[row] = a.w_in[row] + w;
+    L += __shfl_xor_sync(0xffffffffu, L, 16);
+    __syncwarp();
+    if (lane < G) ml[h] = make_float2(M, 1.f / L);
+    __syncwarp();
+    const int t0 = (int)(max(lo, at) - at) * kTile, t1 = min((int)(min(hi, at + tiles) - at) * kTile, len);
+    const int32_t* const pages = a.index.block_table + (long long)b * a.index.pages_per_seq;
+    auto page_of = [&](int t) { return t < t1 ? __ldg(pages + (t >> log2)) : -1; };
+    int page[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) page[j] = page_of(t0 + 32 * j + lane);
+    for (int t = t0 + lane; t < t1 + lane; t += 32 * kAhead) {  // as often in every lane
+      const float* s[kAhead];
+      long long row[kAhead];
+      float w[kAhead], old[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int x = t + 32 * j;
+        const bool there = x < t1 && (unsigned)page[j] < (unsigned)a.index.num_pages;  // else flagged before
+        row[j] = there ? (((long long)page[j] * hkv + kvh) << log2) + (x & ((1 << log2) - 1)) : -1;
+        s[j] = a.scores + (there ? (at + x / kTile) * (G * kTile) + x % kTile : 0);
+        w[j] = 0.f;
+        old[j] = 0.f;
+        if (there) old[j] = __ldcg(a.w_in + row[j]);
+        page[j] = page_of(x + 32 * kAhead);
+      }
+#pragma unroll 4
+      for (int i = 0; i < G; ++i) {
+        const float2 x = ml[i];
+        float y[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) y[j] = __ldcg(s[j] + i * kTile);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) w[j] = fmaf(ex2_ftz(y[j] - x.x), x.y, w[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (row[j] >= 0) a.w_out[row[j]] = old[j] + w[j];
     }
     at += tiles;
+    if (at >= hi) return;
+    if (++kvh == hkv) {
+      kvh = 0;
+      do {
+        ++b;
+        first = __ldcg(a.seq_tiles + b);
+        tiles = (int)(__ldcg(a.seq_tiles + b + 1) - first);
+      } while (tiles == 0);
+    }
   }
 }
 
 template <int D, bool kScored>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args a, int join_blocks) {
+  __shared__ float2 s_ml[kJoinWarps][16];
   allow_dependent_launch();
   grid_dependency_wait();
   if ((int)blockIdx.x < join_blocks) {
     join_rows<D>(a, blockIdx.x);
   } else if constexpr (kScored) {
-    add_weights(a, blockIdx.x - join_blocks, gridDim.x - join_blocks);
+    const int warp = threadIdx.x >> 5;
+    add_weights(a, (long long)(blockIdx.x - join_blocks) * kJoinWarps + warp,
+                (long long)(gridDim.x - join_blocks) * kJoinWarps, s_ml[warp]);
   }
 }
 
@@ -609,7 +662,7 @@ int max_ctas() { return device_sm_count() * 2; }
 
 // Workspace: status word | units | partial results | scores.
 struct Layout {
-  size_t units_off, ml_off, acc_off, scores_off, total;
+  size_t units_off, seq_off, ml_off, acc_off, scores_off, total;
   long long score_tiles;
 };
 
@@ -617,7 +670,8 @@ Layout layout(int batch, int n_kv_heads, int group, int head_dim, long long scor
   const size_t units = (size_t)batch * n_kv_heads, slots = units + max_ctas();
   Layout w;
   w.units_off = kStatusBytes;
-  w.ml_off = w.units_off + up256(units * sizeof(UnitParts));
+  w.seq_off = w.units_off + up256(units * sizeof(UnitParts));
+  w.ml_off = w.seq_off + up256(((size_t)batch + 1) * sizeof(long long));
   w.acc_off = w.ml_off + up256(slots * group * sizeof(float2));
   w.scores_off = w.acc_off + up256(slots * group * head_dim * sizeof(float));
   w.score_tiles = score_tokens / kTile * n_kv_heads;
@@ -651,9 +705,9 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
   cudaError_t e = launch_with_pdl(fn, dim3((unsigned)ctas), dim3(kThreads), p, C::kSmemBytes, stream);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.batch * a.n_q_heads;
-  int join_blocks = (int)((rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+  int join_blocks = (int)((rows + kJoinWarps - 1) / kJoinWarps);
   int blocks = join_blocks;
-  if (kScored) blocks += (int)std::min<long long>(device_sm_count() * 8, (tiles + 7) / 8);
+  if (kScored) blocks += (int)std::min<long long>(device_sm_count() * 16, (tiles + 4 * kJoinWarps - 1) / (4 * kJoinWarps));
   void* p2[] = {&args, &join_blocks};
   return launch_with_pdl(reinterpret_cast<const void*>(&join_kernel<D, kScored>), dim3((unsigned)blocks),
                          dim3(kJoinThreads), p2, 0, stream);
@@ -736,6 +790,7 @@ void place(Args& a, const Layout& w, void* workspace) {
   char* base = static_cast<char*>(workspace);
   a.status = reinterpret_cast<int*>(base);
   a.units = reinterpret_cast<UnitParts*>(base + w.units_off);
+  a.seq_tiles = reinterpret_cast<long long*>(base + w.seq_off);
   a.part_ml = reinterpret_cast<float2*>(base + w.ml_off);
   a.part_acc = reinterpret_cast<float*>(base + w.acc_off);
   a.scores = reinterpret_cast<float*>(base + w.scores_off);

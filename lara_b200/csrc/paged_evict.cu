@@ -30,12 +30,18 @@ using namespace paged;
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kKeysCached = 32768;  // keys of a CTA's slice kept in shared memory
-constexpr int kMaxCluster = 8;
+constexpr int kRows = 2;             // rows of 128 slots that a warp has in flight
+constexpr int kMaxCluster = 16;
+constexpr int kShortSlice = 8192;    // slots of a CTA's slice up to which its CTA is a small one
+constexpr int kLongSlice = 32768;    // slots of a slice above which clusters grow whatever the units
+constexpr int kMostEntries = 2048;   // of the block table in shared memory
+// Dynamic shared memory: three small or two large CTAs to an SM; of slices of up to
+// kMostSlots (2^24 slots to a sequence), whose bits alone are more, one.
+constexpr int kShortSmem = 56 * 1024, kLongSmem = 92 * 1024, kMostSmem = 200 * 1024;
+constexpr long long kMostSlots = 1ll << 24;
 constexpr int kMoveThreads = 256;
+constexpr int kFlight = 8;           // 16-byte accesses of a lane in flight
 
 struct Args {
   uint16_t* k;
@@ -47,7 +53,6 @@ struct Args {
   int32_t* new_lens;  // or null
   int32_t* sources;   // [units][keep], or null
   int batch, head_dim, keep, first, last;
-  int slice_cached;   // keys of a slice that shared memory has room for
   int* status;
   int* counts;        // [units] rows to move
   int* holes;         // [units][keep]
@@ -67,19 +72,56 @@ __device__ __forceinline__ int slots_of(const Args& a, int b, int* raw = nullptr
   return (int)min((long long)max(n, 0), a.index.capacity());
 }
 
-__global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ Args a) {
-  extern __shared__ uint32_t s_keys[];
-  __shared__ uint32_t s_hist[kBins];
-  __shared__ uint32_t s_all[kBins];
-  __shared__ int s_scan[kWarps + 1];
+// Exclusive prefix of one number per thread over the block, and the sum of all.
+template <int kWarpsHere, typename T>
+__device__ __forceinline__ T block_prefix(T x, T* s_scan, T& all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  T incl = x;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += y;
+  }
+  __syncthreads();
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  T w = lane < kWarpsHere ? s_scan[lane] : T(0);
+#pragma unroll
+  for (int off = 1; off < kWarpsHere; off <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, w, off);
+    if (lane >= off) w += y;
+  }
+  all = __shfl_sync(0xffffffffu, w, kWarpsHere - 1);
+  return incl - x + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : T(0));
+}
+
+// What shared memory holds of a CTA's slice: which slots stay (a bit each), the
+// keys of the first slots of each warp's run, the first entries of the table; each
+// a multiple of four words.
+struct SliceRoom {
+  int words, run_keys, entries;
+};
+
+// kLong: clusters of CTAs, and slices that shared memory need not hold; without it, one CTA to a
+// unit, and all of that left out, since code that runs once waits mostly for its own instructions.
+template <int kThreads, int kCtas, bool kLong>
+__global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_constant__ Args a, const SliceRoom room) {
+  constexpr int kWarps = kThreads / 32;
+  constexpr uint32_t kFull = 0xffffffffu;
+  extern __shared__ uint32_t s_kept[];
+  uint32_t* const s_keys = s_kept + room.words;
+  int* const s_entry = reinterpret_cast<int*>(s_keys + room.run_keys * kWarps);
+  __shared__ uint32_t s_hist[2][kBins];  // of even and odd lanes: fewer of a warp meet in a bin
+  __shared__ int s_scan[kWarps];
   __shared__ int s_totals[3];  // this CTA's, read by the cluster: ties, holes, movers
-  __shared__ uint32_t s_pick[2];
+  __shared__ uint32_t s_pick[3];
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = cluster.block_rank(), size = cluster.num_blocks();
+  const int rank = kLong ? cluster.block_rank() : 0, size = kLong ? cluster.num_blocks() : 1;
   const int unit = blockIdx.x / size, hkv = a.index.n_kv_heads, b = unit / hkv, h = unit % hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   allow_dependent_launch();
+  for (int i = threadIdx.x; i < 2 * kBins; i += kThreads) s_hist[0][i] = 0;
   grid_dependency_wait();
 
   int raw;
@@ -90,183 +132,293 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     if (h == 0 && a.new_lens) a.new_lens[b] = min(n, a.keep);
   }
   const bool copies = a.w_in != a.w_out;
-  // this CTA's slots [lo, hi)
-  const int per = ((n + size - 1) / size + 31) / 32 * 32;
+  // this CTA's slots [lo, hi), and of them the warp's, 128 at a time
+  const int per = ((n + size - 1) / size + 127) / 128 * 128;
   const int lo = min(n, rank * per), hi = min(n, lo + per);
-  auto row_of = [&](int t) { return a.index.row(b, h, t, a.status); };
+  const int run = ((hi - lo + kWarps - 1) / kWarps + 127) / 128 * 128;
+  const int r_lo = min(hi, lo + warp * run), r_hi = min(hi, r_lo + run);
+  // where the rows of a page of this kv head start, in pages of one head; -1: a bad page
+  const int32_t* const table = a.index.block_table + (long long)b * a.index.pages_per_seq;
+  const int log2 = a.index.page_log2, entry0 = lo >> log2;
+  auto look_up = [&](int entry) {
+    const int page = __ldg(table + entry);
+    return (unsigned)page < (unsigned)a.index.num_pages ? (long long)page * hkv + h : -1ll;
+  };
+  const int entries = hi > lo ? min(room.entries, ((hi - 1) >> log2) - entry0 + 1) : 0;
+  for (int i = threadIdx.x; i < entries; i += kThreads) s_entry[i] = (int)look_up(entry0 + i);
+  __syncthreads();
+  auto row_of = [&](int t) {
+    const int i = (t >> log2) - entry0;
+    const long long e = !kLong || i < entries ? s_entry[i] : look_up(entry0 + i);
+    return e < 0 ? -1 : (e << log2) + (t & ((1 << log2) - 1));
+  };
   if (n <= a.keep) {
     if (rank == 0 && threadIdx.x == 0) a.counts[unit] = 0;
-    if (copies)
-      for (int t = lo + threadIdx.x; t < hi; t += kThreads) {
-        const long long r = row_of(t);
-        if (r >= 0) a.w_out[r] = a.w_in[r];
-      }
+    for (int t = lo + threadIdx.x; t < hi; t += kThreads) {
+      const long long r = row_of(t);
+      if (r < 0)
+        atomicOr(a.status, kDevBadPage);
+      else if (copies)
+        a.w_out[r] = a.w_in[r];
+    }
     if (src)
       for (int t = rank * kThreads + threadIdx.x; t < a.keep; t += size * kThreads) src[t] = t < n ? t : -1;
     return;
   }
 
-  auto load_key = [&](int t) {
-    const long long r = row_of(t);
-    return ordered(r < 0 ? 0.f : __ldcg(a.w_in + r));
+  // ---- the slots' keys (a bad page's weigh nothing) and the first pass over them, four slots
+  // to a lane.  Where weights are written apart, those before `keep` are copied here (of the
+  // holes too: moved rows' weights replace those) and the ones behind cleared ----
+  const int cached = r_lo + room.run_keys;  // keys of the run's slots before this one are kept
+  uint32_t* const run_keys = s_keys + warp * room.run_keys - r_lo;
+  auto ordered4 = [](const float4& w) {
+    return make_uint4(ordered(w.x), ordered(w.y), ordered(w.z), ordered(w.w));
   };
-  const bool cached = hi - lo <= a.slice_cached;
-  if (cached)
-    for (int t = lo + threadIdx.x; t < hi; t += kThreads) s_keys[t - lo] = load_key(t);
-  auto key = [&](int t) { return cached ? s_keys[t - lo] : load_key(t); };
-  // of the slots that nothing protects, `free_` stay
-  const int m_lo = max(lo, a.first), m_hi = min(hi, n - a.last);
+  auto keys = [&](int t) {  // of slots t .. t + 3 of the warp's run, which only this lane asks for
+    if (!kLong || t < cached) return *reinterpret_cast<const uint4*>(run_keys + t);
+    const long long r = t < r_hi ? row_of(t) : -1;
+    return ordered4(r < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(reinterpret_cast<const float4*>(a.w_in + r)));
+  };
+  const int p_lo = a.first, p_hi = n - a.last;  // slots that nothing protects; of them `free_` stay
+  const int m_lo = max(r_lo, p_lo), m_hi = min(r_hi, p_hi);
   const int free_ = a.keep - a.first - a.last;
-  uint32_t border = 0xffffffffu;
-  int room = 0, ties = 0;  // of the slots at the border: that stay, that there are
-  if (free_ > 0) {
-    uint32_t prefix = 0, mask = 0;
-    int want = free_;
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
-      for (int i = threadIdx.x; i < bins; i += kThreads) s_hist[i] = 0;
-      __syncthreads();
-      for (int t = m_lo + threadIdx.x; t < m_hi; t += kThreads) {
-        const uint32_t x = key(t);
-        if ((x & mask) == prefix) atomicAdd(&s_hist[(x >> shift) & (bins - 1)], 1u);
-      }
-      cluster.sync();
-      if (size > 1) {
-        for (int i = threadIdx.x; i < bins; i += kThreads) {
-          uint32_t sum = 0;
-          for (int r = 0; r < size; ++r) sum += cluster.map_shared_rank(s_hist, r)[i];
-          s_all[i] = sum;
-        }
-        cluster.sync();
-      }
-      const uint32_t* const hist = size > 1 ? s_all : s_hist;
-      // the bin, from the top, in which the want-th slot lies: thread i has bins [top - 4 i - 3, top - 4 i]
-      const int each = bins / kThreads;
-      int mine = 0;
-      for (int i = 0; i < each; ++i) mine += hist[bins - 1 - threadIdx.x * each - i];
-      int incl = mine;
+  auto count = [&](int t, const uint4& x, uint32_t border, uint32_t mask, int shift, int bins) {
+    const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += y;
+    for (int j = 0; j < 4; ++j)
+      if (t + j >= m_lo && t + j < m_hi && (v[j] & mask) == border)
+        atomicAdd(&s_hist[lane & 1][(v[j] >> shift) & (bins - 1)], 1u);
+  };
+  {
+    bool bad = false;
+#pragma unroll 1
+    for (int t0 = r_lo + 4 * lane; t0 < r_hi; t0 += 128 * kRows) {
+      long long row[kRows];
+      float4 w[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {  // no branch but the loads': all are in flight at once
+        const int t = t0 + 128 * j;
+        row[j] = t < r_hi ? row_of(t) : -1;
+        w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row[j] >= 0) w[j] = __ldcg(reinterpret_cast<const float4*>(a.w_in + row[j]));
+        bad |= t < r_hi && row[j] < 0;
       }
-      if (lane == 31) s_scan[warp] = incl;
-      __syncthreads();
-      int before = incl - mine;
-      for (int w = 0; w < warp; ++w) before += s_scan[w];
-      if (before < want && before + mine >= want) {
-        int bin = bins - 1 - threadIdx.x * each, c = hist[bin];
-        while (before + c < want) {
-          before += c;
-          c = hist[--bin];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int t = t0 + 128 * j;
+        if (t >= r_hi) break;
+        const uint4 x = ordered4(w[j]);
+        if (!kLong || t < cached) *reinterpret_cast<uint4*>(run_keys + t) = x;
+        count(t, x, 0, 0, 21, kBins);
+        if (copies && row[j] >= 0) {
+          if (t + 3 < min(n, a.keep)) {
+            *reinterpret_cast<float4*>(a.w_out + row[j]) = w[j];
+          } else {
+            const float v[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (t + i < n) a.w_out[row[j] + i] = t + i < a.keep ? v[i] : 0.f;
+          }
         }
-        s_pick[0] = bin;
-        s_pick[1] = want - before;
-        s_totals[0] = c;
       }
-      __syncthreads();
-      prefix |= s_pick[0] << shift;
-      mask |= (uint32_t)(bins - 1) << shift;
-      want = s_pick[1];
-      ties = s_totals[0];
-      __syncthreads();
     }
-    border = prefix;
-    room = want;
-  } else {
-    __syncthreads();
+    if (bad) atomicOr(a.status, kDevBadPage);
   }
 
-  // ---- each warp takes a run of the slice, 32 slots at a time, in order ----
-  const int run = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int r_lo = min(hi, lo + warp * run), r_hi = min(hi, r_lo + run);
-  // exclusive prefix over the runs of all CTAs of the cluster
-  auto runs_before = [&](int x, int which, int& all) {
-    __syncthreads();
-    if (lane == 0) s_scan[warp] = x;
-    __syncthreads();
-    int before = 0, sum = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += s_scan[w];
-      sum += s_scan[w];
+  // ---- the border: 11 bits a pass, the most significant first ----
+  uint32_t border = 0, mask = 0;
+  int want = free_, ties = free_;  // of the slots that begin as the border does: that stay, that there are
+  for (int pass = 0; pass < 3 && free_ > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    if (pass > 0) {
+#pragma unroll 1
+      for (int t = r_lo + 4 * lane; t < m_hi; t += 128) count(t, keys(t), border, mask, shift, bins);
     }
-    all = sum;
-    if (size > 1) {
-      if (threadIdx.x == 0) s_totals[which] = sum;
+    if (kLong && size > 1) {
       cluster.sync();
-      all = 0;
-      for (int r = 0; r < size; ++r) {
-        const int y = *cluster.map_shared_rank(s_totals + which, r);
-        if (r < rank) before += y;
-        all += y;
+      // each CTA adds up its share of the bins and hands the sums to all, in the place of those
+      // that it alone reads
+      const int part = (bins + size - 1) / size;
+      for (int i = rank * part + threadIdx.x; i < min(bins, (rank + 1) * part); i += kThreads) {
+        uint32_t sum = 0;
+#pragma unroll 8
+        for (int r = 0; r < size; ++r) {
+          const uint32_t* const theirs = cluster.map_shared_rank(&s_hist[0][0], r);
+          sum += theirs[i] + theirs[kBins + i];
+        }
+#pragma unroll 8
+        for (int r = 0; r < size; ++r) {
+          uint32_t* const theirs = cluster.map_shared_rank(&s_hist[0][0], r);
+          theirs[i] = sum;
+          theirs[kBins + i] = 0;
+        }
       }
       cluster.sync();
+    } else {
+      __syncthreads();
+    }
+    // the bin, from the top, in which the want-th slot lies: thread i has bins top, top - 1, ..
+    constexpr int kEach = (kBins + kThreads - 1) / kThreads;
+    const int top = bins - 1 - threadIdx.x * kEach;
+    int mine = 0, all;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (top - i >= 0) mine += s_hist[0][top - i] + s_hist[1][top - i];
+    int before = block_prefix<kWarps>(mine, s_scan, all);
+    if (before < want && before + mine >= want) {
+      int bin = top, c = s_hist[0][bin] + s_hist[1][bin];
+      while (before + c < want) {
+        before += c;
+        --bin;
+        c = s_hist[0][bin] + s_hist[1][bin];
+      }
+      s_pick[0] = bin;
+      s_pick[1] = want - before;
+      s_pick[2] = c;
+    }
+    __syncthreads();
+    border |= s_pick[0] << shift;
+    mask |= (uint32_t)(bins - 1) << shift;
+    want = s_pick[1];
+    ties = s_pick[2];
+    if (want == ties) break;  // all that begin so stay
+    if (pass < 2) {
+      for (int i = threadIdx.x; i < 2 * kBins; i += kThreads) s_hist[0][i] = 0;
+      __syncthreads();
+    }
+  }
+  const bool by_slot = want < ties;  // not all of the slots at the border stay
+
+  // exclusive prefix over the runs of all CTAs of the cluster
+  auto runs_before = [&](int x, int which, int& all) {  // x: of the warp
+    int before = block_prefix<kWarps>(lane == 0 ? x : 0, s_scan, all);
+    before = __shfl_sync(kFull, before, 0);
+    if (kLong && size > 1) {
+      if (threadIdx.x == 0) s_totals[which] = all;
+      cluster.sync();
+      const int theirs = lane < size ? *cluster.map_shared_rank(s_totals + which, lane) : 0;
+      before += __reduce_add_sync(kFull, lane < rank ? theirs : 0);
+      all = __reduce_add_sync(kFull, theirs);
     }
     return before;
   };
-  auto is_free = [&](int t) { return t >= a.first && t < n - a.last; };
-  int tie = 0, unused;
-  const bool by_slot = free_ > 0 && room < ties;  // not all of the slots at the border stay
+  int seen = 0, unused;  // slots at the border before the run
   if (by_slot) {
     int mine = 0;
-    for (int t0 = r_lo; t0 < r_hi; t0 += 32) {
-      const int t = t0 + lane;
-      mine += __popc(__ballot_sync(0xffffffffu, t < r_hi && is_free(t) && key(t) == border));
+#pragma unroll 1
+    for (int t = r_lo + 4 * lane; t < m_hi; t += 128) {
+      const uint4 x = keys(t);
+      const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine += t + j >= m_lo && t + j < m_hi && v[j] == border;
     }
-    tie = runs_before(mine, 0, unused);
+    seen = runs_before(__reduce_add_sync(kFull, mine), 0, unused);
   }
-  auto kept_of = [&](int t, uint32_t x, int& seen) {  // seen: slots at the border before this row of 32
-    const bool at = t < r_hi && is_free(t) && x == border;
-    bool kept = t < r_hi && (!is_free(t) || (free_ > 0 && (x > border || (at && !by_slot))));
+
+  // ---- which slots stay: bit `lane` of word j of a row of 128 is slot 4 lane + j ----
+  uint4* const run_kept = reinterpret_cast<uint4*>(s_kept) + (r_lo - lo) / 128;
+  const uint32_t lower = (1u << lane) - 1;
+#pragma unroll 1
+  for (int t0 = r_lo; t0 < r_hi; t0 += 128) {
+    const int t = t0 + 4 * lane;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (t < r_hi) x = keys(t);
+    uint32_t v[4] = {x.x, x.y, x.z, x.w};
+    bool stays[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      stays[j] = t + j < r_hi && (v[j] >= border ? free_ > 0 || t + j < p_lo || t + j >= p_hi
+                                                 : t + j < p_lo || t + j >= p_hi);
     if (by_slot) {
-      const uint32_t m = __ballot_sync(0xffffffffu, at);
-      if (at) kept = seen + __popc(m & ((1u << lane) - 1)) < room;
-      seen += __popc(m);
+      bool at[4];
+      uint32_t m[4];
+      int before = seen;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        at[j] = t + j >= m_lo && t + j < m_hi && v[j] == border;
+        m[j] = __ballot_sync(kFull, at[j]);
+        before += __popc(m[j] & lower);
+        seen += __popc(m[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (at[j]) stays[j] = before++ < want;
     }
-    return kept;
-  };
-  int holes = 0, movers = 0, seen = tie;
-  for (int t0 = r_lo; t0 < r_hi; t0 += 32) {
-    const int t = t0 + lane;
-    const bool kept = kept_of(t, t < r_hi ? key(t) : 0, seen);
-    holes += __popc(__ballot_sync(0xffffffffu, t < r_hi && t < a.keep && !kept));
-    movers += __popc(__ballot_sync(0xffffffffu, kept && t >= a.keep));
-  }
-  int all_holes;
-  holes = runs_before(holes, 1, all_holes);
-  movers = runs_before(movers, 2, unused);
-  if (rank == 0 && threadIdx.x == 0) a.counts[unit] = all_holes;
-  int* const hole_list = a.holes + (long long)unit * a.keep;
-  int* const mover_list = a.movers + (long long)unit * a.keep;
-  seen = tie;
-  for (int t0 = r_lo; t0 < r_hi; t0 += 32) {
-    const int t = t0 + lane;
-    const bool kept = kept_of(t, t < r_hi ? key(t) : 0, seen);
-    const bool hole = t < r_hi && t < a.keep && !kept, mover = kept && t >= a.keep;
-    const uint32_t hm = __ballot_sync(0xffffffffu, hole), mm = __ballot_sync(0xffffffffu, mover);
-    const uint32_t lower = (1u << lane) - 1;
-    if (hole) hole_list[holes + __popc(hm & lower)] = t;
-    if (mover) mover_list[movers + __popc(mm & lower)] = t;
-    holes += __popc(hm);
-    movers += __popc(mm);
-    if (t < r_hi && !hole && !mover) {
-      if (t < a.keep) {
-        if (src) src[t] = t;
-        if (copies) {
-          const long long r = row_of(t);
-          if (r >= 0) a.w_out[r] = a.w_in[r];
-        }
-      } else {
-        const long long r = row_of(t);
-        if (r >= 0) a.w_out[r] = 0.f;
+    uint32_t m[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = __ballot_sync(kFull, stays[j]);
+    if (lane == 0) run_kept[(t0 - r_lo) / 128] = make_uint4(m[0], m[1], m[2], m[3]);
+    if (src) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // a hole's is replaced with its row
+        const int i = t0 + 32 * j + lane;
+        if (i < min(r_hi, a.keep)) src[i] = i;
       }
     }
   }
+  __syncwarp();
+  // word j of a row from t0 on: the slots below t1
+  auto below = [](int t0, int t1, int j) {
+    const int k = (t1 - t0 - j + 3) >> 2;
+    return k >= 32 ? kFull : k <= 0 ? 0u : (1u << k) - 1;
+  };
+  auto listed = [&](int t0, uint32_t hm[4], uint32_t mm[4]) {  // holes and movers
+    const uint4 x = run_kept[(t0 - r_lo) / 128];
+    const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      hm[j] = ~v[j] & below(t0, min(r_hi, a.keep), j);
+      mm[j] = v[j] & ~below(t0, a.keep, j);
+    }
+  };
+  int holes = 0, movers = 0;
+  for (int t0 = r_lo + 128 * lane; t0 < r_hi; t0 += 128 * 32) {
+    uint32_t hm[4], mm[4];
+    listed(t0, hm, mm);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      holes += __popc(hm[j]);
+      movers += __popc(mm[j]);
+    }
+  }
+  int all_holes;
+  holes = runs_before(__reduce_add_sync(kFull, holes), 1, all_holes);
+  movers = runs_before(__reduce_add_sync(kFull, movers), 2, unused);
+  if (rank == 0 && threadIdx.x == 0) a.counts[unit] = all_holes;
+  int* const hole_list = a.holes + (long long)unit * a.keep;
+  int* const mover_list = a.movers + (long long)unit * a.keep;
+#pragma unroll 1
+  for (int t0 = r_lo; t0 < r_hi; t0 += 128) {
+    uint32_t hm[4], mm[4];
+    listed(t0, hm, mm);
+    auto list = [&](const uint32_t m[4], int* to, int& at) {
+      int here = at, all = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        here += __popc(m[j] & lower);
+        all += __popc(m[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (m[j] >> lane & 1) to[here++] = t0 + 4 * lane + j;
+      at += all;
+    };
+    if (hm[0] | hm[1] | hm[2] | hm[3]) list(hm, hole_list, holes);
+    if (mm[0] | mm[1] | mm[2] | mm[3]) list(mm, mover_list, movers);
+    if (!copies && t0 + 128 > a.keep) {  // in place: weights of the slots behind that nothing moves out of
+      const int t = t0 + 4 * lane;
+      const long long r = t < r_hi && t + 3 >= a.keep ? row_of(t) : -1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (r >= 0 && t + j >= a.keep && t + j < r_hi && !(mm[j] >> lane & 1)) a.w_out[r + j] = 0.f;
+    }
+  }
+  if (kLong && size > 1) cluster.sync();  // s_totals may still be read
 }
 
 // Rows of all units, laid end to end; each warp of the grid takes an equal run.
 template <int D>
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kMoveThreads, 3) move_kernel(const __grid_constant__ Args a) {
   constexpr int kWarpsHere = kMoveThreads / 32;
   constexpr int kLanes = D / 8;             // lanes of a row
   constexpr int kAtOnce = 32 / (2 * kLanes);  // pairs of rows (K and V) in one access
@@ -283,19 +435,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
   const int u_lo = min(units, (int)threadIdx.x * each), u_hi = min(units, u_lo + each);
   long long mine = 0;
   for (int u = u_lo; u < u_hi; ++u) mine += __ldcg(a.counts + u);
-  long long incl = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += y;
-  }
-  if (lane == 31) s_sum[warp] = incl;
-  __syncthreads();
-  long long before = incl - mine, total = 0;
-  for (int w = 0; w < kWarpsHere; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
+  long long total;
+  long long before = block_prefix<kWarpsHere>(mine, s_sum, total);
   const long long per = (total + gridDim.x - 1) / gridDim.x;
   const long long lo = min(total, blockIdx.x * per), hi = min(total, lo + per);
   if (lo >= hi) return;
@@ -322,26 +463,26 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
         if (a.sources) a.sources[list + d] = s;
         if (to >= 0 && from >= 0) a.w_out[to] = a.w_in[from];
         if (from >= 0) a.w_out[from] = 0.f;
-        if (from < 0) to = -1;
+        if (from < 0 || to < 0) to = from = -1;
       }
       const int pairs = min(32, i_hi - i0);
       uint16_t* const pages = lane & kLanes ? a.v : a.k;
       const int sub = lane / (2 * kLanes), chunk = lane % kLanes;
 #pragma unroll 1
-      for (int p0 = 0; p0 < pairs; p0 += 8 * kAtOnce) {
-        uint4 x[8];
-        long long dst[8];
+      for (int p0 = 0; p0 < pairs; p0 += kFlight * kAtOnce) {
+        uint4 x[kFlight];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int p = p0 + j * kAtOnce + sub;
-          dst[j] = __shfl_sync(0xffffffffu, to, p & 31);
-          const long long f = __shfl_sync(0xffffffffu, from, p & 31);
-          if (p >= pairs) dst[j] = -1;
-          if (dst[j] >= 0) x[j] = __ldcg(reinterpret_cast<const uint4*>(pages + f * D) + chunk);
+        for (int j = 0; j < kFlight; ++j) {
+          const int p = p0 + j * kAtOnce + sub;  // below 32
+          const long long f = __shfl_sync(0xffffffffu, from, p);
+          if (f >= 0) x[j] = __ldcg(reinterpret_cast<const uint4*>(pages + f * D) + chunk);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (dst[j] >= 0) reinterpret_cast<uint4*>(pages + dst[j] * D)[chunk] = x[j];
+        for (int j = 0; j < kFlight; ++j) {
+          const int p = p0 + j * kAtOnce + sub;
+          const long long d = __shfl_sync(0xffffffffu, to, p);
+          if (d >= 0) reinterpret_cast<uint4*>(pages + d * D)[chunk] = x[j];
+        }
       }
     }
     at += count;
@@ -363,41 +504,40 @@ Layout layout(int batch, int n_kv_heads, int keep) {
 }
 
 cudaError_t launch(const Args& a, cudaStream_t stream) {
-  const void* fn = reinterpret_cast<const void*>(&select_kernel);
-  constexpr int kMostSmem = kKeysCached * 4;
+  const int units = a.batch * a.index.n_kv_heads, sms = device_sm_count();
+  const long long cap = a.index.capacity();
+  int size = 1;
+  while (size < kMaxCluster && (cap / size > kLongSlice || (cap / size > 4096 && (long long)units * size < sms)))
+    size *= 2;
+  const bool long_ = size > 1 || cap > kShortSlice;
+  const void* const fn = long_ ? reinterpret_cast<const void*>(&select_kernel<768, 2, true>)
+                               : reinterpret_cast<const void*>(&select_kernel<512, 3, false>);
+  const int threads = long_ ? 768 : 512, most_smem = long_ ? kLongSmem : kShortSmem;
+  // per slice: the bits, then the table, then as many keys as there is room for
+  const long long run = ((cap + size - 1) / size + 4 * threads - 1) / (4 * threads) * 128, slice = run * (threads / 32);
+  SliceRoom room;
+  room.words = (int)(slice / 32);
+  room.entries = (int)std::min<long long>(kMostEntries, slice / (1 << a.index.page_log2) + 4) / 4 * 4;
+  const int left = std::max(0, most_smem / 4 - room.words - room.entries) / (4 * threads) * 128;
+  room.run_keys = (int)std::min<long long>(run, left);
+  const size_t smem = 4 * ((size_t)room.words + room.entries + (size_t)room.run_keys * (threads / 32));
   {
     static std::mutex mu;
-    static uint64_t done = 0;  // the shared-memory opt-in is per device
+    static uint64_t done[2] = {0, 0};  // the opt-ins are per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     std::lock_guard<std::mutex> lock(mu);
-    if (dev > 63 || !(done >> dev & 1)) {
+    if (dev > 63 || !(done[long_] >> dev & 1)) {
       e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return e;
-      if (dev <= 63) done |= 1ull << dev;
+      if (dev <= 63) done[long_] |= 1ull << dev;
     }
   }
-  const int units = a.batch * a.index.n_kv_heads, sms = device_sm_count();
-  const long long cap = a.index.capacity();
-  int size = 1;
-  while (size < kMaxCluster && cap / size > 4096 && (long long)units * size < sms) size *= 2;
   Args args = a;
-  const long long slice = ((cap + size - 1) / size + 31) / 32 * 32;
-  args.slice_cached = (int)std::min<long long>(slice, kKeysCached);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)units * size);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)args.slice_cached * 4;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = size;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  void* p[] = {&args};
-  cudaError_t e = cudaLaunchKernelExC(&cfg, fn, p);
+  void* p[] = {&args, &room};
+  cudaError_t e = launch_with_pdl(fn, dim3((unsigned)units * size), dim3(threads), p, smem, stream, size);
   if (e != cudaSuccess) return e;
   // no more CTAs than rows can move, 256 to a CTA
   const long long most = (long long)units * std::min<long long>(a.keep, std::max(0ll, cap - a.keep));
@@ -436,9 +576,15 @@ extern "C" int lara_kv_evict(uint16_t* k_pages, uint16_t* v_pages, const float* 
   if (!weights || !weights_out || !seq_lens || !workspace) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
   if (!aligned(weights, 4) || !aligned(weights_out, 4) || !aligned(seq_lens, 4) || !aligned(workspace, 256))
     return set_last_error(LARA_ERR_STREAM_DEST, "the workspace must be 256-byte aligned, all else 4-byte");
+  if (a.index.capacity() > kMostSlots)
+    return set_last_error(LARA_ERR_UNSUPPORTED, "eviction from sequences of at most 2^24 slots");
+  if ((long long)num_pages * n_kv_heads > 0x7fffffffll)
+    return set_last_error(LARA_ERR_BAD_CFG, "num_pages * n_kv_heads must be below 2^31");
   if (kvq::overlap(new_lens, seq_lens, (size_t)batch * 4))
     return set_last_error(LARA_ERR_STREAM_DEST, "new_lens must lie apart from seq_lens");
   if (const int rc = check_weights(weights, weights_out, n_kv_heads, page_size, num_pages)) return rc;
+  if (!aligned(weights, 16) || !aligned(weights_out, 16))
+    return set_last_error(LARA_ERR_STREAM_DEST, "weights must be 16-byte aligned");
   const Layout w = layout(batch, n_kv_heads, keep);
   if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "eviction workspace too small");
   a.k = k_pages;
