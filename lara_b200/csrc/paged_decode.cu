@@ -59,6 +59,11 @@ struct Args {
   long long* seq_tiles;  // [batch + 1] tiles of one kv head of the sequences before this one
   float2* part_ml;   // [units + CTAs][group] (R, l)
   float* part_acc;   // [units + CTAs][group][D]
+  // behind a shared prefix: its tokens, and what the pass over it leaves of each row
+  int shared_tokens;
+  int splits;
+  const float2* prefix_ml;  // [splits][rows]
+  const float* prefix_acc;  // [splits][rows][D]
   // scoring
   float* scores;          // [tiles][group][kTile], in the order of the units
   long long score_tiles;  // that there is room for
@@ -108,11 +113,22 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 }
 
 // A unit (b, kvh); `base` is the place of its first tile, counted from the
-// start of the CTA's share, `tile0` among the tiles of all units.
+// start of the CTA's share, `tile0` among the tiles of all units.  Its tokens
+// are `start` .. `start` + `len` - 1.
 struct Unit {
   long long tile0;
-  int base, tiles, len, b, kvh;
+  int base, tiles, len, start, b, kvh;
 };
+
+// The tokens that a sequence has for itself: a sequence that covers the shared
+// prefix starts behind it.
+struct Own {
+  int start, len;
+};
+__device__ __forceinline__ Own own_tokens(const Args& a, int len) {
+  const int start = a.shared_tokens > 0 && len >= a.shared_tokens ? a.shared_tokens : 0;
+  return {start, len - start};
+}
 
 // Equal shares of the span: the first `rem` take one more.
 struct Shares {
@@ -145,7 +161,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
   const long long cap = a.index.capacity();
 
   allow_dependent_launch();
-  grid_dependency_wait();
+  // The pass over a prefix has waited for what was before it when this one starts, and nothing
+  // here needs what it leaves; the join does, so that this grid ends after that one.
+  if (a.shared_tokens == 0) grid_dependency_wait();
 
   // ---- this CTA's share of all tiles, and the unit in which it starts ----
   auto load_len = [&](int b) { return (int)min((long long)max(__ldcg(a.lens + b), 0), cap); };
@@ -157,7 +175,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
       u.kvh = 0;
       do {
         ++u.b;
-        u.len = u.b < a.batch ? len_of(u.b) : 0;
+        const Own own = own_tokens(a, u.b < a.batch ? len_of(u.b) : 0);
+        u.start = own.start;
+        u.len = own.len;
         u.tiles = u.b < a.batch ? tiles_of(u.len) : 0x3fffffff;
       } while (u.tiles == 0);
     }
@@ -170,7 +190,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     const int len = (int)min((long long)max(raw, 0), cap);
     if (raw != len) atomicOr(a.status, kDevBadLength);
     if (b < kLensCached) s_lens[b] = len;
-    mine += tiles_of(len) + (len > 0 ? 1ll << 40 : 0);
+    const int own = own_tokens(a, len).len;
+    mine += tiles_of(own) + (own > 0 ? 1ll << 40 : 0);
   }
   long long ahead = mine;
 #pragma unroll
@@ -197,11 +218,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     if (b_hi == a.batch) a.seq_tiles[a.batch] = at;  // of every thread at or behind the last sequence, alike
   }
   const long long total = (all & kLow) * hkv, units = (all >> 40) * hkv;
-  if (total == 0) return;
+  if (total == 0) {
+    grid_dependency_wait();
+    return;
+  }
   const long long span = total + units * kUnitCost;
   const int workers = (int)min((long long)gridDim.x, max((total + kMinTiles - 1) / kMinTiles, units));
   const int me = blockIdx.x;
-  if (me >= workers) return;
+  if (me >= workers) {
+    grid_dependency_wait();
+    return;
+  }
   const Shares sh{quotient(span, workers), span - quotient(span, workers) * workers};
   const int share = (int)(sh.start(me + 1) - sh.start(me));
   {
@@ -211,9 +238,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     const long long x = sh.start(me);
     if (x >= begin && x < stop) {
       long long at = begin, tile0 = (ahead & kLow) * hkv;
-      Unit u{0, 0, 0, 0, b_lo, 0};
+      Unit u{0, 0, 0, 0, 0, b_lo, 0};
       for (;; ++u.b) {  // by whole sequences
-        u.len = len_of(u.b);
+        const Own own = own_tokens(a, len_of(u.b));
+        u.start = own.start;
+        u.len = own.len;
         u.tiles = tiles_of(u.len);
         const long long span_b = u.tiles ? (long long)(u.tiles + kUnitCost) * hkv : 0;
         if (x < at + span_b) break;
@@ -249,13 +278,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
       more = in_share(pu);
     }
     if (!more) return;
-    const int pos = (pid - pu.base) * kTile;
+    const int pos = pu.start + (pid - pu.base) * kTile;
     page = __ldcg(a.index.block_table + (long long)pu.b * a.index.pages_per_seq + (pos >> log2));
   };
   auto fetch_tile = [&](int stage) {
     if (more) {
       const uint32_t st = smem_addr(ring) + stage * C::kStageBytes + copy_at;
-      const int pos = (pid - pu.base) * kTile;
+      const int pos = pu.start + (pid - pu.base) * kTile;
       if ((unsigned)page >= (unsigned)a.index.num_pages) {
         atomicOr(a.status, kDevBadPage);
         page = 0;
@@ -465,13 +494,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     }
   }
   cp_async_wait<0>();
+  grid_dependency_wait();
 }
 
 // ---- the second launch ----
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kAhead = 4;      // tokens of a lane whose scores are in flight
-constexpr int kFewParts = 16;  // parts of a row that one warp joins
+constexpr int kFewParts = 32;  // parts of a row that one warp joins
+
+// What a row's result is joined from.
+struct Parts {
+  long long row;
+  int h, slot0, prefix, all;
+};
 
 // Joins the parts of kJoinWarps output rows: a warp to a row, and the rows of many
 // parts by the whole block, one after the other.
@@ -480,25 +516,33 @@ __device__ __forceinline__ void join_rows(const Args& a, int block) {
   constexpr int kLanes = D / 4, kSub = kJoinThreads / kLanes;  // lanes of a row, parts in flight
   __shared__ float4 s_x[kSub][kLanes];
   __shared__ float s_l[kSub];
-  __shared__ UnitParts s_many[kJoinWarps];
+  __shared__ Parts s_many[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.group;
   const long long rows = (long long)a.batch * a.n_q_heads, row0 = (long long)block * kJoinWarps;
-  auto largest = [&](const UnitParts& up, int h) {
+  // part i of a row: of the prefix, then of the unit
+  auto ml_of = [&](const Parts& up, int i) {
+    return i < up.prefix ? a.prefix_ml + i * rows + up.row
+                         : a.part_ml + (long long)(up.slot0 + i - up.prefix) * G + up.h;
+  };
+  auto acc_of = [&](const Parts& up, int i) {
+    return i < up.prefix ? a.prefix_acc + (i * rows + up.row) * D
+                         : a.part_acc + ((long long)(up.slot0 + i - up.prefix) * G + up.h) * D;
+  };
+  auto largest = [&](const Parts& up) {
     float M = -INFINITY;
-    for (int i = lane; i < up.parts; i += 32) M = fmaxf(M, __ldcg(a.part_ml + (long long)(up.slot0 + i) * G + h).x);
+    for (int i = lane; i < up.all; i += 32) M = fmaxf(M, __ldcg(ml_of(up, i)).x);
 #pragma unroll
     for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
     return M;
   };
   // parts i0, i0 + step, ..
-  auto sum = [&](const UnitParts& up, int h, float M, int i0, int step, int at, float& L) {
+  auto sum = [&](const Parts& up, float M, int i0, int step, int at, float& L) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = i0; i < up.parts; i += step) {
-      const long long p = (long long)(up.slot0 + i) * G + h;
-      const float2 ml = __ldcg(a.part_ml + p);
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_acc + p * D) + at);
+    for (int i = i0; i < up.all; i += step) {
+      const float2 ml = __ldcg(ml_of(up, i));
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(acc_of(up, i)) + at);
       const float f = ml.x == M ? 1.f : ex2_ftz(ml.x - M);
       L = fmaf(ml.y, f, L);
       x.x = fmaf(y.x, f, x.x);
@@ -515,17 +559,24 @@ __device__ __forceinline__ void join_rows(const Args& a, int block) {
   };
   {
     const long long row = row0 + warp;
-    UnitParts up{0, 0, 0};
+    Parts up{row, 0, 0, 0, 0};
     if (row < rows) {
-      const int b = (int)(row / a.n_q_heads), hq = (int)(row % a.n_q_heads), h = hq % G;
-      const int len = __ldcg(a.lens + b);
-      if (len > 0) up = a.units[b * a.index.n_kv_heads + hq / G];
+      const int b = (int)(row / a.n_q_heads), hq = (int)(row % a.n_q_heads);
+      up.h = hq % G;
+      const int len = (int)min((long long)__ldcg(a.lens + b), a.index.capacity());
+      const Own own = own_tokens(a, len);
+      if (own.start > 0) up.prefix = up.all = a.splits;
+      if (own.len > 0) {
+        const UnitParts unit = a.units[b * a.index.n_kv_heads + hq / G];
+        up.slot0 = unit.slot0;
+        up.all += unit.parts;
+      }
       const int at = lane % kLanes;
       if (len <= 0) {
         if (lane < kLanes) reinterpret_cast<uint2*>(a.o + row * D)[at] = make_uint2(0, 0);
-      } else if (up.parts <= kFewParts) {
+      } else if (up.all <= kFewParts) {
         float L = 0.f;
-        const float4 x = sum(up, h, largest(up, h), 0, 1, at, L);
+        const float4 x = sum(up, largest(up), 0, 1, at, L);
         if (lane < kLanes) store(row, at, x, L);
       }
     }
@@ -533,11 +584,11 @@ __device__ __forceinline__ void join_rows(const Args& a, int block) {
   }
   __syncthreads();
   for (int r = 0; r < kJoinWarps; ++r) {
-    const UnitParts up = s_many[r];
-    if (up.parts <= kFewParts) continue;
-    const int h = (int)((row0 + r) % a.n_q_heads) % G, sub = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
+    const Parts up = s_many[r];
+    if (up.all <= kFewParts) continue;
+    const int sub = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
     float L = 0.f;
-    const float4 part = sum(up, h, largest(up, h), sub, kSub, at, L);
+    const float4 part = sum(up, largest(up), sub, kSub, at, L);
     s_x[sub][at] = part;
     if (at == 0) s_l[sub] = L;
     __syncthreads();
@@ -660,13 +711,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 
 int max_ctas() { return device_sm_count() * 2; }
 
-// Workspace: status word | units | partial results | scores.
+// Workspace: status word | units | partial results | scores, or the prefix's results.
 struct Layout {
-  size_t units_off, seq_off, ml_off, acc_off, scores_off, total;
+  size_t units_off, seq_off, ml_off, acc_off, scores_off, prefix_ml_off, prefix_acc_off, total;
   long long score_tiles;
 };
 
-Layout layout(int batch, int n_kv_heads, int group, int head_dim, long long score_tokens) {
+Layout layout(int batch, int n_kv_heads, int group, int head_dim, long long score_tokens, size_t prefix_rows) {
   const size_t units = (size_t)batch * n_kv_heads, slots = units + max_ctas();
   Layout w;
   w.units_off = kStatusBytes;
@@ -675,7 +726,9 @@ Layout layout(int batch, int n_kv_heads, int group, int head_dim, long long scor
   w.acc_off = w.ml_off + up256(slots * group * sizeof(float2));
   w.scores_off = w.acc_off + up256(slots * group * head_dim * sizeof(float));
   w.score_tiles = score_tokens / kTile * n_kv_heads;
-  w.total = w.scores_off + up256((size_t)w.score_tiles * kTile * group * sizeof(float));
+  w.prefix_ml_off = w.scores_off + up256((size_t)w.score_tiles * kTile * group * sizeof(float));
+  w.prefix_acc_off = w.prefix_ml_off + up256(prefix_rows * sizeof(float2));
+  w.total = w.prefix_acc_off + up256(prefix_rows * head_dim * sizeof(float));
   return w;
 }
 
@@ -816,7 +869,7 @@ extern "C" size_t lara_decode_scored_workspace_bytes(int batch, int n_q_heads, i
       num_pages < 1)
     return 0;
   return layout(batch, n_kv_heads, (n_q_heads + n_kv_heads - 1) / n_kv_heads, head_dim,
-                score_tokens(batch, page_size, pages_per_seq, num_pages))
+                score_tokens(batch, page_size, pages_per_seq, num_pages), 0)
       .total;
 }
 
@@ -833,7 +886,7 @@ extern "C" int lara_gqa_decode_scored(const uint16_t* q, const uint16_t* k_pages
   if (batch == 0) return LARA_OK;
   if (const int rc = check_weights(weights, weights_out, n_kv_heads, page_size, num_pages)) return rc;
   const Layout w = layout(batch, n_kv_heads, a.group, head_dim,
-                          score_tokens(batch, page_size, pages_per_seq, num_pages));
+                          score_tokens(batch, page_size, pages_per_seq, num_pages), 0);
   if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "scored decode workspace too small");
   place(a, w, workspace);
   a.w_in = weights;
@@ -846,7 +899,11 @@ extern "C" int lara_gqa_decode_scored(const uint16_t* q, const uint16_t* k_pages
 
 extern "C" size_t lara_decode_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
   if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || head_dim < 1) return 0;
-  return layout(batch, n_kv_heads, (n_q_heads + n_kv_heads - 1) / n_kv_heads, head_dim, 0).total;
+  const int group = std::min(16, (n_q_heads + n_kv_heads - 1) / n_kv_heads);
+  // a wave of CTAs, of two row tiles each, or one split of all rows; of this or any smaller batch
+  const size_t rows = (size_t)batch * n_kv_heads * group, sms = std::max(1, device_sm_count());
+  const size_t most = std::min(rows * std::max<size_t>(1, sms / n_kv_heads), std::max(rows, 256 * sms));
+  return layout(batch, n_kv_heads, group, head_dim, 0, most).total;
 }
 
 extern "C" int lara_gqa_decode_shared(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
@@ -862,10 +919,26 @@ extern "C" int lara_gqa_decode_shared(const uint16_t* q, const uint16_t* k_pages
   if (shared_pages < 0 || shared_pages > pages_per_seq)
     return set_last_error(LARA_ERR_BAD_CFG, "shared_pages must be in [0, pages_per_seq]");
   if (batch == 0) return LARA_OK;
-  const Layout w = layout(batch, n_kv_heads, a.group, head_dim, 0);
+  const long long tokens = (long long)shared_pages * page_size;
+  const PrefixPlan plan = prefix_plan(batch, n_kv_heads, a.group, (int)tokens);
+  const Layout w = layout(batch, n_kv_heads, a.group, head_dim, 0,
+                          tokens ? (size_t)batch * n_q_heads * plan.splits : 0);
   if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "shared decode workspace too small");
   place(a, w, workspace);
-  const cudaError_t e = launch_any<false>(a, head_dim, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (tokens) {
+    char* base = static_cast<char*>(workspace);
+    float2* const ml = reinterpret_cast<float2*>(base + w.prefix_ml_off);
+    float* const acc = reinterpret_cast<float*>(base + w.prefix_acc_off);
+    a.shared_tokens = (int)tokens;
+    a.splits = plan.splits;
+    a.prefix_ml = ml;
+    a.prefix_acc = acc;
+    e = prefix_launch(plan, q, k_pages, v_pages, a.index, (int)tokens, batch, n_q_heads, head_dim, a.scale_log2, ml,
+                      acc, a.status, st);
+  }
+  if (e == cudaSuccess) e = launch_any<false>(a, head_dim, st);
   if (e != cudaSuccess)
     return set_last_error(LARA_ERR_CUDA, std::string("shared decode launch: ") + cudaGetErrorString(e));
   return LARA_OK;
