@@ -19,10 +19,8 @@ using kvq::PoolIndex;
 constexpr size_t kStatusBytes = 256;
 
 // What the own-token pass leaves of a unit, a (sequence, kv head): `parts`
-// partial results from slot `slot0` on, and where its first tile lies among
-// the tiles of all units.
+// partial results from slot `slot0` on.
 struct UnitParts {
-  long long tile0;
   int slot0, parts;
 };
 

@@ -26,21 +26,24 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;            // tokens per warp and stage: never across pages
+constexpr int kGroup = 32;           // tokens whose scores lie together, head by head (a line of 128 bytes)
 constexpr int kMinTiles = kWarps;    // tiles per CTA below which fewer CTAs run
 constexpr int kUnitCost = 8;         // what a unit costs beside its tiles, in tiles
+constexpr int kMostCtasPerSm = 4;
 constexpr int kLensCached = 1024;    // lengths kept in shared memory
 // R moves only when a score passes it by this much (log2): weights stay below 2^8.
 constexpr float kSlack = 8.f;
 
 template <int D, int NG>
 struct Cfg {
-  static constexpr int kStages = D == 128 ? 3 : 6;
-  static constexpr int kCtasPerSm = 2;
+  static constexpr int kStages = D == 64 ? 4 : NG == 1 ? 2 : 3;
+  static constexpr int kCtasPerSm = NG == 1 ? 3 : 2;
   static constexpr int kRowBytes = 2 * D;
   static constexpr int kRowsBytes = kTile * kRowBytes;  // K (or V) of a stage
   static constexpr int kStageBytes = 2 * kRowsBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kSmemBytes = kWarps * kWarpBytes + 128;
+  static_assert(kCtasPerSm <= kMostCtasPerSm);
   static constexpr int kPitch = D + 4;  // floats per head in the join (lanes of a store hit distinct banks)
   static_assert(8 * kPitch * 4 <= kStageBytes, "a stage holds the sums of eight heads");
 };
@@ -56,7 +59,7 @@ struct Args {
   float scale_log2;
   int* status;
   UnitParts* units;  // [batch * kv heads]; of sequences without tokens, undefined
-  long long* seq_tiles;  // [batch + 1] tiles of one kv head of the sequences before this one
+  long long* seq_groups;  // [batch + 1] groups of one kv head of the sequences before this one
   float2* part_ml;   // [units + CTAs][group] (R, l)
   float* part_acc;   // [units + CTAs][group][D]
   // behind a shared prefix: its tokens, and what the pass over it leaves of each row
@@ -65,15 +68,17 @@ struct Args {
   const float2* prefix_ml;  // [splits][rows]
   const float* prefix_acc;  // [splits][rows][D]
   // scoring
-  float* scores;          // [tiles][group][kTile], in the order of the units
-  long long score_tiles;  // that there is room for
+  float* scores;           // [groups][group][kGroup], in the order of the units
+  long long score_groups;  // that there is room for
   const float* w_in;      // [pages][kv heads][page]
   float* w_out;
 };
 
 template <int kDst>
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16;" ::"r"(dst), "l"(src), "n"(kDst) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0+%2], [%1], 16, %3;" ::"r"(dst), "l"(src), "n"(kDst),
+               "l"(policy)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -106,6 +111,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+__device__ __forceinline__ int groups_of(int tiles) { return (tiles + kGroup / kTile - 1) / (kGroup / kTile); }
 
 __device__ __forceinline__ long long quotient(long long a, long long b) {
   if (((a | b) >> 31) == 0) return (uint32_t)a / (uint32_t)b;
@@ -113,10 +119,10 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 }
 
 // A unit (b, kvh); `base` is the place of its first tile, counted from the
-// start of the CTA's share, `tile0` among the tiles of all units.  Its tokens
-// are `start` .. `start` + `len` - 1.
+// start of the CTA's share, `group0` that of its first group of scores.  Its
+// tokens are `start` .. `start` + `len` - 1.
 struct Unit {
-  long long tile0;
+  long long group0;
   int base, tiles, len, start, b, kvh;
 };
 
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
   using C = Cfg<D, NG>;
   constexpr int KS = D / 16;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ long long s_sum[kWarps];
+  __shared__ long long s_sum[2][kWarps];
   __shared__ Unit s_first;
   __shared__ float2 s_ml[kWarps][NG * 8];
   __shared__ int s_idle[kWarps];
@@ -160,7 +166,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
   const int G = a.group, hkv = a.index.n_kv_heads;
   const long long cap = a.index.capacity();
 
-  allow_dependent_launch();
   // The pass over a prefix has waited for what was before it when this one starts, and nothing
   // here needs what it leaves; the join does, so that this grid ends after that one.
   if (a.shared_tokens == 0) grid_dependency_wait();
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
   auto len_of = [&](int b) { return b < kLensCached ? s_lens[b] : load_len(b); };
   auto next_unit = [&](Unit& u) {
     u.base += u.tiles + kUnitCost;
-    u.tile0 += u.tiles;
+    u.group0 += groups_of(u.tiles);
     if (++u.kvh == hkv) {
       u.kvh = 0;
       do {
@@ -184,7 +189,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
   };
   const int per_thread = (a.batch + kThreads - 1) / kThreads;
   const int b_lo = min(a.batch, (int)threadIdx.x * per_thread), b_hi = min(a.batch, b_lo + per_thread);
-  long long mine = 0;  // tiles in the low 40 bits, sequences that have some above
+  long long mine = 0;    // tiles in the low 40 bits, sequences that have some above
+  long long groups = 0;  // scoring: of scores
   for (int b = b_lo; b < b_hi; ++b) {
     const int raw = __ldcg(a.lens + b);
     const int len = (int)min((long long)max(raw, 0), cap);
@@ -192,31 +198,42 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     if (b < kLensCached) s_lens[b] = len;
     const int own = own_tokens(a, len).len;
     mine += tiles_of(own) + (own > 0 ? 1ll << 40 : 0);
+    groups += groups_of(tiles_of(own));
   }
-  long long ahead = mine;
+  // exclusive prefix over the threads, and the sum of all
+  auto prefix = [&](long long x, long long* s_sum, long long& all) {
+    long long ahead = x;
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, ahead, off);
-    if (lane >= off) ahead += y;
-  }
-  if (lane == 31) s_sum[warp] = ahead;
-  __syncthreads();
-  ahead -= mine;
-  long long all = 0;
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, ahead, off);
+      if (lane >= off) ahead += y;
+    }
+    if (lane == 31) s_sum[warp] = ahead;
+    __syncthreads();
+    ahead -= x;
+    all = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) ahead += s_sum[w];
-    all += s_sum[w];
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) ahead += s_sum[w];
+      all += s_sum[w];
+    }
+    return ahead;
+  };
+  long long all, groups_ahead = 0;
+  const long long ahead = prefix(mine, s_sum[0], all);
+  if constexpr (kScored) {
+    long long all_groups;
+    groups_ahead = prefix(groups, s_sum[1], all_groups);
+    if (blockIdx.x == 0) {
+      long long at = groups_ahead;
+      for (int b = b_lo; b < b_hi; ++b) {
+        a.seq_groups[b] = at;
+        at += groups_of(tiles_of(len_of(b)));
+      }
+      if (threadIdx.x == 0) a.seq_groups[a.batch] = all_groups;
+    }
   }
   constexpr long long kLow = (1ll << 40) - 1;
-  if (kScored && blockIdx.x == 0) {
-    long long at = ahead & kLow;
-    for (int b = b_lo; b < b_hi; ++b) {
-      a.seq_tiles[b] = at;
-      at += tiles_of(len_of(b));
-    }
-    if (b_hi == a.batch) a.seq_tiles[a.batch] = at;  // of every thread at or behind the last sequence, alike
-  }
   const long long total = (all & kLow) * hkv, units = (all >> 40) * hkv;
   if (total == 0) {
     grid_dependency_wait();
@@ -237,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     const long long stop = begin + ((mine & kLow) + (mine >> 40) * kUnitCost) * hkv;
     const long long x = sh.start(me);
     if (x >= begin && x < stop) {
-      long long at = begin, tile0 = (ahead & kLow) * hkv;
+      long long at = begin, group0 = groups_ahead * hkv;
       Unit u{0, 0, 0, 0, 0, b_lo, 0};
       for (;; ++u.b) {  // by whole sequences
         const Own own = own_tokens(a, len_of(u.b));
@@ -247,11 +264,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
         const long long span_b = u.tiles ? (long long)(u.tiles + kUnitCost) * hkv : 0;
         if (x < at + span_b) break;
         at += span_b;
-        tile0 += (long long)u.tiles * hkv;
+        group0 += (long long)groups_of(u.tiles) * hkv;
       }
       u.kvh = (int)quotient(x - at, u.tiles + kUnitCost);
       u.base = (int)(at + (long long)u.kvh * (u.tiles + kUnitCost) + kUnitCost - x);
-      u.tile0 = tile0 + (long long)u.kvh * u.tiles;
+      u.group0 = group0 + (long long)u.kvh * groups_of(u.tiles);
       s_first = u;
     }
   }
@@ -260,7 +277,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
   auto in_share = [&](const Unit& u) { return u.base < share; };
   auto tiles_end = [&](const Unit& u) { return min(share, u.base + u.tiles); };
 
-  // ---- the warp's ring ----
+  // ---- the warp's ring.  Rows are read once: they leave L2 before the scores do ----
+  const uint64_t policy = make_evict_first_policy();
   uint8_t* const ring = smem + warp * C::kWarpBytes;
   constexpr int kChunks = D / 8, kRowsPer = 32 / kChunks;  // a warp copies kRowsPer rows (512 bytes) at a time
   // chunk c of row r lies at r kRowBytes + ((c ^ (r & 7)) << 4): eight rows of a matrix hit distinct banks
@@ -295,8 +313,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
 #pragma unroll
       for (int i = 0; i < kTile / kRowsPer; ++i) {
         const uint32_t to = (st ^ ((i * kRowsPer & 7) << 4)) + i * 512;
-        cp_async16<0>(to, ks + i * 512);
-        cp_async16<C::kRowsBytes>(to, vs + i * 512);
+        cp_async16<0>(to, ks + i * 512, policy);
+        cp_async16<C::kRowsBytes>(to, vs + i * 512, policy);
       }
       pid += kWarps;
       fetch_page();
@@ -372,14 +390,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
             if (g + 8 * (i >> 1) >= valid) s[n][i] = -INFINITY;
       }
       if constexpr (kScored) {
-        const long long tile = u.tile0 + (id - u.base);
-        if (tile < a.score_tiles) {
-          float* const dst = a.scores + (tile * G + 2 * t4) * kTile + g;
+        const int tile = id - u.base;
+        const long long group = u.group0 + tile / 2;
+        if (group < a.score_groups) {
+          float* const dst = a.scores + (group * G + 2 * t4) * kGroup + tile % 2 * kTile + g;
 #pragma unroll
           for (int n = 0; n < NG; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (8 * n + 2 * t4 + (i & 1) < G) dst[(8 * n + (i & 1)) * kTile + 8 * (i >> 1)] = s[n][i];
+              if (8 * n + 2 * t4 + (i & 1) < G) dst[(8 * n + (i & 1)) * kGroup + 8 * (i >> 1)] = s[n][i];
         }
       }
 
@@ -452,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     const long long at0 = sh.start(me) + u.base;
     const int index = u.b * hkv + u.kvh, slot = index + me;
     if (threadIdx.x == 0 && u.base >= 0)  // the unit starts here
-      a.units[index] = UnitParts{u.tile0, slot, sh.cta(at0 + u.tiles - 1) - me + 1};
+      a.units[index] = UnitParts{slot, sh.cta(at0 + u.tiles - 1) - me + 1};
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -494,13 +513,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NG>::kCtasPerSm) own_tokens_k
     }
   }
   cp_async_wait<0>();
+  allow_dependent_launch();  // not before: the join's blocks would take the room of this grid's
   grid_dependency_wait();
 }
 
 // ---- the second launch ----
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kAhead = 4;      // tokens of a lane whose scores are in flight
+constexpr int kAhead = 2;      // times four tokens of a thread whose scores are in flight
 constexpr int kFewParts = 32;  // parts of a row that one warp joins
 
 // What a row's result is joined from.
@@ -610,123 +630,146 @@ __device__ __forceinline__ void join_rows(const Args& a, int block) {
   }
 }
 
-// Adds the weights of the tiles [lo, hi) of all, which one warp takes, a token to a lane.
-__device__ __forceinline__ void add_weights(const Args& a, long long warp, long long warps, float2* ml) {
-  const int lane = threadIdx.x & 31;
-  const int G = a.group, hkv = a.index.n_kv_heads;
-  const int log2 = a.index.page_log2;
-  const long long total = __ldcg(a.seq_tiles + a.batch) * hkv;
-  const long long room = min(total, a.score_tiles);
-  if (room < total && warp == 0 && lane == 0) atomicOr(a.status, kDevScoreRoom);
-  const long long per = (room + warps - 1) / warps;
-  const long long lo = warp * per, hi = min(room, lo + per);
+// Adds the weights of an equal run of all groups, four tokens to a thread.
+__device__ __forceinline__ void add_weights(const Args& a, int block, int blocks) {
+  __shared__ float2 s_ml[16];  // each head's (M, 1 / L)
+  __shared__ int s_seq;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.group, hkv = a.index.n_kv_heads, log2 = a.index.page_log2;
+  const long long total = __ldcg(a.seq_groups + a.batch) * hkv;
+  const long long room = min(total, a.score_groups);
+  if (room < total && block == 0 && threadIdx.x == 0) atomicOr(a.status, kDevScoreRoom);
+  const long long per = (room + blocks - 1) / blocks;
+  const long long lo = block * per, hi = min(room, lo + per);
   if (lo >= hi) return;
-  int b = 0;  // the last sequence that starts at or before tile lo, and so one with tokens
-  for (int step = 1 << (31 - __clz(a.batch)); step; step >>= 1)
-    if (b + step < a.batch && __ldcg(a.seq_tiles + b + step) * hkv <= lo) b += step;
-  long long first = __ldcg(a.seq_tiles + b);
-  int tiles = (int)(__ldcg(a.seq_tiles + b + 1) - first);
-  int kvh = (int)quotient(lo - first * hkv, tiles);
-  long long at = first * hkv + (long long)kvh * tiles;  // the unit's first tile
+  for (int b = threadIdx.x; b < a.batch; b += kJoinThreads)  // the sequence with group lo
+    if (__ldcg(a.seq_groups + b) * hkv <= lo && lo < __ldcg(a.seq_groups + b + 1) * hkv) s_seq = b;
+  __syncthreads();
+  int b = s_seq;
+  long long first = __ldcg(a.seq_groups + b);
+  int groups = (int)(__ldcg(a.seq_groups + b + 1) - first);
+  int kvh = (int)quotient(lo - first * hkv, groups);
+  long long at = first * hkv + (long long)kvh * groups;  // the unit's first group
   while (true) {
-    const int unit = b * hkv + kvh;
-    const UnitParts up = a.units[unit];
+    const UnitParts up = a.units[b * hkv + kvh];
     const int len = (int)min((long long)__ldcg(a.lens + b), a.index.capacity());
-    // each head's (M, 1 / L): lanes h and h + 16 take every other part
-    float M = -INFINITY, L = 0.f;
-    const int h = lane & 15;
-    const float2* const src = a.part_ml + (long long)up.slot0 * G + h;
-    if (h < G)
-      for (int p = lane >> 4; p < up.parts; p += 2) M = fmaxf(M, __ldcg(src + (long long)p * G).x);
-    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
-    if (h < G)
-      for (int p = lane >> 4; p < up.parts; p += 2) {
-        const float2 x = __ldcg(src + (long long)p * G);
-        L = fmaf(x.y, x.x == M ? 1.f : ex2_ftz(x.x - M), L);
-      }
-    L += __shfl_xor_sync(0xffffffffu, L, 16);
-    __syncwarp();
-    if (lane < G) ml[h] = make_float2(M, 1.f / L);
-    __syncwarp();
-    const int t0 = (int)(max(lo, at) - at) * kTile, t1 = min((int)(min(hi, at + tiles) - at) * kTile, len);
+    const int t0 = (int)(max(lo, at) - at) * kGroup, t1 = min((int)(min(hi, at + groups) - at) * kGroup, len);
     const int32_t* const pages = a.index.block_table + (long long)b * a.index.pages_per_seq;
     auto page_of = [&](int t) { return t < t1 ? __ldg(pages + (t >> log2)) : -1; };
+    constexpr int kStep = 4 * kJoinThreads;
     int page[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) page[j] = page_of(t0 + 32 * j + lane);
-    for (int t = t0 + lane; t < t1 + lane; t += 32 * kAhead) {  // as often in every lane
-      const float* s[kAhead];
+    for (int j = 0; j < kAhead; ++j) page[j] = page_of(t0 + kStep * j + 4 * threadIdx.x);
+    for (int h = warp; h < G; h += kJoinWarps) {
+      float M = -INFINITY, L = 0.f;
+      auto join = [&](float m, float l) {
+        const float to = fmaxf(M, m);
+        L = L * (M == to ? 1.f : ex2_ftz(M - to)) + l * (m == to ? 1.f : ex2_ftz(m - to));
+        M = to;
+      };
+      for (int p = lane; p < up.parts; p += 32) {
+        const float2 x = __ldcg(a.part_ml + (long long)(up.slot0 + p) * G + h);
+        join(x.x, x.y);
+      }
+#pragma unroll
+      for (int off = 16; off; off >>= 1)
+        join(__shfl_xor_sync(0xffffffffu, M, off), __shfl_xor_sync(0xffffffffu, L, off));
+      if (lane == 0) s_ml[h] = make_float2(M, 1.f / L);
+    }
+    __syncthreads();
+    for (int t = t0 + 4 * threadIdx.x; t < t1; t += kStep * kAhead) {
+      const float4* s[kAhead];
       long long row[kAhead];
-      float w[kAhead], old[kAhead];
+      float4 w[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const int x = t + 32 * j;
+        const int x = t + kStep * j;
         const bool there = x < t1 && (unsigned)page[j] < (unsigned)a.index.num_pages;  // else flagged before
         row[j] = there ? (((long long)page[j] * hkv + kvh) << log2) + (x & ((1 << log2) - 1)) : -1;
-        s[j] = a.scores + (there ? (at + x / kTile) * (G * kTile) + x % kTile : 0);
-        w[j] = 0.f;
-        old[j] = 0.f;
-        if (there) old[j] = __ldcg(a.w_in + row[j]);
-        page[j] = page_of(x + 32 * kAhead);
+        s[j] = reinterpret_cast<const float4*>(
+            a.scores + (there ? (at + x / kGroup) * (G * kGroup) + x % kGroup : 0));
+        w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (there) w[j] = __ldcg(reinterpret_cast<const float4*>(a.w_in + row[j]));
+        page[j] = page_of(x + kStep * kAhead);
       }
+      float4 sum[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int i = 0; i < G; ++i) {
-        const float2 x = ml[i];
-        float y[kAhead];
+        const float2 x = s_ml[i];
+        float4 y[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) y[j] = __ldcg(s[j] + i * kTile);
+        for (int j = 0; j < kAhead; ++j) y[j] = __ldcg(s[j] + i * (kGroup / 4));
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) w[j] = fmaf(ex2_ftz(y[j] - x.x), x.y, w[j]);
+        for (int j = 0; j < kAhead; ++j) {
+          sum[j].x = fmaf(ex2_ftz(y[j].x - x.x), x.y, sum[j].x);
+          sum[j].y = fmaf(ex2_ftz(y[j].y - x.x), x.y, sum[j].y);
+          sum[j].z = fmaf(ex2_ftz(y[j].z - x.x), x.y, sum[j].z);
+          sum[j].w = fmaf(ex2_ftz(y[j].w - x.x), x.y, sum[j].w);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (row[j] >= 0) a.w_out[row[j]] = old[j] + w[j];
+      for (int j = 0; j < kAhead; ++j) {
+        if (row[j] < 0) continue;
+        const int left = t1 - (t + kStep * j);
+        const float4 v =
+            make_float4(w[j].x + sum[j].x, w[j].y + sum[j].y, w[j].z + sum[j].z, w[j].w + sum[j].w);
+        float* const to = a.w_out + row[j];
+        if (left >= 4) {
+          *reinterpret_cast<float4*>(to) = v;
+        } else {
+          to[0] = v.x;
+          if (left > 1) to[1] = v.y;
+          if (left > 2) to[2] = v.z;
+        }
+      }
     }
-    at += tiles;
+    at += groups;
     if (at >= hi) return;
     if (++kvh == hkv) {
       kvh = 0;
       do {
         ++b;
-        first = __ldcg(a.seq_tiles + b);
-        tiles = (int)(__ldcg(a.seq_tiles + b + 1) - first);
-      } while (tiles == 0);
+        first = __ldcg(a.seq_groups + b);
+        groups = (int)(__ldcg(a.seq_groups + b + 1) - first);
+      } while (groups == 0);
     }
+    __syncthreads();  // s_ml is free again
   }
 }
 
+// The blocks of weights, of one wave, come first: they take longer than the others.
 template <int D, bool kScored>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args a, int join_blocks) {
-  __shared__ float2 s_ml[kJoinWarps][16];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Args a, int weight_blocks) {
   allow_dependent_launch();
   grid_dependency_wait();
-  if ((int)blockIdx.x < join_blocks) {
-    join_rows<D>(a, blockIdx.x);
-  } else if constexpr (kScored) {
-    const int warp = threadIdx.x >> 5;
-    add_weights(a, (long long)(blockIdx.x - join_blocks) * kJoinWarps + warp,
-                (long long)(gridDim.x - join_blocks) * kJoinWarps, s_ml[warp]);
+  if constexpr (kScored) {
+    if ((int)blockIdx.x < weight_blocks) {
+      add_weights(a, blockIdx.x, weight_blocks);
+      return;
+    }
   }
+  join_rows<D>(a, blockIdx.x - weight_blocks);
 }
-
-int max_ctas() { return device_sm_count() * 2; }
 
 // Workspace: status word | units | partial results | scores, or the prefix's results.
 struct Layout {
   size_t units_off, seq_off, ml_off, acc_off, scores_off, prefix_ml_off, prefix_acc_off, total;
-  long long score_tiles;
+  long long score_groups;
 };
 
 Layout layout(int batch, int n_kv_heads, int group, int head_dim, long long score_tokens, size_t prefix_rows) {
-  const size_t units = (size_t)batch * n_kv_heads, slots = units + max_ctas();
+  const size_t units = (size_t)batch * n_kv_heads, slots = units + kMostCtasPerSm * (size_t)std::max(1, device_sm_count());
   Layout w;
   w.units_off = kStatusBytes;
   w.seq_off = w.units_off + up256(units * sizeof(UnitParts));
   w.ml_off = w.seq_off + up256(((size_t)batch + 1) * sizeof(long long));
   w.acc_off = w.ml_off + up256(slots * group * sizeof(float2));
   w.scores_off = w.acc_off + up256(slots * group * head_dim * sizeof(float));
-  w.score_tiles = score_tokens / kTile * n_kv_heads;
-  w.prefix_ml_off = w.scores_off + up256((size_t)w.score_tiles * kTile * group * sizeof(float));
+  // every sequence's scores start in a group of their own
+  w.score_groups = score_tokens ? (score_tokens / kGroup + batch) * n_kv_heads : 0;
+  w.prefix_ml_off = w.scores_off + up256((size_t)w.score_groups * kGroup * group * sizeof(float));
   w.prefix_acc_off = w.prefix_ml_off + up256(prefix_rows * sizeof(float2));
   w.total = w.prefix_acc_off + up256(prefix_rows * head_dim * sizeof(float));
   return w;
@@ -752,16 +795,16 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
   // no more CTAs than a full cache could feed, one for each unit at least
   const long long units = (long long)a.batch * a.index.n_kv_heads;
   const long long tiles = units * ((a.index.capacity() + kTile - 1) / kTile);
-  const long long ctas = std::min<long long>(max_ctas(), std::max(units, (tiles + kMinTiles - 1) / kMinTiles));
+  const long long ctas = std::min<long long>(device_sm_count() * C::kCtasPerSm, std::max(units, (tiles + kMinTiles - 1) / kMinTiles));
   Args args = a;
   void* p[] = {&args};
   cudaError_t e = launch_with_pdl(fn, dim3((unsigned)ctas), dim3(kThreads), p, C::kSmemBytes, stream);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.batch * a.n_q_heads;
-  int join_blocks = (int)((rows + kJoinWarps - 1) / kJoinWarps);
-  int blocks = join_blocks;
-  if (kScored) blocks += (int)std::min<long long>(device_sm_count() * 16, (tiles + 4 * kJoinWarps - 1) / (4 * kJoinWarps));
-  void* p2[] = {&args, &join_blocks};
+  int weight_blocks = 0;
+  if (kScored) weight_blocks = (int)std::min<long long>(device_sm_count() * 3, (tiles + 31) / 32);
+  const int blocks = weight_blocks + (int)((rows + kJoinWarps - 1) / kJoinWarps);
+  void* p2[] = {&args, &weight_blocks};
   return launch_with_pdl(reinterpret_cast<const void*>(&join_kernel<D, kScored>), dim3((unsigned)blocks),
                          dim3(kJoinThreads), p2, 0, stream);
 }
@@ -795,7 +838,8 @@ int check_paged_pool(const void* k_pages, const void* v_pages, const void* block
 
 int check_weights(const float* in, const float* out, int n_kv_heads, int page_size, int num_pages) {
   if (!in || !out) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
-  if (!aligned(in, 4) || !aligned(out, 4)) return set_last_error(LARA_ERR_STREAM_DEST, "weights must be 4-byte aligned");
+  if (!aligned(in, 16) || !aligned(out, 16))
+    return set_last_error(LARA_ERR_STREAM_DEST, "weights must be 16-byte aligned");
   if (in != out && kvq::overlap(in, out, (size_t)num_pages * n_kv_heads * page_size * 4))
     return set_last_error(LARA_ERR_STREAM_DEST, "weights_out must be weights or lie apart from them");
   return LARA_OK;
@@ -843,11 +887,11 @@ void place(Args& a, const Layout& w, void* workspace) {
   char* base = static_cast<char*>(workspace);
   a.status = reinterpret_cast<int*>(base);
   a.units = reinterpret_cast<UnitParts*>(base + w.units_off);
-  a.seq_tiles = reinterpret_cast<long long*>(base + w.seq_off);
+  a.seq_groups = reinterpret_cast<long long*>(base + w.seq_off);
   a.part_ml = reinterpret_cast<float2*>(base + w.ml_off);
   a.part_acc = reinterpret_cast<float*>(base + w.acc_off);
   a.scores = reinterpret_cast<float*>(base + w.scores_off);
-  a.score_tiles = w.score_tiles;
+  a.score_groups = w.score_groups;
 }
 
 template <bool kScored>

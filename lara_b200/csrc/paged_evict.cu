@@ -40,8 +40,15 @@ constexpr int kMostEntries = 2048;   // of the block table in shared memory
 // kMostSlots (2^24 slots to a sequence), whose bits alone are more, one.
 constexpr int kShortSmem = 56 * 1024, kLongSmem = 92 * 1024, kMostSmem = 200 * 1024;
 constexpr long long kMostSlots = 1ll << 24;
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 256, kMoveCtas = 3;  // one wave: more CTAs took 122 us for 110
 constexpr int kFlight = 8;           // 16-byte accesses of a lane in flight
+
+// A slot of a unit, and the pool's row that it is; kBadRow on a bad page.
+struct __align__(8) Listed {
+  int slot;
+  uint32_t row;
+};
+constexpr uint32_t kBadRow = 0xffffffffu;
 
 struct Args {
   uint16_t* k;
@@ -55,8 +62,8 @@ struct Args {
   int batch, head_dim, keep, first, last;
   int* status;
   int* counts;        // [units] rows to move
-  int* holes;         // [units][keep]
-  int* movers;        // [units][keep]
+  Listed* holes;      // [units][keep]
+  Listed* movers;     // [units][keep]
 };
 
 // Weights as integers of the same order: negative ones flipped, -0 as 0, NaN on top.
@@ -108,6 +115,7 @@ template <int kThreads, int kCtas, bool kLong>
 __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_constant__ Args a, const SliceRoom room) {
   constexpr int kWarps = kThreads / 32;
   constexpr uint32_t kFull = 0xffffffffu;
+  constexpr int kUnroll = kLong ? 4 : 1;
   extern __shared__ uint32_t s_kept[];
   uint32_t* const s_keys = s_kept + room.words;
   int* const s_entry = reinterpret_cast<int*>(s_keys + room.run_keys * kWarps);
@@ -115,6 +123,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   __shared__ int s_scan[kWarps];
   __shared__ int s_totals[3];  // this CTA's, read by the cluster: ties, holes, movers
   __shared__ uint32_t s_pick[3];
+  __shared__ __align__(16) float s_zero[4];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = kLong ? cluster.block_rank() : 0, size = kLong ? cluster.num_blocks() : 1;
   const int unit = blockIdx.x / size, hkv = a.index.n_kv_heads, b = unit / hkv, h = unit % hkv;
@@ -122,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
 
   allow_dependent_launch();
   for (int i = threadIdx.x; i < 2 * kBins; i += kThreads) s_hist[0][i] = 0;
+  if (threadIdx.x < 4) s_zero[threadIdx.x] = 0.f;
   grid_dependency_wait();
 
   int raw;
@@ -169,15 +179,20 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   // ---- the slots' keys (a bad page's weigh nothing) and the first pass over them, four slots
   // to a lane.  Where weights are written apart, those before `keep` are copied here (of the
   // holes too: moved rows' weights replace those) and the ones behind cleared ----
-  const int cached = r_lo + room.run_keys;  // keys of the run's slots before this one are kept
-  uint32_t* const run_keys = s_keys + warp * room.run_keys - r_lo;
+  const int cached = r_lo + room.run_keys;  // weights of the run's slots before this one are kept
+  float* const run_w = reinterpret_cast<float*>(s_keys) + warp * room.run_keys - r_lo;
   auto ordered4 = [](const float4& w) {
     return make_uint4(ordered(w.x), ordered(w.y), ordered(w.z), ordered(w.w));
   };
-  auto keys = [&](int t) {  // of slots t .. t + 3 of the warp's run, which only this lane asks for
-    if (!kLong || t < cached) return *reinterpret_cast<const uint4*>(run_keys + t);
-    const long long r = t < r_hi ? row_of(t) : -1;
-    return ordered4(r < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(reinterpret_cast<const float4*>(a.w_in + r)));
+  // Of slots t .. t + 3 of the warp's run, which only this lane asks for.  One load, wherever it
+  // goes, so that those of several rows are in flight at once.
+  auto keys = [&](int t) {
+    const float* from = run_w + t;
+    if (kLong && t >= cached) {
+      const long long r = t < r_hi ? row_of(t) : -1;
+      from = r < 0 ? s_zero : a.w_in + r;
+    }
+    return ordered4(*reinterpret_cast<const float4*>(from));
   };
   const int p_lo = a.first, p_hi = n - a.last;  // slots that nothing protects; of them `free_` stay
   const int m_lo = max(r_lo, p_lo), m_hi = min(r_hi, p_hi);
@@ -208,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
         const int t = t0 + 128 * j;
         if (t >= r_hi) break;
         const uint4 x = ordered4(w[j]);
-        if (!kLong || t < cached) *reinterpret_cast<uint4*>(run_keys + t) = x;
+        if (!kLong || t < cached) *reinterpret_cast<float4*>(run_w + t) = w[j];
         count(t, x, 0, 0, 21, kBins);
         if (copies && row[j] >= 0) {
           if (t + 3 < min(n, a.keep)) {
@@ -231,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   for (int pass = 0; pass < 3 && free_ > 0; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
     if (pass > 0) {
-#pragma unroll 1
+#pragma unroll kUnroll
       for (int t = r_lo + 4 * lane; t < m_hi; t += 128) count(t, keys(t), border, mask, shift, bins);
     }
     if (kLong && size > 1) {
@@ -305,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   int seen = 0, unused;  // slots at the border before the run
   if (by_slot) {
     int mine = 0;
-#pragma unroll 1
+#pragma unroll kUnroll
     for (int t = r_lo + 4 * lane; t < m_hi; t += 128) {
       const uint4 x = keys(t);
       const uint32_t v[4] = {x.x, x.y, x.z, x.w};
@@ -318,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   // ---- which slots stay: bit `lane` of word j of a row of 128 is slot 4 lane + j ----
   uint4* const run_kept = reinterpret_cast<uint4*>(s_kept) + (r_lo - lo) / 128;
   const uint32_t lower = (1u << lane) - 1;
-#pragma unroll 1
+#pragma unroll kUnroll
   for (int t0 = r_lo; t0 < r_hi; t0 += 128) {
     const int t = t0 + 4 * lane;
     uint4 x = make_uint4(0, 0, 0, 0);
@@ -385,22 +400,25 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   holes = runs_before(__reduce_add_sync(kFull, holes), 1, all_holes);
   movers = runs_before(__reduce_add_sync(kFull, movers), 2, unused);
   if (rank == 0 && threadIdx.x == 0) a.counts[unit] = all_holes;
-  int* const hole_list = a.holes + (long long)unit * a.keep;
-  int* const mover_list = a.movers + (long long)unit * a.keep;
+  Listed* const hole_list = a.holes + (long long)unit * a.keep;
+  Listed* const mover_list = a.movers + (long long)unit * a.keep;
 #pragma unroll 1
   for (int t0 = r_lo; t0 < r_hi; t0 += 128) {
     uint32_t hm[4], mm[4];
     listed(t0, hm, mm);
-    auto list = [&](const uint32_t m[4], int* to, int& at) {
+    auto list = [&](const uint32_t m[4], Listed* to, int& at) {
       int here = at, all = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         here += __popc(m[j] & lower);
         all += __popc(m[j]);
       }
+      if ((m[0] | m[1] | m[2] | m[3]) >> lane & 1) {
+        const long long r = row_of(t0 + 4 * lane);  // of the lane's four slots' first
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (m[j] >> lane & 1) to[here++] = t0 + 4 * lane + j;
+        for (int j = 0; j < 4; ++j)
+          if (m[j] >> lane & 1) to[here++] = Listed{t0 + 4 * lane + j, r < 0 ? kBadRow : (uint32_t)r + j};
+      }
       at += all;
     };
     if (hm[0] | hm[1] | hm[2] | hm[3]) list(hm, hole_list, holes);
@@ -418,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
 
 // Rows of all units, laid end to end; each warp of the grid takes an equal run.
 template <int D>
-__global__ void __launch_bounds__(kMoveThreads, 3) move_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kMoveThreads, kMoveCtas) move_kernel(const __grid_constant__ Args a) {
   constexpr int kWarpsHere = kMoveThreads / 32;
   constexpr int kLanes = D / 8;             // lanes of a row
   constexpr int kAtOnce = 32 / (2 * kLanes);  // pairs of rows (K and V) in one access
@@ -450,21 +468,22 @@ __global__ void __launch_bounds__(kMoveThreads, 3) move_kernel(const __grid_cons
   long long at = s_at;
   for (int u = s_unit; u < units && at < hi; ++u) {
     const int count = __ldcg(a.counts + u);
-    const int b = u / hkv, h = u % hkv;
     const int i_lo = (int)(max(lo, at) - at), i_hi = (int)(min(hi, at + count) - at);
     const long long list = (long long)u * a.keep;
+    auto listed = [&](const Listed* from, int i) {
+      Listed x{0, kBadRow};
+      if (i < i_hi) *reinterpret_cast<int2*>(&x) = __ldcg(reinterpret_cast<const int2*>(from + list + i));
+      return x;
+    };
+    Listed hole = listed(a.holes, i_lo + warp * 32 + lane), mover = listed(a.movers, i_lo + warp * 32 + lane);
     for (int i0 = i_lo + warp * 32; i0 < i_hi; i0 += kWarpsHere * 32) {
-      const int i = i0 + lane;
-      long long to = -1, from = -1;
-      if (i < i_hi) {
-        const int d = __ldcg(a.holes + list + i), s = __ldcg(a.movers + list + i);
-        to = a.index.row(b, h, d, nullptr);  // flagged where its weight was read
-        from = a.index.row(b, h, s, nullptr);
-        if (a.sources) a.sources[list + d] = s;
-        if (to >= 0 && from >= 0) a.w_out[to] = a.w_in[from];
-        if (from >= 0) a.w_out[from] = 0.f;
-        if (from < 0 || to < 0) to = from = -1;
-      }
+      const int next = i0 + kWarpsHere * 32 + lane;
+      const bool moves = hole.row != kBadRow && mover.row != kBadRow;  // else flagged where weights were read
+      const uint32_t to = moves ? hole.row : kBadRow, from = moves ? mover.row : kBadRow;
+      float w = 0.f;
+      if (moves) w = __ldcg(a.w_in + from);
+      if (a.sources && i0 + lane < i_hi) a.sources[list + hole.slot] = mover.slot;
+      const Listed next_hole = listed(a.holes, next), next_mover = listed(a.movers, next);
       const int pairs = min(32, i_hi - i0);
       uint16_t* const pages = lane & kLanes ? a.v : a.k;
       const int sub = lane / (2 * kLanes), chunk = lane % kLanes;
@@ -474,16 +493,20 @@ __global__ void __launch_bounds__(kMoveThreads, 3) move_kernel(const __grid_cons
 #pragma unroll
         for (int j = 0; j < kFlight; ++j) {
           const int p = p0 + j * kAtOnce + sub;  // below 32
-          const long long f = __shfl_sync(0xffffffffu, from, p);
-          if (f >= 0) x[j] = __ldcg(reinterpret_cast<const uint4*>(pages + f * D) + chunk);
+          const uint32_t f = __shfl_sync(0xffffffffu, from, p);
+          if (f != kBadRow) x[j] = __ldcg(reinterpret_cast<const uint4*>(pages + (long long)f * D) + chunk);
         }
 #pragma unroll
         for (int j = 0; j < kFlight; ++j) {
           const int p = p0 + j * kAtOnce + sub;
-          const long long d = __shfl_sync(0xffffffffu, to, p);
-          if (d >= 0) reinterpret_cast<uint4*>(pages + d * D)[chunk] = x[j];
+          const uint32_t d = __shfl_sync(0xffffffffu, to, p);
+          if (d != kBadRow) reinterpret_cast<uint4*>(pages + (long long)d * D)[chunk] = x[j];
         }
       }
+      if (moves) a.w_out[to] = w;
+      if (mover.row != kBadRow) a.w_out[mover.row] = 0.f;
+      hole = next_hole;
+      mover = next_mover;
     }
     at += count;
   }
@@ -498,8 +521,8 @@ Layout layout(int batch, int n_kv_heads, int keep) {
   Layout w;
   w.counts_off = kStatusBytes;
   w.holes_off = w.counts_off + up256(units * sizeof(int));
-  w.movers_off = w.holes_off + up256(units * keep * sizeof(int));
-  w.total = w.movers_off + up256(units * keep * sizeof(int));
+  w.movers_off = w.holes_off + up256(units * keep * sizeof(Listed));
+  w.total = w.movers_off + up256(units * keep * sizeof(Listed));
   return w;
 }
 
@@ -542,7 +565,7 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
   // no more CTAs than rows can move, 256 to a CTA
   const long long most = (long long)units * std::min<long long>(a.keep, std::max(0ll, cap - a.keep));
   if (most == 0) return cudaSuccess;
-  const int blocks = (int)std::min<long long>(sms * 8, (most + 31) / 32);
+  const int blocks = (int)std::min<long long>(sms * kMoveCtas, (most + 31) / 32);
   const void* mv = a.head_dim == 128 ? reinterpret_cast<const void*>(&move_kernel<128>)
                                      : reinterpret_cast<const void*>(&move_kernel<64>);
   return launch_with_pdl(mv, dim3((unsigned)blocks), dim3(kMoveThreads), p, 0, stream);
@@ -574,17 +597,16 @@ extern "C" int lara_kv_evict(uint16_t* k_pages, uint16_t* v_pages, const float* 
   if ((long long)batch * n_kv_heads > 0x7fffffffll / kMaxCluster)
     return set_last_error(LARA_ERR_BAD_CFG, "batch * n_kv_heads must be below 2^28");
   if (!weights || !weights_out || !seq_lens || !workspace) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
-  if (!aligned(weights, 4) || !aligned(weights_out, 4) || !aligned(seq_lens, 4) || !aligned(workspace, 256))
-    return set_last_error(LARA_ERR_STREAM_DEST, "the workspace must be 256-byte aligned, all else 4-byte");
+  if (!aligned(seq_lens, 4) || !aligned(new_lens, 4) || !aligned(sources, 4) || !aligned(workspace, 256))
+    return set_last_error(LARA_ERR_STREAM_DEST, "lengths and sources must be 4-byte aligned, the workspace 256-byte");
   if (a.index.capacity() > kMostSlots)
     return set_last_error(LARA_ERR_UNSUPPORTED, "eviction from sequences of at most 2^24 slots");
-  if ((long long)num_pages * n_kv_heads > 0x7fffffffll)
-    return set_last_error(LARA_ERR_BAD_CFG, "num_pages * n_kv_heads must be below 2^31");
+  if ((long long)num_pages * n_kv_heads * page_size >= (long long)kBadRow ||
+      (long long)num_pages * n_kv_heads > 0x7fffffffll)
+    return set_last_error(LARA_ERR_BAD_CFG, "pools of less than 2^32 - 1 rows, 2^31 pages of one head");
   if (kvq::overlap(new_lens, seq_lens, (size_t)batch * 4))
     return set_last_error(LARA_ERR_STREAM_DEST, "new_lens must lie apart from seq_lens");
   if (const int rc = check_weights(weights, weights_out, n_kv_heads, page_size, num_pages)) return rc;
-  if (!aligned(weights, 16) || !aligned(weights_out, 16))
-    return set_last_error(LARA_ERR_STREAM_DEST, "weights must be 16-byte aligned");
   const Layout w = layout(batch, n_kv_heads, keep);
   if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "eviction workspace too small");
   a.k = k_pages;
@@ -602,8 +624,8 @@ extern "C" int lara_kv_evict(uint16_t* k_pages, uint16_t* v_pages, const float* 
   char* base = static_cast<char*>(workspace);
   a.status = reinterpret_cast<int*>(base);
   a.counts = reinterpret_cast<int*>(base + w.counts_off);
-  a.holes = reinterpret_cast<int*>(base + w.holes_off);
-  a.movers = reinterpret_cast<int*>(base + w.movers_off);
+  a.holes = reinterpret_cast<Listed*>(base + w.holes_off);
+  a.movers = reinterpret_cast<Listed*>(base + w.movers_off);
   const cudaError_t e = launch(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess)
     return set_last_error(LARA_ERR_CUDA, std::string("evict launch: ") + cudaGetErrorString(e));
