@@ -19,6 +19,8 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <set>
+#include <utility>
 
 #include "paged.cuh"
 
@@ -40,8 +42,10 @@ constexpr int kMostEntries = 2048;   // of the block table in shared memory
 // kMostSlots (2^24 slots to a sequence), whose bits alone are more, one.
 constexpr int kShortSmem = 56 * 1024, kLongSmem = 92 * 1024, kMostSmem = 200 * 1024;
 constexpr long long kMostSlots = 1ll << 24;
-constexpr int kMoveThreads = 256, kMoveCtas = 3;  // one wave: more CTAs took 122 us for 110
-constexpr int kFlight = 8;           // 16-byte accesses of a lane in flight
+// Rows up to which a unit's CTA moves them itself.
+constexpr int kFewMoves = 64;
+constexpr int kMoveThreads = 192;
+constexpr int kMoveSmem = kMoveThreads / 32 * 2 * 32 * 512;
 
 // A slot of a unit, and the pool's row that it is; kBadRow on a bad page.
 struct __align__(8) Listed {
@@ -68,9 +72,8 @@ struct Args {
 
 // Weights as integers of the same order: negative ones flipped, -0 as 0, NaN on top.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  if (x != x) return 0xffffffffu;
   const uint32_t u = __float_as_uint(x + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return x == x ? u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u) : 0xfffffffeu;
 }
 
 __device__ __forceinline__ int slots_of(const Args& a, int b, int* raw = nullptr) {
@@ -111,7 +114,8 @@ struct SliceRoom {
 
 // kLong: clusters of CTAs, and slices that shared memory need not hold; without it, one CTA to a
 // unit, and all of that left out, since code that runs once waits mostly for its own instructions.
-template <int kThreads, int kCtas, bool kLong>
+// kMoves: no unit has more than kFewMoves rows to move, and its CTA moves them itself.
+template <int kThreads, int kCtas, bool kLong, bool kMoves>
 __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_constant__ Args a, const SliceRoom room) {
   constexpr int kWarps = kThreads / 32;
   constexpr uint32_t kFull = 0xffffffffu;
@@ -124,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   __shared__ int s_totals[3];  // this CTA's, read by the cluster: ties, holes, movers
   __shared__ uint32_t s_pick[3];
   __shared__ __align__(16) float s_zero[4];
+  __shared__ Listed s_listed[2][kMoves ? kFewMoves : 1];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = kLong ? cluster.block_rank() : 0, size = kLong ? cluster.num_blocks() : 1;
   const int unit = blockIdx.x / size, hkv = a.index.n_kv_heads, b = unit / hkv, h = unit % hkv;
@@ -163,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
     return e < 0 ? -1 : (e << log2) + (t & ((1 << log2) - 1));
   };
   if (n <= a.keep) {
-    if (rank == 0 && threadIdx.x == 0) a.counts[unit] = 0;
+    if (!kMoves && rank == 0 && threadIdx.x == 0) a.counts[unit] = 0;
     for (int t = lo + threadIdx.x; t < hi; t += kThreads) {
       const long long r = row_of(t);
       if (r < 0)
@@ -195,14 +200,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
     return ordered4(*reinterpret_cast<const float4*>(from));
   };
   const int p_lo = a.first, p_hi = n - a.last;  // slots that nothing protects; of them `free_` stay
-  const int m_lo = max(r_lo, p_lo), m_hi = min(r_hi, p_hi);
+  const int m_lo = max(r_lo, p_lo), m_hi = min(r_hi, p_hi), m_count = max(0, m_hi - m_lo);
   const int free_ = a.keep - a.first - a.last;
   auto count = [&](int t, const uint4& x, uint32_t border, uint32_t mask, int shift, int bins) {
     const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+    uint32_t* const hist = s_hist[lane & 1];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (t + j >= m_lo && t + j < m_hi && (v[j] & mask) == border)
-        atomicAdd(&s_hist[lane & 1][(v[j] >> shift) & (bins - 1)], 1u);
+      if ((unsigned)(t + j - m_lo) < (unsigned)m_count && (v[j] & mask) == border)
+        atomicAdd(hist + ((v[j] >> shift) & (bins - 1)), 1u);
   };
   {
     bool bad = false;
@@ -330,6 +336,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
     seen = runs_before(__reduce_add_sync(kFull, mine), 0, unused);
   }
 
+  const uint32_t least = free_ > 0 ? border : 0xffffffffu;  // which no weight has
   // ---- which slots stay: bit `lane` of word j of a row of 128 is slot 4 lane + j ----
   uint4* const run_kept = reinterpret_cast<uint4*>(s_kept) + (r_lo - lo) / 128;
   const uint32_t lower = (1u << lane) - 1;
@@ -341,9 +348,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
     uint32_t v[4] = {x.x, x.y, x.z, x.w};
     bool stays[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      stays[j] = t + j < r_hi && (v[j] >= border ? free_ > 0 || t + j < p_lo || t + j >= p_hi
-                                                 : t + j < p_lo || t + j >= p_hi);
+    for (int j = 0; j < 4; ++j) {
+      const bool in = (unsigned)(t + j - p_lo) < (unsigned)(p_hi - p_lo);
+      stays[j] = t + j < r_hi && (!in || v[j] >= least);
+    }
     if (by_slot) {
       bool at[4];
       uint32_t m[4];
@@ -399,9 +407,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   int all_holes;
   holes = runs_before(__reduce_add_sync(kFull, holes), 1, all_holes);
   movers = runs_before(__reduce_add_sync(kFull, movers), 2, unused);
-  if (rank == 0 && threadIdx.x == 0) a.counts[unit] = all_holes;
-  Listed* const hole_list = a.holes + (long long)unit * a.keep;
-  Listed* const mover_list = a.movers + (long long)unit * a.keep;
+  if (!kMoves && rank == 0 && threadIdx.x == 0) a.counts[unit] = all_holes;
+  Listed* const hole_list = kMoves ? s_listed[0] : a.holes + (long long)unit * a.keep;
+  Listed* const mover_list = kMoves ? s_listed[1] : a.movers + (long long)unit * a.keep;
 #pragma unroll 1
   for (int t0 = r_lo; t0 < r_hi; t0 += 128) {
     uint32_t hm[4], mm[4];
@@ -432,14 +440,38 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
     }
   }
   if (kLong && size > 1) cluster.sync();  // s_totals may still be read
+  if constexpr (kMoves) {
+    __syncthreads();
+    const int row_words = a.head_dim / 8;  // lanes 0-15 have K's row, 16-31 V's
+    for (int i = warp; i < all_holes; i += kWarps) {
+      const Listed hole = s_listed[0][i], mover = s_listed[1][i];
+      if (lane == 0 && src) src[hole.slot] = mover.slot;
+      if (hole.row == kBadRow || mover.row == kBadRow) {  // flagged before
+        if (lane == 0 && mover.row != kBadRow) a.w_out[mover.row] = 0.f;
+        continue;
+      }
+      uint4* const rows = reinterpret_cast<uint4*>(lane < 16 ? a.k : a.v) + (lane & 15);
+      if ((lane & 15) < row_words)
+        rows[(long long)hole.row * row_words] = __ldcg(rows + (long long)mover.row * row_words);
+      if (lane == 0) {
+        a.w_out[hole.row] = __ldcg(a.w_in + mover.row);
+        a.w_out[mover.row] = 0.f;
+      }
+    }
+  }
 }
 
-// Rows of all units, laid end to end; each warp of the grid takes an equal run.
+// Rows of all units, laid end to end; each CTA takes an equal run.  A warp copies 32
+// pairs of rows (K and V) at a time through shared memory, the loads of one lot under
+// way while the one before is stored: two lots of 16 KB for each of six warps keep
+// about 96 KB of an SM's loads in flight, which registers had no room for.
 template <int D>
-__global__ void __launch_bounds__(kMoveThreads, kMoveCtas) move_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kMoveThreads, 1) move_kernel(const __grid_constant__ Args a) {
   constexpr int kWarpsHere = kMoveThreads / 32;
-  constexpr int kLanes = D / 8;             // lanes of a row
-  constexpr int kAtOnce = 32 / (2 * kLanes);  // pairs of rows (K and V) in one access
+  constexpr int kLanes = D / 8;               // lanes of a row
+  constexpr int kAtOnce = 32 / (2 * kLanes);  // pairs of rows in one access
+  constexpr int kAccesses = 32 / kAtOnce;     // of 32 pairs
+  extern __shared__ uint4 s_rows[];           // [warps][2][kAccesses][32]
   __shared__ long long s_sum[kWarpsHere];
   __shared__ int s_unit;
   __shared__ long long s_at;
@@ -465,6 +497,20 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveCtas) move_kernel(const __g
     s_at = before;
   }
   __syncthreads();
+  uint4* const buffer = s_rows + warp * (2 * kAccesses * 32) + lane;
+  uint16_t* const pages = lane & kLanes ? a.v : a.k;
+  const int sub = lane / (2 * kLanes), chunk = lane % kLanes;
+  // the lot whose loads are under way: where its rows go
+  uint32_t to = kBadRow;
+  int lot = 0;
+  auto store = [&] {  // of the lot before the last one
+    const uint4* const from = buffer + (lot & 1) * (kAccesses * 32);
+#pragma unroll 8
+    for (int j = 0; j < kAccesses; ++j) {
+      const uint32_t d = __shfl_sync(0xffffffffu, to, j * kAtOnce + sub);
+      if (d != kBadRow) reinterpret_cast<uint4*>(pages + (long long)d * D)[chunk] = from[j * 32];
+    }
+  };
   long long at = s_at;
   for (int u = s_unit; u < units && at < hi; ++u) {
     const int count = __ldcg(a.counts + u);
@@ -479,30 +525,25 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveCtas) move_kernel(const __g
     for (int i0 = i_lo + warp * 32; i0 < i_hi; i0 += kWarpsHere * 32) {
       const int next = i0 + kWarpsHere * 32 + lane;
       const bool moves = hole.row != kBadRow && mover.row != kBadRow;  // else flagged where weights were read
-      const uint32_t to = moves ? hole.row : kBadRow, from = moves ? mover.row : kBadRow;
       float w = 0.f;
-      if (moves) w = __ldcg(a.w_in + from);
+      if (moves) w = __ldcg(a.w_in + mover.row);
       if (a.sources && i0 + lane < i_hi) a.sources[list + hole.slot] = mover.slot;
       const Listed next_hole = listed(a.holes, next), next_mover = listed(a.movers, next);
-      const int pairs = min(32, i_hi - i0);
-      uint16_t* const pages = lane & kLanes ? a.v : a.k;
-      const int sub = lane / (2 * kLanes), chunk = lane % kLanes;
-#pragma unroll 1
-      for (int p0 = 0; p0 < pairs; p0 += kFlight * kAtOnce) {
-        uint4 x[kFlight];
-#pragma unroll
-        for (int j = 0; j < kFlight; ++j) {
-          const int p = p0 + j * kAtOnce + sub;  // below 32
-          const uint32_t f = __shfl_sync(0xffffffffu, from, p);
-          if (f != kBadRow) x[j] = __ldcg(reinterpret_cast<const uint4*>(pages + (long long)f * D) + chunk);
-        }
-#pragma unroll
-        for (int j = 0; j < kFlight; ++j) {
-          const int p = p0 + j * kAtOnce + sub;
-          const uint32_t d = __shfl_sync(0xffffffffu, to, p);
-          if (d != kBadRow) reinterpret_cast<uint4*>(pages + (long long)d * D)[chunk] = x[j];
-        }
+      const uint32_t from = moves ? mover.row : kBadRow;
+      const uint32_t into = smem_addr(buffer + (lot & 1) * (kAccesses * 32));
+#pragma unroll 8
+      for (int j = 0; j < kAccesses; ++j) {
+        const uint32_t f = __shfl_sync(0xffffffffu, from, j * kAtOnce + sub);
+        if (f != kBadRow)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(into + j * 512),
+                       "l"(reinterpret_cast<const uint4*>(pages + (long long)f * D) + chunk)
+                       : "memory");
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ++lot;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");  // a lane reads what it copied itself
+      store();
+      to = moves ? hole.row : kBadRow;
       if (moves) a.w_out[to] = w;
       if (mover.row != kBadRow) a.w_out[mover.row] = 0.f;
       hole = next_hole;
@@ -510,6 +551,9 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveCtas) move_kernel(const __g
     }
     at += count;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  ++lot;
+  store();
 }
 
 struct Layout {
@@ -526,6 +570,21 @@ Layout layout(int batch, int n_kv_heads, int keep) {
   return w;
 }
 
+// A kernel's shared memory (and clusters above eight), once per kernel and device.
+cudaError_t opt_in(const void* fn, int smem, bool clusters) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({fn, dev})) return cudaSuccess;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && clusters) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.insert({fn, dev});
+  return e;
+}
+
 cudaError_t launch(const Args& a, cudaStream_t stream) {
   const int units = a.batch * a.index.n_kv_heads, sms = device_sm_count();
   const long long cap = a.index.capacity();
@@ -533,9 +592,14 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
   while (size < kMaxCluster && (cap / size > kLongSlice || (cap / size > 4096 && (long long)units * size < sms)))
     size *= 2;
   const bool long_ = size > 1 || cap > kShortSlice;
-  const void* const fn = long_ ? reinterpret_cast<const void*>(&select_kernel<768, 2, true>)
-                               : reinterpret_cast<const void*>(&select_kernel<512, 3, false>);
-  const int threads = long_ ? 768 : 512, most_smem = long_ ? kLongSmem : kShortSmem;
+  const long long most = std::min<long long>(a.keep, std::max(0ll, cap - a.keep));  // rows of a unit to move
+  const bool moves = !long_ && most <= kFewMoves;
+  const bool alone = moves && units <= sms;  // a CTA has an SM to itself
+  const void* const fn = long_   ? reinterpret_cast<const void*>(&select_kernel<768, 2, true, false>)
+                         : alone ? reinterpret_cast<const void*>(&select_kernel<1024, 1, false, true>)
+                         : moves ? reinterpret_cast<const void*>(&select_kernel<512, 3, false, true>)
+                                 : reinterpret_cast<const void*>(&select_kernel<512, 3, false, false>);
+  const int threads = long_ ? 768 : alone ? 1024 : 512, most_smem = long_ ? kLongSmem : kShortSmem;
   // per slice: the bits, then the table, then as many keys as there is room for
   const long long run = ((cap + size - 1) / size + 4 * threads - 1) / (4 * threads) * 128, slice = run * (threads / 32);
   SliceRoom room;
@@ -544,31 +608,21 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
   const int left = std::max(0, most_smem / 4 - room.words - room.entries) / (4 * threads) * 128;
   room.run_keys = (int)std::min<long long>(run, left);
   const size_t smem = 4 * ((size_t)room.words + room.entries + (size_t)room.run_keys * (threads / 32));
-  {
-    static std::mutex mu;
-    static uint64_t done[2] = {0, 0};  // the opt-ins are per device
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev > 63 || !(done[long_] >> dev & 1)) {
-      e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
-      if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-      if (dev <= 63) done[long_] |= 1ull << dev;
-    }
-  }
+  cudaError_t e = opt_in(fn, kMostSmem, true);
+  if (e != cudaSuccess) return e;
   Args args = a;
   void* p[] = {&args, &room};
-  cudaError_t e = launch_with_pdl(fn, dim3((unsigned)units * size), dim3(threads), p, smem, stream, size);
+  e = launch_with_pdl(fn, dim3((unsigned)units * size), dim3(threads), p, smem, stream, size);
   if (e != cudaSuccess) return e;
-  // no more CTAs than rows can move, 256 to a CTA
-  const long long most = (long long)units * std::min<long long>(a.keep, std::max(0ll, cap - a.keep));
-  if (most == 0) return cudaSuccess;
-  const int blocks = (int)std::min<long long>(sms * kMoveCtas, (most + 31) / 32);
+  if (moves || most == 0) return cudaSuccess;
+  // no more CTAs than rows can move, 32 to a CTA
+  const int blocks = (int)std::min<long long>(sms, (units * most + 31) / 32);
   const void* mv = a.head_dim == 128 ? reinterpret_cast<const void*>(&move_kernel<128>)
                                      : reinterpret_cast<const void*>(&move_kernel<64>);
-  return launch_with_pdl(mv, dim3((unsigned)blocks), dim3(kMoveThreads), p, 0, stream);
+  const int move_smem = kMoveSmem * a.head_dim / 128;
+  e = opt_in(mv, move_smem, false);
+  if (e != cudaSuccess) return e;
+  return launch_with_pdl(mv, dim3((unsigned)blocks), dim3(kMoveThreads), p, move_smem, stream);
 }
 
 }  // namespace
