@@ -33,17 +33,11 @@ int check_paged_pool(const void* k_pages, const void* v_pages, const void* block
 int check_weights(const float* in, const float* out, int n_kv_heads, int page_size, int num_pages);
 
 // The pass over a shared prefix: row tiles of `seqs` sequences, taken in pairs
-// where there are two, `units` of them to a kv head; the prefix in `splits`
-// ranges.  Leaves (reference, sum) and unnormalised sums of every row of the
-// batch and every split.
+// where there are two; `units` of them (pairs) to a kv head, of `rows` rows each.
 struct PrefixPlan {
-  int seqs, units, splits;
-  bool pair;
+  int seqs, units, rows;
 };
-PrefixPlan prefix_plan(int batch, int n_kv_heads, int group, int tokens);
-cudaError_t prefix_launch(const PrefixPlan& plan, const uint16_t* q, const uint16_t* k, const uint16_t* v,
-                          const PoolIndex& index, int tokens, int batch, int n_q_heads, int head_dim, float scale_log2,
-                          float2* ml, float* acc, int* status, cudaStream_t stream);
+PrefixPlan prefix_plan(int batch, int group);
 
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
