@@ -145,15 +145,15 @@ struct OwnTokens {
   static constexpr long long kLow = (1ll << 40) - 1;
   struct Shared {
     long long sum[2][W];
-    Unit first[W];
+    long long ahead[W * 32];                       // of each thread's sequences, packed as `mine`
+    long long groups_ahead[kScored ? W * 32 : 1];
     float2 ml[W][NG * 8];
     int idle[W];
     int lens[kLensCached];
   };
   const DecodeArgs& a;
   Shared& sh_;
-  long long mine = 0, ahead = 0, groups_ahead = 0;  // of the thread's sequences, of those before them
-  long long total = 0, units = 0;                    // tiles, and units with tokens
+  long long total = 0, units = 0;  // tiles, and units with tokens
   int covering = 0;  // of the thread's sequences, those behind the shared prefix
 
   __device__ __forceinline__ OwnTokens(const DecodeArgs& args, Shared& shared) : a(args), sh_(shared) {}
@@ -188,6 +188,7 @@ struct OwnTokens {
   __device__ __forceinline__ void totals() {
     const int per_thread = (a.batch + C::kThreads - 1) / C::kThreads;
     const int b_lo = min(a.batch, (int)threadIdx.x * per_thread), b_hi = min(a.batch, b_lo + per_thread);
+    long long mine = 0;    // tiles in the low 40 bits, sequences that have some above
     long long groups = 0;  // scoring: of scores
     for (int b = b_lo; b < b_hi; ++b) {
       const int raw = __ldcg(a.lens + b);
@@ -195,15 +196,17 @@ struct OwnTokens {
       if (raw != len) atomicOr(a.status, kDevBadLength);
       if (b < kLensCached) sh_.lens[b] = len;
       const Own own = own_tokens(a, len);
-      mine += tiles_of(own.len) + (own.len > 0 ? 1ll << 40 : 0);  // tiles in the low 40 bits
+      mine += tiles_of(own.len) + (own.len > 0 ? 1ll << 40 : 0);
       groups += groups_of(tiles_of(own.len));
       covering += own.start > 0;
     }
     long long all;
-    ahead = prefix(mine, sh_.sum[0], all);
+    const long long ahead = prefix(mine, sh_.sum[0], all);
+    if (threadIdx.x < C::kThreads) sh_.ahead[threadIdx.x] = ahead;
     if constexpr (kScored) {
       long long all_groups;
-      groups_ahead = prefix(groups, sh_.sum[1], all_groups);
+      const long long groups_ahead = prefix(groups, sh_.sum[1], all_groups);
+      sh_.groups_ahead[threadIdx.x] = groups_ahead;
       if (blockIdx.x == 0) {
         long long at = groups_ahead;
         for (int b = b_lo; b < b_hi; ++b) {
@@ -215,6 +218,7 @@ struct OwnTokens {
     }
     total = (all & kLow) * a.index.n_kv_heads;
     units = (all >> 40) * a.index.n_kv_heads;
+    __syncthreads();
   }
 
   __device__ __forceinline__ bool solo_units(int ctas) const {
@@ -251,40 +255,36 @@ struct OwnTokens {
     const int workers = solo ? (int)min((long long)ctas * W, total)
                              : (int)min((long long)ctas, max((total + C::kMinTiles - 1) / C::kMinTiles, units));
     const int me = solo ? part * W + warp : part;
-    if ((solo ? part * W : part) >= workers) return;
+    if (me >= workers) return;  // no warp of a CTA that joins, or this warp for itself
     const Shares sh{quotient(span, workers), span - quotient(span, workers) * workers};
-    const int share = me < workers ? (int)(sh.start(me + 1) - sh.start(me)) : 0;
+    const int share = (int)(sh.start(me + 1) - sh.start(me));
+    Unit u0;
     {
-      // found by the thread that counted the sequence in which the share starts
-      const long long begin = ((ahead & kLow) + (ahead >> 40) * kUnitCost) * hkv;
-      const long long stop = begin + ((mine & kLow) + (mine >> 40) * kUnitCost) * hkv;
-      for (int w = 0; w < (solo ? W : 1); ++w) {
-        const int of = solo ? part * W + w : part;
-        if (of >= workers) break;
-        const long long x = sh.start(of);
-        if (x < begin || x >= stop) continue;
-        long long at = begin, group0 = groups_ahead * hkv;
-        const int per_thread = (a.batch + C::kThreads - 1) / C::kThreads;
-        Unit u{0, 0, 0, 0, 0, min(a.batch, (int)threadIdx.x * per_thread), 0};
-        for (;; ++u.b) {  // by whole sequences
-          const Own own = own_tokens(a, len_of(u.b));
-          u.start = own.start;
-          u.len = own.len;
-          u.tiles = tiles_of(u.len);
-          const long long span_b = u.tiles ? (long long)(u.tiles + kUnitCost) * hkv : 0;
-          if (x < at + span_b) break;
-          at += span_b;
-          group0 += (long long)groups_of(u.tiles) * hkv;
-        }
-        u.kvh = (int)quotient(x - at, u.tiles + kUnitCost);
-        u.base = (int)(at + (long long)u.kvh * (u.tiles + kUnitCost) + kUnitCost - x);
-        u.group0 = group0 + (long long)u.kvh * groups_of(u.tiles);
-        sh_.first[w] = u;
+      // the unit in which the share starts: the last thread that counted from at or before there,
+      // then by whole sequences
+      const long long x = sh.start(me);
+      auto place = [&](long long packed) { return ((packed & kLow) + (packed >> 40) * kUnitCost) * hkv; };
+      int of = 0;
+      for (int bit = 1 << (31 - __clz(C::kThreads)); bit; bit >>= 1)
+        if (of + bit < C::kThreads && place(sh_.ahead[of + bit]) <= x) of += bit;
+      const int per_thread = (a.batch + C::kThreads - 1) / C::kThreads;
+      long long at = place(sh_.ahead[of]), group0 = kScored ? sh_.groups_ahead[of] * hkv : 0;
+      Unit u{0, 0, 0, 0, 0, of * per_thread, 0};
+      for (;; ++u.b) {
+        const Own own = own_tokens(a, len_of(u.b));
+        u.start = own.start;
+        u.len = own.len;
+        u.tiles = tiles_of(u.len);
+        const long long span_b = u.tiles ? (long long)(u.tiles + kUnitCost) * hkv : 0;
+        if (x < at + span_b) break;
+        at += span_b;
+        group0 += (long long)groups_of(u.tiles) * hkv;
       }
+      u.kvh = (int)quotient(x - at, u.tiles + kUnitCost);
+      u.base = (int)(at + (long long)u.kvh * (u.tiles + kUnitCost) + kUnitCost - x);
+      u.group0 = group0 + (long long)u.kvh * groups_of(u.tiles);
+      u0 = u;
     }
-    sync();
-    if (share == 0) return;  // a warp without a share of its own
-    const Unit u0 = sh_.first[solo ? warp : 0];
     auto in_share = [&](const Unit& u) { return u.base < share; };
     auto tiles_end = [&](const Unit& u) { return min(share, u.base + u.tiles); };
 
@@ -297,25 +297,30 @@ struct OwnTokens {
     const uint32_t copy_at = c_row * C::kRowBytes + (((lane % kChunks) ^ c_row) << 4);
     Unit pu = u0;                           // where the next tile to fetch lies
     int pid = max(pu.base, 0) + offset;     // its number
-    int page = 0;                           // its page, fetched a tile ahead
+    int pages = 0, page_at = 32;            // pages of the unit's next tiles, one to a lane, and the next one's
     bool more = in_share(pu);
     const int log2 = a.index.page_log2;
-    auto fetch_page = [&] {
+    auto fetch_pages = [&] {  // a tile ahead
+      bool moved = page_at == 32;
       while (more && pid >= tiles_end(pu)) {
         next_unit(pu);
         pid = pu.base + offset;
         more = in_share(pu);
+        moved = true;
       }
-      if (!more) return;
-      const int pos = pu.start + (pid - pu.base) * kTile;
-      page = __ldcg(a.index.block_table + (long long)pu.b * a.index.pages_per_seq + (pos >> log2));
+      if (!more || !moved) return;
+      page_at = 0;
+      const int t = (pid - pu.base + lane * step) * kTile;
+      if (t < pu.len)
+        pages = __ldcg(a.index.block_table + (long long)pu.b * a.index.pages_per_seq + ((pu.start + t) >> log2));
     };
     auto fetch_tile = [&](int stage) {
       if (more) {
         const uint32_t st = smem_addr(ring) + stage * C::kStageBytes + copy_at;
         const int pos = pu.start + (pid - pu.base) * kTile;
+        int page = __shfl_sync(0xffffffffu, pages, page_at++);
         if ((unsigned)page >= (unsigned)a.index.num_pages) {
-          atomicOr(a.status, kDevBadPage);
+          if (lane == 0) atomicOr(a.status, kDevBadPage);
           page = 0;
         }
         const long long row0 = (((long long)page * hkv + pu.kvh) << log2) + (pos & ((1 << log2) - 1));
@@ -328,11 +333,11 @@ struct OwnTokens {
           cp_async16<C::kRowsBytes>(to, vs + i * 512, policy);
         }
         pid += step;
-        fetch_page();
+        fetch_pages();
       }
       cp_async_commit();
     };
-    fetch_page();
+    fetch_pages();
 #pragma unroll
     for (int s = 0; s < C::kStages - 1; ++s) fetch_tile(s);
 

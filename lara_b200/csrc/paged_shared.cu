@@ -58,8 +58,8 @@ struct Prefix {
   static constexpr int kVStages = D == 128 ? 2 : 4;
   static constexpr int kKOff = kQTiles * kTileBytes;
   static constexpr int kVOff = kKOff + kKStages * kTileBytes;
-  static constexpr int kBarOff = kVOff + kVStages * kTileBytes;
-  static constexpr int kRedOff = kBarOff + 256;     // exchange of the pairs: per stream, row maxima, then sums [2][2][2][128] floats
+  // exchange of the pairs: per stream, row maxima, then sums, [2][2][2][128] floats
+  static constexpr int kRedOff = kVOff + kVStages * kTileBytes;
   static constexpr int kSmem = kRedOff + 2 * 2 * 2 * kTileM * 4 + 1024;
   static constexpr int kRows = kQTiles * kTileM;
 };
@@ -74,7 +74,47 @@ struct Bars {
   int abort;
   int k_issued, v_issued, q_issued;
 };
-static_assert(sizeof(Bars) <= 256, "barrier block");
+// What one lane of a whole warp issues.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one;
+}
+__device__ __forceinline__ void mma_ss_one(uint32_t one, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_one(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_one(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+      "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort));
+}
 
 struct PrefixArgs {
   int units;  // of all kv heads
@@ -88,10 +128,10 @@ struct Segment {
 
 template <int D, bool kPair>
 __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
-                                            const DecodeArgs& a, const PrefixArgs& p, int me, int ctas, uint8_t* smem_raw) {
+                                            const DecodeArgs& a, const PrefixArgs& p, int me, int ctas,
+                                            uint8_t* smem_raw, Bars* bars, uint32_t tmem) {
   using C = Prefix<D, kPair>;
   uint8_t* const smem = smem_raw + (-smem_addr(smem_raw) & 1023);
-  Bars* const bars = reinterpret_cast<Bars*>(smem + C::kBarOff);
   volatile int* const abort = &bars->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long all = (long long)p.units * p.tiles;
@@ -110,36 +150,6 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
   auto seq_of = [&](const Segment& g) { return g.unit % a.prefix.units * (C::kQTiles * a.prefix.seqs); };
   // step i of a segment: stream i & 1, tile i / 2 (pair) or i
   auto steps_of = [](const Segment& g) { return kPair ? 2 * g.n : g.n; };
-
-  if (threadIdx.x == 0) {
-    mbar_init(&bars->q_full, 1);
-    mbar_init(&bars->q_empty, 1);
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(&bars->k_full[s], 1);
-      mbar_init(&bars->k_empty[s], 1);
-      mbar_init(&bars->v_full[s], 1);
-      mbar_init(&bars->v_empty[s], 1);
-    }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&bars->s_full[t], 1);
-      mbar_init(&bars->p_full[t], kSoftmaxWarps * 32);
-      mbar_init(&bars->o_full[t], 1);
-    }
-    mbar_init(&bars->drain, 1);
-    bars->abort = 0;
-    bars->k_issued = bars->v_issued = bars->q_issued = 0;
-    mbar_fence_init();
-  }
-  if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem_base)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
 
   if (warp == kTmaWarp) {
     // ---------------------------------------------------------------- TMA
@@ -205,41 +215,48 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
     }
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
+    // The whole warp goes through the steps and one lane issues, so that what a product needs is made
+    // in uniform registers: made by one thread alone, it took longer than the product takes.
+    {
+      const uint32_t one = elect_one();
       const uint32_t id_s = idesc_bf16(kTileM, kTileN, 0), id_pv = idesc_bf16(kTileM, D, 1);
+      // descriptors differ in their address field alone, whose unit is 16 bytes
+      const uint64_t q_desc0 = desc_sw128(smem_addr(smem), 16, 1024);
+      const uint64_t k_desc0 = desc_sw128(smem_addr(smem + C::kKOff), 16, 1024);
+      const uint64_t v_desc0 = desc_sw128(smem_addr(smem + C::kVOff), C::kHalfBytes, 1024);
       int tiles = 0;             // before this segment
       int done0 = 0, done1 = 0;  // steps of each stream before it
       auto tile_of = [&](int i) { return tiles + (kPair ? i >> 1 : i); };
       auto issue_s = [&](int i) {
         const int t = i & 1, j = tile_of(i), st = j % C::kKStages;
-        if (!wait_or_abort(&bars->k_full[st], (j / C::kKStages) & 1, abort)) return false;
+        if (!wait_all(&bars->k_full[st], (j / C::kKStages) & 1, abort)) return false;
         tc_fence_after();
-        const uint32_t k_base = smem_addr(smem + C::kKOff + st * C::kTileBytes);
-        const uint32_t q_base = smem_addr(smem + (kPair ? t : 0) * C::kTileBytes);
+        const uint64_t k_desc = k_desc0 + st * (C::kTileBytes >> 4);
+        const uint64_t q_desc = q_desc0 + (kPair ? t : 0) * (C::kTileBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * C::kHalfBytes + (kk & 3) * 32;
-          mma_ss(tmem + t * 128, desc_sw128(q_base + off, 16, 1024), desc_sw128(k_base + off, 16, 1024), id_s, kk > 0);
+          mma_ss_one(one, tmem + t * 128, q_desc + (off >> 4), k_desc + (off >> 4), id_s, kk > 0);
         }
-        mma_commit(&bars->s_full[t]);
-        if (!kPair || t == 1) mma_commit(&bars->k_empty[st]);
+        mma_commit_one(one, &bars->s_full[t]);
+        if (!kPair || t == 1) mma_commit_one(one, &bars->k_empty[st]);
         return true;
       };
       auto issue_pv = [&](int i) {
         const int t = i & 1, j = tile_of(i), st = j % C::kVStages;
-        if (!wait_or_abort(&bars->v_full[st], (j / C::kVStages) & 1, abort)) return false;
+        if (!wait_all(&bars->v_full[st], (j / C::kVStages) & 1, abort)) return false;
         tc_fence_after();
-        const uint32_t v_base = smem_addr(smem + C::kVOff + st * C::kTileBytes);
+        const uint64_t v_desc = v_desc0 + st * (C::kTileBytes >> 4);
         const uint32_t p_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * 128;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma_ts(o_tmem, p_tmem + kk * 8, desc_sw128(v_base + kk * 16 * 128, C::kHalfBytes, 1024), id_pv,
+          mma_ts_one(one, o_tmem, p_tmem + kk * 8, v_desc + (kk * 16 * 128 >> 4), id_pv,
                  (i > 1 || kk > 0) ? 1u : 0u);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma_ts(o_tmem, p_tmem + 64 + kk * 8, desc_sw128(v_base + kk * 16 * 128, C::kHalfBytes, 1024), id_pv, 1u);
-        mma_commit(&bars->o_full[t]);
-        if (!kPair || t == 1) mma_commit(&bars->v_empty[st]);
+          mma_ts_one(one, o_tmem, p_tmem + 64 + kk * 8, v_desc + (kk * 16 * 128 >> 4), id_pv, 1u);
+        mma_commit_one(one, &bars->o_full[t]);
+        if (!kPair || t == 1) mma_commit_one(one, &bars->v_empty[st]);
         return true;
       };
       bool ok = true;
@@ -247,22 +264,22 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
       for (long long at = begin; ok && at < end; ++segments) {
         const Segment g = next_segment(at);
         const int steps = steps_of(g);
-        ok = wait_or_abort(&bars->q_full, segments & 1, abort) && issue_s(0) && (steps < 2 || issue_s(1));
+        ok = wait_all(&bars->q_full, segments & 1, abort) && issue_s(0) && (steps < 2 || issue_s(1));
         for (int i = 0; ok && i < steps; ++i) {
           const int t = i & 1;
-          if (!wait_or_abort(&bars->p_full[t], ((t ? done1 : done0) + (i >> 1)) & 1, abort)) {
+          if (!wait_all(&bars->p_full[t], ((t ? done1 : done0) + (i >> 1)) & 1, abort)) {
             ok = false;
             break;
           }
           tc_fence_after();
           ok = issue_pv(i) && (i + 2 >= steps || issue_s(i + 2));  // in order: P(i) is read before S(i + 2) replaces it
         }
-        mma_commit(&bars->q_empty);  // every score of the segment is there
+        mma_commit_one(one, &bars->q_empty);  // every score of the segment is there
         tiles += g.n;
         done0 += (steps + 1) / 2;
         done1 += steps / 2;
       }
-      mma_commit(&bars->drain);
+      mma_commit_one(one, &bars->drain);
       (void)mbar_wait_bounded(&bars->drain, 0);
     }
   } else if (warp < kSoftmaxWarps) {
@@ -422,7 +439,6 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
     }
   }
 
-  tc_fence_before();
   __syncthreads();
   if (*abort) {
     if (threadIdx.x == 0) atomicOr(a.status, kDevWaitTimeout);
@@ -434,16 +450,11 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
         (void)mbar_wait_bounded(&bars->v_full[j % C::kVStages], (j / C::kVStages) & 1);
     }
   }
-  __syncthreads();
-  if (warp == kMmaWarp) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-  }
 }
 
 // What the passes cost, in nanoseconds of one SM: a tile of 128 tokens for a pair of row tiles or
 // for one, and what a CTA spends beside its tiles; 16 own tokens.  (head_dim 64: half as much.)
-constexpr int kPairTileNs = 2600, kTileNs = 1600, kPassNs = 8000, kOwnTileNs = 130, kUnitNs = 3000,
+constexpr int kPairTileNs = 2600, kTileNs = 1600, kPassNs = 8000, kOwnTileNs = 130, kUnitNs = 6000,
               kSoloUnitNs = 500;
 
 template <int D, int NG, bool kPair>
@@ -457,10 +468,41 @@ __global__ void __launch_bounds__(kThreads, 1)
   using Own = OwnOf<D, NG, kPair>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ typename Own::Shared shared;
+  __shared__ Bars bars;
+  // what the prefix needs is set up while the kernel before this one ends
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, 1);
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&bars.k_full[s], 1);
+      mbar_init(&bars.k_empty[s], 1);
+      mbar_init(&bars.v_full[s], 1);
+      mbar_init(&bars.v_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars.s_full[t], 1);
+      mbar_init(&bars.p_full[t], kSoftmaxWarps * 32);
+      mbar_init(&bars.o_full[t], 1);
+    }
+    mbar_init(&bars.drain, 1);
+    bars.abort = 0;
+    bars.k_issued = bars.v_issued = bars.q_issued = 0;
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars.tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
   grid_dependency_wait();
   Own own(a, shared);
   own.totals();
   const bool covered = __syncthreads_or(own.covering);  // by the prefix: some sequence is as long
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem_base;
   // CTAs for the own tokens: as many as make both passes end together
   const long long own_ns =
       own.total * (kOwnTileNs * D / 128) + own.units * (own.solo_units(gridDim.x / 4) ? kSoloUnitNs : kUnitNs);
@@ -469,13 +511,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                                       : 0;
   int ctas = (int)gridDim.x;
   if (prefix_ns > 0)
-    ctas = own_ns == 0 ? 0 : max(1, min(ctas - 1, (int)((double)own_ns / (double)(own_ns + prefix_ns) * ctas + 0.5)));
+    ctas = own_ns == 0 ? 0 : max(1, min(ctas - 1, (int)((float)own_ns / (float)(own_ns + prefix_ns) * ctas + 0.5f)));
   if ((int)blockIdx.x < ctas) {
     own.run(blockIdx.x, ctas, smem_raw + (-smem_addr(smem_raw) & 127));
   } else {
-    prefix_pass<D, kPair>(tm_q, tm_k, tm_v, a, p, blockIdx.x - ctas, gridDim.x - ctas, smem_raw);
+    prefix_pass<D, kPair>(tm_q, tm_k, tm_v, a, p, blockIdx.x - ctas, gridDim.x - ctas, smem_raw, &bars, tmem);
   }
   allow_dependent_launch();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
 }
 
 template <int D, int NG, bool kPair>
