@@ -454,7 +454,7 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
 
 // What the passes cost, in nanoseconds of one SM: a tile of 128 tokens for a pair of row tiles or
 // for one, and what a CTA spends beside its tiles; 16 own tokens.  (head_dim 64: half as much.)
-constexpr int kPairTileNs = 2600, kTileNs = 1600, kPassNs = 8000, kOwnTileNs = 130, kUnitNs = 6000,
+constexpr int kPairTileNs = 2800, kTileNs = 1600, kPassNs = 8000, kOwnTileNs = 100, kUnitNs = 6000,
               kSoloUnitNs = 500;
 
 template <int D, int NG, bool kPair>
