@@ -435,11 +435,11 @@ LARA_API int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool, c
 /* ------------------------------------------------------------------------ */
 
 /* lara_gqa_decode_paged for a batch whose sequences begin with the same pages:
- * the first shared_pages entries of every row of block_table name the same
- * pages, which are read once for all sequences that are at least that long
- * (from row 0's entries), instead of once for each.  A sequence that ends
- * within them is read through its own row, whatever that holds.  A sequence
- * of length 0 gives zeros.  o may be q. */
+ * the first shared_pages entries of the rows of block_table name the same
+ * pages for all sequences that are at least that long, and are read once for
+ * them instead of once for each.  A sequence that ends within them is read
+ * through its own row, whatever that holds.  A sequence of length 0 gives
+ * zeros.  o may be q. */
 LARA_API size_t lara_decode_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim);
 LARA_API int lara_gqa_decode_shared(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
                                     const int32_t* block_table, const int32_t* seq_lens, uint16_t* o, int batch,

@@ -154,7 +154,7 @@ struct OwnTokens {
   const DecodeArgs& a;
   Shared& sh_;
   long long total = 0, units = 0;  // tiles, and units with tokens
-  int covering = 0;  // of the thread's sequences, those behind the shared prefix
+  int covering = 0x7fffffff;  // the first of the thread's sequences that covers the shared prefix
 
   __device__ __forceinline__ OwnTokens(const DecodeArgs& args, Shared& shared) : a(args), sh_(shared) {}
 
@@ -198,7 +198,7 @@ struct OwnTokens {
       const Own own = own_tokens(a, len);
       mine += tiles_of(own.len) + (own.len > 0 ? 1ll << 40 : 0);
       groups += groups_of(tiles_of(own.len));
-      covering += own.start > 0;
+      if (own.start > 0) covering = min(covering, b);
     }
     long long all;
     const long long ahead = prefix(mine, sh_.sum[0], all);

@@ -128,7 +128,7 @@ struct Segment {
 
 template <int D, bool kPair>
 __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
-                                            const DecodeArgs& a, const PrefixArgs& p, int me, int ctas,
+                                            const DecodeArgs& a, const PrefixArgs& p, int seq, int me, int ctas,
                                             uint8_t* smem_raw, Bars* bars, uint32_t tmem) {
   using C = Prefix<D, kPair>;
   uint8_t* const smem = smem_raw + (-smem_addr(smem_raw) & 1023);
@@ -154,12 +154,13 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
   if (warp == kTmaWarp) {
     // ---------------------------------------------------------------- TMA
     const int log2 = a.index.page_log2, piece = min(kTileN, 1 << log2), pieces = kTileN / piece;
+    const int32_t* const table = a.index.block_table + (long long)seq * a.index.pages_per_seq;
     // lane i copies piece i of every tile; its page is looked up a tile ahead.  Behind the
     // prefix's end a page that is not there: the copy writes zeros
     auto page_of = [&](int j) {
       const int tok = j * kTileN + lane * piece;
       if (lane >= pieces || tok >= a.shared_tokens) return a.index.num_pages;
-      int pg = __ldg(a.index.block_table + (tok >> log2));
+      int pg = __ldg(table + (tok >> log2));
       if ((unsigned)pg >= (unsigned)a.index.num_pages) {
         atomicOr(a.status, kDevBadPage);
         pg = 0;
@@ -469,6 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ typename Own::Shared shared;
   __shared__ Bars bars;
+  __shared__ int covering;  // the first sequence that is as long as the prefix
   // what the prefix needs is set up while the kernel before this one ends
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
@@ -488,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.drain, 1);
     bars.abort = 0;
     bars.k_issued = bars.v_issued = bars.q_issued = 0;
+    covering = 0x7fffffff;
     mbar_fence_init();
   }
   if (warp == kMmaWarp) {
@@ -500,22 +503,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_dependency_wait();
   Own own(a, shared);
   own.totals();
-  const bool covered = __syncthreads_or(own.covering);  // by the prefix: some sequence is as long
+  if (own.covering != 0x7fffffff) atomicMin(&covering, own.covering);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
   // CTAs for the own tokens: as many as make both passes end together
   const long long own_ns =
       own.total * (kOwnTileNs * D / 128) + own.units * (own.solo_units(gridDim.x / 4) ? kSoloUnitNs : kUnitNs);
-  const long long prefix_ns = covered ? (long long)p.units * p.tiles * ((kPair ? kPairTileNs : kTileNs) * D / 128) +
+  const long long prefix_ns = covering < a.batch ? (long long)p.units * p.tiles * ((kPair ? kPairTileNs : kTileNs) * D / 128) +
                                             kPassNs * min((long long)p.units * p.tiles, (long long)gridDim.x)
                                       : 0;
   int ctas = (int)gridDim.x;
-  if (prefix_ns > 0)
-    ctas = own_ns == 0 ? 0 : max(1, min(ctas - 1, (int)((float)own_ns / (float)(own_ns + prefix_ns) * ctas + 0.5f)));
+  if (prefix_ns > 0) {
+    // at least as many as keep a share below 2^30 tiles
+    const int least = own_ns == 0 ? 0 : 1 + (int)((own.total + own.units * kUnitCost) >> 30);
+    ctas = max(least, min(ctas - 1, (int)((float)own_ns / (float)(own_ns + prefix_ns) * ctas + 0.5f)));
+  }
   if ((int)blockIdx.x < ctas) {
     own.run(blockIdx.x, ctas, smem_raw + (-smem_addr(smem_raw) & 127));
   } else {
-    prefix_pass<D, kPair>(tm_q, tm_k, tm_v, a, p, blockIdx.x - ctas, gridDim.x - ctas, smem_raw, &bars, tmem);
+    prefix_pass<D, kPair>(tm_q, tm_k, tm_v, a, p, covering, blockIdx.x - ctas, gridDim.x - ctas, smem_raw,
+                          &bars, tmem);
   }
   allow_dependent_launch();
   tc_fence_before();

@@ -59,8 +59,8 @@ def gqa_decode_shared(q, k_pages, v_pages, block_table, seq_lens, shared_pages: 
     """One new token per sequence, of a batch whose sequences begin with the same pages (``lara_gqa_decode_shared``).
 
     q ``[B, Hq, D]`` (bf16) attends the first ``seq_lens[b]`` tokens that ``block_table[b]`` names in ``k_pages`` and
-    ``v_pages`` ``[num_pages, Hkv, page_size, D]``.  The first ``shared_pages`` columns of the table are the same in
-    every row: they are read once for all sequences that are at least as long (a shorter sequence is read by itself).
+    ``v_pages`` ``[num_pages, Hkv, page_size, D]``.  The first ``shared_pages`` columns of the table are the same for
+    all sequences that are at least as long, and read once for them (a shorter sequence is read by itself).
     ``Hq`` is any multiple of ``Hkv`` up to 16 per kv head, ``D`` 64 or 128.  A sequence of length 0 gives zeros.
     ``workspace`` comes from :func:`shared_workspace` (``None`` allocates one for the call).  Returns ``o[B, Hq, D]``
     (``out``, which may be q).
@@ -140,7 +140,7 @@ class PagedKVCache:
     """Page pool, block tables and lengths of many sequences.
 
     ``scored=True`` also keeps a weight for every slot and kv head (``weights``, float32), the attention it has got from
-    :meth:`decode_scored` since its token was appended, by which :meth:`evict` chooses.
+    :meth:`decode_scored` since its token was appended, by which :meth:`evict` chooses.  (Files hold no weights.)
     """
 
     def __init__(self, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, max_seqs: int,
@@ -319,11 +319,10 @@ class PagedKVCache:
 
     def _own_pages(self, slots, what: str) -> None:
         """Refuse slots whose pages another sequence has too."""
-        for slot in slots:
-            pages = self._table[slot]
-            if np.any(self._refs[pages[pages >= 0]] > 1):
-                raise ValueError(f"{what}: sequence {int(slot)} has pages in common with another")
-        if len(set(slots.tolist())) != len(slots):
+        pages = self._table[slots]
+        if np.any(self._refs[pages[pages >= 0]] > 1):
+            raise ValueError(f"{what}: a sequence has pages in common with another")
+        if len(np.unique(slots)) != len(slots):
             raise ValueError(f"{what}: a slot is named twice")
 
     def _need_weights(self, what: str) -> None:
@@ -338,6 +337,8 @@ class PagedKVCache:
 
     def decode_shared(self, q, slots=None, scale=None):
         """:meth:`decode`, reading the pages that all slots begin with (:meth:`share_prefix`) once for the batch."""
+        if not hasattr(self, "k_pages"):
+            raise ValueError("decode_shared needs a cache of bf16 rows")
         slots = self._slots(slots)
         _check_words("q", q, (len(slots), q.shape[1], self.head_dim))
         _, table, lens = self._rows_of(slots)
@@ -363,19 +364,20 @@ class PagedKVCache:
         self._need_weights("evict")
         slots = self._slots(slots)
         self._own_pages(slots, "evict")
-        idx, table, lens = self._rows_of(slots)
+        _, table, lens = self._rows_of(slots)
         ws = self._serving("evict", int(lib.lara_kv_evict_workspace_bytes(len(slots), self.n_kv_heads,
                                                                           max(int(keep), 1))))
-        new_lens = kv_evict(self.k_pages, self.v_pages, self.weights, table, lens, keep, first=first, last=last,
-                            sources=sources, workspace=ws)
-        self.lens.index_copy_(0, idx, new_lens)
-        self._lens[slots] = np.minimum(self._lens[slots], keep)
-        for slot in slots:
+        kv_evict(self.k_pages, self.v_pages, self.weights, table, lens, keep, first=first, last=last,
+                 sources=sources, workspace=ws)
+        cut = slots[self._lens[slots] > keep]
+        self._lens[cut] = keep
+        for slot in cut:
             for j in range(-(-int(self._lens[slot]) // self.page_size), self.pages_per_seq):
                 if self._table[slot, j] >= 0:
                     self._release(int(self._table[slot, j]))
                     self._table[slot, j] = -1
-        self._sync_rows(slots)
+        if len(cut):
+            self._sync_rows(cut)
 
     def status(self) -> int:
         """Device status bits of the last appends, decodes and evictions (read and cleared)."""

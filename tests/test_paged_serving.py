@@ -322,3 +322,254 @@ def test_serving_loop():
             assert [cache.seq_len(s) for s in (0, 1)] == [have[0], have[1]]
             assert cache.free_pages == 24 - sum(-(-n // page) for n in have.values())
     assert cache.status() == 0
+
+
+# ------------------------------------------------------------------ what else a call may meet
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (10, 2, 64)])
+def test_shared_decode_of_a_padded_batch(hq, hkv, d):
+    """Rows that do not cover the prefix need not name it: padding without pages, a short sequence with its own."""
+    from lara_b200 import ops, paged
+
+    page, shared, lens = 32, 3, [0, 40, 96, 200, 0, 97]
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=2, shared=shared, spare=1)
+    own = torch.tensor([[x for x in range(k.shape[0]) if x not in set(table.flatten().tolist())]])  # two, of no sequence
+    g = torch.Generator().manual_seed(8)
+    for x in (k, v):
+        x[own[0]] = torch.randn(x[own[0]].shape, generator=g).bfloat16()
+        x[own[0, 1], :, 8:] = math.nan
+    table[0], table[4], table[1] = -1, 1 << 30, -7
+    table[1, :2] = own[0].int()
+    q = torch.randn((len(lens), hq, d), generator=g).bfloat16()
+    o, kappa, A, _ = decode64(q, k, v, table, n, page, d ** -0.5)
+    qd, kd, vd, td, nd = dev(q, k, v, table, n)
+    ws = paged.shared_workspace(len(lens), hq, hkv, d, "cuda")
+    check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, shared, workspace=ws), o, kappa, A, n)
+    assert ops.workspace_status(ws) == 0
+    # no sequence covers it: nothing of it is read
+    table[:, 2:] = -1
+    n = torch.minimum(n, torch.tensor(64, dtype=torch.int32))
+    o, kappa, A, _ = decode64(q, k, v, table, n, page, d ** -0.5)
+    check_out(paged.gqa_decode_shared(qd, kd, vd, table.cuda(), n.cuda(), shared, workspace=ws), o, kappa, A, n)
+    assert ops.workspace_status(ws) == 0
+
+
+@pytest.mark.gpu
+def test_lengths_and_pages_out_of_range():
+    """Lengths are clamped and bad pages not written; both are flagged."""
+    from lara_b200 import ops, paged
+
+    hq, hkv, d, page = 8, 2, 64, 16
+    k, v, table, n = make_cache([40, 64, 20], hkv, d, page, seed=4)
+    k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    w = torch.rand(k.shape[:3])
+    q = torch.randn((3, hq, d)).bfloat16()
+    table[0, 1] = k.shape[0]
+    raw = torch.tensor([40, 70, -3], dtype=torch.int32)  # past the capacity of 64, below 0
+    qd, kd, vd, wd, td, nd = dev(q, k, v, w, table, raw)
+    want = torch.tensor([40, 64, 0], dtype=torch.int32)
+    seen = table.clone()
+    seen[0, 1] = 0  # page 0 is read in its place
+    o, kappa, A, _ = decode64(q, k, v, seen, want, page, 0.125)
+    ws = paged.scored_workspace(3, hq, kd, table.shape[1])
+    check_out(paged.gqa_decode_scored(qd, kd, vd, wd, td, nd, scale=0.125, workspace=ws), o, kappa, A, want)
+    assert ops.workspace_status(ws) == 2 + 8 and ops.workspace_status(ws) == 0
+    ws = paged.shared_workspace(3, hq, hkv, d, "cuda")
+    check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, 0, scale=0.125, workspace=ws), o, kappa, A, want)
+    assert ops.workspace_status(ws) == 2 + 8
+    wd.copy_(w)
+    ws = paged.evict_workspace(3, hkv, 10, "cuda")
+    new = paged.kv_evict(kd, vd, wd, td, nd, 10, workspace=ws)
+    assert new.tolist() == [10, 10, 0]
+    assert ops.workspace_status(ws) == 2 + 8
+    used = set(table[0, [0, 2]].tolist()) | set(table[1].tolist())
+    others = [p for p in range(k.shape[0]) if p not in used]
+    assert torch.equal(words(kd)[others], words(k)[others]) and torch.equal(wd.cpu()[others], w[others])
+
+
+@pytest.mark.gpu
+def test_infinities_and_nan():
+    """A NaN or an infinity in a visible row shows where the definition shows it, and in no other sequence or head."""
+    from lara_b200 import paged
+
+    hq, hkv, d, page = 4, 2, 64, 16
+    k, v, table, n = make_cache([300, 300, 300, 300], hkv, d, page, seed=6, shared=2)
+    q = torch.randn((4, hq, d), generator=torch.Generator().manual_seed(1)).bfloat16()
+    at = lambda b, t: (int(table[b, t // page]), 0, t % page)  # noqa: E731
+    v[at(0, 299)][5] = math.nan
+    v[at(1, 130)][7] = math.inf
+    k[at(2, 77)][3] = math.nan
+    w = torch.zeros(k.shape[:3])
+    for scored in (True, False):
+        qd, kd, vd, wd, td, nd = dev(q, k, v, w, table, n)
+        if scored:
+            got = paged.gqa_decode_scored(qd, kd, vd, wd, td, nd)  # shared pages: their weights are not looked at
+        else:
+            got = paged.gqa_decode_shared(qd, kd, vd, td, nd, 2)
+        bad = ~torch.isfinite(got.float().cpu())
+        want = torch.zeros_like(bad)
+        want[0, :2, 5] = want[1, :2, 7] = True
+        want[2, :2] = True
+        assert torch.equal(bad, want)
+    v[at(3, 3)] = math.nan  # in the shared part: in every sequence's first kv head
+    got = paged.gqa_decode_shared(qd, k.cuda(), v.cuda(), td, nd, 2).float().cpu()
+    assert torch.isnan(got[:, :2]).all() and torch.isfinite(got[[0, 1, 2, 3], 2:]).all()
+
+
+@pytest.mark.gpu
+def test_graphs_streams_and_views():
+    """Calls captured in two graphs with a workspace each, replayed in turn; another stream; 16-bit views."""
+    from lara_b200 import paged
+
+    hq, hkv, d, page = 16, 2, 128, 64
+    k, v, table, n = make_cache([700, 513, 90], hkv, d, page, seed=12, shared=1)
+    q = torch.randn((2, 3, hq, d), generator=torch.Generator().manual_seed(2)).bfloat16()
+    w = torch.rand(k.shape[:3], generator=torch.Generator().manual_seed(3))
+    qd, kd, vd, wd, td, nd = dev(q, k, v, w, table, n)
+    k2, v2, t2, n2 = dev(*make_cache([700, 513, 90], hkv, d, page, seed=12))
+    w2 = torch.rand(k2.shape[:3], device="cuda")
+    runs = []
+    for i in range(2):
+        ws = (paged.shared_workspace(3, hq, hkv, d, "cuda"), paged.scored_workspace(3, hq, k2, t2.shape[1]),
+              paged.evict_workspace(3, hkv, 300, "cuda"))
+        keep = [x.clone() for x in (k2, v2, w2)]
+        out = [torch.empty_like(qd[i]) for _ in range(2)]
+        w_out, src, new = torch.empty_like(w2), torch.empty((3, hkv, 300), dtype=torch.int32, device="cuda"), n2.clone()
+        w_out.copy_(w2)
+
+        def call(i=i, ws=ws, keep=keep, out=out, w_out=w_out, src=src, new=new):
+            paged.gqa_decode_shared(qd[i], kd, vd, td, nd, 1, workspace=ws[0], out=out[0])
+            paged.gqa_decode_scored(qd[i], keep[0], keep[1], keep[2], t2, n2, weights_out=w_out, workspace=ws[1],
+                                    out=out[1])
+            paged.kv_evict(keep[0], keep[1], w_out, t2, n2, 300, first=1, last=9, new_lens=new, sources=src,
+                           workspace=ws[2])
+
+        runs.append((call, keep, out, w_out, src, new))
+    want = []
+    for call, keep, out, w_out, src, new in runs:
+        call()
+        torch.cuda.synchronize()
+        want.append([x.clone() for x in (*keep, *out, w_out, src, new)])
+    graphs = []
+    for call, keep, *_ in runs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        graphs.append(g)
+
+    def reset():
+        for _, keep, out, w_out, src, new in runs:
+            for x, y in zip(keep, (k2, v2, w2)):
+                x.copy_(y)
+            w_out.copy_(w2)
+            for x in (*out, src, new):
+                x.zero_()
+
+    def check():
+        torch.cuda.synchronize()
+        for (_, keep, out, w_out, src, new), ref in zip(runs, want):
+            for x, y in zip((*keep, *out, w_out, src, new), ref):
+                assert torch.equal(words(x), words(y))
+
+    for order in ((0, 1), (1, 0)):
+        reset()
+        for i in order:
+            graphs[i].replay()
+        check()
+    reset()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for s, g in zip(streams, graphs):  # at the same time
+        with torch.cuda.stream(s):
+            g.replay()
+    check()
+    reset()
+    torch.cuda.synchronize()
+    for s, (call, *_) in zip(streams, runs):
+        with torch.cuda.stream(s):
+            call()
+    check()
+    view = paged.gqa_decode_shared(qd[0].view(torch.int16), kd.view(torch.int16), vd.view(torch.int16), td, nd, 1)
+    assert torch.equal(view.cpu(), words(runs[0][2][0]))
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bit_offsets():
+    """Pages whose elements lie past 2^32 in the pool."""
+    from lara_b200 import paged
+
+    hq, hkv, d, page = 8, 4, 128, 256
+    num = (1 << 32) // (hkv * page * d) + 40  # 2^32 elements and some pages
+    lens = [900, 300, 513]
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=21)
+    used = k.shape[0]
+    big = [torch.empty((num, hkv, page, d), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    w = torch.rand(k.shape[:3], generator=torch.Generator().manual_seed(3))
+    w_big = torch.zeros((num, hkv, page), device="cuda")
+    for x, y in zip((*big, w_big), (k, v, w)):
+        x[num - used:] = y.cuda()
+    there = torch.where(table >= 0, table + (num - used), table)
+    q = torch.randn((3, hq, d), generator=torch.Generator().manual_seed(5)).bfloat16()
+    o, kappa, A, ps = decode64(q, k, v, table, n, page, d ** -0.5)
+    td, nd, qd = dev(there, n, q)
+    check_out(paged.gqa_decode_shared(qd, *big, td, nd, 0), o, kappa, A, n)
+    check_out(paged.gqa_decode_scored(qd, *big, w_big, td, nd), o, kappa, A, n)
+    check_weights(w_big[num - used:], w, ps, A, table, n, page, d)
+    w = w_big[num - used:].cpu()
+    want = evict64(k, v, w, table, n, page, 200, 4, 30)
+    paged.kv_evict(*big, w_big, td, nd, 200, first=4, last=30)
+    for x, y in zip((*big, w_big), want):
+        assert torch.equal(words(x[num - used:]), words(y))
+    k, v, table, n = make_cache([900, 800], hkv, d, page, seed=22, shared=3)
+    used = k.shape[0]
+    for x, y in zip(big, (k, v)):
+        x[num - used:] = y.cuda()
+    there = torch.where(table >= 0, table + (num - used), table)
+    o, kappa, A, _ = decode64(q[:2], k, v, table, n, page, d ** -0.5)
+    check_out(paged.gqa_decode_shared(qd[:2].contiguous(), *big, there.cuda(), n.cuda(), 3), o, kappa, A, n)
+
+
+@pytest.mark.gpu
+def test_scored_decode_names_more_pages_than_there_are():
+    """Sequences that share pages: the output is right, weights past the room are left and flagged."""
+    from lara_b200 import ops, paged
+
+    hq, hkv, d, page = 4, 1, 64, 16
+    k, v, table, n = make_cache([320], hkv, d, page, seed=30)
+    table, n = table.repeat(40, 1), n.repeat(40)
+    q = torch.randn((40, hq, d), generator=torch.Generator().manual_seed(1)).bfloat16()
+    o, kappa, A, _ = decode64(q, k, v, table, n, page, 0.125)
+    qd, kd, vd, td, nd = dev(q, k, v, table, n)
+    ws = paged.scored_workspace(40, hq, kd, table.shape[1])
+    wd = torch.zeros(k.shape[:3], device="cuda")
+    check_out(paged.gqa_decode_scored(qd, kd, vd, wd, td, nd, scale=0.125, workspace=ws), o, kappa, A, n)
+    assert ops.workspace_status(ws) == 32
+
+
+@pytest.mark.gpu
+def test_many_sequences():
+    """More sequences than cached lengths and than threads that count them, most of them short or empty."""
+    from lara_b200 import paged
+
+    hq, hkv, d, page = 4, 2, 64, 16
+    g = torch.Generator().manual_seed(17)
+    lens = torch.randint(0, 40, (2500,), generator=g).tolist()
+    lens[1700] = 2000
+    lens[:300] = [0] * 300
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=3)
+    q = torch.randn((len(lens), hq, d), generator=g).bfloat16()
+    w = torch.rand(k.shape[:3], generator=g)
+    o, kappa, A, ps = decode64(q, k, v, table, n, page, 0.125)
+    qd, kd, vd, wd, td, nd = dev(q, k, v, w, table, n)
+    check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, 0, scale=0.125), o, kappa, A, n)
+    check_out(paged.gqa_decode_scored(qd, kd, vd, wd, td, nd, scale=0.125), o, kappa, A, n)
+    check_weights(wd, w, ps, A, table, n, page, d)
+    w = wd.cpu()
+    want = evict64(k, v, w, table, n, page, 20, 2, 3)
+    paged.kv_evict(kd, vd, wd, td, nd, 20, first=2, last=3)
+    for x, y in zip((kd, vd, wd), want):
+        assert torch.equal(words(x), words(y))
+    k, v, table, n = make_cache([64 + x for x in lens], hkv, d, page, seed=5, shared=4)
+    o, kappa, A, _ = decode64(q, k, v, table, n, page, 0.125)
+    qd, kd, vd, td, nd = dev(q, k, v, table, n)
+    check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, 4, scale=0.125), o, kappa, A, n)
