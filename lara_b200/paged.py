@@ -68,8 +68,8 @@ def gqa_decode_shared(q, k_pages, v_pages, block_table, seq_lens, shared_pages: 
     if out is None:
         out = torch.empty_like(q)
     if workspace is None:
-        workspace = shared_workspace(max(q.shape[0], 1), q.shape[1], k_pages.shape[1], q.shape[2], k_pages.device)
-    sc = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+        workspace = shared_workspace(max(q.shape[0], 1), q.shape[1], k_pages.shape[1], k_pages.shape[3], k_pages.device)
+    sc = q.shape[-1] ** -0.5 if scale is None else scale
     rc = _binding.decode_shared(q, k_pages, v_pages, block_table, seq_lens, shared_pages, out, sc, workspace)
     if rc:
         check(rc, "lara_gqa_decode_shared")
@@ -100,7 +100,7 @@ def gqa_decode_scored(q, k_pages, v_pages, weights, block_table, seq_lens, *, we
         out = torch.empty_like(q)
     if workspace is None:
         workspace = scored_workspace(max(q.shape[0], 1), q.shape[1], k_pages, block_table.shape[1])
-    sc = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+    sc = q.shape[-1] ** -0.5 if scale is None else scale
     rc = _binding.decode_scored(q, k_pages, v_pages, weights, weights if weights_out is None else weights_out,
                                 block_table, seq_lens, out, sc, workspace)
     if rc:

@@ -573,3 +573,169 @@ def test_many_sequences():
     o, kappa, A, _ = decode64(q, k, v, table, n, page, 0.125)
     qd, kd, vd, td, nd = dev(q, k, v, table, n)
     check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, 4, scale=0.125), o, kappa, A, n)
+
+
+# ------------------------------------------------------------------ refusals
+BAD_CFG, DEST, RESULT, UNSUPPORTED = 0x01, 0x11, 0x12, 0x22
+P = 1 << 20  # an address that is aligned and never used: every call here is refused on the host
+
+
+def c_call(name, **change):
+    """A valid call's arguments with some replaced; the status code."""
+    from lara_b200._native import lib
+
+    pool = dict(n_kv_heads=2, head_dim=64, page_size=16, pages_per_seq=4, num_pages=9)
+    if name == "evict":
+        a = dict(k=P, v=P, w=P, w_out=P, table=P, lens=P, new_lens=2 * P, sources=0, batch=3, **pool, keep=8, first=1,
+                 last=2, ws=P, nbytes=1 << 40, stream=0)
+        fn = lib.lara_kv_evict
+    elif name == "scored":
+        a = dict(q=P, k=P, v=P, w=P, w_out=P, table=P, lens=P, o=P, batch=3, n_q_heads=8, **pool, scale=0.5, ws=P,
+                 nbytes=1 << 40, stream=0)
+        fn = lib.lara_gqa_decode_scored
+    else:
+        a = dict(q=P, k=P, v=P, table=P, lens=P, o=P, batch=3, n_q_heads=8, **pool, shared=1, scale=0.5, ws=P,
+                 nbytes=1 << 40, stream=0)
+        fn = lib.lara_gqa_decode_shared
+    assert set(change) <= set(a)
+    a.update(change)
+    return fn(*a.values())
+
+
+EVERY = [(dict(head_dim=96), UNSUPPORTED), (dict(page_size=8), BAD_CFG), (dict(page_size=48), BAD_CFG),
+         (dict(batch=-1), BAD_CFG), (dict(batch=65536), BAD_CFG), (dict(n_kv_heads=0), BAD_CFG),
+         (dict(num_pages=0), BAD_CFG), (dict(pages_per_seq=0), BAD_CFG), (dict(pages_per_seq=1 << 26), BAD_CFG),
+         (dict(batch=65535, n_kv_heads=8, pages_per_seq=1 << 25, n_q_heads=8), BAD_CFG),
+         (dict(k=0), DEST), (dict(v=0), DEST), (dict(table=0), DEST), (dict(lens=0), DEST), (dict(ws=0), DEST),
+         (dict(k=P + 8), DEST), (dict(v=P + 2), DEST), (dict(table=P + 2), DEST), (dict(lens=P + 1), DEST),
+         (dict(ws=P + 16), DEST), (dict(nbytes=256), RESULT), (dict(nbytes=0), RESULT)]
+DECODE = [(dict(n_q_heads=0), BAD_CFG), (dict(n_q_heads=7), BAD_CFG), (dict(n_q_heads=34), UNSUPPORTED),
+          (dict(scale=0.0), BAD_CFG), (dict(scale=-1.0), BAD_CFG), (dict(scale=math.nan), BAD_CFG),
+          (dict(scale=math.inf), BAD_CFG), (dict(q=0), DEST), (dict(o=0), DEST), (dict(q=P + 8), DEST),
+          (dict(o=P + 4), DEST)]
+WEIGHTS = [(dict(w=0), DEST), (dict(w_out=0), DEST), (dict(w=P + 4), DEST), (dict(w_out=P + 8), DEST),
+           (dict(w_out=P + 64), DEST)]
+
+
+@pytest.mark.parametrize("name", ["shared", "scored", "evict"])
+def test_refused_on_the_host(name):
+    own = {"shared": DECODE + [(dict(shared=-1), BAD_CFG), (dict(shared=5), BAD_CFG)], "scored": DECODE + WEIGHTS,
+           "evict": WEIGHTS + [(dict(keep=0), BAD_CFG), (dict(first=-1), BAD_CFG), (dict(last=-1), BAD_CFG),
+                               (dict(first=6, last=3), BAD_CFG), (dict(first=9), BAD_CFG),
+                               (dict(first=0x7fffffff, last=0x7fffffff), BAD_CFG), (dict(new_lens=P), DEST),
+                               (dict(new_lens=P + 8), DEST), (dict(sources=P + 2), DEST),
+                               (dict(pages_per_seq=(1 << 20) + 1), UNSUPPORTED),
+                               (dict(num_pages=1 << 30, n_kv_heads=4), BAD_CFG)]}[name]
+    for change, code in EVERY + own:
+        if name == "evict":
+            change = {x: y for x, y in change.items() if x != "n_q_heads"}
+        assert c_call(name, **change) == code, change
+    assert c_call(name, batch=0, k=0, v=0, table=0, ws=0) == 0  # nothing to do
+
+
+def test_workspaces_serve_smaller_calls():
+    from lara_b200._native import lib
+
+    for d in (64, 128):
+        for hkv in (1, 2, 8):
+            for group in (1, 5, 8, 16):
+                sizes = [lib.lara_decode_shared_workspace_bytes(b, hkv * group, hkv, d) for b in range(1, 300, 7)]
+                assert sizes == sorted(sizes) and sizes[0] > 0
+                assert lib.lara_decode_shared_workspace_bytes(64, hkv, hkv, d) <= \
+                    lib.lara_decode_shared_workspace_bytes(64, hkv * group, hkv, d)
+                sizes = [lib.lara_decode_scored_workspace_bytes(b, hkv * group, hkv, d, 16, 100, 900)
+                         for b in range(1, 300, 7)]
+                assert sizes == sorted(sizes) and sizes[0] > 0
+    assert lib.lara_kv_evict_workspace_bytes(2, 8, 100) < lib.lara_kv_evict_workspace_bytes(3, 8, 101)
+    for bad in ((0, 8, 2, 64), (3, 0, 2, 64), (3, 8, 0, 64)):
+        assert lib.lara_decode_shared_workspace_bytes(*bad) == 0
+    assert lib.lara_kv_evict_workspace_bytes(3, 2, 0) == 0
+
+
+def test_refused_by_the_binding():
+    """What the Python binding refuses before any address is used (CPU tensors stand for the wrong device)."""
+    from lara_b200 import paged
+
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    q, w = torch.zeros((1, 8, 64), dtype=torch.bfloat16), torch.zeros((4, 2, 16))
+    table, n, ws = torch.zeros((1, 4), dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(4096)
+    with pytest.raises(TypeError, match="k_pages must hold bf16"):
+        paged.gqa_decode_shared(q, k.float(), k, table, n, 1, workspace=ws)
+    with pytest.raises(ValueError, match="k_pages must be on the CUDA device"):
+        paged.gqa_decode_shared(q, k, k, table, n, 1, workspace=ws)
+    with pytest.raises(ValueError, match="num_pages, Hkv, page_size, D"):
+        paged.gqa_decode_scored(q, k[0], k, w, table, n, workspace=ws)
+    with pytest.raises(ValueError, match="k_pages must be on the CUDA device"):
+        paged.kv_evict(k, k, w, table, n, 3, workspace=ws)
+    with pytest.raises(TypeError, match="must be a tensor"):
+        paged.kv_evict(None, k, w, table, n, 3, workspace=ws)
+
+
+@pytest.mark.gpu
+def test_refused_tensors():
+    from lara_b200 import paged
+    from lara_b200._native import LaraConfigError
+    from lara_b200.kvquant import QuantKVCache
+
+    k, v, table, n = dev(*make_cache([40, 20], 2, 64, 16, seed=1))
+    q = torch.zeros((2, 8, 64), dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(k.shape[:3], device="cuda")
+    ws = paged.shared_workspace(2, 8, 2, 64, "cuda")
+    ok = dict(q=q, k=k, v=v, table=table, n=n, shared=0)
+
+    def shared(**change):
+        a = {**ok, **change}
+        return paged.gqa_decode_shared(a["q"], a["k"], a["v"], a["table"], a["n"], a["shared"],
+                                       scale=a.get("scale"), workspace=a.get("ws", ws), out=a.get("out"))
+
+    for error, change in [(ValueError, dict(q=q[:, :, :32])), (ValueError, dict(q=q[0])), (TypeError, dict(q=q.float())),
+                          (ValueError, dict(q=q.cpu())), (ValueError, dict(q=q.transpose(0, 1).contiguous().transpose(0, 1))),
+                          (ValueError, dict(v=v[:1])), (ValueError, dict(k=k[:, :, ::2], v=v[:, :, ::2])),
+                          (ValueError, dict(table=table.long())), (ValueError, dict(table=table[:1])),
+                          (ValueError, dict(table=table.t().contiguous().t())), (ValueError, dict(n=n.long())),
+                          (ValueError, dict(n=n[:1])), (ValueError, dict(shared=-1)), (ValueError, dict(shared=99)),
+                          (TypeError, dict(shared=1.5)), (ValueError, dict(scale=0.0)), (TypeError, dict(scale="x")),
+                          (ValueError, dict(out=q[:1])), (ValueError, dict(ws=ws[:256])), (ValueError, dict(ws=ws.cpu())),
+                          (ValueError, dict(out=q[:, :1].expand(2, 8, 64)))]:
+        with pytest.raises(error):
+            shared(**change)
+    with pytest.raises(ValueError):
+        paged.gqa_decode_scored(q, k, v, w[:1], table, n)
+    with pytest.raises(TypeError):
+        paged.gqa_decode_scored(q, k, v, w.half(), table, n)
+    for change in (dict(keep=0), dict(keep=3, first=2, last=2), dict(keep=3, new_lens=n), dict(keep=3, first=-1),
+                   dict(keep=4, sources=torch.zeros((2, 2, 3), dtype=torch.int32, device="cuda"))):
+        with pytest.raises((ValueError, LaraConfigError)):
+            paged.kv_evict(k, v, w, table, n, change.pop("keep"), **change)
+    assert shared(q=q[:0], table=table[:0], n=n[:0]).shape == (0, 8, 64)
+    cache = paged.PagedKVCache(8, 16, 2, 64, 3, 64, "cuda")
+    cache.new_sequence()
+    with pytest.raises(ValueError, match="scored=True"):
+        cache.decode_scored(q[:1])
+    with pytest.raises(ValueError, match="scored=True"):
+        cache.evict(3)
+    with pytest.raises(ValueError, match="bf16"):
+        quant = QuantKVCache(8, 16, 2, 64, 3, 64, "cuda")
+        quant.new_sequence()
+        quant.decode_shared(q[:1])
+    cache = paged.PagedKVCache(12, 16, 2, 64, 3, 64, "cuda", scored=True)
+    rows = torch.zeros((1, 2, 40, 64), dtype=torch.bfloat16, device="cuda")
+    cache.new_sequence(), cache.new_sequence()
+    cache.append(rows, rows, [0])
+    cache.share_prefix(0, 1, 40)
+    for call in (lambda: cache.decode_scored(q), lambda: cache.evict(8), lambda: cache.evict(8, [0])):
+        with pytest.raises(ValueError, match="in common"):
+            call()
+    cache.free_sequence(1)
+    with pytest.raises(ValueError, match="twice"):
+        cache.evict(8, [0, 0])
+    cache.decode_scored(q[:1])
+    assert cache.weights.sum() > 7  # eight heads' weights
+    cache.reserve([0], 20)
+    free = cache.free_pages
+    cache.evict(60)
+    assert cache.free_pages == free and cache.seq_len(0) == 40  # nothing cut, nothing freed
+    cache.free_sequence(0)
+    cache.new_sequence()
+    cache.append(rows, rows, [0])
+    assert not cache.weights[cache.block_table[0, :3].long()].any()  # pages start anew
