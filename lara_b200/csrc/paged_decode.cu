@@ -193,7 +193,9 @@ __device__ __forceinline__ void join_rows(const DecodeArgs& a, int block) {
   }
 }
 
-// Adds the weights of an equal run of all groups, four tokens to a thread.
+// Adds the weights of an equal run of all groups, four tokens to a thread, from its end to its
+// start: the scores written last are still in L2, and those read are dropped there, which spares
+// writing them to memory.
 __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int blocks) {
   __shared__ float2 s_ml[16];  // each head's (M, 1 / L)
   __shared__ int s_seq;
@@ -206,9 +208,9 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
   const long long per = (room + blocks - 1) / blocks;
   const long long lo = block * per, hi = min(room, lo + per);
   if (lo >= hi) return;
-  for (int b = threadIdx.x; b < a.batch; b += kJoinThreads) {  // the sequence with group lo
+  for (int b = threadIdx.x; b < a.batch; b += kJoinThreads) {  // the sequence with group hi - 1
     const long long from = __ldcg(a.seq_groups + b), to = __ldcg(a.seq_groups + b + 1);
-    if (from * hkv <= lo && lo < to * hkv) {
+    if (from * hkv < hi && hi <= to * hkv) {
       s_seq = b;
       s_first[0] = from;
       s_first[1] = to;
@@ -218,7 +220,7 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
   int b = s_seq;
   long long first = s_first[0];
   int groups = (int)(s_first[1] - first);
-  int kvh = (int)quotient(lo - first * hkv, groups);
+  int kvh = (int)quotient(hi - 1 - first * hkv, groups);
   long long at = first * hkv + (long long)kvh * groups;  // the unit's first group
   while (true) {
     const UnitParts up = a.units[b * hkv + kvh];
@@ -227,9 +229,10 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
     const int32_t* const pages = a.index.block_table + (long long)b * a.index.pages_per_seq;
     auto page_of = [&](int t) { return t < t1 ? __ldg(pages + (t >> log2)) : -1; };
     constexpr int kStep = 4 * kJoinThreads;
+    const int last = t0 + (max(0, t1 - t0 - 1)) / (kStep * kAhead) * (kStep * kAhead);
     int page[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) page[j] = page_of(t0 + kStep * j + 4 * threadIdx.x);
+    for (int j = 0; j < kAhead; ++j) page[j] = page_of(last + kStep * j + 4 * threadIdx.x);
     for (int h = warp; h < G; h += kJoinWarps) {
       float M = -INFINITY, L = 0.f;
       auto join = [&](float m, float l) {
@@ -247,7 +250,8 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
       if (lane == 0) s_ml[h] = make_float2(M, 1.f / L);
     }
     __syncthreads();
-    for (int t = t0 + 4 * threadIdx.x; t < t1; t += kStep * kAhead) {
+    for (int base = last; base >= t0; base -= kStep * kAhead) {
+      const int t = base + 4 * threadIdx.x;
       const float4* s[kAhead];
       long long row[kAhead];
       float4 w[kAhead];
@@ -260,7 +264,7 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
             a.scores + (there ? (at + x / kGroup) * (G * kGroup) + x % kGroup : 0));
         w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (there) w[j] = __ldcg(reinterpret_cast<const float4*>(a.w_in + row[j]));
-        page[j] = page_of(x + kStep * kAhead);
+        page[j] = base > t0 ? page_of(x - kStep * kAhead) : -1;
       }
       float4 sum[kAhead];
 #pragma unroll
@@ -282,6 +286,11 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         if (row[j] < 0) continue;
+        if (lane % 8 == 0) {  // a group's line, which this warp alone has read, eight lanes together
+#pragma unroll 1
+          for (int i = 0; i < G; ++i)
+            asm volatile("discard.global.L2 [%0], 128;" ::"l"(s[j] + i * (kGroup / 4)), "f"(sum[j].x) : "memory");
+        }
         const int left = t1 - (t + kStep * j);
         const float4 v =
             make_float4(w[j].x + sum[j].x, w[j].y + sum[j].y, w[j].z + sum[j].z, w[j].w + sum[j].w);
@@ -295,16 +304,16 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
         }
       }
     }
-    at += groups;
-    if (at >= hi) return;
-    if (++kvh == hkv) {
-      kvh = 0;
+    if (at <= lo) return;
+    if (--kvh < 0) {
+      kvh = hkv - 1;
       do {
-        ++b;
+        --b;
         first = __ldcg(a.seq_groups + b);
         groups = (int)(__ldcg(a.seq_groups + b + 1) - first);
       } while (groups == 0);
     }
+    at -= groups;
     __syncthreads();  // s_ml is free again
   }
 }
