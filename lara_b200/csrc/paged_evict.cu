@@ -119,7 +119,6 @@ template <int kThreads, int kCtas, bool kLong, bool kMoves>
 __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_constant__ Args a, const SliceRoom room) {
   constexpr int kWarps = kThreads / 32;
   constexpr uint32_t kFull = 0xffffffffu;
-  constexpr int kUnroll = kLong ? 4 : 1;
   extern __shared__ uint32_t s_kept[];
   uint32_t* const s_keys = s_kept + room.words;
   int* const s_entry = reinterpret_cast<int*>(s_keys + room.run_keys * kWarps);
@@ -205,10 +204,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   auto count = [&](int t, const uint4& x, uint32_t border, uint32_t mask, int shift, int bins) {
     const uint32_t v[4] = {x.x, x.y, x.z, x.w};
     uint32_t* const hist = s_hist[lane & 1];
+    if (t >= m_lo && t + 3 < m_hi) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if ((unsigned)(t + j - m_lo) < (unsigned)m_count && (v[j] & mask) == border)
-        atomicAdd(hist + ((v[j] >> shift) & (bins - 1)), 1u);
+      for (int j = 0; j < 4; ++j)
+        if ((v[j] & mask) == border) atomicAdd(hist + ((v[j] >> shift) & (bins - 1)), 1u);
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j)
+        if ((unsigned)(t + j - m_lo) < (unsigned)m_count && (v[j] & mask) == border)
+          atomicAdd(hist + ((v[j] >> shift) & (bins - 1)), 1u);
+    }
   };
   {
     bool bad = false;
@@ -232,8 +237,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
         if (!kLong || t < cached) *reinterpret_cast<float4*>(run_w + t) = w[j];
         count(t, x, 0, 0, 21, kBins);
         if (copies && row[j] >= 0) {
-          if (t + 3 < min(n, a.keep)) {
-            *reinterpret_cast<float4*>(a.w_out + row[j]) = w[j];
+          if (t + 3 < n && (t + 3 < a.keep || t >= a.keep)) {
+            *reinterpret_cast<float4*>(a.w_out + row[j]) = t < a.keep ? w[j] : make_float4(0.f, 0.f, 0.f, 0.f);
           } else {
             const float v[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   for (int pass = 0; pass < 3 && free_ > 0; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
     if (pass > 0) {
-#pragma unroll kUnroll
+#pragma unroll 1
       for (int t = r_lo + 4 * lane; t < m_hi; t += 128) count(t, keys(t), border, mask, shift, bins);
     }
     if (kLong && size > 1) {
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   int seen = 0, unused;  // slots at the border before the run
   if (by_slot) {
     int mine = 0;
-#pragma unroll kUnroll
+#pragma unroll 1
     for (int t = r_lo + 4 * lane; t < m_hi; t += 128) {
       const uint4 x = keys(t);
       const uint32_t v[4] = {x.x, x.y, x.z, x.w};
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) select_kernel(const __grid_co
   // ---- which slots stay: bit `lane` of word j of a row of 128 is slot 4 lane + j ----
   uint4* const run_kept = reinterpret_cast<uint4*>(s_kept) + (r_lo - lo) / 128;
   const uint32_t lower = (1u << lane) - 1;
-#pragma unroll kUnroll
+#pragma unroll 1
   for (int t0 = r_lo; t0 < r_hi; t0 += 128) {
     const int t = t0 + 4 * lane;
     uint4 x = make_uint4(0, 0, 0, 0);
@@ -595,11 +600,11 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
   const long long most = std::min<long long>(a.keep, std::max(0ll, cap - a.keep));  // rows of a unit to move
   const bool moves = !long_ && most <= kFewMoves;
   const bool alone = moves && units <= sms;  // a CTA has an SM to itself
-  const void* const fn = long_   ? reinterpret_cast<const void*>(&select_kernel<768, 2, true, false>)
+  const void* const fn = long_   ? reinterpret_cast<const void*>(&select_kernel<512, 2, true, false>)
                          : alone ? reinterpret_cast<const void*>(&select_kernel<1024, 1, false, true>)
                          : moves ? reinterpret_cast<const void*>(&select_kernel<512, 3, false, true>)
                                  : reinterpret_cast<const void*>(&select_kernel<512, 3, false, false>);
-  const int threads = long_ ? 768 : alone ? 1024 : 512, most_smem = long_ ? kLongSmem : kShortSmem;
+  const int threads = alone ? 1024 : 512, most_smem = long_ ? kLongSmem : kShortSmem;
   // per slice: the bits, then the table, then as many keys as there is room for
   const long long run = ((cap + size - 1) / size + 4 * threads - 1) / (4 * threads) * 128, slice = run * (threads / 32);
   SliceRoom room;
