@@ -6,7 +6,8 @@
   (decode, split-KV partials + LSE combine, KV append, bf16 pack, dense
   transaction, prefill).
 * ``lara_b200.paged`` / ``lara_b200.kvquant`` -- paged KV caches in bf16 and in 8
-  bits (int8, fp8 e4m3), with the decode that reads them.
+  bits (int8, fp8 e4m3), with the decode that reads them; in bf16 also a decode
+  behind a shared prefix, one that scores its slots, and eviction.
 * ``lara_b200.workloads`` -- seeded synthetic inputs of the benchmark configs.
 * ``lara_b200.build`` -- compiles liblara_b200.so (nvcc) and the _binding of
   the calls made once per layer and token, in-tree.

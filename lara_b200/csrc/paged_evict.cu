@@ -12,8 +12,13 @@
 // 11 and 10 bits, the most significant first, weights as ordered integers) with
 // a cluster of CTAs to a unit where a unit is long and units are few, then lists
 // holes and movers in order by ballots and scans.  The second moves the rows,
-// shared out equally over the GPU.  Bound by HBM: 8 bytes of weight per slot,
-// 8 D bytes per row moved.
+// shared out equally over the GPU; where a unit has few, its CTA moves them in the
+// first.  The bytes are 8 per slot and 8 D per row moved, in rows of 2 D bytes in
+// random order.  Measured (8 kv heads, head_dim 128): 32 x 8192 slots cut to 2048
+// 111 us, of which the moves take 87 (5.2 TB/s, 0.79 of the copy rate; 64 KB in
+// flight per SM in place of 96 cost 5 us) and the selection 23; 524288 slots cut to
+// 65536 176 us (95 and 76); 16 x 2049 cut by one 9.9 us.  The selection is bound by
+// latency: barriers, scans, and instructions that run once and are not in the cache.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -34,16 +39,21 @@ namespace {
 
 constexpr int kBins = 2048;
 constexpr int kRows = 2;             // rows of 128 slots that a warp has in flight
-constexpr int kMaxCluster = 16;
-constexpr int kShortSlice = 8192;    // slots of a CTA's slice up to which its CTA is a small one
-constexpr int kLongSlice = 32768;    // slots of a slice above which clusters grow whatever the units
+constexpr int kShortSlice = 8192;    // slots that a CTA selects from alone, all of them in shared memory
+// Clusters grow while a CTA has more slots than kSlice and there are fewer CTAs than SMs (8 units of
+// 8192 slots 23.2 us, 28.5 without; of 65536 31, 67; from 2048 slots on 16 x 2112 slots 24.0 for
+// 10.8, from 8192 on 8 units of 8192 28.5), and while it has more than kLongSlice whatever the units
+// (512 units of 32768 slots 239 us, 307 in clusters from 8192 on).
+constexpr int kMaxCluster = 16, kSlice = 4096, kLongSlice = 32768;
 constexpr int kMostEntries = 2048;   // of the block table in shared memory
 // Dynamic shared memory: three small or two large CTAs to an SM; of slices of up to
 // kMostSlots (2^24 slots to a sequence), whose bits alone are more, one.
 constexpr int kShortSmem = 56 * 1024, kLongSmem = 92 * 1024, kMostSmem = 200 * 1024;
 constexpr long long kMostSlots = 1ll << 24;
-// Rows up to which a unit's CTA moves them itself.
-constexpr int kFewMoves = 64;
+// Rows up to which a unit's CTA moves them itself, with an SM of its own and without.  128 units of
+// 2304 slots cut by 256 12.7 us, 20.6 in two launches, by 512 20.0 against 24.4; 512 units cut by 128
+// 31.0 against 33.8, by 256 54 against 50.
+constexpr int kFewMoves = 512, kFewMovesShared = 128;
 constexpr int kMoveThreads = 192;
 constexpr int kMoveSmem = kMoveThreads / 32 * 2 * 32 * 512;
 
@@ -594,12 +604,13 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
   const int units = a.batch * a.index.n_kv_heads, sms = device_sm_count();
   const long long cap = a.index.capacity();
   int size = 1;
-  while (size < kMaxCluster && (cap / size > kLongSlice || (cap / size > 4096 && (long long)units * size < sms)))
+  while (size < kMaxCluster && (cap / size > kLongSlice || (cap / size > kSlice && (long long)units * size < sms)))
     size *= 2;
   const bool long_ = size > 1 || cap > kShortSlice;
   const long long most = std::min<long long>(a.keep, std::max(0ll, cap - a.keep));  // rows of a unit to move
-  const bool moves = !long_ && most <= kFewMoves;
-  const bool alone = moves && units <= sms;  // a CTA has an SM to itself
+  const bool moves = !long_ && most <= (units <= sms ? kFewMoves : kFewMovesShared);
+  // With an SM to itself a CTA has 1024 threads: 128 units cut by one slot 9.9 us, 14.0 with 512.
+  const bool alone = moves && units <= sms;
   const void* const fn = long_   ? reinterpret_cast<const void*>(&select_kernel<512, 2, true, false>)
                          : alone ? reinterpret_cast<const void*>(&select_kernel<1024, 1, false, true>)
                          : moves ? reinterpret_cast<const void*>(&select_kernel<512, 3, false, true>)

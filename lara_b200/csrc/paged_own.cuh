@@ -11,7 +11,10 @@ constexpr int kTile = 16;            // tokens per warp and stage: never across 
 constexpr int kGroup = 32;           // tokens whose scores lie together, head by head (a line of 128 bytes)
 constexpr int kUnitCost = 8;         // what a unit costs beside its tiles, in tiles
 constexpr int kMostPerSm = 12;       // CTAs or, of short units, warps to an SM that take parts of units
-constexpr int kSoloParts = 4;        // tiles go to warps, not CTAs, while that leaves this many parts of a unit
+// Tiles go to warps, not CTAs, while that leaves at most this many parts of a unit: 64 sequences of up
+// to 512 own tokens behind 8192 42 us, 70 by CTAs; 4 of up to 48 12.2 against 13.7; 37 of up to 333 (16
+// parts) 22.4 by warps, 19.7 by CTAs.  Scored, always CTAs: 64 x 4096 tokens 193 us by warps, 181.
+constexpr int kSoloParts = 4;
 constexpr int kLensCached = 1024;    // lengths kept in shared memory
 // R moves only when a score passes it by this much (log2): weights stay below 2^8.
 constexpr float kSlack = 8.f;

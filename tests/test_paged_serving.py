@@ -333,7 +333,8 @@ def test_shared_decode_of_a_padded_batch(hq, hkv, d):
 
     page, shared, lens = 32, 3, [0, 40, 96, 200, 0, 97]
     k, v, table, n = make_cache(lens, hkv, d, page, seed=2, shared=shared, spare=1)
-    own = torch.tensor([[x for x in range(k.shape[0]) if x not in set(table.flatten().tolist())]])  # two, of no sequence
+    used = set(table.flatten().tolist())
+    own = torch.tensor([[x for x in range(k.shape[0]) if x not in used]])  # two pages, of no sequence
     g = torch.Generator().manual_seed(8)
     for x in (k, v):
         x[own[0]] = torch.randn(x[own[0]].shape, generator=g).bfloat16()
@@ -688,14 +689,16 @@ def test_refused_tensors():
         return paged.gqa_decode_shared(a["q"], a["k"], a["v"], a["table"], a["n"], a["shared"],
                                        scale=a.get("scale"), workspace=a.get("ws", ws), out=a.get("out"))
 
-    for error, change in [(ValueError, dict(q=q[:, :, :32])), (ValueError, dict(q=q[0])), (TypeError, dict(q=q.float())),
-                          (ValueError, dict(q=q.cpu())), (ValueError, dict(q=q.transpose(0, 1).contiguous().transpose(0, 1))),
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)
+    for error, change in [(ValueError, dict(q=q[:, :, :32])), (ValueError, dict(q=q[0])),
+                          (TypeError, dict(q=q.float())), (ValueError, dict(q=q.cpu())), (ValueError, dict(q=turned)),
                           (ValueError, dict(v=v[:1])), (ValueError, dict(k=k[:, :, ::2], v=v[:, :, ::2])),
                           (ValueError, dict(table=table.long())), (ValueError, dict(table=table[:1])),
                           (ValueError, dict(table=table.t().contiguous().t())), (ValueError, dict(n=n.long())),
                           (ValueError, dict(n=n[:1])), (ValueError, dict(shared=-1)), (ValueError, dict(shared=99)),
                           (TypeError, dict(shared=1.5)), (ValueError, dict(scale=0.0)), (TypeError, dict(scale="x")),
-                          (ValueError, dict(out=q[:1])), (ValueError, dict(ws=ws[:256])), (ValueError, dict(ws=ws.cpu())),
+                          (ValueError, dict(out=q[:1])), (ValueError, dict(ws=ws[:256])),
+                          (ValueError, dict(ws=ws.cpu())),
                           (ValueError, dict(out=q[:, :1].expand(2, 8, 64)))]:
         with pytest.raises(error):
             shared(**change)
