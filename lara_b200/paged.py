@@ -163,6 +163,7 @@ class PagedKVCache:
         self._refs = np.zeros(self.num_pages, np.int32)
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._active = np.zeros(self.max_seqs, bool)
+        self._cut = np.zeros(self.max_seqs, bool)  # slots no longer in the order of the positions
         self._ws = None
         self._serving_ws = {}  # of decode_shared, decode_scored and evict
         self._status = new_workspace(256, self.device)
@@ -190,6 +191,7 @@ class PagedKVCache:
             raise RuntimeError("no free sequence slot")
         slot = int(idle[0])
         self._active[slot] = True
+        self._cut[slot] = False
         self._lens[slot] = 0
         self._sync_rows([slot])
         return slot
@@ -209,6 +211,8 @@ class PagedKVCache:
         tokens (reference-counted, read-only); returns the tokens shared."""
         if self._lens[dst] != 0 or not self._active[src] or not self._active[dst]:
             raise ValueError("share_prefix needs an active source and an empty active destination")
+        if self._cut[src]:
+            raise ValueError(f"sequence {src} has been cut by evict: its first slots are not its first tokens")
         n_pages = min(int(n_tokens), int(self._lens[src])) // self.page_size
         for j in range(n_pages):
             page = int(self._table[src, j])
@@ -360,7 +364,10 @@ class PagedKVCache:
         return gqa_decode_scored(q, self.k_pages, self.v_pages, self.weights, table, lens, scale=scale, workspace=ws)
 
     def evict(self, keep: int, slots=None, *, first: int = 0, last: int = 0, sources=None) -> None:
-        """:func:`kv_evict` of the given slots (default: all active); pages behind ``keep`` are free again."""
+        """:func:`kv_evict` of the given slots (default: all active); pages behind ``keep`` are free again.
+
+        A sequence that was cut has its rows out of order: it decodes as before, but is nobody's prefix.
+        """
         self._need_weights("evict")
         slots = self._slots(slots)
         self._own_pages(slots, "evict")
@@ -371,6 +378,7 @@ class PagedKVCache:
                  sources=sources, workspace=ws)
         cut = slots[self._lens[slots] > keep]
         self._lens[cut] = keep
+        self._cut[cut] = True
         for slot in cut:
             for j in range(-(-int(self._lens[slot]) // self.page_size), self.pages_per_seq):
                 if self._table[slot, j] >= 0:

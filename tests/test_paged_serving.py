@@ -738,7 +738,14 @@ def test_refused_tensors():
     free = cache.free_pages
     cache.evict(60)
     assert cache.free_pages == free and cache.seq_len(0) == 40  # nothing cut, nothing freed
+    cache.evict(30)
+    cache.new_sequence()
+    with pytest.raises(ValueError, match="cut"):
+        cache.share_prefix(0, 1, 16)
+    cache.free_sequence(1)
     cache.free_sequence(0)
     cache.new_sequence()
     cache.append(rows, rows, [0])
+    cache.new_sequence()
+    assert cache.share_prefix(0, 1, 16) == 16
     assert not cache.weights[cache.block_table[0, :3].long()].any()  # pages start anew
