@@ -431,7 +431,8 @@ LARA_API int lara_gqa_decode_kvq(const uint16_t* q, const lara_kvq_pool* pool, c
 /* workspace (zeroed once by lara_workspace_init) serves one stream at a      */
 /* time and any call that it is large enough for; a length outside            */
 /* [0, capacity] and a bad page are flagged in its status word, the length    */
-/* clamped, page 0 read and nothing written for the bad page.                 */
+/* clamped, page 0 read and nothing written for the bad page.  Tokens whose   */
+/* score is -inf weigh nothing; a row of no others gives zeros.               */
 /* ------------------------------------------------------------------------ */
 
 /* lara_gqa_decode_paged for a batch whose sequences begin with the same pages:

@@ -112,7 +112,7 @@ __device__ __forceinline__ void join_rows(const DecodeArgs& a, int block) {
     return x;
   };
   auto store = [&](long long row, int at, const float4& x, float L) {
-    const float inv = 1.f / L;
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // scores of -inf alone: zeros, as the other decodes give
     reinterpret_cast<uint2*>(a.o + row * D)[at] =
         make_uint2(pack2_rn(x.x * inv, x.y * inv), pack2_rn(x.z * inv, x.w * inv));
   };
@@ -255,7 +255,7 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
 #pragma unroll
       for (int off = 16; off; off >>= 1)
         join(__shfl_xor_sync(0xffffffffu, M, off), __shfl_xor_sync(0xffffffffu, L, off));
-      if (lane == 0) s_ml[h] = make_float2(M, 1.f / L);
+      if (lane == 0) s_ml[h] = L == 0.f ? make_float2(0.f, 0.f) : make_float2(M, 1.f / L);  // scores of -inf alone
     }
     __syncthreads();
     for (int base = last; base >= t0; base -= kStep * kAhead) {

@@ -450,16 +450,19 @@ struct OwnTokens {
         // ---- weights as the second operand: tokens 2 t4, 2 t4 + 1 (and + 8) of column g ----
         uint32_t pf[NG][2], pr[NG][2];
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+        for (int n = 0; n < NG; ++n) {
+          // while all scores were -inf they weigh nothing: -inf - -inf would be NaN
+          const float r0 = R[n][0] == -INFINITY ? 0.f : R[n][0], r1 = R[n][1] == -INFINITY ? 0.f : R[n][1];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float p0 = ex2_ftz(s[n][2 * i] - R[n][0]), p1 = ex2_ftz(s[n][2 * i + 1] - R[n][1]);
+            const float p0 = ex2_ftz(s[n][2 * i] - r0), p1 = ex2_ftz(s[n][2 * i + 1] - r1);
             l[n][0] += p0;
             l[n][1] += p1;
             const uint32_t hi = pack2_rn(p0, p1);
             pf[n][i] = transpose8x8(hi);
             pr[n][i] = transpose8x8(pack2_rn(p0 - bf16lo(hi), p1 - bf16hi(hi)));
           }
+        }
 
         // ---- O^T += V^T P^T: block c holds dims 16 c + g and 16 c + g + 8 ----
 #pragma unroll

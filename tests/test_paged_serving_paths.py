@@ -1,0 +1,69 @@
+"""Paths of the paged cache's serving operators that short calls do not take, each against its definition in 64 bits.
+
+Tolerances are those of ``test_paged_serving``.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_paged_serving import check_out, check_weights, decode64, dev, make_cache, rows64, words  # noqa: E402
+
+
+# ------------------------------------------------------------------ scores of minus infinity
+def masked64(q, k, v, table, lens, page, scale, masked):
+    """:func:`decode64` where the tokens of ``masked[b]`` have scores of -inf; rows that have no others give zeros."""
+    B, hq, d = q.shape
+    hkv = k.shape[1]
+    o = torch.zeros((B, hq, d), dtype=torch.float64)
+    kappa, A, ps = torch.zeros_like(o), torch.zeros((B, hq, 1), dtype=torch.float64), []
+    for b in range(B):
+        n = int(lens[b])
+        ks, vs = (rows64(x, table, b, n, page).transpose(0, 1) for x in (k, v))
+        off = torch.zeros(n, dtype=torch.bool)
+        off[torch.tensor(masked[b], dtype=torch.long)] = True
+        ks = ks.masked_fill(off[None, :, None], 0.0)
+        qs = q[b].double().view(hkv, -1, d)
+        p = torch.softmax((qs @ ks.transpose(1, 2) * scale).masked_fill(off, -math.inf), -1).nan_to_num(0.0)
+        ps.append(p)
+        o[b] = (p @ vs).view(hq, d)
+        kappa[b] = (p @ vs.abs()).view(hq, d)
+        A[b] = ((qs.abs() @ ks.abs().transpose(1, 2)) * scale).amax(-1).view(hq, 1)
+    return o, kappa, A, ps
+
+
+def mask_tokens(k, table, page, masked, word):
+    """Keys whose products with queries of 8 in the first two places are -inf (in fp32, where ``word`` is finite)."""
+    for b, ts in enumerate(masked):
+        for t in ts:
+            k[int(table[b, t // page]), :, t % page, :2] = word
+
+
+LOWEST = -3.3895e38  # of bf16: 8 times it is -inf in fp32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (10, 2, 64), (32, 2, 128)])
+@pytest.mark.parametrize("word", [-math.inf, LOWEST])
+def test_scored_decode_of_scores_of_minus_infinity(hq, hkv, d, word):
+    """Pages of keys that mask, first, in the middle and last; the last sequence has no other tokens."""
+    from lara_b200 import ops, paged
+
+    page, lens = 16, [400, 1000, 37, 400, 48]
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=d + hq)
+    masked = [range(16), range(320, 352), range(32, 37), [t for t in range(400) if t // 16 % 3 != 1], range(48)]
+    mask_tokens(k, table, page, masked, word)
+    g = torch.Generator().manual_seed(31)
+    q = torch.randn((len(lens), hq, d), generator=g).bfloat16()
+    q[..., :2] = 8.0
+    w = torch.rand(k.shape[:3], generator=g)
+    o, kappa, A, ps = masked64(q, k, v, table, n, page, d ** -0.5, masked)
+    qd, kd, vd, wd, td, nd = dev(q, k, v, w, table, n)
+    ws = paged.scored_workspace(len(lens), hq, kd, table.shape[1])
+    check_out(paged.gqa_decode_scored(qd, kd, vd, wd, td, nd, workspace=ws), o, kappa, A, n)
+    check_weights(wd, w, ps, A, table, n, page, d)
+    assert ops.workspace_status(ws) == 0
