@@ -341,7 +341,8 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
         const float m_new = move ? m_tile : m_ref_t;
         const float corr = move ? ex2_ftz(m_ref_t - m_new) : 1.f;
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_new, -m_new);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // while all scores were -inf they weigh nothing
+        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_use, -m_use);
 #pragma unroll
         for (int c = 0; c < CW; c += 32) {
           uint32_t pw[16], lw[16];

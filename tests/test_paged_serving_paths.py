@@ -67,3 +67,31 @@ def test_scored_decode_of_scores_of_minus_infinity(hq, hkv, d, word):
     check_out(paged.gqa_decode_scored(qd, kd, vd, wd, td, nd, workspace=ws), o, kappa, A, n)
     check_weights(wd, w, ps, A, table, n, page, d)
     assert ops.workspace_status(ws) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,batch", [(8, 2, 128, 3), (10, 2, 64, 3), (32, 2, 128, 20), (16, 2, 64, 40)])
+@pytest.mark.parametrize("word", [-math.inf, LOWEST])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "all", "own"])
+def test_shared_decode_of_scores_of_minus_infinity(hq, hkv, d, batch, word, where):
+    """Keys that mask in the prefix (in tiles of 128 tokens, whole and half) or in the own tokens; one sequence without
+    own tokens, which has nothing to attend where the whole prefix masks."""
+    from lara_b200 import ops, paged
+
+    page, shared = 64, 8
+    prefix = shared * page
+    lens = [prefix + 50] * batch
+    lens[1], lens[2] = prefix, 300  # at the prefix's end, and within it, of pages that it has in common
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=d + hq, shared=shared)
+    tokens = {"first": range(192), "middle": range(128, 320), "last": range(prefix - 192, prefix),
+              "all": range(prefix), "own": range(prefix, prefix + 50)}[where]
+    masked = [[t for t in tokens if t < m] for m in lens]
+    mask_tokens(k, table, page, masked, word)
+    q = torch.randn((batch, hq, d), generator=torch.Generator().manual_seed(32)).bfloat16()
+    q[..., :2] = 8.0
+    o, kappa, A, _ = masked64(q, k, v, table, n, page, d ** -0.5, masked)
+    qd, kd, vd, td, nd = dev(q, k, v, table, n)
+    ws = paged.shared_workspace(batch, hq, hkv, d, "cuda")
+    for front in (shared, 0):  # and every sequence for itself
+        check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, front, workspace=ws), o, kappa, A, n)
+    assert ops.workspace_status(ws) == 0
