@@ -603,13 +603,6 @@ LARA_API int lara_read_layer_perf(lara_ctx* ctx, uint64_t* prologue_ns, uint64_t
 LARA_API int lara_selftest_wait_timeout(void* workspace, int limit_us, void* stream);
 LARA_API int lara_ctx_selftest_timeout(lara_ctx* ctx, int limit_us);
 
-/* Warps that exchange values give up together: `warps` (1 .. 32) of them meet
- * `steps` (0 .. 1e6) times as the warps of a row do, warp w failing by itself
- * before its meeting leave_at[w].  met[w] (device int32[warps], as leave_at)
- * receives the meetings after which it went on: the least of steps and all
- * leave_at that are not negative. */
-LARA_API int lara_selftest_group_exit(const int32_t* leave_at, int32_t* met, int warps, int steps, void* stream);
-
 /* Asynchronous, stream-ordered forms on device buffers (the reference's
  * start() / wait_done() split, sw/attn_driver.py:361-464): they return once
  * the work is queued on `stream` (NULL: the context's stream); lara_sync then

@@ -100,32 +100,6 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
-// ---- warps that give up together ---------------------------------------------
-// Warps that exchange values meet at a named barrier, which waits without a limit
-// of its own.  So each says there whether it goes on, and all leave once one does
-// not: a warp whose bounded wait ran out goes to leave(), and the others find that
-// out at their next meeting, whichever it is.  After it none waits for another.
-struct WarpGroup {
-  int bar, threads;  // hardware barrier, threads of all the group's warps
-  bool open = true;  // no warp has left
-
-  __device__ __forceinline__ bool meet(bool go_on) {
-    uint32_t all;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %3, 0;\n\t"
-        "bar.red.and.pred q, %1, %2, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(all)
-        : "r"(bar), "r"(threads), "r"((uint32_t)go_on)
-        : "memory");
-    return open = all != 0;
-  }
-  __device__ __forceinline__ void leave() {
-    if (open) (void)meet(false);
-  }
-};
-
 // ---- bulk async copy (TMA, non-tensor, no multicast) ------------------------
 
 __device__ __forceinline__ uint64_t make_evict_first_policy() {

@@ -33,17 +33,6 @@ __global__ void selftest_wait_kernel(int* status, unsigned long long limit_ns) {
   if (!__syncthreads_and(ok) && threadIdx.x == 0) atomicOr(status, lara::kDevWaitTimeout);
 }
 
-// Each warp goes through `steps` meetings of one WarpGroup, or fails by itself
-// before its meeting leave_at[warp]; met[warp]: the meetings after which it went on.
-__global__ void selftest_group_kernel(const int* leave_at, int* met, int steps) {
-  const int warp = threadIdx.x >> 5;
-  lara::WarpGroup group{1, (int)blockDim.x};
-  int i = 0;
-  while (i < steps && i != leave_at[warp] && group.meet(true)) ++i;
-  group.leave();
-  if ((threadIdx.x & 31) == 0) met[warp] = i;
-}
-
 }  // namespace
 
 namespace lara {
@@ -58,17 +47,6 @@ extern "C" int lara_selftest_wait_timeout(void* workspace, int limit_us, void* s
   if (limit_us < 1 || limit_us > 2000000) return lara::set_last_error(LARA_ERR_BAD_CFG, "limit_us must be in [1, 2e6]");
   const cudaError_t e = lara::selftest_wait_launch(static_cast<int*>(workspace), limit_us,
                                                     static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess)
-    return lara::set_last_error(LARA_ERR_CUDA, std::string("self-test launch: ") + cudaGetErrorString(e));
-  return LARA_OK;
-}
-
-extern "C" int lara_selftest_group_exit(const int32_t* leave_at, int32_t* met, int warps, int steps, void* stream) {
-  if (!leave_at || !met) return lara::set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
-  if (warps < 1 || warps > 32 || steps < 0 || steps > 1000000)
-    return lara::set_last_error(LARA_ERR_BAD_CFG, "warps must be in [1, 32], steps in [0, 1e6]");
-  selftest_group_kernel<<<1, 32 * warps, 0, static_cast<cudaStream_t>(stream)>>>(leave_at, met, steps);
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)
     return lara::set_last_error(LARA_ERR_CUDA, std::string("self-test launch: ") + cudaGetErrorString(e));
   return LARA_OK;

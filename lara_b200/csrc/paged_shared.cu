@@ -30,8 +30,8 @@
 // (690 TFLOP/s in all; the prefix alone runs at 860, counted for all SMs), bound by
 // the softmax: 2287 cycles a step, of which 1430 are exponentials and the two bf16
 // numbers, while the products take 1536.  4 sequences behind 1024 12.8 us, latency.
-// Every wait is bounded, and the two warps of a row give up together; on a timeout
-// the CTA flags the status word, drains its own work and returns.
+// Every wait is bounded; on a timeout the CTA
+// flags the status word, drains its own work and returns.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -295,7 +295,7 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
     constexpr int CW = 64, OW = D / 2;   // a thread's columns of S and of O
     const int quarter = warp & 3, ch = warp >> 2, r = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    WarpGroup pair{1 + quarter, 64};
+    const int pair_bar = 1 + quarter;
     float* const red = reinterpret_cast<float*>(smem + C::kRedOff);  // [maxima, sums][stream][half][row]
     int done0 = 0, done1 = 0;  // steps of each stream before this segment
     bool ok = true;
@@ -335,10 +335,7 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
           asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[(c >> 1) & 3]) : "f"(sv[c]), "f"(sv[c + 1]));
         float* const rbuf = red + t * 2 * kTileM;  // its last readers have let this step's scores come
         rbuf[ch * kTileM + r] = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        if (!pair.meet(true)) {
-          ok = false;
-          break;
-        }
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
         const float m_tile = fmaxf(rbuf[r], rbuf[kTileM + r]) * a.scale_log2;  // scale > 0 keeps the order
         const bool move = m_tile > m_ref_t + kRescaleThreshold;
         const float m_new = move ? m_tile : m_ref_t;
@@ -418,10 +415,7 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
         }
         float* const lbuf = red + (2 + t) * 2 * kTileM;
         lbuf[ch * kTileM + r] = l;
-        if (!pair.meet(true)) {
-          ok = false;
-          break;
-        }
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
         l = lbuf[r] + lbuf[kTileM + r];
         const bool there = r < valid_rows(kPair ? t : 0);
         const long long row = (long long)slot * C::kRows + (kPair ? t : 0) * kTileM + r;
@@ -452,7 +446,6 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
       done0 += (steps + 1) / 2;
       done1 += steps / 2;
     }
-    pair.leave();
   }
 
   __syncthreads();
