@@ -83,6 +83,7 @@ SIGNATURES = {
     "lara_status_name": (c_char_p, [c_int]),
     "lara_device_count": (c_int, [POINTER(c_int)]),
     "lara_selftest_wait_timeout": (c_int, [c_void_p, c_int, c_void_p]),
+    "lara_selftest_withhold_tiles": (None, [c_int]),
     "lara_device_query": (c_int, [c_int, POINTER(LaraDeviceInfo)]),
     "lara_decode_plan": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, POINTER(c_int), POINTER(c_int)]),
     "lara_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),

@@ -33,9 +33,13 @@ __global__ void selftest_wait_kernel(int* status, unsigned long long limit_ns) {
   if (!__syncthreads_and(ok) && threadIdx.x == 0) atomicOr(status, lara::kDevWaitTimeout);
 }
 
+thread_local int tiles_brought = 0x7fffffff;
+
 }  // namespace
 
 namespace lara {
+int selftest_tiles_brought() { return tiles_brought; }
+
 cudaError_t selftest_wait_launch(int* status, int limit_us, cudaStream_t stream) {
   selftest_wait_kernel<<<1, 64, 0, stream>>>(status, (unsigned long long)limit_us * 1000ull);
   return cudaGetLastError();
@@ -51,6 +55,8 @@ extern "C" int lara_selftest_wait_timeout(void* workspace, int limit_us, void* s
     return lara::set_last_error(LARA_ERR_CUDA, std::string("self-test launch: ") + cudaGetErrorString(e));
   return LARA_OK;
 }
+
+extern "C" void lara_selftest_withhold_tiles(int brought) { tiles_brought = brought < 0 ? 0x7fffffff : brought; }
 
 extern "C" int lara_device_count(int* count) {
   if (!count) return lara::set_last_error(LARA_ERR_STREAM_DEST, "null output pointer");

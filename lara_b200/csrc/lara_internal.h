@@ -133,6 +133,9 @@ cudaError_t decode_tc_launch(const DecodeParams& p, cudaStream_t stream);
 // Failure-detection self test: a bounded wait on a phase nothing completes;
 // sets kDevWaitTimeout in *status after limit_us.
 cudaError_t selftest_wait_launch(int* status, int limit_us, cudaStream_t stream);
+// K/V tiles that the loads of a CTA bring in this thread's launches: all (the largest
+// int), but in the self-test of kernels whose waits run out.
+int selftest_tiles_brought();
 
 // Tensor-core (tcgen05/TMEM) attention of n_q query rows per sequence over a
 // bf16 KV cache [batch][Hkv][kv_rows][128].  Sequence b has

@@ -126,6 +126,7 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatil
 struct PrefixArgs {
   int units;  // of all kv heads
   int tiles;  // of 128 tokens
+  int brought;  // of a CTA's: all, but in the self-test of waits that run out
 };
 
 // The part of a unit that a CTA takes: token tiles [j0, j0 + n).
@@ -209,6 +210,10 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
       }
       ok = __shfl_sync(0xffffffffu, good, 0);
       for (int j = 0; ok && j < g.n; ++j, ++count) {
+        if (count >= p.brought) {
+          ok = false;
+          break;
+        }
         // the tile after this one: of this segment, or the next unit's first
         const int next = page_of(j + 1 < g.n ? g.j0 + j + 1 : 0);
         const int ks = count % C::kKStages, vs = count % C::kVStages;
@@ -298,22 +303,25 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
     const int pair_bar = 1 + quarter;
     float* const red = reinterpret_cast<float*>(smem + C::kRedOff);  // [maxima, sums][stream][half][row]
     int done0 = 0, done1 = 0;  // steps of each stream before this segment
+    // A wait that ran out leaves the order as it is: each warp goes on through all steps, without further
+    // waits and with results that are not written.  So no warp stands alone at its pair's barrier, which has
+    // no limit, and every unit's parts are entered, by which the join finds its way.
     bool ok = true;
-    for (long long at = begin; ok && at < end;) {
+    auto wait = [&](uint64_t* bar, int phase) {
+      if (!wait_all(bar, phase & 1, abort)) ok = false;
+    };
+    for (long long at = begin; at < end;) {
       const Segment g = next_segment(at);
       const int steps = steps_of(g), kvh = head_of(g), b0 = seq_of(g);
       auto valid_rows = [&](int t) { return min(a.prefix.seqs, max(0, a.batch - (b0 + t * a.prefix.seqs))) * a.group; };
       float m_ref0 = -INFINITY, m_ref1 = -INFINITY, l_part0 = 0.f, l_part1 = 0.f;
 #pragma unroll 1
-      for (int i = 0; ok && i < steps; ++i) {
+      for (int i = 0; i < steps; ++i) {
         const int t = i & 1;
         const float m_ref_t = t ? m_ref1 : m_ref0;
         const uint32_t s_tm = tmem + lane_off + t * 128;
         const uint32_t o_tm = tmem + lane_off + 256 + t * 128 + ch * OW;
-        if (!__all_sync(0xffffffffu, wait_or_abort(&bars->s_full[t], ((t ? done1 : done0) + (i >> 1)) & 1, abort))) {
-          ok = false;
-          break;
-        }
+        wait(&bars->s_full[t], (t ? done1 : done0) + (i >> 1));
         if (quarter * 32 >= valid_rows(kPair ? t : 0)) {  // no row of these warps counts
           mbar_arrive(&bars->p_full[t]);
           continue;
@@ -371,10 +379,7 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
         tmem_wait_st();
         if (i > 1 && __any_sync(0xffffffffu, corr != 1.f)) {
           // O must hold the stream's last PV before it is rescaled
-          if (!wait_all(&bars->o_full[t], ((t ? done1 : done0) + (i >> 1) - 1) & 1, abort)) {
-            ok = false;
-            break;
-          }
+          wait(&bars->o_full[t], (t ? done1 : done0) + (i >> 1) - 1);
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < OW; c += 32) {
@@ -397,12 +402,9 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
       if (threadIdx.x == 0 && g.j0 == 0)  // the unit starts here
         a.prefix_units[g.unit] = UnitParts{slot, sh.cta((long long)(g.unit + 1) * p.tiles - 1) - me + 1};
 #pragma unroll 1
-      for (int t = 0; ok && t < 2; ++t) {
+      for (int t = 0; t < 2; ++t) {
         const int n_t = (steps + 1 - t) / 2;  // steps of the stream
-        if (n_t && !wait_all(&bars->o_full[t], ((t ? done1 : done0) + n_t - 1) & 1, abort)) {
-          ok = false;
-          break;
-        }
+        if (n_t) wait(&bars->o_full[t], (t ? done1 : done0) + n_t - 1);
         if (!kPair && t == 0) continue;  // both streams' at once
         tc_fence_after();
         if (quarter * 32 >= valid_rows(kPair ? t : 0)) continue;
@@ -417,7 +419,7 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
         lbuf[ch * kTileM + r] = l;
         asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
         l = lbuf[r] + lbuf[kTileM + r];
-        const bool there = r < valid_rows(kPair ? t : 0);
+        const bool there = ok && r < valid_rows(kPair ? t : 0);
         const long long row = (long long)slot * C::kRows + (kPair ? t : 0) * kTileM + r;
         if (there && ch == 0) a.prefix_ml[row] = make_float2(m, l);
         float* const dst = a.prefix_acc + row * D + ch * OW;
@@ -598,6 +600,7 @@ cudaError_t shared_launch(const DecodeArgs& a, int head_dim, cudaStream_t stream
   PrefixArgs p;
   p.tiles = (a.shared_tokens + kTileN - 1) / kTileN;
   p.units = p.tiles ? a.prefix.units * a.index.n_kv_heads : 0;
+  p.brought = selftest_tiles_brought();
   const bool pair = a.prefix.rows > kTileM;
 #define LARA_CASE(d, ng)         \
   if (head_dim == d && (a.group > 8 ? 2 : 1) == ng) \

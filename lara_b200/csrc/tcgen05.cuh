@@ -157,9 +157,10 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Bounded wait that also gives up once another role has aborted.
+// Bounded wait that also gives up once another role has aborted, after that at once.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
   if (mbar_try_wait(bar, parity)) return true;
+  if (*abort) return false;
   const unsigned long long t0 = global_timer_ns();
   while (true) {
     for (int i = 0; i < 32; ++i)
