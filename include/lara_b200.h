@@ -604,10 +604,11 @@ LARA_API int lara_selftest_wait_timeout(void* workspace, int limit_us, void* str
 LARA_API int lara_ctx_selftest_timeout(lara_ctx* ctx, int limit_us);
 
 /* The same inside a pipeline: in this thread's later calls of
- * lara_gqa_decode_shared each CTA's loads bring only the first `brought` tiles
- * of K/V (negative: all again), so that a call with more ends after two seconds
- * of waiting, its outputs undefined, with the timeout bit of its workspace's
- * status word; the calls after it are not affected. */
+ * lara_gqa_decode_shared and lara_gqa_prefill each CTA's loads bring only the
+ * first `brought` tiles of K/V (negative: all again), so that a call with more
+ * ends after two seconds of waiting (for each wave of CTAs), its outputs
+ * undefined, with the timeout bit of its workspace's status word; the calls
+ * after it are not affected. */
 LARA_API void lara_selftest_withhold_tiles(int brought);
 
 /* Asynchronous, stream-ordered forms on device buffers (the reference's

@@ -69,6 +69,7 @@ struct TcArgs {
   int kv_rows;             // Lmax: rows per (sequence, kv head) in the K/V tensor map
   float scale_log2;
   int* status;
+  int brought;             // K/V tiles that the loads bring: all, but in the self-test of waits that run out
 };
 
 // ---------------------------------------------------------------------------
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
         tma_load_4d(q_smem + t * kTileBytes + kHalfBytes, &tm_q, 64, h, q0 + t * kTileM, b, &bars->q_full);
       }
       const int zrow = b * a.n_kv_heads + kvh;
-      for (int j = 0; j < ntiles; ++j) {
+      for (int j = 0; j < min(ntiles, a.brought); ++j) {
         const int st = j % kPPStages;
         if (j >= kPPStages && !wait_or_abort(&bars->kv_empty[st], ((j / kPPStages) - 1) & 1, abort)) break;
         uint8_t* ks = smem + kPPKOff + st * kTileBytes;
@@ -283,9 +284,12 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
       const long long vis_min0 = a.causal ? min((long long)kv_len, (long long)q_off + q0 + 1) : (long long)kv_len;
       const long long vis_min1 =
           a.causal ? min((long long)kv_len, (long long)q_off + q0 + kTileM + 1) : (long long)kv_len;
+      // A wait that ran out leaves the order as it is: each warp goes on through all steps, without further
+      // waits and with results that are not written, so that none stands alone at its row group's barrier,
+      // which has no limit.
       bool ok = true;
       int step = 0;  // parity of the exchange buffer
-      for (int j = 0; ok && j < ntiles; ++j) {
+      for (int j = 0; j < ntiles; ++j) {
   #pragma unroll 1
         for (int t = 0; t < 2; ++t, ++step) {
           const float m_ref_t = t ? m_ref1 : m_ref0;
@@ -293,10 +297,7 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
           const long long vis_min_t = t ? vis_min1 : vis_min0;
           const uint32_t s_tm = tmem + lane_off + t * 128;
           const uint32_t o_tm = tmem + lane_off + 256 + t * 128 + ch * CW;
-          if (!__all_sync(0xffffffffu, wait_or_abort(&bars->s_full[t], j & 1, abort))) {
-            ok = false;
-            break;
-          }
+          if (!__all_sync(0xffffffffu, wait_or_abort(&bars->s_full[t], j & 1, abort))) ok = false;
           tc_fence_after();
           float sv[CW];
   #pragma unroll
@@ -361,10 +362,7 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
           tmem_wait_st();
           if (j >= 1 && __any_sync(0xffffffffu, corr != 1.f)) {
             // O_t must hold PV_t(j-1) before it is rescaled
-            if (!__all_sync(0xffffffffu, wait_or_abort(&bars->o_full[t], (j - 1) & 1, abort))) {
-              ok = false;
-              break;
-            }
+            if (!__all_sync(0xffffffffu, wait_or_abort(&bars->o_full[t], (j - 1) & 1, abort))) ok = false;
             tc_fence_after();
   #pragma unroll
             for (int c = 0; c < CW; c += 32) {
@@ -385,8 +383,8 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
       }
       // epilogue: O_t / l -> bf16 (l = the pair's two partial sums)
   #pragma unroll 1
-      for (int t = 0; ok && t < 2; ++t, ++step) {
-        if (!__all_sync(0xffffffffu, wait_or_abort(&bars->o_full[t], (ntiles - 1) & 1, abort))) break;
+      for (int t = 0; t < 2; ++t, ++step) {
+        if (!__all_sync(0xffffffffu, wait_or_abort(&bars->o_full[t], (ntiles - 1) & 1, abort))) ok = false;
         tc_fence_after();
         float* lbuf = red + (step & 1) * RT * kTileM;
         lbuf[ch * kTileM + r] = t ? l_part1 : l_part0;
@@ -403,7 +401,7 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
           float ov[32];
           tmem_ld32(o_tm + c, ov);
           tmem_wait_ld();
-          if (q_row < a.n_q) {
+          if (ok && q_row < a.n_q) {
   #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               uint4 w;
@@ -637,6 +635,7 @@ cudaError_t prefill_tc_launch(const PrefillTcParams& p, cudaStream_t stream) {
   a.kv_rows = p.kv_rows;
   a.scale_log2 = p.scale_log2;
   a.status = p.status;
+  a.brought = selftest_tiles_brought();
   dim3 grid2(p.n_q_heads, (p.n_q + 2 * kTileM - 1) / (2 * kTileM), p.batch);
   // split P: several softmax threads per row (one per row would spill); bf16 P:
   // one thread per row, warps 0-3 on tile A and 4-7 on tile B

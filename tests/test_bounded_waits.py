@@ -40,3 +40,28 @@ def test_shared_decode_whose_waits_run_out(withhold, hq, hkv, d, batch, page, sh
     o, kappa, A, _ = decode64(qd, kd, vd, td, nd, page, d ** -0.5)
     check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, shared, workspace=ws), o, kappa, A, n)
     assert ops.workspace_status(ws) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["split", "bf16"])
+@pytest.mark.parametrize("brought", [0, 1, 3])
+def test_prefill_whose_waits_run_out(withhold, monkeypatch, precision, brought):
+    from lara_b200 import ops
+    from lara_b200._native import lib
+
+    if precision == "bf16":
+        monkeypatch.setenv("LARA_TC_SPLIT_P", "0")
+    hq, hkv, d, n, rows = 4, 2, 128, 300, 900
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((2, hkv, rows, d), generator=g).bfloat16().cuda() for _ in "kv")
+    q = torch.randn((2, n, hq, d), generator=g).bfloat16().cuda()
+    lens = torch.tensor([rows - n, 290], dtype=torch.int32, device="cuda")
+    ws = ops.new_workspace(lib.lara_prefill_workspace_bytes(2, n, hq, hkv, d, rows), "cuda")
+    want = ops.gqa_prefill(q, k, v, lens, workspace=ws)
+    assert ops.workspace_status(ws) == 0
+    withhold(brought)
+    ops.gqa_prefill(q, k, v, lens, workspace=ws)
+    withhold(-1)
+    assert ops.workspace_status(ws) == 1  # a wait ran out
+    assert torch.equal(ops.gqa_prefill(q, k, v, lens, workspace=ws).view(torch.int16), want.view(torch.int16))
+    assert ops.workspace_status(ws) == 0
