@@ -291,6 +291,7 @@ __device__ __forceinline__ void add_weights(const DecodeArgs& a, int block, int 
           sum[j].w = fmaf(ex2_ftz(y[j].w - x.x), x.y, sum[j].w);
         }
       }
+      __syncwarp();  // every lane's scores are read: what is discarded may be written at once
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         if (row[j] < 0) continue;
