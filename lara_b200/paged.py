@@ -223,9 +223,9 @@ class PagedKVCache:
         return n_pages * self.page_size
 
     def reserve(self, slots, n_new: int) -> None:
-        """Make sure each slot has pages for n_new more tokens."""
-        changed, fresh = [], []
-        for slot in slots:
+        """Make sure each slot has pages for n_new more tokens; a call that is refused takes none."""
+        wanted = []
+        for slot in dict.fromkeys(int(s) for s in slots):
             need_end = int(self._lens[slot]) + int(n_new)
             if need_end > self.capacity:
                 raise ValueError(f"sequence {slot} would hold {need_end} tokens > capacity {self.capacity}")
@@ -236,17 +236,18 @@ class PagedKVCache:
                 if page >= 0 and self._refs[page] > 1:
                     raise ValueError(f"sequence {slot} would append into shared page {page}")
                 if page < 0:
-                    if not self._free:
-                        raise MemoryError("page pool exhausted")
-                    page = self._free.pop()
-                    self._refs[page] = 1
-                    self._table[slot, j] = page
-                    changed.append(slot)
-                    fresh.append(page)
-        if fresh and self.weights is not None:  # what an earlier sequence's tokens gathered
+                    wanted.append((slot, j))
+        if len(wanted) > len(self._free):
+            raise MemoryError("page pool exhausted")
+        if not wanted:
+            return
+        fresh = [self._free.pop() for _ in wanted]
+        for (slot, j), page in zip(wanted, fresh):
+            self._refs[page] = 1
+            self._table[slot, j] = page
+        if self.weights is not None:  # what an earlier sequence's tokens gathered
             self.weights.index_fill_(0, torch.as_tensor(np.asarray(fresh, np.int64), device=self.device), 0.0)
-        if changed:
-            self._sync_rows(sorted(set(changed)))
+        self._sync_rows(sorted({slot for slot, _ in wanted}))
 
     def _release(self, page: int) -> None:
         self._refs[page] -= 1

@@ -1,0 +1,98 @@
+"""What ``PagedKVCache`` keeps of its sequences beside the kernels' work: pages, prefixes, files, status.
+
+On the CPU the kernels' workspaces are plain memory, and no kernel runs.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_paged_serving import check_out, check_weights, decode64  # noqa: E402
+
+
+@pytest.fixture
+def cpu_cache(monkeypatch):
+    from lara_b200 import paged
+
+    monkeypatch.setattr(paged, "new_workspace",
+                        lambda nbytes, device: torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device))
+
+    def make(num_pages, page_size, max_seqs, max_seq_len, **kw):
+        return paged.PagedKVCache(num_pages, page_size, 2, 64, max_seqs, max_seq_len, "cpu", **kw)
+
+    return make
+
+
+def hold(cache, slot, n):
+    """n more tokens without their rows."""
+    cache.reserve([slot], n)
+    cache._lens[slot] += n
+    cache._sync_rows([slot])
+
+
+def consistent(cache):
+    assert torch.equal(cache.block_table.cpu(), torch.from_numpy(cache._table))
+    assert torch.equal(cache.lens.cpu(), torch.from_numpy(cache._lens))
+    taken = cache._table[cache._table >= 0]
+    assert np.array_equal(np.bincount(taken, minlength=cache.num_pages), cache._refs)
+    assert sorted(cache._free) == np.flatnonzero(cache._refs == 0).tolist()
+
+
+# ------------------------------------------------------------------ pages
+def test_reserve_that_is_refused_takes_no_pages(cpu_cache):
+    cache = cpu_cache(5, 16, 3, 64, scored=True)
+    cache.weights += 3.0  # what earlier sequences gathered
+    a, b = cache.new_sequence(), cache.new_sequence()
+    hold(cache, a, 32), hold(cache, b, 32)
+    cache.weights += 3.0
+    before = cache._table.copy(), cache.weights.clone()
+    with pytest.raises(MemoryError):
+        cache.reserve([a, b], 1)  # one page is left for two
+    with pytest.raises(ValueError, match="capacity"):
+        hold(cache, b, 16), cache.reserve([a, b], 17)
+    cache.free_sequence(b)
+    assert np.array_equal(cache._table[a], before[0][a])
+    consistent(cache)
+    b = cache.new_sequence()
+    cache.reserve([a, b, a], 1)
+    consistent(cache)
+    new = [int(cache._table[a, 2]), int(cache._table[b, 0])]
+    assert not cache.weights[new].any()
+    assert torch.equal(cache.weights[cache._table[a, :2]], before[1][cache._table[a, :2]])
+    assert cache.free_pages == 1
+
+
+@pytest.mark.gpu
+def test_append_again_after_the_pool_was_exhausted():
+    from lara_b200.paged import PagedKVCache
+
+    hq, hkv, d, page = 8, 2, 64, 16
+    g = torch.Generator().manual_seed(4)
+    rows = lambda b, n: torch.randn((b, hkv, n, d), generator=g).bfloat16().cuda()  # noqa: E731
+    query = lambda b: torch.randn((b, hq, d), generator=g).bfloat16().cuda()  # noqa: E731
+    cache = PagedKVCache(6, page, hkv, d, 3, 64, "cuda", scored=True)
+    for _ in range(3):
+        cache.new_sequence()
+    cache.append(rows(3, 32), rows(3, 32))
+    cache.decode_scored(query(3))  # every page has weights
+    cache.free_sequence(2)
+    cache.append(rows(1, 16), rows(1, 16), [0])  # one page is left
+    with pytest.raises(MemoryError):
+        cache.append(rows(2, 1), rows(2, 1), [0, 1])
+    assert cache.free_pages == 1
+    cache.evict(16, [0])
+    cache.append(rows(2, 1), rows(2, 1), [0, 1])
+    consistent(cache)
+    lens, table = cache.lens[:2].cpu(), cache.block_table.cpu()
+    assert lens.tolist() == [17, 33]
+    before = cache.weights.cpu()
+    assert not before[table[0, 1], :, 0].any() and not before[table[1, 2]].any()
+    q = query(2)
+    o, kappa, A, ps = decode64(q.cpu(), cache.k_pages.cpu(), cache.v_pages.cpu(), table, lens, page, d ** -0.5)
+    check_out(cache.decode(q), o, kappa, A, lens)
+    check_out(cache.decode_scored(q), o, kappa, A, lens)
+    check_weights(cache.weights, before, ps, A, table, lens, page, d)
+    assert cache.status() == 0
