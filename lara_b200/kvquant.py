@@ -216,8 +216,7 @@ class QuantKVCache(PagedKVCache):
         _check_words("q", q, (len(slots), q.shape[1], self.head_dim))
         _, table, lens = self._rows(slots)
         need = int(lib.lara_kvq_decode_workspace_bytes(len(slots), q.shape[1], self.n_kv_heads, self.head_dim))
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = decode_workspace(len(slots), q.shape[1], self.n_kv_heads, self.head_dim, self.device)
+        self._ws = self._large_enough(self._ws, need)
         return gqa_decode_kvq(q, self.pool, table, lens, scale=scale, workspace=self._ws)
 
     def read(self, slots=None, out=None):

@@ -301,8 +301,7 @@ class PagedKVCache:
         check(lib.lara_decode_plan(B, hq, self.n_kv_heads, d, self.capacity, lens_host.ctypes.data,
                                    ctypes.byref(ns), ctypes.byref(ch)), "lara_decode_plan")
         nbytes = int(lib.lara_decode_workspace_bytes(B, hq, self.n_kv_heads, d, ns.value))
-        if self._ws is None or self._ws.numel() < nbytes:
-            self._ws = new_workspace(nbytes, self.device)
+        self._ws = self._large_enough(self._ws, nbytes)
         o = torch.empty_like(q)
         sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
         check(lib.lara_gqa_decode_paged(q.data_ptr(), self.k_pages.data_ptr(), self.v_pages.data_ptr(),
@@ -312,10 +311,18 @@ class PagedKVCache:
               "lara_gqa_decode_paged")
         return o
 
+    def _large_enough(self, ws, nbytes: int) -> torch.Tensor:
+        """``ws``, or a larger workspace in its place; the status bits of the one that goes are kept."""
+        if ws is not None:
+            if ws.numel() >= nbytes:
+                return ws
+            self._status[:4].view(torch.int32).bitwise_or_(ws[:4].view(torch.int32))
+            if ws.is_cuda:  # the last call that used it may still run
+                ws.record_stream(torch.cuda.current_stream(ws.device))
+        return _workspace(nbytes, self.device)
+
     def _serving(self, name: str, nbytes: int) -> torch.Tensor:
-        ws = self._serving_ws.get(name)
-        if ws is None or ws.numel() < nbytes:
-            ws = self._serving_ws[name] = _workspace(nbytes, self.device)
+        ws = self._serving_ws[name] = self._large_enough(self._serving_ws.get(name), nbytes)
         return ws
 
     def _rows_of(self, slots):

@@ -92,7 +92,44 @@ def test_append_again_after_the_pool_was_exhausted():
     assert not before[table[0, 1], :, 0].any() and not before[table[1, 2]].any()
     q = query(2)
     o, kappa, A, ps = decode64(q.cpu(), cache.k_pages.cpu(), cache.v_pages.cpu(), table, lens, page, d ** -0.5)
-    check_out(cache.decode(q), o, kappa, A, lens)
+    check_out(cache.decode_shared(q), o, kappa, A, lens)
     check_out(cache.decode_scored(q), o, kappa, A, lens)
     check_weights(cache.weights, before, ps, A, table, lens, page, d)
     assert cache.status() == 0
+
+
+# ------------------------------------------------------------------ status
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", ["decode", "decode_shared", "decode_scored", "evict", "quant"])
+def test_status_outlasts_the_workspace(call):
+    """A bad page that a small call met is reported also when a larger call has come since."""
+    from lara_b200.kvquant import QuantKVCache
+    from lara_b200.paged import PagedKVCache
+
+    hkv, d, page = 1, 64, 16
+    if call == "quant":
+        cache = QuantKVCache(400, page, hkv, d, 40, 1 << 16, "cuda")
+    else:
+        cache = PagedKVCache(400, page, hkv, d, 40, 1 << 16, "cuda", scored=True)
+    for _ in range(40):
+        cache.new_sequence()
+    rows = torch.zeros((40, hkv, 20, d), dtype=torch.bfloat16, device="cuda")
+    cache.append(rows, rows)
+
+    def go(slots, heads):
+        if call == "evict":
+            cache.evict(18 + heads // 8, slots)
+        else:
+            q = torch.zeros((len(slots), heads, d), dtype=torch.bfloat16, device="cuda")
+            getattr(cache, "decode" if call == "quant" else call)(q, slots)
+
+    good = cache.block_table.clone()
+    cache.block_table[0, 0] = 1 << 20
+    go([0], 1)
+    small = cache._ws if call in ("decode", "quant") else cache._serving_ws[call.removeprefix("decode_")]
+    cache.block_table.copy_(good)
+    more = torch.zeros((1, hkv, 4000, d), dtype=torch.bfloat16, device="cuda")
+    cache.append(more, more, [39])
+    go(list(range(40)), 8)
+    assert small is not (cache._ws if call in ("decode", "quant") else cache._serving_ws[call.removeprefix("decode_")])
+    assert cache.status() == 8 and cache.status() == 0
