@@ -425,11 +425,11 @@ class PagedKVCache:
             n = ks.shape[1]
             k[i, :, :n] = ks.view(torch.int16).cpu().numpy().view(np.uint16)
             v[i, :, :n] = vs.view(torch.int16).cpu().numpy().view(np.uint16)
-        kvfile.save(path, k, v, self._lens[slots])
+        kvfile.save(path, k, v, self._lens[slots], self._cut[slots])
 
     def load(self, path) -> list[int]:
         """Create one new sequence per stored sequence; returns their slots."""
-        k, v, lens = kvfile.load(path)
+        k, v, lens, cut = kvfile.load_any(path)
         if k.shape[1] != self.n_kv_heads or k.shape[3] != self.head_dim:
             raise ValueError(f"{path}: geometry {k.shape} does not match this cache")
         slots = []
@@ -441,4 +441,5 @@ class PagedKVCache:
                 t = lambda a: torch.from_numpy(np.ascontiguousarray(a[None, :, :n]).view(np.int16)).to(  # noqa: E731
                     self.device).view(torch.bfloat16)
                 self.append(t(k[i]), t(v[i]), slots=[s])
+            self._cut[s] = cut[i]
         return slots

@@ -133,3 +133,64 @@ def test_status_outlasts_the_workspace(call):
     go(list(range(40)), 8)
     assert small is not (cache._ws if call in ("decode", "quant") else cache._serving_ws[call.removeprefix("decode_")])
     assert cache.status() == 8 and cache.status() == 0
+
+
+# ------------------------------------------------------------------ files
+def test_files_say_which_sequences_are_cut(tmp_path):
+    from lara_b200 import kvfile
+
+    g = np.random.default_rng(1)
+    k, v = (g.integers(0, 1 << 16, (3, 2, 5, 64), dtype=np.uint16) for _ in "kv")
+    lens = np.array([5, 0, 3], np.int32)
+    whole, cut = tmp_path / "whole.npz", tmp_path / "cut.npz"
+    kvfile.save(whole, k, v, lens, np.zeros(3, bool))
+    with np.load(whole) as z:
+        assert "cut" not in z  # as before
+    kvfile.save(cut, k, v, lens, np.array([False, False, True]))
+    for x, y in zip(kvfile.load(whole), (k, v, lens)):
+        assert np.array_equal(x, y)
+    for path, want in ((whole, [0, 0, 0]), (cut, [0, 0, 1])):
+        for x, y in zip(kvfile.load_any(path), (k, v, lens, np.array(want, bool))):
+            assert np.array_equal(x, y)
+    with pytest.raises(ValueError, match=r"\[2\] have been cut"):
+        kvfile.load(cut)
+    with np.load(cut) as z:
+        held = dict(z)
+    for change in (dict(cut=np.array([True, False, True])), dict(cut=None)):
+        np.savez(cut, **{x: y for x, y in {**held, **change}.items() if y is not None})
+        with pytest.raises(ValueError, match="checksum"):
+            kvfile.load_any(cut)
+    with pytest.raises(ValueError, match="cut"):
+        kvfile.save(cut, k, v, lens, np.ones(2, bool))
+
+
+@pytest.mark.gpu
+def test_a_cut_sequence_from_a_file_is_nobodys_prefix(tmp_path):
+    from lara_b200.attn_driver import AttentionAccelerator
+    from lara_b200.paged import PagedKVCache
+
+    cache = PagedKVCache(24, 16, 2, 64, 6, 64, "cuda", scored=True)
+    g = torch.Generator().manual_seed(2)
+    for n in (40, 33):
+        s = cache.new_sequence()
+        rows = torch.randn((1, 2, n, 64), generator=g).bfloat16().cuda()
+        cache.append(rows, rows, [s])
+    cache.decode_scored(torch.randn((2, 4, 64), generator=g).bfloat16().cuda())
+    cache.evict(32, [0])
+    cache.save(tmp_path / "kv")
+    a, b = cache.load(tmp_path / "kv")
+    for x, y in zip((*cache.gather(a), *cache.gather(b)), (*cache.gather(0), *cache.gather(1))):
+        assert torch.equal(x, y)
+    c = cache.new_sequence()
+    with pytest.raises(ValueError, match="cut"):
+        cache.share_prefix(a, c, 16)
+    assert cache.share_prefix(b, c, 33) == 32
+    with AttentionAccelerator() as acc:
+        acc.configure_heads(4, 2, 64, max_seq_len=64, batch=2)
+        with pytest.raises(ValueError, match="cut"):
+            acc.restore_kv(tmp_path / "kv")
+    cache.free_sequence(a)
+    assert cache.new_sequence() == a  # whole again
+    rows = torch.zeros((1, 2, 20, 64), dtype=torch.bfloat16, device="cuda")
+    cache.append(rows, rows, [a])
+    assert cache.share_prefix(a, cache.new_sequence(), 16) == 16
