@@ -342,10 +342,24 @@ class PagedKVCache:
             raise ValueError(f"{what} needs a cache with weights (scored=True)")
 
     def shared_pages(self, slots=None) -> int:
-        """How many pages all of the slots begin with in common."""
-        rows = self._table[self._slots(slots)]
-        same = (rows == rows[0]).all(0) & (rows[0] >= 0)
-        return int(same.size if same.all() else same.argmin())
+        """How many pages the slots begin with in common, those aside that end within them.
+
+        Every sequence that holds that many whole pages begins with the same ones, and of such prefixes it is the one
+        whose single reading spares the most pages.
+        """
+        slots = self._slots(slots)
+        rows = self._table[slots]
+        if len(slots) == 1:
+            return int((rows[0] >= 0).cumprod().sum())
+        whole = self._lens[slots] // self.page_size
+        same = (rows == rows[whole.argmax()]).cumprod(1).sum(1)  # leading pages that are the longest sequence's
+        reach = np.arange(1, int(whole.max()) + 1)
+        holders = len(slots) - np.searchsorted(np.sort(whole), reach)
+        differ = np.zeros(len(reach) + 1, np.int64)  # sequences that hold so many pages, but other ones
+        np.add.at(differ, np.minimum(same, whole), 1)
+        np.add.at(differ, whole, -1)
+        spared = np.where(differ.cumsum()[:-1] == 0, reach * (holders - 1), 0)
+        return int(reach[spared.argmax()]) if spared.any() else 0
 
     def decode_shared(self, q, slots=None, scale=None):
         """:meth:`decode`, reading the pages that all slots begin with (:meth:`share_prefix`) once for the batch."""

@@ -194,3 +194,88 @@ def test_a_cut_sequence_from_a_file_is_nobodys_prefix(tmp_path):
     rows = torch.zeros((1, 2, 20, 64), dtype=torch.bfloat16, device="cuda")
     cache.append(rows, rows, [a])
     assert cache.share_prefix(a, cache.new_sequence(), 16) == 16
+
+
+# ------------------------------------------------------------------ common prefixes
+def most_spared(rows, lens, page):
+    """The definition of ``shared_pages``, prefix by prefix."""
+    best, pages = 0, 0
+    for n in range(1, max(lens) // page + 1):
+        holders = [r[:n].tolist() for r, m in zip(rows, lens) if m // page >= n]
+        if all(x == holders[0] for x in holders) and n * (len(holders) - 1) > best:
+            best, pages = n * (len(holders) - 1), n
+    return pages
+
+
+def test_shared_pages_leaves_short_sequences_aside(cpu_cache):
+    cache = cpu_cache(400, 16, 40, 640)
+    doc = cache.new_sequence()
+    hold(cache, doc, 330)
+    group = [doc]
+    for n in range(5):
+        s = cache.new_sequence()
+        assert cache.share_prefix(doc, s, 330) == 320
+        if n:
+            hold(cache, s, 17 * n)
+        group.append(s)
+    assert cache.shared_pages() == cache.shared_pages(group) == 20
+    empty, short, other = cache.new_sequence(), cache.new_sequence(), cache.new_sequence()
+    hold(cache, short, 100)  # pages of its own, fewer than the prefix has
+    assert cache.shared_pages([empty] + group) == cache.shared_pages(group + [empty, short]) == 20
+    inside = cache.new_sequence()
+    assert cache.share_prefix(doc, inside, 200) == 192
+    assert cache.shared_pages([inside] + group) == 20
+    hold(cache, other, 321)  # as long, and other pages
+    assert cache.shared_pages(group + [other]) == 0
+    assert cache.shared_pages([empty, short]) == cache.shared_pages([empty, cache.new_sequence()]) == 0
+    assert cache.shared_pages([doc]) == 21 and cache.shared_pages([empty]) == 0
+    assert cache.shared_pages([short, short]) == 6  # whole pages
+
+
+def test_shared_pages_of_any_slots(cpu_cache):
+    rng = np.random.default_rng(7)
+    for _ in range(60):
+        cache = cpu_cache(600, 16, 12, 320)
+        slots = []
+        for i in range(12):
+            s = cache.new_sequence()
+            if slots and rng.random() < 0.7:
+                src = int(rng.choice(slots))
+                cache.share_prefix(src, s, int(rng.integers(0, cache.seq_len(src) + 1)))
+            hold(cache, s, int(rng.integers(0, 321 - cache.seq_len(s)) * rng.random()))
+            slots.append(s)
+        for _ in range(8):
+            pick = rng.choice(slots, rng.integers(2, 13), replace=bool(rng.random() < 0.3))
+            want = most_spared(cache._table[pick], [cache.seq_len(s) for s in pick], 16)
+            assert cache.shared_pages(pick) == want
+
+
+@pytest.mark.gpu
+def test_decode_shared_beside_sequences_that_end_within_the_prefix():
+    """An empty slot, a short sequence, and one that shares less read for themselves what the others read together."""
+    from lara_b200 import paged
+
+    hq, hkv, d, page = 8, 2, 64, 16
+    g = torch.Generator().manual_seed(6)
+    rows = lambda n: torch.randn((1, hkv, n, d), generator=g).bfloat16().cuda()  # noqa: E731
+    cache = paged.PagedKVCache(64, page, hkv, d, 8, 400, "cuda")
+    doc = cache.new_sequence()
+    x = rows(200)
+    cache.append(x, x, [doc])
+    for n in (0, 5, 40):
+        s = cache.new_sequence()
+        assert cache.share_prefix(doc, s, 200) == 192
+        if n:
+            x = rows(n)
+            cache.append(x, x, [s])
+    cache.new_sequence()
+    short = cache.new_sequence()
+    x = rows(70)
+    cache.append(x, x, [short])
+    assert cache.share_prefix(doc, cache.new_sequence(), 100) == 96
+    assert cache.shared_pages() == 12
+    q = torch.randn((7, hq, d), generator=g).bfloat16()
+    lens = torch.tensor([200, 192, 197, 232, 0, 70, 96])
+    o, kappa, A, _ = decode64(q, cache.k_pages.cpu(), cache.v_pages.cpu(), cache.block_table.cpu(), lens, page, d ** -0.5)
+    check_out(cache.decode_shared(q.cuda()), o, kappa, A, lens)
+    assert cache.status() == 0
