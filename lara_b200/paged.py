@@ -338,6 +338,8 @@ class PagedKVCache:
             raise ValueError(f"{what}: a slot is named twice")
 
     def _need_weights(self, what: str) -> None:
+        if not hasattr(self, "k_pages"):
+            raise ValueError(f"{what} needs a cache of bf16 rows")
         if self.weights is None:
             raise ValueError(f"{what} needs a cache with weights (scored=True)")
 

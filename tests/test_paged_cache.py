@@ -279,3 +279,15 @@ def test_decode_shared_beside_sequences_that_end_within_the_prefix():
     o, kappa, A, _ = decode64(q, cache.k_pages.cpu(), cache.v_pages.cpu(), cache.block_table.cpu(), lens, page, d ** -0.5)
     check_out(cache.decode_shared(q.cuda()), o, kappa, A, lens)
     assert cache.status() == 0
+
+
+# ------------------------------------------------------------------ refusals
+def test_8_bit_cache_names_what_it_lacks():
+    from lara_b200.kvquant import QuantKVCache
+
+    cache = QuantKVCache.__new__(QuantKVCache)  # before any memory is asked for
+    cache.weights = None
+    q = torch.zeros((1, 8, 64), dtype=torch.bfloat16)
+    for call in (lambda: cache.decode_scored(q), lambda: cache.decode_shared(q), lambda: cache.evict(8)):
+        with pytest.raises(ValueError, match="bf16 rows"):
+            call()
