@@ -472,7 +472,8 @@ LARA_API int lara_gqa_decode_scored(const uint16_t* q, const uint16_t* k_pages, 
  *   weights_out: kept slots' weights below `keep`, 0 from there to the old length
  *   sources[b][h][j] (NULL, or int32 [B][Hkv][keep]): the slot that slot j's row came from
  *                (j where it stayed, -1 at and past the new length)
- *   new_lens[b] (NULL, or int32 [B], apart from seq_lens) = min(seq_lens[b], keep)
+ *   new_lens[b] (NULL, or int32 [B]) = min(seq_lens[b], keep)
+ * sources and new_lens lie apart from each other, from block_table and seq_lens.
  * seq_lens stays as it is; weights_out may be weights.  The order of the slots
  * no longer is that of the positions, which no decode needs.  A page belongs to
  * one sequence of the call.  keep >= 1, first + last <= keep. */

@@ -674,8 +674,20 @@ extern "C" int lara_kv_evict(uint16_t* k_pages, uint16_t* v_pages, const float* 
   if ((long long)num_pages * n_kv_heads * page_size >= (long long)kBadRow ||
       (long long)num_pages * n_kv_heads > 0x7fffffffll)
     return set_last_error(LARA_ERR_BAD_CFG, "pools of less than 2^32 - 1 rows, 2^31 pages of one head");
-  if (kvq::overlap(new_lens, seq_lens, (size_t)batch * 4))
+  // CTAs of a cluster read lengths and tables at different times, and have to agree on them
+  const size_t lens_bytes = (size_t)batch * 4, table_bytes = lens_bytes * pages_per_seq,
+               sources_bytes = lens_bytes * n_kv_heads * keep;
+  auto apart = [](const void* x, size_t x_bytes, const void* y, size_t y_bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    return !x || !y || a >= b + y_bytes || b >= a + x_bytes;
+  };
+  if (!apart(new_lens, lens_bytes, seq_lens, lens_bytes))
     return set_last_error(LARA_ERR_STREAM_DEST, "new_lens must lie apart from seq_lens");
+  if (!apart(new_lens, lens_bytes, block_table, table_bytes) ||
+      !apart(sources, sources_bytes, block_table, table_bytes) ||
+      !apart(sources, sources_bytes, seq_lens, lens_bytes) || !apart(sources, sources_bytes, new_lens, lens_bytes))
+    return set_last_error(LARA_ERR_STREAM_DEST,
+                          "new_lens and sources must lie apart from each other, from block_table and seq_lens");
   if (const int rc = check_weights(weights, weights_out, n_kv_heads, page_size, num_pages)) return rc;
   const Layout w = layout(batch, n_kv_heads, keep);
   if (workspace_bytes < w.total) return set_last_error(LARA_ERR_RESULT_LEN, "eviction workspace too small");

@@ -291,3 +291,18 @@ def test_8_bit_cache_names_what_it_lacks():
     for call in (lambda: cache.decode_scored(q), lambda: cache.decode_shared(q), lambda: cache.evict(8)):
         with pytest.raises(ValueError, match="bf16 rows"):
             call()
+
+
+def test_evict_refuses_outputs_over_what_it_reads():
+    from test_paged_serving import DEST, P, c_call
+
+    # 3 sequences, 4 pages each, 2 kv heads, 8 slots kept: 12 bytes of lengths, 48 of table, 192 of sources
+    far = dict(table=3 * P, lens=4 * P, new_lens=5 * P, sources=6 * P)
+    for change in (dict(new_lens=4 * P + 8), dict(new_lens=4 * P - 8), dict(new_lens=3 * P + 44), dict(new_lens=3 * P - 8),
+                   dict(sources=3 * P + 44), dict(sources=3 * P - 188), dict(sources=4 * P + 8), dict(sources=4 * P - 188),
+                   dict(sources=5 * P + 8), dict(sources=5 * P - 188)):
+        assert c_call("evict", **{**far, **change}) == DEST, change
+    # next to each other they are accepted, and refused for the workspace alone
+    for change in (dict(new_lens=4 * P + 12), dict(new_lens=3 * P + 48), dict(sources=3 * P - 192), dict(sources=5 * P + 12),
+                   dict(sources=4 * P - 192), dict(new_lens=0, sources=0)):
+        assert c_call("evict", **{**far, **change}, nbytes=0) == 0x12, change
