@@ -665,7 +665,7 @@ extern "C" int lara_kv_evict(uint16_t* k_pages, uint16_t* v_pages, const float* 
     return set_last_error(LARA_ERR_BAD_CFG, "keep must be positive and at least first + last");
   if (batch == 0) return LARA_OK;
   if ((long long)batch * n_kv_heads > 0x7fffffffll / kMaxCluster)
-    return set_last_error(LARA_ERR_BAD_CFG, "batch * n_kv_heads must be below 2^28");
+    return set_last_error(LARA_ERR_BAD_CFG, "batch * n_kv_heads must be below 2^27");
   if (!weights || !weights_out || !seq_lens || !workspace) return set_last_error(LARA_ERR_STREAM_DEST, "null pointer");
   if (!aligned(seq_lens, 4) || !aligned(new_lens, 4) || !aligned(sources, 4) || !aligned(workspace, 256))
     return set_last_error(LARA_ERR_STREAM_DEST, "lengths and sources must be 4-byte aligned, the workspace 256-byte");

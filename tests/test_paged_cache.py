@@ -306,3 +306,13 @@ def test_evict_refuses_outputs_over_what_it_reads():
     for change in (dict(new_lens=4 * P + 12), dict(new_lens=3 * P + 48), dict(sources=3 * P - 192), dict(sources=5 * P + 12),
                    dict(sources=4 * P - 192), dict(new_lens=0, sources=0)):
         assert c_call("evict", **{**far, **change}, nbytes=0) == 0x12, change
+
+
+def test_evict_names_its_bound_of_units():
+    from lara_b200._native import lib
+    from test_paged_serving import BAD_CFG, c_call
+
+    few = dict(page_size=16, pages_per_seq=1, num_pages=1, nbytes=0)
+    assert c_call("evict", **few, batch=1 << 15, n_kv_heads=1 << 12) == BAD_CFG
+    assert b"below 2^27" in lib.lara_last_error_string()
+    assert c_call("evict", **few, batch=(1 << 15) - 1, n_kv_heads=1 << 12) == 0x12  # the workspace alone
