@@ -95,3 +95,84 @@ def test_shared_decode_of_scores_of_minus_infinity(hq, hkv, d, batch, word, wher
     for front in (shared, 0):  # and every sequence for itself
         check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, front, workspace=ws), o, kappa, A, n)
     assert ops.workspace_status(ws) == 0
+
+
+# ------------------------------------------------------------------ long prefixes
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,batch,page,shared", [
+    (32, 8, 128, 4, 256, 160),   # one row tile, 320 token tiles to a kv head: runs that cross kv heads in mid-prefix
+    (28, 4, 64, 3, 16, 2507),    # the same of pages smaller than a tile, the last tile in part
+    (8, 2, 128, 70, 64, 315),    # row tiles: one pair and one alone
+    (64, 4, 64, 30, 128, 157),   # groups of 16, four row tiles
+    (6, 1, 128, 150, 32, 1001)])
+def test_shared_decode_behind_a_long_prefix(hq, hkv, d, batch, page, shared):
+    """Many token tiles for each CTA, and scores that grow along the prefix, so that references move late."""
+    from lara_b200 import ops, paged
+
+    prefix = shared * page
+    lens = [prefix + (7 * b) % 90 for b in range(batch)]
+    lens[1] = prefix - 3
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=hq + batch, shared=shared)
+    grow = (1.0 + 2.0 * torch.arange(shared) / shared).view(-1, 1, 1, 1)
+    at = table[0, :shared].long()
+    k[at] = (k[at].float() * grow).bfloat16()
+    q = torch.randn((batch, hq, d), generator=torch.Generator().manual_seed(33)).bfloat16()
+    qd, kd, vd, td, nd = dev(q, k, v, table, n)
+    o, kappa, A, _ = decode64(qd, kd, vd, td, nd, page, d ** -0.5)
+    ws = paged.shared_workspace(batch, hq, hkv, d, "cuda")
+    got = paged.gqa_decode_shared(qd, kd, vd, td, nd, shared, workspace=ws)
+    check_out(got, o, kappa, A, n)
+    assert torch.equal(words(paged.gqa_decode_shared(qd, kd, vd, td, nd, shared, workspace=ws)), words(got))
+    assert ops.workspace_status(ws) == 0
+
+
+# ------------------------------------------------------------------ long evictions
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,page,keep,hkv", [
+    ([700000], 64, 100003, 1),          # more keys to a CTA than its shared memory holds
+    ([640000, 13, 520001], 16, 300007, 1),  # and more table entries
+    ([1 << 20], 256, 1000, 2), ([600000], 16, 599999, 1)])
+@pytest.mark.parametrize("kind", ["many", "ties"])
+def test_evict_of_very_long_sequences(lens, page, keep, hkv, kind):
+    from lara_b200 import ops, paged
+
+    d = 64
+    used = [-(-m // page) for m in lens]
+    g = torch.Generator(device="cuda").manual_seed(len(lens) + keep)
+    order = torch.randperm(sum(used) + 3, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(lens), max(used) + 1), -1, dtype=torch.int32, device="cuda")
+    for b, u in enumerate(used):
+        table[b, :u] = order[sum(used[:b]):sum(used[:b + 1])]
+    shape = (sum(used) + 3, hkv, page)
+    k, v = (torch.randint(-32768, 32768, (*shape, d), generator=g, device="cuda", dtype=torch.int16) for _ in "kv")
+    w = torch.randint(0, 3 if kind == "ties" else 1 << 22, shape, generator=g, device="cuda").float() / 64
+    k0, v0, w0 = k.clone(), v.clone(), w.clone()
+    src = torch.empty((len(lens), hkv, keep), dtype=torch.int32, device="cuda")
+    ws = paged.evict_workspace(len(lens), hkv, keep, "cuda")
+    new = paged.kv_evict(k, v, w, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), keep, first=3, last=77,
+                         sources=src, workspace=ws)
+    assert new.tolist() == [min(m, keep) for m in lens]
+    free = torch.ones(shape[0], dtype=torch.bool, device="cuda")
+    for b, m in enumerate(lens):
+        t = torch.arange(m, device="cuda")
+        pages, rows = table[b].long()[t // page], t % page
+        free[pages] = False
+        for h in range(hkv):
+            at = (pages, h, rows)
+            want = torch.arange(keep, device="cuda")
+            if m <= keep:
+                want[m:] = -1
+                assert torch.equal(src[b, h].long(), want)
+                assert torch.equal(k[at], k0[at]) and torch.equal(v[at], v0[at]) and torch.equal(w[at], w0[at])
+                continue
+            x = w0[at].clone()
+            x[:3] = x[m - 77:] = math.inf
+            kept = torch.zeros(m, dtype=torch.bool, device="cuda")
+            kept[torch.sort(x, descending=True, stable=True).indices[:keep]] = True
+            want[~kept[:keep]] = torch.nonzero(kept[keep:]).flatten() + keep
+            assert torch.equal(src[b, h].long(), want)
+            assert torch.equal(w[at][:keep], w0[at][want]) and not w[at][keep:].any()
+            assert torch.equal(k[at][:keep], k0[at][want]) and torch.equal(v[at][:keep], v0[at][want])
+            assert torch.equal(k[at][keep:], k0[at][keep:])
+    assert torch.equal(w[free], w0[free]) and torch.equal(k[free], k0[free])
+    assert ops.workspace_status(ws) == 0
