@@ -12,11 +12,12 @@
 // weights (G fp32 numbers per token and kv head written and read beside the 4 D
 // bytes of its rows: at G = 4, D = 128 6 % of them, against 50 % for reading K twice).
 //
-// Bound by HBM.  Measured, scored: 64 x 4096 tokens (32 heads on 8) 175 us, of which
-// the first launch takes 168 (6.4 TB/s, 0.97 of the copy rate) and the second 8 to
-// 16 beside the next call; 524288 tokens (64 heads) 397 us (351 and 46); 33
-// sequences of up to 9000, head_dim 64, 7 heads to a kv head 48 us (30 and 13);
-// 500 tokens 9 us.  What is left is in the second launch: a chain of loads per unit,
+// Bound by HBM.  Measured, scored, one state replayed in a graph and, in brackets,
+// inputs that change from pass to pass: 64 x 4096 tokens (32 heads on 8) 175 us (180 to
+// 184), of which the first launch takes 168 (6.4 TB/s, 0.97 of the copy rate) and the
+// second 8 to 16 beside the next call; 524288 tokens (64 heads) 397 us (391 to 404; 351
+// and 46); 33 sequences of up to 9000, head_dim 64, 7 heads to a kv head 48 us (48 to
+// 51; 30 and 13); 500 tokens 9 us (9).  What is left is in the second launch: a chain of loads per unit,
 // and of long contexts scores that L2 no longer holds.
 #include <algorithm>
 #include <cmath>

