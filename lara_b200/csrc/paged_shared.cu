@@ -57,6 +57,11 @@ constexpr int kTileM = 128, kTileN = 128;
 constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kTmaWarp = 9;
 constexpr int kOwnWarps = 12, kThreads = kOwnWarps * 32;  // two warps of the prefix's CTAs idle
 constexpr float kRescaleThreshold = 8.0f;
+// A score less its reference is one fused operation, exact but for its end.  The reference is a
+// rounded product, so what is left of the largest score is up to 2^-24 of it: past this bound, which
+// keys that mask with the type's lowest value pass, an exponent too large.  There the scores are
+// rounded products too, and none is above the reference by more than the threshold.
+constexpr float kLargeScore = 0x1p27f;
 constexpr uint32_t kTmemCols = 512;  // S_0 | S_1 | O_0 | O_1, 128 columns each
 
 template <int D, bool kPair>
@@ -346,15 +351,22 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
         for (int c = 4; c < CW; c += 2)
           asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[(c >> 1) & 3]) : "f"(sv[c]), "f"(sv[c + 1]));
         float* const rbuf = red + t * 2 * kTileM;  // its last readers have let this step's scores come
-        rbuf[ch * kTileM + r] = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;  // scale > 0 keeps the order
+        rbuf[ch * kTileM + r] = top;
+        float unit = a.scale_log2;  // of sv
+        if (__any_sync(0xffffffffu, fabsf(top) > kLargeScore && top != -INFINITY)) {
+#pragma unroll
+          for (int c = 0; c < CW; ++c) sv[c] *= a.scale_log2;
+          unit = 1.f;
+        }
         asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-        const float m_tile = fmaxf(rbuf[r], rbuf[kTileM + r]) * a.scale_log2;  // scale > 0 keeps the order
+        const float m_tile = fmaxf(rbuf[r], rbuf[kTileM + r]);
         const bool move = m_tile > m_ref_t + kRescaleThreshold;
         const float m_new = move ? m_tile : m_ref_t;
         const float corr = move ? ex2_ftz(m_ref_t - m_new) : 1.f;
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const float m_use = m_new == -INFINITY ? 0.f : m_new;  // while all scores were -inf they weigh nothing
-        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_use, -m_use);
+        const float2 sc2 = make_float2(unit, unit), nm2 = make_float2(-m_use, -m_use);
 #pragma unroll
         for (int c = 0; c < CW; c += 32) {
           uint32_t pw[16], lw[16];

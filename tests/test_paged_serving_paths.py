@@ -97,6 +97,59 @@ def test_shared_decode_of_scores_of_minus_infinity(hq, hkv, d, batch, word, wher
     assert ops.workspace_status(ws) == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,batch", [(8, 2, 128, 3), (10, 2, 64, 3), (32, 2, 128, 20), (16, 2, 64, 40)])
+@pytest.mark.parametrize("size", [2.0 ** -6, 0.5, 1.0])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "all", "own"])
+def test_decodes_of_finite_scores_that_mask(hq, hkv, d, batch, size, where):
+    """Keys of the type's lowest value whose scores are finite, -10^35 to -10^38: they weigh nothing beside others."""
+    from lara_b200 import paged
+
+    page, shared = 64, 8
+    prefix = shared * page
+    lens = [prefix + 50 + b % 7 for b in range(batch)]
+    k, v, table, n = make_cache(lens, hkv, d, page, seed=d + hq, shared=shared)
+    tokens = {"first": range(192), "middle": range(128, 320), "last": range(prefix - 192, prefix),
+              "all": range(prefix), "own": range(prefix, prefix + 50 - 13)}[where]
+    masked = [list(tokens)] * batch
+    mask_tokens(k, table, page, masked, LOWEST)
+    q = torch.randn((batch, hq, d), generator=torch.Generator().manual_seed(34)).bfloat16()
+    q[..., :2] = size
+    o, kappa, A, _ = masked64(q, k, v, table, n, page, d ** -0.5, masked)
+    qd, kd, vd, td, nd = dev(q, k, v, table, n)
+    for front in (shared, 0):
+        check_out(paged.gqa_decode_shared(qd, kd, vd, td, nd, front), o, kappa, A, n)
+    if batch == 3:  # a sequence of its own, scored
+        w = torch.zeros(k.shape[:3])
+        o, kappa, A, ps = masked64(q[:1], k, v, table[:1], n[:1], page, d ** -0.5, masked[:1])
+        wd = w.cuda()
+        check_out(paged.gqa_decode_scored(qd[:1], kd, vd, wd, td[:1], nd[:1]), o, kappa, A, n[:1])
+        check_weights(wd, w, ps, A, table[:1], n[:1], page, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,batch", [(8, 2, 128, 3), (10, 2, 64, 3), (16, 2, 64, 40)])
+@pytest.mark.parametrize("size", [2.0 ** -96, 2.0 ** -6, 0.5])
+def test_decodes_of_one_score_above_all(hq, hkv, d, batch, size):
+    """A finite score of 10^9 to 10^38 takes all the weight, wherever it is: the output is that token's value."""
+    from lara_b200 import paged
+
+    page, shared = 64, 8
+    prefix = shared * page
+    lens = [prefix + 50] * batch
+    for at in (0, 200, prefix - 1, prefix + 20):
+        k, v, table, n = make_cache(lens, hkv, d, page, seed=d + hq, shared=shared)
+        mask_tokens(k, table, page, [[at]] * batch, -LOWEST)
+        q = torch.randn((batch, hq, d), generator=torch.Generator().manual_seed(35)).bfloat16()
+        q[..., :2] = size
+        qd, kd, vd, td, nd = dev(q, k, v, table, n)
+        for front in (shared, 0):
+            got = paged.gqa_decode_shared(qd, kd, vd, td, nd, front).cpu().view(batch, hkv, -1, d)
+            for b in range(batch):
+                want = v[int(table[b, at // page]), :, at % page]
+                assert torch.equal(got[b], want[:, None].expand_as(got[b]))
+
+
 # ------------------------------------------------------------------ long prefixes
 @pytest.mark.gpu
 @pytest.mark.parametrize("hq,hkv,d,batch,page,shared", [
