@@ -57,11 +57,6 @@ constexpr int kTileM = 128, kTileN = 128;
 constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kTmaWarp = 9;
 constexpr int kOwnWarps = 12, kThreads = kOwnWarps * 32;  // two warps of the prefix's CTAs idle
 constexpr float kRescaleThreshold = 8.0f;
-// A score less its reference is one fused operation, exact but for its end.  The reference is a
-// rounded product, so what is left of the largest score is up to 2^-24 of it: past this bound, which
-// keys that mask with the type's lowest value pass, an exponent too large.  There the scores are
-// rounded products too, and none is above the reference by more than the threshold.
-constexpr float kLargeScore = 0x1p27f;
 constexpr uint32_t kTmemCols = 512;  // S_0 | S_1 | O_0 | O_1, 128 columns each
 
 template <int D, bool kPair>
@@ -353,12 +348,7 @@ __device__ __forceinline__ void prefix_pass(const CUtensorMap& tm_q, const CUten
         float* const rbuf = red + t * 2 * kTileM;  // its last readers have let this step's scores come
         const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;  // scale > 0 keeps the order
         rbuf[ch * kTileM + r] = top;
-        float unit = a.scale_log2;  // of sv
-        if (__any_sync(0xffffffffu, fabsf(top) > kLargeScore && top != -INFINITY)) {
-#pragma unroll
-          for (int c = 0; c < CW; ++c) sv[c] *= a.scale_log2;
-          unit = 1.f;
-        }
+        const float unit = score_unit(sv, top, a.scale_log2);
         asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
         const float m_tile = fmaxf(rbuf[r], rbuf[kTileM + r]);
         const bool move = m_tile > m_ref_t + kRescaleThreshold;

@@ -315,12 +315,13 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
           for (int c = 4; c < CW; c += 2)
             asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[(c >> 1) & 3]) : "f"(sv[c]), "f"(sv[c + 1]));
           float* rbuf = red + (step & 1) * RT * kTileM;
-          rbuf[ch * kTileM + r] = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;  // scale > 0 keeps the order
+          rbuf[ch * kTileM + r] = top;
+          const float unit = score_unit(sv, top, a.scale_log2);
           asm volatile("bar.sync %0, %1;" ::"r"(pair_bar), "r"(bar_threads) : "memory");
-          float mx = rbuf[r];
+          float m_tile = rbuf[r];
   #pragma unroll
-          for (int c2 = 1; c2 < RT; ++c2) mx = fmaxf(mx, rbuf[c2 * kTileM + r]);
-          const float m_tile = mx * a.scale_log2;  // scale > 0 keeps the order
+          for (int c2 = 1; c2 < RT; ++c2) m_tile = fmaxf(m_tile, rbuf[c2 * kTileM + r]);
           const bool move = m_tile > m_ref_t + kRescaleThreshold || (m_ref_t == -INFINITY && m_tile != -INFINITY);
           const float m_new = move ? m_tile : m_ref_t;
           const float corr = move ? ex2_ftz(m_ref_t - m_new) : 1.f;
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
           // take one FFMA2 / FADD2 per two scores; exp2 is the MUFU instruction
           // (ex2.approx.ftz, relative error ~2^-22, far below the 2^-16 of split P)
           float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+          const float2 sc2 = make_float2(unit, unit);
           const float2 nm2 = make_float2(-m_use, -m_use);
   #pragma unroll
           for (int c = 0; c < CW; c += 32) {
@@ -454,6 +455,7 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
         const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                                fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
         const float m_tile = mx * a.scale_log2;
+        const float unit = score_unit(sv, m_tile, a.scale_log2);
         const bool move = m_tile > m_ref + kRescaleThreshold || (m_ref == -INFINITY && m_tile != -INFINITY);
         const float m_new = move ? m_tile : m_ref;
         const float corr = move ? ex2_ftz(m_ref - m_new) : 1.f;
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(PPLayout<kRowThreads>::kThreads, 1)
         float2 sum4[4];
   #pragma unroll
         for (int i = 0; i < 4; ++i) sum4[i] = make_float2(0.f, 0.f);
-        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+        const float2 sc2 = make_float2(unit, unit);
         const float2 nm2 = make_float2(-m_use, -m_use);
   #pragma unroll
         for (int c = 0; c < 128; c += 32) {

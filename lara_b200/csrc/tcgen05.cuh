@@ -4,6 +4,8 @@
 
 #include <cuda.h>
 
+#include <cmath>
+
 #include "common.cuh"
 
 namespace lara {
@@ -180,6 +182,21 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
           "r"(smem_addr(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y)
       : "memory");
+}
+
+// A score less its reference, the softmax's exponent, is one fused operation, exact but
+// for its end: score * unit - reference, where unit is the scale.  The reference is a
+// rounded product, so what is left of the largest score is up to 2^-24 of it: past this
+// bound, which keys that mask with the type's lowest value pass, an exponent too large.
+// There the scores become rounded products too, none of them above the largest's, and
+// the unit is 1.  `top`: the scaled largest of the thread's scores; by whole warps.
+constexpr float kLargeScore = 0x1p27f;
+template <int N>
+__device__ __forceinline__ float score_unit(float (&scores)[N], float top, float scale) {
+  if (!__any_sync(0xffffffffu, fabsf(top) > kLargeScore && top != -INFINITY)) return scale;
+#pragma unroll
+  for (int c = 0; c < N; ++c) scores[c] *= scale;
+  return 1.f;
 }
 
 }  // namespace tc
