@@ -27,13 +27,13 @@
 //
 // Measured (32 heads on 8, head_dim 128), one state replayed in a graph and, in
 // brackets, inputs that change from pass to pass: 64 sequences behind 8192 tokens, with
-// up to 512 of their own, 37 us (41), 132 with shared_pages = 0; 256 (64 heads) behind
-// 16384 233 to 260 us (263 to 277; 1127 with 0), 545 to 610 TFLOP/s at 4 head_dim
+// up to 512 of their own, 38 us (41), 132 with shared_pages = 0; 256 (64 heads) behind
+// 16384 231 to 260 us (263 to 277; 1127 to 1235 with 0), 545 to 615 TFLOP/s at 4 head_dim
 // operations a head and token, half as many again on the tensor cores (P in two
 // numbers).  That is bound by the softmax: 2287 cycles a step, of which 1430 are
 // exponentials and the two bf16 numbers, while the products take 1536.  4 sequences
-// behind 1024 12.6 us (12.6; 12.2 with 0), and 37 behind 2000 (head_dim 64) 17.2 (17.7;
-// 15.5 with 0): latency, and sharing gains nothing yet.
+// behind 1024 12.9 us (13.0; 12.2 with 0), and 37 behind 2000 (head_dim 64) 17.2 (17.1;
+// 15.9 with 0): latency, and sharing gains nothing yet.
 // Every wait is bounded; on a timeout the CTA
 // flags the status word, drains its own work and returns.
 #include <cuda.h>
